@@ -409,6 +409,67 @@ int mlxhip_layernorm_vjp_rows(const float* dy, const float* x, float* dx,
 int mlxhip_rmsnorm_vjp_rows(const float* dy, const float* x, float* dx,
                             int64_t rows, int64_t cols, float eps, void* stream);
 
+/* LayerNorm with a weight and a bias over the last axis of [rows, cols]:
+ * y = (x - mean) / sqrt(var + eps) * w + b (layer_norm, cpu_kernels.rs:338-363,
+ * then Mul and Add of the [cols] vectors w and b), and its gradients
+ *   g = dy w, xh = (x - mean) / sqrt(var + eps),
+ *   dx = (g - mean(g) - xh mean(g xh)) / sqrt(var + eps),
+ *   dw = sum over rows of dy xh, db = sum over rows of dy.
+ * dtype: F32, BF16 or F16, of every operand; statistics, products and sums are
+ * f32, a 16-bit result is rounded once. The sums over rows are formed in a
+ * fixed order. Operands contiguous, at any address aligned to their elements;
+ * results must not overlap operands. cols up to 2^23, rows up to 2^31 - 1; with no
+ * rows dw and db are zeros. The gradient keeps partial sums in a per-stream
+ * workspace. No reference counterpart (its LayerNorm has no weight). */
+int mlxhip_layernorm_affine_rows(int32_t dtype, const void* x, const void* w, const void* b, void* y,
+                                 int64_t rows, int64_t cols, float eps, void* stream);
+int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* x, const void* w,
+                                     void* dx, void* dw, void* db, int64_t rows, int64_t cols,
+                                     float eps, void* stream);
+
+/* Rows of w [vocab, dim] at ids[0..n), scaled: y[i] = scale * w[id_i] (n rows
+ * of dim values), ids clamped to [0, vocab - 1] (embedding_lookup,
+ * cpu_kernels.rs:317-336), and the gradient with respect to w,
+ *   dw[v] = scale * sum over the i with id_i = v (after the clamp) of dy[i],
+ * all vocab rows written, zeros where no id names them. dtype: F32, BF16 or
+ * F16, of w, y, dy and dw; each product is rounded once, the sums are f32 in
+ * an order that only the ids fix (no atomics: the same bits every time).
+ * Operands contiguous, at any address aligned to their elements; results must
+ * not overlap operands. n and vocab up to 2^31 - 1, dim up to 2^23. The
+ * gradient sorts the positions by id in a per-stream workspace (8 or 16
+ * bytes per id and 4096 rows of dim f32 sums at most). No reference
+ * counterpart for the gradient (crates/mlx-autograd/src/vjp.rs:173-176). */
+int mlxhip_embedding_rows(int32_t dtype, const void* w, const int32_t* ids, void* y, int64_t n,
+                          int64_t vocab, int64_t dim, float scale, void* stream);
+int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids, void* dw, int64_t n,
+                              int64_t vocab, int64_t dim, float scale, void* stream);
+
+/* Softmax cross entropy of the logits z = x w^T of an output projection
+ * (x [rows, dim], w [vocab, dim]) against targets[rows]:
+ *   lse[r] = log sum_v exp(z[r][v]),  loss[r] = lse[r] - z[r][targets[r]],
+ * and its gradients for the cotangent dloss[rows] of loss,
+ *   dS[r][v] = dloss[r] (exp(z[r][v] - lse[r]) - [v = targets[r]]),
+ *   dx = dS w,  dw = dS^T x.
+ * A target outside [0, vocab) takes its row out: loss 0, no gradient to dx
+ * (zeros) or dw, whatever x and dloss hold in that row (lse is still given).
+ * The logits are formed in pieces of the vocabulary and never kept; the
+ * gradient forms them again from x, w and the forward's lse. dx or dw may be
+ * NULL: that gradient is then not formed.
+ * dtype: F32, BF16 or F16, of x, w, dx and dw; loss, lse and dloss are f32, as
+ * are the logits, sums and products' accumulators. dS is rounded to bf16 or
+ * f16 (scaled by a power of two, so that small probabilities stay normal) for
+ * the products of 16-bit operands, and dx and dw once as they are stored.
+ * Sums are formed in a fixed order. Operands contiguous, at any address
+ * aligned to their elements; results must not overlap operands. rows and
+ * vocab up to 2^31 - 1, dim up to 2^20, rows * dim below 2^31. Workspace per
+ * stream. No reference counterpart. */
+int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,
+                                float* loss, float* lse, int64_t rows, int64_t dim, int64_t vocab,
+                                void* stream);
+int mlxhip_linear_cross_entropy_vjp(int32_t dtype, const void* x, const void* w, const int32_t* targets,
+                                    const float* lse, const float* dloss, void* dx, void* dw,
+                                    int64_t rows, int64_t dim, int64_t vocab, void* stream);
+
 /* Fused elementwise chain. acc starts as inputs[0][i]; each instruction
  * updates it in order; out[i] = acc. Every input is read once and out is
  * written once, whatever the chain length. Each instruction's arithmetic is

@@ -208,6 +208,12 @@ PROTOTYPES = {
     "mlxhip_softmax_vjp_rows": (_i, [_fp, _fp, _fp, _i64, _i64, _vp]),
     "mlxhip_layernorm_vjp_rows": (_i, [_fp, _fp, _fp, _i64, _i64, _f, _vp]),
     "mlxhip_rmsnorm_vjp_rows": (_i, [_fp, _fp, _fp, _i64, _i64, _f, _vp]),
+    "mlxhip_layernorm_affine_rows": (_i, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _f, _vp]),
+    "mlxhip_layernorm_affine_vjp_rows": (_i, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _vp]),
+    "mlxhip_embedding_rows": (_i, [_i32, _vp, _vp, _vp, _i64, _i64, _i64, _f, _vp]),
+    "mlxhip_embedding_vjp_rows": (_i, [_i32, _vp, _vp, _vp, _i64, _i64, _i64, _f, _vp]),
+    "mlxhip_linear_cross_entropy": (_i, [_i32, _vp, _vp, _vp, _fp, _fp, _i64, _i64, _i64, _vp]),
+    "mlxhip_linear_cross_entropy_vjp": (_i, [_i32, _vp, _vp, _vp, _fp, _fp, _vp, _vp, _i64, _i64, _i64, _vp]),
     "mlxhip_ew_chain": (_i, [C.POINTER(mlxhip_ew_instr_t), _sz, C.POINTER(_vp), _sz,
                              _fp, _i64, _vp]),
     "mlxhip_attention": (_i, [_fp, _fp, _fp, _fp, _i64, _i64, _i64, _i64, _f, _i32, _vp]),

@@ -296,6 +296,47 @@ def rmsnorm_vjp_rows(dy, x, dx, rows, cols, eps, stream=None) -> None:
     abi.check(lib().mlxhip_rmsnorm_vjp_rows(_p(dy), _p(x), _p(dx), rows, cols, eps, stream))
 
 
+def layernorm_affine_rows(dtype: int, x, w, b, y, rows: int, cols: int, eps: float, stream=None) -> None:
+    """LayerNorm with a weight and a bias [cols] over the rows of x
+    [rows, cols]; ``dtype`` abi.F32, BF16 or F16 for every operand."""
+    abi.check(lib().mlxhip_layernorm_affine_rows(dtype, _p(x), _p(w), _p(b), _p(y), rows, cols, eps, stream))
+
+
+def layernorm_affine_vjp_rows(dtype: int, dy, x, w, dx, dw, db, rows: int, cols: int, eps: float,
+                              stream=None) -> None:
+    """dx [rows, cols], dw and db [cols] of ``layernorm_affine_rows``."""
+    abi.check(lib().mlxhip_layernorm_affine_vjp_rows(dtype, _p(dy), _p(x), _p(w), _p(dx), _p(dw), _p(db), rows, cols,
+                                                     eps, stream))
+
+
+def embedding_rows(dtype: int, w, ids, y, n: int, vocab: int, dim: int, scale: float = 1.0, stream=None) -> None:
+    """y[i] = scale * w[ids[i]] for n int32 ids (clamped to the table's rows)."""
+    abi.check(lib().mlxhip_embedding_rows(dtype, _p(w), _p(ids), _p(y), n, vocab, dim, scale, stream))
+
+
+def embedding_vjp_rows(dtype: int, dy, ids, dw, n: int, vocab: int, dim: int, scale: float = 1.0,
+                       stream=None) -> None:
+    """dw [vocab, dim] of ``embedding_rows``: the dy rows of each id summed in
+    f32 in the order of their positions; zeros for ids that do not occur."""
+    abi.check(lib().mlxhip_embedding_vjp_rows(dtype, _p(dy), _p(ids), _p(dw), n, vocab, dim, scale, stream))
+
+
+def linear_cross_entropy(dtype: int, x, w, targets, loss, lse, rows: int, dim: int, vocab: int, stream=None) -> None:
+    """Cross entropy of the logits x w^T (x [rows, dim], w [vocab, dim]) against
+    int32 targets; f32 loss and lse [rows]. A target outside [0, vocab) takes
+    its row out (loss 0). The logits are not kept."""
+    abi.check(lib().mlxhip_linear_cross_entropy(dtype, _p(x), _p(w), _p(targets), _p(loss), _p(lse), rows, dim, vocab,
+                                                stream))
+
+
+def linear_cross_entropy_vjp(dtype: int, x, w, targets, lse, dloss, dx, dw, rows: int, dim: int, vocab: int,
+                             stream=None) -> None:
+    """dx and dw of ``linear_cross_entropy`` for the loss's cotangent dloss
+    [rows] and the forward's lse; dx or dw may be None (not formed)."""
+    abi.check(lib().mlxhip_linear_cross_entropy_vjp(dtype, _p(x), _p(w), _p(targets), _p(lse), _p(dloss), _p(dx), _p(dw),
+                                                    rows, dim, vocab, stream))
+
+
 EW = {"add": 0, "sub": 1, "rsub": 2, "mul": 3, "div": 4, "rdiv": 5, "neg": 6, "exp": 7,
       "log": 8, "sqrt": 9, "silu": 10, "gelu": 11, "silu_vjp": 12, "gelu_vjp": 13}
 

@@ -50,6 +50,9 @@ SOURCES = [
     "autograd.cpp",
     "decoder.cpp",
     "kernels/rows.hip",
+    "kernels/norm_affine.hip",
+    "kernels/embedding.hip",
+    "kernels/cross_entropy.hip",
     "kernels/elementwise.hip",
     "kernels/gemm.hip",
     "kernels/gemm_small.hip",

@@ -13,6 +13,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -979,6 +980,41 @@ int mlxhip_gemm_noalloc(int32_t ab_dtype, int32_t c_dtype, int32_t trans_a, int3
                         ldc, stride_c, as_stream(stream));
 }
 
+namespace {
+constexpr int64_t MAX_ROW = int64_t(1) << 23;  // columns of the row operators below
+
+int check_sizes(const char* what, std::initializer_list<int64_t> sizes, std::initializer_list<int64_t> most) {
+    auto m = most.begin();
+    for (int64_t v : sizes) {
+        if (v < 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+        if (v > *m)
+            return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: size %lld is over %lld", what, (long long)v, (long long)*m);
+        ++m;
+    }
+    return MLXHIP_OK;
+}
+
+// f32, bf16 or f16 operands and 4-byte ones (ids, f32 rows): not null, at
+// addresses aligned to their elements.
+int check_operands(const char* what, int dtype, std::initializer_list<const void*> typed,
+                   std::initializer_list<const void*> words = {}) {
+    if (dtype != MLXHIP_DTYPE_F32 && dtype != MLXHIP_DTYPE_BF16 && dtype != MLXHIP_DTYPE_F16)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: dtype %d (f32, bf16 or f16)", what, dtype);
+    const uintptr_t size = dtype == MLXHIP_DTYPE_F32 ? 4 : 2;
+    for (const void* p : typed) {
+        if (!p) return fail(MLXHIP_ERR_NULL_PTR, "%s: null operand", what);
+        if (reinterpret_cast<uintptr_t>(p) % size)
+            return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: operand not aligned to its elements", what);
+    }
+    for (const void* p : words) {
+        if (!p) return fail(MLXHIP_ERR_NULL_PTR, "%s: null operand", what);
+        if (reinterpret_cast<uintptr_t>(p) % 4)
+            return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: operand not aligned to its elements", what);
+    }
+    return MLXHIP_OK;
+}
+}  // namespace
+
 size_t mlxhip_gemm_noalloc_scratch_bytes(void) { return GEMM_NOALLOC_SCRATCH_BYTES; }
 
 int mlxhip_softmax_rows(const float* x, float* y, int64_t rows, int64_t cols, void* stream) {
@@ -1024,6 +1060,81 @@ int mlxhip_rmsnorm_vjp_rows(const float* dy, const float* x, float* dx, int64_t 
     if ((rows * cols) && (!dy || !x || !dx)) return fail(MLXHIP_ERR_NULL_PTR, "rmsnorm_vjp_rows: null pointer");
     MLXHIP_TRY(ensure_device());
     return row_op(ROW_RMSNORM_VJP, dy, x, dx, rows, cols, eps, 0, as_stream(stream));
+}
+
+int mlxhip_layernorm_affine_rows(int32_t dtype, const void* x, const void* w, const void* b, void* y, int64_t rows,
+                                 int64_t cols, float eps, void* stream) {
+    MLXHIP_TRY(check_sizes("layernorm_affine_rows", {rows, cols}, {INT32_MAX, MAX_ROW}));
+    if (cols == 0 || rows == 0) return check_operands("layernorm_affine_rows", dtype, {});
+    MLXHIP_TRY(check_operands("layernorm_affine_rows", dtype, {x, w, b, y}));
+    MLXHIP_TRY(ensure_device());
+    return layernorm_affine(dtype, x, w, b, y, rows, cols, eps, as_stream(stream));
+}
+
+int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* x, const void* w, void* dx, void* dw,
+                                     void* db, int64_t rows, int64_t cols, float eps, void* stream) {
+    MLXHIP_TRY(check_sizes("layernorm_affine_vjp_rows", {rows, cols}, {INT32_MAX, MAX_ROW}));
+    if (cols == 0) return check_operands("layernorm_affine_vjp_rows", dtype, {});
+    if (rows == 0) MLXHIP_TRY(check_operands("layernorm_affine_vjp_rows", dtype, {dw, db}));
+    else MLXHIP_TRY(check_operands("layernorm_affine_vjp_rows", dtype, {dy, x, w, dx, dw, db}));
+    MLXHIP_TRY(ensure_device());
+    return layernorm_affine_vjp(dtype, dy, x, w, dx, dw, db, rows, cols, eps, as_stream(stream));
+}
+
+int mlxhip_embedding_rows(int32_t dtype, const void* w, const int32_t* ids, void* y, int64_t n, int64_t vocab,
+                          int64_t dim, float scale, void* stream) {
+    MLXHIP_TRY(check_sizes("embedding_rows", {n, vocab, dim}, {INT32_MAX, INT32_MAX, MAX_ROW}));
+    if (n == 0 || dim == 0) return check_operands("embedding_rows", dtype, {});
+    if (vocab == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding_rows: empty table");
+    MLXHIP_TRY(check_operands("embedding_rows", dtype, {w, y}, {ids}));
+    MLXHIP_TRY(ensure_device());
+    return embedding_rows(dtype, w, ids, y, n, vocab, dim, scale, as_stream(stream));
+}
+
+int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids, void* dw, int64_t n, int64_t vocab,
+                              int64_t dim, float scale, void* stream) {
+    MLXHIP_TRY(check_sizes("embedding_vjp_rows", {n, vocab, dim}, {INT32_MAX, INT32_MAX, MAX_ROW}));
+    if (dim == 0) return check_operands("embedding_vjp_rows", dtype, {});
+    if (vocab == 0)
+        return n ? fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding_vjp_rows: empty table")
+                 : check_operands("embedding_vjp_rows", dtype, {});
+    if (n == 0) MLXHIP_TRY(check_operands("embedding_vjp_rows", dtype, {dw}));
+    else MLXHIP_TRY(check_operands("embedding_vjp_rows", dtype, {dy, dw}, {ids}));
+    MLXHIP_TRY(ensure_device());
+    return embedding_vjp_rows(dtype, dy, ids, dw, n, vocab, dim, scale, as_stream(stream));
+}
+
+namespace {
+// Sizes of the cross entropy's entry points.
+int check_cross_entropy(const char* what, int64_t rows, int64_t dim, int64_t vocab) {
+    MLXHIP_TRY(check_sizes(what, {rows, dim, vocab}, {INT32_MAX, 1 << 20, INT32_MAX}));
+    if (dim == 0 || vocab == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: no logits (dim or vocab is 0)", what);
+    if (rows * dim > INT32_MAX)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: rows * dim = %lld is over 2^31 - 1", what, (long long)(rows * dim));
+    return MLXHIP_OK;
+}
+}  // namespace
+
+int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets, float* loss,
+                                float* lse, int64_t rows, int64_t dim, int64_t vocab, void* stream) {
+    MLXHIP_TRY(check_cross_entropy("linear_cross_entropy", rows, dim, vocab));
+    if (rows == 0) return check_operands("linear_cross_entropy", dtype, {});
+    MLXHIP_TRY(check_operands("linear_cross_entropy", dtype, {x, w}, {targets, loss, lse}));
+    MLXHIP_TRY(ensure_device());
+    return linear_cross_entropy(dtype, x, w, targets, loss, lse, rows, dim, vocab, as_stream(stream));
+}
+
+int mlxhip_linear_cross_entropy_vjp(int32_t dtype, const void* x, const void* w, const int32_t* targets,
+                                    const float* lse, const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim,
+                                    int64_t vocab, void* stream) {
+    const char* what = "linear_cross_entropy_vjp";
+    MLXHIP_TRY(check_cross_entropy(what, rows, dim, vocab));
+    if (rows > 0) MLXHIP_TRY(check_operands(what, dtype, {x, w}, {targets, lse, dloss}));
+    if (dx) MLXHIP_TRY(check_operands(what, dtype, {dx}));
+    if (dw) MLXHIP_TRY(check_operands(what, dtype, {dw}));
+    if (!dx && !dw) return check_operands(what, dtype, {});
+    MLXHIP_TRY(ensure_device());
+    return linear_cross_entropy_vjp(dtype, x, w, targets, lse, dloss, dx, dw, rows, dim, vocab, as_stream(stream));
 }
 
 int mlxhip_ew_chain(const mlxhip_ew_instr_t* prog, size_t n_instr, const float* const* inputs, size_t n_inputs,

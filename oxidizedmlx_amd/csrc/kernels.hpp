@@ -78,6 +78,25 @@ int rope_mlx(const float* x, float* y, int64_t n_rows, int64_t head_dim, int64_t
              float base, int traditional, hipStream_t s);
 int fill(float* y, float v, int64_t n, hipStream_t s);
 
+// ── norm_affine.hip, embedding.hip, cross_entropy.hip ─────────────────────
+// Operands of dtype `dt` (f32, bf16, f16), contiguous, at any element-aligned
+// address; see the entry points of the same names in mlxhip.h. Sizes within
+// the bounds those check.
+int layernorm_affine(int dt, const void* x, const void* w, const void* b, void* y, int64_t rows, int64_t cols,
+                     float eps, hipStream_t s);
+int layernorm_affine_vjp(int dt, const void* dy, const void* x, const void* w, void* dx, void* dw, void* db,
+                         int64_t rows, int64_t cols, float eps, hipStream_t s);
+int embedding_rows(int dt, const void* w, const int32_t* ids, void* y, int64_t n, int64_t vocab, int64_t dim,
+                   float scale, hipStream_t s);
+int embedding_vjp_rows(int dt, const void* dy, const int32_t* ids, void* dw, int64_t n, int64_t vocab, int64_t dim,
+                       float scale, hipStream_t s);
+int linear_cross_entropy(int dt, const void* x, const void* w, const int32_t* targets, float* loss, float* lse,
+                         int64_t rows, int64_t dim, int64_t vocab, hipStream_t s);
+// dx or dw may be null (that gradient is not formed).
+int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t* targets, const float* lse,
+                             const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
+                             hipStream_t s);
+
 // ── decode.hip (greedy decode step of a decoder-only model) ───────────────
 constexpr int DEC_MAX_BATCH = 8;          // sequences per decode step
 constexpr int DEC_LDS_LIMIT = 159 * 1024; // dynamic LDS (a CDNA4 CU has 160 KiB; 1 KiB kept for static LDS)

@@ -1,0 +1,486 @@
+// embedding.hip — rows of a weight matrix at integer ids, scaled, and the
+// gradient with respect to the weight, for f32, bf16 and f16.
+//
+//   y_i  = scale * W[id_i]                         (ids clamped to [0, vocab - 1],
+//   dW_v = scale * sum over i with id_i = v of dy_i  as embedding_lookup does,
+//                                   crates/mlx-core/src/cpu_kernels.rs:317-336)
+//
+// The lookup copies rows, a wave to each: it is bound by memory (or, for a
+// few rows, by the launch).
+//
+// The gradient adds up the dy rows of equal ids in f32, in the order of the
+// positions, and rounds once. Text has words that are a tenth of all tokens
+// beside thousands that occur once, so a workgroup per id would wait for its
+// one longest sum, and atomics would give other bits every time. Instead the
+// positions are sorted by id (a stable radix sort of 8 bits a pass, so equal
+// ids stay in the order of their positions) and the sorted list is cut into
+// equal shares, one to a wave: a share writes the rows that begin and end in
+// it, and leaves the sums of the ids that cross its borders as partial rows,
+// which a last launch adds up in the order of the shares. Rows of ids that do
+// not occur are zeroed by the launch that begins the sort, on the compute
+// units that the sort leaves idle.
+#include "../common.hpp"
+#include "../kernels.hpp"
+#include "elem.hpp"
+
+#include <algorithm>
+
+namespace mlxhip {
+namespace {
+
+using dev::Elem;
+using dev::load_raw;
+using dev::store_vec;
+using dev::unpack;
+using dev::Vec16;
+
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+constexpr int BITS = 8, BINS = 1 << BITS;
+// Positions that one workgroup sorts in its LDS (key and position, 8 bytes
+// each: 128 KiB), and those of a workgroup's block in a longer sort.
+constexpr int LDS_SORT = 16384;
+constexpr int BLOCK_SORT = 8192;
+// Shares of the sorted list, about.
+constexpr int SHARES = 2048;
+
+template <int DT>
+__global__ __launch_bounds__(256) void embed_kernel(const typename Elem<DT>::type* __restrict__ w,
+                                                    const int32_t* __restrict__ ids,
+                                                    typename Elem<DT>::type* __restrict__ y, int64_t n, int64_t vocab,
+                                                    int64_t dim, float scale) {
+    constexpr int VEC = Elem<DT>::VEC;
+    const int lane = threadIdx.x & 63;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
+        const int64_t id = min(max((int64_t)ids[i], (int64_t)0), vocab - 1);
+        for (int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC; c < dim; c += (int64_t)gridDim.y * 64 * VEC) {
+            float v[VEC];
+            unpack<DT>(load_raw<DT>(w + id * dim, c, dim), v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] *= scale;
+            store_vec<DT>(y + i * dim, c, dim, v);
+        }
+    }
+}
+
+// Zeros for `bytes` (a multiple of 2) from p, by workgroup b of nb.
+__device__ inline void zero_fill(char* p, int64_t bytes, int64_t b, int64_t nb) {
+    const int64_t step = nb * SORT_THREADS;
+    // The 16-byte words inside, and the bytes before and after them by pairs.
+    const int64_t head = min((int64_t)(-reinterpret_cast<intptr_t>(p) & 15), bytes);
+    const int64_t words = (bytes - head) / 16, tail = (bytes - head) % 16;
+    uint4* q = reinterpret_cast<uint4*>(p + head);
+    for (int64_t i = b * SORT_THREADS + threadIdx.x; i < words; i += step) q[i] = make_uint4(0, 0, 0, 0);
+    if (b == 0 && threadIdx.x < 16) {
+        const int o = threadIdx.x * 2;
+        if (o < head) *reinterpret_cast<uint16_t*>(p + o) = 0;
+        if (o < tail) *reinterpret_cast<uint16_t*>(p + head + words * 16 + o) = 0;
+    }
+}
+
+// Of the 64 lanes' digits: how many lower lanes hold this lane's, how many in
+// all, both over the lanes with `in`.
+__device__ inline void match(uint32_t digit, bool in, int lane, uint32_t* below, uint32_t* count) {
+    uint64_t same = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+        const uint64_t ones = __ballot((digit >> b) & 1);
+        same &= (digit >> b) & 1 ? ones : ~ones;
+    }
+    *below = (uint32_t)__popcll(same & ((uint64_t(1) << lane) - 1));
+    *count = (uint32_t)__popcll(same);
+}
+
+// Where each of a workgroup's elements goes by its digit, stably: wave w owns
+// elements [w * steps * 64, (w + 1) * steps * 64), step s of them at lane
+// offset s * 64. hist[d * SORT_WAVES + w] counts wave w's digits d and, after
+// the scan, is the place of the first of them in the workgroup's order.
+template <int STEPS>
+__device__ inline void local_ranks(const uint32_t (&digit)[STEPS], int steps, int first, int n, uint32_t* hist,
+                                   uint32_t (&rank)[STEPS]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < BINS * SORT_WAVES; i += SORT_THREADS) hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        if (s >= steps) break;
+        const bool in = first + s * 64 + lane < n;
+        uint32_t below, count;
+        match(digit[s], in, lane, &below, &count);
+        // Only this wave touches its counters, and its LDS accesses complete
+        // in order: every lane reads before the first lane of a digit writes.
+        volatile uint32_t* h = hist + digit[s] * SORT_WAVES + wave;
+        const uint32_t had = in ? *h : 0;
+        rank[s] = had + below;
+        __builtin_amdgcn_wave_barrier();
+        if (in && below == 0) *h = had + count;
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+}
+
+// Exclusive scan of hist (BINS * SORT_WAVES counters) in place by the
+// workgroup, four counters a thread.
+__device__ inline void scan_hist(uint32_t* hist, uint32_t* wave_sums) {
+    static_assert(BINS * SORT_WAVES == 4 * SORT_THREADS, "four counters a thread");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t v[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = sum;
+        sum += hist[threadIdx.x * 4 + i];
+    }
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 63) wave_sums[wave] = incl;
+    __syncthreads();
+    uint32_t base = incl - sum;
+    for (int w = 0; w < wave; ++w) base += wave_sums[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hist[threadIdx.x * 4 + i] = base + v[i];
+    __syncthreads();
+}
+
+__device__ inline uint32_t clamped(int32_t id, uint32_t vocab) {
+    return id < 0 ? 0u : min((uint32_t)id, vocab - 1);
+}
+
+// Up to LDS_SORT positions: workgroup 0 sorts them, the others zero dW.
+__global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const int32_t* __restrict__ ids, int n, uint32_t vocab,
+                                                                  int passes, uint32_t* __restrict__ keys,
+                                                                  uint32_t* __restrict__ order, char* dw,
+                                                                  int64_t dw_bytes) {
+    constexpr int STEPS = LDS_SORT / SORT_THREADS;
+    __shared__ uint32_t skey[LDS_SORT], spos[LDS_SORT], hist[BINS * SORT_WAVES], wave_sums[SORT_WAVES];
+    if (blockIdx.x > 0) {
+        zero_fill(dw, dw_bytes, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int steps = (n + SORT_THREADS - 1) / SORT_THREADS, first = wave * steps * 64;
+    uint32_t key[STEPS], pos[STEPS], digit[STEPS], rank[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int i = first + s * 64 + lane;
+        key[s] = s < steps && i < n ? clamped(ids[i], vocab) : 0;
+        pos[s] = i;
+    }
+    for (int p = 0; p < passes; ++p) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) digit[s] = (key[s] >> (BITS * p)) & (BINS - 1);
+        local_ranks<STEPS>(digit, steps, first, n, hist, rank);
+        scan_hist(hist, wave_sums);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if (s < steps && first + s * 64 + lane < n) {
+                const uint32_t to = hist[digit[s] * SORT_WAVES + wave] + rank[s];
+                skey[to] = key[s];
+                spos[to] = pos[s];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int i = first + s * 64 + lane;
+            if (s < steps && i < n) {
+                key[s] = skey[i];
+                pos[s] = spos[i];
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS) {
+        keys[i] = skey[i];
+        order[i] = spos[i];
+    }
+}
+
+// One pass of a longer sort, in blocks of BLOCK_SORT positions: the blocks'
+// counts of each digit (counts[digit * blocks + block]), their scan along the
+// blocks, and the move to the places that follow. The first pass reads the
+// ids; its counting launch also zeroes dW with the workgroups past the blocks.
+constexpr int BSTEPS = BLOCK_SORT / SORT_THREADS;
+
+__device__ inline void load_block(const int32_t* ids, const uint32_t* keys, int64_t n, uint32_t vocab, int64_t base,
+                                  int64_t left, uint32_t (&key)[BSTEPS]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int s = 0; s < BSTEPS; ++s) {
+        const int i = wave * BSTEPS * 64 + s * 64 + lane;
+        key[s] = i < left ? (ids ? clamped(ids[base + i], vocab) : keys[base + i]) : 0;
+    }
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int32_t* __restrict__ ids,
+                                                                  const uint32_t* __restrict__ keys, int64_t n,
+                                                                  uint32_t vocab, int shift, int blocks,
+                                                                  uint32_t* __restrict__ counts, char* dw,
+                                                                  int64_t dw_bytes) {
+    __shared__ uint32_t hist[BINS];
+    if ((int)blockIdx.x >= blocks) {
+        zero_fill(dw, dw_bytes, blockIdx.x - blocks, gridDim.x - blocks);
+        return;
+    }
+    if (threadIdx.x < BINS) hist[threadIdx.x] = 0;
+    __syncthreads();
+    const int64_t base = (int64_t)blockIdx.x * BLOCK_SORT, left = min((int64_t)BLOCK_SORT, n - base);
+    uint32_t key[BSTEPS];
+    load_block(ids, keys, n, vocab, base, left, key);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int s = 0; s < BSTEPS; ++s)
+        if (wave * BSTEPS * 64 + s * 64 + lane < left) atomicAdd(&hist[(key[s] >> shift) & (BINS - 1)], 1u);
+    __syncthreads();
+    if (threadIdx.x < BINS) counts[(int64_t)threadIdx.x * blocks + blockIdx.x] = hist[threadIdx.x];
+}
+
+// counts[d][*] becomes its exclusive scan, totals[d] its sum: a wave per digit.
+__global__ __launch_bounds__(64) void sort_scan_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ totals,
+                                                       int blocks) {
+    uint32_t* c = counts + (int64_t)blockIdx.x * blocks;
+    const int lane = threadIdx.x;
+    uint32_t base = 0;
+    for (int b = 0; b < blocks; b += 64) {
+        const uint32_t v = b + lane < blocks ? c[b + lane] : 0;
+        uint32_t incl = v;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t u = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += u;
+        }
+        if (b + lane < blocks) c[b + lane] = base + incl - v;
+        base += __shfl(incl, 63, 64);
+    }
+    if (lane == 0) totals[blockIdx.x] = base;
+}
+
+__global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* __restrict__ ids,
+                                                                 const uint32_t* __restrict__ keys,
+                                                                 const uint32_t* __restrict__ order, int64_t n,
+                                                                 uint32_t vocab, int shift, int blocks,
+                                                                 const uint32_t* __restrict__ counts,
+                                                                 const uint32_t* __restrict__ totals,
+                                                                 uint32_t* __restrict__ keys_out,
+                                                                 uint32_t* __restrict__ order_out) {
+    __shared__ uint32_t hist[BINS * SORT_WAVES], wave_sums[SORT_WAVES], start[BINS];
+    const int64_t base = (int64_t)blockIdx.x * BLOCK_SORT, left = min((int64_t)BLOCK_SORT, n - base);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t key[BSTEPS], digit[BSTEPS], rank[BSTEPS];
+    load_block(ids, keys, n, vocab, base, left, key);
+#pragma unroll
+    for (int s = 0; s < BSTEPS; ++s) digit[s] = (key[s] >> shift) & (BINS - 1);
+    local_ranks<BSTEPS>(digit, BSTEPS, wave * BSTEPS * 64, (int)left, hist, rank);
+    scan_hist(hist, wave_sums);
+    // Where the block's elements of a digit begin in the whole order, less
+    // their place in the block's.
+    if (wave == 0) {
+        uint32_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < BINS / 64; ++i) sum += totals[lane * (BINS / 64) + i];
+        uint32_t incl = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t u = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += u;
+        }
+        uint32_t at = incl - sum;
+#pragma unroll
+        for (int i = 0; i < BINS / 64; ++i) {
+            const int d = lane * (BINS / 64) + i;
+            start[d] = at + counts[(int64_t)d * blocks + blockIdx.x] - hist[d * SORT_WAVES];
+            at += totals[d];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < BSTEPS; ++s) {
+        const int i = wave * BSTEPS * 64 + s * 64 + lane;
+        if (i < left) {
+            const uint32_t to = start[digit[s]] + hist[digit[s] * SORT_WAVES + wave] + rank[s];
+            keys_out[to] = key[s];
+            order_out[to] = order ? order[base + i] : (uint32_t)(base + i);
+        }
+    }
+}
+
+// A wave's share of the sorted positions and chunk of 64 * VEC columns. part
+// holds two rows of dim sums per share: of the id that began before it, and
+// of the one that goes on after it (an id that does both: the first only).
+template <int DT>
+__global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>::type* __restrict__ dy,
+                                                        const uint32_t* __restrict__ keys,
+                                                        const uint32_t* __restrict__ order, int64_t n, int share,
+                                                        int64_t shares, int64_t dim, float scale,
+                                                        typename Elem<DT>::type* __restrict__ dw,
+                                                        float* __restrict__ part) {
+    constexpr int VEC = Elem<DT>::VEC, AHEAD = 4;
+    const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (sh >= shares) return;
+    const int64_t c = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * VEC;
+    if (c >= dim) return;
+    const int64_t lo = sh * share, hi = min(n, lo + share);
+    float acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    uint32_t cur = keys[lo];
+    bool head = lo > 0 && keys[lo - 1] == cur;
+    auto leave = [&](float* to) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (c + e < dim) to[c + e] = acc[e];
+    };
+    auto flush = [&] {
+        if (head) {
+            leave(part + 2 * sh * dim);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] *= scale;
+            store_vec<DT>(dw + (int64_t)cur * dim, c, dim, acc);
+        }
+        head = false;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    };
+    for (int64_t i = lo; i < hi; i += AHEAD) {
+        Vec16<DT> raw[AHEAD];
+        uint32_t key[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            const int64_t j = min(i + a, hi - 1);
+            key[a] = keys[j];
+            raw[a] = load_raw<DT>(dy + (int64_t)order[j] * dim, c, dim);
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+            if (i + a >= hi) break;
+            if (key[a] != cur) {
+                flush();
+                cur = key[a];
+            }
+            float v[VEC];
+            unpack<DT>(raw[a], v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+        }
+    }
+    if (hi < n && keys[hi] == cur) leave(part + (2 * sh + (head ? 0 : 1)) * dim);
+    else flush();
+}
+
+// The ids that go on after share sh and began in it: their shares' sums, in order.
+template <int DT>
+__global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t* __restrict__ keys, int64_t n, int share,
+                                                         int64_t shares, int64_t dim, float scale,
+                                                         typename Elem<DT>::type* __restrict__ dw,
+                                                         const float* __restrict__ part) {
+    const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (sh + 1 >= shares) return;
+    const int64_t lo = sh * share, hi = lo + share;
+    const uint32_t key = keys[hi - 1];
+    if (keys[hi] != key || (keys[lo] == key && lo > 0 && keys[lo - 1] == key)) return;
+    // The last share that the id reaches: 64 of their first keys at a time.
+    int64_t last = sh + 1;
+    for (;;) {
+        const int64_t k = last + 1 + (threadIdx.x & 63);
+        const uint64_t go = __ballot(k < shares && keys[min(k, shares - 1) * share] == key);
+        const int run = ~go ? __builtin_ctzll(~go) : 64;
+        last += run;
+        if (run < 64) break;
+    }
+    for (int64_t c = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63); c < dim; c += (int64_t)gridDim.y * 64) {
+        float acc = part[(2 * sh + 1) * dim + c];
+#pragma unroll 16
+        for (int64_t k = sh + 1; k <= last; ++k) acc += part[2 * k * dim + c];
+        dw[(int64_t)key * dim + c] = dev::from_f32<DT>(acc * scale);
+    }
+}
+
+template <int DT>
+int run_embed(const void* w, const int32_t* ids, void* y, int64_t n, int64_t vocab, int64_t dim, float scale,
+              hipStream_t s) {
+    typedef typename Elem<DT>::type T;
+    // At most 2^30 work-items, which a dispatch counts in 32 bits.
+    const int64_t gy = std::min<int64_t>(ceil_div(dim, 64 * Elem<DT>::VEC), 64);
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, 4), (1 << 22) / gy), (unsigned)gy);
+    hipLaunchKernelGGL((embed_kernel<DT>), grid, dim3(256), 0, s, (const T*)w, ids, (T*)y, n, vocab, dim, scale);
+    return launch_check("embed_kernel");
+}
+
+template <int DT>
+int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64_t vocab, int64_t dim, float scale,
+                  hipStream_t s) {
+    typedef typename Elem<DT>::type T;
+    const int64_t dw_bytes = vocab * dim * (int64_t)sizeof(T);
+    const int fill = (int)std::min<int64_t>(ceil_div(dw_bytes, 16 * SORT_THREADS), 512);
+    const int64_t blocks = n <= LDS_SORT ? 0 : ceil_div(n, BLOCK_SORT);
+    // 2048 shares fill the compute units (8 waves each, times the chunks of
+    // columns) and leave a frequent id few partial sums to add up.
+    const int share = (int)std::max<int64_t>(ceil_div(n, SHARES), 4);
+    const int64_t shares = ceil_div(n, share);
+    const size_t list = ((size_t)n * 4 + 255) / 256 * 256;
+    const size_t sums = (size_t)shares * 2 * dim * sizeof(float);
+    const size_t counts = blocks ? ((size_t)BINS * blocks + BINS) * 4 : 0;
+    char* ws = nullptr;
+    MLXHIP_TRY(stream_workspace(s, WS_EMBED, (blocks ? 4 : 2) * list + sums + counts, reinterpret_cast<void**>(&ws)));
+    uint32_t *keys = reinterpret_cast<uint32_t*>(ws), *order = reinterpret_cast<uint32_t*>(ws + list);
+    float* part = reinterpret_cast<float*>(ws + (blocks ? 4 : 2) * list);
+    int passes = 1;
+    while (passes < 4 && (vocab - 1) >> (BITS * passes)) ++passes;
+    if (!blocks) {
+        hipLaunchKernelGGL(sort_small_kernel, dim3((unsigned)(1 + fill)), dim3(SORT_THREADS), 0, s, ids, (int)n,
+                           (uint32_t)vocab, passes, keys, order, (char*)dw, dw_bytes);
+        MLXHIP_TRY(launch_check("sort_small_kernel"));
+    } else {
+        uint32_t *keys2 = reinterpret_cast<uint32_t*>(ws + 2 * list), *order2 = reinterpret_cast<uint32_t*>(ws + 3 * list);
+        uint32_t* cnt = reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(part) + sums);
+        uint32_t* totals = cnt + BINS * blocks;
+        for (int p = 0; p < passes; ++p) {
+            const int32_t* src = p == 0 ? ids : nullptr;
+            hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)(blocks + (p == 0 ? fill : 0))), dim3(SORT_THREADS), 0, s,
+                               src, keys, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt, (char*)dw, dw_bytes);
+            MLXHIP_TRY(launch_check("sort_count_kernel"));
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS), dim3(64), 0, s, cnt, totals, (int)blocks);
+            MLXHIP_TRY(launch_check("sort_scan_kernel"));
+            hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)blocks), dim3(SORT_THREADS), 0, s, src, keys,
+                               p == 0 ? nullptr : order, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt, totals, keys2,
+                               order2);
+            MLXHIP_TRY(launch_check("sort_move_kernel"));
+            std::swap(keys, keys2);
+            std::swap(order, order2);
+        }
+    }
+    if (n == 0) return MLXHIP_OK;
+    const dim3 grid((unsigned)ceil_div(shares, 4), (unsigned)ceil_div(dim, 64 * Elem<DT>::VEC));
+    hipLaunchKernelGGL((embed_sum_kernel<DT>), grid, dim3(256), 0, s, (const T*)dy, keys, order, n, share, shares, dim,
+                       scale, (T*)dw, part);
+    MLXHIP_TRY(launch_check("embed_sum_kernel"));
+    if (shares == 1) return MLXHIP_OK;
+    const dim3 jgrid((unsigned)ceil_div(shares, 4), (unsigned)std::min<int64_t>(ceil_div(dim, 64), 65535));
+    hipLaunchKernelGGL((embed_join_kernel<DT>), jgrid, dim3(256), 0, s, keys, n, share, shares, dim, scale, (T*)dw, part);
+    return launch_check("embed_join_kernel");
+}
+
+}  // namespace
+
+int embedding_rows(int dt, const void* w, const int32_t* ids, void* y, int64_t n, int64_t vocab, int64_t dim,
+                   float scale, hipStream_t s) {
+    if (n == 0 || dim == 0) return MLXHIP_OK;
+    int rc = MLXHIP_OK;
+    if (!with_float_dtype(dt, [&](auto d) { rc = run_embed<d.value>(w, ids, y, n, vocab, dim, scale, s); }))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding: dtype %d (f32, bf16 or f16)", dt);
+    return rc;
+}
+
+int embedding_vjp_rows(int dt, const void* dy, const int32_t* ids, void* dw, int64_t n, int64_t vocab, int64_t dim,
+                       float scale, hipStream_t s) {
+    if (vocab == 0 || dim == 0) return MLXHIP_OK;
+    int rc = MLXHIP_OK;
+    if (!with_float_dtype(dt, [&](auto d) { rc = run_embed_vjp<d.value>(dy, ids, dw, n, vocab, dim, scale, s); }))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding gradient: dtype %d (f32, bf16 or f16)", dt);
+    return rc;
+}
+
+}  // namespace mlxhip

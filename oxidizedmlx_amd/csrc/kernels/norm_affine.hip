@@ -1,0 +1,442 @@
+// norm_affine.hip — layer norm over the last axis with a weight and a bias,
+// and its gradients, for f32, bf16 and f16 rows.
+//
+//   xh = (x - mean) rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   y  = xh w + b
+//   g  = dy w;  dx = rstd (g - mean(g) - xh mean(g xh))
+//   dw = sum over rows of dy xh;  db = sum over rows of dy
+//
+// The normalisation is the reference's layer_norm (crates/mlx-core/src/
+// cpu_kernels.rs:338-363) and its gradient layer_norm_vjp (:403-454), neither
+// of which has a weight or bias. All sums, statistics and products are f32;
+// a 16-bit result is rounded once, as it is stored.
+//
+// Rows of up to 16384 columns stay in registers: WPR waves own a row, each
+// lane NV 16-byte vectors of it (at most 16 values), so x and dy are read
+// once and y or dx written once. The statistics take two exchanges between a
+// row's lanes: the mean, then the sums of (x - mean)^2 and, going back, of g
+// and g (x - mean) as well (the deviations are from the true mean, so a large
+// mean costs no digits). Workgroups walk over rows with the weights held in
+// registers; going back each lane also keeps its columns' dw and db sums and
+// writes them at the end as one partial row per workgroup, which a second
+// launch adds up in a fixed order (no atomics: the same bits every time).
+// Longer rows are read again from the caches: a launch for the rows'
+// statistics, then one over tiles of columns.
+#include "../common.hpp"
+#include "../kernels.hpp"
+#include "device_math.hpp"
+#include "elem.hpp"
+
+#include <algorithm>
+
+namespace mlxhip {
+namespace {
+
+using dev::Elem;
+using dev::load_raw;
+using dev::store_vec;
+using dev::to_f32;
+using dev::unpack;
+using dev::Vec16;
+
+constexpr int MAX_COLS = 16384;    // of rows held in registers
+constexpr int PARTIALS = 256;      // workgroups, and partial sums, of the gradient
+constexpr int LONG_TILE = 1024;    // columns of a workgroup's tile for longer rows
+
+// N sums over the WPR waves of a row; every lane gets them. Two rounds of
+// slots alternate, so one barrier per call is enough.
+template <int WPR, int N>
+__device__ inline void row_sums(float (&v)[N], float* slots, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = dev::wave_sum(v[i]);
+    if constexpr (WPR > 1) {
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) slots[i * WPR + wave] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = slots[i * WPR];
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) s += slots[i * WPR + w];
+            v[i] = s;
+        }
+    }
+}
+
+// The row's vectors of lane t of 64 * WPR: columns (j * 64 * WPR + t) * VEC.
+// Every j but the last is whole in all lanes (the launch picks NV so).
+template <int DT, int WPR, int NV>
+__device__ inline void load_row(const typename Elem<DT>::type* p, int64_t cols, int t, Vec16<DT> (&out)[NV]) {
+    constexpr int VEC = Elem<DT>::VEC;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int64_t c = (int64_t)(j * 64 * WPR + t) * VEC;
+        if (j < NV - 1) out[j] = *reinterpret_cast<const Vec16<DT>*>(p + c);
+        else out[j] = load_raw<DT>(p, c, cols);
+    }
+}
+
+// x (as f32, zeros past the row's end) becomes x - mean, zeros past the end.
+template <int VEC, int WPR, int NV>
+__device__ inline void centre(float (&x)[NV * VEC], float mean, int64_t cols, int t) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const bool in = j < NV - 1 || (int64_t)(j * 64 * WPR + t) * VEC + e < cols;
+            x[j * VEC + e] = in ? x[j * VEC + e] - mean : 0.0f;
+        }
+}
+
+template <int DT, int WPR, int NV>
+__global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_fwd_kernel(
+    const typename Elem<DT>::type* __restrict__ x, const typename Elem<DT>::type* __restrict__ w,
+    const typename Elem<DT>::type* __restrict__ b, typename Elem<DT>::type* __restrict__ y, int64_t rows, int64_t cols,
+    float eps) {
+    constexpr int VEC = Elem<DT>::VEC, RPB = WPR < 4 ? 4 / WPR : 1;  // rows of a workgroup
+    __shared__ float slots[2][RPB][WPR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave / WPR, wr = wave % WPR;
+    const int t = wr * 64 + lane;
+    const float inv = 1.0f / (float)cols;
+    Vec16<DT> wv[NV], bv[NV];
+    load_row<DT, WPR, NV>(w, cols, t, wv);
+    load_row<DT, WPR, NV>(b, cols, t, bv);
+    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < rows; r += (int64_t)gridDim.x * RPB) {
+        Vec16<DT> raw[NV];
+        load_row<DT, WPR, NV>(x + r * cols, cols, t, raw);
+        float v[NV * VEC], s[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) unpack<DT>(raw[j], v + j * VEC);
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) s[0] += v[i];
+        row_sums<WPR, 1>(s, slots[0][sub], wr, lane);
+        centre<VEC, WPR, NV>(v, s[0] / (float)cols, cols, t);
+        s[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) s[0] += v[i] * v[i];
+        row_sums<WPR, 1>(s, slots[1][sub], wr, lane);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float wf[VEC], bf[VEC];
+            unpack<DT>(wv[j], wf);
+            unpack<DT>(bv[j], bf);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) wf[e] = v[j * VEC + e] * rstd * wf[e] + bf[e];
+            store_vec<DT>(y + r * cols, (int64_t)(j * 64 * WPR + t) * VEC, cols, wf);
+        }
+    }
+}
+
+// dx, and the workgroup's sums of dw (part[2 * blockIdx.x]) and db (the row after).
+template <int DT, int WPR, int NV>
+__global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
+    const typename Elem<DT>::type* __restrict__ dy, const typename Elem<DT>::type* __restrict__ x,
+    const typename Elem<DT>::type* __restrict__ w, typename Elem<DT>::type* __restrict__ dx, float* __restrict__ part,
+    int64_t rows, int64_t cols, float eps) {
+    constexpr int VEC = Elem<DT>::VEC, RPB = WPR < 4 ? 4 / WPR : 1, EPL = NV * VEC;
+    __shared__ float slots[2][RPB][3 * WPR];
+    __shared__ float fold[RPB > 1 ? RPB * 64 * EPL : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave / WPR, wr = wave % WPR;
+    const int t = wr * 64 + lane;
+    const float inv = 1.0f / (float)cols;
+    Vec16<DT> wv[NV];
+    load_row<DT, WPR, NV>(w, cols, t, wv);
+    float aw[EPL], ab[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) aw[i] = ab[i] = 0.0f;
+    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < rows; r += (int64_t)gridDim.x * RPB) {
+        Vec16<DT> xr[NV], gr[NV];
+        load_row<DT, WPR, NV>(x + r * cols, cols, t, xr);
+        load_row<DT, WPR, NV>(dy + r * cols, cols, t, gr);
+        float v[EPL], g[EPL], s1[1] = {0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) unpack<DT>(xr[j], v + j * VEC);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) s1[0] += v[i];
+        row_sums<WPR, 1>(s1, slots[0][sub], wr, lane);
+        centre<VEC, WPR, NV>(v, s1[0] / (float)cols, cols, t);
+        float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float wf[VEC];
+            unpack<DT>(gr[j], g + j * VEC);
+            unpack<DT>(wv[j], wf);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int i = j * VEC + e;
+                ab[i] += g[i];
+                const float gw = g[i] * wf[e];
+                s[0] += v[i] * v[i];
+                s[1] += gw;
+                s[2] += gw * v[i];
+            }
+        }
+        row_sums<WPR, 3>(s, slots[1][sub], wr, lane);
+        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+        const float c1 = s[1] * inv, c2 = s[2] * inv * rstd;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float wf[VEC];
+            unpack<DT>(wv[j], wf);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int i = j * VEC + e;
+                const float xh = v[i] * rstd;
+                aw[i] += g[i] * xh;
+                wf[e] = rstd * (g[i] * wf[e] - c1 - xh * c2);
+            }
+            store_vec<DT>(dx + r * cols, (int64_t)(j * 64 * WPR + t) * VEC, cols, wf);
+        }
+    }
+    float* out = part + (int64_t)blockIdx.x * 2 * cols;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float (&a)[EPL] = which ? ab : aw;
+        if constexpr (RPB > 1) {
+            // The rows' waves of a workgroup add up through LDS.
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) fold[(sub * EPL + i) * 64 + lane] = a[i];
+            __syncthreads();
+            if (sub == 0)
+#pragma unroll
+                for (int i = 0; i < EPL; ++i)
+                    for (int k = 1; k < RPB; ++k) a[i] += fold[(k * EPL + i) * 64 + lane];
+        }
+        if (sub == 0)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int64_t c = (int64_t)(j * 64 * WPR + t) * VEC;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (c + e < cols) out[which * cols + c + e] = a[j * VEC + e];
+            }
+    }
+}
+
+// Sums of n partial rows of 2 * cols values into dw and db: 32 columns of a
+// workgroup, 8 threads to each, which fold every eighth row and then each other.
+template <int DT>
+__global__ __launch_bounds__(256) void affine_fold_kernel(const float* __restrict__ part, int64_t n, int64_t cols,
+                                                          typename Elem<DT>::type* __restrict__ dw,
+                                                          typename Elem<DT>::type* __restrict__ db) {
+    __shared__ float sums[8][32];
+    const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + c;
+    float s = 0.0f;
+    if (col < 2 * cols)
+        for (int64_t i = k; i < n; i += 8) s += part[i * 2 * cols + col];
+    sums[k][c] = s;
+    __syncthreads();
+    if (k == 0 && col < 2 * cols) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += sums[i][c];
+        if (col < cols) dw[col] = dev::from_f32<DT>(s);
+        else db[col - cols] = dev::from_f32<DT>(s);
+    }
+}
+
+// Longer rows: mean, rstd and, with dy, the means of g and g xh of a row per workgroup.
+template <int DT, bool GRAD>
+__global__ __launch_bounds__(1024) void long_stats_kernel(const typename Elem<DT>::type* __restrict__ dy,
+                                                          const typename Elem<DT>::type* __restrict__ x,
+                                                          const typename Elem<DT>::type* __restrict__ w,
+                                                          float4* __restrict__ stats, int64_t rows, int64_t cols,
+                                                          float eps) {
+    constexpr int VEC = Elem<DT>::VEC;
+    __shared__ float slots[2][3 * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const typename Elem<DT>::type *xr = x + r * cols, *gr = GRAD ? dy + r * cols : nullptr;
+        float s1[1] = {0.0f}, s[3] = {0.0f, 0.0f, 0.0f};
+        for (int64_t c = (int64_t)threadIdx.x * VEC; c < cols; c += 1024 * VEC) {
+            float v[VEC];
+            unpack<DT>(load_raw<DT>(xr, c, cols), v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s1[0] += v[e];
+        }
+        row_sums<16, 1>(s1, slots[0], wave, lane);
+        const float mean = s1[0] / (float)cols;
+        for (int64_t c = (int64_t)threadIdx.x * VEC; c < cols; c += 1024 * VEC) {
+            float v[VEC], g[VEC], wf[VEC];
+            unpack<DT>(load_raw<DT>(xr, c, cols), v);
+            if constexpr (GRAD) {
+                unpack<DT>(load_raw<DT>(gr, c, cols), g);
+                unpack<DT>(load_raw<DT>(w, c, cols), wf);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = c + e < cols ? v[e] - mean : 0.0f;
+                s[0] += d * d;
+                if constexpr (GRAD) {
+                    s[1] += g[e] * wf[e];
+                    s[2] += g[e] * wf[e] * d;
+                }
+            }
+        }
+        row_sums<16, 3>(s, slots[1], wave, lane);
+        if (threadIdx.x == 0) {
+            const float rstd = 1.0f / sqrtf(s[0] / (float)cols + eps);
+            stats[r] = make_float4(mean, rstd, s[1] / (float)cols, s[2] / (float)cols * rstd);
+        }
+    }
+}
+
+// Longer rows, one tile of columns of every gridDim.y-th row: y, or dx and the
+// tile's sums of dw and db over those rows (part, as affine_bwd_kernel's).
+template <int DT, bool GRAD>
+__global__ __launch_bounds__(LONG_TILE / Elem<DT>::VEC) void long_apply_kernel(
+    const typename Elem<DT>::type* __restrict__ dy, const typename Elem<DT>::type* __restrict__ x,
+    const typename Elem<DT>::type* __restrict__ w, const typename Elem<DT>::type* __restrict__ b,
+    const float4* __restrict__ stats, typename Elem<DT>::type* __restrict__ out, float* __restrict__ part, int64_t rows,
+    int64_t cols) {
+    constexpr int VEC = Elem<DT>::VEC;
+    const int64_t c = (int64_t)blockIdx.x * LONG_TILE + threadIdx.x * VEC;
+    if (c >= cols) return;
+    float wf[VEC], bf[VEC], aw[VEC], ab[VEC];
+    unpack<DT>(load_raw<DT>(w, c, cols), wf);
+    if constexpr (!GRAD) unpack<DT>(load_raw<DT>(b, c, cols), bf);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) aw[e] = ab[e] = 0.0f;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        const float4 st = stats[r];
+        float v[VEC], g[VEC];
+        unpack<DT>(load_raw<DT>(x + r * cols, c, cols), v);
+        if constexpr (GRAD) unpack<DT>(load_raw<DT>(dy + r * cols, c, cols), g);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float xh = (v[e] - st.x) * st.y;
+            if constexpr (GRAD) {
+                aw[e] += g[e] * xh;
+                ab[e] += g[e];
+                v[e] = st.y * (g[e] * wf[e] - st.z - xh * st.w);
+            } else {
+                v[e] = xh * wf[e] + bf[e];
+            }
+        }
+        store_vec<DT>(out + r * cols, c, cols, v);
+    }
+    if constexpr (GRAD) {
+        float* p = part + (int64_t)blockIdx.y * 2 * cols;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (c + e < cols) {
+                p[c + e] = aw[e];
+                p[cols + c + e] = ab[e];
+            }
+    }
+}
+
+template <int DT>
+struct Args {
+    typedef typename Elem<DT>::type T;
+    const T *dy, *x, *w, *b;
+    T *out, *dw, *db;
+    float* part;
+    int64_t rows, cols;
+    float eps;
+    bool grad;
+    hipStream_t s;
+};
+
+template <int DT, int WPR, int NV>
+int launch_registers(const Args<DT>& a, int64_t groups) {
+    const int threads = WPR < 4 ? 256 : 64 * WPR;
+    if (a.grad) {
+        hipLaunchKernelGGL((affine_bwd_kernel<DT, WPR, NV>), dim3((unsigned)groups), dim3(threads), 0, a.s, a.dy, a.x, a.w,
+                           a.out, a.part, a.rows, a.cols, a.eps);
+        return launch_check("affine_bwd_kernel");
+    }
+    hipLaunchKernelGGL((affine_fwd_kernel<DT, WPR, NV>), dim3((unsigned)groups), dim3(threads), 0, a.s, a.x, a.w, a.b,
+                       a.out, a.rows, a.cols, a.eps);
+    return launch_check("affine_fwd_kernel");
+}
+
+template <int DT, int WPR>
+int launch_waves(const Args<DT>& a, int64_t groups) {
+    const int nv = (int)ceil_div(a.cols, 64 * WPR * Elem<DT>::VEC);
+    if constexpr (DT == MLXHIP_DTYPE_F32) {
+        if (nv == 4) return launch_registers<DT, WPR, 4>(a, groups);
+        if (nv == 3) return launch_registers<DT, WPR, 3>(a, groups);
+    }
+    if (nv == 2) return launch_registers<DT, WPR, 2>(a, groups);
+    // Four times the waves start at four times the columns: one vector is
+    // left to f32 rows of a single wave and to 16-bit rows.
+    if constexpr (DT != MLXHIP_DTYPE_F32 || WPR == 1) return launch_registers<DT, WPR, 1>(a, groups);
+    return fail(MLXHIP_ERR_INVALID_ARGUMENT, "layernorm_affine: no kernel for %lld columns", (long long)a.cols);
+}
+
+template <int DT>
+int run_affine(Args<DT> a) {
+    const bool registers = a.cols <= MAX_COLS;
+    const int rpb = a.cols <= 1024 ? 4 : 1;  // rows of a workgroup at a time
+    // Forward: eight workgroups to a CU at most, so that each has its weights'
+    // load to share between rows when there are many.
+    int64_t groups = registers ? std::min<int64_t>(ceil_div(a.rows, rpb), a.grad ? PARTIALS : 2048)
+                               : std::min<int64_t>(a.rows, 64);
+    const size_t part = a.grad ? (size_t)groups * 2 * a.cols * sizeof(float) : 0;
+    const size_t stats = registers ? 0 : (size_t)a.rows * sizeof(float4);
+    char* ws = nullptr;
+    if (part + stats) MLXHIP_TRY(stream_workspace(a.s, WS_NORM, part + stats, reinterpret_cast<void**>(&ws)));
+    a.part = reinterpret_cast<float*>(ws + stats);
+    if (a.rows == 0) {
+        // No rows: the fold below writes the zeros of dw and db.
+    } else if (!registers) {
+        float4* st = reinterpret_cast<float4*>(ws);
+        const dim3 grid((unsigned)ceil_div(a.cols, LONG_TILE), (unsigned)groups);
+        const int threads = LONG_TILE / Elem<DT>::VEC;
+        const unsigned blocks = (unsigned)std::min<int64_t>(a.rows, 4096);
+        if (a.grad) {
+            hipLaunchKernelGGL((long_stats_kernel<DT, true>), dim3(blocks), dim3(1024), 0, a.s, a.dy, a.x, a.w, st, a.rows,
+                               a.cols, a.eps);
+            MLXHIP_TRY(launch_check("long_stats_kernel"));
+            hipLaunchKernelGGL((long_apply_kernel<DT, true>), grid, dim3(threads), 0, a.s, a.dy, a.x, a.w, a.b, st, a.out,
+                               a.part, a.rows, a.cols);
+        } else {
+            hipLaunchKernelGGL((long_stats_kernel<DT, false>), dim3(blocks), dim3(1024), 0, a.s, a.dy, a.x, a.w, st, a.rows,
+                               a.cols, a.eps);
+            MLXHIP_TRY(launch_check("long_stats_kernel"));
+            hipLaunchKernelGGL((long_apply_kernel<DT, false>), grid, dim3(threads), 0, a.s, a.dy, a.x, a.w, a.b, st, a.out,
+                               a.part, a.rows, a.cols);
+        }
+        MLXHIP_TRY(launch_check("long_apply_kernel"));
+    } else if (a.cols <= 1024) {
+        MLXHIP_TRY((launch_waves<DT, 1>(a, groups)));
+    } else if (a.cols <= 4096) {
+        MLXHIP_TRY((launch_waves<DT, 4>(a, groups)));
+    } else {
+        MLXHIP_TRY((launch_waves<DT, 16>(a, groups)));
+    }
+    if (!a.grad) return MLXHIP_OK;
+    hipLaunchKernelGGL((affine_fold_kernel<DT>), dim3((unsigned)ceil_div(2 * a.cols, 32)), dim3(256), 0, a.s, a.part, groups,
+                       a.cols, a.dw, a.db);
+    return launch_check("affine_fold_kernel");
+}
+
+int affine(int dt, const void* dy, const void* x, const void* w, const void* b, void* out, void* dw, void* db,
+           int64_t rows, int64_t cols, float eps, bool grad, hipStream_t s) {
+    int rc = MLXHIP_OK;
+    if (!with_float_dtype(dt, [&](auto d) {
+            typedef typename Elem<d.value>::type T;
+            rc = run_affine<d.value>({(const T*)dy, (const T*)x, (const T*)w, (const T*)b, (T*)out, (T*)dw, (T*)db, nullptr,
+                                      rows, cols, eps, grad, s});
+        }))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "layernorm_affine: dtype %d (f32, bf16 or f16)", dt);
+    return rc;
+}
+
+}  // namespace
+
+int layernorm_affine(int dt, const void* x, const void* w, const void* b, void* y, int64_t rows, int64_t cols,
+                     float eps, hipStream_t s) {
+    return affine(dt, nullptr, x, w, b, y, nullptr, nullptr, rows, cols, eps, false, s);
+}
+
+int layernorm_affine_vjp(int dt, const void* dy, const void* x, const void* w, void* dx, void* dw, void* db,
+                         int64_t rows, int64_t cols, float eps, hipStream_t s) {
+    return affine(dt, dy, x, w, nullptr, dx, dw, db, rows, cols, eps, true, s);
+}
+
+}  // namespace mlxhip
