@@ -460,9 +460,12 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * f16 (scaled by a power of two, so that small probabilities stay normal) for
  * the products of 16-bit operands, and dx and dw once as they are stored.
  * Sums are formed in a fixed order. Operands contiguous, at any address
- * aligned to their elements; results must not overlap operands. rows and
- * vocab up to 2^31 - 1, dim up to 2^20, rows * dim below 2^31. Workspace per
- * stream. No reference counterpart. */
+ * aligned to their elements; results must not overlap operands. A non-finite x
+ * or w makes the logits it enters NaN. rows up to 2^21, dim up to 2^20, vocab up
+ * to 2^31 - 1, rows times dim (rounded up to a multiple of 8) up to 2^29: cut a
+ * larger batch by its rows. The workspace (per stream) holds dS for one piece of
+ * the vocabulary, 256 MiB or 256 columns, copies of x and of a piece of w where
+ * needed, and f32 sums of dx. No reference counterpart. */
 int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,
                                 float* loss, float* lse, int64_t rows, int64_t dim, int64_t vocab,
                                 void* stream);

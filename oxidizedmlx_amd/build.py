@@ -53,6 +53,9 @@ SOURCES = [
     "kernels/norm_affine.hip",
     "kernels/embedding.hip",
     "kernels/cross_entropy.hip",
+    "kernels/ce_bf16.hip",
+    "kernels/ce_f16.hip",
+    "kernels/ce_f32.hip",
     "kernels/elementwise.hip",
     "kernels/gemm.hip",
     "kernels/gemm_small.hip",

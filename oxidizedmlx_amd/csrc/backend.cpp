@@ -1107,10 +1107,11 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
 namespace {
 // Sizes of the cross entropy's entry points.
 int check_cross_entropy(const char* what, int64_t rows, int64_t dim, int64_t vocab) {
-    MLXHIP_TRY(check_sizes(what, {rows, dim, vocab}, {INT32_MAX, 1 << 20, INT32_MAX}));
+    MLXHIP_TRY(check_sizes(what, {rows, dim, vocab}, {1 << 21, 1 << 20, INT32_MAX}));
     if (dim == 0 || vocab == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: no logits (dim or vocab is 0)", what);
-    if (rows * dim > INT32_MAX)
-        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: rows * dim = %lld is over 2^31 - 1", what, (long long)(rows * dim));
+    // The kernels' offsets within x's three planes are 32-bit bytes.
+    if (rows * (ceil_div(dim, 8) * 8) > (1 << 29))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: rows * dim = %lld is over 2^29", what, (long long)(rows * dim));
     return MLXHIP_OK;
 }
 }  // namespace

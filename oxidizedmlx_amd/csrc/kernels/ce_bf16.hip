@@ -1,0 +1,10 @@
+// ce_bf16.hip — the linear cross entropy's products of bf16 operands (ce_gemm.hpp).
+#include "ce_gemm.hpp"
+
+namespace mlxhip {
+
+int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s) {
+    return ce::dispatch<MLXHIP_DTYPE_BF16, MLXHIP_DTYPE_BF16, 1>(which, large, a, s);
+}
+
+}  // namespace mlxhip

@@ -1,0 +1,454 @@
+// ce_gemm.hpp — the matrix products of the linear cross entropy on the 16-bit
+// matrix cores, with the loss's row operations in their epilogues.
+//
+//   CE_STATS  z = x W^T; per tile and row the maximum and the sum of
+//             exp(z - max), and the target's logit: the logits leave the
+//             registers only as these.
+//   CE_DS     z again; dS = exp(z - lse) - [v = target], times the row's
+//             factor, stored in 16 bits (f32: as three bf16 planes).
+//   CE_DX     f32 sums of dS W over a slice of K, added to those of the
+//             pieces of the vocabulary before.
+//   CE_DW     dS^T x times a power of two, in the operands' type.
+//
+// Operands are bf16 or f16, or f32 as three bf16 planes whose sum is the value
+// (P = 3: the six plane products above 2^-24 of the whole, smallest first, as
+// the f32 products of gemm16_x6.hip). Tiles are fed by direct global->LDS
+// loads, STAGES K tiles of 32 deep, with the building blocks and LDS layouts of
+// gemm16_impl.hpp.
+#pragma once
+
+#include "elem.hpp"
+#include "gemm16_impl.hpp"
+
+namespace mlxhip {
+namespace ce {
+
+using gemm16::BK;
+using gemm16::f32x16;
+using gemm16::f32x4;
+using gemm16::u32x2;
+using gemm16::u32x4;
+
+// 16 bytes at an element's alignment.
+typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
+typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
+
+enum Product { CE_STATS = 0, CE_DS = 1, CE_DX = 2, CE_DW = 3 };
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// WM x WN waves of TM x TN 32x32 tiles, P planes of both operands in each of
+// STAGES stages.
+template <int WM_, int WN_, int TM_, int TN_, int STAGES_, int P_>
+struct Cfg {
+    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, STAGES = STAGES_, P = P_;
+    static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
+    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;  // one plane of one stage
+    static constexpr int STAGE_BYTES = P * (A_BYTES + B_BYTES);         // A's planes, then B's
+    static constexpr int LA = A_BYTES / (THREADS * 16), LB = B_BYTES / (THREADS * 16);  // loads per thread and plane
+    static_assert(BM >= 128 && BN >= 128, "MN-contiguous LDS rows need >= 16 chunks for the swizzle");
+    static_assert(LA * THREADS * 16 == A_BYTES && LB * THREADS * 16 == B_BYTES, "whole 1 KiB blocks per wave");
+    static_assert(STAGES >= 2 && STAGES * STAGE_BYTES <= 160 * 1024, "LDS budget");
+};
+template <int P>
+using Large = std::conditional_t<P == 1, Cfg<2, 4, 4, 2, 4, 1>, Cfg<4, 2, 2, 2, 2, 3>>;  // 256 x 256, 256 x 128
+template <int P>
+using Small = std::conditional_t<P == 1, Cfg<2, 2, 2, 2, 4, 1>, Cfg<2, 4, 2, 1, 3, 3>>;  // 128 x 128, two to a CU / one
+
+struct Args {
+    // op(A) [m, k], op(B) [k, n]; planes of an operand *_plane elements apart.
+    const uint16_t *a = nullptr, *b = nullptr;
+    int64_t lda = 0, ldb = 0, a_plane = 0, b_plane = 0;
+    int64_t m = 0, n = 0;
+    int64_t ka = 0, kb = 0;  // K extent of each operand's memory; zeros beyond
+    int tiles_m = 0, tiles_n = 0;
+    int splits = 1;          // CE_DX: slices of K, of k_chunk (a multiple of 32) each
+    int64_t k_chunk = 0;
+    // Rows of x: target column relative to n = 0 (the piece's first), and
+    // (-lse log2 e, factor) with factor 0 for a row that is not counted.
+    const int32_t* targets = nullptr;
+    int64_t v0 = 0;
+    const float2* row = nullptr;
+    float2* stats = nullptr;    // CE_STATS: [tiles_n][m], this launch's first tile
+    float* target_z = nullptr;  // CE_STATS: [m]
+    uint16_t* ds = nullptr;     // CE_DS: [P][m][ldc]
+    float* dx = nullptr;        // CE_DX: [splits][m][ldc]
+    bool add = false;           // CE_DX: add to what is there
+    void* dw = nullptr;         // CE_DW: [m][ldc]
+    const float* scale = nullptr;
+    int64_t ldc = 0;
+};
+
+// Max and sum of exp(z - max) of two groups of a row.
+__device__ inline void merge(float& m, float& s, float m2, float s2) {
+    const float mn = fmaxf(m, m2);
+    const float base = mn == -INFINITY ? 0.0f : mn;
+    s = s * __builtin_amdgcn_exp2f((m - base) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - base) * LOG2E);
+    m = mn;
+}
+
+// A target's place from column v on, -1 where it is not among `width` of them.
+__device__ inline int column_of(int32_t target, int64_t v, int width) {
+    const int64_t c = target - v;
+    return c >= 0 && c < width ? (int)c : -1;
+}
+
+// The tile of a workgroup: consecutive ids go to the 8 XCDs in turn, so each
+// XCD takes a contiguous range of tiles, in groups of four tile rows.
+template <class C>
+__device__ inline void tile_of(const Args& g, int64_t* m0, int64_t* n0, int* split) {
+    const int nwg = g.tiles_m * g.tiles_n, total = nwg * g.splits;
+    const int xcd = blockIdx.x & 7, per = total >> 3, rest = total & 7;
+    const int lin = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
+    *split = lin / nwg;
+    const int id = lin - *split * nwg;
+    constexpr int GROUP_M = 4;
+    const int in_group = GROUP_M * g.tiles_n, first = id / in_group * GROUP_M;
+    const int rows = min(g.tiles_m - first, GROUP_M);
+    *m0 = (int64_t)(first + id % in_group % rows) * C::BM;
+    *n0 = (int64_t)(id % in_group / rows) * C::BN;
+}
+
+// Descriptor of an operand's part that the tile at row / column r0 (of R) and
+// k from k0 on reads. KC: [R][k] in memory, else [k][R] with rows of ld.
+template <bool KC, int ROWS, int P>
+__device__ inline __amdgpu_buffer_rsrc_t operand(const uint16_t* p, int64_t plane, int64_t ld, int64_t r0, int64_t R,
+                                                 int64_t k0, int64_t k) {
+    const uint16_t* at = p + (KC ? r0 * ld + k0 : k0 * ld + r0);
+    const int64_t rows = min(R - r0, (int64_t)ROWS);
+    const int64_t ext = (KC ? (rows - 1) * ld + k : (k - 1) * ld + min((rows + 7) / 8 * 8, ld - r0)) + (P - 1) * plane;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, (int)(uint32_t)(ext * 2), gemm16::BUF_FLAGS);
+}
+
+// Stores the tile of values v(i, j, e) = acc[i][j][e] through the wave's LDS
+// rows, whole row segments at a time: 16-byte vectors at any element alignment
+// where they end before column `cap`, single elements up to column g.n else.
+// ACC (f32): added to what is there.
+template <int CT, class C, int PIPE_BYTES, bool ACC, bool NT>
+__device__ inline void store_tile(const f32x16 (&acc)[C::TM][C::TN], MLXHIP_LDS char* smem, typename dev::Elem<CT>::type* out,
+                                  int64_t ld, int64_t m, int64_t n, int64_t cap, int64_t m0, int64_t n0, int wave,
+                                  int lane, bool add) {
+    typedef typename dev::Elem<CT>::type T;
+    typedef std::conditional_t<sizeof(T) == 4, u32x4_at4, u32x4_at2> any;
+    constexpr int TM = C::TM, TN = C::TN, ES = sizeof(T), VEC = 16 / ES;
+    constexpr int PASS = gemm16::pass_rows<C, ES>(PIPE_BYTES);
+    constexpr int ROW_BYTES = 32 * TN * ES, PITCH = ROW_BYTES + 16;
+    constexpr int LANES = ROW_BYTES / 16, ROWS = 64 / LANES;
+    const int wm = wave / C::WN, wn = wave % C::WN;
+    MLXHIP_LDS char* region = smem + wave * PASS * PITCH;
+    const int64_t row0 = m0 + 32 * TM * wm, col0 = n0 + 32 * TN * wn;
+#pragma unroll
+    for (int pass = 0; pass < 32 * TM / PASS; ++pass) {
+#pragma unroll
+        for (int i = 0; i < PASS / 32; ++i) {
+            const int r = 32 * i + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    MLXHIP_LDS char* p = region + r * PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * ES;
+                    const f32x16& a = acc[pass * (PASS / 32) + i][j];
+                    if constexpr (ES == 4)
+                        *(MLXHIP_LDS f32x4*)p = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                    else
+                        *(MLXHIP_LDS u32x2*)p = u32x2{gemm16::pack2<CT>(a[4 * q], a[4 * q + 1]),
+                                                      gemm16::pack2<CT>(a[4 * q + 2], a[4 * q + 3])};
+                }
+        }
+        // Read back by the same wave, whose LDS accesses complete in order.
+#pragma unroll 4
+        for (int rr = 0; rr < PASS; rr += ROWS) {
+            const int r = rr + lane / LANES, cb = lane % LANES * 16;
+            u32x4 v = *(const MLXHIP_LDS u32x4*)(region + r * PITCH + cb);
+            const int64_t row = row0 + pass * PASS + r, col = col0 + cb / ES;
+            if (row >= m || col >= n) continue;
+            T* dst = out + row * ld + col;
+            if (col + VEC <= cap) {
+                if constexpr (ACC) {
+                    if (add) {
+                        const u32x4 had = *reinterpret_cast<const u32x4*>(dst);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = __float_as_uint(__uint_as_float(had[e]) + __uint_as_float(v[e]));
+                    }
+                }
+                if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<any*>(dst));
+                else *reinterpret_cast<any*>(dst) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (col + e >= n) break;
+                    if constexpr (ES == 4) dst[e] = __uint_as_float(v[e]);
+                    else dst[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+                }
+            }
+        }
+    }
+}
+
+// MT: type of the planes (BF16, F16); OT: type of the operator's operands.
+template <int PRODUCT, int MT, int OT, class C>
+__global__ __attribute__((amdgpu_flat_work_group_size(C::THREADS, C::THREADS), amdgpu_waves_per_eu(2, 2)))
+void ce_gemm_kernel(Args g) {
+    constexpr bool KCA = PRODUCT != CE_DW, KCB = PRODUCT <= CE_DS;
+    constexpr int STAGES = C::STAGES, TM = C::TM, TN = C::TN, WAVES = C::WAVES, P = C::P;
+    constexpr int PAIRS = P == 1 ? 1 : gemm16::X6_SEGS;
+    constexpr int PIPE_BYTES = STAGES * C::STAGE_BYTES;
+    constexpr int STORED = PRODUCT == CE_DX ? MLXHIP_DTYPE_F32 : PRODUCT == CE_DW ? OT : MT;
+    constexpr int EPI_BYTES = gemm16::epi_bytes<STORED, C, PIPE_BYTES>();
+    constexpr int SMEM_BYTES = PIPE_BYTES > EPI_BYTES ? PIPE_BYTES : EPI_BYTES;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[SMEM_BYTES];
+    MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / C::WN, wn = wave % C::WN;
+    int64_t m0, n0;
+    int split;
+    tile_of<C>(g, &m0, &n0, &split);
+
+    const int64_t k0 = PRODUCT == CE_DX ? split * g.k_chunk : 0;
+    const int64_t most = PRODUCT == CE_DX && g.splits > 1 ? g.k_chunk : INT64_MAX;
+    const int64_t ka = min(g.ka - k0, most), kb = min(g.kb - k0, most);
+    const __amdgpu_buffer_rsrc_t ra = operand<KCA, C::BM, P>(g.a, g.a_plane, g.lda, m0, g.m, k0, ka);
+    const __amdgpu_buffer_rsrc_t rb = operand<KCB, C::BN, P>(g.b, g.b_plane, g.ldb, n0, g.n, k0, kb);
+    const uint32_t plane_a = (uint32_t)(g.a_plane * 2), plane_b = (uint32_t)(g.b_plane * 2);
+    constexpr int ROWB_A = C::BM * 2, ROWB_B = C::BN * 2;
+    gemm16::Loader<KCA, C::BM, WAVES> la;
+    gemm16::Loader<KCB, C::BN, WAVES> lb;
+    la.init(tid, 0, g.m - m0, g.lda, ka);
+    lb.init(tid, 0, g.n - n0, g.ldb, kb);
+    gemm16::FragAddr<KCA, TM, ROWB_A> fa;
+    gemm16::FragAddr<KCB, TN, ROWB_B> fb;
+    fa.init(lane, 32 * TM * wm);
+    fb.init(lane, 32 * TN * wn);
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+
+    const int nk = (int)((max(ka, kb) + BK - 1) / BK);
+    constexpr int LA = C::LA, LB = C::LB, LPT = P * (LA + LB), B0 = P * C::A_BYTES;
+#pragma unroll
+    for (int t = 0; t < STAGES; ++t) {
+        MLXHIP_LDS char* st = smem + t * C::STAGE_BYTES;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            la.issue(ra, st + p * C::A_BYTES, wave, t * BK, (uint32_t)p * plane_a);
+            lb.issue(rb, st + B0 + p * C::B_BYTES, wave, t * BK, (uint32_t)p * plane_b);
+        }
+    }
+    gemm16::wait_vmcnt<(STAGES - 1) * LPT>();
+    gemm16::lds_barrier();
+
+    constexpr int NA = KCA ? TM : 2 * TM, NB = KCB ? TN : 2 * TN, NR = P * (NA + NB);
+    u32x4 af[2][P][TM], bf[2][P][TN];
+    auto read_op = [&](const MLXHIP_LDS char* st, int s, int o) {
+        if (o < P * NA) {
+            const int p = o / NA;
+            gemm16::read_one<KCA, TM, ROWB_A>(st + p * C::A_BYTES, fa, s, o - p * NA, af[s][p]);
+        } else {
+            const int ob = o - P * NA, p = ob / NB;
+            gemm16::read_one<KCB, TN, ROWB_B>(st + B0 + p * C::B_BYTES, fb, s, ob - p * NB, bf[s][p]);
+        }
+    };
+#pragma unroll
+    for (int o = 0; o < NR; ++o) read_op(smem, 0, o);
+
+    // Per K tile two steps of 16: each step's MFMAs with the next step's LDS
+    // reads, and in the second the loads of the tile STAGES on, between them.
+    constexpr int NM = TM * TN, NMI = PAIRS * NM, OPS = NR + LPT;
+    for (int kt = 0; kt < nk; ++kt) {
+        const int cur = kt % STAGES;
+        const MLXHIP_LDS char* st = smem + cur * C::STAGE_BYTES;
+#pragma unroll
+        for (int q = 0; q < NMI; ++q) {
+            const int e = q / NM, t = q % NM;
+            gemm16::mfma<MT>(bf[0][P == 1 ? 0 : gemm16::seg_plane_b(e)][t % TN],
+                             af[0][P == 1 ? 0 : gemm16::seg_plane_a(e)][t / TN], acc[t / TN][t % TN]);
+#pragma unroll
+            for (int o = NR <= NMI ? (q < NR ? q : NR) : (q * NR) / NMI; o < (NR <= NMI ? (q < NR ? q + 1 : NR) : ((q + 1) * NR) / NMI); ++o)
+                read_op(st, 1, o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // Tile kt+1 has landed for every wave; every wave has read this tile's
+        // stage, which then receives tile kt+STAGES.
+        gemm16::wait_vmcnt<(STAGES - 2) * LPT>();
+        gemm16::lds_barrier();
+        MLXHIP_LDS char* dst = smem + cur * C::STAGE_BYTES;
+        const int kl = (kt + STAGES) * BK;
+        const MLXHIP_LDS char* nx = smem + ((kt + 1) % STAGES) * C::STAGE_BYTES;
+#pragma unroll
+        for (int q = 0; q < NMI; ++q) {
+            const int e = q / NM, t = q % NM;
+            gemm16::mfma<MT>(bf[1][P == 1 ? 0 : gemm16::seg_plane_b(e)][t % TN],
+                             af[1][P == 1 ? 0 : gemm16::seg_plane_a(e)][t / TN], acc[t / TN][t % TN]);
+#pragma unroll
+            for (int o = (q * OPS) / NMI; o < ((q + 1) * OPS) / NMI; ++o) {
+                if (o < NR) {
+                    read_op(nx, 0, o);
+                } else if (o < NR + P * LA) {
+                    const int p = (o - NR) / LA;
+                    la.issue_one(ra, dst + p * C::A_BYTES, wave, kl, o - NR - p * LA, (uint32_t)p * plane_a);
+                } else {
+                    const int ob = o - NR - P * LA, p = ob / LB;
+                    lb.issue_one(rb, dst + B0 + p * C::B_BYTES, wave, kl, ob - p * LB, (uint32_t)p * plane_b);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    gemm16::wait_vmcnt<0>();
+    gemm16::lds_barrier();  // every wave is done with the operand stages
+
+    // acc[i][j][4 q + e] is row 32 i + lane % 32, column 32 j + 8 q +
+    // 4 (lane / 32) + e of the wave's part.
+    const int64_t row0 = m0 + 32 * TM * wm + (lane & 31), col0 = n0 + 32 * TN * wn + 4 * (lane >> 5);
+    if constexpr (PRODUCT == CE_STATS) {
+        MLXHIP_LDS float* red = (MLXHIP_LDS float*)smem;  // [WN][2][BM]
+        const bool edge = n0 + C::BN > g.n;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t r = row0 + 32 * i;
+            // The target's logit, from the lane that holds its column.
+            const int tc = r < g.m ? column_of(g.targets[r], g.v0 + col0, 32 * TN) : -1;
+            const bool mine = tc >= 0 && (tc & 4) == 0 && tc + col0 < g.n;
+            if (__ballot(mine)) {
+                float z = 0.0f;
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) z = acc[i][j][v];
+                if (mine) g.target_z[r] = z;
+            }
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (col0 + 32 * j + 8 * (v >> 2) + (v & 3) >= g.n) acc[i][j][v] = -INFINITY;
+            }
+            float mx = acc[i][0][0];
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, acc[i][j][v]);
+            // exp(z - mx) as exp2(z log2 e - mb), mb = mx log2 e rounded; what
+            // that rounding leaves is put right in the sum.
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            const float mb = base * LOG2E;
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], LOG2E, -mb));
+            s *= __builtin_amdgcn_exp2f(__builtin_fmaf(-base, LOG2E, mb));
+            merge(mx, s, __shfl_xor(mx, 32, 64), __shfl_xor(s, 32, 64));
+            if (lane < 32) {
+                MLXHIP_LDS float* p = red + 2 * wn * C::BM + 32 * TM * wm + 32 * i + lane;
+                p[0] = mx;
+                p[C::BM] = s;
+            }
+        }
+        __syncthreads();
+        if (tid < C::BM && m0 + tid < g.m) {
+            float2 a = make_float2(red[tid], red[C::BM + tid]);
+#pragma unroll
+            for (int w = 1; w < C::WN; ++w) merge(a.x, a.y, red[2 * w * C::BM + tid], red[(2 * w + 1) * C::BM + tid]);
+            g.stats[n0 / C::BN * g.m + m0 + tid] = a;
+        }
+    } else if constexpr (PRODUCT == CE_DS) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t r = row0 + 32 * i;
+            const float2 p = r < g.m ? g.row[r] : make_float2(0.0f, 0.0f);
+            const int tc = r < g.m ? column_of(g.targets[r], g.v0 + col0, 32 * TN) : -1;
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int c = 32 * j + 8 * (v >> 2) + (v & 3);
+                    float q = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], LOG2E, p.x));
+                    if (tc == c) q -= 1.0f;
+                    // A row that is not counted is 0 whatever its lse is.
+                    acc[i][j][v] = p.y == 0.0f || col0 + c >= g.n ? 0.0f : q * p.y;
+                }
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            store_tile<MT, C, PIPE_BYTES, false, false>(acc, smem, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, m0, n0,
+                                                        wave, lane, false);
+            if (p + 1 < P) {
+                // What the plane leaves (exact in f32).
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)
+                            acc[i][j][v] -= dev::to_f32<MT>(dev::from_f32<MT>(acc[i][j][v]));
+            }
+        }
+    } else {
+        if constexpr (PRODUCT == CE_DW) {
+            const float f = g.scale[0];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
+            store_tile<OT, C, PIPE_BYTES, false, true>(acc, smem, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m,
+                                                       g.n, g.n, m0, n0, wave, lane, false);
+        } else {
+            store_tile<MLXHIP_DTYPE_F32, C, PIPE_BYTES, true, false>(acc, smem, g.dx + split * g.m * g.ldc, g.ldc, g.m, g.n,
+                                                                     g.ldc, m0, n0, wave, lane, g.add);
+        }
+    }
+}
+
+template <int PRODUCT, int MT, int OT, class C>
+int launch(Args a, hipStream_t s) {
+    a.tiles_m = (int)ceil_div(a.m, C::BM);
+    a.tiles_n = (int)ceil_div(a.n, C::BN);
+    hipLaunchKernelGGL((ce_gemm_kernel<PRODUCT, MT, OT, C>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)),
+                       dim3(C::THREADS), 0, s, a);
+    return launch_check("ce_gemm_kernel");
+}
+
+// The product's large or small tiles.
+template <int PRODUCT, int MT, int OT, int P>
+int product(bool large, const Args& a, hipStream_t s) {
+    return large ? launch<PRODUCT, MT, OT, Large<P>>(a, s) : launch<PRODUCT, MT, OT, Small<P>>(a, s);
+}
+
+template <int MT, int OT, int P>
+int dispatch(int which, bool large, const Args& a, hipStream_t s) {
+    switch (which) {
+        case CE_STATS: return product<CE_STATS, MT, OT, P>(large, a, s);
+        case CE_DS: return product<CE_DS, MT, OT, P>(large, a, s);
+        case CE_DX: return product<CE_DX, MT, OT, P>(large, a, s);
+        default: return product<CE_DW, MT, OT, P>(large, a, s);
+    }
+}
+
+// Tile sizes of the two forms.
+template <int P>
+constexpr int large_bm() { return Large<P>::BM; }
+template <int P>
+constexpr int large_bn() { return Large<P>::BN; }
+
+}  // namespace ce
+
+// ce_bf16.hip, ce_f16.hip, ce_f32.hip: the products of operands of each type.
+int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s);
+int ce_gemm_f16(int which, bool large, const ce::Args& a, hipStream_t s);
+int ce_gemm_f32(int which, bool large, const ce::Args& a, hipStream_t s);
+
+}  // namespace mlxhip

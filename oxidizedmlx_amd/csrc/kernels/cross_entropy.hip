@@ -1,14 +1,27 @@
 // cross_entropy.hip — softmax cross entropy of the logits x W^T of an output
 // projection, and the gradients of x and W, in pieces of the vocabulary: the
-// logits are never held whole.
+// logits are never held.
 //
 //   z_rv   = sum_k x_rk W_vk
-//   lse_r  = log sum_v exp(z_rv)          (running maximum and sum)
+//   lse_r  = log sum_v exp(z_rv)
 //   loss_r = lse_r - z_r,t(r)             (0 for a target outside [0, vocab))
 //   dS_rv  = dloss_r (exp(z_rv - lse_r) - [v = t(r)])   (0 for such a target)
 //   dx = dS W,  dW = dS^T x
+//
+// Forward: one product whose tiles leave each row's maximum and sum over their
+// columns (ce_gemm.hpp), and a launch that joins them. Backward, per piece of
+// the vocabulary: the product again, stored as dS in 16 bits (f32: three bf16
+// planes), then dW of the piece whole and dx's share added to f32 sums, which
+// a last launch scales and rounds. Four products of 2 R D V operations; at
+// several hundred rows the matrix cores bound them.
+//
+// x is copied once with zeros in the rows without a target (whatever they hold
+// must not reach dW through a product with 0) and its rows rounded up to whole
+// 16-byte chunks; W is read in place where its rows are such chunks, else
+// copied piece by piece; f32 operands are split into planes by the same copies.
 #include "../common.hpp"
 #include "../kernels.hpp"
+#include "ce_gemm.hpp"
 #include "device_math.hpp"
 #include "elem.hpp"
 
@@ -17,108 +30,137 @@
 namespace mlxhip {
 namespace {
 
+using ce::Args;
 using dev::Elem;
 
-constexpr float LOG2E = 1.44269504088896340736f;
-// Bytes of one piece's logits.
-constexpr int64_t PIECE_BYTES = int64_t(128) << 20;
+constexpr float LN2 = 0.69314718055994530942f;
+// Bytes of a piece's dS, and of a copied piece of W.
+constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
 
 __device__ inline bool counted(int32_t t, int64_t vocab) { return t >= 0 && t < vocab; }
 
-// Running maximum and sum of a row over one more piece of its logits, and the
-// target's logit where the piece holds it; a workgroup per row.
-__global__ __launch_bounds__(256) void ce_stats_kernel(const float* __restrict__ z, int64_t rows, int64_t width, int64_t v0,
-                                                       const int32_t* __restrict__ targets, float2* __restrict__ stats,
-                                                       float* __restrict__ target_z, bool first) {
-    __shared__ float2 waves[4];
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const float* p = z + r * width;
-        float m = -INFINITY;
-        for (int64_t c = threadIdx.x; c < width; c += 256) m = fmaxf(m, p[c]);
-        m = dev::wave_max(m);
-        float s = 0.0f;
-        const float base = m == -INFINITY ? 0.0f : m;
-        for (int64_t c = threadIdx.x; c < width; c += 256) s += exp2f((p[c] - base) * LOG2E);
-        s = dev::wave_sum(s);
-        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(m, s);
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float2 a = first ? make_float2(-INFINITY, 0.0f) : stats[r];
-            for (int w = 0; w < 4; ++w) {
-                const float2 b = waves[w];
-                const float mn = fmaxf(a.x, b.x);
-                const float mb = mn == -INFINITY ? 0.0f : mn;
-                a = make_float2(mn, a.y * exp2f((a.x - mb) * LOG2E) + b.y * exp2f((b.x - mb) * LOG2E));
+// src [rows][dim] as planes of [rows][dim_p] (zeros past dim, and in the rows
+// without a target where targets are given), 8 columns a thread.
+template <int OT, int P>
+__global__ __launch_bounds__(256) void pack_kernel(const typename Elem<OT>::type* __restrict__ src, int64_t rows,
+                                                   int64_t dim, int64_t dim_p, const int32_t* __restrict__ targets,
+                                                   int64_t vocab, uint16_t* __restrict__ dst) {
+    constexpr int VEC = Elem<OT>::VEC;
+    const int64_t chunks = dim_p / 8, plane = rows * dim_p;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+        const bool on = !targets || counted(targets[r], vocab);
+        union {
+            uint16_t h[8];
+            uint4 q;
+        } out;
+        if constexpr (P == 1) {
+            const dev::Vec16<OT> v = dev::load_raw<OT>(src + r * dim, c, dim);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out.h[e] = on ? v.v[e] : 0;
+            *reinterpret_cast<uint4*>(dst + r * dim_p + c) = out.q;
+        } else {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8 / VEC; ++k) dev::unpack<OT>(dev::load_raw<OT>(src + r * dim, c + k * VEC, dim), v + k * VEC);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (p == 0 && !on) v[e] = 0.0f;
+                    out.h[e] = dev::from_f32<MLXHIP_DTYPE_BF16>(v[e]);
+                    v[e] -= dev::to_f32<MLXHIP_DTYPE_BF16>(out.h[e]);
+                }
+                *reinterpret_cast<uint4*>(dst + p * plane + r * dim_p + c) = out.q;
             }
-            stats[r] = a;
-            const int64_t t = (int64_t)targets[r] - v0;
-            if (t >= 0 && t < width) target_z[r] = p[t];
         }
-        __syncthreads();
     }
 }
 
-__global__ __launch_bounds__(256) void ce_loss_kernel(const float2* __restrict__ stats, const float* __restrict__ target_z,
-                                                      const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
-                                                      float* __restrict__ loss, float* __restrict__ lse) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r >= rows) return;
-    const float2 a = stats[r];
-    const float l = a.x + logf(a.y);
+// A row's maxima and sums over the tiles joined, 8 threads to a row.
+__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t tiles,
+                                                   const float* __restrict__ target_z, const int32_t* __restrict__ targets,
+                                                   int64_t rows, int64_t vocab, float* __restrict__ loss,
+                                                   float* __restrict__ lse) {
+    __shared__ float2 part[8][32];
+    const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const int64_t r = (int64_t)blockIdx.x * 32 + c;
+    float m = -INFINITY, s = 0.0f;
+    if (r < rows)
+        for (int64_t t = k; t < tiles; t += 8) {
+            const float2 a = stats[t * rows + r];
+            ce::merge(m, s, a.x, a.y);
+        }
+    part[k][c] = make_float2(m, s);
+    __syncthreads();
+    if (k || r >= rows) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) ce::merge(m, s, part[i][c].x, part[i][c].y);
+    const float l = m + LN2 * __builtin_amdgcn_logf(s);
     lse[r] = l;
     loss[r] = counted(targets[r], vocab) ? l - target_z[r] : 0.0f;
 }
 
-// z becomes dS.
-__global__ __launch_bounds__(256) void ce_grad_kernel(float* __restrict__ z, int64_t rows, int64_t width, int64_t v0,
-                                                      int64_t vocab, const int32_t* __restrict__ targets,
-                                                      const float* __restrict__ lse, const float* __restrict__ dloss) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int32_t t = targets[r];
-        const bool on = counted(t, vocab);
-        const float l = lse[r], g = dloss[r];
-        for (int64_t c = threadIdx.x; c < width; c += 256) {
-            const float p = exp2f((z[r * width + c] - l) * LOG2E);
-            z[r * width + c] = on ? g * (v0 + c == t ? p - 1.0f : p) : 0.0f;
+// f16: the factor that brings the largest dloss of a counted row to 2^15 times
+// a value in [1/2, 1], so that dS's small probabilities stay normal numbers
+// (scale[1]), and its inverse for the results (scale[0]); both powers of two.
+// The other types hold dS as it is.
+__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ dloss, const int32_t* __restrict__ targets,
+                                                     int64_t rows, int64_t vocab, bool f16, float* __restrict__ scale) {
+    __shared__ float waves[16];
+    float m = 0.0f;
+    if (f16)
+        for (int64_t r = threadIdx.x; r < rows; r += 1024)
+            if (counted(targets[r], vocab)) m = fmaxf(m, fabsf(dloss[r]));
+    m = dev::wave_max(m);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, waves[i]);
+    int e = 15;
+    if (f16 && m > 0.0f && m < INFINITY) e = min(max(ilogbf(m) + 1, -100), 128);
+    scale[0] = ldexpf(1.0f, e - 15);
+    scale[1] = ldexpf(1.0f, 15 - e);
+}
+
+__global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ lse, const float* __restrict__ dloss,
+                                                   const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
+                                                   const float* __restrict__ scale, float2* __restrict__ row) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= rows) return;
+    row[r] = counted(targets[r], vocab) ? make_float2(-lse[r] * ce::LOG2E, dloss[r] * scale[1]) : make_float2(0.0f, 0.0f);
+}
+
+// dx from the f32 sums of its slices of K, zeros where there is no target.
+template <int OT>
+__global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums, int splits, int64_t rows, int64_t dim,
+                                                 int64_t ld, const int32_t* __restrict__ targets, int64_t vocab,
+                                                 const float* __restrict__ scale, typename Elem<OT>::type* __restrict__ dx) {
+    const int64_t quads = ld / 4, n = rows * quads;
+    const float f = scale[0];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / quads, c = (i - r * quads) * 4;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (counted(targets[r], vocab)) {
+#pragma unroll 4
+            for (int k = 0; k < splits; ++k) {
+                const float4 v = *reinterpret_cast<const float4*>(sums + ((int64_t)k * rows + r) * ld + c);
+                a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
+            }
         }
+        const float v[4] = {a.x * f, a.y * f, a.z * f, a.w * f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < dim) dx[r * dim + c + e] = dev::from_f32<OT>(v[e]);
     }
-}
-
-// x as f32, zeros in the rows without a target (whatever they hold must not
-// reach dW through a product with 0).
-template <int DT>
-__global__ __launch_bounds__(256) void ce_rows_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows,
-                                                      int64_t dim, int64_t vocab, const int32_t* __restrict__ targets,
-                                                      float* __restrict__ out) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const bool on = !targets || counted(targets[r], vocab);
-        for (int64_t c = threadIdx.x; c < dim; c += 256) out[r * dim + c] = on ? dev::to_f32<DT>(x[r * dim + c]) : 0.0f;
-    }
-}
-
-// Rows of sum (f32) into dx, zeros where there is no target.
-template <int DT>
-__global__ __launch_bounds__(256) void ce_out_kernel(const float* __restrict__ sum, int64_t rows, int64_t dim, int64_t vocab,
-                                                     const int32_t* __restrict__ targets,
-                                                     typename Elem<DT>::type* __restrict__ out) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const bool on = !targets || counted(targets[r], vocab);
-        for (int64_t c = threadIdx.x; c < dim; c += 256) out[r * dim + c] = dev::from_f32<DT>(on ? sum[r * dim + c] : 0.0f);
-    }
-}
-
-__global__ __launch_bounds__(256) void ce_add_kernel(float* __restrict__ acc, const float* __restrict__ v, int64_t n,
-                                                     bool first) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        acc[i] = first ? v[i] : acc[i] + v[i];
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ce_zero_kernel(T* __restrict__ p, int64_t n) {
+__global__ __launch_bounds__(256) void zero_kernel(T* __restrict__ p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = T(0);
 }
 
-unsigned row_grid(int64_t rows) { return (unsigned)std::min<int64_t>(rows, 1 << 20); }
+unsigned grid_for(int64_t threads) { return (unsigned)std::min<int64_t>(ceil_div(threads, 256), 8192); }
 
 // Sub-blocks of one workspace.
 struct Carve {
@@ -130,104 +172,174 @@ struct Carve {
     }
 };
 
-int64_t piece_width(int64_t rows, int64_t vocab) {
-    const int64_t w = std::max<int64_t>(PIECE_BYTES / 4 / std::max<int64_t>(rows, 1) / 256 * 256, 1024);
-    return std::min(w, vocab);
-}
+template <int OT>
+struct Op {
+    typedef typename Elem<OT>::type T;
+    static constexpr int P = OT == MLXHIP_DTYPE_F32 ? 3 : 1;
+    const T *x, *w;
+    const int32_t* targets;
+    int64_t rows, dim, vocab;
+    hipStream_t s;
+    int64_t dim_p() const { return ceil_div(dim, 8) * 8; }
+    // Whether a matrix of rows of dim is read as it is.
+    bool in_place(const T* p) const { return P == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+    size_t packed(int64_t n) const { return (size_t)n * dim_p() * P * 2; }
+    int pack(const T* src, int64_t n, const int32_t* t, uint16_t* dst) const {
+        hipLaunchKernelGGL((pack_kernel<OT, P>), dim3(grid_for(n * dim_p() / 8)), dim3(256), 0, s, src, n, dim, dim_p(), t,
+                           vocab, dst);
+        return launch_check("pack_kernel");
+    }
+    int product(int which, bool large, const Args& a) const {
+        if (OT == MLXHIP_DTYPE_F32) return ce_gemm_f32(which, large, a, s);
+        return OT == MLXHIP_DTYPE_BF16 ? ce_gemm_bf16(which, large, a, s) : ce_gemm_f16(which, large, a, s);
+    }
+    static int64_t tiles(int64_t m, int64_t n, bool large) {
+        const int64_t bm = large ? ce::large_bm<P>() : 128, bn = large ? ce::large_bn<P>() : 128;
+        return ceil_div(m, bm) * ceil_div(n, bn);
+    }
+    // Large tiles where they fill most of the compute units, one each.
+    static bool large(int64_t m, int64_t n) { return tiles(m, n, true) >= 192; }
+    // Columns of a piece: a copied piece of W and, with `ds`, dS within
+    // PIECE_BYTES, and offsets within a piece within 32 bits.
+    int64_t width(bool ds, bool copy) const {
+        int64_t w = std::min<int64_t>(vocab, (int64_t(1) << 29) / dim_p());
+        if (ds) w = std::min(w, PIECE_BYTES / (2 * P) / rows);
+        if (copy) w = std::min(w, PIECE_BYTES / (2 * P) / dim_p());
+        return w >= vocab ? vocab : std::max<int64_t>(w / 256 * 256, 256);
+    }
+};
 
-template <int DT>
-int run_loss(const void* x, const void* w, const int32_t* targets, float* loss, float* lse, int64_t rows, int64_t dim,
-             int64_t vocab, hipStream_t s) {
-    typedef typename Elem<DT>::type T;
-    const int64_t width = piece_width(rows, vocab);
+template <int OT>
+int run_loss(const Op<OT>& o, float* loss, float* lse) {
+    const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
+    const int64_t width = o.width(false, copy_w);
+    // One tile size for all pieces, whose widths are multiples of its columns.
+    const bool large = Op<OT>::large(o.rows, o.vocab);
+    const int64_t bn = large ? ce::large_bn<Op<OT>::P>() : 128, tiles = ceil_div(o.vocab, bn);
     Carve c;
-    const size_t oz = c.take((size_t)rows * width * 4), os = c.take((size_t)rows * 8), ot = c.take((size_t)rows * 4);
-    const bool wide = DT == MLXHIP_DTYPE_F32;
-    const size_t ox = c.take(wide ? 0 : (size_t)rows * dim * 4), ow = c.take(wide ? 0 : (size_t)width * dim * 4);
+    const size_t os = c.take((size_t)tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4),
+                 ox = c.take(copy_x ? o.packed(o.rows) : 0), ow = c.take(copy_w ? o.packed(width) : 0);
     char* ws = nullptr;
-    MLXHIP_TRY(stream_workspace(s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
-    float *z = (float*)(ws + oz), *tz = (float*)(ws + ot);
-    float2* stats = (float2*)(ws + os);
-    const float* xf = (const float*)x;
-    if (!wide) {
-        xf = (float*)(ws + ox);
-        hipLaunchKernelGGL((ce_rows_kernel<DT>), dim3(row_grid(rows)), dim3(256), 0, s, (const T*)x, rows, dim, vocab,
-                           nullptr, (float*)(ws + ox));
-        MLXHIP_TRY(launch_check("ce_rows_kernel"));
+    MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
+    Args a;
+    a.a = copy_x ? (uint16_t*)(ws + ox) : (const uint16_t*)o.x;
+    a.lda = a.ldb = a.ka = a.kb = o.dim_p();
+    a.a_plane = o.rows * o.dim_p();
+    a.m = o.rows;
+    a.targets = o.targets;
+    a.target_z = (float*)(ws + oz);
+    if (copy_x) MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, (uint16_t*)(ws + ox)));
+    for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
+        a.n = std::min(width, o.vocab - v0);
+        a.b = copy_w ? (uint16_t*)(ws + ow) : (const uint16_t*)o.w + v0 * o.dim;
+        a.b_plane = a.n * o.dim_p();
+        a.v0 = v0;
+        a.stats = (float2*)(ws + os) + v0 / bn * o.rows;
+        if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, (uint16_t*)(ws + ow)));
+        MLXHIP_TRY(o.product(ce::CE_STATS, large, a));
     }
-    for (int64_t v0 = 0; v0 < vocab; v0 += width) {
-        const int64_t n = std::min(width, vocab - v0);
-        const float* wf = (const float*)w + v0 * dim;
-        if (!wide) {
-            wf = (float*)(ws + ow);
-            hipLaunchKernelGGL((ce_rows_kernel<DT>), dim3(row_grid(n)), dim3(256), 0, s, (const T*)w + v0 * dim, n, dim,
-                               vocab, nullptr, (float*)(ws + ow));
-            MLXHIP_TRY(launch_check("ce_rows_kernel"));
-        }
-        MLXHIP_TRY(gemm(MLXHIP_DTYPE_F32, MLXHIP_DTYPE_F32, 0, 1, rows, n, dim, 1, xf, dim, 0, wf, dim, 0, z, n, 0, s));
-        hipLaunchKernelGGL(ce_stats_kernel, dim3(row_grid(rows)), dim3(256), 0, s, z, rows, n, v0, targets, stats, tz,
-                           v0 == 0);
-        MLXHIP_TRY(launch_check("ce_stats_kernel"));
-    }
-    hipLaunchKernelGGL(ce_loss_kernel, dim3((unsigned)ceil_div(rows, 256)), dim3(256), 0, s, stats, tz, targets, rows, vocab,
-                       loss, lse);
-    return launch_check("ce_loss_kernel");
+    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(o.rows, 32)), dim3(256), 0, o.s, (const float2*)(ws + os), tiles,
+                       (const float*)(ws + oz), o.targets, o.rows, o.vocab, loss, lse);
+    return launch_check("loss_kernel");
 }
 
-template <int DT>
-int run_grad(const void* x, const void* w, const int32_t* targets, const float* lse, const float* dloss, void* dx,
-             void* dw, int64_t rows, int64_t dim, int64_t vocab, hipStream_t s) {
-    typedef typename Elem<DT>::type T;
-    if (rows == 0) {  // a sum over no rows
+template <int OT>
+int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Elem<OT>::type* dx,
+             typename Elem<OT>::type* dw) {
+    typedef typename Elem<OT>::type T;
+    constexpr int P = Op<OT>::P;
+    if (o.rows == 0) {  // a sum over no rows
         if (!dw) return MLXHIP_OK;
-        hipLaunchKernelGGL((ce_zero_kernel<T>), dim3((unsigned)std::min<int64_t>(ceil_div(vocab * dim, 256), 4096)),
-                           dim3(256), 0, s, (T*)dw, vocab * dim);
-        return launch_check("ce_zero_kernel");
+        hipLaunchKernelGGL((zero_kernel<T>), dim3(grid_for(o.vocab * o.dim)), dim3(256), 0, o.s, dw, o.vocab * o.dim);
+        return launch_check("zero_kernel");
     }
-    const int64_t width = piece_width(rows, vocab);
-    const bool wide = DT == MLXHIP_DTYPE_F32;
+    const bool copy_w = !o.in_place(o.w);
+    const int64_t width = o.width(true, copy_w), ld = ceil_div(width, 256) * 256, dim_p = o.dim_p();
+    // dx: few tiles, so K is cut into slices until every compute unit has one
+    // (two of the small tiles), of at least 512 each.
+    const bool dx_large = Op<OT>::tiles(o.rows, o.dim, true) >= 16;
+    const int64_t dx_tiles = Op<OT>::tiles(o.rows, o.dim, dx_large), room = dx_large || P > 1 ? 256 : 512;
+    const int64_t most = std::max<int64_t>(1, std::min(room / dx_tiles, width / 512));
+    const int64_t chunk = ceil_div(ceil_div(width, most), 32) * 32;
+    const int splits = (int)ceil_div(width, chunk);
+    const int64_t ldx = ceil_div(o.dim, 4) * 4;
     Carve c;
-    const size_t oz = c.take((size_t)rows * width * 4), oa = c.take((size_t)rows * dim * 4),
-                 op = c.take((size_t)rows * dim * 4), ox = c.take((size_t)rows * dim * 4),
-                 ow = c.take(wide ? 0 : (size_t)width * dim * 4), od = c.take(wide ? 0 : (size_t)width * dim * 4);
+    const size_t ods = c.take((size_t)P * o.rows * ld * 2), ox = c.take(o.packed(o.rows)),
+                 ow = c.take(copy_w ? o.packed(width) : 0), orow = c.take((size_t)o.rows * sizeof(float2)),
+                 osc = c.take(8), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
     char* ws = nullptr;
-    MLXHIP_TRY(stream_workspace(s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
-    float *z = (float*)(ws + oz), *acc = (float*)(ws + oa), *part = (float*)(ws + op), *xf = (float*)(ws + ox);
-    hipLaunchKernelGGL((ce_rows_kernel<DT>), dim3(row_grid(rows)), dim3(256), 0, s, (const T*)x, rows, dim, vocab, targets,
-                       xf);
-    MLXHIP_TRY(launch_check("ce_rows_kernel"));
-    for (int64_t v0 = 0; v0 < vocab; v0 += width) {
-        const int64_t n = std::min(width, vocab - v0);
-        const float* wf = (const float*)w + v0 * dim;
-        if (!wide) {
-            wf = (float*)(ws + ow);
-            hipLaunchKernelGGL((ce_rows_kernel<DT>), dim3(row_grid(n)), dim3(256), 0, s, (const T*)w + v0 * dim, n, dim,
-                               vocab, nullptr, (float*)(ws + ow));
-            MLXHIP_TRY(launch_check("ce_rows_kernel"));
+    MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
+    uint16_t *ds = (uint16_t*)(ws + ods), *xp = (uint16_t*)(ws + ox);
+    float *scale = (float*)(ws + osc), *sums = (float*)(ws + osum);
+    hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, o.s, dloss, o.targets, o.rows, o.vocab,
+                       OT == MLXHIP_DTYPE_F16, scale);
+    MLXHIP_TRY(launch_check("scale_kernel"));
+    hipLaunchKernelGGL(rows_kernel, dim3((unsigned)ceil_div(o.rows, 256)), dim3(256), 0, o.s, lse, dloss, o.targets, o.rows,
+                       o.vocab, scale, (float2*)(ws + orow));
+    MLXHIP_TRY(launch_check("rows_kernel"));
+    MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, xp));
+    for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
+        const int64_t n = std::min(width, o.vocab - v0);
+        const uint16_t* wp = (const uint16_t*)o.w + v0 * o.dim;
+        if (copy_w) {
+            wp = (uint16_t*)(ws + ow);
+            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, (uint16_t*)(ws + ow)));
         }
-        MLXHIP_TRY(gemm(MLXHIP_DTYPE_F32, MLXHIP_DTYPE_F32, 0, 1, rows, n, dim, 1, xf, dim, 0, wf, dim, 0, z, n, 0, s));
-        hipLaunchKernelGGL(ce_grad_kernel, dim3(row_grid(rows)), dim3(256), 0, s, z, rows, n, v0, vocab, targets, lse,
-                           dloss);
-        MLXHIP_TRY(launch_check("ce_grad_kernel"));
-        if (dx) {
-            MLXHIP_TRY(gemm(MLXHIP_DTYPE_F32, MLXHIP_DTYPE_F32, 0, 0, rows, dim, n, 1, z, n, 0, wf, dim, 0, part, dim, 0, s));
-            hipLaunchKernelGGL(ce_add_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(rows * dim, 256), 4096)), dim3(256),
-                               0, s, acc, part, rows * dim, v0 == 0);
-            MLXHIP_TRY(launch_check("ce_add_kernel"));
-        }
+        Args z;
+        z.a = xp;
+        z.b = wp;
+        z.lda = z.ldb = z.ka = z.kb = dim_p;
+        z.a_plane = o.rows * dim_p;
+        z.b_plane = n * dim_p;
+        z.m = o.rows;
+        z.n = n;
+        z.targets = o.targets;
+        z.v0 = v0;
+        z.row = (const float2*)(ws + orow);
+        z.ds = ds;
+        z.ldc = ceil_div(n, 256) * 256;
+        MLXHIP_TRY(o.product(ce::CE_DS, Op<OT>::large(o.rows, n), z));
         if (dw) {
-            float* to = wide ? (float*)dw + v0 * dim : (float*)(ws + od);
-            MLXHIP_TRY(gemm(MLXHIP_DTYPE_F32, MLXHIP_DTYPE_F32, 1, 0, n, dim, rows, 1, z, n, 0, xf, dim, 0, to, dim, 0, s));
-            if (!wide) {
-                hipLaunchKernelGGL((ce_out_kernel<DT>), dim3(row_grid(n)), dim3(256), 0, s, to, n, dim, vocab, nullptr,
-                                   (T*)dw + v0 * dim);
-                MLXHIP_TRY(launch_check("ce_out_kernel"));
-            }
+            Args p;
+            p.a = ds;
+            p.lda = z.ldc;
+            p.a_plane = o.rows * z.ldc;
+            p.b = xp;
+            p.ldb = dim_p;
+            p.b_plane = z.a_plane;
+            p.ka = p.kb = o.rows;
+            p.m = n;
+            p.n = o.dim;
+            p.dw = dw + v0 * o.dim;
+            p.ldc = o.dim;
+            p.scale = scale;
+            MLXHIP_TRY(o.product(ce::CE_DW, Op<OT>::large(n, o.dim), p));
+        }
+        if (dx) {
+            Args p;
+            p.a = ds;
+            p.lda = z.ldc;
+            p.a_plane = o.rows * z.ldc;
+            p.ka = ceil_div(n, 8) * 8;  // dS holds zeros behind the piece
+            p.b = wp;
+            p.ldb = dim_p;
+            p.b_plane = z.b_plane;
+            p.kb = n;
+            p.m = o.rows;
+            p.n = o.dim;
+            // A last piece may have fewer slices; the others keep their sums.
+            p.splits = (int)std::min<int64_t>(splits, ceil_div(p.ka, chunk));
+            p.k_chunk = chunk;
+            p.dx = sums;
+            p.ldc = ldx;
+            p.add = v0 > 0;
+            MLXHIP_TRY(o.product(ce::CE_DX, dx_large, p));
         }
     }
     if (!dx) return MLXHIP_OK;
-    hipLaunchKernelGGL((ce_out_kernel<DT>), dim3(row_grid(rows)), dim3(256), 0, s, acc, rows, dim, vocab, targets, (T*)dx);
-    return launch_check("ce_out_kernel");
+    hipLaunchKernelGGL((dx_kernel<OT>), dim3(grid_for(o.rows * ldx / 4)), dim3(256), 0, o.s, sums, splits, o.rows, o.dim, ldx,
+                       o.targets, o.vocab, scale, dx);
+    return launch_check("dx_kernel");
 }
 
 }  // namespace
@@ -235,7 +347,10 @@ int run_grad(const void* x, const void* w, const int32_t* targets, const float* 
 int linear_cross_entropy(int dt, const void* x, const void* w, const int32_t* targets, float* loss, float* lse,
                          int64_t rows, int64_t dim, int64_t vocab, hipStream_t s) {
     int rc = MLXHIP_OK;
-    if (!with_float_dtype(dt, [&](auto d) { rc = run_loss<d.value>(x, w, targets, loss, lse, rows, dim, vocab, s); }))
+    if (!with_float_dtype(dt, [&](auto d) {
+            typedef typename Elem<d.value>::type T;
+            rc = run_loss<d.value>({(const T*)x, (const T*)w, targets, rows, dim, vocab, s}, loss, lse);
+        }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "linear_cross_entropy: dtype %d (f32, bf16 or f16)", dt);
     return rc;
 }
@@ -245,7 +360,8 @@ int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t
                              hipStream_t s) {
     int rc = MLXHIP_OK;
     if (!with_float_dtype(dt, [&](auto d) {
-            rc = run_grad<d.value>(x, w, targets, lse, dloss, dx, dw, rows, dim, vocab, s);
+            typedef typename Elem<d.value>::type T;
+            rc = run_grad<d.value>({(const T*)x, (const T*)w, targets, rows, dim, vocab, s}, lse, dloss, (T*)dx, (T*)dw);
         }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "linear_cross_entropy gradient: dtype %d (f32, bf16 or f16)", dt);
     return rc;
