@@ -65,18 +65,18 @@ struct Args {
     int tiles_m = 0, tiles_n = 0;
     int splits = 1;          // CE_DX: slices of K, of k_chunk (a multiple of 32) each
     int64_t k_chunk = 0;
-    // Rows of x: target column relative to n = 0 (the piece's first), and
-    // (-lse log2 e, factor) with factor 0 for a row that is not counted.
+    // Of each row of x: its target, and for CE_DS the forward's lse and dloss.
     const int32_t* targets = nullptr;
-    int64_t v0 = 0;
-    const float2* row = nullptr;
-    float2* stats = nullptr;    // CE_STATS: [tiles_n][m], this launch's first tile
+    int64_t v0 = 0, vocab = 0;  // the piece's first column, the whole vocabulary
+    const float *lse = nullptr, *dloss = nullptr;
+    float2* stats = nullptr;    // CE_STATS: [m][stat_tiles], from this launch's first tile on
+    int64_t stat_tiles = 0;
     float* target_z = nullptr;  // CE_STATS: [m]
     uint16_t* ds = nullptr;     // CE_DS: [P][m][ldc]
     float* dx = nullptr;        // CE_DX: [splits][m][ldc]
     bool add = false;           // CE_DX: add to what is there
     void* dw = nullptr;         // CE_DW: [m][ldc]
-    const float* scale = nullptr;
+    const float* scale = nullptr;  // of dS and, inverted, of the results ([1], [0]); null: 1
     int64_t ldc = 0;
 };
 
@@ -87,6 +87,8 @@ __device__ inline void merge(float& m, float& s, float m2, float s2) {
     s = s * __builtin_amdgcn_exp2f((m - base) * LOG2E) + s2 * __builtin_amdgcn_exp2f((m2 - base) * LOG2E);
     m = mn;
 }
+
+__device__ inline bool counted(int32_t target, int64_t vocab) { return target >= 0 && target < vocab; }
 
 // A target's place from column v on, -1 where it is not among `width` of them.
 __device__ inline int column_of(int32_t target, int64_t v, int width) {
@@ -361,24 +363,46 @@ void ce_gemm_kernel(Args g) {
             float2 a = make_float2(red[tid], red[C::BM + tid]);
 #pragma unroll
             for (int w = 1; w < C::WN; ++w) merge(a.x, a.y, red[2 * w * C::BM + tid], red[(2 * w + 1) * C::BM + tid]);
-            g.stats[n0 / C::BN * g.m + m0 + tid] = a;
+            g.stats[(m0 + tid) * g.stat_tiles + n0 / C::BN] = a;
         }
     } else if constexpr (PRODUCT == CE_DS) {
+        const float up = g.scale ? g.scale[1] : 1.0f;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int64_t r = row0 + 32 * i;
-            const float2 p = r < g.m ? g.row[r] : make_float2(0.0f, 0.0f);
-            const int tc = r < g.m ? column_of(g.targets[r], g.v0 + col0, 32 * TN) : -1;
+            // A row without a target has zeros in x, so z = 0: with lse taken
+            // as infinite its dS is 0 whatever lse and dloss hold.
+            float shift = -INFINITY, f = 0.0f;
+            int tc = -1;
+            if (r < g.m) {
+                const int32_t t = g.targets[r];
+                if (counted(t, g.vocab)) {
+                    shift = -g.lse[r] * LOG2E;
+                    f = g.dloss[r] * up;
+                }
+                tc = column_of(t, g.v0 + col0, 32 * TN);
+            }
 #pragma unroll
             for (int j = 0; j < TN; ++j)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int c = 32 * j + 8 * (v >> 2) + (v & 3);
-                    float q = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], LOG2E, p.x));
-                    if (tc == c) q -= 1.0f;
-                    // A row that is not counted is 0 whatever its lse is.
-                    acc[i][j][v] = p.y == 0.0f || col0 + c >= g.n ? 0.0f : q * p.y;
-                }
+                for (int v = 0; v < 16; ++v)
+                    acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], LOG2E, shift)) * f;
+            if (__ballot(tc >= 0)) {  // some lane holds its row's target
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) acc[i][j][v] -= f;
+            }
+        }
+        if (n0 + C::BN > g.n) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    if (col0 + 32 * j + 8 * (v >> 2) + (v & 3) >= g.n)
+#pragma unroll
+                        for (int i = 0; i < TM; ++i) acc[i][j][v] = 0.0f;
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
@@ -397,13 +421,15 @@ void ce_gemm_kernel(Args g) {
         }
     } else {
         if constexpr (PRODUCT == CE_DW) {
-            const float f = g.scale[0];
+            if (g.scale) {
+                const float f = g.scale[0];
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
+                    for (int j = 0; j < TN; ++j)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
+                        for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
+            }
             store_tile<OT, C, PIPE_BYTES, false, true>(acc, smem, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m,
                                                        g.n, g.n, m0, n0, wave, lane, false);
         } else {

@@ -31,13 +31,12 @@ namespace mlxhip {
 namespace {
 
 using ce::Args;
+using ce::counted;
 using dev::Elem;
 
 constexpr float LN2 = 0.69314718055994530942f;
 // Bytes of a piece's dS, and of a copied piece of W.
 constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
-
-__device__ inline bool counted(int32_t t, int64_t vocab) { return t >= 0 && t < vocab; }
 
 // src [rows][dim] as planes of [rows][dim_p] (zeros past dim, and in the rows
 // without a target where targets are given), 8 columns a thread.
@@ -77,25 +76,22 @@ __global__ __launch_bounds__(256) void pack_kernel(const typename Elem<OT>::type
     }
 }
 
-// A row's maxima and sums over the tiles joined, 8 threads to a row.
+// A row's maxima and sums over the tiles joined, a wave to each row.
 __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t tiles,
                                                    const float* __restrict__ target_z, const int32_t* __restrict__ targets,
                                                    int64_t rows, int64_t vocab, float* __restrict__ loss,
                                                    float* __restrict__ lse) {
-    __shared__ float2 part[8][32];
-    const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int64_t r = (int64_t)blockIdx.x * 32 + c;
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
     float m = -INFINITY, s = 0.0f;
-    if (r < rows)
-        for (int64_t t = k; t < tiles; t += 8) {
-            const float2 a = stats[t * rows + r];
-            ce::merge(m, s, a.x, a.y);
-        }
-    part[k][c] = make_float2(m, s);
-    __syncthreads();
-    if (k || r >= rows) return;
+    for (int64_t t = lane; t < tiles; t += 64) {
+        const float2 a = stats[r * tiles + t];
+        ce::merge(m, s, a.x, a.y);
+    }
 #pragma unroll
-    for (int i = 1; i < 8; ++i) ce::merge(m, s, part[i][c].x, part[i][c].y);
+    for (int o = 32; o > 0; o >>= 1) ce::merge(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
+    if (lane) return;
     const float l = m + LN2 * __builtin_amdgcn_logf(s);
     lse[r] = l;
     loss[r] = counted(targets[r], vocab) ? l - target_z[r] : 0.0f;
@@ -104,31 +100,21 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
 // f16: the factor that brings the largest dloss of a counted row to 2^15 times
 // a value in [1/2, 1], so that dS's small probabilities stay normal numbers
 // (scale[1]), and its inverse for the results (scale[0]); both powers of two.
-// The other types hold dS as it is.
 __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ dloss, const int32_t* __restrict__ targets,
-                                                     int64_t rows, int64_t vocab, bool f16, float* __restrict__ scale) {
+                                                     int64_t rows, int64_t vocab, float* __restrict__ scale) {
     __shared__ float waves[16];
     float m = 0.0f;
-    if (f16)
-        for (int64_t r = threadIdx.x; r < rows; r += 1024)
-            if (counted(targets[r], vocab)) m = fmaxf(m, fabsf(dloss[r]));
+    for (int64_t r = threadIdx.x; r < rows; r += 1024)
+        if (counted(targets[r], vocab)) m = fmaxf(m, fabsf(dloss[r]));
     m = dev::wave_max(m);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x) return;
     for (int i = 1; i < 16; ++i) m = fmaxf(m, waves[i]);
     int e = 15;
-    if (f16 && m > 0.0f && m < INFINITY) e = min(max(ilogbf(m) + 1, -100), 128);
+    if (m > 0.0f && m < INFINITY) e = min(max(ilogbf(m) + 1, -100), 128);
     scale[0] = ldexpf(1.0f, e - 15);
     scale[1] = ldexpf(1.0f, 15 - e);
-}
-
-__global__ __launch_bounds__(256) void rows_kernel(const float* __restrict__ lse, const float* __restrict__ dloss,
-                                                   const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
-                                                   const float* __restrict__ scale, float2* __restrict__ row) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r >= rows) return;
-    row[r] = counted(targets[r], vocab) ? make_float2(-lse[r] * ce::LOG2E, dloss[r] * scale[1]) : make_float2(0.0f, 0.0f);
 }
 
 // dx from the f32 sums of its slices of K, zeros where there is no target.
@@ -137,7 +123,7 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums,
                                                  int64_t ld, const int32_t* __restrict__ targets, int64_t vocab,
                                                  const float* __restrict__ scale, typename Elem<OT>::type* __restrict__ dx) {
     const int64_t quads = ld / 4, n = rows * quads;
-    const float f = scale[0];
+    const float f = scale ? scale[0] : 1.0f;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / quads, c = (i - r * quads) * 4;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -227,18 +213,20 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
     a.a_plane = o.rows * o.dim_p();
     a.m = o.rows;
     a.targets = o.targets;
+    a.vocab = o.vocab;
     a.target_z = (float*)(ws + oz);
+    a.stat_tiles = tiles;
     if (copy_x) MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, (uint16_t*)(ws + ox)));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         a.n = std::min(width, o.vocab - v0);
         a.b = copy_w ? (uint16_t*)(ws + ow) : (const uint16_t*)o.w + v0 * o.dim;
         a.b_plane = a.n * o.dim_p();
         a.v0 = v0;
-        a.stats = (float2*)(ws + os) + v0 / bn * o.rows;
+        a.stats = (float2*)(ws + os) + v0 / bn;
         if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, (uint16_t*)(ws + ow)));
         MLXHIP_TRY(o.product(ce::CE_STATS, large, a));
     }
-    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(o.rows, 32)), dim3(256), 0, o.s, (const float2*)(ws + os), tiles,
+    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(o.rows, 4)), dim3(256), 0, o.s, (const float2*)(ws + os), tiles,
                        (const float*)(ws + oz), o.targets, o.rows, o.vocab, loss, lse);
     return launch_check("loss_kernel");
 }
@@ -265,18 +253,16 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
     const int64_t ldx = ceil_div(o.dim, 4) * 4;
     Carve c;
     const size_t ods = c.take((size_t)P * o.rows * ld * 2), ox = c.take(o.packed(o.rows)),
-                 ow = c.take(copy_w ? o.packed(width) : 0), orow = c.take((size_t)o.rows * sizeof(float2)),
-                 osc = c.take(8), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
+                 ow = c.take(copy_w ? o.packed(width) : 0), osc = c.take(8), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     uint16_t *ds = (uint16_t*)(ws + ods), *xp = (uint16_t*)(ws + ox);
-    float *scale = (float*)(ws + osc), *sums = (float*)(ws + osum);
-    hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, o.s, dloss, o.targets, o.rows, o.vocab,
-                       OT == MLXHIP_DTYPE_F16, scale);
-    MLXHIP_TRY(launch_check("scale_kernel"));
-    hipLaunchKernelGGL(rows_kernel, dim3((unsigned)ceil_div(o.rows, 256)), dim3(256), 0, o.s, lse, dloss, o.targets, o.rows,
-                       o.vocab, scale, (float2*)(ws + orow));
-    MLXHIP_TRY(launch_check("rows_kernel"));
+    float *scale = nullptr, *sums = (float*)(ws + osum);
+    if (OT == MLXHIP_DTYPE_F16) {
+        scale = (float*)(ws + osc);
+        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, o.s, dloss, o.targets, o.rows, o.vocab, scale);
+        MLXHIP_TRY(launch_check("scale_kernel"));
+    }
     MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, xp));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         const int64_t n = std::min(width, o.vocab - v0);
@@ -295,7 +281,10 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         z.n = n;
         z.targets = o.targets;
         z.v0 = v0;
-        z.row = (const float2*)(ws + orow);
+        z.vocab = o.vocab;
+        z.lse = lse;
+        z.dloss = dloss;
+        z.scale = scale;
         z.ds = ds;
         z.ldc = ceil_div(n, 256) * 256;
         MLXHIP_TRY(o.product(ce::CE_DS, Op<OT>::large(o.rows, n), z));
