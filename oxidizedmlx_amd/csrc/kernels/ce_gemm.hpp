@@ -49,7 +49,11 @@ struct Cfg {
     static constexpr int LA = A_BYTES / (THREADS * 16), LB = B_BYTES / (THREADS * 16);  // loads per thread and plane
     static_assert(BM >= 128 && BN >= 128, "MN-contiguous LDS rows need >= 16 chunks for the swizzle");
     static_assert(LA * THREADS * 16 == A_BYTES && LB * THREADS * 16 == B_BYTES, "whole 1 KiB blocks per wave");
-    static_assert(STAGES >= 2 && STAGES * STAGE_BYTES <= 160 * 1024, "LDS budget");
+    // LDS of the epilogue per wave, and workgroups to a compute unit.
+    static constexpr int EPI = P == 1 ? 4096 : 2048;
+    static constexpr int LDS = STAGES * STAGE_BYTES + WAVES * EPI, PER_CU = 160 * 1024 / LDS;
+    static_assert(STAGES >= 2 && LDS <= 160 * 1024, "LDS budget");
+    static_assert(WN * 2 * BM * 4 <= WAVES * EPI, "row statistics of a tile");
 };
 template <int P>
 using Large = std::conditional_t<P == 1, Cfg<2, 4, 4, 2, 4, 1>, Cfg<4, 2, 2, 2, 2, 3>>;  // 256 x 256, 256 x 128
@@ -96,20 +100,39 @@ __device__ inline int column_of(int32_t target, int64_t v, int width) {
     return c >= 0 && c < width ? (int)c : -1;
 }
 
-// The tile of a workgroup: consecutive ids go to the 8 XCDs in turn, so each
-// XCD takes a contiguous range of tiles, in groups of four tile rows.
-template <class C>
-__device__ inline void tile_of(const Args& g, int64_t* m0, int64_t* n0, int* split) {
-    const int nwg = g.tiles_m * g.tiles_n, total = nwg * g.splits;
-    const int xcd = blockIdx.x & 7, per = total >> 3, rest = total & 7;
-    const int lin = xcd * per + min(xcd, rest) + (blockIdx.x >> 3);
-    *split = lin / nwg;
-    const int id = lin - *split * nwg;
+// A workgroup's tiles: consecutive workgroup ids go to the 8 XCDs in turn, so
+// each XCD takes a contiguous range of tiles, which its workgroups share out one
+// by one; a range runs through groups of four tile rows.
+struct Tiles {
+    int at, end, step;
+    __device__ inline Tiles(int total) {
+        const int xcd = blockIdx.x & 7, per = total >> 3, rest = total & 7;
+        const int first = xcd * per + min(xcd, rest);
+        at = first + (blockIdx.x >> 3);
+        end = first + per + (xcd < rest);
+        step = gridDim.x >> 3;
+    }
+};
+struct Tile {
+    int64_t m0, n0, k0, ka, kb;
+    int split;
+};
+template <int PRODUCT, class C>
+__device__ inline Tile tile_of(const Args& g, int lin) {
+    Tile t;
+    const int nwg = g.tiles_m * g.tiles_n;
+    t.split = PRODUCT == CE_DX ? lin / nwg : 0;
+    const int id = lin - t.split * nwg;
     constexpr int GROUP_M = 4;
     const int in_group = GROUP_M * g.tiles_n, first = id / in_group * GROUP_M;
     const int rows = min(g.tiles_m - first, GROUP_M);
-    *m0 = (int64_t)(first + id % in_group % rows) * C::BM;
-    *n0 = (int64_t)(id % in_group / rows) * C::BN;
+    t.m0 = (int64_t)(first + id % in_group % rows) * C::BM;
+    t.n0 = (int64_t)(id % in_group / rows) * C::BN;
+    t.k0 = PRODUCT == CE_DX ? t.split * g.k_chunk : 0;
+    const int64_t most = PRODUCT == CE_DX && g.splits > 1 ? g.k_chunk : INT64_MAX;
+    t.ka = min(g.ka - t.k0, most);
+    t.kb = min(g.kb - t.k0, most);
+    return t;
 }
 
 // Descriptor of an operand's part that the tile at row / column r0 (of R) and
@@ -123,127 +146,138 @@ __device__ inline __amdgpu_buffer_rsrc_t operand(const uint16_t* p, int64_t plan
     return __builtin_amdgcn_make_buffer_rsrc((void*)at, (short)0, (int)(uint32_t)(ext * 2), gemm16::BUF_FLAGS);
 }
 
-// Stores the tile of values v(i, j, e) = acc[i][j][e] through the wave's LDS
-// rows, whole row segments at a time: 16-byte vectors at any element alignment
-// where they end before column `cap`, single elements up to column g.n else.
-// ACC (f32): added to what is there.
-template <int CT, class C, int PIPE_BYTES, bool ACC, bool NT>
-__device__ inline void store_tile(const f32x16 (&acc)[C::TM][C::TN], MLXHIP_LDS char* smem, typename dev::Elem<CT>::type* out,
-                                  int64_t ld, int64_t m, int64_t n, int64_t cap, int64_t m0, int64_t n0, int wave,
-                                  int lane, bool add) {
+// Stores the tile of values acc through the wave's LDS region (C::EPI bytes),
+// whole row segments at a time: 16-byte vectors at any element alignment where
+// they end before column `cap`, single elements up to column n else. 16-byte
+// chunks of a region's row are permuted by its place among the rows that share
+// 256 bytes' worth of banks. ACC (f32): added to what is there.
+template <int CT, class C, bool ACC, bool NT>
+__device__ inline void store_tile(const f32x16 (&acc)[C::TM][C::TN], MLXHIP_LDS char* region, typename dev::Elem<CT>::type* out,
+                                  int64_t ld, int64_t m, int64_t n, int64_t cap, int64_t row0, int64_t col0, int lane,
+                                  bool add) {
     typedef typename dev::Elem<CT>::type T;
     typedef std::conditional_t<sizeof(T) == 4, u32x4_at4, u32x4_at2> any;
     constexpr int TM = C::TM, TN = C::TN, ES = sizeof(T), VEC = 16 / ES;
-    constexpr int PASS = gemm16::pass_rows<C, ES>(PIPE_BYTES);
-    constexpr int ROW_BYTES = 32 * TN * ES, PITCH = ROW_BYTES + 16;
-    constexpr int LANES = ROW_BYTES / 16, ROWS = 64 / LANES;
-    const int wm = wave / C::WN, wn = wave % C::WN;
-    MLXHIP_LDS char* region = smem + wave * PASS * PITCH;
-    const int64_t row0 = m0 + 32 * TM * wm, col0 = n0 + 32 * TN * wn;
+    constexpr int ROW_BYTES = 32 * TN * ES, CHUNKS = ROW_BYTES / 16, SHARE = CHUNKS >= 16 ? 1 : 16 / CHUNKS;
+    constexpr int PASS = C::EPI / ROW_BYTES < 32 ? C::EPI / ROW_BYTES : 32;  // rows staged at a time
+    constexpr int ROWS = 64 / CHUNKS;
+    static_assert(32 % PASS == 0 && PASS % ROWS == 0, "epilogue passes");
+    auto place = [](int r, int chunk) { return r * ROW_BYTES + ((chunk ^ ((r / SHARE) & (CHUNKS - 1))) * 16); };
 #pragma unroll
-    for (int pass = 0; pass < 32 * TM / PASS; ++pass) {
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int i = 0; i < PASS / 32; ++i) {
-            const int r = 32 * i + (lane & 31);
+        for (int h = 0; h < 32 / PASS; ++h) {
+            if (PASS == 32 || (lane & 31) / PASS == h) {
+                const int r = lane & (PASS - 1);
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+                for (int j = 0; j < TN; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    MLXHIP_LDS char* p = region + r * PITCH + (32 * j + 8 * q + 4 * (lane >> 5)) * ES;
-                    const f32x16& a = acc[pass * (PASS / 32) + i][j];
-                    if constexpr (ES == 4)
-                        *(MLXHIP_LDS f32x4*)p = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
-                    else
-                        *(MLXHIP_LDS u32x2*)p = u32x2{gemm16::pack2<CT>(a[4 * q], a[4 * q + 1]),
-                                                      gemm16::pack2<CT>(a[4 * q + 2], a[4 * q + 3])};
-                }
-        }
-        // Read back by the same wave, whose LDS accesses complete in order.
-#pragma unroll 4
-        for (int rr = 0; rr < PASS; rr += ROWS) {
-            const int r = rr + lane / LANES, cb = lane % LANES * 16;
-            u32x4 v = *(const MLXHIP_LDS u32x4*)(region + r * PITCH + cb);
-            const int64_t row = row0 + pass * PASS + r, col = col0 + cb / ES;
-            if (row >= m || col >= n) continue;
-            T* dst = out + row * ld + col;
-            if (col + VEC <= cap) {
-                if constexpr (ACC) {
-                    if (add) {
-                        const u32x4 had = *reinterpret_cast<const u32x4*>(dst);
+                    for (int q = 0; q < 4; ++q) {
+                        const int b = (32 * j + 8 * q + 4 * (lane >> 5)) * ES;
+                        MLXHIP_LDS char* p = region + place(r, b / 16) + b % 16;
+                        const f32x16& a = acc[i][j];
+                        if constexpr (ES == 4)
+                            *(MLXHIP_LDS f32x4*)p = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                        else
+                            *(MLXHIP_LDS u32x2*)p = u32x2{gemm16::pack2<CT>(a[4 * q], a[4 * q + 1]),
+                                                          gemm16::pack2<CT>(a[4 * q + 2], a[4 * q + 3])};
+                    }
+            }
+            // Read back by other lanes of the same wave: its LDS accesses complete
+            // in order, so only the compiler has to keep them in it.
+            asm volatile("" ::: "memory");
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] = __float_as_uint(__uint_as_float(had[e]) + __uint_as_float(v[e]));
+            for (int rr = 0; rr < PASS; rr += ROWS) {
+                const int r = rr + lane / CHUNKS, chunk = lane % CHUNKS;
+                u32x4 v = *(const MLXHIP_LDS u32x4*)(region + place(r, chunk));
+                const int64_t row = row0 + 32 * i + h * PASS + r, col = col0 + chunk * VEC;
+                if (row >= m || col >= n) continue;
+                T* dst = out + row * ld + col;
+                if (col + VEC <= cap) {
+                    if constexpr (ACC) {
+                        if (add) {
+                            const u32x4 had = *reinterpret_cast<const u32x4*>(dst);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                v[e] = __float_as_uint(__uint_as_float(had[e]) + __uint_as_float(v[e]));
+                        }
+                    }
+                    if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<any*>(dst));
+                    else *reinterpret_cast<any*>(dst) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        if (col + e >= n) break;
+                        if constexpr (ES == 4) dst[e] = __uint_as_float(v[e]);
+                        else dst[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
                     }
                 }
-                if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<any*>(dst));
-                else *reinterpret_cast<any*>(dst) = v;
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (col + e >= n) break;
-                    if constexpr (ES == 4) dst[e] = __uint_as_float(v[e]);
-                    else dst[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
-                }
             }
+            asm volatile("" ::: "memory");
         }
-    }
 }
 
 // MT: type of the planes (BF16, F16); OT: type of the operator's operands.
+//
+// A workgroup runs through its tiles without draining its loads: behind a
+// tile's last K tile come the first of the next one, which land while the
+// epilogue runs (it has LDS of its own).
 template <int PRODUCT, int MT, int OT, class C>
 __global__ __attribute__((amdgpu_flat_work_group_size(C::THREADS, C::THREADS), amdgpu_waves_per_eu(2, 2)))
 void ce_gemm_kernel(Args g) {
     constexpr bool KCA = PRODUCT != CE_DW, KCB = PRODUCT <= CE_DS;
     constexpr int STAGES = C::STAGES, TM = C::TM, TN = C::TN, WAVES = C::WAVES, P = C::P;
     constexpr int PAIRS = P == 1 ? 1 : gemm16::X6_SEGS;
-    constexpr int PIPE_BYTES = STAGES * C::STAGE_BYTES;
-    constexpr int STORED = PRODUCT == CE_DX ? MLXHIP_DTYPE_F32 : PRODUCT == CE_DW ? OT : MT;
-    constexpr int EPI_BYTES = gemm16::epi_bytes<STORED, C, PIPE_BYTES>();
-    constexpr int SMEM_BYTES = PIPE_BYTES > EPI_BYTES ? PIPE_BYTES : EPI_BYTES;
-    __shared__ __attribute__((aligned(1024))) char smem_raw[SMEM_BYTES];
+    __shared__ __attribute__((aligned(1024))) char smem_raw[STAGES * C::STAGE_BYTES + WAVES * C::EPI];
     MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw;
+    MLXHIP_LDS char* epi = smem + STAGES * C::STAGE_BYTES;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / C::WN, wn = wave % C::WN;
-    int64_t m0, n0;
-    int split;
-    tile_of<C>(g, &m0, &n0, &split);
-
-    const int64_t k0 = PRODUCT == CE_DX ? split * g.k_chunk : 0;
-    const int64_t most = PRODUCT == CE_DX && g.splits > 1 ? g.k_chunk : INT64_MAX;
-    const int64_t ka = min(g.ka - k0, most), kb = min(g.kb - k0, most);
-    const __amdgpu_buffer_rsrc_t ra = operand<KCA, C::BM, P>(g.a, g.a_plane, g.lda, m0, g.m, k0, ka);
-    const __amdgpu_buffer_rsrc_t rb = operand<KCB, C::BN, P>(g.b, g.b_plane, g.ldb, n0, g.n, k0, kb);
     const uint32_t plane_a = (uint32_t)(g.a_plane * 2), plane_b = (uint32_t)(g.b_plane * 2);
     constexpr int ROWB_A = C::BM * 2, ROWB_B = C::BN * 2;
-    gemm16::Loader<KCA, C::BM, WAVES> la;
-    gemm16::Loader<KCB, C::BN, WAVES> lb;
-    la.init(tid, 0, g.m - m0, g.lda, ka);
-    lb.init(tid, 0, g.n - n0, g.ldb, kb);
     gemm16::FragAddr<KCA, TM, ROWB_A> fa;
     gemm16::FragAddr<KCB, TN, ROWB_B> fb;
     fa.init(lane, 32 * TM * wm);
     fb.init(lane, 32 * TN * wn);
 
-    f32x16 acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+    // What is loaded next: K tile `lk` of the tile at `lat` of the list; past
+    // the list's end, loads that no chunk is in range of.
+    const Tiles list(g.tiles_m * g.tiles_n * (PRODUCT == CE_DX ? g.splits : 1));
+    if (list.at >= list.end) return;
+    gemm16::Loader<KCA, C::BM, WAVES> la;
+    gemm16::Loader<KCB, C::BN, WAVES> lb;
+    __amdgpu_buffer_rsrc_t ra, rb;
+    int lat = list.at, lk = 0, lnk = 0;
+    auto seek = [&] {
+        const Tile t = tile_of<PRODUCT, C>(g, lat);
+        ra = operand<KCA, C::BM, P>(g.a, g.a_plane, g.lda, t.m0, g.m, t.k0, t.ka);
+        rb = operand<KCB, C::BN, P>(g.b, g.b_plane, g.ldb, t.n0, g.n, t.k0, t.kb);
+        la.init(tid, 0, g.m - t.m0, g.lda, t.ka);
+        lb.init(tid, 0, g.n - t.n0, g.ldb, t.kb);
+        lk = 0;
+        lnk = (int)((max(t.ka, t.kb) + BK - 1) / BK);
+    };
+    auto next = [&] {
+        if (++lk < lnk || lat >= list.end) return;
+        lat += list.step;
+        if (lat < list.end) seek();
+    };
+    auto next_k = [&] { return lat < list.end ? lk * BK : INT32_MAX; };
+    seek();
 
-    const int nk = (int)((max(ka, kb) + BK - 1) / BK);
     constexpr int LA = C::LA, LB = C::LB, LPT = P * (LA + LB), B0 = P * C::A_BYTES;
 #pragma unroll
     for (int t = 0; t < STAGES; ++t) {
         MLXHIP_LDS char* st = smem + t * C::STAGE_BYTES;
+        const int k = next_k();
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            la.issue(ra, st + p * C::A_BYTES, wave, t * BK, (uint32_t)p * plane_a);
-            lb.issue(rb, st + B0 + p * C::B_BYTES, wave, t * BK, (uint32_t)p * plane_b);
+            la.issue(ra, st + p * C::A_BYTES, wave, k, (uint32_t)p * plane_a);
+            lb.issue(rb, st + B0 + p * C::B_BYTES, wave, k, (uint32_t)p * plane_b);
         }
+        next();
     }
     gemm16::wait_vmcnt<(STAGES - 1) * LPT>();
     gemm16::lds_barrier();
@@ -262,29 +296,43 @@ void ce_gemm_kernel(Args g) {
 #pragma unroll
     for (int o = 0; o < NR; ++o) read_op(smem, 0, o);
 
+    int cur = 0;  // stage of the K tile at hand
+    for (int at = list.at; at < list.end; at += list.step) {
+    const Tile tile = tile_of<PRODUCT, C>(g, at);
+    const int nk = (int)((max(tile.ka, tile.kb) + BK - 1) / BK);
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+
     // Per K tile two steps of 16: each step's MFMAs with the next step's LDS
-    // reads, and in the second the loads of the tile STAGES on, between them.
+    // reads, and in the second the loads of the K tile STAGES on, between them.
     constexpr int NM = TM * TN, NMI = PAIRS * NM, OPS = NR + LPT;
     for (int kt = 0; kt < nk; ++kt) {
-        const int cur = kt % STAGES;
         const MLXHIP_LDS char* st = smem + cur * C::STAGE_BYTES;
 #pragma unroll
         for (int q = 0; q < NMI; ++q) {
             const int e = q / NM, t = q % NM;
             gemm16::mfma<MT>(bf[0][P == 1 ? 0 : gemm16::seg_plane_b(e)][t % TN],
                              af[0][P == 1 ? 0 : gemm16::seg_plane_a(e)][t / TN], acc[t / TN][t % TN]);
+            constexpr bool ONE = NR <= NMI;  // a read a step, the first ones first
 #pragma unroll
-            for (int o = NR <= NMI ? (q < NR ? q : NR) : (q * NR) / NMI; o < (NR <= NMI ? (q < NR ? q + 1 : NR) : ((q + 1) * NR) / NMI); ++o)
+            for (int o = ONE ? min(q, NR) : (q * NR) / NMI; o < (ONE ? min(q + 1, NR) : ((q + 1) * NR) / NMI); ++o)
                 read_op(st, 1, o);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // Tile kt+1 has landed for every wave; every wave has read this tile's
-        // stage, which then receives tile kt+STAGES.
+        // The next K tile has landed for every wave (stores of an epilogue in
+        // between only make the wait longer); every wave has read this one's
+        // stage, which then receives the K tile STAGES on.
         gemm16::wait_vmcnt<(STAGES - 2) * LPT>();
         gemm16::lds_barrier();
         MLXHIP_LDS char* dst = smem + cur * C::STAGE_BYTES;
-        const int kl = (kt + STAGES) * BK;
-        const MLXHIP_LDS char* nx = smem + ((kt + 1) % STAGES) * C::STAGE_BYTES;
+        cur = cur + 1 == STAGES ? 0 : cur + 1;
+        const MLXHIP_LDS char* nx = smem + cur * C::STAGE_BYTES;
+        const int kl = next_k();
 #pragma unroll
         for (int q = 0; q < NMI; ++q) {
             const int e = q / NM, t = q % NM;
@@ -304,15 +352,16 @@ void ce_gemm_kernel(Args g) {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        next();
     }
-    gemm16::wait_vmcnt<0>();
-    gemm16::lds_barrier();  // every wave is done with the operand stages
 
     // acc[i][j][4 q + e] is row 32 i + lane % 32, column 32 j + 8 q +
     // 4 (lane / 32) + e of the wave's part.
-    const int64_t row0 = m0 + 32 * TM * wm + (lane & 31), col0 = n0 + 32 * TN * wn + 4 * (lane >> 5);
+    const int64_t m0 = tile.m0, n0 = tile.n0, wrow = m0 + 32 * TM * wm, wcol = n0 + 32 * TN * wn;
+    const int64_t row0 = wrow + (lane & 31), col0 = wcol + 4 * (lane >> 5);
+    MLXHIP_LDS char* region = epi + wave * C::EPI;
     if constexpr (PRODUCT == CE_STATS) {
-        MLXHIP_LDS float* red = (MLXHIP_LDS float*)smem;  // [WN][2][BM]
+        MLXHIP_LDS float* red = (MLXHIP_LDS float*)epi;  // [WN][2][BM]
         const bool edge = n0 + C::BN > g.n;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -358,7 +407,7 @@ void ce_gemm_kernel(Args g) {
                 p[C::BM] = s;
             }
         }
-        __syncthreads();
+        gemm16::lds_barrier();
         if (tid < C::BM && m0 + tid < g.m) {
             float2 a = make_float2(red[tid], red[C::BM + tid]);
 #pragma unroll
@@ -406,8 +455,8 @@ void ce_gemm_kernel(Args g) {
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            store_tile<MT, C, PIPE_BYTES, false, false>(acc, smem, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, m0, n0,
-                                                        wave, lane, false);
+            store_tile<MT, C, false, false>(acc, region, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, wrow, wcol, lane,
+                                            false);
             if (p + 1 < P) {
                 // What the plane leaves (exact in f32).
 #pragma unroll
@@ -430,21 +479,27 @@ void ce_gemm_kernel(Args g) {
 #pragma unroll
                         for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
             }
-            store_tile<OT, C, PIPE_BYTES, false, true>(acc, smem, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m,
-                                                       g.n, g.n, m0, n0, wave, lane, false);
+            store_tile<OT, C, false, true>(acc, region, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m, g.n, g.n,
+                                           wrow, wcol, lane, false);
         } else {
-            store_tile<MLXHIP_DTYPE_F32, C, PIPE_BYTES, true, false>(acc, smem, g.dx + split * g.m * g.ldc, g.ldc, g.m, g.n,
-                                                                     g.ldc, m0, n0, wave, lane, g.add);
+            store_tile<MLXHIP_DTYPE_F32, C, true, false>(acc, region, g.dx + tile.split * g.m * g.ldc, g.ldc, g.m, g.n, g.ldc,
+                                                         wrow, wcol, lane, g.add);
         }
     }
+    }
+    // The loads past the last tile write (zeros) to this workgroup's LDS.
+    gemm16::wait_vmcnt<0>();
 }
 
 template <int PRODUCT, int MT, int OT, class C>
 int launch(Args a, hipStream_t s) {
     a.tiles_m = (int)ceil_div(a.m, C::BM);
     a.tiles_n = (int)ceil_div(a.n, C::BN);
-    hipLaunchKernelGGL((ce_gemm_kernel<PRODUCT, MT, OT, C>), dim3((unsigned)(a.tiles_m * a.tiles_n * a.splits)),
-                       dim3(C::THREADS), 0, s, a);
+    // One workgroup for each place on the chip (a multiple of the 8 XCDs), or
+    // for each tile if those are fewer.
+    const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+    const int64_t groups = std::min<int64_t>(ceil_div(tiles, 8) * 8, 256 * C::PER_CU);
+    hipLaunchKernelGGL((ce_gemm_kernel<PRODUCT, MT, OT, C>), dim3((unsigned)groups), dim3(C::THREADS), 0, s, a);
     return launch_check("ce_gemm_kernel");
 }
 
