@@ -458,7 +458,10 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * dtype: F32, BF16 or F16, of x, w, dx and dw; loss, lse and dloss are f32, as
  * are the logits, sums and products' accumulators. dS is rounded to bf16 or
  * f16 (scaled by a power of two, so that small probabilities stay normal) for
- * the products of 16-bit operands, and dx and dw once as they are stored.
+ * the products of 16-bit operands, and dx and dw once as they are stored. F32
+ * operands and their dS enter the matrix cores as two f16 values each (22 bits;
+ * scaled by a power of two, absolute error 2^-39 of the operand's largest value
+ * where that is more), products below 2^-22 of a term left out.
  * Sums are formed in a fixed order. Operands contiguous, at any address
  * aligned to their elements; results must not overlap operands. A non-finite x
  * or w makes the logits it enters NaN. rows up to 2^21, dim up to 2^20, vocab up

@@ -1109,7 +1109,7 @@ namespace {
 int check_cross_entropy(const char* what, int64_t rows, int64_t dim, int64_t vocab) {
     MLXHIP_TRY(check_sizes(what, {rows, dim, vocab}, {1 << 21, 1 << 20, INT32_MAX}));
     if (dim == 0 || vocab == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: no logits (dim or vocab is 0)", what);
-    // The kernels' offsets within x's three planes are 32-bit bytes.
+    // The kernels' offsets within x's planes are 32-bit bytes.
     if (rows * (ceil_div(dim, 8) * 8) > (1 << 29))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: rows * dim = %lld is over 2^29", what, (long long)(rows * dim));
     return MLXHIP_OK;

@@ -5,16 +5,20 @@
 //             exp(z - max), and the target's logit: the logits leave the
 //             registers only as these.
 //   CE_DS     z again; dS = exp(z - lse) - [v = target], times the row's
-//             factor, stored in 16 bits (f32: as three bf16 planes).
+//             factor, stored in 16 bits (f32: as two f16 planes).
 //   CE_DX     f32 sums of dS W over a slice of K, added to those of the
 //             pieces of the vocabulary before.
 //   CE_DW     dS^T x times a power of two, in the operands' type.
 //
-// Operands are bf16 or f16, or f32 as three bf16 planes whose sum is the value
-// (P = 3: the six plane products above 2^-24 of the whole, smallest first, as
-// the f32 products of gemm16_x6.hip). Tiles are fed by direct global->LDS
-// loads, STAGES K tiles of 32 deep, with the building blocks and LDS layouts of
-// gemm16_impl.hpp.
+// Operands are bf16 or f16, or f32 as two f16 planes of the value times a power
+// of two (P = 2): hi is the value rounded to f16, lo what it leaves, rounded, so
+// hi + lo holds 22 bits of every value above 2^-18 of the largest (scaled to
+// 2^15), and the three products hi hi + hi lo + lo hi leave out less than
+// 2^-22 of a term. That is within what f32 sums of some hundred terms are off
+// by anyway, at half the matrix operations of the exact split into three bf16
+// planes (six products, gemm16_x6.hip: 2048 x 1024 over 32000 forward and
+// backward 2.80 ms). Tiles are fed by direct global->LDS loads, STAGES K tiles
+// of 32 deep, with the building blocks and LDS layouts of gemm16_impl.hpp.
 #pragma once
 
 #include "elem.hpp"
@@ -56,9 +60,26 @@ struct Cfg {
     static_assert(WN * 2 * BM * 4 <= WAVES * EPI, "row statistics of a tile");
 };
 template <int P>
-using Large = std::conditional_t<P == 1, Cfg<2, 4, 4, 2, 4, 1>, Cfg<4, 2, 2, 2, 2, 3>>;  // 256 x 256, 256 x 128
+using Large = std::conditional_t<P == 1, Cfg<2, 4, 4, 2, 4, 1>, Cfg<4, 2, 2, 2, 3, 2>>;  // 256 x 256, 256 x 128
 template <int P>
-using Small = std::conditional_t<P == 1, Cfg<2, 2, 2, 2, 4, 1>, Cfg<2, 4, 2, 1, 3, 3>>;  // 128 x 128, two to a CU / one
+using Small = std::conditional_t<P == 1, Cfg<2, 2, 2, 2, 4, 1>, Cfg<2, 4, 2, 1, 4, 2>>;  // 128 x 128, two to a CU / one
+
+// Factors of the products' operands and results, all powers of two.
+enum Scale {
+    SCALE_DW = 0,  // dW is this times dS^T x
+    SCALE_DS = 1,  // dS is formed from dloss times this
+    SCALE_Z = 2,   // z is this times the product (CE_STATS: and times row_scale)
+    SCALE_DX = 3,  // dx is this times dS W
+    SCALE_X = 4,   // planes hold this times x
+    SCALE_W = 5,   // and this times W
+    SCALES = 6
+};
+
+// The planes of product e: smallest first, hi hi last.
+template <int P>
+__host__ __device__ constexpr int plane_of_a(int e) { return P == 2 && e == 0; }
+template <int P>
+__host__ __device__ constexpr int plane_of_b(int e) { return P == 2 && e == 1; }
 
 struct Args {
     // op(A) [m, k], op(B) [k, n]; planes of an operand *_plane elements apart.
@@ -80,7 +101,8 @@ struct Args {
     float* dx = nullptr;        // CE_DX: [splits][m][ldc]
     bool add = false;           // CE_DX: add to what is there
     void* dw = nullptr;         // CE_DW: [m][ldc]
-    const float* scale = nullptr;  // of dS and, inverted, of the results ([1], [0]); null: 1
+    const float* scale = nullptr;  // Scale's factors; null: all 1
+    const float* row_scale = nullptr;  // CE_STATS of planes: x is row_scale[r] times its planes
     int64_t ldc = 0;
 };
 
@@ -227,7 +249,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(C::THREADS, C::THREADS), a
 void ce_gemm_kernel(Args g) {
     constexpr bool KCA = PRODUCT != CE_DW, KCB = PRODUCT <= CE_DS;
     constexpr int STAGES = C::STAGES, TM = C::TM, TN = C::TN, WAVES = C::WAVES, P = C::P;
-    constexpr int PAIRS = P == 1 ? 1 : gemm16::X6_SEGS;
+    constexpr int PAIRS = 2 * P - 1;
     __shared__ __attribute__((aligned(1024))) char smem_raw[STAGES * C::STAGE_BYTES + WAVES * C::EPI];
     MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw;
     MLXHIP_LDS char* epi = smem + STAGES * C::STAGE_BYTES;
@@ -298,194 +320,195 @@ void ce_gemm_kernel(Args g) {
 
     int cur = 0;  // stage of the K tile at hand
     for (int at = list.at; at < list.end; at += list.step) {
-    const Tile tile = tile_of<PRODUCT, C>(g, at);
-    const int nk = (int)((max(tile.ka, tile.kb) + BK - 1) / BK);
-    f32x16 acc[TM][TN];
+        const Tile tile = tile_of<PRODUCT, C>(g, at);
+        const int nk = (int)((max(tile.ka, tile.kb) + BK - 1) / BK);
+        f32x16 acc[TM][TN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+            for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+                for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
 
-    // Per K tile two steps of 16: each step's MFMAs with the next step's LDS
-    // reads, and in the second the loads of the K tile STAGES on, between them.
-    constexpr int NM = TM * TN, NMI = PAIRS * NM, OPS = NR + LPT;
-    for (int kt = 0; kt < nk; ++kt) {
-        const MLXHIP_LDS char* st = smem + cur * C::STAGE_BYTES;
+        // Per K tile two steps of 16: each step's MFMAs with the next step's LDS
+        // reads, and in the second the loads of the K tile STAGES on, between them.
+        constexpr int NM = TM * TN, NMI = PAIRS * NM, OPS = NR + LPT;
+        for (int kt = 0; kt < nk; ++kt) {
+            const MLXHIP_LDS char* st = smem + cur * C::STAGE_BYTES;
 #pragma unroll
-        for (int q = 0; q < NMI; ++q) {
-            const int e = q / NM, t = q % NM;
-            gemm16::mfma<MT>(bf[0][P == 1 ? 0 : gemm16::seg_plane_b(e)][t % TN],
-                             af[0][P == 1 ? 0 : gemm16::seg_plane_a(e)][t / TN], acc[t / TN][t % TN]);
-            constexpr bool ONE = NR <= NMI;  // a read a step, the first ones first
+            for (int q = 0; q < NMI; ++q) {
+                const int e = q / NM, t = q % NM;
+                gemm16::mfma<MT>(bf[0][plane_of_b<P>(e)][t % TN], af[0][plane_of_a<P>(e)][t / TN], acc[t / TN][t % TN]);
+                constexpr bool ONE = NR <= NMI;  // a read a step, the first ones first
 #pragma unroll
-            for (int o = ONE ? min(q, NR) : (q * NR) / NMI; o < (ONE ? min(q + 1, NR) : ((q + 1) * NR) / NMI); ++o)
-                read_op(st, 1, o);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        // The next K tile has landed for every wave (stores of an epilogue in
-        // between only make the wait longer); every wave has read this one's
-        // stage, which then receives the K tile STAGES on.
-        gemm16::wait_vmcnt<(STAGES - 2) * LPT>();
-        gemm16::lds_barrier();
-        MLXHIP_LDS char* dst = smem + cur * C::STAGE_BYTES;
-        cur = cur + 1 == STAGES ? 0 : cur + 1;
-        const MLXHIP_LDS char* nx = smem + cur * C::STAGE_BYTES;
-        const int kl = next_k();
-#pragma unroll
-        for (int q = 0; q < NMI; ++q) {
-            const int e = q / NM, t = q % NM;
-            gemm16::mfma<MT>(bf[1][P == 1 ? 0 : gemm16::seg_plane_b(e)][t % TN],
-                             af[1][P == 1 ? 0 : gemm16::seg_plane_a(e)][t / TN], acc[t / TN][t % TN]);
-#pragma unroll
-            for (int o = (q * OPS) / NMI; o < ((q + 1) * OPS) / NMI; ++o) {
-                if (o < NR) {
-                    read_op(nx, 0, o);
-                } else if (o < NR + P * LA) {
-                    const int p = (o - NR) / LA;
-                    la.issue_one(ra, dst + p * C::A_BYTES, wave, kl, o - NR - p * LA, (uint32_t)p * plane_a);
-                } else {
-                    const int ob = o - NR - P * LA, p = ob / LB;
-                    lb.issue_one(rb, dst + B0 + p * C::B_BYTES, wave, kl, ob - p * LB, (uint32_t)p * plane_b);
-                }
+                for (int o = ONE ? min(q, NR) : (q * NR) / NMI; o < (ONE ? min(q + 1, NR) : ((q + 1) * NR) / NMI); ++o)
+                    read_op(st, 1, o);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            // The next K tile has landed for every wave (stores of an epilogue in
+            // between only make the wait longer); every wave has read this one's
+            // stage, which then receives the K tile STAGES on.
+            gemm16::wait_vmcnt<(STAGES - 2) * LPT>();
+            gemm16::lds_barrier();
+            MLXHIP_LDS char* dst = smem + cur * C::STAGE_BYTES;
+            cur = cur + 1 == STAGES ? 0 : cur + 1;
+            const MLXHIP_LDS char* nx = smem + cur * C::STAGE_BYTES;
+            const int kl = next_k();
+#pragma unroll
+            for (int q = 0; q < NMI; ++q) {
+                const int e = q / NM, t = q % NM;
+                gemm16::mfma<MT>(bf[1][plane_of_b<P>(e)][t % TN], af[1][plane_of_a<P>(e)][t / TN], acc[t / TN][t % TN]);
+#pragma unroll
+                for (int o = (q * OPS) / NMI; o < ((q + 1) * OPS) / NMI; ++o) {
+                    if (o < NR) {
+                        read_op(nx, 0, o);
+                    } else if (o < NR + P * LA) {
+                        const int p = (o - NR) / LA;
+                        la.issue_one(ra, dst + p * C::A_BYTES, wave, kl, o - NR - p * LA, (uint32_t)p * plane_a);
+                    } else {
+                        const int ob = o - NR - P * LA, p = ob / LB;
+                        lb.issue_one(rb, dst + B0 + p * C::B_BYTES, wave, kl, ob - p * LB, (uint32_t)p * plane_b);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            next();
         }
-        next();
-    }
 
-    // acc[i][j][4 q + e] is row 32 i + lane % 32, column 32 j + 8 q +
-    // 4 (lane / 32) + e of the wave's part.
-    const int64_t m0 = tile.m0, n0 = tile.n0, wrow = m0 + 32 * TM * wm, wcol = n0 + 32 * TN * wn;
-    const int64_t row0 = wrow + (lane & 31), col0 = wcol + 4 * (lane >> 5);
-    MLXHIP_LDS char* region = epi + wave * C::EPI;
-    if constexpr (PRODUCT == CE_STATS) {
-        MLXHIP_LDS float* red = (MLXHIP_LDS float*)epi;  // [WN][2][BM]
-        const bool edge = n0 + C::BN > g.n;
+        // acc[i][j][4 q + e] is row 32 i + lane % 32, column 32 j + 8 q +
+        // 4 (lane / 32) + e of the wave's part.
+        const int64_t m0 = tile.m0, n0 = tile.n0, wrow = m0 + 32 * TM * wm, wcol = n0 + 32 * TN * wn;
+        const int64_t row0 = wrow + (lane & 31), col0 = wcol + 4 * (lane >> 5);
+        MLXHIP_LDS char* region = epi + wave * C::EPI;
+        if constexpr (PRODUCT == CE_STATS) {
+            MLXHIP_LDS float* red = (MLXHIP_LDS float*)epi;  // [WN][2][BM]
+            const bool edge = n0 + C::BN > g.n;
+            const float zs = P == 1 ? 1.0f : g.scale[SCALE_Z];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t r = row0 + 32 * i;
-            // The target's logit, from the lane that holds its column.
-            const int tc = r < g.m ? column_of(g.targets[r], g.v0 + col0, 32 * TN) : -1;
-            const bool mine = tc >= 0 && (tc & 4) == 0 && tc + col0 < g.n;
-            if (__ballot(mine)) {
-                float z = 0.0f;
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) z = acc[i][j][v];
-                if (mine) g.target_z[r] = z;
-            }
-            if (edge) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (col0 + 32 * j + 8 * (v >> 2) + (v & 3) >= g.n) acc[i][j][v] = -INFINITY;
-            }
-            float mx = acc[i][0][0];
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) mx = fmaxf(mx, acc[i][j][v]);
-            // exp(z - mx) as exp2(z log2 e - mb), mb = mx log2 e rounded; what
-            // that rounding leaves is put right in the sum.
-            const float base = mx == -INFINITY ? 0.0f : mx;
-            const float mb = base * LOG2E;
-            float s = 0.0f;
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], LOG2E, -mb));
-            s *= __builtin_amdgcn_exp2f(__builtin_fmaf(-base, LOG2E, mb));
-            merge(mx, s, __shfl_xor(mx, 32, 64), __shfl_xor(s, 32, 64));
-            if (lane < 32) {
-                MLXHIP_LDS float* p = red + 2 * wn * C::BM + 32 * TM * wm + 32 * i + lane;
-                p[0] = mx;
-                p[C::BM] = s;
-            }
-        }
-        gemm16::lds_barrier();
-        if (tid < C::BM && m0 + tid < g.m) {
-            float2 a = make_float2(red[tid], red[C::BM + tid]);
-#pragma unroll
-            for (int w = 1; w < C::WN; ++w) merge(a.x, a.y, red[2 * w * C::BM + tid], red[(2 * w + 1) * C::BM + tid]);
-            g.stats[(m0 + tid) * g.stat_tiles + n0 / C::BN] = a;
-        }
-    } else if constexpr (PRODUCT == CE_DS) {
-        const float up = g.scale ? g.scale[1] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t r = row0 + 32 * i;
-            // A row without a target has zeros in x, so z = 0: with lse taken
-            // as infinite its dS is 0 whatever lse and dloss hold.
-            float shift = -INFINITY, f = 0.0f;
-            int tc = -1;
-            if (r < g.m) {
-                const int32_t t = g.targets[r];
-                if (counted(t, g.vocab)) {
-                    shift = -g.lse[r] * LOG2E;
-                    f = g.dloss[r] * up;
-                }
-                tc = column_of(t, g.v0 + col0, 32 * TN);
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], LOG2E, shift)) * f;
-            if (__ballot(tc >= 0)) {  // some lane holds its row's target
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) acc[i][j][v] -= f;
-            }
-        }
-        if (n0 + C::BN > g.n) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    if (col0 + 32 * j + 8 * (v >> 2) + (v & 3) >= g.n)
-#pragma unroll
-                        for (int i = 0; i < TM; ++i) acc[i][j][v] = 0.0f;
-        }
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            store_tile<MT, C, false, false>(acc, region, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, wrow, wcol, lane,
-                                            false);
-            if (p + 1 < P) {
-                // What the plane leaves (exact in f32).
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
+            for (int i = 0; i < TM; ++i) {
+                const int64_t r = row0 + 32 * i;
+                const float f = P == 1 || r >= g.m ? 1.0f : zs * g.row_scale[r];
+                // The target's logit, from the lane that holds its column.
+                const int tc = r < g.m ? column_of(g.targets[r], g.v0 + col0, 32 * TN) : -1;
+                const bool mine = tc >= 0 && (tc & 4) == 0 && tc + col0 < g.n;
+                if (__ballot(mine)) {
+                    float z = 0.0f;
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int v = 0; v < 16; ++v)
-                            acc[i][j][v] -= dev::to_f32<MT>(dev::from_f32<MT>(acc[i][j][v]));
-            }
-        }
-    } else {
-        if constexpr (PRODUCT == CE_DW) {
-            if (g.scale) {
-                const float f = g.scale[0];
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
+                            if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) z = acc[i][j][v];
+                    if (mine) g.target_z[r] = z * f;
+                }
+                if (edge) {
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
+                        for (int v = 0; v < 16; ++v)
+                            if (col0 + 32 * j + 8 * (v >> 2) + (v & 3) >= g.n) acc[i][j][v] = -INFINITY;
+                }
+                float mx = acc[i][0][0];
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) mx = fmaxf(mx, acc[i][j][v]);
+                // exp(z - mx) as exp2(z log2 e - mb), mb = mx log2 e rounded; what
+                // that rounding leaves is put right in the sum.
+                const float base = mx == -INFINITY ? 0.0f : mx, up = LOG2E * f;
+                const float mb = base * up;
+                float s = 0.0f;
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], up, -mb));
+                s *= __builtin_amdgcn_exp2f(__builtin_fmaf(-base, up, mb));
+                mx *= f;
+                merge(mx, s, __shfl_xor(mx, 32, 64), __shfl_xor(s, 32, 64));
+                if (lane < 32) {
+                    MLXHIP_LDS float* p = red + 2 * wn * C::BM + 32 * TM * wm + 32 * i + lane;
+                    p[0] = mx;
+                    p[C::BM] = s;
+                }
             }
-            store_tile<OT, C, false, true>(acc, region, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m, g.n, g.n,
-                                           wrow, wcol, lane, false);
+            gemm16::lds_barrier();
+            if (tid < C::BM && m0 + tid < g.m) {
+                float2 a = make_float2(red[tid], red[C::BM + tid]);
+#pragma unroll
+                for (int w = 1; w < C::WN; ++w) merge(a.x, a.y, red[2 * w * C::BM + tid], red[(2 * w + 1) * C::BM + tid]);
+                g.stats[(m0 + tid) * g.stat_tiles + n0 / C::BN] = a;
+            }
+        } else if constexpr (PRODUCT == CE_DS) {
+            const float up = g.scale ? g.scale[SCALE_DS] : 1.0f, zs = P == 1 ? LOG2E : LOG2E * g.scale[SCALE_Z];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int64_t r = row0 + 32 * i;
+                // A row without a target has zeros in x, so z = 0: with lse taken
+                // as infinite its dS is 0 whatever lse and dloss hold.
+                float shift = -INFINITY, f = 0.0f;
+                int tc = -1;
+                if (r < g.m) {
+                    const int32_t t = g.targets[r];
+                    if (counted(t, g.vocab)) {
+                        shift = -g.lse[r] * LOG2E;
+                        f = g.dloss[r] * up;
+                    }
+                    tc = column_of(t, g.v0 + col0, 32 * TN);
+                }
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], zs, shift)) * f;
+                if (__ballot(tc >= 0)) {  // some lane holds its row's target
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v)
+                            if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) acc[i][j][v] -= f;
+                }
+            }
+            if (n0 + C::BN > g.n) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (col0 + 32 * j + 8 * (v >> 2) + (v & 3) >= g.n)
+#pragma unroll
+                            for (int i = 0; i < TM; ++i) acc[i][j][v] = 0.0f;
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                store_tile<MT, C, false, false>(acc, region, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, wrow, wcol, lane,
+                                                false);
+                if (p + 1 < P) {
+                    // What the plane leaves (exact in f32).
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+#pragma unroll
+                            for (int v = 0; v < 16; ++v)
+                                acc[i][j][v] -= dev::to_f32<MT>(dev::from_f32<MT>(acc[i][j][v]));
+                }
+            }
         } else {
-            store_tile<MLXHIP_DTYPE_F32, C, true, false>(acc, region, g.dx + tile.split * g.m * g.ldc, g.ldc, g.m, g.n, g.ldc,
-                                                         wrow, wcol, lane, g.add);
+            if constexpr (PRODUCT == CE_DW) {
+                if (g.scale) {
+                    const float f = g.scale[SCALE_DW];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
+                }
+                store_tile<OT, C, false, true>(acc, region, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m, g.n, g.n,
+                                               wrow, wcol, lane, false);
+            } else {
+                store_tile<MLXHIP_DTYPE_F32, C, true, false>(acc, region, g.dx + tile.split * g.m * g.ldc, g.ldc, g.m, g.n, g.ldc,
+                                                             wrow, wcol, lane, g.add);
+            }
         }
-    }
     }
     // The loads past the last tile write (zeros) to this workgroup's LDS.
     gemm16::wait_vmcnt<0>();

@@ -10,7 +10,7 @@
 //
 // Forward: one product whose tiles leave each row's maximum and sum over their
 // columns (ce_gemm.hpp), and a launch that joins them. Backward, per piece of
-// the vocabulary: the product again, stored as dS in 16 bits (f32: three bf16
+// the vocabulary: the product again, stored as dS in 16 bits (f32: two f16
 // planes), then dW of the piece whole and dx's share added to f32 sums, which
 // a last launch scales and rounds. Four products of 2 R D V operations; at
 // several hundred rows the matrix cores bound them.
@@ -38,42 +38,136 @@ constexpr float LN2 = 0.69314718055994530942f;
 // Bytes of a piece's dS, and of a copied piece of W.
 constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
 
+// 2^e with the largest magnitude m below it (1/2 of it at least); 15 for an m
+// that says nothing, so that the factors made from it are 1.
+__device__ inline int exponent(float m) { return m > 0.0f && m < INFINITY ? min(max(ilogbf(m) + 1, -100), 128) : 15; }
+
+__device__ inline float finite_abs(float v) { return __builtin_isfinite(v) ? fabsf(v) : 0.0f; }
+
+// Eight columns from c on of a row, as the planes of v times f.
+template <int OT, int P>
+__device__ inline void pack8(const typename Elem<OT>::type* src, int64_t c, int64_t dim, bool on, float f, uint16_t* dst,
+                             int64_t plane) {
+    constexpr int VEC = Elem<OT>::VEC;
+    union {
+        uint16_t h[8];
+        uint4 q;
+    } out;
+    if constexpr (P == 1) {
+        const dev::Vec16<OT> v = dev::load_raw<OT>(src, c, dim);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out.h[e] = on ? v.v[e] : 0;
+        *reinterpret_cast<uint4*>(dst + c) = out.q;
+    } else {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8 / VEC; ++k) dev::unpack<OT>(dev::load_raw<OT>(src, c + k * VEC, dim), v + k * VEC);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = on ? v[e] * f : 0.0f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                out.h[e] = dev::from_f32<MLXHIP_DTYPE_F16>(v[e]);
+                v[e] -= dev::to_f32<MLXHIP_DTYPE_F16>(out.h[e]);
+            }
+            *reinterpret_cast<uint4*>(dst + p * plane + c) = out.q;
+        }
+    }
+}
+
 // src [rows][dim] as planes of [rows][dim_p] (zeros past dim, and in the rows
 // without a target where targets are given), 8 columns a thread.
 template <int OT, int P>
 __global__ __launch_bounds__(256) void pack_kernel(const typename Elem<OT>::type* __restrict__ src, int64_t rows,
                                                    int64_t dim, int64_t dim_p, const int32_t* __restrict__ targets,
-                                                   int64_t vocab, uint16_t* __restrict__ dst) {
-    constexpr int VEC = Elem<OT>::VEC;
+                                                   int64_t vocab, const float* __restrict__ scale,
+                                                   uint16_t* __restrict__ dst) {
     const int64_t chunks = dim_p / 8, plane = rows * dim_p;
+    const float f = P == 1 ? 1.0f : *scale;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / chunks, c = (i - r * chunks) * 8;
-        const bool on = !targets || counted(targets[r], vocab);
-        union {
-            uint16_t h[8];
-            uint4 q;
-        } out;
-        if constexpr (P == 1) {
-            const dev::Vec16<OT> v = dev::load_raw<OT>(src + r * dim, c, dim);
+        pack8<OT, P>(src + r * dim, c, dim, !targets || counted(targets[r], vocab), f, dst + r * dim_p, plane);
+    }
+}
+
+// As pack_kernel for f32, each row scaled by its own largest magnitude
+// (row_scale: what undoes it), a wave to a row: a row of the forward pass takes
+// no digits from another, whatever that holds.
+template <int P>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t dim,
+                                                        int64_t dim_p, float* __restrict__ row_scale,
+                                                        uint16_t* __restrict__ dst) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    float m = 0.0f;
+    for (int64_t c = lane; c < dim; c += 64) m = fmaxf(m, finite_abs(src[r * dim + c]));
+    const int e = exponent(dev::wave_max(m));
+    if (lane == 0) row_scale[r] = ldexpf(1.0f, e - 15);
+    for (int64_t c = lane * 8; c < dim_p; c += 512)
+        pack8<MLXHIP_DTYPE_F32, P>(src + r * dim, c, dim, true, ldexpf(1.0f, 15 - e), dst + r * dim_p, rows * dim_p);
+}
+
+// Largest finite magnitudes, one of each workgroup: of W in part[0..MAXIMA), of
+// the rows of x with a target in part[MAXIMA..2 MAXIMA) (blockIdx.y = 1).
+constexpr int MAXIMA = 1024;
+__global__ __launch_bounds__(256) void maxima_kernel(const float* __restrict__ w, int64_t nw, const float* __restrict__ x,
+                                                     int64_t dim, int64_t nx, const int32_t* __restrict__ targets,
+                                                     int64_t vocab, float* __restrict__ part) {
+    __shared__ float waves[4];
+    const float* p = blockIdx.y ? x : w;
+    const int64_t n = blockIdx.y ? nx : nw;
+    float m = 0.0f;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += MAXIMA * 256 * 8) {
+        const dev::Vec16<MLXHIP_DTYPE_F32> a = dev::load_raw<MLXHIP_DTYPE_F32>(p, i, n),
+                                           b = dev::load_raw<MLXHIP_DTYPE_F32>(p, i + 4, n);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) out.h[e] = on ? v.v[e] : 0;
-            *reinterpret_cast<uint4*>(dst + r * dim_p + c) = out.q;
-        } else {
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8 / VEC; ++k) dev::unpack<OT>(dev::load_raw<OT>(src + r * dim, c + k * VEC, dim), v + k * VEC);
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (p == 0 && !on) v[e] = 0.0f;
-                    out.h[e] = dev::from_f32<MLXHIP_DTYPE_BF16>(v[e]);
-                    v[e] -= dev::to_f32<MLXHIP_DTYPE_BF16>(out.h[e]);
-                }
-                *reinterpret_cast<uint4*>(dst + p * plane + r * dim_p + c) = out.q;
-            }
+        for (int e = 0; e < 8; ++e) {
+            const float v = finite_abs(e < 4 ? a.v[e] : b.v[e - 4]);
+            if (blockIdx.y == 0 || (i + e < n && counted(targets[(i + e) / dim], vocab))) m = fmaxf(m, v);
         }
     }
+    m = dev::wave_max(m);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        part[blockIdx.y * MAXIMA + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+}
+
+__device__ inline float block_max(float m, float* waves) {
+    m = dev::wave_max(m);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, waves[i]);
+    __syncthreads();
+    return m;
+}
+
+// The factors of ce::Scale, by one workgroup. Planes of W and x (part given, x
+// in the backward pass) and, in it, dS (f16 and f32) are scaled so that the
+// largest magnitude lies between 2^14 and 2^15: small probabilities then stay
+// normal f16 numbers.
+__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ part, const float* __restrict__ dloss,
+                                                     const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
+                                                     float* __restrict__ scale) {
+    __shared__ float waves[16];
+    int ew = 15, ex = 15, eg = 15;
+    if (part) ew = exponent(block_max(part[threadIdx.x], waves));
+    if (dloss) {
+        float m = 0.0f;
+        for (int64_t r = threadIdx.x; r < rows; r += 1024)
+            if (counted(targets[r], vocab)) m = fmaxf(m, finite_abs(dloss[r]));
+        eg = exponent(block_max(m, waves));
+        if (part) ex = exponent(block_max(part[MAXIMA + threadIdx.x], waves));
+    }
+    if (threadIdx.x) return;
+    scale[ce::SCALE_DW] = ldexpf(1.0f, eg + ex - 30);
+    scale[ce::SCALE_DS] = ldexpf(1.0f, 15 - eg);
+    scale[ce::SCALE_Z] = ldexpf(1.0f, ex + ew - 30);
+    scale[ce::SCALE_DX] = ldexpf(1.0f, eg + ew - 30);
+    scale[ce::SCALE_X] = ldexpf(1.0f, 15 - ex);
+    scale[ce::SCALE_W] = ldexpf(1.0f, 15 - ew);
 }
 
 // A row's maxima and sums over the tiles joined, a wave to each row.
@@ -97,33 +191,13 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
     loss[r] = counted(targets[r], vocab) ? l - target_z[r] : 0.0f;
 }
 
-// f16: the factor that brings the largest dloss of a counted row to 2^15 times
-// a value in [1/2, 1], so that dS's small probabilities stay normal numbers
-// (scale[1]), and its inverse for the results (scale[0]); both powers of two.
-__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ dloss, const int32_t* __restrict__ targets,
-                                                     int64_t rows, int64_t vocab, float* __restrict__ scale) {
-    __shared__ float waves[16];
-    float m = 0.0f;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024)
-        if (counted(targets[r], vocab)) m = fmaxf(m, fabsf(dloss[r]));
-    m = dev::wave_max(m);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x) return;
-    for (int i = 1; i < 16; ++i) m = fmaxf(m, waves[i]);
-    int e = 15;
-    if (m > 0.0f && m < INFINITY) e = min(max(ilogbf(m) + 1, -100), 128);
-    scale[0] = ldexpf(1.0f, e - 15);
-    scale[1] = ldexpf(1.0f, 15 - e);
-}
-
 // dx from the f32 sums of its slices of K, zeros where there is no target.
 template <int OT>
 __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums, int splits, int64_t rows, int64_t dim,
                                                  int64_t ld, const int32_t* __restrict__ targets, int64_t vocab,
                                                  const float* __restrict__ scale, typename Elem<OT>::type* __restrict__ dx) {
     const int64_t quads = ld / 4, n = rows * quads;
-    const float f = scale ? scale[0] : 1.0f;
+    const float f = scale ? scale[ce::SCALE_DX] : 1.0f;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / quads, c = (i - r * quads) * 4;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -161,7 +235,7 @@ struct Carve {
 template <int OT>
 struct Op {
     typedef typename Elem<OT>::type T;
-    static constexpr int P = OT == MLXHIP_DTYPE_F32 ? 3 : 1;
+    static constexpr int P = OT == MLXHIP_DTYPE_F32 ? 2 : 1;
     const T *x, *w;
     const int32_t* targets;
     int64_t rows, dim, vocab;
@@ -170,10 +244,22 @@ struct Op {
     // Whether a matrix of rows of dim is read as it is.
     bool in_place(const T* p) const { return P == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
     size_t packed(int64_t n) const { return (size_t)n * dim_p() * P * 2; }
-    int pack(const T* src, int64_t n, const int32_t* t, uint16_t* dst) const {
+    int pack(const T* src, int64_t n, const int32_t* t, const float* scale, uint16_t* dst) const {
         hipLaunchKernelGGL((pack_kernel<OT, P>), dim3(grid_for(n * dim_p() / 8)), dim3(256), 0, s, src, n, dim, dim_p(), t,
-                           vocab, dst);
+                           vocab, scale, dst);
         return launch_check("pack_kernel");
+    }
+    // The factors into scale (part: room for the maxima of f32 operands).
+    int scales(const float* dloss, float* part, float* scale) const {
+        if constexpr (P > 1) {
+            hipLaunchKernelGGL(maxima_kernel, dim3(MAXIMA, dloss ? 2 : 1), dim3(256), 0, s, w, vocab * dim, x, dim, rows * dim,
+                               targets, vocab, part);
+            MLXHIP_TRY(launch_check("maxima_kernel"));
+        } else {
+            part = nullptr;
+        }
+        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, part, dloss, targets, rows, vocab, scale);
+        return launch_check("scale_kernel");
     }
     int product(int which, bool large, const Args& a) const {
         if (OT == MLXHIP_DTYPE_F32) return ce_gemm_f32(which, large, a, s);
@@ -204,7 +290,9 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
     const int64_t bn = large ? ce::large_bn<Op<OT>::P>() : 128, tiles = ceil_div(o.vocab, bn);
     Carve c;
     const size_t os = c.take((size_t)tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4),
-                 ox = c.take(copy_x ? o.packed(o.rows) : 0), ow = c.take(copy_w ? o.packed(width) : 0);
+                 ox = c.take(copy_x ? o.packed(o.rows) : 0), ow = c.take(copy_w ? o.packed(width) : 0),
+                 osc = c.take(ce::SCALES * 4), op = c.take(Op<OT>::P > 1 ? 2 * MAXIMA * 4 : 0),
+                 ors = c.take(Op<OT>::P > 1 ? (size_t)o.rows * 4 : 0);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     Args a;
@@ -216,14 +304,24 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
     a.vocab = o.vocab;
     a.target_z = (float*)(ws + oz);
     a.stat_tiles = tiles;
-    if (copy_x) MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, (uint16_t*)(ws + ox)));
+    float* scale = (float*)(ws + osc);
+    if constexpr (Op<OT>::P > 1) {
+        a.scale = scale;
+        a.row_scale = (float*)(ws + ors);
+        MLXHIP_TRY(o.scales(nullptr, (float*)(ws + op), scale));
+        hipLaunchKernelGGL((pack_rows_kernel<Op<OT>::P>), dim3((unsigned)ceil_div(o.rows, 4)), dim3(256), 0, o.s, o.x, o.rows,
+                           o.dim, o.dim_p(), (float*)(ws + ors), (uint16_t*)(ws + ox));
+        MLXHIP_TRY(launch_check("pack_rows_kernel"));
+    } else if (copy_x) {
+        MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, nullptr, (uint16_t*)(ws + ox)));
+    }
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         a.n = std::min(width, o.vocab - v0);
         a.b = copy_w ? (uint16_t*)(ws + ow) : (const uint16_t*)o.w + v0 * o.dim;
         a.b_plane = a.n * o.dim_p();
         a.v0 = v0;
         a.stats = (float2*)(ws + os) + v0 / bn;
-        if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, (uint16_t*)(ws + ow)));
+        if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, scale + ce::SCALE_W, (uint16_t*)(ws + ow)));
         MLXHIP_TRY(o.product(ce::CE_STATS, large, a));
     }
     hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(o.rows, 4)), dim3(256), 0, o.s, (const float2*)(ws + os), tiles,
@@ -253,23 +351,23 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
     const int64_t ldx = ceil_div(o.dim, 4) * 4;
     Carve c;
     const size_t ods = c.take((size_t)P * o.rows * ld * 2), ox = c.take(o.packed(o.rows)),
-                 ow = c.take(copy_w ? o.packed(width) : 0), osc = c.take(8), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
+                 ow = c.take(copy_w ? o.packed(width) : 0), osc = c.take(ce::SCALES * 4),
+                 op = c.take(P > 1 ? 2 * MAXIMA * 4 : 0), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     uint16_t *ds = (uint16_t*)(ws + ods), *xp = (uint16_t*)(ws + ox);
     float *scale = nullptr, *sums = (float*)(ws + osum);
-    if (OT == MLXHIP_DTYPE_F16) {
+    if (OT != MLXHIP_DTYPE_BF16) {  // bf16 has f32's range: dS as it is
         scale = (float*)(ws + osc);
-        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, o.s, dloss, o.targets, o.rows, o.vocab, scale);
-        MLXHIP_TRY(launch_check("scale_kernel"));
+        MLXHIP_TRY(o.scales(dloss, (float*)(ws + op), scale));
     }
-    MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, xp));
+    MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, scale ? scale + ce::SCALE_X : nullptr, xp));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         const int64_t n = std::min(width, o.vocab - v0);
         const uint16_t* wp = (const uint16_t*)o.w + v0 * o.dim;
         if (copy_w) {
             wp = (uint16_t*)(ws + ow);
-            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, (uint16_t*)(ws + ow)));
+            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, scale ? scale + ce::SCALE_W : nullptr, (uint16_t*)(ws + ow)));
         }
         Args z;
         z.a = xp;

@@ -146,11 +146,24 @@ def embedding_vjp(dy, ids, vocab, scale, dt):
 
 # ── linear cross entropy ──────────────────────────────────────────────────
 
-def _logits(x, w):
-    """z, and its error: dim terms of a product in f32, and six roundings more
-    of the largest terms where an f32 product runs in bf16 planes."""
-    z = x @ w.T
-    return z, (x.shape[1] + 8) * U * (np.abs(x) @ np.abs(w).T)
+def _product(a, b, dt, ea=0.0):
+    """a @ b for operands of the type, a off by ea, and its error: the terms of
+    an f32 sum. f32 operands are two f16 values each: hi + lo is off by half a
+    step of lo, 2^-23 = 2u of the value, and lo lo (up to 2^-24 = u) is left
+    out: 5u more of each term; and where lo is a subnormal number by half of
+    2^-24 at a scale whose largest value is 2^14 at least, 2^-39 of it."""
+    mag = (np.abs(a) + ea) @ np.abs(b)
+    e = (a.shape[1] + 8) * U * mag
+    if np.ndim(ea):
+        e = e + ea @ np.abs(b)
+    if dt == abi.F32:
+        low = 2.0 ** -39
+        e = e + low * (np.abs(a).max(initial=0.0) * np.abs(b).sum(0) + np.abs(b).max(initial=0.0) * np.abs(a).sum(1)[:, None])
+    return a @ b, e
+
+
+def _logits(x, w, dt):
+    return _product(x, w.T, dt)
 
 
 def _lse(z, ez):
@@ -167,7 +180,7 @@ def _lse(z, ez):
 def cross_entropy(x, w, t, dt):
     """[(loss, bound), (lse, bound)]."""
     x, w = np.asarray(x, np.float64), np.asarray(w, np.float64)
-    z, ez = _logits(x, w)
+    z, ez = _logits(x, w, dt)
     lse, el = _lse(z, ez)
     on = (t >= 0) & (t < len(w))
     at = np.where(on, t, 0)
@@ -176,9 +189,11 @@ def cross_entropy(x, w, t, dt):
 
 
 def cross_entropy_vjp(x, w, t, dloss, dt):
-    """[(dx, bound), (dw, bound)] with the kernel's own lse."""
+    """[(dx, bound), (dw, bound)] with the kernel's own lse. What rows without a
+    target hold does not enter (zeros here)."""
     x, w, g = (np.asarray(a, np.float64) for a in (x, w, dloss))
-    z, ez = _logits(x, w)
+    x = np.where(((t >= 0) & (t < len(w)))[:, None], x, 0.0)
+    z, ez = _logits(x, w, dt)
     lse, el = _lse(z, ez)
     on = (t >= 0) & (t < len(w))
     p = np.exp(z - lse[:, None])
@@ -190,11 +205,13 @@ def cross_entropy_vjp(x, w, t, dloss, dt):
     gg = np.where(on, g, 0.0)[:, None]
     xx = np.where(on[:, None], x, 0.0)
     ds, eds = p * gg, (ep + 2 * U * np.abs(p)) * np.abs(gg)
-    if dt != abi.F32:  # dS is stored in 16 bits (f16: scaled, so its smallest values are 2^-40 of the largest)
-        eds = eds * (1 + HALF[dt]) + HALF[dt] * np.abs(ds) + 2.0 ** -38 * np.abs(g[on]).max(initial=0.0)
+    # dS is stored in 16 bits, f32's in two f16 values (_product); both f16 forms
+    # scaled, so that half the smallest step is 2^-39 of the largest dloss.
+    if dt != abi.F32:
+        eds = eds * (1 + HALF[dt]) + HALF[dt] * np.abs(ds)
+    eds = eds + 2.0 ** -39 * np.abs(g[on]).max(initial=0.0)
     out = []
     for a, ea, m in ((ds, eds, w), (ds.T, eds.T, xx)):
-        v = a @ m
-        b = ea @ np.abs(m) + (a.shape[1] + 8) * U * ((np.abs(a) + ea) @ np.abs(m))
+        v, b = _product(a, m, dt, ea)
         out.append((v, b * (1 + HALF[dt]) + HALF[dt] * np.abs(v) + TINY[dt]))
     return out

@@ -103,6 +103,33 @@ def test_far_apart_logits_with_other_targets(rows, dt):
     check_all(run(x, w, t, g, dt), x, w, t, g, dt, "spread 100, other targets")
 
 
+@pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
+@pytest.mark.parametrize("rows,dim", [(5, 64), (270, 264)])
+def test_values_of_very_different_size(rows, dim, dt):
+    """Elements, rows and dloss over some twenty binary orders of magnitude
+    (f32 and f16 hold their small parts scaled), a vocabulary entry that is all
+    zeros, and rows without a target that hold huge values."""
+    vocab = 515
+    x, w, t, g = inputs(rows, dim, vocab, dt)
+    spread = lambda seed, shape, n: np.exp2(-np.floor(n * synth.uniform01(seed, int(np.prod(shape))))).reshape(shape)
+    x = R.rounded((x * spread(1, (rows, 1), 6) * spread(2, (rows, dim), 8)).astype(np.float32), dt)
+    w = R.rounded((w * spread(3, (vocab, 1), 6) * spread(4, (vocab, dim), 8)).astype(np.float32), dt)
+    w[3] = 0.0
+    x[0] = 0.0
+    t[0] = 3
+    g = (g * spread(5, (rows,), 12)).astype(np.float32)
+    off = (t < 0) | (t >= vocab)
+    if dt != abi.F16:
+        x[off] *= 2.0 ** 60
+    got = run(x, w, t, g, dt)
+    fine = ~off
+    want = R.cross_entropy(x[fine], w, t[fine], dt)
+    R.check(got[0][fine], *want[0], "loss")
+    R.check(got[1][fine], *want[1], "lse")
+    for name, a, b in zip(("dx", "dw"), got[2:], R.cross_entropy_vjp(x, w, t, g, dt)):
+        R.check(a, *b, name)
+
+
 @pytest.mark.parametrize("rows", [4, 300])
 def test_non_finite_rows_stay_in_their_rows(rows):
     """NaN and infinity in x of counted rows: NaN loss, lse and dx there and
