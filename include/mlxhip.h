@@ -101,7 +101,27 @@ typedef enum {
      * axis; output [3, <input shape>] = dQ, dK, dV (mlxhip_attention_vjp). */
     MLXHIP_OP_HEAD_ATTENTION = 34,        /* scale, causal, axis (heads per row, if has_axis) */
     MLXHIP_OP_HEAD_ATTENTION_VJP = 35,    /* scale, causal, axis (heads per row, if has_axis) */
-    MLXHIP_OP_COUNT_ = 36
+    /* Extensions for training a language model (no reference counterpart: its
+     * Embedding has no VJP, its LayerNorm no weight, and it has no loss over a
+     * vocabulary). ids and targets are f32 values of whole numbers (below 2^24,
+     * which bounds the vocabulary), as Embedding's.
+     * ScaledEmbedding: w [vocab, dim], ids -> ids' shape + [dim]
+     * (mlxhip_embedding_rows). EmbeddingVjp: dy, ids -> [vocab, dim], the output's
+     * shape (mlxhip_embedding_vjp_rows); also the VJP of Embedding, with scale 1.
+     * LayerNormAffine: x, w, b -> x's shape (mlxhip_layernorm_affine_rows).
+     * LayerNormAffineVjp: dy, x, w -> [rows + 2, cols]: dx, then dw, then db.
+     * LinearCrossEntropy: x [rows, dim], w [vocab, dim], targets [rows] -> loss
+     * [rows] (mlxhip_linear_cross_entropy; a target that is no whole number of
+     * [0, vocab), NaN among them, takes its row out). LinearCrossEntropyVjp:
+     * dloss, x, w, targets, loss -> [rows + vocab, dim]: dx, then dw; with
+     * has_axis dx alone (axis 0) or dw alone (axis 1). */
+    MLXHIP_OP_SCALED_EMBEDDING = 36,      /* scale */
+    MLXHIP_OP_EMBEDDING_VJP = 37,         /* scale */
+    MLXHIP_OP_LAYER_NORM_AFFINE = 38,     /* eps */
+    MLXHIP_OP_LAYER_NORM_AFFINE_VJP = 39, /* eps */
+    MLXHIP_OP_LINEAR_CROSS_ENTROPY = 40,
+    MLXHIP_OP_LINEAR_CROSS_ENTROPY_VJP = 41, /* axis (one gradient, if has_axis) */
+    MLXHIP_OP_COUNT_ = 42
 } mlxhip_op_kind_t;
 
 /* One OpKind value with its parameters. Fields an op does not use are
@@ -651,7 +671,12 @@ void mlxhip_stream_destroy_hip(void* stream);
  * kernel entry points called on `stream` between mlxhip_graph_begin and
  * mlxhip_graph_end, by the calling thread, are recorded instead of run;
  * mlxhip_graph_launch replays the whole sequence with the same arguments.
- * `stream` must be a created stream (not NULL). The Stream and decoder
+ * `stream` must be a created stream (not NULL). A graph holds workspaces of its
+ * own for the calls recorded in it until it is freed (which waits for the
+ * device): different graphs may replay at once, on any streams, but one graph's
+ * launches must not overlap each other. A graph captured by other means uses the
+ * workspaces of the stream it was captured on, as eager calls on that stream do:
+ * none of these may overlap. The Stream and decoder
  * objects and mlxhip_eval_node synchronise internally and cannot be
  * recorded. No reference counterpart (the reference evaluates each node
  * when asked, crates/mlx-core/src/backend.rs:85-159). */

@@ -49,7 +49,8 @@ const char* op_name(int k) {
         "MatMul", "Reshape", "Transpose", "Softmax", "Silu", "Gelu", "LayerNorm", "RmsNorm", "Rope",
         "Broadcast", "Embedding", "ScaledMaskedSoftmax", "Attention", "LayerNormVjp", "RmsNormVjp",
         "SoftmaxVjp", "SiluVjp", "GeluVjp", "Sqrt", "RoPE", "Narrow", "Concatenate", "HeadAttention",
-        "HeadAttentionVjp"};
+        "HeadAttentionVjp", "ScaledEmbedding", "EmbeddingVjp", "LayerNormAffine", "LayerNormAffineVjp",
+        "LinearCrossEntropy", "LinearCrossEntropyVjp"};
     return (k >= 0 && k < MLXHIP_OP_COUNT_) ? names[k] : "?";
 }
 
@@ -148,6 +149,16 @@ struct Builder {
     uint64_t reshape(uint64_t a, const std::vector<int64_t>& shp) {
         if (!a) return 0;
         return node(op(MLXHIP_OP_RESHAPE), {a}, shp, meta(a).dtype, &shp);
+    }
+
+    // Rows [start, start + length) of a matrix, as a tensor of shape shp.
+    uint64_t part(uint64_t a, int64_t start, int64_t length, const std::vector<int64_t>& shp) {
+        mlxhip_op_t o = op(MLXHIP_OP_NARROW);
+        o.axis = 0;
+        o.has_axis = 1;
+        o.start = start;
+        o.length = length;
+        return reshape(node(o, {a}, {length, shape(a)[1]}, meta(a).dtype), shp);
     }
 
     uint64_t broadcast_to(uint64_t a, const std::vector<int64_t>& target) {
@@ -319,6 +330,57 @@ int vjp(Builder& b, uint64_t id, const Node& n, uint64_t g, const std::vector<bo
                 no.length = 1;
                 MLXHIP_SET(i, b.reshape(b.node(no, {all}, one, b.meta(id).dtype), sh));
             }
+            return MLXHIP_OK;
+        }
+        case MLXHIP_OP_EMBEDDING:
+        case MLXHIP_OP_SCALED_EMBEDDING: {
+            if (!arity(2)) return MLXHIP_ERR_INVALID_ARGUMENT;
+            if (need[1])
+                return fail(MLXHIP_ERR_INVALID_ARGUMENT, "VJP not implemented for %s: ids have no gradient", op_name(k));
+            if (!b.same_shape(g, id, op_name(k))) return recorded_status();
+            mlxhip_op_t o = Builder::op(MLXHIP_OP_EMBEDDING_VJP);
+            o.scale = k == MLXHIP_OP_EMBEDDING ? 1.0f : n.op.op.scale;
+            MLXHIP_SET(0, b.node(o, {g, in[1]}, b.shape(in[0]), b.meta(in[0]).dtype));
+            return MLXHIP_OK;
+        }
+        case MLXHIP_OP_LAYER_NORM_AFFINE: {
+            // One LayerNormAffineVjp node [rows + 2, cols]: dx, dw and db are
+            // Narrows of it along the leading axis, read in place.
+            if (!arity(3)) return MLXHIP_ERR_INVALID_ARGUMENT;
+            if (!b.same_shape(g, in[0], op_name(k))) return recorded_status();
+            const std::vector<int64_t> sh = b.shape(in[0]);
+            const int64_t cols = sh.empty() ? 0 : sh.back();
+            if (cols == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "LayerNormAffine gradient: rows of no columns");
+            const int64_t rows = b.meta(in[0]).numel() / cols;
+            mlxhip_op_t o = Builder::op(MLXHIP_OP_LAYER_NORM_AFFINE_VJP);
+            o.eps = n.op.op.eps;
+            const uint64_t all = b.node(o, {g, in[0], in[1]}, {rows + 2, cols}, b.meta(in[0]).dtype);
+            if (!all) return recorded_status();
+            MLXHIP_SET(0, b.part(all, 0, rows, sh));
+            MLXHIP_SET(1, b.part(all, rows, 1, b.shape(in[1])));
+            MLXHIP_SET(2, b.part(all, rows + 1, 1, b.shape(in[2])));
+            return MLXHIP_OK;
+        }
+        case MLXHIP_OP_LINEAR_CROSS_ENTROPY: {
+            if (!arity(3)) return MLXHIP_ERR_INVALID_ARGUMENT;
+            if (need[2])
+                return fail(MLXHIP_ERR_INVALID_ARGUMENT, "VJP not implemented for %s: targets have no gradient", op_name(k));
+            if (!b.same_shape(g, id, op_name(k))) return recorded_status();
+            const std::vector<int64_t> xs = b.shape(in[0]), ws = b.shape(in[1]);
+            if (xs.size() != 2 || ws.size() != 2) return fail_shape(xs, ws, op_name(k));
+            mlxhip_op_t o = Builder::op(MLXHIP_OP_LINEAR_CROSS_ENTROPY_VJP);
+            const std::vector<uint64_t> ins = {g, in[0], in[1], in[2], id};
+            const int dt = b.meta(in[0]).dtype;
+            if (need[0] && need[1]) {
+                const uint64_t all = b.node(o, ins, {xs[0] + ws[0], xs[1]}, dt);
+                if (!all) return recorded_status();
+                MLXHIP_SET(0, b.part(all, 0, xs[0], xs));
+                MLXHIP_SET(1, b.part(all, xs[0], ws[0], ws));
+                return MLXHIP_OK;
+            }
+            o.has_axis = 1;
+            o.axis = need[0] ? 0 : 1;
+            MLXHIP_SET(o.axis, b.node(o, ins, o.axis ? ws : xs, dt));
             return MLXHIP_OK;
         }
         case MLXHIP_OP_SILU:

@@ -260,6 +260,13 @@ struct WsCache {
     std::mutex mu;
     std::map<WsKey, WsBlock> live;
     std::multimap<std::pair<int, hipStream_t>, void*> retired;
+    // Recordings under way (mlxhip_graph_begin): a recording's blocks by slot,
+    // those outgrown during it among `all`. They go to its graph.
+    struct Recording {
+        std::map<int, WsBlock> live;
+        std::vector<void*> all;
+    };
+    std::map<std::pair<int, hipStream_t>, Recording> recordings;
 };
 WsCache& ws_cache() {
     static WsCache* c = new WsCache();  // never destroyed: outlives late calls at exit
@@ -272,7 +279,9 @@ int stream_workspace(hipStream_t s, int slot, size_t bytes, void** out) {
     MLXHIP_HIP(hipGetDevice(&dev));
     WsCache& C = ws_cache();
     std::lock_guard<std::mutex> g(C.mu);
-    WsBlock& b = C.live[WsKey{dev, s, slot}];
+    auto rec = C.recordings.find(std::make_pair(dev, s));
+    const bool recording = rec != C.recordings.end();
+    WsBlock& b = recording ? rec->second.live[slot] : C.live[WsKey{dev, s, slot}];
     if (b.cap < bytes || !b.p) {
         // Grow geometrically (256-byte granules) so a slowly growing sequence
         // of requests allocates O(log) times.
@@ -280,21 +289,48 @@ int stream_workspace(hipStream_t s, int slot, size_t bytes, void** out) {
         cap = std::max<size_t>((cap + 255) & ~size_t(255), 256);
         // During stream capture (mlxhip_graph_begin) an allocation is not a
         // stream operation: switch this thread to relaxed capture mode around
-        // it, then back. The block outlives the recorded graph (retired
-        // blocks are kept), so a replay never sees freed memory.
+        // it, then back. A recorded graph keeps the blocks of its recording
+        // until it is freed, so a replay never sees memory that is freed, or
+        // that another graph or an eager call uses.
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
         const bool exchanged = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
         void* p = pool_alloc(cap);
         if (exchanged) (void)hipThreadExchangeStreamCaptureMode(&mode);
         (void)hipGetLastError();
         if (!p) return fail(MLXHIP_ERR_FFI_FAILED, "workspace: device allocation of %zu bytes failed", cap);
-        if (b.p) C.retired.emplace(std::make_pair(dev, s), b.p);
+        if (recording) rec->second.all.push_back(p);
+        else if (b.p) C.retired.emplace(std::make_pair(dev, s), b.p);
         b.p = p;
         b.cap = cap;
     }
     *out = b.p;
     return MLXHIP_OK;
 }
+
+namespace {
+// Workspaces asked for on `s` from now on belong to a recording; false if one
+// is under way there already.
+bool begin_recording(hipStream_t s) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    WsCache& C = ws_cache();
+    std::lock_guard<std::mutex> g(C.mu);
+    return C.recordings.emplace(std::make_pair(dev, s), WsCache::Recording{}).second;
+}
+
+// Ends it (on any device: the caller's may have changed) and hands over its blocks.
+std::vector<void*> end_recording(hipStream_t s) {
+    WsCache& C = ws_cache();
+    std::lock_guard<std::mutex> g(C.mu);
+    for (auto it = C.recordings.begin(); it != C.recordings.end(); ++it)
+        if (it->first.second == s) {
+            std::vector<void*> blocks = std::move(it->second.all);
+            C.recordings.erase(it);
+            return blocks;
+        }
+    return {};
+}
+}  // namespace
 
 void release_stream_workspaces(hipStream_t s) {
     int dev = 0;
@@ -523,6 +559,103 @@ int eval_head_attention_vjp(const mlxhip_op_t& op, const mlxhip_input_t* in, siz
                          g * hg, t, w / hg, op.scale, op.causal, s, hg, w);
 }
 
+// Whole numbers below 2^24 held as f32 (ids, targets) as int32 in scratch.
+int ids_of(const mlxhip_input_t& in, bool targets, int32_t** out, hipStream_t s, Scratch& scratch) {
+    *out = static_cast<int32_t*>(scratch.get_bytes(std::max<size_t>(in.len, 1) * sizeof(int32_t)));
+    if (!*out) return fail(MLXHIP_ERR_FFI_FAILED, "scratch allocation failed");
+    return ids_from_f32(in.data, *out, (int64_t)in.len, targets, s);
+}
+
+int check_vocab(const char* what, int64_t vocab) {
+    if (vocab < 1 || vocab > (1 << 24))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: %lld rows of the table (f32 ids reach 2^24)", what, (long long)vocab);
+    return MLXHIP_OK;
+}
+
+int eval_scaled_embedding(const mlxhip_op_t& op, const mlxhip_input_t* in, size_t n_inputs, const mlxhip_meta_t& meta,
+                          float* out, hipStream_t s, Scratch& scratch) {
+    if (n_inputs != 2) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "ScaledEmbedding requires exactly 2 inputs [w, ids]");
+    if (in[0].ndim != 2) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "ScaledEmbedding weight must be 2D [vocab, dim]");
+    const int64_t n = (int64_t)in[1].len, vocab = in[0].shape[0], dim = in[0].shape[1];
+    MLXHIP_TRY(expect_len(n * dim, numel_of(meta.shape, meta.ndim), "ScaledEmbedding"));
+    if (n * dim == 0) return MLXHIP_OK;
+    MLXHIP_TRY(check_vocab("ScaledEmbedding", vocab));
+    int32_t* ids = nullptr;
+    MLXHIP_TRY(ids_of(in[1], false, &ids, s, scratch));
+    return mlxhip_embedding_rows(MLXHIP_DTYPE_F32, in[0].data, ids, out, n, vocab, dim, op.scale, s);
+}
+
+int eval_embedding_vjp(const mlxhip_op_t& op, const mlxhip_input_t* in, size_t n_inputs, const mlxhip_meta_t& meta,
+                       float* out, hipStream_t s, Scratch& scratch) {
+    if (n_inputs != 2) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "EmbeddingVjp requires exactly 2 inputs [dy, ids]");
+    if (meta.ndim != 2) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "EmbeddingVjp output must be 2D [vocab, dim]");
+    const int64_t n = (int64_t)in[1].len, vocab = meta.shape[0], dim = meta.shape[1];
+    MLXHIP_TRY(expect_len((int64_t)in[0].len, n * dim, "EmbeddingVjp"));
+    if (vocab * dim == 0) return MLXHIP_OK;
+    MLXHIP_TRY(check_vocab("EmbeddingVjp", vocab));
+    int32_t* ids = nullptr;
+    MLXHIP_TRY(ids_of(in[1], false, &ids, s, scratch));
+    return mlxhip_embedding_vjp_rows(MLXHIP_DTYPE_F32, in[0].data, ids, out, n, vocab, dim, op.scale, s);
+}
+
+int eval_layer_norm_affine(const mlxhip_op_t& op, const mlxhip_input_t* in, size_t n_inputs, const mlxhip_meta_t& meta,
+                           float* out, hipStream_t s) {
+    const bool grad = op.kind == MLXHIP_OP_LAYER_NORM_AFFINE_VJP;
+    const char* what = grad ? "LayerNormAffineVjp" : "LayerNormAffine";
+    if (n_inputs != 3)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s requires exactly 3 inputs %s", what, grad ? "[dy, x, w]" : "[x, w, b]");
+    const mlxhip_input_t &x = in[grad ? 1 : 0], &w = in[grad ? 2 : 1];
+    if (x.ndim == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s requires at least 1D input", what);
+    const int64_t cols = x.shape[x.ndim - 1], rows = cols ? (int64_t)x.len / cols : 0;
+    MLXHIP_TRY(expect_len((int64_t)w.len, cols, what));
+    if (grad) {
+        if (!same_shape(in[0], x))
+            return fail_shape(std::vector<int64_t>(x.shape, x.shape + x.ndim),
+                              std::vector<int64_t>(in[0].shape, in[0].shape + in[0].ndim), what);
+        MLXHIP_TRY(expect_len((rows + 2) * cols, numel_of(meta.shape, meta.ndim), what));
+        float* dw = out + rows * cols;
+        return mlxhip_layernorm_affine_vjp_rows(MLXHIP_DTYPE_F32, in[0].data, x.data, w.data, out, dw, dw + cols, rows, cols,
+                                                op.eps, s);
+    }
+    MLXHIP_TRY(expect_len((int64_t)in[2].len, cols, what));
+    MLXHIP_TRY(expect_len((int64_t)x.len, numel_of(meta.shape, meta.ndim), what));
+    return mlxhip_layernorm_affine_rows(MLXHIP_DTYPE_F32, x.data, w.data, in[2].data, out, rows, cols, op.eps, s);
+}
+
+int eval_linear_cross_entropy(const mlxhip_op_t& op, const mlxhip_input_t* in, size_t n_inputs, const mlxhip_meta_t& meta,
+                              float* out, hipStream_t s, Scratch& scratch) {
+    const bool grad = op.kind == MLXHIP_OP_LINEAR_CROSS_ENTROPY_VJP;
+    const char* what = grad ? "LinearCrossEntropyVjp" : "LinearCrossEntropy";
+    if (n_inputs != (grad ? 5 : 3))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s requires exactly %s", what,
+                    grad ? "5 inputs [dloss, x, w, targets, loss]" : "3 inputs [x, w, targets]");
+    const mlxhip_input_t &x = in[grad ? 1 : 0], &w = in[grad ? 2 : 1], &t = in[grad ? 3 : 2];
+    if (x.ndim != 2 || w.ndim != 2 || x.shape[1] != w.shape[1])
+        return fail_shape(std::vector<int64_t>(x.shape, x.shape + x.ndim), std::vector<int64_t>(w.shape, w.shape + w.ndim),
+                          what);
+    const int64_t rows = x.shape[0], dim = x.shape[1], vocab = w.shape[0], out_n = numel_of(meta.shape, meta.ndim);
+    MLXHIP_TRY(expect_len((int64_t)t.len, rows, what));
+    MLXHIP_TRY(check_vocab(what, vocab));
+    int32_t* ids = nullptr;
+    MLXHIP_TRY(ids_of(t, true, &ids, s, scratch));
+    // lse of the forward pass: given out, or what the loss says it was.
+    float* lse = scratch.get((size_t)std::max<int64_t>(rows, 1));
+    if (!lse) return fail(MLXHIP_ERR_FFI_FAILED, "%s: scratch allocation failed", what);
+    if (!grad) {
+        MLXHIP_TRY(expect_len(rows, out_n, what));
+        return mlxhip_linear_cross_entropy(MLXHIP_DTYPE_F32, x.data, w.data, ids, out, lse, rows, dim, vocab, s);
+    }
+    MLXHIP_TRY(expect_len((int64_t)in[0].len, rows, what));
+    MLXHIP_TRY(expect_len((int64_t)in[4].len, rows, what));
+    if (op.has_axis && op.axis != 0 && op.axis != 1)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: axis %d (0: dx, 1: dw)", what, op.axis);
+    const bool dx = !op.has_axis || op.axis == 0, dw = !op.has_axis || op.axis == 1;
+    MLXHIP_TRY(expect_len((dx ? rows * dim : 0) + (dw ? vocab * dim : 0), out_n, what));
+    MLXHIP_TRY(linear_cross_entropy_lse(x.data, w.data, ids, in[4].data, lse, rows, dim, vocab, s));
+    return mlxhip_linear_cross_entropy_vjp(MLXHIP_DTYPE_F32, x.data, w.data, ids, lse, in[0].data, dx && rows ? out : nullptr,
+                                           dw ? out + (dx ? rows * dim : 0) : nullptr, rows, dim, vocab, s);
+}
+
 }  // namespace
 
 int eval_matmul_group(int groups, const mlxhip_input_t* in, const int* hints, float* const* outs, hipStream_t s,
@@ -726,6 +859,13 @@ int eval_node_device(const mlxhip_op_t& op, const mlxhip_input_t* in, size_t n_i
         case MLXHIP_OP_ATTENTION: return eval_attention(op, in, n_inputs, meta, out, s, scratch);
         case MLXHIP_OP_HEAD_ATTENTION: return eval_head_attention(op, in, n_inputs, meta, out, s, scratch);
         case MLXHIP_OP_HEAD_ATTENTION_VJP: return eval_head_attention_vjp(op, in, n_inputs, meta, out, s);
+        case MLXHIP_OP_SCALED_EMBEDDING: return eval_scaled_embedding(op, in, n_inputs, meta, out, s, scratch);
+        case MLXHIP_OP_EMBEDDING_VJP: return eval_embedding_vjp(op, in, n_inputs, meta, out, s, scratch);
+        case MLXHIP_OP_LAYER_NORM_AFFINE:
+        case MLXHIP_OP_LAYER_NORM_AFFINE_VJP: return eval_layer_norm_affine(op, in, n_inputs, meta, out, s);
+        case MLXHIP_OP_LINEAR_CROSS_ENTROPY:
+        case MLXHIP_OP_LINEAR_CROSS_ENTROPY_VJP:
+            return eval_linear_cross_entropy(op, in, n_inputs, meta, out, s, scratch);
         case MLXHIP_OP_LAYER_NORM_VJP:
         case MLXHIP_OP_RMS_NORM_VJP: {
             REQUIRE(0);
@@ -1232,12 +1372,16 @@ void mlxhip_stream_destroy_hip(void* stream) {
 struct mlxhip_graph_t {
     hipGraph_t graph = nullptr;
     hipGraphExec_t exec = nullptr;
+    std::vector<void*> blocks;  // workspaces that its kernels use
+    int device = 0;
 };
 
 int mlxhip_graph_begin(void* stream) {
     MLXHIP_TRY(ensure_device());
     if (!stream) return fail(MLXHIP_ERR_NULL_PTR, "graph_begin: the null stream cannot be recorded");
     MLXHIP_HIP(hipStreamBeginCapture(as_stream(stream), hipStreamCaptureModeThreadLocal));
+    for (void* p : end_recording(as_stream(stream))) pool_release(p);  // of a stream destroyed while recorded
+    (void)begin_recording(as_stream(stream));
     return MLXHIP_OK;
 }
 
@@ -1248,8 +1392,13 @@ mlxhip_graph_t* mlxhip_graph_end(void* stream) {
     }
     hipGraph_t g = nullptr;
     const hipError_t e = hipStreamEndCapture(as_stream(stream), &g);
+    std::vector<void*> blocks = end_recording(as_stream(stream));
+    auto release = [&] {  // nothing recorded has run
+        for (void* p : blocks) pool_release(p);
+    };
     if (e != hipSuccess || !g) {
         if (g) (void)hipGraphDestroy(g);
+        release();
         hip_fail(e != hipSuccess ? e : hipErrorInvalidValue, "hipStreamEndCapture");
         return nullptr;
     }
@@ -1257,10 +1406,13 @@ mlxhip_graph_t* mlxhip_graph_end(void* stream) {
     const hipError_t ei = hipGraphInstantiate(&x, g, nullptr, nullptr, 0);
     if (ei != hipSuccess) {
         (void)hipGraphDestroy(g);
+        release();
         hip_fail(ei, "hipGraphInstantiate");
         return nullptr;
     }
-    return new mlxhip_graph_t{g, x};
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    return new mlxhip_graph_t{g, x, std::move(blocks), dev};
 }
 
 int mlxhip_graph_launch(mlxhip_graph_t* g, void* stream) {
@@ -1271,6 +1423,17 @@ int mlxhip_graph_launch(mlxhip_graph_t* g, void* stream) {
 
 void mlxhip_graph_free(mlxhip_graph_t* g) {
     if (!g) return;
+    // Launches may still use the workspaces: they return to the pool once the
+    // device is idle (and stay allocated where that cannot be known).
+    if (!g->blocks.empty()) {
+        int cur = 0;
+        (void)hipGetDevice(&cur);
+        if (cur != g->device) (void)hipSetDevice(g->device);
+        if (hipDeviceSynchronize() == hipSuccess)
+            for (void* p : g->blocks) pool_release(p);
+        (void)hipGetLastError();
+        if (cur != g->device) (void)hipSetDevice(cur);
+    }
     (void)hipGraphExecDestroy(g->exec);
     (void)hipGraphDestroy(g->graph);
     delete g;

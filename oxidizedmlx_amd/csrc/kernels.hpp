@@ -97,6 +97,13 @@ int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t
                              const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
                              hipStream_t s);
 
+// lse of rows with a target from their loss: loss + x_r . w_target (f32).
+int linear_cross_entropy_lse(const float* x, const float* w, const int32_t* targets, const float* loss, float* lse,
+                             int64_t rows, int64_t dim, int64_t vocab, hipStream_t s);
+// Whole numbers held as f32 as int32: saturating, NaN to 0 (the Embedding
+// op's ids), or with `targets` -1 for NaN and what is out of int32's range.
+int ids_from_f32(const float* x, int32_t* ids, int64_t n, bool targets, hipStream_t s);
+
 // ── decode.hip (greedy decode step of a decoder-only model) ───────────────
 constexpr int DEC_MAX_BATCH = 8;          // sequences per decode step
 constexpr int DEC_LDS_LIMIT = 159 * 1024; // dynamic LDS (a CDNA4 CU has 160 KiB; 1 KiB kept for static LDS)

@@ -215,6 +215,20 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums,
     }
 }
 
+__global__ __launch_bounds__(256) void lse_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                                                  const int32_t* __restrict__ targets, const float* __restrict__ loss,
+                                                  float* __restrict__ lse, int64_t rows, int64_t dim, int64_t vocab) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    const int32_t t = targets[r];
+    float z = 0.0f;
+    if (counted(t, vocab))
+        for (int64_t c = lane; c < dim; c += 64) z = fmaf(x[r * dim + c], w[t * dim + c], z);
+    z = dev::wave_sum(z);
+    if (lane == 0) lse[r] = loss[r] + z;
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void zero_kernel(T* __restrict__ p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = T(0);
@@ -440,6 +454,14 @@ int linear_cross_entropy(int dt, const void* x, const void* w, const int32_t* ta
         }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "linear_cross_entropy: dtype %d (f32, bf16 or f16)", dt);
     return rc;
+}
+
+int linear_cross_entropy_lse(const float* x, const float* w, const int32_t* targets, const float* loss, float* lse,
+                             int64_t rows, int64_t dim, int64_t vocab, hipStream_t s) {
+    if (rows == 0) return MLXHIP_OK;
+    hipLaunchKernelGGL(lse_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, x, w, targets, loss, lse, rows, dim,
+                       vocab);
+    return launch_check("lse_kernel");
 }
 
 int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t* targets, const float* lse,

@@ -716,6 +716,14 @@ __global__ __launch_bounds__(BLOCK) void embedding_kernel(const float* __restric
     }
 }
 
+__global__ __launch_bounds__(BLOCK) void ids_kernel(const float* __restrict__ x, int32_t* __restrict__ ids, int64_t n,
+                                                    bool targets) {
+    FOR_EACH_ELEMENT(i, n) {
+        const float f = x[i];
+        ids[i] = targets && !(f >= 0.0f && f < 2147483648.0f) ? -1 : f2i_sat(f);
+    }
+}
+
 __global__ __launch_bounds__(BLOCK) void narrow_kernel(const float* __restrict__ x,
                                                        float* __restrict__ y, int64_t outer,
                                                        int64_t dim, int64_t inner, int64_t start,
@@ -1099,6 +1107,12 @@ int embedding(const float* w, const float* idx, float* y, int64_t n_idx, int64_t
     hipLaunchKernelGGL(embedding_kernel, dim3(grid_for(n_idx * dim)), dim3(BLOCK), 0, s, w, idx, y,
                        n_idx, num_emb, dim);
     return launch_check("embedding_kernel");
+}
+
+int ids_from_f32(const float* x, int32_t* ids, int64_t n, bool targets, hipStream_t s) {
+    if (n == 0) return MLXHIP_OK;
+    hipLaunchKernelGGL(ids_kernel, dim3(grid_for(n)), dim3(BLOCK), 0, s, x, ids, n, targets);
+    return launch_check("ids_kernel");
 }
 
 int narrow(const float* x, float* y, int64_t outer, int64_t dim, int64_t inner, int64_t start,

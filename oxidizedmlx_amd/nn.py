@@ -59,14 +59,21 @@ class RmsNorm:
 
 
 class LayerNorm:
-    """(x - mean) / sqrt(var + eps) over the last axis (crates/mlx-nn/src/norm.rs:12-36)."""
+    """(x - mean) / sqrt(var + eps) over the last axis (crates/mlx-nn/src/norm.rs:12-36),
+    times ``weight`` plus ``bias`` ([dim] each) where given (one op with its own
+    gradients; HIP streams only)."""
 
-    def __init__(self, dim: int, eps: float = 1e-5):
+    def __init__(self, dim: int, eps: float = 1e-5, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None):
+        if (weight is None) != (bias is None):
+            raise abi.InvalidArgument("LayerNorm takes a weight and a bias, or neither")
         self.dim, self.eps = dim, eps
+        self.weight, self.bias = weight, bias
 
     def forward(self, x: Tensor) -> Tensor:
         if not x.shape or x.shape[-1] != self.dim:
             raise abi.InvalidArgument(f"LayerNorm expected last dim {self.dim}")
+        if self.weight is not None:
+            return x.layer_norm_affine(self.weight, self.bias, self.eps)
         return x.layer_norm(self.eps)
 
     __call__ = forward
@@ -313,13 +320,40 @@ def decoder_params(cfg: DecoderConfig, seed: int, std: float = 0.02) -> dict:
 
 
 class Embedding:
-    """Rows of weight [num_embeddings, dim] at integer ids (crates/mlx-nn/src/embed.rs)."""
+    """Rows of weight [num_embeddings, dim] at integer ids (crates/mlx-nn/src/embed.rs),
+    times ``scale`` where one is given (HIP streams only). The weight's
+    gradient sums the rows of each id (HIP streams)."""
+
+    def __init__(self, weight: Tensor, scale: Optional[float] = None):
+        self.weight, self.scale = weight, scale
+
+    def forward(self, ids: Tensor) -> Tensor:
+        if self.scale is not None:
+            return self.weight.scaled_embedding(ids, self.scale)
+        return self.weight.embedding_lookup(ids)
+
+    __call__ = forward
+
+
+class LinearCrossEntropy:
+    """Mean cross entropy of the logits x W^T of an output projection (weight
+    [vocab, dim], no bias) over the rows whose target lies in [0, vocab); HIP
+    streams only. The logits are never kept."""
 
     def __init__(self, weight: Tensor):
         self.weight = weight
 
-    def forward(self, ids: Tensor) -> Tensor:
-        return self.weight.embedding_lookup(ids)
+    def forward(self, x: Tensor, targets: np.ndarray) -> Tensor:
+        """x [rows, dim], targets [rows] whole numbers -> a scalar; 0 where no
+        row has a target."""
+        t = np.asarray(targets).reshape(-1)
+        vocab = self.weight.shape[0]
+        counted = max(1, int(np.count_nonzero((t >= 0) & (t < vocab))))
+        # Whole numbers up to 2^24 are exact in f32: a larger id must not round into the vocabulary.
+        ids = Tensor.from_f32_on_stream(np.where((t >= 0) & (t < vocab), t, -1).astype(np.float32), t.shape, x.stream)
+        share = Tensor.from_f32_on_stream(np.array([1.0 / counted], np.float32), (1,), x.stream)
+        loss = x.linear_cross_entropy(self.weight, ids)
+        return loss.mul(share.broadcast_to(loss.shape)).sum_all()
 
     __call__ = forward
 
@@ -339,13 +373,31 @@ class DecoderLM:
                              for lp in params["layers"]]
         self.norm = RmsNorm(d, cfg.eps)
 
-    def forward(self, tokens: np.ndarray) -> Tensor:
+    def hidden(self, tokens: np.ndarray) -> Tensor:
+        """The normed hidden states [batch*seq, d_model] that the LM head reads."""
         tokens = np.asarray(tokens)
         b, s = tokens.shape
         ids = Tensor.from_f32_on_stream(tokens.reshape(-1).astype(np.float32), (b * s,), self.stream)
         x = self.embed(ids)
         for lp in self.layer_params:
             x = TransformerBlock(self.cfg.block(b, s), lp)(x)
-        return self.lm_head(self.norm(x))
+        return self.norm(x)
+
+    def forward(self, tokens: np.ndarray) -> Tensor:
+        return self.lm_head(self.hidden(tokens))
+
+    def loss(self, tokens: np.ndarray, targets: np.ndarray) -> Tensor:
+        """Mean cross entropy of the next-token logits against ``targets``
+        [batch, seq] (an id outside [0, vocab), such as -100, counts for
+        nothing), without keeping the logits; HIP streams only.
+        ``value_and_grad`` differentiates it with respect to ``parameters()``."""
+        return LinearCrossEntropy(self.lm_head.weight)(self.hidden(tokens), targets)
+
+    def parameters(self) -> Dict[str, Tensor]:
+        """Every trained parameter by name (``layers.<i>.<name>`` in the blocks)."""
+        out = {"embedding": self.embed.weight, "lm_head": self.lm_head.weight}
+        for i, lp in enumerate(self.layer_params):
+            out.update({f"layers.{i}.{name}": t for name, t in lp.items()})
+        return out
 
     __call__ = forward

@@ -25,6 +25,8 @@ KIND = {
     "ScaledMaskedSoftmax": 23, "Attention": 24, "LayerNormVjp": 25, "RmsNormVjp": 26,
     "SoftmaxVjp": 27, "SiluVjp": 28, "GeluVjp": 29, "Sqrt": 30, "RoPE": 31,
     "Narrow": 32, "Concatenate": 33, "HeadAttention": 34, "HeadAttentionVjp": 35,
+    "ScaledEmbedding": 36, "EmbeddingVjp": 37, "LayerNormAffine": 38, "LayerNormAffineVjp": 39,
+    "LinearCrossEntropy": 40, "LinearCrossEntropyVjp": 41,
 }
 NAME = {v: k for k, v in KIND.items()}
 
@@ -126,6 +128,7 @@ class OpKind:
     Silu = Op("Silu")
     Gelu = Op("Gelu")
     Embedding = Op("Embedding")
+    LinearCrossEntropy = Op("LinearCrossEntropy")
     SiluVjp = Op("SiluVjp")
     GeluVjp = Op("GeluVjp")
     Sqrt = Op("Sqrt")
@@ -188,6 +191,33 @@ class OpKind:
     @staticmethod
     def HeadAttentionVjp(scale: float, causal: bool, heads: Optional[int] = None) -> Op:
         return Op("HeadAttentionVjp", scale=scale, causal=causal, axis=heads)
+
+    @staticmethod
+    def ScaledEmbedding(scale: float) -> Op:
+        """scale * w[ids] (no reference counterpart; differentiable)."""
+        return Op("ScaledEmbedding", scale=scale)
+
+    @staticmethod
+    def EmbeddingVjp(scale: float) -> Op:
+        """[dy, ids] -> the weight's gradient [vocab, dim] (the output's shape)."""
+        return Op("EmbeddingVjp", scale=scale)
+
+    @staticmethod
+    def LayerNormAffine(eps: float) -> Op:
+        """[x, w, b]: LayerNorm with a weight and a bias (no reference
+        counterpart; differentiable)."""
+        return Op("LayerNormAffine", eps=eps)
+
+    @staticmethod
+    def LayerNormAffineVjp(eps: float) -> Op:
+        """[dy, x, w] -> [rows + 2, cols]: dx, dw, db."""
+        return Op("LayerNormAffineVjp", eps=eps)
+
+    @staticmethod
+    def LinearCrossEntropyVjp(which: Optional[int] = None) -> Op:
+        """[dloss, x, w, targets, loss] -> [rows + vocab, dim]: dx, dw; or dx
+        (``which`` 0) or dw (1) alone."""
+        return Op("LinearCrossEntropyVjp", axis=which)
 
     @staticmethod
     def LayerNormVjp(eps: float) -> Op:

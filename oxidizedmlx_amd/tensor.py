@@ -230,6 +230,27 @@ class Tensor:
             raise abi.InvalidArgument("embedding weight must be 2D [num_embeddings, embedding_dim]")
         return self._lazy(OpKind.Embedding, [self, indices], indices.shape + (self.shape[1],))
 
+    def scaled_embedding(self, indices: "Tensor", scale: float) -> "Tensor":
+        """``scale`` times the rows of this [vocab, dim] weight at ``indices``
+        (ids as f32, clamped); HIP streams only, with a VJP for the weight."""
+        if len(self.shape) != 2:
+            raise abi.InvalidArgument("embedding weight must be 2D [vocab, dim]")
+        return self._lazy(OpKind.ScaledEmbedding(scale), [self, indices], indices.shape + (self.shape[1],))
+
+    def linear_cross_entropy(self, weight: "Tensor", targets: "Tensor") -> "Tensor":
+        """Cross entropy of the logits x W^T of this x [rows, dim] and a weight
+        [vocab, dim] against ``targets`` [rows] (ids as f32; one outside
+        [0, vocab) takes its row out): the loss of each row. The logits are
+        formed in pieces of the vocabulary and never kept. HIP streams only;
+        with VJPs for x and the weight."""
+        if len(self.shape) != 2 or len(weight.shape) != 2 or self.shape[1] != weight.shape[1]:
+            raise abi.ShapeMismatch(f"expected x [rows, dim] and weight [vocab, dim], got {list(self.shape)} and "
+                                    f"{list(weight.shape)}", list(self.shape), list(weight.shape))
+        if targets.shape != self.shape[:1]:
+            raise abi.ShapeMismatch(f"expected targets {list(self.shape[:1])}, got {list(targets.shape)}",
+                                    list(self.shape[:1]), list(targets.shape))
+        return self._lazy(OpKind.LinearCrossEntropy, [self, weight, targets], self.shape[:1])
+
     # ── shape ops (tensor.rs:322-374, 769-801) ───────────────────────────
     def reshape(self, shape: Sequence[int]) -> "Tensor":
         shape = _shape(shape)
@@ -339,6 +360,17 @@ class Tensor:
 
     def layer_norm(self, eps: float) -> "Tensor":
         return self._lazy(OpKind.LayerNorm(eps), [self], self.shape)
+
+    def layer_norm_affine(self, weight: "Tensor", bias: "Tensor", eps: float) -> "Tensor":
+        """LayerNorm over the last axis times ``weight`` plus ``bias`` (both
+        [cols]); HIP streams only, with VJPs for all three."""
+        if not self.shape:
+            raise abi.InvalidArgument("layer_norm_affine requires at least 1D input")
+        for t in (weight, bias):
+            if t.shape != self.shape[-1:]:
+                raise abi.ShapeMismatch(f"expected {list(self.shape[-1:])}, got {list(t.shape)}", list(self.shape[-1:]),
+                                        list(t.shape))
+        return self._lazy(OpKind.LayerNormAffine(eps), [self, weight, bias], self.shape)
 
     def rms_norm(self, eps: float) -> "Tensor":
         return self._lazy(OpKind.RmsNorm(eps), [self], self.shape)
