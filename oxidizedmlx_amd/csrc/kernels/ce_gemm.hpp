@@ -33,10 +33,6 @@ using gemm16::f32x4;
 using gemm16::u32x2;
 using gemm16::u32x4;
 
-// 16 bytes at an element's alignment.
-typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
-typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
-
 enum Product { CE_STATS = 0, CE_DS = 1, CE_DX = 2, CE_DW = 3 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -178,7 +174,7 @@ __device__ inline void store_tile(const f32x16 (&acc)[C::TM][C::TN], MLXHIP_LDS 
                                   int64_t ld, int64_t m, int64_t n, int64_t cap, int64_t row0, int64_t col0, int lane,
                                   bool add) {
     typedef typename dev::Elem<CT>::type T;
-    typedef std::conditional_t<sizeof(T) == 4, u32x4_at4, u32x4_at2> any;
+    typedef dev::AnyVec<CT> any;
     constexpr int TM = C::TM, TN = C::TN, ES = sizeof(T), VEC = 16 / ES;
     constexpr int ROW_BYTES = 32 * TN * ES, CHUNKS = ROW_BYTES / 16, SHARE = CHUNKS >= 16 ? 1 : 16 / CHUNKS;
     constexpr int PASS = C::EPI / ROW_BYTES < 32 ? C::EPI / ROW_BYTES : 32;  // rows staged at a time

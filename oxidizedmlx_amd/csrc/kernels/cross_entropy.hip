@@ -49,15 +49,9 @@ template <int OT, int P>
 __device__ inline void pack8(const typename Elem<OT>::type* src, int64_t c, int64_t dim, bool on, float f, uint16_t* dst,
                              int64_t plane) {
     constexpr int VEC = Elem<OT>::VEC;
-    union {
-        uint16_t h[8];
-        uint4 q;
-    } out;
     if constexpr (P == 1) {
-        const dev::Vec16<OT> v = dev::load_raw<OT>(src, c, dim);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out.h[e] = on ? v.v[e] : 0;
-        *reinterpret_cast<uint4*>(dst + c) = out.q;
+        const dev::u32x4 v = dev::load_raw<OT>(src, c, dim).q, none = {0, 0, 0, 0};
+        *reinterpret_cast<dev::u32x4*>(dst + c) = on ? v : none;
     } else {
         float v[8];
 #pragma unroll
@@ -66,12 +60,9 @@ __device__ inline void pack8(const typename Elem<OT>::type* src, int64_t c, int6
         for (int e = 0; e < 8; ++e) v[e] = on ? v[e] * f : 0.0f;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
+            dev::store_vec<MLXHIP_DTYPE_F16>(dst + p * plane, c, c + 8, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                out.h[e] = dev::from_f32<MLXHIP_DTYPE_F16>(v[e]);
-                v[e] -= dev::to_f32<MLXHIP_DTYPE_F16>(out.h[e]);
-            }
-            *reinterpret_cast<uint4*>(dst + p * plane + c) = out.q;
+            for (int e = 0; e < 8; ++e) v[e] -= dev::to_f32<MLXHIP_DTYPE_F16>(dev::from_f32<MLXHIP_DTYPE_F16>(v[e]));
         }
     }
 }
@@ -124,7 +115,7 @@ __global__ __launch_bounds__(256) void maxima_kernel(const float* __restrict__ w
                                            b = dev::load_raw<MLXHIP_DTYPE_F32>(p, i + 4, n);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = finite_abs(e < 4 ? a.v[e] : b.v[e - 4]);
+            const float v = finite_abs(__uint_as_float(e < 4 ? a.q[e] : b.q[e - 4]));
             if (blockIdx.y == 0 || (i + e < n && counted(targets[(i + e) / dim], vocab))) m = fmaxf(m, v);
         }
     }

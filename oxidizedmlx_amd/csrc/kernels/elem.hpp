@@ -38,11 +38,18 @@ __device__ inline typename Elem<DT>::type from_f32(float v) {
     else return __builtin_bit_cast(uint16_t, (_Float16)v);
 }
 
-// A 16-byte vector at any element-aligned address: one dwordx4 access (gfx950
-// allows unaligned global accesses).
+// A 16-byte vector of elements, as the four dwords that a load gives: kept so
+// until it is unpacked, a load in a branch waits for nothing where the branch
+// ends. At any element-aligned address: one dwordx4 access (gfx950 allows
+// unaligned global accesses).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
+typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
 template <int DT>
-struct __attribute__((packed, aligned(sizeof(typename Elem<DT>::type)))) Vec16 {
-    typename Elem<DT>::type v[Elem<DT>::VEC];
+using AnyVec = std::conditional_t<DT == MLXHIP_DTYPE_F32, u32x4_at4, u32x4_at2>;
+template <int DT>
+struct Vec16 {
+    u32x4 q;
 };
 
 // Elements [i, i + VEC) of p as they are, zeros from element n on. Separate
@@ -50,28 +57,37 @@ struct __attribute__((packed, aligned(sizeof(typename Elem<DT>::type)))) Vec16 {
 template <int DT>
 __device__ inline Vec16<DT> load_raw(const typename Elem<DT>::type* p, int64_t i, int64_t n) {
     constexpr int VEC = Elem<DT>::VEC;
-    if (i + VEC <= n) return *reinterpret_cast<const Vec16<DT>*>(p + i);
-    Vec16<DT> x{};
+    if (i + VEC <= n) return {*reinterpret_cast<const AnyVec<DT>*>(p + i)};
+    u32x4 q = {0, 0, 0, 0};
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-        if (i + e < n) x.v[e] = p[i + e];
-    return x;
+        if (i + e < n) {
+            if constexpr (DT == MLXHIP_DTYPE_F32) q[e] = __float_as_uint(p[i + e]);
+            else q[e / 2] |= (uint32_t)p[i + e] << (16 * (e & 1));
+        }
+    return {q};
 }
 
 template <int DT>
 __device__ inline void unpack(const Vec16<DT>& x, float* out) {
 #pragma unroll
-    for (int e = 0; e < Elem<DT>::VEC; ++e) out[e] = to_f32<DT>(x.v[e]);
+    for (int e = 0; e < Elem<DT>::VEC; ++e) {
+        if constexpr (DT == MLXHIP_DTYPE_F32) out[e] = __uint_as_float(x.q[e]);
+        else out[e] = to_f32<DT>((uint16_t)(x.q[e / 2] >> (16 * (e & 1))));
+    }
 }
 
 template <int DT>
 __device__ inline void store_vec(typename Elem<DT>::type* p, int64_t i, int64_t n, const float* v) {
     constexpr int VEC = Elem<DT>::VEC;
     if (i + VEC <= n) {
-        Vec16<DT> x;
+        u32x4 q;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x.v[e] = from_f32<DT>(v[e]);
-        *reinterpret_cast<Vec16<DT>*>(p + i) = x;
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (DT == MLXHIP_DTYPE_F32) q[k] = __float_as_uint(v[k]);
+            else q[k] = from_f32<DT>(v[2 * k]) | (uint32_t)from_f32<DT>(v[2 * k + 1]) << 16;
+        }
+        *reinterpret_cast<AnyVec<DT>*>(p + i) = q;
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)

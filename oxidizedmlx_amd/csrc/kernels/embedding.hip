@@ -39,25 +39,38 @@ constexpr int BITS = 8, BINS = 1 << BITS;
 // Positions that one workgroup sorts in its LDS (key and position, 8 bytes
 // each: 128 KiB), and those of a workgroup's block in a longer sort.
 constexpr int LDS_SORT = 16384;
-constexpr int BLOCK_SORT = 8192;
+constexpr int BLOCK_SORT = 2048;
+// Blocks whose counts the moving launch adds up itself.
+constexpr int SCAN_BLOCKS = 64;
 // Shares of the sorted list, about.
 constexpr int SHARES = 2048;
 
+// A wave copies ROWS rows at a time, all their loads in flight.
 template <int DT>
 __global__ __launch_bounds__(256) void embed_kernel(const typename Elem<DT>::type* __restrict__ w,
                                                     const int32_t* __restrict__ ids,
                                                     typename Elem<DT>::type* __restrict__ y, int64_t n, int64_t vocab,
                                                     int64_t dim, float scale) {
-    constexpr int VEC = Elem<DT>::VEC;
+    constexpr int VEC = Elem<DT>::VEC, ROWS = 4;
     const int lane = threadIdx.x & 63;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int64_t)gridDim.x * 4) {
-        const int64_t id = min(max((int64_t)ids[i], (int64_t)0), vocab - 1);
-        for (int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC; c < dim; c += (int64_t)gridDim.y * 64 * VEC) {
-            float v[VEC];
-            unpack<DT>(load_raw<DT>(w + id * dim, c, dim), v);
+    for (int64_t i = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS; i < n; i += (int64_t)gridDim.x * 4 * ROWS) {
+        int64_t id[ROWS];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] *= scale;
-            store_vec<DT>(y + i * dim, c, dim, v);
+        for (int k = 0; k < ROWS; ++k) id[k] = min(max((int64_t)ids[min(i + k, n - 1)], (int64_t)0), vocab - 1);
+        for (int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC; c < dim; c += (int64_t)gridDim.y * 64 * VEC) {
+            Vec16<DT> raw[ROWS];
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k)
+                if (i + k < n) raw[k] = load_raw<DT>(w + id[k] * dim, c, dim);
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                if (i + k >= n) break;
+                float v[VEC];
+                unpack<DT>(raw[k], v);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] *= scale;
+                store_vec<DT>(y + (i + k) * dim, c, dim, v);
+            }
         }
     }
 }
@@ -200,8 +213,9 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const int32_t*
 
 // One pass of a longer sort, in blocks of BLOCK_SORT positions: the blocks'
 // counts of each digit (counts[digit * blocks + block]), their scan along the
-// blocks, and the move to the places that follow. The first pass reads the
-// ids; its counting launch also zeroes dW with the workgroups past the blocks.
+// blocks (of few blocks: by the launch that follows), and the move to the places
+// that follow. The first pass reads the ids; its counting launch also zeroes dW
+// with the workgroups past the blocks.
 constexpr int BSTEPS = BLOCK_SORT / SORT_THREADS;
 
 __device__ inline void load_block(const int32_t* ids, const uint32_t* keys, int64_t n, uint32_t vocab, int64_t base,
@@ -265,7 +279,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
                                                                  const uint32_t* __restrict__ totals,
                                                                  uint32_t* __restrict__ keys_out,
                                                                  uint32_t* __restrict__ order_out) {
-    __shared__ uint32_t hist[BINS * SORT_WAVES], wave_sums[SORT_WAVES], start[BINS];
+    __shared__ uint32_t hist[BINS * SORT_WAVES], wave_sums[SORT_WAVES], start[BINS], total[BINS], before[BINS];
     const int64_t base = (int64_t)blockIdx.x * BLOCK_SORT, left = min((int64_t)BLOCK_SORT, n - base);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t key[BSTEPS], digit[BSTEPS], rank[BSTEPS];
@@ -274,12 +288,31 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
     for (int s = 0; s < BSTEPS; ++s) digit[s] = (key[s] >> shift) & (BINS - 1);
     local_ranks<BSTEPS>(digit, BSTEPS, wave * BSTEPS * 64, (int)left, hist, rank);
     scan_hist(hist, wave_sums);
+    // Digit d's elements in all blocks, and in those before this one.
+    if (threadIdx.x < BINS) {
+        const uint32_t* c = counts + (int64_t)threadIdx.x * blocks;
+        uint32_t all = 0, mine = 0;
+        if (totals) {
+            all = totals[threadIdx.x];
+            mine = c[blockIdx.x];
+        } else {
+#pragma unroll 8
+            for (int b = 0; b < blocks; ++b) {
+                const uint32_t v = c[b];
+                all += v;
+                if (b < (int)blockIdx.x) mine += v;
+            }
+        }
+        total[threadIdx.x] = all;
+        before[threadIdx.x] = mine;
+    }
+    __syncthreads();
     // Where the block's elements of a digit begin in the whole order, less
     // their place in the block's.
     if (wave == 0) {
         uint32_t sum = 0;
 #pragma unroll
-        for (int i = 0; i < BINS / 64; ++i) sum += totals[lane * (BINS / 64) + i];
+        for (int i = 0; i < BINS / 64; ++i) sum += total[lane * (BINS / 64) + i];
         uint32_t incl = sum;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -290,8 +323,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
 #pragma unroll
         for (int i = 0; i < BINS / 64; ++i) {
             const int d = lane * (BINS / 64) + i;
-            start[d] = at + counts[(int64_t)d * blocks + blockIdx.x] - hist[d * SORT_WAVES];
-            at += totals[d];
+            start[d] = at + before[d] - hist[d * SORT_WAVES];
+            at += total[d];
         }
     }
     __syncthreads();
@@ -309,6 +342,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
 // A wave's share of the sorted positions and chunk of 64 * VEC columns. part
 // holds two rows of dim sums per share: of the id that began before it, and
 // of the one that goes on after it (an id that does both: the first only).
+// The lanes hold 64 positions' keys and places, so the rows' addresses come
+// from registers and AHEAD of their loads are in flight.
 template <int DT>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                         const uint32_t* __restrict__ keys,
@@ -316,17 +351,20 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>:
                                                         int64_t shares, int64_t dim, float scale,
                                                         typename Elem<DT>::type* __restrict__ dw,
                                                         float* __restrict__ part) {
-    constexpr int VEC = Elem<DT>::VEC, AHEAD = 4;
+    constexpr int VEC = Elem<DT>::VEC, AHEAD = 8;
+    const int lane = threadIdx.x & 63;
     const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (sh >= shares) return;
-    const int64_t c = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * VEC;
-    if (c >= dim) return;
+    const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC;
+    const bool in = c < dim;  // every lane stays: its keys are the others' too
     const int64_t lo = sh * share, hi = min(n, lo + share);
     float acc[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    // The keys around the share, and its first one.
+    const uint32_t before = lo > 0 ? keys[lo - 1] : 0, after = hi < n ? keys[hi] : 0;
     uint32_t cur = keys[lo];
-    bool head = lo > 0 && keys[lo - 1] == cur;
+    bool head = lo > 0 && before == cur;
     auto leave = [&](float* to) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
@@ -335,7 +373,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>:
     auto flush = [&] {
         if (head) {
             leave(part + 2 * sh * dim);
-        } else {
+        } else if (in) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] *= scale;
             store_vec<DT>(dw + (int64_t)cur * dim, c, dim, acc);
@@ -344,57 +382,95 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>:
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
     };
-    for (int64_t i = lo; i < hi; i += AHEAD) {
-        Vec16<DT> raw[AHEAD];
-        uint32_t key[AHEAD];
+    for (int64_t i0 = lo; i0 < hi; i0 += 64) {
+        const int count = (int)min(hi - i0, (int64_t)64);
+        const int64_t mine = min(i0 + lane, hi - 1);
+        const int key_l = (int)keys[mine], pos_l = (int)order[mine];
+        for (int i = 0; i < count; i += AHEAD) {
+            Vec16<DT> raw[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            const int64_t j = min(i + a, hi - 1);
-            key[a] = keys[j];
-            raw[a] = load_raw<DT>(dy + (int64_t)order[j] * dim, c, dim);
-        }
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (i + a >= hi) break;
-            if (key[a] != cur) {
-                flush();
-                cur = key[a];
+            for (int a = 0; a < AHEAD; ++a) {
+                const uint32_t pos = (uint32_t)__builtin_amdgcn_readlane(pos_l, min(i + a, count - 1));
+                if (in) raw[a] = load_raw<DT>(dy + (int64_t)pos * dim, c, dim);
             }
-            float v[VEC];
-            unpack<DT>(raw[a], v);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+            for (int a = 0; a < AHEAD; ++a) {
+                if (i + a >= count) break;
+                const uint32_t key = (uint32_t)__builtin_amdgcn_readlane(key_l, i + a);
+                if (key != cur) {
+                    flush();
+                    cur = key;
+                }
+                if (in) {
+                    float v[VEC];
+                    unpack<DT>(raw[a], v);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] += v[e];
+                }
+            }
         }
     }
-    if (hi < n && keys[hi] == cur) leave(part + (2 * sh + (head ? 0 : 1)) * dim);
+    if (hi < n && after == cur) leave(part + (2 * sh + (head ? 0 : 1)) * dim);
     else flush();
 }
 
-// The ids that go on after share sh and began in it: their shares' sums, in order.
+// The ids that go on after a share and began in it: their shares' sums in
+// order, 64 columns at a time. A workgroup's four waves have a share each; an
+// id that reaches over more than ALONE of them (a frequent word's some hundred)
+// is added up by all four, a contiguous part of the shares each.
+constexpr int ALONE = 16;
 template <int DT>
 __global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t* __restrict__ keys, int64_t n, int share,
                                                          int64_t shares, int64_t dim, float scale,
                                                          typename Elem<DT>::type* __restrict__ dw,
                                                          const float* __restrict__ part) {
-    const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (sh + 1 >= shares) return;
-    const int64_t lo = sh * share, hi = lo + share;
-    const uint32_t key = keys[hi - 1];
-    if (keys[hi] != key || (keys[lo] == key && lo > 0 && keys[lo - 1] == key)) return;
-    // The last share that the id reaches: 64 of their first keys at a time.
-    int64_t last = sh + 1;
-    for (;;) {
-        const int64_t k = last + 1 + (threadIdx.x & 63);
-        const uint64_t go = __ballot(k < shares && keys[min(k, shares - 1) * share] == key);
-        const int run = ~go ? __builtin_ctzll(~go) : 64;
-        last += run;
-        if (run < 64) break;
+    __shared__ int64_t runs[4];  // the last share of a wave's id; 0: nothing to add up
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t sh = (int64_t)blockIdx.x * 4 + wave, c = (int64_t)blockIdx.y * 64 + lane;
+    int64_t last = 0;
+    uint32_t key = 0;
+    if (sh + 1 < shares) {
+        const int64_t lo = sh * share, hi = lo + share;
+        const uint32_t first = keys[lo], before = lo > 0 ? keys[lo - 1] : ~keys[lo], after = keys[hi];
+        key = keys[hi - 1];
+        if (after == key && (first != key || before != key)) {
+            // The last share that the id reaches: 64 of their first keys at a time.
+            last = sh + 1;
+            for (;;) {
+                const int64_t k = last + 1 + lane;
+                const uint64_t go = __ballot(k < shares && keys[min(k, shares - 1) * share] == key);
+                const int run = ~go ? __builtin_ctzll(~go) : 64;
+                last += run;
+                if (run < 64) break;
+            }
+        }
     }
-    for (int64_t c = (int64_t)blockIdx.y * 64 + (threadIdx.x & 63); c < dim; c += (int64_t)gridDim.y * 64) {
+    const bool alone = last - sh <= ALONE;
+    if (last && alone && c < dim) {
         float acc = part[(2 * sh + 1) * dim + c];
-#pragma unroll 16
+#pragma unroll 8
         for (int64_t k = sh + 1; k <= last; ++k) acc += part[2 * k * dim + c];
         dw[(int64_t)key * dim + c] = dev::from_f32<DT>(acc * scale);
+    }
+    if (lane == 0) runs[wave] = alone ? 0 : last;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+        const int64_t end = runs[w], from = (int64_t)blockIdx.x * 4 + w;
+        if (end == 0) continue;
+        const int64_t each = (end - from + 3) / 4, k0 = from + 1 + wave * each, k1 = min(k0 + each, end + 1);
+        float acc = 0.0f;
+        if (c < dim) {
+            if (wave == 0) acc = part[(2 * from + 1) * dim + c];
+#pragma unroll 16
+            for (int64_t k = k0; k < k1; ++k) acc += part[2 * k * dim + c];
+        }
+        sums[wave][lane] = acc;
+        __syncthreads();
+        if (wave == w && c < dim)
+            dw[(int64_t)key * dim + c] =
+                dev::from_f32<DT>((((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * scale);
+        __syncthreads();
     }
 }
 
@@ -404,7 +480,7 @@ int run_embed(const void* w, const int32_t* ids, void* y, int64_t n, int64_t voc
     typedef typename Elem<DT>::type T;
     // At most 2^30 work-items, which a dispatch counts in 32 bits.
     const int64_t gy = std::min<int64_t>(ceil_div(dim, 64 * Elem<DT>::VEC), 64);
-    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, 4), (1 << 22) / gy), (unsigned)gy);
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, 16), (1 << 22) / gy), (unsigned)gy);
     hipLaunchKernelGGL((embed_kernel<DT>), grid, dim3(256), 0, s, (const T*)w, ids, (T*)y, n, vocab, dim, scale);
     return launch_check("embed_kernel");
 }
@@ -442,10 +518,13 @@ int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64
             hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)(blocks + (p == 0 ? fill : 0))), dim3(SORT_THREADS), 0, s,
                                src, keys, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt, (char*)dw, dw_bytes);
             MLXHIP_TRY(launch_check("sort_count_kernel"));
-            hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS), dim3(64), 0, s, cnt, totals, (int)blocks);
-            MLXHIP_TRY(launch_check("sort_scan_kernel"));
+            if (blocks > SCAN_BLOCKS) {
+                hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS), dim3(64), 0, s, cnt, totals, (int)blocks);
+                MLXHIP_TRY(launch_check("sort_scan_kernel"));
+            }
             hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)blocks), dim3(SORT_THREADS), 0, s, src, keys,
-                               p == 0 ? nullptr : order, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt, totals, keys2,
+                               p == 0 ? nullptr : order, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt,
+                               blocks > SCAN_BLOCKS ? totals : nullptr, keys2,
                                order2);
             MLXHIP_TRY(launch_check("sort_move_kernel"));
             std::swap(keys, keys2);
@@ -458,7 +537,7 @@ int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64
                        scale, (T*)dw, part);
     MLXHIP_TRY(launch_check("embed_sum_kernel"));
     if (shares == 1) return MLXHIP_OK;
-    const dim3 jgrid((unsigned)ceil_div(shares, 4), (unsigned)std::min<int64_t>(ceil_div(dim, 64), 65535));
+    const dim3 jgrid((unsigned)ceil_div(shares, 4), (unsigned)ceil_div(dim, 64));
     hipLaunchKernelGGL((embed_join_kernel<DT>), jgrid, dim3(256), 0, s, keys, n, share, shares, dim, scale, (T*)dw, part);
     return launch_check("embed_join_kernel");
 }

@@ -72,7 +72,7 @@ __device__ inline void load_row(const typename Elem<DT>::type* p, int64_t cols, 
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int64_t c = (int64_t)(j * 64 * WPR + t) * VEC;
-        if (j < NV - 1) out[j] = *reinterpret_cast<const Vec16<DT>*>(p + c);
+        if (j < NV - 1) out[j].q = *reinterpret_cast<const dev::AnyVec<DT>*>(p + c);
         else out[j] = load_raw<DT>(p, c, cols);
     }
 }
@@ -146,10 +146,25 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
     float aw[EPL], ab[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) aw[i] = ab[i] = 0.0f;
-    for (int64_t r = (int64_t)blockIdx.x * RPB + sub; r < rows; r += (int64_t)gridDim.x * RPB) {
+    // The next row's loads are in flight while this one is reduced.
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r = (int64_t)blockIdx.x * RPB + sub;
+    Vec16<DT> xn[NV], gn[NV];
+    if (r < rows) {
+        load_row<DT, WPR, NV>(x + r * cols, cols, t, xn);
+        load_row<DT, WPR, NV>(dy + r * cols, cols, t, gn);
+    }
+    for (; r < rows; r += step) {
         Vec16<DT> xr[NV], gr[NV];
-        load_row<DT, WPR, NV>(x + r * cols, cols, t, xr);
-        load_row<DT, WPR, NV>(dy + r * cols, cols, t, gr);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            xr[j] = xn[j];
+            gr[j] = gn[j];
+        }
+        if (r + step < rows) {
+            load_row<DT, WPR, NV>(x + (r + step) * cols, cols, t, xn);
+            load_row<DT, WPR, NV>(dy + (r + step) * cols, cols, t, gn);
+        }
         float v[EPL], g[EPL], s1[1] = {0.0f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) unpack<DT>(xr[j], v + j * VEC);
@@ -217,25 +232,32 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
 }
 
 // Sums of n partial rows of 2 * cols values into dw and db: 32 columns of a
-// workgroup, 8 threads to each, which fold every eighth row and then each other.
+// workgroup, 32 threads to each, which fold every 32nd row (their loads all in
+// flight: a fold of 256 rows by 8 threads waited 9 us for 32 loads in turn) and
+// then each other.
+constexpr int FOLD = 32;
 template <int DT>
-__global__ __launch_bounds__(256) void affine_fold_kernel(const float* __restrict__ part, int64_t n, int64_t cols,
-                                                          typename Elem<DT>::type* __restrict__ dw,
-                                                          typename Elem<DT>::type* __restrict__ db) {
-    __shared__ float sums[8][32];
+__global__ __launch_bounds__(32 * FOLD) void affine_fold_kernel(const float* __restrict__ part, int64_t n, int64_t cols,
+                                                                typename Elem<DT>::type* __restrict__ dw,
+                                                                typename Elem<DT>::type* __restrict__ db) {
+    __shared__ float sums[FOLD][33];
     const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int64_t col = (int64_t)blockIdx.x * 32 + c;
     float s = 0.0f;
-    if (col < 2 * cols)
-        for (int64_t i = k; i < n; i += 8) s += part[i * 2 * cols + col];
+    if (col < 2 * cols) {
+#pragma unroll 8
+        for (int64_t i = k; i < n; i += FOLD) s += part[i * 2 * cols + col];
+    }
     sums[k][c] = s;
     __syncthreads();
-    if (k == 0 && col < 2 * cols) {
+    // Lane c of wave-half k now adds up column k's sums.
+    s = sums[c][k];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += sums[i][c];
-        if (col < cols) dw[col] = dev::from_f32<DT>(s);
-        else db[col - cols] = dev::from_f32<DT>(s);
-    }
+    for (int o = FOLD / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 32);
+    const int64_t to = (int64_t)blockIdx.x * 32 + k;
+    if (c || to >= 2 * cols) return;
+    if (to < cols) dw[to] = dev::from_f32<DT>(s);
+    else db[to - cols] = dev::from_f32<DT>(s);
 }
 
 // Longer rows: mean, rstd and, with dy, the means of g and g xh of a row per workgroup.
@@ -410,7 +432,7 @@ int run_affine(Args<DT> a) {
         MLXHIP_TRY((launch_waves<DT, 16>(a, groups)));
     }
     if (!a.grad) return MLXHIP_OK;
-    hipLaunchKernelGGL((affine_fold_kernel<DT>), dim3((unsigned)ceil_div(2 * a.cols, 32)), dim3(256), 0, a.s, a.part, groups,
+    hipLaunchKernelGGL((affine_fold_kernel<DT>), dim3((unsigned)ceil_div(2 * a.cols, 32)), dim3(32 * FOLD), 0, a.s, a.part, groups,
                        a.cols, a.dw, a.db);
     return launch_check("affine_fold_kernel");
 }
