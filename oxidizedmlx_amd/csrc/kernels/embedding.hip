@@ -29,8 +29,8 @@ namespace mlxhip {
 namespace {
 
 using dev::Elem;
-using dev::load_raw;
 using dev::store_vec;
+using dev::u32x4;
 using dev::unpack;
 using dev::Vec16;
 
@@ -43,33 +43,64 @@ constexpr int BLOCK_SORT = 2048;
 // Blocks whose counts the moving launch adds up itself.
 constexpr int SCAN_BLOCKS = 64;
 // Shares of the sorted list, about.
-constexpr int SHARES = 2048;
+constexpr int SHARES = 4096;
+
+// N elements of a row from column c on, N = VEC (16 bytes) or 1, at any element
+// alignment. A row's last N columns serve the lanes that would run past its end
+// (column_of): two lanes then hold some columns both, with the same values.
+template <int DT, int N>
+struct Piece {
+    std::conditional_t<N == 1, typename Elem<DT>::type, u32x4> q;
+};
+template <int DT, int N>
+__device__ inline Piece<DT, N> load_piece(const typename Elem<DT>::type* p) {
+    if constexpr (N == 1) return {*p};
+    else return {*reinterpret_cast<const dev::AnyVec<DT>*>(p)};
+}
+template <int DT, int N>
+__device__ inline void widen(const Piece<DT, N>& x, float (&v)[N]) {
+    if constexpr (N == 1) v[0] = dev::to_f32<DT>(x.q);
+    else unpack<DT>(Vec16<DT>{x.q}, v);
+}
+template <int DT, int N>
+__device__ inline void store_piece(typename Elem<DT>::type* p, const float (&v)[N]) {
+    if constexpr (N == 1) {
+        *p = dev::from_f32<DT>(v[0]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += Elem<DT>::VEC) store_vec<DT>(p + k, 0, Elem<DT>::VEC, v + k);
+    }
+}
+template <int N>
+__device__ inline int64_t column_of(int64_t unit, int64_t dim) {
+    return min(unit * N, dim - N);
+}
 
 // A wave copies ROWS rows at a time, all their loads in flight.
-template <int DT>
+template <int DT, int N>
 __global__ __launch_bounds__(256) void embed_kernel(const typename Elem<DT>::type* __restrict__ w,
                                                     const int32_t* __restrict__ ids,
                                                     typename Elem<DT>::type* __restrict__ y, int64_t n, int64_t vocab,
                                                     int64_t dim, float scale) {
-    constexpr int VEC = Elem<DT>::VEC, ROWS = 4;
+    constexpr int ROWS = 4;
     const int lane = threadIdx.x & 63;
     for (int64_t i = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS; i < n; i += (int64_t)gridDim.x * 4 * ROWS) {
         int64_t id[ROWS];
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) id[k] = min(max((int64_t)ids[min(i + k, n - 1)], (int64_t)0), vocab - 1);
-        for (int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC; c < dim; c += (int64_t)gridDim.y * 64 * VEC) {
-            Vec16<DT> raw[ROWS];
+        for (int64_t u = (int64_t)blockIdx.y * 64 + lane; u * N < dim; u += (int64_t)gridDim.y * 64) {
+            const int64_t c = column_of<N>(u, dim);
+            Piece<DT, N> raw[ROWS];
 #pragma unroll
-            for (int k = 0; k < ROWS; ++k)
-                if (i + k < n) raw[k] = load_raw<DT>(w + id[k] * dim, c, dim);
+            for (int k = 0; k < ROWS; ++k) raw[k] = load_piece<DT, N>(w + id[k] * dim + c);
 #pragma unroll
             for (int k = 0; k < ROWS; ++k) {
                 if (i + k >= n) break;
-                float v[VEC];
-                unpack<DT>(raw[k], v);
+                float v[N];
+                widen<DT, N>(raw[k], v);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] *= scale;
-                store_vec<DT>(y + (i + k) * dim, c, dim, v);
+                for (int e = 0; e < N; ++e) v[e] *= scale;
+                store_piece<DT, N>(y + (i + k) * dim + c, v);
             }
         }
     }
@@ -339,60 +370,60 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
     }
 }
 
-// A wave's share of the sorted positions and chunk of 64 * VEC columns. part
+// A wave's share of the sorted positions and chunk of 64 * N columns. part
 // holds two rows of dim sums per share: of the id that began before it, and
 // of the one that goes on after it (an id that does both: the first only).
 // The lanes hold 64 positions' keys and places, so the rows' addresses come
-// from registers and AHEAD of their loads are in flight.
-template <int DT>
+// from registers and AHEAD rows are loaded at once. A load that follows a store
+// waits for it too: shares of 32 rows in four such steps took 51-56 us for
+// 65536 bf16 rows of 1024, shares of 16 in one step
+template <int DT, int N>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                         const uint32_t* __restrict__ keys,
                                                         const uint32_t* __restrict__ order, int64_t n, int share,
                                                         int64_t shares, int64_t dim, float scale,
                                                         typename Elem<DT>::type* __restrict__ dw,
                                                         float* __restrict__ part) {
-    constexpr int VEC = Elem<DT>::VEC, AHEAD = 8;
+    constexpr int AHEAD = 16;
     const int lane = threadIdx.x & 63;
-    const int64_t sh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t sh = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
     if (sh >= shares) return;
-    const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * VEC;
-    const bool in = c < dim;  // every lane stays: its keys are the others' too
+    const int64_t unit = (int64_t)blockIdx.x * 64 + lane, c = column_of<N>(unit, dim);
+    const bool in = unit * N < dim;  // other lanes load what the last one does and store nothing
     const int64_t lo = sh * share, hi = min(n, lo + share);
-    float acc[VEC];
+    const typename Elem<DT>::type* from = dy + c;
+    float acc[N];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+    for (int e = 0; e < N; ++e) acc[e] = 0.0f;
     // The keys around the share, and its first one.
     const uint32_t before = lo > 0 ? keys[lo - 1] : 0, after = hi < n ? keys[hi] : 0;
-    uint32_t cur = keys[lo];
+    uint32_t cur = __builtin_amdgcn_readfirstlane(keys[lo]);
     bool head = lo > 0 && before == cur;
     auto leave = [&](float* to) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-            if (c + e < dim) to[c + e] = acc[e];
+        if (in) store_piece<MLXHIP_DTYPE_F32, N>(to + c, acc);
     };
     auto flush = [&] {
         if (head) {
             leave(part + 2 * sh * dim);
         } else if (in) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] *= scale;
-            store_vec<DT>(dw + (int64_t)cur * dim, c, dim, acc);
+            for (int e = 0; e < N; ++e) acc[e] *= scale;
+            store_piece<DT, N>(dw + (int64_t)cur * dim + c, acc);
         }
         head = false;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+        for (int e = 0; e < N; ++e) acc[e] = 0.0f;
     };
     for (int64_t i0 = lo; i0 < hi; i0 += 64) {
         const int count = (int)min(hi - i0, (int64_t)64);
         const int64_t mine = min(i0 + lane, hi - 1);
         const int key_l = (int)keys[mine], pos_l = (int)order[mine];
         for (int i = 0; i < count; i += AHEAD) {
-            Vec16<DT> raw[AHEAD];
+            Piece<DT, N> raw[AHEAD];
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const uint32_t pos = (uint32_t)__builtin_amdgcn_readlane(pos_l, min(i + a, count - 1));
-                if (in) raw[a] = load_raw<DT>(dy + (int64_t)pos * dim, c, dim);
-            }
+            for (int a = 0; a < AHEAD; ++a)
+                if (i + a < count)
+                    raw[a] = load_piece<DT, N>(from + (int64_t)(uint32_t)__builtin_amdgcn_readlane(pos_l, i + a) * dim);
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
                 if (i + a >= count) break;
@@ -401,12 +432,10 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>:
                     flush();
                     cur = key;
                 }
-                if (in) {
-                    float v[VEC];
-                    unpack<DT>(raw[a], v);
+                float v[N];
+                widen<DT, N>(raw[a], v);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) acc[e] += v[e];
-                }
+                for (int e = 0; e < N; ++e) acc[e] += v[e];
             }
         }
     }
@@ -474,25 +503,26 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t* __restr
     }
 }
 
-template <int DT>
+// Rows of at least 16 bytes in pieces of that size (N values), others one by one.
+template <int DT, int N>
 int run_embed(const void* w, const int32_t* ids, void* y, int64_t n, int64_t vocab, int64_t dim, float scale,
               hipStream_t s) {
     typedef typename Elem<DT>::type T;
     // At most 2^30 work-items, which a dispatch counts in 32 bits.
-    const int64_t gy = std::min<int64_t>(ceil_div(dim, 64 * Elem<DT>::VEC), 64);
+    const int64_t gy = std::min<int64_t>(ceil_div(dim, 64 * N), 64);
     const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, 16), (1 << 22) / gy), (unsigned)gy);
-    hipLaunchKernelGGL((embed_kernel<DT>), grid, dim3(256), 0, s, (const T*)w, ids, (T*)y, n, vocab, dim, scale);
+    hipLaunchKernelGGL((embed_kernel<DT, N>), grid, dim3(256), 0, s, (const T*)w, ids, (T*)y, n, vocab, dim, scale);
     return launch_check("embed_kernel");
 }
 
-template <int DT>
+template <int DT, int N>
 int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64_t vocab, int64_t dim, float scale,
                   hipStream_t s) {
     typedef typename Elem<DT>::type T;
     const int64_t dw_bytes = vocab * dim * (int64_t)sizeof(T);
     const int fill = (int)std::min<int64_t>(ceil_div(dw_bytes, 16 * SORT_THREADS), 512);
     const int64_t blocks = n <= LDS_SORT ? 0 : ceil_div(n, BLOCK_SORT);
-    // 2048 shares fill the compute units (8 waves each, times the chunks of
+    // 4096 shares fill the compute units (16 waves each, times the chunks of
     // columns) and leave a frequent id few partial sums to add up.
     const int share = (int)std::max<int64_t>(ceil_div(n, SHARES), 4);
     const int64_t shares = ceil_div(n, share);
@@ -532,8 +562,8 @@ int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64
         }
     }
     if (n == 0) return MLXHIP_OK;
-    const dim3 grid((unsigned)ceil_div(shares, 4), (unsigned)ceil_div(dim, 64 * Elem<DT>::VEC));
-    hipLaunchKernelGGL((embed_sum_kernel<DT>), grid, dim3(256), 0, s, (const T*)dy, keys, order, n, share, shares, dim,
+    const dim3 grid((unsigned)ceil_div(dim, 64 * N), (unsigned)ceil_div(shares, 4));
+    hipLaunchKernelGGL((embed_sum_kernel<DT, N>), grid, dim3(256), 0, s, (const T*)dy, keys, order, n, share, shares, dim,
                        scale, (T*)dw, part);
     MLXHIP_TRY(launch_check("embed_sum_kernel"));
     if (shares == 1) return MLXHIP_OK;
@@ -548,7 +578,11 @@ int embedding_rows(int dt, const void* w, const int32_t* ids, void* y, int64_t n
                    float scale, hipStream_t s) {
     if (n == 0 || dim == 0) return MLXHIP_OK;
     int rc = MLXHIP_OK;
-    if (!with_float_dtype(dt, [&](auto d) { rc = run_embed<d.value>(w, ids, y, n, vocab, dim, scale, s); }))
+    if (!with_float_dtype(dt, [&](auto d) {
+            constexpr int VEC = Elem<d.value>::VEC;
+            rc = dim < VEC ? run_embed<d.value, 1>(w, ids, y, n, vocab, dim, scale, s)
+                           : run_embed<d.value, VEC>(w, ids, y, n, vocab, dim, scale, s);
+        }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding: dtype %d (f32, bf16 or f16)", dt);
     return rc;
 }
@@ -557,7 +591,11 @@ int embedding_vjp_rows(int dt, const void* dy, const int32_t* ids, void* dw, int
                        float scale, hipStream_t s) {
     if (vocab == 0 || dim == 0) return MLXHIP_OK;
     int rc = MLXHIP_OK;
-    if (!with_float_dtype(dt, [&](auto d) { rc = run_embed_vjp<d.value>(dy, ids, dw, n, vocab, dim, scale, s); }))
+    if (!with_float_dtype(dt, [&](auto d) {
+            constexpr int VEC = Elem<d.value>::VEC;
+            rc = dim < VEC ? run_embed_vjp<d.value, 1>(dy, ids, dw, n, vocab, dim, scale, s)
+                           : run_embed_vjp<d.value, VEC>(dy, ids, dw, n, vocab, dim, scale, s);
+        }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding gradient: dtype %d (f32, bf16 or f16)", dt);
     return rc;
 }

@@ -84,18 +84,27 @@ def test_runs_across_every_share(n, kind):
 
 @pytest.mark.parametrize("n", [3000, 20000])
 def test_equal_ids_are_summed_in_the_order_of_their_positions(n):
-    """1, 2^-24 (n times): in order of the positions within a share of few
-    values nothing is added to 1, so a share that holds the 1 first sums to
-    exactly 1 + 0; any other order of that share gives another value. All
-    shares' sums are exact otherwise (multiples of 2^-24 under 2^-9)."""
+    """A 1 and then 2^-24 (half its last place) everywhere: in the order of the
+    positions the first share adds nothing to its 1, any other order does. The
+    shares' sums (exact but the first) are then joined in order too, in four
+    contiguous parts where there are more than 16 of them behind the first."""
     ids = np.zeros(n, np.int32)
     dy = np.full((n, 8), 2.0 ** -24, np.float32)
     dy[0] = 1.0
     got = gradient(dy, ids, 3, 1.0, abi.F32)
-    share = max(-(-n // 2048), 4)
-    acc = np.float32(1.0)
-    for lo in range(share, n, share):
-        acc = np.float32(acc + np.float32((min(n, lo + share) - lo) * 2.0 ** -24))
+    share = max(-(-n // 4096), 4)
+    sums = [np.float32((min(n, lo + share) - lo) * 2.0 ** -24) for lo in range(0, n, share)]
+    sums[0] = np.float32(1.0)
+    each = -(-(len(sums) - 1) // 4)
+    parts = []
+    for w in range(4):
+        acc = sums[0] if w == 0 else np.float32(0)
+        for v in sums[1 + w * each:1 + (w + 1) * each]:
+            acc = np.float32(acc + v)
+        parts.append(acc)
+    acc = parts[0]
+    for v in parts[1:]:
+        acc = np.float32(acc + v)
     np.testing.assert_array_equal(got[0], np.full(8, acc, np.float64))
     assert not got[1:].any()
 
