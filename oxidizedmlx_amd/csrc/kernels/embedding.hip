@@ -37,13 +37,13 @@ using dev::Vec16;
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr int BITS = 8, BINS = 1 << BITS;
 // Positions that one workgroup sorts in its LDS (key and position, 8 bytes
-// each: 128 KiB), and those of a workgroup's block in a longer sort.
-constexpr int LDS_SORT = 16384;
+// each: 64 KiB; 8192 take 29 us that way and 31 in blocks), and those of a workgroup's block in a longer sort.
+constexpr int LDS_SORT = 8192;
 constexpr int BLOCK_SORT = 2048;
 // Blocks whose counts the moving launch adds up itself.
 constexpr int SCAN_BLOCKS = 64;
 // Shares of the sorted list, about.
-constexpr int SHARES = 4096;
+constexpr int SHARES = 2048;
 
 // N elements of a row from column c on, N = VEC (16 bytes) or 1, at any element
 // alignment. A row's last N columns serve the lanes that would run past its end
@@ -106,8 +106,12 @@ __global__ __launch_bounds__(256) void embed_kernel(const typename Elem<DT>::typ
     }
 }
 
-// Zeros for `bytes` (a multiple of 2) from p, by workgroup b of nb.
-__device__ inline void zero_fill(char* p, int64_t bytes, int64_t b, int64_t nb) {
+// Zeros for part `part` of `parts` of the `bytes` (a multiple of 2) from p, by
+// workgroup b of nb.
+__device__ inline void zero_fill(char* p, int64_t bytes, int part, int parts, int64_t b, int64_t nb) {
+    const int64_t from = bytes / 2 * part / parts * 2, to = bytes / 2 * (part + 1) / parts * 2;
+    p += from;
+    bytes = to - from;
     const int64_t step = nb * SORT_THREADS;
     // The 16-byte words inside, and the bytes before and after them by pairs.
     const int64_t head = min((int64_t)(-reinterpret_cast<intptr_t>(p) & 15), bytes);
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const int32_t*
     constexpr int STEPS = LDS_SORT / SORT_THREADS;
     __shared__ uint32_t skey[LDS_SORT], spos[LDS_SORT], hist[BINS * SORT_WAVES], wave_sums[SORT_WAVES];
     if (blockIdx.x > 0) {
-        zero_fill(dw, dw_bytes, blockIdx.x - 1, gridDim.x - 1);
+        zero_fill(dw, dw_bytes, 0, 1, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -245,8 +249,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const int32_t*
 // One pass of a longer sort, in blocks of BLOCK_SORT positions: the blocks'
 // counts of each digit (counts[digit * blocks + block]), their scan along the
 // blocks (of few blocks: by the launch that follows), and the move to the places
-// that follow. The first pass reads the ids; its counting launch also zeroes dW
-// with the workgroups past the blocks.
+// that follow. The first pass reads the ids. Each of these launches also zeroes
+// its part of dW with the workgroups past the blocks.
 constexpr int BSTEPS = BLOCK_SORT / SORT_THREADS;
 
 __device__ inline void load_block(const int32_t* ids, const uint32_t* keys, int64_t n, uint32_t vocab, int64_t base,
@@ -263,10 +267,10 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const int32_t*
                                                                   const uint32_t* __restrict__ keys, int64_t n,
                                                                   uint32_t vocab, int shift, int blocks,
                                                                   uint32_t* __restrict__ counts, char* dw,
-                                                                  int64_t dw_bytes) {
+                                                                  int64_t dw_bytes, int part, int parts) {
     __shared__ uint32_t hist[BINS];
     if ((int)blockIdx.x >= blocks) {
-        zero_fill(dw, dw_bytes, blockIdx.x - blocks, gridDim.x - blocks);
+        zero_fill(dw, dw_bytes, part, parts, blockIdx.x - blocks, gridDim.x - blocks);
         return;
     }
     if (threadIdx.x < BINS) hist[threadIdx.x] = 0;
@@ -309,7 +313,12 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
                                                                  const uint32_t* __restrict__ counts,
                                                                  const uint32_t* __restrict__ totals,
                                                                  uint32_t* __restrict__ keys_out,
-                                                                 uint32_t* __restrict__ order_out) {
+                                                                 uint32_t* __restrict__ order_out, char* dw,
+                                                                 int64_t dw_bytes, int part, int parts) {
+    if ((int)blockIdx.x >= blocks) {
+        zero_fill(dw, dw_bytes, part, parts, blockIdx.x - blocks, gridDim.x - blocks);
+        return;
+    }
     __shared__ uint32_t hist[BINS * SORT_WAVES], wave_sums[SORT_WAVES], start[BINS], total[BINS], before[BINS];
     const int64_t base = (int64_t)blockIdx.x * BLOCK_SORT, left = min((int64_t)BLOCK_SORT, n - base);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -374,9 +383,10 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
 // holds two rows of dim sums per share: of the id that began before it, and
 // of the one that goes on after it (an id that does both: the first only).
 // The lanes hold 64 positions' keys and places, so the rows' addresses come
-// from registers and AHEAD rows are loaded at once. A load that follows a store
-// waits for it too: shares of 32 rows in four such steps took 51-56 us for
-// 65536 bf16 rows of 1024, shares of 16 in one step
+// from registers and AHEAD rows are loaded at once. 65536 bf16 rows of 1024 with
+// ids as frequent as words: 40 us for some 190 MB (rows read, sums and partial
+// sums written), 4.7 TB/s, whatever the length of the shares; the join then takes
+// 9 us for shares of 32 rows, 16 for 16 and 31 for 8.
 template <int DT, int N>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                         const uint32_t* __restrict__ keys,
@@ -522,7 +532,7 @@ int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64
     const int64_t dw_bytes = vocab * dim * (int64_t)sizeof(T);
     const int fill = (int)std::min<int64_t>(ceil_div(dw_bytes, 16 * SORT_THREADS), 512);
     const int64_t blocks = n <= LDS_SORT ? 0 : ceil_div(n, BLOCK_SORT);
-    // 4096 shares fill the compute units (16 waves each, times the chunks of
+    // 2048 shares fill the compute units (8 waves each, times the chunks of
     // columns) and leave a frequent id few partial sums to add up.
     const int share = (int)std::max<int64_t>(ceil_div(n, SHARES), 4);
     const int64_t shares = ceil_div(n, share);
@@ -545,17 +555,17 @@ int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64
         uint32_t* totals = cnt + BINS * blocks;
         for (int p = 0; p < passes; ++p) {
             const int32_t* src = p == 0 ? ids : nullptr;
-            hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)(blocks + (p == 0 ? fill : 0))), dim3(SORT_THREADS), 0, s,
-                               src, keys, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt, (char*)dw, dw_bytes);
+            hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)(blocks + fill)), dim3(SORT_THREADS), 0, s, src, keys, n,
+                               (uint32_t)vocab, BITS * p, (int)blocks, cnt, (char*)dw, dw_bytes, 2 * p, 2 * passes);
             MLXHIP_TRY(launch_check("sort_count_kernel"));
             if (blocks > SCAN_BLOCKS) {
                 hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS), dim3(64), 0, s, cnt, totals, (int)blocks);
                 MLXHIP_TRY(launch_check("sort_scan_kernel"));
             }
-            hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)blocks), dim3(SORT_THREADS), 0, s, src, keys,
+            hipLaunchKernelGGL(sort_move_kernel, dim3((unsigned)(blocks + fill)), dim3(SORT_THREADS), 0, s, src, keys,
                                p == 0 ? nullptr : order, n, (uint32_t)vocab, BITS * p, (int)blocks, cnt,
-                               blocks > SCAN_BLOCKS ? totals : nullptr, keys2,
-                               order2);
+                               blocks > SCAN_BLOCKS ? totals : nullptr, keys2, order2, (char*)dw, dw_bytes, 2 * p + 1,
+                               2 * passes);
             MLXHIP_TRY(launch_check("sort_move_kernel"));
             std::swap(keys, keys2);
             std::swap(order, order2);

@@ -92,7 +92,7 @@ def test_equal_ids_are_summed_in_the_order_of_their_positions(n):
     dy = np.full((n, 8), 2.0 ** -24, np.float32)
     dy[0] = 1.0
     got = gradient(dy, ids, 3, 1.0, abi.F32)
-    share = max(-(-n // 4096), 4)
+    share = max(-(-n // 2048), 4)
     sums = [np.float32((min(n, lo + share) - lo) * 2.0 ** -24) for lo in range(0, n, share)]
     sums[0] = np.float32(1.0)
     each = -(-(len(sums) - 1) // 4)
