@@ -56,6 +56,7 @@ SOURCES = [
     "kernels/ce_bf16.hip",
     "kernels/ce_f16.hip",
     "kernels/ce_f32.hip",
+    "kernels/ce_few.hip",
     "kernels/elementwise.hip",
     "kernels/gemm.hip",
     "kernels/gemm_small.hip",

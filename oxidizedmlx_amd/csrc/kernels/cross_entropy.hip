@@ -286,8 +286,68 @@ struct Op {
     }
 };
 
+int finish_loss(const float2* stats, int64_t tiles, const float* target_z, const int32_t* targets, int64_t rows,
+                int64_t vocab, float* loss, float* lse, hipStream_t s) {
+    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, stats, tiles, target_z, targets, rows,
+                       vocab, loss, lse);
+    return launch_check("loss_kernel");
+}
+
+// A few f32 rows: reading W as it is once a product beats copying it as planes.
+// 2048 .. 8 rows of 1024 over 32000, forward and backward, us (these / planes):
+ce::FewArgs few_args(const Op<MLXHIP_DTYPE_F32>& o) {
+    ce::FewArgs g;
+    g.x = o.x;
+    g.w = o.w;
+    g.rows = o.rows;
+    g.dim = o.dim;
+    g.vocab = o.vocab;
+    g.targets = o.targets;
+    return g;
+}
+
+int few_loss(const Op<MLXHIP_DTYPE_F32>& o, float* loss, float* lse) {
+    ce::FewArgs g = few_args(o);
+    g.stat_tiles = ceil_div(o.vocab, 64);
+    Carve c;
+    const size_t os = c.take((size_t)g.stat_tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4);
+    char* ws = nullptr;
+    MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
+    g.stats = (float2*)(ws + os);
+    g.target_z = (float*)(ws + oz);
+    MLXHIP_TRY(ce_few(ce::CE_STATS, g, o.s));
+    return finish_loss(g.stats, g.stat_tiles, g.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
+}
+
+int few_grad(const Op<MLXHIP_DTYPE_F32>& o, const float* lse, const float* dloss, float* dx, float* dw) {
+    ce::FewArgs g = few_args(o);
+    g.lse = lse;
+    g.dloss = dloss;
+    g.dw = dw;
+    // Eight waves to a compute unit, four of a workgroup along the vocabulary.
+    g.ldx = ceil_div(o.dim, 4) * 4;
+    const int64_t most = std::max<int64_t>(512 / ceil_div(o.dim, 64), 1);
+    g.slice = ceil_div(ceil_div(o.vocab, 4 * most), 16) * 16;
+    g.slices = ceil_div(o.vocab, 4 * g.slice);
+    Carve c;
+    const size_t od = c.take((size_t)o.vocab * ce::few_ds_rows(o.rows) * 4),
+                 ox = c.take(dx ? (size_t)g.slices * o.rows * g.ldx * 4 : 0);
+    char* ws = nullptr;
+    MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
+    g.ds = (float*)(ws + od);
+    g.dx = dx ? (float*)(ws + ox) : nullptr;
+    MLXHIP_TRY(ce_few(ce::CE_DS, g, o.s));
+    MLXHIP_TRY(ce_few(ce::CE_DX, g, o.s));
+    if (!dx) return MLXHIP_OK;
+    hipLaunchKernelGGL((dx_kernel<MLXHIP_DTYPE_F32>), dim3(grid_for(o.rows * g.ldx / 4)), dim3(256), 0, o.s, g.dx,
+                       (int)g.slices, o.rows, o.dim, g.ldx, o.targets, o.vocab, nullptr, dx);
+    return launch_check("dx_kernel");
+}
+
 template <int OT>
 int run_loss(const Op<OT>& o, float* loss, float* lse) {
+    if constexpr (OT == MLXHIP_DTYPE_F32)
+        if (o.rows <= ce::FEW_ROWS) return few_loss(o, loss, lse);
     const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
     const int64_t width = o.width(false, copy_w);
     // One tile size for all pieces, whose widths are multiples of its columns.
@@ -329,9 +389,7 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
         if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, scale + ce::SCALE_W, (uint16_t*)(ws + ow)));
         MLXHIP_TRY(o.product(ce::CE_STATS, large, a));
     }
-    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(o.rows, 4)), dim3(256), 0, o.s, (const float2*)(ws + os), tiles,
-                       (const float*)(ws + oz), o.targets, o.rows, o.vocab, loss, lse);
-    return launch_check("loss_kernel");
+    return finish_loss((const float2*)(ws + os), tiles, a.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
 }
 
 template <int OT>
@@ -344,6 +402,8 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         hipLaunchKernelGGL((zero_kernel<T>), dim3(grid_for(o.vocab * o.dim)), dim3(256), 0, o.s, dw, o.vocab * o.dim);
         return launch_check("zero_kernel");
     }
+    if constexpr (OT == MLXHIP_DTYPE_F32)
+        if (o.rows <= ce::FEW_ROWS) return few_grad(o, lse, dloss, dx, dw);
     const bool copy_w = !o.in_place(o.w);
     const int64_t width = o.width(true, copy_w), ld = ceil_div(width, 256) * 256, dim_p = o.dim_p();
     // dx: few tiles, so K is cut into slices until every compute unit has one
