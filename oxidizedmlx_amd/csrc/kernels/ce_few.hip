@@ -1,9 +1,9 @@
-// ce_few.hip — the linear cross entropy of a few f32 rows (up to 64), which
-// reading W (and writing dW) bounds: W goes from memory straight into the f32
+// ce_few.hip — the linear cross entropy of a few f32 rows (the loss of up to 64,
+// the gradients of up to 32), which reading W (and writing dW) bounds: W goes from memory straight into the f32
 // matrix instructions, with no copies and no planes.
 //
-//   stats: z = x W^T, a wave per 16 entries of the vocabulary; the row maxima and
-//          sums of a workgroup's 64 entries, and the targets' logits.
+//   stats: z = x W^T, a wave per 16 or 32 entries of the vocabulary; the row maxima
+//          and sums of a workgroup's entries, and the targets' logits.
 //   ds:    z again, kept as dS^T [vocab][16 NB] (zeros behind the rows).
 //   grad:  a wave per 64 columns and slice of the vocabulary: dW = dS^T x of 16
 //          entries at a time, and its sums of dx = dS W.
@@ -14,8 +14,11 @@
 // permutation of the sum, along the columns of W and x one of the columns, which
 // the stores undo.
 //
-// 8 rows of 1024 over 32000 entries: forward 131 MB of W, floor 27 us; backward
-// W twice and dW once.
+// Measured over 32000 entries of 1024: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds), 49
+// (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69; 64 rows 58 for stats. On
+// two f16 planes each (ce_gemm.hpp), whose copies read W twice and write it once
+// before, 1 to 64 rows take 107 - 113 us forward and 157 - 182 backward; the
+// gradients of 64 rows took 191 here, bound by the f32 matrix instructions.
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "ce_gemm.hpp"
@@ -31,66 +34,102 @@ constexpr int F = MLXHIP_DTYPE_F32;
 
 __device__ inline f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// z[v][r] of the wave's 16 entries from v0 on and NB tiles of 16 rows.
+// Tiles of 16 entries of a wave: with more rows two, so that a load of x serves
+// twice (64 rows of 1024 over 32000: 82 us with one).
 template <int NB>
-__device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 (&acc)[NB]) {
+constexpr int TILES = NB == 1 ? 1 : 2;
+template <int NB>
+constexpr int ENTRIES = 64 * TILES<NB>;  // of a workgroup
+
+// z[v][r] of the wave's TILES * 16 entries from v0 on and NB tiles of 16 rows. KB
+// blocks of 16 along K are loaded at once.
+template <int NB>
+__device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 (&acc)[TILES<NB>][NB]) {
+    constexpr int KB = NB == 1 ? 6 : NB == 2 ? 4 : 3, T = TILES<NB>;
     const int i = lane & 15, q = lane >> 4;
-    const float* w = g.w + min(v0 + i, g.vocab - 1) * g.dim;
-    const float* x[NB];
+    const float *w[T], *x[NB];
+#pragma unroll
+    for (int t = 0; t < T; ++t) w[t] = g.w + min(v0 + 16 * t + i, g.vocab - 1) * g.dim + 4 * q;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        x[b] = g.x + min((int64_t)(16 * b + i), g.rows - 1) * g.dim;
-        acc[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    const int64_t whole = g.dim / 16 * 16;
-#pragma unroll 8
-    for (int64_t k = 0; k < whole; k += 16) {
-        float a[4], c[NB][4];
-        dev::unpack<F>(dev::Vec16<F>{*reinterpret_cast<const dev::AnyVec<F>*>(w + k + 4 * q)}, a);
+        x[b] = g.x + min((int64_t)(16 * b + i), g.rows - 1) * g.dim + 4 * q;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-            dev::unpack<F>(dev::Vec16<F>{*reinterpret_cast<const dev::AnyVec<F>*>(x[b] + k + 4 * q)}, c[b]);
+        for (int t = 0; t < T; ++t) acc[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    typedef dev::AnyVec<F> any;
+    auto step = [&](const dev::u32x4 (&a)[T], const dev::u32x4 (&c)[NB]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) acc[b] = mfma4(a[e], c[b][e], acc[b]);
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+                    acc[t][b] = mfma4(__uint_as_float(a[t][e]), __uint_as_float(c[b][e]), acc[t][b]);
+    };
+    // Two batches of loads in turn: one on its way while the other is used.
+    dev::u32x4 a[2][KB][T], c[2][KB][NB];
+    auto fetch = [&](int64_t k, dev::u32x4 (&fa)[KB][T], dev::u32x4 (&fc)[KB][NB]) {
+#pragma unroll
+        for (int s = 0; s < KB; ++s)
+#pragma unroll
+            for (int t = 0; t < T; ++t) fa[s][t] = *reinterpret_cast<const any*>(w[t] + k + 16 * s);
+#pragma unroll
+        for (int s = 0; s < KB; ++s)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) fc[s][b] = *reinterpret_cast<const any*>(x[b] + k + 16 * s);
+    };
+    const int64_t batches = g.dim / (16 * KB);
+    if (batches) fetch(0, a[0], c[0]);
+    for (int64_t n = 0; n < batches; n += 2) {
+        if (n + 1 < batches) fetch((n + 1) * 16 * KB, a[1], c[1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < KB; ++s) step(a[0][s], c[0][s]);
+        if (n + 1 == batches) break;
+        if (n + 2 < batches) fetch((n + 2) * 16 * KB, a[0], c[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < KB; ++s) step(a[1][s], c[1][s]);
     }
-    if (whole < g.dim) {
-        float a[4], c[NB][4];
-        dev::unpack<F>(dev::load_raw<F>(w, whole + 4 * q, g.dim), a);
+    for (int64_t k = batches * 16 * KB; k < g.dim; k += 16) {
+        dev::u32x4 ta[T], tc[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) dev::unpack<F>(dev::load_raw<F>(x[b], whole + 4 * q, g.dim), c[b]);
+        for (int t = 0; t < T; ++t) ta[t] = dev::load_raw<F>(w[t], k, g.dim - 4 * q).q;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) acc[b] = mfma4(a[e], c[b][e], acc[b]);
+        for (int b = 0; b < NB; ++b) tc[b] = dev::load_raw<F>(x[b], k, g.dim - 4 * q).q;
+        step(ta, tc);
     }
 }
 
 template <int NB>
 __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
+    constexpr int T = TILES<NB>;
     __shared__ float red[4][2][16 * NB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-    const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 16;
-    f32x4 acc[NB];
+    const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 16 * T;
+    f32x4 acc[T][NB];
     if (v0 < g.vocab) few_logits<NB>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = 16 * b + i;
         float m = -INFINITY, s = 0.0f;
         if (v0 < g.vocab) {
-            const int64_t t = r < g.rows ? g.targets[r] - (v0 + 4 * q) : -1;
+            const int64_t target = r < g.rows ? g.targets[r] : -1;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool in = v0 + 4 * q + e < g.vocab;
-                if (in && t == e) g.target_z[r] = acc[b][e];
-                // fmaxf would drop a NaN; the sum below keeps it.
-                if (in) m = fmaxf(m, acc[b][e]);
-            }
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t v = v0 + 16 * t + 4 * q + e;
+                    if (v < g.vocab && v == target) g.target_z[r] = acc[t][b][e];
+                    // fmaxf drops a NaN; the sum below keeps it.
+                    if (v < g.vocab) m = fmaxf(m, acc[t][b][e]);
+                }
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (v0 + 4 * q + e < g.vocab) s += __builtin_amdgcn_exp2f((acc[b][e] - base) * LOG2E);
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (v0 + 16 * t + 4 * q + e < g.vocab) s += __builtin_amdgcn_exp2f((acc[t][b][e] - base) * LOG2E);
         }
         merge(m, s, __shfl_xor(m, 16, 64), __shfl_xor(s, 16, 64));
         merge(m, s, __shfl_xor(m, 32, 64), __shfl_xor(s, 32, 64));
@@ -110,22 +149,26 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
 
 template <int NB>
 __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
+    constexpr int T = TILES<NB>;
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
-    const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16;
+    const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * T;
     if (v0 >= g.vocab) return;
-    f32x4 acc[NB];
+    f32x4 acc[T][NB];
     few_logits<NB>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = 16 * b + i;
-        const bool on = r < g.rows && counted(g.targets[r], g.vocab);
+        const int64_t target = r < g.rows ? g.targets[r] : -1;
+        const bool on = target >= 0 && target < g.vocab;
         const float lse = on ? g.lse[r] : 0.0f, f = on ? g.dloss[r] : 0.0f;
-        const int64_t t = on ? g.targets[r] - (v0 + 4 * q) : -1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f((acc[b][e] - lse) * LOG2E) - (t == e ? 1.0f : 0.0f);
-            if (v0 + 4 * q + e < g.vocab) g.ds[(v0 + 4 * q + e) * (16 * NB) + r] = on ? p * f : 0.0f;
-        }
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t v = v0 + 16 * t + 4 * q + e;
+                const float p = __builtin_amdgcn_exp2f((acc[t][b][e] - lse) * LOG2E) - (v == target ? 1.0f : 0.0f);
+                if (v < g.vocab) g.ds[v * (16 * NB) + r] = on ? p * f : 0.0f;
+            }
     }
 }
 
@@ -210,16 +253,15 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
 }
 
 template <int NB>
-int few(int which, const FewArgs& g, hipStream_t s) {
-    const dim3 entries((unsigned)ceil_div(g.vocab, 64));
-    if (which == CE_STATS) {
-        hipLaunchKernelGGL((few_stats_kernel<NB>), entries, dim3(256), 0, s, g);
-        return launch_check("few_stats_kernel");
-    }
-    if (which == CE_DS) {
-        hipLaunchKernelGGL((few_ds_kernel<NB>), entries, dim3(256), 0, s, g);
-        return launch_check("few_ds_kernel");
-    }
+int few_loss(const FewArgs& g, hipStream_t s) {
+    hipLaunchKernelGGL((few_stats_kernel<NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
+    return launch_check("few_stats_kernel");
+}
+
+template <int NB>
+int few_grad(const FewArgs& g, hipStream_t s) {
+    hipLaunchKernelGGL((few_ds_kernel<NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
+    MLXHIP_TRY(launch_check("few_ds_kernel"));
     hipLaunchKernelGGL((few_grad_kernel<NB>), dim3((unsigned)ceil_div(g.dim, 64), (unsigned)g.slices), dim3(256), 0, s, g);
     return launch_check("few_grad_kernel");
 }
@@ -227,10 +269,17 @@ int few(int which, const FewArgs& g, hipStream_t s) {
 }  // namespace
 }  // namespace ce
 
-int ce_few(int which, const ce::FewArgs& g, hipStream_t s) {
-    if (g.rows <= 16) return ce::few<1>(which, g, s);
-    if (g.rows <= 32) return ce::few<2>(which, g, s);
-    return ce::few<4>(which, g, s);
+int64_t ce_few_tiles(int64_t rows, int64_t vocab) {
+    return ceil_div(vocab, rows <= 16 ? ce::ENTRIES<1> : rows <= 32 ? ce::ENTRIES<2> : ce::ENTRIES<4>);
+}
+
+int ce_few_loss(const ce::FewArgs& g, hipStream_t s) {
+    if (g.rows <= 16) return ce::few_loss<1>(g, s);
+    return g.rows <= 32 ? ce::few_loss<2>(g, s) : ce::few_loss<4>(g, s);
+}
+
+int ce_few_grad(const ce::FewArgs& g, hipStream_t s) {
+    return g.rows <= 16 ? ce::few_grad<1>(g, s) : ce::few_grad<2>(g, s);
 }
 
 }  // namespace mlxhip

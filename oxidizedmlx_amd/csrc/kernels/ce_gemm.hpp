@@ -102,22 +102,23 @@ struct Args {
     int64_t ldc = 0;
 };
 
-// Up to FEW_ROWS f32 rows (ce_few.hip).
-constexpr int FEW_ROWS = 64;
+// Few f32 rows (ce_few.hip): the loss of up to FEW_LOSS, the gradients of up to
+// FEW_GRAD.
+constexpr int FEW_LOSS = 64, FEW_GRAD = 32;
 struct FewArgs {
     const float *x = nullptr, *w = nullptr;
     int64_t rows = 0, dim = 0, vocab = 0;
     const int32_t* targets = nullptr;
     const float *lse = nullptr, *dloss = nullptr;
-    float2* stats = nullptr;    // CE_STATS: [rows][stat_tiles], a tile per 64 entries
+    float2* stats = nullptr;    // CE_STATS: [rows][stat_tiles]
     int64_t stat_tiles = 0;
     float* target_z = nullptr;
     float* ds = nullptr;        // dS^T [vocab][few_ds_rows(rows)]
-    float* dx = nullptr;        // CE_DX: [slices][rows][ldx] or null
+    float* dx = nullptr;        // [slices][rows][ldx] or null
     float* dw = nullptr;        // [vocab][dim] or null
     int64_t ldx = 0, slices = 0, slice = 0;  // of 4 * slice entries each; slice a multiple of 16
 };
-inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
 // Max and sum of exp(z - max) of two groups of a row.
 __device__ inline void merge(float& m, float& s, float m2, float s2) {
@@ -567,7 +568,9 @@ constexpr int large_bn() { return Large<P>::BN; }
 int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f32(int which, bool large, const ce::Args& a, hipStream_t s);
-// ce_few.hip: which = CE_STATS, CE_DS, or CE_DX for both gradients from dS.
-int ce_few(int which, const ce::FewArgs& g, hipStream_t s);
+// ce_few.hip
+int ce_few_loss(const ce::FewArgs& g, hipStream_t s);
+int ce_few_grad(const ce::FewArgs& g, hipStream_t s);
+int64_t ce_few_tiles(int64_t rows, int64_t vocab);  // of the loss's statistics
 
 }  // namespace mlxhip

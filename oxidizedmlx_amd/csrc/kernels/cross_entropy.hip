@@ -293,8 +293,8 @@ int finish_loss(const float2* stats, int64_t tiles, const float* target_z, const
     return launch_check("loss_kernel");
 }
 
-// A few f32 rows: reading W as it is once a product beats copying it as planes.
-// 2048 .. 8 rows of 1024 over 32000, forward and backward, us (these / planes):
+// Few f32 rows: reading W as it is in each product beats copying it as planes
+// (measured in ce_few.hip).
 ce::FewArgs few_args(const Op<MLXHIP_DTYPE_F32>& o) {
     ce::FewArgs g;
     g.x = o.x;
@@ -308,14 +308,14 @@ ce::FewArgs few_args(const Op<MLXHIP_DTYPE_F32>& o) {
 
 int few_loss(const Op<MLXHIP_DTYPE_F32>& o, float* loss, float* lse) {
     ce::FewArgs g = few_args(o);
-    g.stat_tiles = ceil_div(o.vocab, 64);
+    g.stat_tiles = ce_few_tiles(o.rows, o.vocab);
     Carve c;
     const size_t os = c.take((size_t)g.stat_tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     g.stats = (float2*)(ws + os);
     g.target_z = (float*)(ws + oz);
-    MLXHIP_TRY(ce_few(ce::CE_STATS, g, o.s));
+    MLXHIP_TRY(ce_few_loss(g, o.s));
     return finish_loss(g.stats, g.stat_tiles, g.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
 }
 
@@ -336,8 +336,7 @@ int few_grad(const Op<MLXHIP_DTYPE_F32>& o, const float* lse, const float* dloss
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     g.ds = (float*)(ws + od);
     g.dx = dx ? (float*)(ws + ox) : nullptr;
-    MLXHIP_TRY(ce_few(ce::CE_DS, g, o.s));
-    MLXHIP_TRY(ce_few(ce::CE_DX, g, o.s));
+    MLXHIP_TRY(ce_few_grad(g, o.s));
     if (!dx) return MLXHIP_OK;
     hipLaunchKernelGGL((dx_kernel<MLXHIP_DTYPE_F32>), dim3(grid_for(o.rows * g.ldx / 4)), dim3(256), 0, o.s, g.dx,
                        (int)g.slices, o.rows, o.dim, g.ldx, o.targets, o.vocab, nullptr, dx);
@@ -347,7 +346,7 @@ int few_grad(const Op<MLXHIP_DTYPE_F32>& o, const float* lse, const float* dloss
 template <int OT>
 int run_loss(const Op<OT>& o, float* loss, float* lse) {
     if constexpr (OT == MLXHIP_DTYPE_F32)
-        if (o.rows <= ce::FEW_ROWS) return few_loss(o, loss, lse);
+        if (o.rows <= ce::FEW_LOSS) return few_loss(o, loss, lse);
     const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
     const int64_t width = o.width(false, copy_w);
     // One tile size for all pieces, whose widths are multiples of its columns.
@@ -403,7 +402,7 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         return launch_check("zero_kernel");
     }
     if constexpr (OT == MLXHIP_DTYPE_F32)
-        if (o.rows <= ce::FEW_ROWS) return few_grad(o, lse, dloss, dx, dw);
+        if (o.rows <= ce::FEW_GRAD) return few_grad(o, lse, dloss, dx, dw);
     const bool copy_w = !o.in_place(o.w);
     const int64_t width = o.width(true, copy_w), ld = ceil_div(width, 256) * 256, dim_p = o.dim_p();
     // dx: few tiles, so K is cut into slices until every compute unit has one
