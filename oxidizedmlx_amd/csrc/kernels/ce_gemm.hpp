@@ -60,7 +60,8 @@ using Large = std::conditional_t<P == 1, Cfg<2, 4, 4, 2, 4, 1>, Cfg<4, 2, 2, 2, 
 template <int P>
 using Small = std::conditional_t<P == 1, Cfg<2, 2, 2, 2, 4, 1>, Cfg<2, 4, 2, 1, 4, 2>>;  // 128 x 128, two to a CU / one
 
-// Factors of the products' operands and results, all powers of two.
+// Factors of the products' operands and results; those of planes are powers of
+// two.
 enum Scale {
     SCALE_DW = 0,  // dW is this times dS^T x
     SCALE_DS = 1,  // dS is formed from dloss times this
@@ -97,7 +98,7 @@ struct Args {
     float* dx = nullptr;        // CE_DX: [splits][m][ldc]
     bool add = false;           // CE_DX: add to what is there
     void* dw = nullptr;         // CE_DW: [m][ldc]
-    const float* scale = nullptr;  // Scale's factors; null: all 1
+    const float* scale = nullptr;  // Scale's factors (not for CE_STATS of 16-bit operands, CE_DX)
     const float* row_scale = nullptr;  // CE_STATS of planes: x is row_scale[r] times its planes
     int64_t ldc = 0;
 };
@@ -452,7 +453,7 @@ void ce_gemm_kernel(Args g) {
                 g.stats[(m0 + tid) * g.stat_tiles + n0 / C::BN] = a;
             }
         } else if constexpr (PRODUCT == CE_DS) {
-            const float up = g.scale ? g.scale[SCALE_DS] : 1.0f, zs = P == 1 ? LOG2E : LOG2E * g.scale[SCALE_Z];
+            const float up = g.scale[SCALE_DS], zs = P == 1 ? LOG2E : LOG2E * g.scale[SCALE_Z];
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 const int64_t r = row0 + 32 * i;
@@ -507,15 +508,13 @@ void ce_gemm_kernel(Args g) {
             }
         } else {
             if constexpr (PRODUCT == CE_DW) {
-                if (g.scale) {
-                    const float f = g.scale[SCALE_DW];
+                const float f = g.scale[SCALE_DW];
 #pragma unroll
-                    for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int j = 0; j < TN; ++j)
+                    for (int j = 0; j < TN; ++j)
 #pragma unroll
-                            for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
-                }
+                        for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
                 store_tile<OT, C, false, true>(acc, region, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m, g.n, g.n,
                                                wrow, wcol, lane, false);
             } else {

@@ -67,16 +67,85 @@ __device__ inline void pack8(const typename Elem<OT>::type* src, int64_t c, int6
     }
 }
 
+// Largest m of a workgroup of 1024 threads.
+__device__ inline float block_max(float m, float* waves) {
+    m = dev::wave_max(m);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, waves[i]);
+    __syncthreads();
+    return m;
+}
+
+// The factors of ce::Scale, by one workgroup of 1024 threads; part: the maxima
+// of f32 operands (maxima_kernel), null for the others.
+//
+// dS is formed from dloss times a factor that brings its largest magnitude to
+// 2^15, so that the smallest probabilities in use stay normal f16 numbers. For
+// 16-bit operands the factor is that exactly: where all rows weigh the same, as
+// in a mean, the -1 of a target is then a power of two, and its rounding, which
+// would be one relative error of the whole gradient (0.4 % for 1/7 in bf16), is
+// none. Planes of f32 operands, whose dS has 22 bits, and the factor of their dS
+// are scaled by powers of two to between 2^14 and 2^15.
+constexpr int MAXIMA = 1024;
+__device__ inline void write_scales(const float* part, const float* dloss, const int32_t* targets, int64_t rows,
+                                    int64_t vocab, float* scale) {
+    __shared__ float waves[16];
+    int ew = 15, ex = 15;
+    float up = 1.0f, down = 1.0f;
+    if (part) ew = exponent(block_max(part[threadIdx.x], waves));
+    if (dloss) {
+        float m = 0.0f;
+#pragma unroll 4
+        for (int64_t r = threadIdx.x; r < rows; r += 1024)
+            if (counted(targets[r], vocab)) m = fmaxf(m, finite_abs(dloss[r]));
+        m = block_max(m, waves);
+        if (part) {
+            ex = exponent(block_max(part[MAXIMA + threadIdx.x], waves));
+            m = ldexpf(1.0f, exponent(m));
+        }
+        if (m > 0.0f) {
+            m = fmaxf(m, 0x1p-100f);  // 2^15 / m and its inverse stay in range
+            up = 0x1p15f / m;
+            down = m * 0x1p-15f;
+        }
+    }
+    if (threadIdx.x) return;
+    scale[ce::SCALE_DW] = ldexpf(down, ex - 15);
+    scale[ce::SCALE_DS] = up;
+    scale[ce::SCALE_Z] = ldexpf(1.0f, ex + ew - 30);
+    scale[ce::SCALE_DX] = ldexpf(down, ew - 15);
+    scale[ce::SCALE_X] = ldexpf(1.0f, 15 - ex);
+    scale[ce::SCALE_W] = ldexpf(1.0f, 15 - ew);
+}
+
+__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ part, const float* __restrict__ dloss,
+                                                     const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
+                                                     float* __restrict__ scale) {
+    write_scales(part, dloss, targets, rows, vocab, scale);
+}
+
 // src [rows][dim] as planes of [rows][dim_p] (zeros past dim, and in the rows
-// without a target where targets are given), 8 columns a thread.
+// without a target where targets are given), 8 columns a thread. With `dloss`,
+// workgroup 0 writes the factors of 16-bit operands instead.
 template <int OT, int P>
-__global__ __launch_bounds__(256) void pack_kernel(const typename Elem<OT>::type* __restrict__ src, int64_t rows,
-                                                   int64_t dim, int64_t dim_p, const int32_t* __restrict__ targets,
-                                                   int64_t vocab, const float* __restrict__ scale,
-                                                   uint16_t* __restrict__ dst) {
+__global__ __launch_bounds__(1024) void pack_kernel(const typename Elem<OT>::type* __restrict__ src, int64_t rows,
+                                                    int64_t dim, int64_t dim_p, const int32_t* __restrict__ targets,
+                                                    int64_t vocab, const float* __restrict__ factor,
+                                                    uint16_t* __restrict__ dst, const float* __restrict__ dloss,
+                                                    float* __restrict__ scale) {
     const int64_t chunks = dim_p / 8, plane = rows * dim_p;
-    const float f = P == 1 ? 1.0f : *scale;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 256) {
+    const float f = P == 1 ? 1.0f : *factor;
+    int64_t block = blockIdx.x, blocks = gridDim.x;
+    if (P == 1 && dloss) {
+        if (block == 0) {
+            write_scales(nullptr, dloss, targets, rows, vocab, scale);
+            return;
+        }
+        --block;
+        --blocks;
+    }
+    for (int64_t i = block * 1024 + threadIdx.x; i < rows * chunks; i += blocks * 1024) {
         const int64_t r = i / chunks, c = (i - r * chunks) * 8;
         pack8<OT, P>(src + r * dim, c, dim, !targets || counted(targets[r], vocab), f, dst + r * dim_p, plane);
     }
@@ -102,7 +171,6 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict_
 
 // Largest finite magnitudes, one of each workgroup: of W in part[0..MAXIMA), of
 // the rows of x with a target in part[MAXIMA..2 MAXIMA) (blockIdx.y = 1).
-constexpr int MAXIMA = 1024;
 __global__ __launch_bounds__(256) void maxima_kernel(const float* __restrict__ w, int64_t nw, const float* __restrict__ x,
                                                      int64_t dim, int64_t nx, const int32_t* __restrict__ targets,
                                                      int64_t vocab, float* __restrict__ part) {
@@ -124,41 +192,6 @@ __global__ __launch_bounds__(256) void maxima_kernel(const float* __restrict__ w
     __syncthreads();
     if (threadIdx.x == 0)
         part[blockIdx.y * MAXIMA + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
-}
-
-__device__ inline float block_max(float m, float* waves) {
-    m = dev::wave_max(m);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, waves[i]);
-    __syncthreads();
-    return m;
-}
-
-// The factors of ce::Scale, by one workgroup. Planes of W and x (part given, x
-// in the backward pass) and, in it, dS (f16 and f32) are scaled so that the
-// largest magnitude lies between 2^14 and 2^15: small probabilities then stay
-// normal f16 numbers.
-__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ part, const float* __restrict__ dloss,
-                                                     const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
-                                                     float* __restrict__ scale) {
-    __shared__ float waves[16];
-    int ew = 15, ex = 15, eg = 15;
-    if (part) ew = exponent(block_max(part[threadIdx.x], waves));
-    if (dloss) {
-        float m = 0.0f;
-        for (int64_t r = threadIdx.x; r < rows; r += 1024)
-            if (counted(targets[r], vocab)) m = fmaxf(m, finite_abs(dloss[r]));
-        eg = exponent(block_max(m, waves));
-        if (part) ex = exponent(block_max(part[MAXIMA + threadIdx.x], waves));
-    }
-    if (threadIdx.x) return;
-    scale[ce::SCALE_DW] = ldexpf(1.0f, eg + ex - 30);
-    scale[ce::SCALE_DS] = ldexpf(1.0f, 15 - eg);
-    scale[ce::SCALE_Z] = ldexpf(1.0f, ex + ew - 30);
-    scale[ce::SCALE_DX] = ldexpf(1.0f, eg + ew - 30);
-    scale[ce::SCALE_X] = ldexpf(1.0f, 15 - ex);
-    scale[ce::SCALE_W] = ldexpf(1.0f, 15 - ew);
 }
 
 // A row's maxima and sums over the tiles joined, a wave to each row.
@@ -249,20 +282,20 @@ struct Op {
     // Whether a matrix of rows of dim is read as it is.
     bool in_place(const T* p) const { return P == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
     size_t packed(int64_t n) const { return (size_t)n * dim_p() * P * 2; }
-    int pack(const T* src, int64_t n, const int32_t* t, const float* scale, uint16_t* dst) const {
-        hipLaunchKernelGGL((pack_kernel<OT, P>), dim3(grid_for(n * dim_p() / 8)), dim3(256), 0, s, src, n, dim, dim_p(), t,
-                           vocab, scale, dst);
+    // factor: what planes hold their values times; with dloss (16-bit operands,
+    // x's rows) also the factors into scale.
+    int pack(const T* src, int64_t n, const int32_t* t, const float* factor, uint16_t* dst, const float* dloss = nullptr,
+             float* scale = nullptr) const {
+        const int64_t groups = std::min<int64_t>(ceil_div(n * dim_p() / 8, 1024), 2048) + (dloss ? 1 : 0);
+        hipLaunchKernelGGL((pack_kernel<OT, P>), dim3((unsigned)groups), dim3(1024), 0, s, src, n, dim, dim_p(), t, vocab,
+                           factor, dst, dloss, scale);
         return launch_check("pack_kernel");
     }
-    // The factors into scale (part: room for the maxima of f32 operands).
+    // The factors of f32 operands into scale (part: room for the maxima).
     int scales(const float* dloss, float* part, float* scale) const {
-        if constexpr (P > 1) {
-            hipLaunchKernelGGL(maxima_kernel, dim3(MAXIMA, dloss ? 2 : 1), dim3(256), 0, s, w, vocab * dim, x, dim, rows * dim,
-                               targets, vocab, part);
-            MLXHIP_TRY(launch_check("maxima_kernel"));
-        } else {
-            part = nullptr;
-        }
+        hipLaunchKernelGGL(maxima_kernel, dim3(MAXIMA, dloss ? 2 : 1), dim3(256), 0, s, (const float*)w, vocab * dim,
+                           (const float*)x, dim, rows * dim, targets, vocab, part);
+        MLXHIP_TRY(launch_check("maxima_kernel"));
         hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, part, dloss, targets, rows, vocab, scale);
         return launch_check("scale_kernel");
     }
@@ -420,18 +453,19 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     uint16_t *ds = (uint16_t*)(ws + ods), *xp = (uint16_t*)(ws + ox);
-    float *scale = nullptr, *sums = (float*)(ws + osum);
-    if (OT != MLXHIP_DTYPE_BF16) {  // bf16 has f32's range: dS as it is
-        scale = (float*)(ws + osc);
+    float *scale = (float*)(ws + osc), *sums = (float*)(ws + osum);
+    if constexpr (P > 1) {
         MLXHIP_TRY(o.scales(dloss, (float*)(ws + op), scale));
+        MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, scale + ce::SCALE_X, xp));
+    } else {
+        MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, nullptr, xp, dloss, scale));
     }
-    MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, scale ? scale + ce::SCALE_X : nullptr, xp));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         const int64_t n = std::min(width, o.vocab - v0);
         const uint16_t* wp = (const uint16_t*)o.w + v0 * o.dim;
         if (copy_w) {
             wp = (uint16_t*)(ws + ow);
-            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, scale ? scale + ce::SCALE_W : nullptr, (uint16_t*)(ws + ow)));
+            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, scale + ce::SCALE_W, (uint16_t*)(ws + ow)));
         }
         Args z;
         z.a = xp;
