@@ -455,7 +455,7 @@ int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* 
  * F16, of w, y, dy and dw; each product is rounded once, the sums are f32 in
  * an order that only the ids fix (no atomics: the same bits every time).
  * Operands contiguous, at any address aligned to their elements; results must
- * not overlap operands. n and vocab up to 2^31 - 1, dim up to 2^23. The
+ * not overlap operands. n and vocab up to 2^31 - 1, dim up to 2^20. The
  * gradient sorts the positions by id in a per-stream workspace (8 or 16
  * bytes per id and 4096 rows of dim f32 sums at most). No reference
  * counterpart for the gradient (crates/mlx-autograd/src/vjp.rs:173-176). */
@@ -476,19 +476,22 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * gradient forms them again from x, w and the forward's lse. dx or dw may be
  * NULL: that gradient is then not formed.
  * dtype: F32, BF16 or F16, of x, w, dx and dw; loss, lse and dloss are f32, as
- * are the logits, sums and products' accumulators. dS is rounded to bf16 or
- * f16 (scaled by a power of two, so that small probabilities stay normal) for
- * the products of 16-bit operands, and dx and dw once as they are stored. F32
- * operands and their dS enter the matrix cores as two f16 values each (22 bits;
- * scaled by a power of two, absolute error 2^-39 of the operand's largest value
- * where that is more), products below 2^-22 of a term left out.
+ * are the logits, sums and products' accumulators. dx and dw are rounded once,
+ * as they are stored. dS of 16-bit operands is rounded to their type for its
+ * products, scaled so that the largest dloss in magnitude is near 2^15 (small
+ * probabilities stay normal; a row whose dloss is that largest one has exact
+ * -1 of its target); of up to 16 rows (vocab up to 2^22) it stays f32. F32 products
+ * are f32 for the loss of up to 64 rows and the gradients of up to 32 (vocab up to
+ * 2^22); beyond that operands and dS enter the matrix cores as two f16 values each
+ * (22 bits; scaled by a power of two, absolute error 2^-39 of the operand's largest
+ * value where that is more), products below 2^-22 of a term left out.
  * Sums are formed in a fixed order. Operands contiguous, at any address
  * aligned to their elements; results must not overlap operands. A non-finite x
  * or w makes the logits it enters NaN. rows up to 2^21, dim up to 2^20, vocab up
  * to 2^31 - 1, rows times dim (rounded up to a multiple of 8) up to 2^29: cut a
  * larger batch by its rows. The workspace (per stream) holds dS for one piece of
- * the vocabulary, 256 MiB or 256 columns, copies of x and of a piece of w where
- * needed, and f32 sums of dx. No reference counterpart. */
+ * the vocabulary, 256 MiB or 256 columns (the few rows above: of the whole, up to
+ * 512 MiB), copies of x and of a piece of w where needed, and f32 sums of dx. No reference counterpart. */
 int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,
                                 float* loss, float* lse, int64_t rows, int64_t dim, int64_t vocab,
                                 void* stream);

@@ -1121,7 +1121,8 @@ int mlxhip_gemm_noalloc(int32_t ab_dtype, int32_t c_dtype, int32_t trans_a, int3
 }
 
 namespace {
-constexpr int64_t MAX_ROW = int64_t(1) << 23;  // columns of the row operators below
+constexpr int64_t MAX_ROW = int64_t(1) << 23;  // columns of a normalised row
+constexpr int64_t MAX_DIM = int64_t(1) << 20;  // columns of a table (grids within 2^32 work items)
 
 int check_sizes(const char* what, std::initializer_list<int64_t> sizes, std::initializer_list<int64_t> most) {
     auto m = most.begin();
@@ -1223,7 +1224,7 @@ int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* 
 
 int mlxhip_embedding_rows(int32_t dtype, const void* w, const int32_t* ids, void* y, int64_t n, int64_t vocab,
                           int64_t dim, float scale, void* stream) {
-    MLXHIP_TRY(check_sizes("embedding_rows", {n, vocab, dim}, {INT32_MAX, INT32_MAX, MAX_ROW}));
+    MLXHIP_TRY(check_sizes("embedding_rows", {n, vocab, dim}, {INT32_MAX, INT32_MAX, MAX_DIM}));
     if (n == 0 || dim == 0) return check_operands("embedding_rows", dtype, {});
     if (vocab == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding_rows: empty table");
     MLXHIP_TRY(check_operands("embedding_rows", dtype, {w, y}, {ids}));
@@ -1233,7 +1234,7 @@ int mlxhip_embedding_rows(int32_t dtype, const void* w, const int32_t* ids, void
 
 int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids, void* dw, int64_t n, int64_t vocab,
                               int64_t dim, float scale, void* stream) {
-    MLXHIP_TRY(check_sizes("embedding_vjp_rows", {n, vocab, dim}, {INT32_MAX, INT32_MAX, MAX_ROW}));
+    MLXHIP_TRY(check_sizes("embedding_vjp_rows", {n, vocab, dim}, {INT32_MAX, INT32_MAX, MAX_DIM}));
     if (dim == 0) return check_operands("embedding_vjp_rows", dtype, {});
     if (vocab == 0)
         return n ? fail(MLXHIP_ERR_INVALID_ARGUMENT, "embedding_vjp_rows: empty table")
@@ -1247,7 +1248,7 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
 namespace {
 // Sizes of the cross entropy's entry points.
 int check_cross_entropy(const char* what, int64_t rows, int64_t dim, int64_t vocab) {
-    MLXHIP_TRY(check_sizes(what, {rows, dim, vocab}, {1 << 21, 1 << 20, INT32_MAX}));
+    MLXHIP_TRY(check_sizes(what, {rows, dim, vocab}, {1 << 21, MAX_DIM, INT32_MAX}));
     if (dim == 0 || vocab == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: no logits (dim or vocab is 0)", what);
     // The kernels' offsets within x's planes are 32-bit bytes.
     if (rows * (ceil_div(dim, 8) * 8) > (1 << 29))

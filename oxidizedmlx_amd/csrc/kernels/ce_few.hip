@@ -1,24 +1,32 @@
-// ce_few.hip — the linear cross entropy of a few f32 rows (the loss of up to 64,
-// the gradients of up to 32), which reading W (and writing dW) bounds: W goes from memory straight into the f32
-// matrix instructions, with no copies and no planes.
+// ce_few.hip — the linear cross entropy of a few rows (f32: the loss of up to 64,
+// the gradients of up to 32; bf16 and f16: the gradients of up to 16), which
+// reading W (and writing dW) bounds: W goes from memory straight into the matrix
+// instructions (f32 ones but for the logits of 16-bit operands), with no copies
+// and no planes. dS stays f32: with a few rows one value may make most of a
+// gradient, and its rounding to 16 bits would not average out (one f16 row: dx
+// twice as far off as its own rounding).
 //
 //   stats: z = x W^T, a wave per 16 or 32 entries of the vocabulary; the row maxima
 //          and sums of a workgroup's entries, and the targets' logits.
 //   ds:    z again, kept as dS^T [vocab][16 NB] (zeros behind the rows).
-//   grad:  a wave per 64 columns and slice of the vocabulary: dW = dS^T x of 16
-//          entries at a time, and its sums of dx = dS W.
+//   grad:  a wave per 16 VEC columns (VEC values in 16 bytes) and slice of the
+//          vocabulary: dW = dS^T x of 16 entries at a time, and its sums of
+//          dx = dS W.
 //
 // v_mfma_f32_16x16x4_f32: lane l gives row (column) l % 16 of A (B) at k = l / 16
-// and holds rows 4 (l / 16) + i of column l % 16 of the result. A lane loads four
-// consecutive floats and gives them to four instructions: along K that is a
+// and holds rows 4 (l / 16) + i of column l % 16 of the result. A lane loads VEC
+// consecutive values and gives them to VEC instructions: along K that is a
 // permutation of the sum, along the columns of W and x one of the columns, which
 // the stores undo.
 //
-// Measured over 32000 entries of 1024: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds), 49
-// (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69; 64 rows 58 for stats. On
+// Measured over 32000 entries of 1024, f32: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds),
+// 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69; 64 rows 58 for stats. On
 // two f16 planes each (ce_gemm.hpp), whose copies read W twice and write it once
 // before, 1 to 64 rows take 107 - 113 us forward and 157 - 182 backward; the
 // gradients of 64 rows took 191 here, bound by the f32 matrix instructions.
+// bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s). Their loss has no path
+// here: the tiles of ce_gemm.hpp read W once too (8 rows of 768 over 32000: 15 us a
+// call there, 21 here).
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "ce_gemm.hpp"
@@ -30,9 +38,20 @@ namespace mlxhip {
 namespace ce {
 namespace {
 
-constexpr int F = MLXHIP_DTYPE_F32;
+using dev::Elem;
 
 __device__ inline f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// The eight values of a lane at once (k = 8 (l / 16) + 0..7): 16-bit products.
+template <int DT>
+__device__ inline f32x4 mfma32(const dev::u32x4& a, const dev::u32x4& b, f32x4 c) {
+    if constexpr (DT == MLXHIP_DTYPE_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gemm16::bf16x8, a),
+                                                       __builtin_bit_cast(gemm16::bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gemm16::f16x8, a),
+                                                      __builtin_bit_cast(gemm16::f16x8, b), c, 0, 0, 0);
+}
 
 // Tiles of 16 entries of a wave: with more rows two, so that a load of x serves
 // twice (64 rows of 1024 over 32000: 82 us with one).
@@ -43,28 +62,36 @@ constexpr int ENTRIES = 64 * TILES<NB>;  // of a workgroup
 
 // z[v][r] of the wave's TILES * 16 entries from v0 on and NB tiles of 16 rows. KB
 // blocks of 16 along K are loaded at once.
-template <int NB>
+template <int DT, int NB>
 __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 (&acc)[TILES<NB>][NB]) {
-    constexpr int KB = NB == 1 ? 6 : NB == 2 ? 4 : 3, T = TILES<NB>;
+    constexpr int KB = NB == 1 ? 6 : NB == 2 ? 4 : 3, T = TILES<NB>, VEC = Elem<DT>::VEC, BLOCK = 4 * VEC;
+    typedef typename Elem<DT>::type E;
     const int i = lane & 15, q = lane >> 4;
-    const float *w[T], *x[NB];
+    const E *w[T], *x[NB];
 #pragma unroll
-    for (int t = 0; t < T; ++t) w[t] = g.w + min(v0 + 16 * t + i, g.vocab - 1) * g.dim + 4 * q;
+    for (int t = 0; t < T; ++t) w[t] = static_cast<const E*>(g.w) + min(v0 + 16 * t + i, g.vocab - 1) * g.dim + VEC * q;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        x[b] = g.x + min((int64_t)(16 * b + i), g.rows - 1) * g.dim + 4 * q;
+        x[b] = static_cast<const E*>(g.x) + min((int64_t)(16 * b + i), g.rows - 1) * g.dim + VEC * q;
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    typedef dev::AnyVec<F> any;
+    typedef dev::AnyVec<DT> any;
     auto step = [&](const dev::u32x4 (&a)[T], const dev::u32x4 (&c)[NB]) {
+        if constexpr (DT == MLXHIP_DTYPE_F32) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < VEC; ++e)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int t = 0; t < T; ++t)
+                        acc[t][b] = mfma4(__uint_as_float(a[t][e]), __uint_as_float(c[b][e]), acc[t][b]);
+        } else {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int t = 0; t < T; ++t)
-                    acc[t][b] = mfma4(__uint_as_float(a[t][e]), __uint_as_float(c[b][e]), acc[t][b]);
+                for (int t = 0; t < T; ++t) acc[t][b] = mfma32<DT>(a[t], c[b], acc[t][b]);
+        }
     };
     // Two batches of loads in turn: one on its way while the other is used.
     dev::u32x4 a[2][KB][T], c[2][KB][NB];
@@ -72,43 +99,43 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
 #pragma unroll
         for (int s = 0; s < KB; ++s)
 #pragma unroll
-            for (int t = 0; t < T; ++t) fa[s][t] = *reinterpret_cast<const any*>(w[t] + k + 16 * s);
+            for (int t = 0; t < T; ++t) fa[s][t] = *reinterpret_cast<const any*>(w[t] + k + BLOCK * s);
 #pragma unroll
         for (int s = 0; s < KB; ++s)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) fc[s][b] = *reinterpret_cast<const any*>(x[b] + k + 16 * s);
+            for (int b = 0; b < NB; ++b) fc[s][b] = *reinterpret_cast<const any*>(x[b] + k + BLOCK * s);
     };
-    const int64_t batches = g.dim / (16 * KB);
+    const int64_t batches = g.dim / (BLOCK * KB);
     if (batches) fetch(0, a[0], c[0]);
     for (int64_t n = 0; n < batches; n += 2) {
-        if (n + 1 < batches) fetch((n + 1) * 16 * KB, a[1], c[1]);
+        if (n + 1 < batches) fetch((n + 1) * BLOCK * KB, a[1], c[1]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < KB; ++s) step(a[0][s], c[0][s]);
         if (n + 1 == batches) break;
-        if (n + 2 < batches) fetch((n + 2) * 16 * KB, a[0], c[0]);
+        if (n + 2 < batches) fetch((n + 2) * BLOCK * KB, a[0], c[0]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int s = 0; s < KB; ++s) step(a[1][s], c[1][s]);
     }
-    for (int64_t k = batches * 16 * KB; k < g.dim; k += 16) {
+    for (int64_t k = batches * BLOCK * KB; k < g.dim; k += BLOCK) {
         dev::u32x4 ta[T], tc[NB];
 #pragma unroll
-        for (int t = 0; t < T; ++t) ta[t] = dev::load_raw<F>(w[t], k, g.dim - 4 * q).q;
+        for (int t = 0; t < T; ++t) ta[t] = dev::load_raw<DT>(w[t], k, g.dim - VEC * q).q;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) tc[b] = dev::load_raw<F>(x[b], k, g.dim - 4 * q).q;
+        for (int b = 0; b < NB; ++b) tc[b] = dev::load_raw<DT>(x[b], k, g.dim - VEC * q).q;
         step(ta, tc);
     }
 }
 
 template <int NB>
 __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
-    constexpr int T = TILES<NB>;
+    constexpr int DT = MLXHIP_DTYPE_F32, T = TILES<NB>;
     __shared__ float red[4][2][16 * NB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 16 * T;
     f32x4 acc[T][NB];
-    if (v0 < g.vocab) few_logits<NB>(g, v0, lane, acc);
+    if (v0 < g.vocab) few_logits<DT, NB>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = 16 * b + i;
@@ -147,14 +174,14 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
     g.stats[r * g.stat_tiles + blockIdx.x] = make_float2(m, s);
 }
 
-template <int NB>
+template <int DT, int NB>
 __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
     constexpr int T = TILES<NB>;
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
     const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * T;
     if (v0 >= g.vocab) return;
     f32x4 acc[T][NB];
-    few_logits<NB>(g, v0, lane, acc);
+    few_logits<DT, NB>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = 16 * b + i;
@@ -172,62 +199,69 @@ __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
     }
 }
 
-template <int NB>
+template <int DT, int NB>
 __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
-    constexpr int RP = 16 * NB;
-    __shared__ float sums[4][RP][64];
+    constexpr int RP = 16 * NB, VEC = Elem<DT>::VEC, COLS = 16 * VEC;
+    typedef typename Elem<DT>::type E;
+    __shared__ float sums[4][RP][COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 64 + 4 * i;  // the lane's four columns
+    const int64_t n0 = (int64_t)blockIdx.x * COLS + VEC * i;  // the lane's columns
     const int64_t from = ((int64_t)blockIdx.y * 4 + wave) * g.slice, to = min(from + g.slice, g.vocab);
     // x at k = 4 t + q, columns n0 + j; zeros in rows without a target.
-    float xr[4 * NB][4];
+    float xr[4 * NB][VEC];
 #pragma unroll
     for (int t = 0; t < 4 * NB; ++t) {
         const int64_t r = 4 * t + q;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) xr[t][j] = 0.0f;
+        for (int j = 0; j < VEC; ++j) xr[t][j] = 0.0f;
         if (r < g.rows && counted(g.targets[r], g.vocab) && n0 < g.dim)
-            dev::unpack<F>(dev::load_raw<F>(g.x + r * g.dim, n0, g.dim), xr[t]);
+            dev::unpack<DT>(dev::load_raw<DT>(static_cast<const E*>(g.x) + r * g.dim, n0, g.dim), xr[t]);
     }
-    f32x4 dx[NB][4];
+    f32x4 dx[NB][VEC];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dx[b][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < VEC; ++j) dx[b][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int64_t v = from; v < to; v += 16) {
         if (g.dx) {
-            float w[4][4], a[4][NB];
+            dev::Vec16<DT> w[4];
+            float a[4][NB];
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const int64_t at = v + 4 * s + q;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[s][j] = 0.0f;
-                if (at < to && n0 < g.dim) dev::unpack<F>(dev::load_raw<F>(g.w + at * g.dim, n0, g.dim), w[s]);
+                w[s].q = dev::u32x4{0, 0, 0, 0};
+                if (at < to && n0 < g.dim) w[s] = dev::load_raw<DT>(static_cast<const E*>(g.w) + at * g.dim, n0, g.dim);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) a[s][b] = at < to ? g.ds[at * RP + 16 * b + i] : 0.0f;
             }
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < 4; ++s) {
+                float wf[VEC];
+                dev::unpack<DT>(w[s], wf);
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) dx[b][j] = mfma4(a[s][b], w[s][j], dx[b][j]);
+                    for (int j = 0; j < VEC; ++j) dx[b][j] = mfma4(a[s][b], wf[j], dx[b][j]);
+            }
         }
         if (g.dw) {
-            f32x4 o[4];
+            f32x4 o[VEC];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < VEC; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             const float* ds = g.ds + min(v + i, g.vocab - 1) * RP + q;
 #pragma unroll
             for (int t = 0; t < 4 * NB; ++t) {
                 const float a = ds[4 * t];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = mfma4(a, xr[t][j], o[j]);
+                for (int j = 0; j < VEC; ++j) o[j] = mfma4(a, xr[t][j], o[j]);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float out[4] = {o[0][e], o[1][e], o[2][e], o[3][e]};
-                if (v + 4 * q + e < to && n0 < g.dim) dev::store_vec<F>(g.dw + (v + 4 * q + e) * g.dim, n0, g.dim, out);
+                float out[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) out[j] = o[j][e];
+                if (v + 4 * q + e < to && n0 < g.dim)
+                    dev::store_vec<DT>(static_cast<E*>(g.dw) + (v + 4 * q + e) * g.dim, n0, g.dim, out);
             }
         }
     }
@@ -235,12 +269,12 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < VEC; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[wave][16 * b + 4 * q + e][4 * i + j] = dx[b][j][e];
+            for (int e = 0; e < 4; ++e) sums[wave][16 * b + 4 * q + e][VEC * i + j] = dx[b][j][e];
     __syncthreads();
-    for (int k = threadIdx.x; k < RP * 16; k += 256) {
-        const int64_t r = k >> 4, c = 4 * (k & 15), n = (int64_t)blockIdx.x * 64 + c;
+    for (int k = threadIdx.x; k < RP * COLS / 4; k += 256) {
+        const int64_t r = k / (COLS / 4), c = 4 * (k % (COLS / 4)), n = (int64_t)blockIdx.x * COLS + c;
         if (r >= g.rows || n >= g.ldx) continue;
         float4 s = *reinterpret_cast<const float4*>(&sums[0][r][c]);
 #pragma unroll
@@ -253,16 +287,17 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
 }
 
 template <int NB>
-int few_loss(const FewArgs& g, hipStream_t s) {
+int launch_loss(const FewArgs& g, hipStream_t s) {
     hipLaunchKernelGGL((few_stats_kernel<NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
     return launch_check("few_stats_kernel");
 }
 
-template <int NB>
-int few_grad(const FewArgs& g, hipStream_t s) {
-    hipLaunchKernelGGL((few_ds_kernel<NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
+template <int DT, int NB>
+int launch_grad(const FewArgs& g, hipStream_t s) {
+    hipLaunchKernelGGL((few_ds_kernel<DT, NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
     MLXHIP_TRY(launch_check("few_ds_kernel"));
-    hipLaunchKernelGGL((few_grad_kernel<NB>), dim3((unsigned)ceil_div(g.dim, 64), (unsigned)g.slices), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((few_grad_kernel<DT, NB>), dim3((unsigned)ceil_div(g.dim, 16 * Elem<DT>::VEC), (unsigned)g.slices),
+                       dim3(256), 0, s, g);
     return launch_check("few_grad_kernel");
 }
 
@@ -274,12 +309,14 @@ int64_t ce_few_tiles(int64_t rows, int64_t vocab) {
 }
 
 int ce_few_loss(const ce::FewArgs& g, hipStream_t s) {
-    if (g.rows <= 16) return ce::few_loss<1>(g, s);
-    return g.rows <= 32 ? ce::few_loss<2>(g, s) : ce::few_loss<4>(g, s);
+    if (g.rows <= 16) return ce::launch_loss<1>(g, s);
+    return g.rows <= 32 ? ce::launch_loss<2>(g, s) : ce::launch_loss<4>(g, s);
 }
 
-int ce_few_grad(const ce::FewArgs& g, hipStream_t s) {
-    return g.rows <= 16 ? ce::few_grad<1>(g, s) : ce::few_grad<2>(g, s);
+int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s) {
+    if (dt == MLXHIP_DTYPE_BF16) return ce::launch_grad<MLXHIP_DTYPE_BF16, 1>(g, s);
+    if (dt == MLXHIP_DTYPE_F16) return ce::launch_grad<MLXHIP_DTYPE_F16, 1>(g, s);
+    return g.rows <= 16 ? ce::launch_grad<MLXHIP_DTYPE_F32, 1>(g, s) : ce::launch_grad<MLXHIP_DTYPE_F32, 2>(g, s);
 }
 
 }  // namespace mlxhip

@@ -103,11 +103,18 @@ struct Args {
     int64_t ldc = 0;
 };
 
-// Few f32 rows (ce_few.hip): the loss of up to FEW_LOSS, the gradients of up to
-// FEW_GRAD.
-constexpr int FEW_LOSS = 64, FEW_GRAD = 32;
+// Few rows (ce_few.hip, with what each bound measured): the loss of up to 64 and
+// the gradients of up to 32 f32 rows, the gradients of up to 16 of 16 bits. Beyond
+// FEW_VOCAB entries the grids would pass 2^32 work items and dS^T 512 MiB.
+constexpr int64_t FEW_VOCAB = int64_t(1) << 22;
+inline bool few_loss(int dt, int64_t rows, int64_t vocab) {
+    return dt == MLXHIP_DTYPE_F32 && rows <= 64 && vocab <= FEW_VOCAB;
+}
+inline bool few_grad(int dt, int64_t rows, int64_t vocab) {
+    return rows <= (dt == MLXHIP_DTYPE_F32 ? 32 : 16) && vocab <= FEW_VOCAB;
+}
 struct FewArgs {
-    const float *x = nullptr, *w = nullptr;
+    const void *x = nullptr, *w = nullptr;
     int64_t rows = 0, dim = 0, vocab = 0;
     const int32_t* targets = nullptr;
     const float *lse = nullptr, *dloss = nullptr;
@@ -116,7 +123,7 @@ struct FewArgs {
     float* target_z = nullptr;
     float* ds = nullptr;        // dS^T [vocab][few_ds_rows(rows)]
     float* dx = nullptr;        // [slices][rows][ldx] or null
-    float* dw = nullptr;        // [vocab][dim] or null
+    void* dw = nullptr;         // [vocab][dim] or null
     int64_t ldx = 0, slices = 0, slice = 0;  // of 4 * slice entries each; slice a multiple of 16
 };
 inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
@@ -568,8 +575,8 @@ int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f32(int which, bool large, const ce::Args& a, hipStream_t s);
 // ce_few.hip
-int ce_few_loss(const ce::FewArgs& g, hipStream_t s);
-int ce_few_grad(const ce::FewArgs& g, hipStream_t s);
+int ce_few_loss(const ce::FewArgs& g, hipStream_t s);  // f32
+int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s);
 int64_t ce_few_tiles(int64_t rows, int64_t vocab);  // of the loss's statistics
 
 }  // namespace mlxhip

@@ -215,27 +215,54 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
     loss[r] = counted(targets[r], vocab) ? l - target_z[r] : 0.0f;
 }
 
-// dx from the f32 sums of its slices of K, zeros where there is no target.
+// dx from the f32 sums of its slices of K, zeros where there is no target: 64
+// quads of columns of a workgroup, four threads to each, which add up a quarter
+// of the slices each and then those, in order.
 template <int OT>
 __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums, int splits, int64_t rows, int64_t dim,
                                                  int64_t ld, const int32_t* __restrict__ targets, int64_t vocab,
                                                  const float* __restrict__ scale, typename Elem<OT>::type* __restrict__ dx) {
+    __shared__ float4 part[4][64];
     const int64_t quads = ld / 4, n = rows * quads;
     const float f = scale ? scale[ce::SCALE_DX] : 1.0f;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / quads, c = (i - r * quads) * 4;
+    const int q = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const int each = (splits + 3) / 4, k0 = g * each, k1 = min(k0 + each, splits);
+    for (int64_t base = (int64_t)blockIdx.x * 64; base < n; base += (int64_t)gridDim.x * 64) {
+        const int64_t i = base + q, r = i / quads, c = (i - r * quads) * 4;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (counted(targets[r], vocab)) {
+        const bool on = i < n && counted(targets[r], vocab);
+        if (on) {
+            const float* p = sums + r * ld + c;
 #pragma unroll 4
-            for (int k = 0; k < splits; ++k) {
-                const float4 v = *reinterpret_cast<const float4*>(sums + ((int64_t)k * rows + r) * ld + c);
+            for (int k = k0; k < k1; ++k) {
+                const float4 v = *reinterpret_cast<const float4*>(p + k * (rows * ld));
                 a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
             }
         }
-        const float v[4] = {a.x * f, a.y * f, a.z * f, a.w * f};
+        part[g][q] = a;
+        __syncthreads();
+        if (g == 0 && i < n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < dim) dx[r * dim + c + e] = dev::from_f32<OT>(v[e]);
+            for (int k = 1; k < 4; ++k) {
+                const float4 v = part[k][q];
+                a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
+            }
+            const float v[4] = {a.x * f, a.y * f, a.z * f, a.w * f};
+            typename Elem<OT>::type* to = dx + r * dim + c;
+            if (c + 4 <= dim) {
+                if constexpr (OT == MLXHIP_DTYPE_F32) {
+                    dev::store_vec<OT>(to, 0, 4, v);
+                } else {
+                    typedef uint32_t u32x2 __attribute__((ext_vector_type(2), aligned(2)));
+                    *reinterpret_cast<u32x2*>(to) = {gemm16::pack2<OT>(v[0], v[1]), gemm16::pack2<OT>(v[2], v[3])};
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < dim) to[e] = dev::from_f32<OT>(v[e]);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -310,9 +337,10 @@ struct Op {
     // Large tiles where they fill most of the compute units, one each.
     static bool large(int64_t m, int64_t n) { return tiles(m, n, true) >= 192; }
     // Columns of a piece: a copied piece of W and, with `ds`, dS within
-    // PIECE_BYTES, and offsets within a piece within 32 bits.
+    // PIECE_BYTES, offsets within a piece and the count of its tiles within 32 bits.
     int64_t width(bool ds, bool copy) const {
         int64_t w = std::min<int64_t>(vocab, (int64_t(1) << 29) / dim_p());
+        w = std::min(w, (int64_t(1) << 43) / rows);
         if (ds) w = std::min(w, PIECE_BYTES / (2 * P) / rows);
         if (copy) w = std::min(w, PIECE_BYTES / (2 * P) / dim_p());
         return w >= vocab ? vocab : std::max<int64_t>(w / 256 * 256, 256);
@@ -326,9 +354,9 @@ int finish_loss(const float2* stats, int64_t tiles, const float* target_z, const
     return launch_check("loss_kernel");
 }
 
-// Few f32 rows: reading W as it is in each product beats copying it as planes
-// (measured in ce_few.hip).
-ce::FewArgs few_args(const Op<MLXHIP_DTYPE_F32>& o) {
+// Few rows: W as it is in each product (measured in ce_few.hip).
+template <int OT>
+ce::FewArgs few_args(const Op<OT>& o) {
     ce::FewArgs g;
     g.x = o.x;
     g.w = o.w;
@@ -339,7 +367,8 @@ ce::FewArgs few_args(const Op<MLXHIP_DTYPE_F32>& o) {
     return g;
 }
 
-int few_loss(const Op<MLXHIP_DTYPE_F32>& o, float* loss, float* lse) {
+template <int OT>
+int few_loss(const Op<OT>& o, float* loss, float* lse) {
     ce::FewArgs g = few_args(o);
     g.stat_tiles = ce_few_tiles(o.rows, o.vocab);
     Carve c;
@@ -352,14 +381,16 @@ int few_loss(const Op<MLXHIP_DTYPE_F32>& o, float* loss, float* lse) {
     return finish_loss(g.stats, g.stat_tiles, g.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
 }
 
-int few_grad(const Op<MLXHIP_DTYPE_F32>& o, const float* lse, const float* dloss, float* dx, float* dw) {
+template <int OT>
+int few_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Elem<OT>::type* dx,
+             typename Elem<OT>::type* dw) {
     ce::FewArgs g = few_args(o);
     g.lse = lse;
     g.dloss = dloss;
     g.dw = dw;
     // Eight waves to a compute unit, four of a workgroup along the vocabulary.
     g.ldx = ceil_div(o.dim, 4) * 4;
-    const int64_t most = std::max<int64_t>(512 / ceil_div(o.dim, 64), 1);
+    const int64_t most = std::max<int64_t>(512 / ceil_div(o.dim, 16 * Elem<OT>::VEC), 1);
     g.slice = ceil_div(ceil_div(o.vocab, 4 * most), 16) * 16;
     g.slices = ceil_div(o.vocab, 4 * g.slice);
     Carve c;
@@ -369,17 +400,16 @@ int few_grad(const Op<MLXHIP_DTYPE_F32>& o, const float* lse, const float* dloss
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     g.ds = (float*)(ws + od);
     g.dx = dx ? (float*)(ws + ox) : nullptr;
-    MLXHIP_TRY(ce_few_grad(g, o.s));
+    MLXHIP_TRY(ce_few_grad(OT, g, o.s));
     if (!dx) return MLXHIP_OK;
-    hipLaunchKernelGGL((dx_kernel<MLXHIP_DTYPE_F32>), dim3(grid_for(o.rows * g.ldx / 4)), dim3(256), 0, o.s, g.dx,
+    hipLaunchKernelGGL((dx_kernel<OT>), dim3(grid_for(o.rows * g.ldx)), dim3(256), 0, o.s, g.dx,
                        (int)g.slices, o.rows, o.dim, g.ldx, o.targets, o.vocab, nullptr, dx);
     return launch_check("dx_kernel");
 }
 
 template <int OT>
 int run_loss(const Op<OT>& o, float* loss, float* lse) {
-    if constexpr (OT == MLXHIP_DTYPE_F32)
-        if (o.rows <= ce::FEW_LOSS) return few_loss(o, loss, lse);
+    if (ce::few_loss(OT, o.rows, o.vocab)) return few_loss(o, loss, lse);
     const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
     const int64_t width = o.width(false, copy_w);
     // One tile size for all pieces, whose widths are multiples of its columns.
@@ -434,8 +464,7 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         hipLaunchKernelGGL((zero_kernel<T>), dim3(grid_for(o.vocab * o.dim)), dim3(256), 0, o.s, dw, o.vocab * o.dim);
         return launch_check("zero_kernel");
     }
-    if constexpr (OT == MLXHIP_DTYPE_F32)
-        if (o.rows <= ce::FEW_GRAD) return few_grad(o, lse, dloss, dx, dw);
+    if (ce::few_grad(OT, o.rows, o.vocab)) return few_grad(o, lse, dloss, dx, dw);
     const bool copy_w = !o.in_place(o.w);
     const int64_t width = o.width(true, copy_w), ld = ceil_div(width, 256) * 256, dim_p = o.dim_p();
     // dx: few tiles, so K is cut into slices until every compute unit has one
@@ -522,7 +551,7 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         }
     }
     if (!dx) return MLXHIP_OK;
-    hipLaunchKernelGGL((dx_kernel<OT>), dim3(grid_for(o.rows * ldx / 4)), dim3(256), 0, o.s, sums, splits, o.rows, o.dim, ldx,
+    hipLaunchKernelGGL((dx_kernel<OT>), dim3(grid_for(o.rows * ldx)), dim3(256), 0, o.s, sums, splits, o.rows, o.dim, ldx,
                        o.targets, o.vocab, scale, dx);
     return launch_check("dx_kernel");
 }

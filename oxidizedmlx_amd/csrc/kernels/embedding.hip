@@ -36,8 +36,9 @@ using dev::Vec16;
 
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr int BITS = 8, BINS = 1 << BITS;
-// Positions that one workgroup sorts in its LDS (key and position, 8 bytes
-// each: 64 KiB; 8192 take 29 us that way and 31 in blocks), and those of a workgroup's block in a longer sort.
+// Positions that one workgroup sorts in its LDS (key and position, 8 bytes each:
+// 64 KiB; 8192 take 29 us that way and 31 in blocks), and those of a
+// workgroup's block in a longer sort.
 constexpr int LDS_SORT = 8192;
 constexpr int BLOCK_SORT = 2048;
 // Blocks whose counts the moving launch adds up itself.

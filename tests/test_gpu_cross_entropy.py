@@ -41,7 +41,7 @@ def check_all(got, x, w, t, dloss, dt, what):
 
 
 SIZES = [(1, 1, 1), (1, 8, 2), (2, 3, 5), (5, 64, 1), (1, 64, 1000), (7, 33, 37), (8, 768, 1003), (16, 128, 256),
-         (17, 100, 257), (33, 32, 4099), (64, 96, 512), (100, 256, 300), (128, 64, 128), (129, 70, 1025),
+         (16, 2011, 130), (17, 100, 257), (32, 200, 321), (33, 32, 4099), (64, 96, 512), (65, 333, 190), (100, 256, 300), (128, 64, 128), (129, 70, 1025),
          (256, 256, 512), (257, 40, 2001), (300, 520, 777), (513, 288, 1536), (1000, 77, 3203)]
 
 
@@ -149,6 +149,14 @@ def test_non_finite_rows_stay_in_their_rows(rows):
 def test_several_pieces_of_the_vocabulary(rows, dim, vocab, dt):
     a = inputs(rows, dim, vocab, dt)
     check_all(run(*a, dt), *a, dt, f"{rows}x{dim}x{vocab}")
+
+
+@pytest.mark.parametrize("dt", [abi.F32, abi.BF16], ids=R.NAMES.get)
+@pytest.mark.parametrize("vocab", [1 << 22, (1 << 22) + 77])
+def test_few_rows_of_millions_of_entries(vocab, dt):
+    """Either side of the vocabulary that the few rows' own kernels take."""
+    a = inputs(3, 8, vocab, dt)
+    check_all(run(*a, dt), *a, dt, f"3x8x{vocab}")
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)

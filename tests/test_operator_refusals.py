@@ -66,8 +66,10 @@ def test_other_types(f, dt):
 @pytest.mark.parametrize("f,sizes", [
     (ln, [{"rows": -1}, {"cols": -1}, {"rows": BIG}, {"cols": ROW}]),
     (ln_vjp, [{"rows": -1}, {"cols": -1}, {"rows": BIG}, {"cols": ROW}]),
-    (emb, [{"n": -1}, {"vocab": -1}, {"dim": -1}, {"n": BIG}, {"vocab": BIG}, {"dim": ROW}, {"vocab": 0}]),
-    (emb_vjp, [{"n": -1}, {"vocab": -1}, {"dim": -1}, {"n": BIG}, {"vocab": BIG}, {"dim": ROW}, {"vocab": 0}]),
+    (emb, [{"n": -1}, {"vocab": -1}, {"dim": -1}, {"n": BIG}, {"vocab": BIG}, {"dim": (1 << 20) + 1},
+           {"vocab": 0}]),
+    (emb_vjp, [{"n": -1}, {"vocab": -1}, {"dim": -1}, {"n": BIG}, {"vocab": BIG}, {"dim": (1 << 20) + 1},
+               {"vocab": 0}]),
     (ce, [{"rows": -1}, {"dim": -1}, {"vocab": -1}, {"rows": BIG}, {"vocab": BIG}, {"dim": (1 << 20) + 1}, {"dim": 0},
           {"vocab": 0}, {"rows": 1 << 12, "dim": 1 << 19}]),
     (ce_vjp, [{"rows": -1}, {"dim": -1}, {"vocab": -1}, {"rows": BIG}, {"vocab": BIG}, {"dim": (1 << 20) + 1}, {"dim": 0},
