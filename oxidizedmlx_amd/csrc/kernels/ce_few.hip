@@ -1,6 +1,7 @@
-// ce_few.hip — the linear cross entropy of a few rows (f32: the loss of up to 64,
-// the gradients of up to 32; bf16 and f16: the gradients of up to 16), which
-// reading W (and writing dW) bounds: W goes from memory straight into the matrix
+// ce_few.hip — the linear cross entropy of a few rows (the loss of up to 64, of
+// 16-bit operands where W's rows are no whole 16-byte chunks; the gradients of up
+// to 32 f32 rows, or 16 of 16 bits), which reading W (and writing dW) bounds: W
+// goes from memory straight into the matrix
 // instructions (f32 ones but for the logits of 16-bit operands), with no copies
 // and no planes. dS stays f32: with a few rows one value may make most of a
 // gradient, and its rounding to 16 bits would not average out (one f16 row: dx
@@ -24,9 +25,11 @@
 // two f16 planes each (ce_gemm.hpp), whose copies read W twice and write it once
 // before, 1 to 64 rows take 107 - 113 us forward and 157 - 182 backward; the
 // gradients of 64 rows took 191 here, bound by the f32 matrix instructions.
-// bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s). Their loss has no path
-// here: the tiles of ce_gemm.hpp read W once too (8 rows of 768 over 32000: 15 us a
-// call there, 21 here).
+// bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s), 77 with the loss; the tiles of
+// ce_gemm.hpp take 69 for 17, with errors of dx and dw up to twice as large. The
+// loss where the tiles read W in place: 15 us a call there, 21 here (8 rows of 768
+// over 32000); where they would copy it (2044 columns over 50257): 47 - 89 here,
+// 144 there for 65 rows.
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "ce_gemm.hpp"
@@ -60,23 +63,64 @@ constexpr int TILES = NB == 1 ? 1 : 2;
 template <int NB>
 constexpr int ENTRIES = 64 * TILES<NB>;  // of a workgroup
 
+// Rows whose elements may begin in the middle of a dword (16-bit types, ODD): the
+// 16 bytes from the dword that a vector begins in and the dword behind them (of
+// one that begins with its dword: the fourth again, unused), moved together as
+// they are used. Loads at such addresses take several times as long: 8 rows of
+// 2047 over 50257 took 171 us with them.
+template <bool ODD>
+struct Loaded {
+    dev::u32x4 q;
+    uint32_t next[ODD ? 1 : 0];
+};
+template <int DT, bool ODD>
+struct Row {
+    typedef typename Elem<DT>::type E;
+    const E* p;
+    uint32_t shift = 0;  // bits
+    __device__ void set(const E* row) {
+        p = row;
+        if constexpr (ODD) {
+            shift = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 2) * 8;
+            p -= shift / 16;
+        }
+    }
+    __device__ Loaded<ODD> load(int64_t k) const {
+        Loaded<ODD> v;
+        if constexpr (ODD) {
+            v.q = dev::load16<MLXHIP_DTYPE_F32>(reinterpret_cast<const float*>(p + k));
+            v.next[0] = *reinterpret_cast<const uint32_t*>(p + k + 6 + shift / 8);
+        } else {
+            v.q = dev::load16<DT>(p + k);
+        }
+        return v;
+    }
+    __device__ dev::u32x4 join(const Loaded<ODD>& v) const {
+        if constexpr (!ODD) return v.q;
+        else
+            return dev::u32x4{__builtin_amdgcn_alignbit(v.q[1], v.q[0], shift), __builtin_amdgcn_alignbit(v.q[2], v.q[1], shift),
+                              __builtin_amdgcn_alignbit(v.q[3], v.q[2], shift),
+                              __builtin_amdgcn_alignbit(v.next[0], v.q[3], shift)};
+    }
+    __device__ dev::u32x4 load_end(int64_t k, int64_t n) const { return dev::load_raw<DT>(p + shift / 16, k, n).q; }
+};
+
 // z[v][r] of the wave's TILES * 16 entries from v0 on and NB tiles of 16 rows. KB
-// blocks of 16 along K are loaded at once.
-template <int DT, int NB>
+// blocks along K are loaded at once.
+template <int DT, int NB, bool ODD>
 __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 (&acc)[TILES<NB>][NB]) {
     constexpr int KB = NB == 1 ? 6 : NB == 2 ? 4 : 3, T = TILES<NB>, VEC = Elem<DT>::VEC, BLOCK = 4 * VEC;
     typedef typename Elem<DT>::type E;
     const int i = lane & 15, q = lane >> 4;
-    const E *w[T], *x[NB];
+    Row<DT, ODD> w[T], x[NB];
 #pragma unroll
-    for (int t = 0; t < T; ++t) w[t] = static_cast<const E*>(g.w) + min(v0 + 16 * t + i, g.vocab - 1) * g.dim + VEC * q;
+    for (int t = 0; t < T; ++t) w[t].set(static_cast<const E*>(g.w) + min(v0 + 16 * t + i, g.vocab - 1) * g.dim);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        x[b] = static_cast<const E*>(g.x) + min((int64_t)(16 * b + i), g.rows - 1) * g.dim + VEC * q;
+        x[b].set(static_cast<const E*>(g.x) + min((int64_t)(16 * b + i), g.rows - 1) * g.dim);
 #pragma unroll
         for (int t = 0; t < T; ++t) acc[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    typedef dev::AnyVec<DT> any;
     auto step = [&](const dev::u32x4 (&a)[T], const dev::u32x4 (&c)[NB]) {
         if constexpr (DT == MLXHIP_DTYPE_F32) {
 #pragma unroll
@@ -94,48 +138,66 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
         }
     };
     // Two batches of loads in turn: one on its way while the other is used.
-    dev::u32x4 a[2][KB][T], c[2][KB][NB];
-    auto fetch = [&](int64_t k, dev::u32x4 (&fa)[KB][T], dev::u32x4 (&fc)[KB][NB]) {
+    struct Batch {
+        Loaded<ODD> a[KB][T], c[KB][NB];
+    } batch[2];
+    auto fetch = [&](int64_t n, int steps, Batch& to) {
+        const int64_t k = n * BLOCK * KB + VEC * q;
 #pragma unroll
-        for (int s = 0; s < KB; ++s)
+        for (int s = 0; s < KB; ++s) {
+            if (s >= steps) break;
 #pragma unroll
-            for (int t = 0; t < T; ++t) fa[s][t] = *reinterpret_cast<const any*>(w[t] + k + BLOCK * s);
+            for (int t = 0; t < T; ++t) to.a[s][t] = w[t].load(k + BLOCK * s);
 #pragma unroll
-        for (int s = 0; s < KB; ++s)
+            for (int b = 0; b < NB; ++b) to.c[s][b] = x[b].load(k + BLOCK * s);
+        }
+    };
+    auto use = [&](const Batch& from, int steps) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) fc[s][b] = *reinterpret_cast<const any*>(x[b] + k + BLOCK * s);
+        for (int s = 0; s < KB; ++s) {
+            if (s >= steps) break;
+            dev::u32x4 a[T], c[NB];
+#pragma unroll
+            for (int t = 0; t < T; ++t) a[t] = w[t].join(from.a[s][t]);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) c[b] = x[b].join(from.c[s][b]);
+            step(a, c);
+        }
     };
     const int64_t batches = g.dim / (BLOCK * KB);
-    if (batches) fetch(0, a[0], c[0]);
+    if (batches) fetch(0, KB, batch[0]);
     for (int64_t n = 0; n < batches; n += 2) {
-        if (n + 1 < batches) fetch((n + 1) * BLOCK * KB, a[1], c[1]);
+        if (n + 1 < batches) fetch(n + 1, KB, batch[1]);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < KB; ++s) step(a[0][s], c[0][s]);
+        use(batch[0], KB);
         if (n + 1 == batches) break;
-        if (n + 2 < batches) fetch((n + 2) * BLOCK * KB, a[0], c[0]);
+        if (n + 2 < batches) fetch(n + 2, KB, batch[0]);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < KB; ++s) step(a[1][s], c[1][s]);
+        use(batch[1], KB);
     }
-    for (int64_t k = batches * BLOCK * KB; k < g.dim; k += BLOCK) {
-        dev::u32x4 ta[T], tc[NB];
+    // The whole blocks that are left, and a last one that is not.
+    const int left = (int)(g.dim / BLOCK - batches * KB);
+    const int64_t end = g.dim / BLOCK * BLOCK;
+    fetch(batches, left, batch[0]);
+    dev::u32x4 a[T], c[NB];
+    if (end < g.dim) {
 #pragma unroll
-        for (int t = 0; t < T; ++t) ta[t] = dev::load_raw<DT>(w[t], k, g.dim - VEC * q).q;
+        for (int t = 0; t < T; ++t) a[t] = w[t].load_end(end + VEC * q, g.dim);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) tc[b] = dev::load_raw<DT>(x[b], k, g.dim - VEC * q).q;
-        step(ta, tc);
+        for (int b = 0; b < NB; ++b) c[b] = x[b].load_end(end + VEC * q, g.dim);
     }
+    use(batch[0], left);
+    if (end < g.dim) step(a, c);
 }
 
-template <int NB>
+template <int DT, int NB, bool ODD>
 __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
-    constexpr int DT = MLXHIP_DTYPE_F32, T = TILES<NB>;
+    constexpr int T = TILES<NB>;
     __shared__ float red[4][2][16 * NB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 16 * T;
     f32x4 acc[T][NB];
-    if (v0 < g.vocab) few_logits<DT, NB>(g, v0, lane, acc);
+    if (v0 < g.vocab) few_logits<DT, NB, ODD>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = 16 * b + i;
@@ -174,14 +236,14 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
     g.stats[r * g.stat_tiles + blockIdx.x] = make_float2(m, s);
 }
 
-template <int DT, int NB>
+template <int DT, int NB, bool ODD>
 __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
     constexpr int T = TILES<NB>;
     const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
     const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * T;
     if (v0 >= g.vocab) return;
     f32x4 acc[T][NB];
-    few_logits<DT, NB>(g, v0, lane, acc);
+    few_logits<DT, NB, ODD>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int64_t r = 16 * b + i;
@@ -286,15 +348,34 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
     }
 }
 
-template <int NB>
+// Whether a row of x or W begins in the middle of a dword.
+bool odd_rows(const FewArgs& g) {
+    return (reinterpret_cast<uintptr_t>(g.x) | reinterpret_cast<uintptr_t>(g.w) | (uintptr_t)g.dim * 2) & 2;
+}
+
+template <int DT, int NB>
 int launch_loss(const FewArgs& g, hipStream_t s) {
-    hipLaunchKernelGGL((few_stats_kernel<NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
+    const dim3 grid((unsigned)ceil_div(g.vocab, ENTRIES<NB>));
+    if (DT != MLXHIP_DTYPE_F32 && odd_rows(g))
+        hipLaunchKernelGGL((few_stats_kernel<DT, NB, DT != MLXHIP_DTYPE_F32>), grid, dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((few_stats_kernel<DT, NB, false>), grid, dim3(256), 0, s, g);
     return launch_check("few_stats_kernel");
+}
+
+template <int DT>
+int typed_loss(const FewArgs& g, hipStream_t s) {
+    if (g.rows <= 16) return launch_loss<DT, 1>(g, s);
+    return g.rows <= 32 ? launch_loss<DT, 2>(g, s) : launch_loss<DT, 4>(g, s);
 }
 
 template <int DT, int NB>
 int launch_grad(const FewArgs& g, hipStream_t s) {
-    hipLaunchKernelGGL((few_ds_kernel<DT, NB>), dim3((unsigned)ceil_div(g.vocab, ENTRIES<NB>)), dim3(256), 0, s, g);
+    const dim3 grid((unsigned)ceil_div(g.vocab, ENTRIES<NB>));
+    if (DT != MLXHIP_DTYPE_F32 && odd_rows(g))
+        hipLaunchKernelGGL((few_ds_kernel<DT, NB, DT != MLXHIP_DTYPE_F32>), grid, dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((few_ds_kernel<DT, NB, false>), grid, dim3(256), 0, s, g);
     MLXHIP_TRY(launch_check("few_ds_kernel"));
     hipLaunchKernelGGL((few_grad_kernel<DT, NB>), dim3((unsigned)ceil_div(g.dim, 16 * Elem<DT>::VEC), (unsigned)g.slices),
                        dim3(256), 0, s, g);
@@ -308,9 +389,9 @@ int64_t ce_few_tiles(int64_t rows, int64_t vocab) {
     return ceil_div(vocab, rows <= 16 ? ce::ENTRIES<1> : rows <= 32 ? ce::ENTRIES<2> : ce::ENTRIES<4>);
 }
 
-int ce_few_loss(const ce::FewArgs& g, hipStream_t s) {
-    if (g.rows <= 16) return ce::launch_loss<1>(g, s);
-    return g.rows <= 32 ? ce::launch_loss<2>(g, s) : ce::launch_loss<4>(g, s);
+int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s) {
+    if (dt == MLXHIP_DTYPE_F32) return ce::typed_loss<MLXHIP_DTYPE_F32>(g, s);
+    return dt == MLXHIP_DTYPE_BF16 ? ce::typed_loss<MLXHIP_DTYPE_BF16>(g, s) : ce::typed_loss<MLXHIP_DTYPE_F16>(g, s);
 }
 
 int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s) {

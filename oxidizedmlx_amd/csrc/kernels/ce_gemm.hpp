@@ -103,13 +103,12 @@ struct Args {
     int64_t ldc = 0;
 };
 
-// Few rows (ce_few.hip, with what each bound measured): the loss of up to 64 and
-// the gradients of up to 32 f32 rows, the gradients of up to 16 of 16 bits. Beyond
-// FEW_VOCAB entries the grids would pass 2^32 work items and dS^T 512 MiB.
+// Few rows (ce_few.hip, with what each bound measured): the loss of up to 64 rows
+// (of 16 bits: where the tiles would need a copy of W), the gradients of up to 32
+// f32 rows or 16 of 16 bits. Beyond FEW_VOCAB entries the grids would pass 2^32
+// work items and dS^T 512 MiB.
 constexpr int64_t FEW_VOCAB = int64_t(1) << 22;
-inline bool few_loss(int dt, int64_t rows, int64_t vocab) {
-    return dt == MLXHIP_DTYPE_F32 && rows <= 64 && vocab <= FEW_VOCAB;
-}
+inline bool few_loss(bool copy_w, int64_t rows, int64_t vocab) { return copy_w && rows <= 64 && vocab <= FEW_VOCAB; }
 inline bool few_grad(int dt, int64_t rows, int64_t vocab) {
     return rows <= (dt == MLXHIP_DTYPE_F32 ? 32 : 16) && vocab <= FEW_VOCAB;
 }
@@ -200,7 +199,7 @@ __device__ inline void store_tile(const f32x16 (&acc)[C::TM][C::TN], MLXHIP_LDS 
                                   int64_t ld, int64_t m, int64_t n, int64_t cap, int64_t row0, int64_t col0, int lane,
                                   bool add) {
     typedef typename dev::Elem<CT>::type T;
-    typedef dev::AnyVec<CT> any;
+    typedef uint32_t any __attribute__((ext_vector_type(4), aligned(2)));  // at any element
     constexpr int TM = C::TM, TN = C::TN, ES = sizeof(T), VEC = 16 / ES;
     constexpr int ROW_BYTES = 32 * TN * ES, CHUNKS = ROW_BYTES / 16, SHARE = CHUNKS >= 16 ? 1 : 16 / CHUNKS;
     constexpr int PASS = C::EPI / ROW_BYTES < 32 ? C::EPI / ROW_BYTES : 32;  // rows staged at a time
@@ -575,7 +574,7 @@ int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f32(int which, bool large, const ce::Args& a, hipStream_t s);
 // ce_few.hip
-int ce_few_loss(const ce::FewArgs& g, hipStream_t s);  // f32
+int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s);
 int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s);
 int64_t ce_few_tiles(int64_t rows, int64_t vocab);  // of the loss's statistics
 

@@ -377,7 +377,7 @@ int few_loss(const Op<OT>& o, float* loss, float* lse) {
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     g.stats = (float2*)(ws + os);
     g.target_z = (float*)(ws + oz);
-    MLXHIP_TRY(ce_few_loss(g, o.s));
+    MLXHIP_TRY(ce_few_loss(OT, g, o.s));
     return finish_loss(g.stats, g.stat_tiles, g.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
 }
 
@@ -409,8 +409,8 @@ int few_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
 
 template <int OT>
 int run_loss(const Op<OT>& o, float* loss, float* lse) {
-    if (ce::few_loss(OT, o.rows, o.vocab)) return few_loss(o, loss, lse);
     const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
+    if (ce::few_loss(copy_w, o.rows, o.vocab)) return few_loss(o, loss, lse);
     const int64_t width = o.width(false, copy_w);
     // One tile size for all pieces, whose widths are multiples of its columns.
     const bool large = Op<OT>::large(o.rows, o.vocab);

@@ -43,22 +43,40 @@ __device__ inline typename Elem<DT>::type from_f32(float v) {
 // ends. At any element-aligned address: one dwordx4 access (gfx950 allows
 // unaligned global accesses).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 __attribute__((aligned(4))) u32x4_at4;
-typedef u32x4 __attribute__((aligned(2))) u32x4_at2;
+// AnyVec is a struct because a typedef's alignment gets lost as a template's
+// argument, and the compiler then takes the address's low bits to be 0.
 template <int DT>
-using AnyVec = std::conditional_t<DT == MLXHIP_DTYPE_F32, u32x4_at4, u32x4_at2>;
+struct __attribute__((packed, aligned(DT == MLXHIP_DTYPE_F32 ? 4 : 2))) AnyVec {
+    u32x4 q;
+};
+template <int DT>
+__device__ inline u32x4 load16(const typename Elem<DT>::type* p) {
+    return reinterpret_cast<const AnyVec<DT>*>(p)->q;
+}
 template <int DT>
 struct Vec16 {
     u32x4 q;
 };
 
 // Elements [i, i + VEC) of p as they are, zeros from element n on. Separate
-// from unpack so that several loads stay in flight.
+// from unpack so that several loads stay in flight. A vector that runs past n is
+// the last one of the n, moved down (loads of its elements one by one took
+// three times as long as the whole copy of f16 rows of 777).
 template <int DT>
 __device__ inline Vec16<DT> load_raw(const typename Elem<DT>::type* p, int64_t i, int64_t n) {
     constexpr int VEC = Elem<DT>::VEC;
-    if (i + VEC <= n) return {*reinterpret_cast<const AnyVec<DT>*>(p + i)};
+    if (i + VEC <= n) return {load16<DT>(p + i)};
     u32x4 q = {0, 0, 0, 0};
+    if (n >= VEC) {
+        const int past = (int)min(i + VEC - n, (int64_t)VEC);
+        const u32x4 all = load16<DT>(p + (n - VEC));
+        const int words = DT == MLXHIP_DTYPE_F32 ? past : past / 2;
+        u32x4 one = words & 1 ? u32x4{all[1], all[2], all[3], 0} : all;
+        one = words & 2 ? u32x4{one[2], one[3], 0, 0} : one;
+        one = words & 4 ? q : one;
+        if (DT == MLXHIP_DTYPE_F32 || !(past & 1)) return {one};
+        return {u32x4{one[0] >> 16 | one[1] << 16, one[1] >> 16 | one[2] << 16, one[2] >> 16 | one[3] << 16, one[3] >> 16}};
+    }
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
         if (i + e < n) {
@@ -87,7 +105,7 @@ __device__ inline void store_vec(typename Elem<DT>::type* p, int64_t i, int64_t 
             if constexpr (DT == MLXHIP_DTYPE_F32) q[k] = __float_as_uint(v[k]);
             else q[k] = from_f32<DT>(v[2 * k]) | (uint32_t)from_f32<DT>(v[2 * k + 1]) << 16;
         }
-        *reinterpret_cast<AnyVec<DT>*>(p + i) = q;
+        reinterpret_cast<AnyVec<DT>*>(p + i)->q = q;
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)

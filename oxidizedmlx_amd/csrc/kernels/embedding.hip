@@ -56,7 +56,7 @@ struct Piece {
 template <int DT, int N>
 __device__ inline Piece<DT, N> load_piece(const typename Elem<DT>::type* p) {
     if constexpr (N == 1) return {*p};
-    else return {*reinterpret_cast<const dev::AnyVec<DT>*>(p)};
+    else return {dev::load16<DT>(p)};
 }
 template <int DT, int N>
 __device__ inline void widen(const Piece<DT, N>& x, float (&v)[N]) {

@@ -85,8 +85,8 @@ struct Columns {
     __device__ bool own(int j, int e) const { return j < NV - 1 || (e >= from && e < to); }
     __device__ void load(const typename Elem<DT>::type* p, Vec16<DT> (&out)[NV]) const {
 #pragma unroll
-        for (int j = 0; j < NV - 1; ++j) out[j].q = *reinterpret_cast<const dev::AnyVec<DT>*>(p + at(j));
-        if (to == VEC) out[NV - 1].q = *reinterpret_cast<const dev::AnyVec<DT>*>(p + last);
+        for (int j = 0; j < NV - 1; ++j) out[j].q = dev::load16<DT>(p + at(j));
+        if (to == VEC) out[NV - 1].q = dev::load16<DT>(p + last);
         else out[NV - 1] = load_raw<DT>(p, 0, to);
     }
     __device__ void store(typename Elem<DT>::type* p, int j, const float* v) const {
