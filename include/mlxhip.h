@@ -481,7 +481,7 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * products, scaled so that the largest dloss in magnitude is near 2^15 (small
  * probabilities stay normal; a row whose dloss is that largest one has exact
  * -1 of its target); of up to 16 rows (vocab up to 2^22) it stays f32. F32 products
- * are f32 for the loss of up to 64 rows and the gradients of up to 32 (vocab up to
+ * are f32 for the loss of up to 128 rows and the gradients of up to 32 (vocab up to
  * 2^22); beyond that operands and dS enter the matrix cores as two f16 values each
  * (22 bits; scaled by a power of two, absolute error 2^-39 of the operand's largest
  * value where that is more), products below 2^-22 of a term left out.

@@ -1,9 +1,8 @@
-// ce_few.hip — the linear cross entropy of a few rows (the loss of up to 64, of
-// 16-bit operands where W's rows are no whole 16-byte chunks; the gradients of up
-// to 32 f32 rows, or 16 of 16 bits), which reading W (and writing dW) bounds: W
-// goes from memory straight into the matrix
-// instructions (f32 ones but for the logits of 16-bit operands), with no copies
-// and no planes. dS stays f32: with a few rows one value may make most of a
+// ce_few.hip — the linear cross entropy of a few rows (the loss of up to 128 f32
+// rows, or 64 of 16 bits where W's rows are no whole 16-byte chunks; the gradients
+// of up to 32 f32 rows, or 16 of 16 bits), which reading W (and writing dW) bounds:
+// W goes from memory straight into the matrix instructions (f32 ones but for the
+// logits of 16-bit operands), with no copies and no planes. dS stays f32: with a few rows one value may make most of a
 // gradient, and its rounding to 16 bits would not average out (one f16 row: dx
 // twice as far off as its own rounding).
 //
@@ -21,10 +20,10 @@
 // the stores undo.
 //
 // Measured over 32000 entries of 1024, f32: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds),
-// 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69; 64 rows 58 for stats. On
-// two f16 planes each (ce_gemm.hpp), whose copies read W twice and write it once
-// before, 1 to 64 rows take 107 - 113 us forward and 157 - 182 backward; the
-// gradients of 64 rows took 191 here, bound by the f32 matrix instructions.
+// 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69. On two f16 planes each
+// (ce_gemm.hpp), whose copies read W twice and write it once before, 1 to 64 rows
+// take 107 - 113 us forward and 157 - 182 backward; the gradients of 64 rows took
+// 191 here, bound by the f32 matrix instructions, and the loss of 256 rows 164 (130).
 // bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s), 77 with the loss; the tiles of
 // ce_gemm.hpp take 69 for 17, with errors of dx and dw up to twice as large. The
 // loss where the tiles read W in place: 15 us a call there, 21 here (8 rows of 768
@@ -190,17 +189,15 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
     if (end < g.dim) step(a, c);
 }
 
-template <int DT, int NB, bool ODD>
-__global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
-    constexpr int T = TILES<NB>;
+// The maxima and sums of z over the T tiles of 16 entries from v0 on of each of the
+// workgroup's waves, for NB tiles of 16 rows from r0 on, as entry `tile` of stats.
+template <int T, int NB>
+__device__ inline void leave_stats(const FewArgs& g, int64_t v0, int64_t r0, int64_t tile, const f32x4 (&acc)[T][NB]) {
     __shared__ float red[4][2][16 * NB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
-    const int64_t v0 = ((int64_t)blockIdx.x * 4 + wave) * 16 * T;
-    f32x4 acc[T][NB];
-    if (v0 < g.vocab) few_logits<DT, NB, ODD>(g, v0, lane, acc);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int64_t r = 16 * b + i;
+        const int64_t r = r0 + 16 * b + i;
         float m = -INFINITY, s = 0.0f;
         if (v0 < g.vocab) {
             const int64_t target = r < g.rows ? g.targets[r] : -1;
@@ -229,11 +226,104 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
     }
     __syncthreads();
     const int r = threadIdx.x;
-    if (r >= 16 * NB || r >= g.rows) return;
+    if (r >= 16 * NB || r0 + r >= g.rows) return;
     float m = red[0][0][r], s = red[0][1][r];
 #pragma unroll
     for (int w = 1; w < 4; ++w) merge(m, s, red[w][0][r], red[w][1][r]);
-    g.stats[r * g.stat_tiles + blockIdx.x] = make_float2(m, s);
+    g.stats[(r0 + r) * g.stat_tiles + tile] = make_float2(m, s);
+}
+
+template <int DT, int NB, bool ODD>
+__global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
+    constexpr int T = TILES<NB>;
+    const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * T;
+    f32x4 acc[T][NB];
+    if (v0 < g.vocab) few_logits<DT, NB, ODD>(g, v0, threadIdx.x & 63, acc);
+    leave_stats<T, NB>(g, v0, 0, blockIdx.x, acc);
+}
+
+// f32 rows by 64: x goes through LDS, KC columns at a time, and serves a
+// workgroup's four waves of 16 T entries each; W comes straight from memory, a
+// chunk ahead. 128 rows of 1024 over 32000: 82 us, 102 TFLOP/s of f32, and 280 for
+// 2044 over 50257 (whole calls 90 and 290; on planes 121 and 450; a large f32 product
+// reaches 154 TFLOP/s). 32 entries a wave, 32 columns a chunk, or two or five waves
+// to a SIMD: 1 - 15 % slower; 128 rows a workgroup: 64 rows take 97 instead of 57.
+constexpr int WIDE_ROWS = 64, WIDE_T = 1, WIDE_ENTRIES = 64 * WIDE_T;
+__global__ __launch_bounds__(256, 4) void wide_stats_kernel(FewArgs g, int64_t row_blocks, int64_t tiles) {
+    constexpr int NB = WIDE_ROWS / 16, T = WIDE_T, KC = 64, S = KC / 16, PIECES = WIDE_ROWS * KC / 4 / 256;
+    constexpr int DT = MLXHIP_DTYPE_F32;
+    __shared__ __attribute__((aligned(16))) float xs[2][WIDE_ROWS][KC + 4];  // 16 rows' quads in different banks
+    // The row blocks of a tile of entries follow each other on one XCD (every
+    // eighth workgroup), whose cache then holds the tile's part of W.
+    const int64_t xcd = blockIdx.x % 8, at = blockIdx.x / 8, tile = at / row_blocks * 8 + xcd, r0 = at % row_blocks * WIDE_ROWS;
+    if (tile >= tiles) return;
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+    const int64_t v0 = (tile * 4 + (threadIdx.x >> 6)) * 16 * T;
+    const float *w[T], *x = static_cast<const float*>(g.x);
+    int32_t xo[PIECES];  // rows * dim fits
+#pragma unroll
+    for (int t = 0; t < T; ++t) w[t] = static_cast<const float*>(g.w) + min(v0 + 16 * t + i, g.vocab - 1) * g.dim;
+    const int px = (threadIdx.x % (KC / 4)) * 4, pr = threadIdx.x / (KC / 4);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p)
+        xo[p] = (int32_t)(min(r0 + pr + p * (1024 / KC), g.rows - 1) * g.dim);
+    dev::u32x4 wv[2][T][S], xv[PIECES];
+    auto fetch = [&](int64_t k, dev::u32x4 (&to)[T][S]) {
+        if (k + KC <= g.dim) {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int s = 0; s < S; ++s) to[t][s] = dev::load16<DT>(w[t] + k + 16 * s + 4 * q);
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) xv[p] = dev::load16<DT>(x + xo[p] + k + px);
+        } else {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int s = 0; s < S; ++s) to[t][s] = dev::load_raw<DT>(w[t], k + 16 * s + 4 * q, g.dim).q;
+#pragma unroll
+            for (int p = 0; p < PIECES; ++p) xv[p] = dev::load_raw<DT>(x + xo[p], k + px, g.dim).q;
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) *reinterpret_cast<dev::u32x4*>(&xs[buf][pr + p * (1024 / KC)][px]) = xv[p];
+        __syncthreads();
+    };
+    f32x4 acc[T][NB];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto use = [&](const dev::u32x4 (&a)[T][S], int buf) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            dev::u32x4 c[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) c[b] = *reinterpret_cast<const dev::u32x4*>(&xs[buf][16 * b + i][16 * s + 4 * q]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int t = 0; t < T; ++t)
+                        acc[t][b] = mfma4(__uint_as_float(a[t][s][e]), __uint_as_float(c[b][e]), acc[t][b]);
+        }
+    };
+    fetch(0, wv[0]);
+    stage(0);
+    // A chunk's loads are on their way while the one before it is used; a buffer
+    // is written again after a barrier behind its last use.
+    for (int64_t k = 0; k < g.dim; k += 2 * KC) {
+        if (k + KC < g.dim) fetch(k + KC, wv[1]);
+        use(wv[0], 0);
+        if (k + KC >= g.dim) break;
+        stage(1);
+        if (k + 2 * KC < g.dim) fetch(k + 2 * KC, wv[0]);
+        use(wv[1], 1);
+        if (k + 2 * KC < g.dim) stage(0);
+    }
+    leave_stats<T, NB>(g, v0, r0, tile, acc);
 }
 
 template <int DT, int NB, bool ODD>
@@ -366,7 +456,15 @@ int launch_loss(const FewArgs& g, hipStream_t s) {
 template <int DT>
 int typed_loss(const FewArgs& g, hipStream_t s) {
     if (g.rows <= 16) return launch_loss<DT, 1>(g, s);
-    return g.rows <= 32 ? launch_loss<DT, 2>(g, s) : launch_loss<DT, 4>(g, s);
+    if (g.rows <= 32) return launch_loss<DT, 2>(g, s);
+    if constexpr (DT == MLXHIP_DTYPE_F32) {
+        const int64_t blocks = ceil_div(g.rows, WIDE_ROWS);
+        hipLaunchKernelGGL(wide_stats_kernel, dim3((unsigned)(ceil_div(g.stat_tiles, 8) * 8 * blocks)), dim3(256), 0, s, g,
+                           blocks, g.stat_tiles);
+        return launch_check("wide_stats_kernel");
+    } else {
+        return launch_loss<DT, 4>(g, s);
+    }
 }
 
 template <int DT, int NB>
@@ -385,8 +483,10 @@ int launch_grad(const FewArgs& g, hipStream_t s) {
 }  // namespace
 }  // namespace ce
 
-int64_t ce_few_tiles(int64_t rows, int64_t vocab) {
-    return ceil_div(vocab, rows <= 16 ? ce::ENTRIES<1> : rows <= 32 ? ce::ENTRIES<2> : ce::ENTRIES<4>);
+int64_t ce_few_tiles(int dt, int64_t rows, int64_t vocab) {
+    if (rows <= 16) return ceil_div(vocab, ce::ENTRIES<1>);
+    if (rows <= 32) return ceil_div(vocab, ce::ENTRIES<2>);
+    return ceil_div(vocab, dt == MLXHIP_DTYPE_F32 ? ce::WIDE_ENTRIES : ce::ENTRIES<4>);
 }
 
 int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s) {

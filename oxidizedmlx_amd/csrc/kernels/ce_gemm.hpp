@@ -103,12 +103,14 @@ struct Args {
     int64_t ldc = 0;
 };
 
-// Few rows (ce_few.hip, with what each bound measured): the loss of up to 64 rows
-// (of 16 bits: where the tiles would need a copy of W), the gradients of up to 32
-// f32 rows or 16 of 16 bits. Beyond FEW_VOCAB entries the grids would pass 2^32
+// Few rows (ce_few.hip, with what each bound measured): the loss of up to 128 f32
+// rows, or 64 of 16 bits where the tiles would need a copy of W; the gradients of up
+// to 32 f32 rows, or 16 of 16 bits. Beyond FEW_VOCAB entries the grids would pass 2^32
 // work items and dS^T 512 MiB.
 constexpr int64_t FEW_VOCAB = int64_t(1) << 22;
-inline bool few_loss(bool copy_w, int64_t rows, int64_t vocab) { return copy_w && rows <= 64 && vocab <= FEW_VOCAB; }
+inline bool few_loss(int dt, bool copy_w, int64_t rows, int64_t vocab) {
+    return copy_w && rows <= (dt == MLXHIP_DTYPE_F32 ? 128 : 64) && vocab <= FEW_VOCAB;
+}
 inline bool few_grad(int dt, int64_t rows, int64_t vocab) {
     return rows <= (dt == MLXHIP_DTYPE_F32 ? 32 : 16) && vocab <= FEW_VOCAB;
 }
@@ -576,6 +578,6 @@ int ce_gemm_f32(int which, bool large, const ce::Args& a, hipStream_t s);
 // ce_few.hip
 int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s);
 int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s);
-int64_t ce_few_tiles(int64_t rows, int64_t vocab);  // of the loss's statistics
+int64_t ce_few_tiles(int dt, int64_t rows, int64_t vocab);  // of the loss's statistics
 
 }  // namespace mlxhip

@@ -370,7 +370,7 @@ ce::FewArgs few_args(const Op<OT>& o) {
 template <int OT>
 int few_loss(const Op<OT>& o, float* loss, float* lse) {
     ce::FewArgs g = few_args(o);
-    g.stat_tiles = ce_few_tiles(o.rows, o.vocab);
+    g.stat_tiles = ce_few_tiles(OT, o.rows, o.vocab);
     Carve c;
     const size_t os = c.take((size_t)g.stat_tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4);
     char* ws = nullptr;
@@ -410,7 +410,7 @@ int few_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
 template <int OT>
 int run_loss(const Op<OT>& o, float* loss, float* lse) {
     const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
-    if (ce::few_loss(copy_w, o.rows, o.vocab)) return few_loss(o, loss, lse);
+    if (ce::few_loss(OT, copy_w, o.rows, o.vocab)) return few_loss(o, loss, lse);
     const int64_t width = o.width(false, copy_w);
     // One tile size for all pieces, whose widths are multiples of its columns.
     const bool large = Op<OT>::large(o.rows, o.vocab);
