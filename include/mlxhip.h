@@ -486,10 +486,10 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * (22 bits; scaled by a power of two, absolute error 2^-39 of the operand's largest
  * value where that is more), products below 2^-22 of a term left out.
  * Sums are formed in a fixed order. Operands contiguous, at any address
- * aligned to their elements; results must not overlap operands. A non-finite x
- * or w makes the logits it enters NaN. rows up to 2^21, dim up to 2^20, vocab up
- * to 2^31 - 1, rows times dim (rounded up to a multiple of 8) up to 2^29: cut a
- * larger batch by its rows. The workspace (per stream) holds dS for one piece of
+ * aligned to their elements; results must not overlap operands. A non-finite
+ * value of x reaches its row's results, one of w all rows': they may be NaN.
+ * rows up to 2^21, dim up to 2^20, vocab up to 2^31 - 1, rows times dim (rounded
+ * up to a multiple of 8) up to 2^29: cut a larger batch by its rows. The workspace (per stream) holds dS for one piece of
  * the vocabulary, 256 MiB or 256 columns (the few rows above: of the whole, up to
  * 512 MiB), copies of x and of a piece of w where needed, and f32 sums of dx. No reference counterpart. */
 int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,

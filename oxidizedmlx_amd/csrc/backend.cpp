@@ -13,6 +13,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <functional>
 #include <initializer_list>
 #include <map>
 #include <mutex>
@@ -267,6 +268,8 @@ struct WsCache {
         std::vector<void*> all;
     };
     std::map<std::pair<int, hipStream_t>, Recording> recordings;
+    // Blocks, and their devices, of graphs freed while the device could not be waited for.
+    std::vector<std::pair<int, void*>> freed;
 };
 WsCache& ws_cache() {
     static WsCache* c = new WsCache();  // never destroyed: outlives late calls at exit
@@ -308,6 +311,13 @@ int stream_workspace(hipStream_t s, int slot, size_t bytes, void** out) {
 }
 
 namespace {
+// Held while a call puts several kernels that share a workspace on `s`: another
+// thread's on the same stream then come all before or all behind them.
+std::unique_lock<std::mutex> launches_together(hipStream_t s) {
+    static std::mutex locks[64];
+    return std::unique_lock<std::mutex>(locks[std::hash<const void*>()(s) / 64 % 64]);
+}
+
 // Workspaces asked for on `s` from now on belong to a recording; false if one
 // is under way there already.
 bool begin_recording(hipStream_t s) {
@@ -1209,6 +1219,7 @@ int mlxhip_layernorm_affine_rows(int32_t dtype, const void* x, const void* w, co
     if (cols == 0 || rows == 0) return check_operands("layernorm_affine_rows", dtype, {});
     MLXHIP_TRY(check_operands("layernorm_affine_rows", dtype, {x, w, b, y}));
     MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
     return layernorm_affine(dtype, x, w, b, y, rows, cols, eps, as_stream(stream));
 }
 
@@ -1219,6 +1230,7 @@ int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* 
     if (rows == 0) MLXHIP_TRY(check_operands("layernorm_affine_vjp_rows", dtype, {dw, db}));
     else MLXHIP_TRY(check_operands("layernorm_affine_vjp_rows", dtype, {dy, x, w, dx, dw, db}));
     MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
     return layernorm_affine_vjp(dtype, dy, x, w, dx, dw, db, rows, cols, eps, as_stream(stream));
 }
 
@@ -1242,6 +1254,7 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
     if (n == 0) MLXHIP_TRY(check_operands("embedding_vjp_rows", dtype, {dw}));
     else MLXHIP_TRY(check_operands("embedding_vjp_rows", dtype, {dy, dw}, {ids}));
     MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
     return embedding_vjp_rows(dtype, dy, ids, dw, n, vocab, dim, scale, as_stream(stream));
 }
 
@@ -1263,6 +1276,7 @@ int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, con
     if (rows == 0) return check_operands("linear_cross_entropy", dtype, {});
     MLXHIP_TRY(check_operands("linear_cross_entropy", dtype, {x, w}, {targets, loss, lse}));
     MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
     return linear_cross_entropy(dtype, x, w, targets, loss, lse, rows, dim, vocab, as_stream(stream));
 }
 
@@ -1276,6 +1290,7 @@ int mlxhip_linear_cross_entropy_vjp(int32_t dtype, const void* x, const void* w,
     if (dw) MLXHIP_TRY(check_operands(what, dtype, {dw}));
     if (!dx && !dw) return check_operands(what, dtype, {});
     MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
     return linear_cross_entropy_vjp(dtype, x, w, targets, lse, dloss, dx, dw, rows, dim, vocab, as_stream(stream));
 }
 
@@ -1425,13 +1440,20 @@ int mlxhip_graph_launch(mlxhip_graph_t* g, void* stream) {
 void mlxhip_graph_free(mlxhip_graph_t* g) {
     if (!g) return;
     // Launches may still use the workspaces: they return to the pool once the
-    // device is idle (and stay allocated where that cannot be known).
+    // device is idle. While a stream is recorded that cannot be waited for; they
+    // then return with a graph that is freed later.
     if (!g->blocks.empty()) {
         int cur = 0;
         (void)hipGetDevice(&cur);
         if (cur != g->device) (void)hipSetDevice(g->device);
-        if (hipDeviceSynchronize() == hipSuccess)
-            for (void* p : g->blocks) pool_release(p);
+        WsCache& C = ws_cache();
+        std::lock_guard<std::mutex> l(C.mu);
+        for (void* p : g->blocks) C.freed.emplace_back(g->device, p);
+        if (C.recordings.empty() && hipDeviceSynchronize() == hipSuccess) {
+            auto keep = std::partition(C.freed.begin(), C.freed.end(), [&](const auto& b) { return b.first != g->device; });
+            for (auto it = keep; it != C.freed.end(); ++it) pool_release(it->second);
+            C.freed.erase(keep, C.freed.end());
+        }
         (void)hipGetLastError();
         if (cur != g->device) (void)hipSetDevice(cur);
     }

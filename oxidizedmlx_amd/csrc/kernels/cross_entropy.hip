@@ -15,6 +15,11 @@
 // a last launch scales and rounds. Four products of 2 R D V operations; at
 // several hundred rows the matrix cores bound them.
 //
+// Measured, forward and backward (products and copies; what bounds each product:
+// ce_gemm.hpp): bf16 2048 rows of 1024 over 32000 519 us, 8192 of 2048 over 50257
+// 5.8 ms (1.16 PFLOP/s); f32 2048 of 1024 over 32000 1.63 ms, of which the copies to
+// planes take 60 and the maxima before them 56.
+//
 // x is copied once with zeros in the rows without a target (whatever they hold
 // must not reach dW through a product with 0) and its rows rounded up to whole
 // 16-byte chunks; W is read in place where its rows are such chunks, else

@@ -17,8 +17,13 @@
 // equal shares, one to a wave: a share writes the rows that begin and end in
 // it, and leaves the sums of the ids that cross its borders as partial rows,
 // which a last launch adds up in the order of the shares. Rows of ids that do
-// not occur are zeroed by the launch that begins the sort, on the compute
-// units that the sort leaves idle.
+// not occur are zeroed by the launches of the sort, on the compute units that the
+// sort leaves idle.
+//
+// 65536 bf16 rows of 1024 over 50257: lookup 40 us (134 MB written, 3.4 TB/s, and
+// as much read, the frequent rows from the caches), two passes of the sort 34 with
+// the 103 MB of zeros beside them, sums 51, join 12. 2048 f32 rows over 32000: lookup
+// 7.5, sort 20 (its 131 MB of zeros at 6.5 TB/s), sums 6.3, join 5.1.
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "elem.hpp"

@@ -41,7 +41,7 @@ def check_all(got, x, w, t, dloss, dt, what):
 
 
 SIZES = [(1, 1, 1), (1, 8, 2), (2, 3, 5), (5, 64, 1), (1, 64, 1000), (7, 33, 37), (8, 768, 1003), (16, 128, 256),
-         (16, 2011, 130), (17, 100, 257), (32, 200, 321), (33, 32, 4099), (64, 96, 512), (65, 333, 190), (100, 256, 300), (128, 64, 128), (128, 261, 777), (129, 70, 1025),
+         (16, 2011, 130), (17, 100, 257), (32, 200, 321), (33, 32, 4099), (40, 2, 70), (64, 96, 512), (65, 333, 190), (100, 256, 300), (128, 64, 128), (128, 261, 777), (129, 70, 1025),
          (256, 256, 512), (257, 40, 2001), (300, 520, 777), (513, 288, 1536), (1000, 77, 3203)]
 
 

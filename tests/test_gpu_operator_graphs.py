@@ -2,6 +2,8 @@
 recorded graphs: replays equal the eager results, with eager work in between,
 and two graphs recorded on one stream may replay on two streams at once, as each
 holds its own workspaces."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -156,3 +158,60 @@ def test_a_recording_without_memory_fails_and_leaves_the_stream_usable(streams):
     for a, b in zip(step.results(), want):
         np.testing.assert_array_equal(a, b)
     g.close()
+
+
+@pytest.mark.parametrize("dt", [abi.F32, abi.BF16], ids=R.NAMES.get)
+def test_threads_on_one_stream(streams, dt):
+    """Calls of several threads on one stream share its workspaces, one after
+    the other: the kernels of a call stay together."""
+    steps = [Step(k + 1, 900 + 50 * k, 72, 1003, dt) for k in range(3)]
+    want = []
+    for step in steps:
+        step.run(streams[0])
+        hb.synchronize(streams[0])
+        want.append(step.results())
+    for rep in range(5):
+        for step in steps:
+            step.spoil()
+        hb.synchronize()
+        threads = [threading.Thread(target=lambda step=step: [step.run(streams[0]) for _ in range(4)]) for step in steps]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        hb.synchronize(streams[0])
+        for step, w in zip(steps, want):
+            for a, b in zip(step.results(), w):
+                np.testing.assert_array_equal(a, b, err_msg=f"repetition {rep}")
+
+
+def test_a_graph_freed_while_another_is_recorded(streams):
+    """The recording goes on, and nothing of it changes with the other's workspaces."""
+    s = streams[0]
+    steps = [Step(k + 1, 300, 136, 1003, abi.BF16) for k in range(3)]
+    want = []
+    for step in steps:
+        step.run(s)
+        hb.synchronize(s)
+        want.append(step.results())
+    with hb.Graph(s) as first:
+        steps[0].run(s)
+    first.launch()
+    hb.synchronize(s)
+    with hb.Graph(s) as second:
+        steps[1].run(s)
+        first.close()
+    with hb.Graph(s) as third:
+        steps[2].run(s)
+    for rep in range(3):
+        for step in steps:
+            step.spoil()
+        steps[0].run(s)
+        second.launch()
+        third.launch()
+        hb.synchronize(s)
+        for step, w in zip(steps, want):
+            for a, b in zip(step.results(), w):
+                np.testing.assert_array_equal(a, b, err_msg=f"replay {rep}")
+    second.close()
+    third.close()
