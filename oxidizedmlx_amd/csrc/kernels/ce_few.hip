@@ -230,7 +230,7 @@ __device__ inline void leave_stats(const FewArgs& g, int64_t v0, int64_t r0, int
     float m = red[0][0][r], s = red[0][1][r];
 #pragma unroll
     for (int w = 1; w < 4; ++w) merge(m, s, red[w][0][r], red[w][1][r]);
-    g.stats[(r0 + r) * g.stat_tiles + tile] = make_float2(m, s);
+    g.stats[tile * g.rows + r0 + r] = make_float2(m, s);
 }
 
 template <int DT, int NB, bool ODD>
@@ -458,9 +458,9 @@ int typed_loss(const FewArgs& g, hipStream_t s) {
     if (g.rows <= 16) return launch_loss<DT, 1>(g, s);
     if (g.rows <= 32) return launch_loss<DT, 2>(g, s);
     if constexpr (DT == MLXHIP_DTYPE_F32) {
-        const int64_t blocks = ceil_div(g.rows, WIDE_ROWS);
-        hipLaunchKernelGGL(wide_stats_kernel, dim3((unsigned)(ceil_div(g.stat_tiles, 8) * 8 * blocks)), dim3(256), 0, s, g,
-                           blocks, g.stat_tiles);
+        const int64_t blocks = ceil_div(g.rows, WIDE_ROWS), tiles = ceil_div(g.vocab, WIDE_ENTRIES);
+        hipLaunchKernelGGL(wide_stats_kernel, dim3((unsigned)(ceil_div(tiles, 8) * 8 * blocks)), dim3(256), 0, s, g, blocks,
+                           tiles);
         return launch_check("wide_stats_kernel");
     } else {
         return launch_loss<DT, 4>(g, s);

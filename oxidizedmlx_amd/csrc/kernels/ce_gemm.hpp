@@ -100,8 +100,7 @@ struct Args {
     const int32_t* targets = nullptr;
     int64_t v0 = 0, vocab = 0;  // the piece's first column, the whole vocabulary
     const float *lse = nullptr, *dloss = nullptr;
-    float2* stats = nullptr;    // CE_STATS: [m][stat_tiles], from this launch's first tile on
-    int64_t stat_tiles = 0;
+    float2* stats = nullptr;    // CE_STATS: [tiles of columns][m], from this launch's first tile on
     float* target_z = nullptr;  // CE_STATS: [m]
     uint16_t* ds = nullptr;     // CE_DS: [P][m][ldc]
     float* dx = nullptr;        // CE_DX: [splits][m][ldc]
@@ -128,8 +127,7 @@ struct FewArgs {
     int64_t rows = 0, dim = 0, vocab = 0;
     const int32_t* targets = nullptr;
     const float *lse = nullptr, *dloss = nullptr;
-    float2* stats = nullptr;    // CE_STATS: [rows][stat_tiles]
-    int64_t stat_tiles = 0;
+    float2* stats = nullptr;    // [ce_few_tiles()][rows]
     float* target_z = nullptr;
     float* ds = nullptr;        // dS^T [vocab][few_ds_rows(rows)]
     float* dx = nullptr;        // [slices][rows][ldx] or null
@@ -467,7 +465,7 @@ void ce_gemm_kernel(Args g) {
                 float2 a = make_float2(red[tid], red[C::BM + tid]);
 #pragma unroll
                 for (int w = 1; w < C::WN; ++w) merge(a.x, a.y, red[2 * w * C::BM + tid], red[(2 * w + 1) * C::BM + tid]);
-                g.stats[(m0 + tid) * g.stat_tiles + n0 / C::BN] = a;
+                g.stats[n0 / C::BN * g.m + m0 + tid] = a;
             }
         } else if constexpr (PRODUCT == CE_DS) {
             const float up = g.scale[SCALE_DS], zs = P == 1 ? LOG2E : LOG2E * g.scale[SCALE_Z];

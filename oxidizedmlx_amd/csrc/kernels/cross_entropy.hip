@@ -199,19 +199,33 @@ __global__ __launch_bounds__(256) void maxima_kernel(const float* __restrict__ w
         part[blockIdx.y * MAXIMA + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
-// A row's maxima and sums over the tiles joined, a wave to each row.
-__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t tiles,
-                                                   const float* __restrict__ target_z, const int32_t* __restrict__ targets,
-                                                   int64_t rows, int64_t vocab, float* __restrict__ loss,
-                                                   float* __restrict__ lse) {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
+// A row's maxima and sums over the tiles joined: 16 rows of a workgroup, 64
+// threads to each (16 rows of a tile are a line of stats).
+constexpr int JOIN_ROWS = 16, JOIN = 64;
+__global__ __launch_bounds__(JOIN_ROWS * JOIN) void loss_kernel(const float2* __restrict__ stats, int64_t tiles,
+                                                                const float* __restrict__ target_z,
+                                                                const int32_t* __restrict__ targets, int64_t rows,
+                                                                int64_t vocab, float* __restrict__ loss,
+                                                                float* __restrict__ lse) {
+    __shared__ float2 part[JOIN_ROWS][JOIN + 1];
+    const int k = threadIdx.x / JOIN_ROWS, c = threadIdx.x % JOIN_ROWS;
     float m = -INFINITY, s = 0.0f;
-    for (int64_t t = lane; t < tiles; t += 64) {
-        const float2 a = stats[r * tiles + t];
-        ce::merge(m, s, a.x, a.y);
+    if ((int64_t)blockIdx.x * JOIN_ROWS + c < rows) {
+        const float2* p = stats + (int64_t)blockIdx.x * JOIN_ROWS + c;
+#pragma unroll 4
+        for (int64_t t = k; t < tiles; t += JOIN) {
+            const float2 a = p[t * rows];
+            ce::merge(m, s, a.x, a.y);
+        }
     }
+    part[c][k] = make_float2(m, s);
+    __syncthreads();
+    // A wave to each row.
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t r = (int64_t)blockIdx.x * JOIN_ROWS + w;
+    if (r >= rows) return;
+    m = part[w][lane].x;
+    s = part[w][lane].y;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) ce::merge(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64));
     if (lane) return;
@@ -348,14 +362,18 @@ struct Op {
         w = std::min(w, (int64_t(1) << 43) / rows);
         if (ds) w = std::min(w, PIECE_BYTES / (2 * P) / rows);
         if (copy) w = std::min(w, PIECE_BYTES / (2 * P) / dim_p());
-        return w >= vocab ? vocab : std::max<int64_t>(w / 256 * 256, 256);
+        if (w >= vocab) return vocab;
+        w = std::max<int64_t>(w / 256 * 256, 256);
+        // Pieces of like width: a short last one leaves compute units idle (1105 of
+        // 50257 columns: 160 us of small tiles, 60 in proportion).
+        return ceil_div(ceil_div(vocab, ceil_div(vocab, w)), 256) * 256;
     }
 };
 
 int finish_loss(const float2* stats, int64_t tiles, const float* target_z, const int32_t* targets, int64_t rows,
                 int64_t vocab, float* loss, float* lse, hipStream_t s) {
-    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, s, stats, tiles, target_z, targets, rows,
-                       vocab, loss, lse);
+    hipLaunchKernelGGL(loss_kernel, dim3((unsigned)ceil_div(rows, JOIN_ROWS)), dim3(JOIN_ROWS * JOIN), 0, s, stats, tiles,
+                       target_z, targets, rows, vocab, loss, lse);
     return launch_check("loss_kernel");
 }
 
@@ -375,15 +393,15 @@ ce::FewArgs few_args(const Op<OT>& o) {
 template <int OT>
 int few_loss(const Op<OT>& o, float* loss, float* lse) {
     ce::FewArgs g = few_args(o);
-    g.stat_tiles = ce_few_tiles(OT, o.rows, o.vocab);
+    const int64_t tiles = ce_few_tiles(OT, o.rows, o.vocab);
     Carve c;
-    const size_t os = c.take((size_t)g.stat_tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4);
+    const size_t os = c.take((size_t)tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     g.stats = (float2*)(ws + os);
     g.target_z = (float*)(ws + oz);
     MLXHIP_TRY(ce_few_loss(OT, g, o.s));
-    return finish_loss(g.stats, g.stat_tiles, g.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
+    return finish_loss(g.stats, tiles, g.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
 }
 
 template <int OT>
@@ -435,7 +453,6 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
     a.targets = o.targets;
     a.vocab = o.vocab;
     a.target_z = (float*)(ws + oz);
-    a.stat_tiles = tiles;
     float* scale = (float*)(ws + osc);
     if constexpr (Op<OT>::P > 1) {
         a.scale = scale;
@@ -452,7 +469,7 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
         a.b = copy_w ? (uint16_t*)(ws + ow) : (const uint16_t*)o.w + v0 * o.dim;
         a.b_plane = a.n * o.dim_p();
         a.v0 = v0;
-        a.stats = (float2*)(ws + os) + v0 / bn;
+        a.stats = (float2*)(ws + os) + v0 / bn * o.rows;
         if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, scale + ce::SCALE_W, (uint16_t*)(ws + ow)));
         MLXHIP_TRY(o.product(ce::CE_STATS, large, a));
     }
