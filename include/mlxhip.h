@@ -481,7 +481,7 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * products, scaled so that the largest dloss in magnitude is near 2^15 (small
  * probabilities stay normal; a row whose dloss is that largest one has exact
  * -1 of its target); of up to 16 rows (vocab up to 2^22) it stays f32. F32 products
- * are f32 for the loss of up to 128 rows and the gradients of up to 32 (vocab up to
+ * are f32 for the loss of up to 128 rows and the gradients of up to 64 (vocab up to
  * 2^22); beyond that operands and dS enter the matrix cores as two f16 values each
  * (22 bits; scaled by a power of two, absolute error 2^-39 of the operand's largest
  * value where that is more), products below 2^-22 of a term left out.
@@ -491,7 +491,7 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * rows up to 2^21, dim up to 2^20, vocab up to 2^31 - 1, rows times dim (rounded
  * up to a multiple of 8) up to 2^29: cut a larger batch by its rows. The workspace (per stream) holds dS for one piece of
  * the vocabulary, 256 MiB or 256 columns (the few rows above: of the whole, up to
- * 512 MiB), copies of x and of a piece of w where needed, and f32 sums of dx. No reference counterpart. */
+ * 1 GiB), copies of x and of a piece of w where needed, and f32 sums of dx. No reference counterpart. */
 int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,
                                 float* loss, float* lse, int64_t rows, int64_t dim, int64_t vocab,
                                 void* stream);

@@ -1,6 +1,6 @@
 // ce_few.hip — the linear cross entropy of a few rows (the loss of up to 128 f32
 // rows, or 64 of 16 bits where W's rows are no whole 16-byte chunks; the gradients
-// of up to 32 f32 rows, or 16 of 16 bits), which reading W (and writing dW) bounds:
+// of up to 64 f32 rows, or 16 of 16 bits), which reading W (and writing dW) bounds:
 // W goes from memory straight into the matrix instructions (f32 ones but for the
 // logits of 16-bit operands), with no copies and no planes. dS stays f32: with a few rows one value may make most of a
 // gradient, and its rounding to 16 bits would not average out (one f16 row: dx
@@ -22,8 +22,8 @@
 // Measured over 32000 entries of 1024, f32: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds),
 // 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69. On two f16 planes each
 // (ce_gemm.hpp), whose copies read W twice and write it once before, 1 to 64 rows
-// take 107 - 113 us forward and 157 - 182 backward; the gradients of 64 rows took
-// 191 here, bound by the f32 matrix instructions, and the loss of 256 rows 164 (130).
+// take 107 - 113 us forward and 157 - 190 backward; the gradients of 64 rows 179 (ds
+// 51, grad 124), of 2044 over 50257 550 (650 on planes); the loss of 256 rows 164 (130).
 // bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s), 77 with the loss; the tiles of
 // ce_gemm.hpp take 69 for 17, with errors of dx and dw up to twice as large. The
 // loss where the tiles read W in place: 15 us a call there, 21 here (8 rows of 768
@@ -233,6 +233,27 @@ __device__ inline void leave_stats(const FewArgs& g, int64_t v0, int64_t r0, int
     g.stats[tile * g.rows + r0 + r] = make_float2(m, s);
 }
 
+// dS^T of the same from z.
+template <int T, int NB>
+__device__ inline void leave_ds(const FewArgs& g, int64_t v0, const f32x4 (&acc)[T][NB]) {
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int64_t r = 16 * b + i;
+        const int64_t target = r < g.rows ? g.targets[r] : -1;
+        const bool on = target >= 0 && target < g.vocab;
+        const float lse = on ? g.lse[r] : 0.0f, f = on ? g.dloss[r] : 0.0f;
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t v = v0 + 16 * t + 4 * q + e;
+                const float p = __builtin_amdgcn_exp2f((acc[t][b][e] - lse) * LOG2E) - (v == target ? 1.0f : 0.0f);
+                if (v < g.vocab) g.ds[v * (16 * NB) + r] = on ? p * f : 0.0f;
+            }
+    }
+}
+
 template <int DT, int NB, bool ODD>
 __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
     constexpr int T = TILES<NB>;
@@ -249,7 +270,8 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
 // reaches 154 TFLOP/s). 32 entries a wave, 32 columns a chunk, or two or five waves
 // to a SIMD: 1 - 15 % slower; 128 rows a workgroup: 64 rows take 97 instead of 57.
 constexpr int WIDE_ROWS = 64, WIDE_T = 1, WIDE_ENTRIES = 64 * WIDE_T;
-__global__ __launch_bounds__(256, 4) void wide_stats_kernel(FewArgs g, int64_t row_blocks, int64_t tiles) {
+template <bool DS>
+__global__ __launch_bounds__(256, 4) void wide_kernel(FewArgs g, int64_t row_blocks, int64_t tiles) {
     constexpr int NB = WIDE_ROWS / 16, T = WIDE_T, KC = 64, S = KC / 16, PIECES = WIDE_ROWS * KC / 4 / 256;
     constexpr int DT = MLXHIP_DTYPE_F32;
     __shared__ __attribute__((aligned(16))) float xs[2][WIDE_ROWS][KC + 4];  // 16 rows' quads in different banks
@@ -323,32 +345,18 @@ __global__ __launch_bounds__(256, 4) void wide_stats_kernel(FewArgs g, int64_t r
         use(wv[1], 1);
         if (k + 2 * KC < g.dim) stage(0);
     }
-    leave_stats<T, NB>(g, v0, r0, tile, acc);
+    if constexpr (DS) leave_ds<T, NB>(g, v0, acc);  // of one block of rows
+    else leave_stats<T, NB>(g, v0, r0, tile, acc);
 }
 
 template <int DT, int NB, bool ODD>
 __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
     constexpr int T = TILES<NB>;
-    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
     const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * T;
     if (v0 >= g.vocab) return;
     f32x4 acc[T][NB];
-    few_logits<DT, NB, ODD>(g, v0, lane, acc);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int64_t r = 16 * b + i;
-        const int64_t target = r < g.rows ? g.targets[r] : -1;
-        const bool on = target >= 0 && target < g.vocab;
-        const float lse = on ? g.lse[r] : 0.0f, f = on ? g.dloss[r] : 0.0f;
-#pragma unroll
-        for (int t = 0; t < T; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t v = v0 + 16 * t + 4 * q + e;
-                const float p = __builtin_amdgcn_exp2f((acc[t][b][e] - lse) * LOG2E) - (v == target ? 1.0f : 0.0f);
-                if (v < g.vocab) g.ds[v * (16 * NB) + r] = on ? p * f : 0.0f;
-            }
-    }
+    few_logits<DT, NB, ODD>(g, v0, threadIdx.x & 63, acc);
+    leave_ds<T, NB>(g, v0, acc);
 }
 
 template <int DT, int NB>
@@ -359,11 +367,12 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * COLS + VEC * i;  // the lane's columns
     const int64_t from = ((int64_t)blockIdx.y * 4 + wave) * g.slice, to = min(from + g.slice, g.vocab);
-    // x at k = 4 t + q, columns n0 + j; zeros in rows without a target.
+    // x at row 16 (t / 4) + 4 q + t % 4 (so that a lane reads four of dS^T's values
+    // at once), columns n0 + j; zeros in rows without a target.
     float xr[4 * NB][VEC];
 #pragma unroll
     for (int t = 0; t < 4 * NB; ++t) {
-        const int64_t r = 4 * t + q;
+        const int64_t r = 16 * (t / 4) + 4 * q + t % 4;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) xr[t][j] = 0.0f;
         if (r < g.rows && counted(g.targets[r], g.vocab) && n0 < g.dim)
@@ -374,39 +383,49 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) dx[b][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t v = from; v < to; v += 16) {
+    // 16 entries' values: one block on its way while the other is used.
+    struct Block {
+        dev::Vec16<DT> w[4];
+        float a[4][NB];
+        f32x4 d[NB];
+    } block[2];
+    auto fetch = [&](int64_t v, Block& to_) {
         if (g.dx) {
-            dev::Vec16<DT> w[4];
-            float a[4][NB];
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const int64_t at = v + 4 * s + q;
-                w[s].q = dev::u32x4{0, 0, 0, 0};
-                if (at < to && n0 < g.dim) w[s] = dev::load_raw<DT>(static_cast<const E*>(g.w) + at * g.dim, n0, g.dim);
+                to_.w[s].q = dev::u32x4{0, 0, 0, 0};
+                if (at < to && n0 < g.dim) to_.w[s] = dev::load_raw<DT>(static_cast<const E*>(g.w) + at * g.dim, n0, g.dim);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) a[s][b] = at < to ? g.ds[at * RP + 16 * b + i] : 0.0f;
+                for (int b = 0; b < NB; ++b) to_.a[s][b] = at < to ? g.ds[at * RP + 16 * b + i] : 0.0f;
             }
+        }
+        if (g.dw) {
+            const float* ds = g.ds + min(v + i, g.vocab - 1) * RP + 4 * q;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) to_.d[b] = *reinterpret_cast<const f32x4*>(ds + 16 * b);
+        }
+    };
+    auto use = [&](int64_t v, const Block& from_) {
+        if (g.dx) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 float wf[VEC];
-                dev::unpack<DT>(w[s], wf);
+                dev::unpack<DT>(from_.w[s], wf);
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) dx[b][j] = mfma4(a[s][b], wf[j], dx[b][j]);
+                    for (int j = 0; j < VEC; ++j) dx[b][j] = mfma4(from_.a[s][b], wf[j], dx[b][j]);
             }
         }
         if (g.dw) {
             f32x4 o[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const float* ds = g.ds + min(v + i, g.vocab - 1) * RP + q;
 #pragma unroll
-            for (int t = 0; t < 4 * NB; ++t) {
-                const float a = ds[4 * t];
+            for (int t = 0; t < 4 * NB; ++t)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o[j] = mfma4(a, xr[t][j], o[j]);
-            }
+                for (int j = 0; j < VEC; ++j) o[j] = mfma4(from_.d[t / 4][t % 4], xr[t][j], o[j]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float out[VEC];
@@ -416,6 +435,16 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
                     dev::store_vec<DT>(static_cast<E*>(g.dw) + (v + 4 * q + e) * g.dim, n0, g.dim, out);
             }
         }
+    };
+    if (from < to) fetch(from, block[0]);
+    for (int64_t v = from; v < to; v += 32) {
+        if (v + 16 < to) fetch(v + 16, block[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        use(v, block[0]);
+        if (v + 16 >= to) break;
+        if (v + 32 < to) fetch(v + 32, block[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        use(v + 16, block[1]);
     }
     if (!g.dx) return;
 #pragma unroll
@@ -459,9 +488,9 @@ int typed_loss(const FewArgs& g, hipStream_t s) {
     if (g.rows <= 32) return launch_loss<DT, 2>(g, s);
     if constexpr (DT == MLXHIP_DTYPE_F32) {
         const int64_t blocks = ceil_div(g.rows, WIDE_ROWS), tiles = ceil_div(g.vocab, WIDE_ENTRIES);
-        hipLaunchKernelGGL(wide_stats_kernel, dim3((unsigned)(ceil_div(tiles, 8) * 8 * blocks)), dim3(256), 0, s, g, blocks,
+        hipLaunchKernelGGL((wide_kernel<false>), dim3((unsigned)(ceil_div(tiles, 8) * 8 * blocks)), dim3(256), 0, s, g, blocks,
                            tiles);
-        return launch_check("wide_stats_kernel");
+        return launch_check("wide_kernel");
     } else {
         return launch_loss<DT, 4>(g, s);
     }
@@ -469,11 +498,16 @@ int typed_loss(const FewArgs& g, hipStream_t s) {
 
 template <int DT, int NB>
 int launch_grad(const FewArgs& g, hipStream_t s) {
-    const dim3 grid((unsigned)ceil_div(g.vocab, ENTRIES<NB>));
-    if (DT != MLXHIP_DTYPE_F32 && odd_rows(g))
-        hipLaunchKernelGGL((few_ds_kernel<DT, NB, DT != MLXHIP_DTYPE_F32>), grid, dim3(256), 0, s, g);
-    else
-        hipLaunchKernelGGL((few_ds_kernel<DT, NB, false>), grid, dim3(256), 0, s, g);
+    if constexpr (NB == 4) {
+        const int64_t tiles = ceil_div(g.vocab, WIDE_ENTRIES);
+        hipLaunchKernelGGL((wide_kernel<true>), dim3((unsigned)(ceil_div(tiles, 8) * 8)), dim3(256), 0, s, g, (int64_t)1, tiles);
+    } else {
+        const dim3 grid((unsigned)ceil_div(g.vocab, ENTRIES<NB>));
+        if (DT != MLXHIP_DTYPE_F32 && odd_rows(g))
+            hipLaunchKernelGGL((few_ds_kernel<DT, NB, DT != MLXHIP_DTYPE_F32>), grid, dim3(256), 0, s, g);
+        else
+            hipLaunchKernelGGL((few_ds_kernel<DT, NB, false>), grid, dim3(256), 0, s, g);
+    }
     MLXHIP_TRY(launch_check("few_ds_kernel"));
     hipLaunchKernelGGL((few_grad_kernel<DT, NB>), dim3((unsigned)ceil_div(g.dim, 16 * Elem<DT>::VEC), (unsigned)g.slices),
                        dim3(256), 0, s, g);
@@ -497,7 +531,8 @@ int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s) {
 int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s) {
     if (dt == MLXHIP_DTYPE_BF16) return ce::launch_grad<MLXHIP_DTYPE_BF16, 1>(g, s);
     if (dt == MLXHIP_DTYPE_F16) return ce::launch_grad<MLXHIP_DTYPE_F16, 1>(g, s);
-    return g.rows <= 16 ? ce::launch_grad<MLXHIP_DTYPE_F32, 1>(g, s) : ce::launch_grad<MLXHIP_DTYPE_F32, 2>(g, s);
+    if (g.rows <= 16) return ce::launch_grad<MLXHIP_DTYPE_F32, 1>(g, s);
+    return g.rows <= 32 ? ce::launch_grad<MLXHIP_DTYPE_F32, 2>(g, s) : ce::launch_grad<MLXHIP_DTYPE_F32, 4>(g, s);
 }
 
 }  // namespace mlxhip

@@ -113,14 +113,14 @@ struct Args {
 
 // Few rows (ce_few.hip, with what each bound measured): the loss of up to 128 f32
 // rows, or 64 of 16 bits where the tiles would need a copy of W; the gradients of up
-// to 32 f32 rows, or 16 of 16 bits. Beyond FEW_VOCAB entries the grids would pass 2^32
-// work items and dS^T 512 MiB.
+// to 64 f32 rows, or 16 of 16 bits. Beyond FEW_VOCAB entries the grids would pass 2^32
+// work items and dS^T 1 GiB.
 constexpr int64_t FEW_VOCAB = int64_t(1) << 22;
 inline bool few_loss(int dt, bool copy_w, int64_t rows, int64_t vocab) {
     return copy_w && rows <= (dt == MLXHIP_DTYPE_F32 ? 128 : 64) && vocab <= FEW_VOCAB;
 }
 inline bool few_grad(int dt, int64_t rows, int64_t vocab) {
-    return rows <= (dt == MLXHIP_DTYPE_F32 ? 32 : 16) && vocab <= FEW_VOCAB;
+    return rows <= (dt == MLXHIP_DTYPE_F32 ? 64 : 16) && vocab <= FEW_VOCAB;
 }
 struct FewArgs {
     const void *x = nullptr, *w = nullptr;
@@ -134,7 +134,7 @@ struct FewArgs {
     void* dw = nullptr;         // [vocab][dim] or null
     int64_t ldx = 0, slices = 0, slice = 0;  // of 4 * slice entries each; slice a multiple of 16
 };
-inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
+inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 // Max and sum of exp(z - max) of two groups of a row.
 __device__ inline void merge(float& m, float& s, float m2, float s2) {
