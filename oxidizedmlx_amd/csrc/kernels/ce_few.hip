@@ -22,8 +22,8 @@
 // Measured over 32000 entries of 1024, f32: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds),
 // 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69. On two f16 planes each
 // (ce_gemm.hpp), whose copies read W twice and write it once before, 1 to 64 rows
-// take 107 - 113 us forward and 157 - 190 backward; the gradients of 64 rows 179 (ds
-// 51, grad 124), of 2044 over 50257 550 (650 on planes); the loss of 256 rows 164 (130).
+// take 107 - 113 us forward and 157 - 190 backward; the gradients of 64 rows 164 (ds
+// 52, grad 107), of 2044 over 50257 537 (650 on planes); the loss of 256 rows 164 (130).
 // bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s), 77 with the loss; the tiles of
 // ce_gemm.hpp take 69 for 17, with errors of dx and dw up to twice as large. The
 // loss where the tiles read W in place: 15 us a call there, 21 here (8 rows of 768
@@ -360,23 +360,37 @@ __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
 }
 
 template <int DT, int NB>
-__global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
+__global__ __launch_bounds__(256, 2) void few_grad_kernel(FewArgs g) {
     constexpr int RP = 16 * NB, VEC = Elem<DT>::VEC, COLS = 16 * VEC;
     typedef typename Elem<DT>::type E;
     __shared__ float sums[4][RP][COLS];
+    // 64 rows of x leave no registers for two waves to a SIMD (124 us instead of 107):
+    // LDS holds them.
+    constexpr bool XL = NB == 4;
+    __shared__ __attribute__((aligned(16))) float xs[XL ? RP : 1][COLS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * COLS + VEC * i;  // the lane's columns
     const int64_t from = ((int64_t)blockIdx.y * 4 + wave) * g.slice, to = min(from + g.slice, g.vocab);
     // x at row 16 (t / 4) + 4 q + t % 4 (so that a lane reads four of dS^T's values
     // at once), columns n0 + j; zeros in rows without a target.
-    float xr[4 * NB][VEC];
+    float xr[XL ? 1 : 4 * NB][VEC];
+    auto load_x = [&](int64_t r, int64_t n, float* v) {
 #pragma unroll
-    for (int t = 0; t < 4 * NB; ++t) {
-        const int64_t r = 16 * (t / 4) + 4 * q + t % 4;
+        for (int j = 0; j < VEC; ++j) v[j] = 0.0f;
+        if (r < g.rows && counted(g.targets[r], g.vocab) && n < g.dim)
+            dev::unpack<DT>(dev::load_raw<DT>(static_cast<const E*>(g.x) + r * g.dim, n, g.dim), v);
+    };
+    if constexpr (XL) {
+        for (int k = threadIdx.x * VEC; k < RP * COLS; k += 256 * VEC) {
+            float v[VEC];
+            load_x(k / COLS, (int64_t)blockIdx.x * COLS + k % COLS, v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) xr[t][j] = 0.0f;
-        if (r < g.rows && counted(g.targets[r], g.vocab) && n0 < g.dim)
-            dev::unpack<DT>(dev::load_raw<DT>(static_cast<const E*>(g.x) + r * g.dim, n0, g.dim), xr[t]);
+            for (int j = 0; j < VEC; ++j) xs[k / COLS][k % COLS + j] = v[j];
+        }
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4 * NB; ++t) load_x(16 * (t / 4) + 4 * q + t % 4, n0, xr[t]);
     }
     f32x4 dx[NB][VEC];
 #pragma unroll
@@ -423,9 +437,11 @@ __global__ __launch_bounds__(256) void few_grad_kernel(FewArgs g) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int t = 0; t < 4 * NB; ++t)
+            for (int t = 0; t < 4 * NB; ++t) {
+                const float* x = XL ? &xs[16 * (t / 4) + 4 * q + t % 4][VEC * i] : xr[XL ? 0 : t];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) o[j] = mfma4(from_.d[t / 4][t % 4], xr[t][j], o[j]);
+                for (int j = 0; j < VEC; ++j) o[j] = mfma4(from_.d[t / 4][t % 4], x[j], o[j]);
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float out[VEC];

@@ -61,7 +61,7 @@ def test_any_element_alignment(rows, dim, vocab, offset, dt):
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("rows", [5, 40, 300])
 def test_rows_without_a_target(rows, dt):
     """Whatever x and dloss hold there: loss 0, dx 0, nothing in dw; with no
     row left all gradients are 0."""
@@ -85,7 +85,7 @@ def test_rows_without_a_target(rows, dt):
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-@pytest.mark.parametrize("rows", [3, 260])
+@pytest.mark.parametrize("rows", [3, 50, 260])
 def test_far_apart_logits(rows, dt):
     """Logits of some thousands: one probability of 1 and the rest 0, or far
     beyond the range of exp without the maximum taken off."""
@@ -104,7 +104,7 @@ def test_far_apart_logits_with_other_targets(rows, dt):
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-@pytest.mark.parametrize("rows,dim", [(5, 64), (270, 264)])
+@pytest.mark.parametrize("rows,dim", [(5, 64), (50, 77), (270, 264)])
 def test_values_of_very_different_size(rows, dim, dt):
     """Elements, rows and dloss over some twenty binary orders of magnitude
     (f32 and f16 hold their small parts scaled), a vocabulary entry that is all
@@ -160,12 +160,20 @@ def test_few_rows_of_millions_of_entries(vocab, dt):
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-@pytest.mark.parametrize("rows", [6, 300])
+@pytest.mark.parametrize("rows", [6, 40, 300])
 def test_one_gradient_alone(rows, dt):
     a = inputs(rows, 72, 700, dt)
     both = run(*a, dt)
     np.testing.assert_array_equal(run(*a, dt, want="x")[2], both[2])
     np.testing.assert_array_equal(run(*a, dt, want="w")[3], both[3])
+
+
+@pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
+@pytest.mark.parametrize("rows", [6, 40, 300])
+def test_a_cotangent_of_zeros(rows, dt):
+    x, w, t, g = inputs(rows, 72, 700, dt)
+    got = run(x, w, t, np.zeros_like(g), dt)
+    assert not got[2].any() and not got[3].any()
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
