@@ -456,7 +456,7 @@ int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* 
  * an order that only the ids fix (no atomics: the same bits every time).
  * Operands contiguous, at any address aligned to their elements; results must
  * not overlap operands. n and vocab up to 2^31 - 1, dim up to 2^20. The
- * gradient sorts the positions by id in a per-stream workspace (8 or 16
+ * gradient of over 64 ids sorts their positions in a per-stream workspace (8 or 16
  * bytes per id and 4096 rows of dim f32 sums at most). No reference
  * counterpart for the gradient (crates/mlx-autograd/src/vjp.rs:173-176). */
 int mlxhip_embedding_rows(int32_t dtype, const void* w, const int32_t* ids, void* y, int64_t n,

@@ -51,14 +51,15 @@ def test_matches_64_bits(n, vocab, dim, dt):
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 @pytest.mark.parametrize("dim,offset", [(777, 1), (64, 3), (7, 5)])
-def test_any_element_alignment(dim, offset, dt):
-    ids = words(5, 300, 50)
-    w, dy = R.rounded(synth.normal(1, (50, dim)), dt), R.rounded(synth.normal(2, (300, dim)), dt)
+@pytest.mark.parametrize("n", [50, 300])
+def test_any_element_alignment(n, dim, offset, dt):
+    ids = words(5, n, 50)
+    w, dy = R.rounded(synth.normal(1, (50, dim)), dt), R.rounded(synth.normal(2, (n, dim)), dt)
     R.check(forward(w, ids, 0.25, dt, offset), *R.embedding(w, ids, 0.25, dt), "y")
     R.check(gradient(dy, ids, 50, 0.25, dt, offset), *R.embedding_vjp(dy, ids, 50, 0.25, dt), "dw")
 
 
-@pytest.mark.parametrize("n", [5, 4000, 20000])
+@pytest.mark.parametrize("n", [5, 60, 4000, 20000])
 def test_ids_out_of_range_are_clamped(n):
     ids = words(9, n, 40)
     ids[::5] = -1
@@ -70,7 +71,7 @@ def test_ids_out_of_range_are_clamped(n):
     R.check(gradient(dy, ids, 40, 2.0, abi.F32), *R.embedding_vjp(dy, ids, 40, 2.0, abi.F32), "dw")
 
 
-@pytest.mark.parametrize("n", [1, 3, 2000, 16384, 30000])
+@pytest.mark.parametrize("n", [1, 3, 63, 64, 65, 2000, 16384, 30000])
 @pytest.mark.parametrize("kind", ["one id", "descending", "each once", "two ids"])
 def test_runs_across_every_share(n, kind):
     """All positions one id (a run across every share), every id once, orders
@@ -129,7 +130,7 @@ def test_no_tokens():
     assert not D.get().any()
 
 
-@pytest.mark.parametrize("n", [900, 25000])
+@pytest.mark.parametrize("n", [60, 900, 25000])
 def test_same_bits_every_time_and_on_another_stream(n):
     ids, dy = words(3, n, 5000), R.rounded(synth.normal(4, (n, 100)), abi.BF16)
     one = gradient(dy, ids, 5000, 3.0, abi.BF16)
