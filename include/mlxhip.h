@@ -477,20 +477,19 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * NULL: that gradient is then not formed.
  * dtype: F32, BF16 or F16, of x, w, dx and dw; loss, lse and dloss are f32, as
  * are the logits, sums and products' accumulators. dx and dw are rounded once,
- * as they are stored. dS of 16-bit operands is rounded to their type for its
- * products, scaled so that the largest dloss in magnitude is near 2^15 (small
- * probabilities stay normal; a row whose dloss is that largest one has exact
- * -1 of its target); of up to 16 rows (vocab up to 2^22) it stays f32. F32 products
- * are f32 for the loss of up to 128 rows and the gradients of up to 64 (vocab up to
- * 2^22); beyond that operands and dS enter the matrix cores as two f16 values each
- * (22 bits; scaled by a power of two, absolute error 2^-39 of the operand's largest
- * value where that is more), products below 2^-22 of a term left out.
+ * as they are stored. F32 products are f32 for the loss of up to 128 rows and the
+ * gradients of up to 64 (vocab up to 2^22). Beyond that the logits are formed of
+ * operands of 22 bits each, with an absolute error of 2^-39 of the largest value of
+ * the same row of x or w where that is more, products below 2^-22 of a term left out,
+ * and the gradients of operands and dS of 24 bits of any size. dS of 16-bit operands is
+ * held to 16 bits (bf16) or 22 with a floor of 2^-40 of its row's dloss (f16, where
+ * dw's terms dloss x have a floor of 2^-39 of the largest), f32 for up to 16 rows.
  * Sums are formed in a fixed order. Operands contiguous, at any address
  * aligned to their elements; results must not overlap operands. A non-finite
  * value of x reaches its row's results, one of w all rows': they may be NaN.
  * rows up to 2^21, dim up to 2^20, vocab up to 2^31 - 1, rows times dim (rounded
  * up to a multiple of 8) up to 2^29: cut a larger batch by its rows. The workspace (per stream) holds dS for one piece of
- * the vocabulary, 256 MiB or 256 columns (the few rows above: of the whole, up to
+ * the vocabulary, 512 MiB or 256 columns (the few rows above: of the whole, up to
  * 1 GiB), copies of x and of a piece of w where needed, and f32 sums of dx. No reference counterpart. */
 int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,
                                 float* loss, float* lse, int64_t rows, int64_t dim, int64_t vocab,

@@ -4,7 +4,7 @@
 namespace mlxhip {
 
 int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s) {
-    return ce::dispatch<MLXHIP_DTYPE_BF16, MLXHIP_DTYPE_BF16, 1>(which, large, a, s);
+    return ce::dispatch<MLXHIP_DTYPE_BF16>(which, large, a, s);
 }
 
 }  // namespace mlxhip

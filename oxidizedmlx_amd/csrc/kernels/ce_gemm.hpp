@@ -5,28 +5,47 @@
 //             exp(z - max), and the target's logit: the logits leave the
 //             registers only as these.
 //   CE_DS     z again; dS = exp(z - lse) - [v = target], times the row's
-//             factor, stored in 16 bits (f32: as two f16 planes).
+//             dloss, stored as two 16-bit planes (f32 operands: three).
 //   CE_DX     f32 sums of dS W over a slice of K, added to those of the
 //             pieces of the vocabulary before.
-//   CE_DW     dS^T x times a power of two, in the operands' type.
+//   CE_DW     dS^T x, in the operands' type.
 //
-// Operands are bf16 or f16, or f32 as two f16 planes of the value times a power
-// of two (P = 2): hi is the value rounded to f16, lo what it leaves, rounded, so
-// hi + lo holds 22 bits of every value above 2^-18 of the largest (scaled to
-// 2^15), and the three products hi hi + hi lo + lo hi leave out less than
-// 2^-22 of a term. That is within what f32 sums of some hundred terms are off
-// by anyway, at half the matrix operations of the exact split into three bf16
-// planes (six products, gemm16_x6.hip: 2048 x 1024 over 32000 forward and
-// backward 2.80 ms). Tiles are fed by direct global->LDS loads, STAGES K tiles
+// A plane is a 16-bit value: hi is the f32 value rounded, the next plane what that
+// leaves, rounded. The products run over pairs of planes, those whose places add
+// up to the last plane's, smallest first.
+//
+// z of 16-bit operands takes them as they are. z of f32 operands is formed from
+// two f16 planes (22 bits) of x and W, each row of either times a power of two that
+// brings its largest magnitude to between 2^14 and 2^15: a value keeps 22 bits
+// down to 2^-18 of its row's largest, and what is lost below is 2^-39 of that. The
+// three products hi hi + hi lo + lo hi leave out less than 2^-22 of a term. That is
+// within what f32 sums of some hundred terms are off by anyway.
+//
+// The gradients of f32 and bf16 operands take bf16 planes, which have f32's range
+// and need no scale, so that a row, a vocabulary entry or a dloss of any size keeps
+// its digits beside others far larger: dS^T's rows of improbable words are sums of
+// values of 2^-40 and less. f32 operands and their dS are three planes (24 bits, six
+// products); bf16 operands are read as they are against two planes of dS (16 bits, two
+// products). Those of f16 operands take f16 planes: dS without dloss, times
+// 2^15, in two (22 bits, a floor of 2^-40), against W as it is (two products; dloss
+// follows in dx's last launch) and against two planes of dloss x on one scale (three
+// products), whose floor of 2^-40 of the largest is below an f16 result's own.
+// Two f16 planes on one scale each for W, x and dloss took half the time for f32
+// gradients and lost all digits of what lies 2^-40 below the largest; dS in one
+// plane of the operands' type took half the time for 16-bit ones, whose errors beside
+// the results' own rounding were as large as that.
+//
+// Tiles are fed by direct global->LDS loads, STAGES K tiles
 // of 32 deep, with the building blocks and LDS layouts of gemm16_impl.hpp; workgroups
 // stay and walk over tiles, the next tile's loads on their way during an epilogue
 // that has LDS of its own.
 //
-// Bound by the matrix cores. 2048 rows of 1024 over 32000 (134 GFLOP a product):
-// bf16 114 - 135 us each (stats 128, dS 135, dx 117, dW 114: 1.0 - 1.18 PFLOP/s,
-// where a library product of 8192^3 reaches 1.17), f32 335 - 404 (three times the
-// matrix operations: 1.0 - 1.2 PFLOP/s of them). 1000 rows of 777 over 32003, f16:
-// 60 - 67 us each, 0.74 - 0.83 PFLOP/s: 504 tiles of 256 x 256 on 256 compute
+// Bound by the matrix cores. 2048 rows of 1024 over 32000 (134 GFLOP a product of one
+// pair of planes; a library product of 8192^3 reaches 1.17 PFLOP/s), in a trace: bf16
+// stats 152 us, dS 190 (262 MB of its planes stored), dx 253 and dW 246 of two pairs
+// each (1.06 - 1.09 PFLOP/s); f32 stats 374, dS 434 of three pairs, dx 650 and dW 667
+// of six (1.2 PFLOP/s). 1000 rows of 777 over 32003, f16: stats 67, dS 84, dx 120 of
+// two pairs, dW 165 of three, 0.6 - 0.9 PFLOP/s: 504 tiles of 256 x 256 on 256 compute
 // units, of 25 steps of K each, so a workgroup's first loads and last epilogue weigh more.
 #pragma once
 
@@ -46,46 +65,82 @@ enum Product { CE_STATS = 0, CE_DS = 1, CE_DX = 2, CE_DW = 3 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// WM x WN waves of TM x TN 32x32 tiles, P planes of both operands in each of
+// WM x WN waves of TM x TN 32x32 tiles, PA planes of A and PB of B in each of
 // STAGES stages.
-template <int WM_, int WN_, int TM_, int TN_, int STAGES_, int P_>
+template <int WM_, int WN_, int TM_, int TN_, int STAGES_, int PA_, int PB_>
 struct Cfg {
-    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, STAGES = STAGES_, P = P_;
+    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, STAGES = STAGES_, PA = PA_, PB = PB_;
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;  // one plane of one stage
-    static constexpr int STAGE_BYTES = P * (A_BYTES + B_BYTES);         // A's planes, then B's
+    static constexpr int STAGE_BYTES = PA * A_BYTES + PB * B_BYTES;     // A's planes, then B's
     static constexpr int LA = A_BYTES / (THREADS * 16), LB = B_BYTES / (THREADS * 16);  // loads per thread and plane
     static_assert(BM >= 128 && BN >= 128, "MN-contiguous LDS rows need >= 16 chunks for the swizzle");
     static_assert(LA * THREADS * 16 == A_BYTES && LB * THREADS * 16 == B_BYTES, "whole 1 KiB blocks per wave");
     // LDS of the epilogue per wave, and workgroups to a compute unit.
-    static constexpr int EPI = P == 1 ? 4096 : 2048;
+    static constexpr int EPI = PA == 1 ? 4096 : 2048;
     static constexpr int LDS = STAGES * STAGE_BYTES + WAVES * EPI, PER_CU = 160 * 1024 / LDS;
     static_assert(STAGES >= 2 && LDS <= 160 * 1024, "LDS budget");
     static_assert(WN * 2 * BM * 4 <= WAVES * EPI, "row statistics of a tile");
 };
-template <int P>
-using Large = std::conditional_t<P == 1, Cfg<2, 4, 4, 2, 4, 1>, Cfg<4, 2, 2, 2, 3, 2>>;  // 256 x 256, 256 x 128
-template <int P>
-using Small = std::conditional_t<P == 1, Cfg<2, 2, 2, 2, 4, 1>, Cfg<2, 4, 2, 1, 4, 2>>;  // 128 x 128, two to a CU / one
-
-// Factors of the products' operands and results; those of planes are powers of
-// two.
-enum Scale {
-    SCALE_DW = 0,  // dW is this times dS^T x
-    SCALE_DS = 1,  // dS is formed from dloss times this
-    SCALE_Z = 2,   // z is this times the product (CE_STATS: and times row_scale)
-    SCALE_DX = 3,  // dx is this times dS W
-    SCALE_X = 4,   // planes hold this times x
-    SCALE_W = 5,   // and this times W
-    SCALES = 6
+// The tiles of a product of PA and PB planes: 256 x 256 or, where each operand has
+// several planes, 256 x 128; and 128 x 128 (one plane of B: two workgroups to a
+// compute unit).
+template <int PA, int PB>
+struct Tiling;
+template <>
+struct Tiling<1, 1> {
+    using Large = Cfg<2, 4, 4, 2, 4, 1, 1>;
+    using Small = Cfg<2, 2, 2, 2, 4, 1, 1>;
+};
+template <>
+struct Tiling<2, 1> {
+    using Large = Cfg<4, 2, 2, 4, 3, 2, 1>;
+    using Small = Cfg<2, 2, 2, 2, 3, 2, 1>;
+};
+template <>
+struct Tiling<2, 2> {
+    using Large = Cfg<4, 2, 2, 2, 3, 2, 2>;
+    using Small = Cfg<2, 4, 2, 1, 4, 2, 2>;
+};
+template <>
+struct Tiling<3, 3> {
+    using Large = Cfg<4, 2, 2, 2, 2, 3, 3>;
+    using Small = Cfg<2, 4, 2, 1, 3, 3, 3>;
 };
 
-// The planes of product e: smallest first, hi hi last.
-template <int P>
-__host__ __device__ constexpr int plane_of_a(int e) { return P == 2 && e == 0; }
-template <int P>
-__host__ __device__ constexpr int plane_of_b(int e) { return P == 2 && e == 1; }
+// The pairs of planes of a product, smallest first: of PA and PB planes those with
+// i + j < PA.
+template <int PA, int PB>
+struct Pairs {
+    int n = 0, a[6] = {}, b[6] = {};
+    constexpr Pairs() {
+        for (int sum = PA - 1; sum >= 0; --sum)
+            for (int i = sum; i >= 0; --i)
+                if (sum - i < PB) {
+                    a[n] = i;
+                    b[n] = sum - i;
+                    ++n;
+                }
+    }
+};
+
+// Planes of the operands in the logits' product and their type; of dS, x and W in the
+// gradients' and their type.
+template <int OT>
+constexpr int Z_PLANES = OT == MLXHIP_DTYPE_F32 ? 2 : 1;
+template <int OT>
+constexpr int Z_TYPE = OT == MLXHIP_DTYPE_F32 ? MLXHIP_DTYPE_F16 : OT;
+template <int OT>
+constexpr int DS_PLANES = OT == MLXHIP_DTYPE_F32 ? 3 : 2;
+template <int OT>
+constexpr int X_PLANES = OT == MLXHIP_DTYPE_F32 ? 3 : OT == MLXHIP_DTYPE_F16 ? 2 : 1;
+template <int OT>
+constexpr int W_PLANES = OT == MLXHIP_DTYPE_F32 ? 3 : 1;
+template <int OT>
+constexpr int G_TYPE = OT == MLXHIP_DTYPE_F16 ? MLXHIP_DTYPE_F16 : MLXHIP_DTYPE_BF16;
+// dS of f16 operands is without dloss and times this.
+constexpr float DS_F16 = 0x1p15f;
 
 struct Args {
     // op(A) [m, k], op(B) [k, n]; planes of an operand *_plane elements apart.
@@ -102,12 +157,14 @@ struct Args {
     const float *lse = nullptr, *dloss = nullptr;
     float2* stats = nullptr;    // CE_STATS: [tiles of columns][m], from this launch's first tile on
     float* target_z = nullptr;  // CE_STATS: [m]
-    uint16_t* ds = nullptr;     // CE_DS: [P][m][ldc]
+    uint16_t* ds = nullptr;     // CE_DS: [DS_PLANES][m][ldc]
     float* dx = nullptr;        // CE_DX: [splits][m][ldc]
     bool add = false;           // CE_DX: add to what is there
     void* dw = nullptr;         // CE_DW: [m][ldc]
-    const float* scale = nullptr;  // Scale's factors (not for CE_STATS of 16-bit operands, CE_DX)
-    const float* row_scale = nullptr;  // CE_STATS of planes: x is row_scale[r] times its planes
+    // z of planes: x's row r is row_scale[r] times its planes, W's row v
+    // col_scale[v - v0] times its (room for a multiple of 256 columns).
+    const float *row_scale = nullptr, *col_scale = nullptr;
+    const float* scale = nullptr;  // CE_DW of f16 operands: dW is *scale times the product
     int64_t ldc = 0;
 };
 
@@ -269,7 +326,22 @@ __device__ inline void store_tile(const f32x16 (&acc)[C::TM][C::TN], MLXHIP_LDS 
         }
 }
 
-// MT: type of the planes (BF16, F16); OT: type of the operator's operands.
+// acc's columns times col_scale (from the lane's first column on).
+template <int TM, int TN>
+__device__ inline void scale_columns(f32x16 (&acc)[TM][TN], const float* col_scale) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 c = *reinterpret_cast<const f32x4*>(col_scale + 32 * j + 8 * q);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] *= c[e];
+        }
+}
+
+// MT: type of the operands' planes (BF16, F16); OT: type of the operator's operands.
 //
 // A workgroup runs through its tiles without draining its loads: behind a
 // tile's last K tile come the first of the next one, which land while the
@@ -278,8 +350,8 @@ template <int PRODUCT, int MT, int OT, class C>
 __global__ __attribute__((amdgpu_flat_work_group_size(C::THREADS, C::THREADS), amdgpu_waves_per_eu(2, 2)))
 void ce_gemm_kernel(Args g) {
     constexpr bool KCA = PRODUCT != CE_DW, KCB = PRODUCT <= CE_DS;
-    constexpr int STAGES = C::STAGES, TM = C::TM, TN = C::TN, WAVES = C::WAVES, P = C::P;
-    constexpr int PAIRS = 2 * P - 1;
+    constexpr int STAGES = C::STAGES, TM = C::TM, TN = C::TN, WAVES = C::WAVES, PA = C::PA, PB = C::PB;
+    constexpr Pairs<PA, PB> pairs;
     __shared__ __attribute__((aligned(1024))) char smem_raw[STAGES * C::STAGE_BYTES + WAVES * C::EPI];
     MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw;
     MLXHIP_LDS char* epi = smem + STAGES * C::STAGE_BYTES;
@@ -304,8 +376,8 @@ void ce_gemm_kernel(Args g) {
     int lat = list.at, lk = 0, lnk = 0;
     auto seek = [&] {
         const Tile t = tile_of<PRODUCT, C>(g, lat);
-        ra = operand<KCA, C::BM, P>(g.a, g.a_plane, g.lda, t.m0, g.m, t.k0, t.ka);
-        rb = operand<KCB, C::BN, P>(g.b, g.b_plane, g.ldb, t.n0, g.n, t.k0, t.kb);
+        ra = operand<KCA, C::BM, PA>(g.a, g.a_plane, g.lda, t.m0, g.m, t.k0, t.ka);
+        rb = operand<KCB, C::BN, PB>(g.b, g.b_plane, g.ldb, t.n0, g.n, t.k0, t.kb);
         la.init(tid, 0, g.m - t.m0, g.lda, t.ka);
         lb.init(tid, 0, g.n - t.n0, g.ldb, t.kb);
         lk = 0;
@@ -319,29 +391,28 @@ void ce_gemm_kernel(Args g) {
     auto next_k = [&] { return lat < list.end ? lk * BK : INT32_MAX; };
     seek();
 
-    constexpr int LA = C::LA, LB = C::LB, LPT = P * (LA + LB), B0 = P * C::A_BYTES;
+    constexpr int LA = C::LA, LB = C::LB, LPT = PA * LA + PB * LB, B0 = PA * C::A_BYTES;
 #pragma unroll
     for (int t = 0; t < STAGES; ++t) {
         MLXHIP_LDS char* st = smem + t * C::STAGE_BYTES;
         const int k = next_k();
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            la.issue(ra, st + p * C::A_BYTES, wave, k, (uint32_t)p * plane_a);
-            lb.issue(rb, st + B0 + p * C::B_BYTES, wave, k, (uint32_t)p * plane_b);
-        }
+        for (int p = 0; p < PA; ++p) la.issue(ra, st + p * C::A_BYTES, wave, k, (uint32_t)p * plane_a);
+#pragma unroll
+        for (int p = 0; p < PB; ++p) lb.issue(rb, st + B0 + p * C::B_BYTES, wave, k, (uint32_t)p * plane_b);
         next();
     }
     gemm16::wait_vmcnt<(STAGES - 1) * LPT>();
     gemm16::lds_barrier();
 
-    constexpr int NA = KCA ? TM : 2 * TM, NB = KCB ? TN : 2 * TN, NR = P * (NA + NB);
-    u32x4 af[2][P][TM], bf[2][P][TN];
+    constexpr int NA = KCA ? TM : 2 * TM, NB = KCB ? TN : 2 * TN, NR = PA * NA + PB * NB;
+    u32x4 af[2][PA][TM], bf[2][PB][TN];
     auto read_op = [&](const MLXHIP_LDS char* st, int s, int o) {
-        if (o < P * NA) {
+        if (o < PA * NA) {
             const int p = o / NA;
             gemm16::read_one<KCA, TM, ROWB_A>(st + p * C::A_BYTES, fa, s, o - p * NA, af[s][p]);
         } else {
-            const int ob = o - P * NA, p = ob / NB;
+            const int ob = o - PA * NA, p = ob / NB;
             gemm16::read_one<KCB, TN, ROWB_B>(st + B0 + p * C::B_BYTES, fb, s, ob - p * NB, bf[s][p]);
         }
     };
@@ -362,13 +433,13 @@ void ce_gemm_kernel(Args g) {
 
         // Per K tile two steps of 16: each step's MFMAs with the next step's LDS
         // reads, and in the second the loads of the K tile STAGES on, between them.
-        constexpr int NM = TM * TN, NMI = PAIRS * NM, OPS = NR + LPT;
+        constexpr int NM = TM * TN, NMI = pairs.n * NM, OPS = NR + LPT;
         for (int kt = 0; kt < nk; ++kt) {
             const MLXHIP_LDS char* st = smem + cur * C::STAGE_BYTES;
 #pragma unroll
             for (int q = 0; q < NMI; ++q) {
                 const int e = q / NM, t = q % NM;
-                gemm16::mfma<MT>(bf[0][plane_of_b<P>(e)][t % TN], af[0][plane_of_a<P>(e)][t / TN], acc[t / TN][t % TN]);
+                gemm16::mfma<MT>(bf[0][pairs.b[e]][t % TN], af[0][pairs.a[e]][t / TN], acc[t / TN][t % TN]);
                 constexpr bool ONE = NR <= NMI;  // a read a step, the first ones first
 #pragma unroll
                 for (int o = ONE ? min(q, NR) : (q * NR) / NMI; o < (ONE ? min(q + 1, NR) : ((q + 1) * NR) / NMI); ++o)
@@ -387,16 +458,16 @@ void ce_gemm_kernel(Args g) {
 #pragma unroll
             for (int q = 0; q < NMI; ++q) {
                 const int e = q / NM, t = q % NM;
-                gemm16::mfma<MT>(bf[1][plane_of_b<P>(e)][t % TN], af[1][plane_of_a<P>(e)][t / TN], acc[t / TN][t % TN]);
+                gemm16::mfma<MT>(bf[1][pairs.b[e]][t % TN], af[1][pairs.a[e]][t / TN], acc[t / TN][t % TN]);
 #pragma unroll
                 for (int o = (q * OPS) / NMI; o < ((q + 1) * OPS) / NMI; ++o) {
                     if (o < NR) {
                         read_op(nx, 0, o);
-                    } else if (o < NR + P * LA) {
+                    } else if (o < NR + PA * LA) {
                         const int p = (o - NR) / LA;
                         la.issue_one(ra, dst + p * C::A_BYTES, wave, kl, o - NR - p * LA, (uint32_t)p * plane_a);
                     } else {
-                        const int ob = o - NR - P * LA, p = ob / LB;
+                        const int ob = o - NR - PA * LA, p = ob / LB;
                         lb.issue_one(rb, dst + B0 + p * C::B_BYTES, wave, kl, ob - p * LB, (uint32_t)p * plane_b);
                     }
                 }
@@ -413,11 +484,11 @@ void ce_gemm_kernel(Args g) {
         if constexpr (PRODUCT == CE_STATS) {
             MLXHIP_LDS float* red = (MLXHIP_LDS float*)epi;  // [WN][2][BM]
             const bool edge = n0 + C::BN > g.n;
-            const float zs = P == 1 ? 1.0f : g.scale[SCALE_Z];
+            if constexpr (PA > 1) scale_columns(acc, g.col_scale + col0);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 const int64_t r = row0 + 32 * i;
-                const float f = P == 1 || r >= g.m ? 1.0f : zs * g.row_scale[r];
+                const float f = PA == 1 || r >= g.m ? 1.0f : g.row_scale[r];
                 // The target's logit, from the lane that holds its column.
                 const int tc = r < g.m ? column_of(g.targets[r], g.v0 + col0, 32 * TN) : -1;
                 const bool mine = tc >= 0 && (tc & 4) == 0 && tc + col0 < g.n;
@@ -468,33 +539,40 @@ void ce_gemm_kernel(Args g) {
                 g.stats[n0 / C::BN * g.m + m0 + tid] = a;
             }
         } else if constexpr (PRODUCT == CE_DS) {
-            const float up = g.scale[SCALE_DS], zs = P == 1 ? LOG2E : LOG2E * g.scale[SCALE_Z];
+            if constexpr (PA > 1) scale_columns(acc, g.col_scale + col0);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 const int64_t r = row0 + 32 * i;
-                // A row without a target has zeros in x, so z = 0: with lse taken
-                // as infinite its dS is 0 whatever lse and dloss hold.
-                float shift = -INFINITY, f = 0.0f;
+                float shift = 0.0f, f = 0.0f, up = LOG2E;
                 int tc = -1;
                 if (r < g.m) {
                     const int32_t t = g.targets[r];
                     if (counted(t, g.vocab)) {
                         shift = -g.lse[r] * LOG2E;
-                        f = g.dloss[r] * up;
+                        f = OT == MLXHIP_DTYPE_F16 ? DS_F16 : g.dloss[r];
                     }
+                    if constexpr (PA > 1) up *= g.row_scale[r];
                     tc = column_of(t, g.v0 + col0, 32 * TN);
                 }
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
-                        acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], zs, shift)) * f;
+                        acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], up, shift)) * f;
                 if (__ballot(tc >= 0)) {  // some lane holds its row's target
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int v = 0; v < 16; ++v)
                             if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) acc[i][j][v] -= f;
+                }
+                // A row without a target has no dS, whatever x, lse and dloss hold.
+                const bool on = r < g.m && counted(g.targets[r], g.vocab);
+                if (__ballot(!on)) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) acc[i][j][v] = on ? acc[i][j][v] : 0.0f;
                 }
             }
             if (n0 + C::BN > g.n) {
@@ -506,11 +584,12 @@ void ce_gemm_kernel(Args g) {
 #pragma unroll
                             for (int i = 0; i < TM; ++i) acc[i][j][v] = 0.0f;
             }
+            constexpr int GT = G_TYPE<OT>, SP = DS_PLANES<OT>;
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                store_tile<MT, C, false, false>(acc, region, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, wrow, wcol, lane,
-                                                false);
-                if (p + 1 < P) {
+            for (int p = 0; p < SP; ++p) {
+                store_tile<GT, C, false, false>(acc, region, g.ds + p * g.m * g.ldc, g.ldc, g.m, g.ldc, g.ldc, wrow, wcol,
+                                                  lane, false);
+                if (p + 1 < SP) {
                     // What the plane leaves (exact in f32).
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
@@ -518,24 +597,24 @@ void ce_gemm_kernel(Args g) {
                         for (int j = 0; j < TN; ++j)
 #pragma unroll
                             for (int v = 0; v < 16; ++v)
-                                acc[i][j][v] -= dev::to_f32<MT>(dev::from_f32<MT>(acc[i][j][v]));
+                                acc[i][j][v] -= dev::to_f32<GT>(dev::from_f32<GT>(acc[i][j][v]));
                 }
             }
-        } else {
-            if constexpr (PRODUCT == CE_DW) {
-                const float f = g.scale[SCALE_DW];
+        } else if constexpr (PRODUCT == CE_DW) {
+            if constexpr (OT == MLXHIP_DTYPE_F16) {
+                const float f = *g.scale;
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) acc[i][j][v] *= f;
-                store_tile<OT, C, false, true>(acc, region, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m, g.n, g.n,
-                                               wrow, wcol, lane, false);
-            } else {
-                store_tile<MLXHIP_DTYPE_F32, C, true, false>(acc, region, g.dx + tile.split * g.m * g.ldc, g.ldc, g.m, g.n, g.ldc,
-                                                             wrow, wcol, lane, g.add);
             }
+            store_tile<OT, C, false, true>(acc, region, static_cast<typename dev::Elem<OT>::type*>(g.dw), g.ldc, g.m, g.n, g.n,
+                                           wrow, wcol, lane, false);
+        } else {
+            store_tile<MLXHIP_DTYPE_F32, C, true, false>(acc, region, g.dx + tile.split * g.m * g.ldc, g.ldc, g.m, g.n, g.ldc,
+                                                         wrow, wcol, lane, g.add);
         }
     }
     // The loads past the last tile write (zeros) to this workgroup's LDS.
@@ -555,26 +634,22 @@ int launch(Args a, hipStream_t s) {
 }
 
 // The product's large or small tiles.
-template <int PRODUCT, int MT, int OT, int P>
+template <int PRODUCT, int MT, int OT, int PA, int PB>
 int product(bool large, const Args& a, hipStream_t s) {
-    return large ? launch<PRODUCT, MT, OT, Large<P>>(a, s) : launch<PRODUCT, MT, OT, Small<P>>(a, s);
+    return large ? launch<PRODUCT, MT, OT, typename Tiling<PA, PB>::Large>(a, s)
+                 : launch<PRODUCT, MT, OT, typename Tiling<PA, PB>::Small>(a, s);
 }
 
-template <int MT, int OT, int P>
+template <int OT>
 int dispatch(int which, bool large, const Args& a, hipStream_t s) {
+    constexpr int ZP = Z_PLANES<OT>, ZT = Z_TYPE<OT>, SP = DS_PLANES<OT>, GT = G_TYPE<OT>;
     switch (which) {
-        case CE_STATS: return product<CE_STATS, MT, OT, P>(large, a, s);
-        case CE_DS: return product<CE_DS, MT, OT, P>(large, a, s);
-        case CE_DX: return product<CE_DX, MT, OT, P>(large, a, s);
-        default: return product<CE_DW, MT, OT, P>(large, a, s);
+        case CE_STATS: return product<CE_STATS, ZT, OT, ZP, ZP>(large, a, s);
+        case CE_DS: return product<CE_DS, ZT, OT, ZP, ZP>(large, a, s);
+        case CE_DX: return product<CE_DX, GT, OT, SP, W_PLANES<OT>>(large, a, s);
+        default: return product<CE_DW, GT, OT, SP, X_PLANES<OT>>(large, a, s);
     }
 }
-
-// Tile sizes of the two forms.
-template <int P>
-constexpr int large_bm() { return Large<P>::BM; }
-template <int P>
-constexpr int large_bn() { return Large<P>::BN; }
 
 }  // namespace ce
 

@@ -10,20 +10,20 @@
 //
 // Forward: one product whose tiles leave each row's maximum and sum over their
 // columns (ce_gemm.hpp), and a launch that joins them. Backward, per piece of
-// the vocabulary: the product again, stored as dS in 16 bits (f32: two f16
-// planes), then dW of the piece whole and dx's share added to f32 sums, which
-// a last launch scales and rounds. Four products of 2 R D V operations; at
-// several hundred rows the matrix cores bound them.
+// the vocabulary: the product again, stored as dS in two or three bf16 planes, then
+// dW of the piece whole and dx's share added to f32 sums, which a last launch
+// rounds. At several hundred rows the matrix cores bound the products.
 //
 // Measured, forward and backward (products and copies; what bounds each product:
-// ce_gemm.hpp): bf16 2048 rows of 1024 over 32000 519 us, 8192 of 2048 over 50257
-// 5.8 ms (1.16 PFLOP/s); f32 2048 of 1024 over 32000 1.63 ms, of which the copies to
-// planes take 60 and the maxima before them 56.
+// ce_gemm.hpp): bf16 2048 rows of 1024 over 32000 730 - 785 us, 8192 of 2048 over 50257
+// 9.2 ms (1.1 PFLOP/s); f32 2048 of 1024 over 32000 2.3 ms, of which the copies of W
+// to planes take 50 (forward, two planes) and 100 (backward, five).
 //
-// x is copied once with zeros in the rows without a target (whatever they hold
-// must not reach dW through a product with 0) and its rows rounded up to whole
-// 16-byte chunks; W is read in place where its rows are such chunks, else
-// copied piece by piece; f32 operands are split into planes by the same copies.
+// For dW, x is copied once with zeros in the rows without a target (whatever they
+// hold must not reach dW through a product with 0) and its rows rounded up to whole
+// 16-byte chunks; W is read in place where its rows are such chunks and their
+// type is the product's, else copied piece by piece; the same copies split operands
+// into planes.
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "ce_gemm.hpp"
@@ -41,7 +41,7 @@ using dev::Elem;
 
 constexpr float LN2 = 0.69314718055994530942f;
 // Bytes of a piece's dS, and of a copied piece of W.
-constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
+constexpr int64_t PIECE_BYTES = int64_t(512) << 20;
 
 // 2^e with the largest magnitude m below it (1/2 of it at least); 15 for an m
 // that says nothing, so that the factors made from it are 1.
@@ -49,154 +49,126 @@ __device__ inline int exponent(float m) { return m > 0.0f && m < INFINITY ? min(
 
 __device__ inline float finite_abs(float v) { return __builtin_isfinite(v) ? fabsf(v) : 0.0f; }
 
-// Eight columns from c on of a row, as the planes of v times f.
-template <int OT, int P>
-__device__ inline void pack8(const typename Elem<OT>::type* src, int64_t c, int64_t dim, bool on, float f, uint16_t* dst,
-                             int64_t plane) {
-    constexpr int VEC = Elem<OT>::VEC;
-    if constexpr (P == 1) {
-        const dev::u32x4 v = dev::load_raw<OT>(src, c, dim).q, none = {0, 0, 0, 0};
-        *reinterpret_cast<dev::u32x4*>(dst + c) = on ? v : none;
-    } else {
-        float v[8];
+// v as P planes of type MT, from column c on, `plane` elements apart.
+template <int MT, int P>
+__device__ inline void store_planes(float (&v)[8], int64_t c, int64_t plane, uint16_t* dst) {
 #pragma unroll
-        for (int k = 0; k < 8 / VEC; ++k) dev::unpack<OT>(dev::load_raw<OT>(src, c + k * VEC, dim), v + k * VEC);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = on ? v[e] * f : 0.0f;
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            dev::store_vec<MLXHIP_DTYPE_F16>(dst + p * plane, c, c + 8, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] -= dev::to_f32<MLXHIP_DTYPE_F16>(dev::from_f32<MLXHIP_DTYPE_F16>(v[e]));
-        }
-    }
-}
-
-// Largest m of a workgroup of 1024 threads.
-__device__ inline float block_max(float m, float* waves) {
-    m = dev::wave_max(m);
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
-    __syncthreads();
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, waves[i]);
-    __syncthreads();
-    return m;
-}
-
-// The factors of ce::Scale, by one workgroup of 1024 threads; part: the maxima
-// of f32 operands (maxima_kernel), null for the others.
-//
-// dS is formed from dloss times a factor that brings its largest magnitude to
-// 2^15, so that the smallest probabilities in use stay normal f16 numbers. For
-// 16-bit operands the factor is that exactly: where all rows weigh the same, as
-// in a mean, the -1 of a target is then a power of two, and its rounding, which
-// would be one relative error of the whole gradient (0.4 % for 1/7 in bf16), is
-// none. Planes of f32 operands, whose dS has 22 bits, and the factor of their dS
-// are scaled by powers of two to between 2^14 and 2^15.
-constexpr int MAXIMA = 1024;
-__device__ inline void write_scales(const float* part, const float* dloss, const int32_t* targets, int64_t rows,
-                                    int64_t vocab, float* scale) {
-    __shared__ float waves[16];
-    int ew = 15, ex = 15;
-    float up = 1.0f, down = 1.0f;
-    if (part) ew = exponent(block_max(part[threadIdx.x], waves));
-    if (dloss) {
-        float m = 0.0f;
-#pragma unroll 4
-        for (int64_t r = threadIdx.x; r < rows; r += 1024)
-            if (counted(targets[r], vocab)) m = fmaxf(m, finite_abs(dloss[r]));
-        m = block_max(m, waves);
-        if (part) {
-            ex = exponent(block_max(part[MAXIMA + threadIdx.x], waves));
-            m = ldexpf(1.0f, exponent(m));
-        }
-        if (m > 0.0f) {
-            m = fmaxf(m, 0x1p-100f);  // 2^15 / m and its inverse stay in range
-            up = 0x1p15f / m;
-            down = m * 0x1p-15f;
-        }
-    }
-    if (threadIdx.x) return;
-    scale[ce::SCALE_DW] = ldexpf(down, ex - 15);
-    scale[ce::SCALE_DS] = up;
-    scale[ce::SCALE_Z] = ldexpf(1.0f, ex + ew - 30);
-    scale[ce::SCALE_DX] = ldexpf(down, ew - 15);
-    scale[ce::SCALE_X] = ldexpf(1.0f, 15 - ex);
-    scale[ce::SCALE_W] = ldexpf(1.0f, 15 - ew);
-}
-
-__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ part, const float* __restrict__ dloss,
-                                                     const int32_t* __restrict__ targets, int64_t rows, int64_t vocab,
-                                                     float* __restrict__ scale) {
-    write_scales(part, dloss, targets, rows, vocab, scale);
-}
-
-// src [rows][dim] as planes of [rows][dim_p] (zeros past dim, and in the rows
-// without a target where targets are given), 8 columns a thread. With `dloss`,
-// workgroup 0 writes the factors of 16-bit operands instead.
-template <int OT, int P>
-__global__ __launch_bounds__(1024) void pack_kernel(const typename Elem<OT>::type* __restrict__ src, int64_t rows,
-                                                    int64_t dim, int64_t dim_p, const int32_t* __restrict__ targets,
-                                                    int64_t vocab, const float* __restrict__ factor,
-                                                    uint16_t* __restrict__ dst, const float* __restrict__ dloss,
-                                                    float* __restrict__ scale) {
-    const int64_t chunks = dim_p / 8, plane = rows * dim_p;
-    const float f = P == 1 ? 1.0f : *factor;
-    int64_t block = blockIdx.x, blocks = gridDim.x;
-    if (P == 1 && dloss) {
-        if (block == 0) {
-            write_scales(nullptr, dloss, targets, rows, vocab, scale);
-            return;
-        }
-        --block;
-        --blocks;
-    }
-    for (int64_t i = block * 1024 + threadIdx.x; i < rows * chunks; i += blocks * 1024) {
-        const int64_t r = i / chunks, c = (i - r * chunks) * 8;
-        pack8<OT, P>(src + r * dim, c, dim, !targets || counted(targets[r], vocab), f, dst + r * dim_p, plane);
-    }
-}
-
-// As pack_kernel for f32, each row scaled by its own largest magnitude
-// (row_scale: what undoes it), a wave to a row: a row of the forward pass takes
-// no digits from another, whatever that holds.
-template <int P>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t dim,
-                                                        int64_t dim_p, float* __restrict__ row_scale,
-                                                        uint16_t* __restrict__ dst) {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
-    float m = 0.0f;
-    for (int64_t c = lane; c < dim; c += 64) m = fmaxf(m, finite_abs(src[r * dim + c]));
-    const int e = exponent(dev::wave_max(m));
-    if (lane == 0) row_scale[r] = ldexpf(1.0f, e - 15);
-    for (int64_t c = lane * 8; c < dim_p; c += 512)
-        pack8<MLXHIP_DTYPE_F32, P>(src + r * dim, c, dim, true, ldexpf(1.0f, 15 - e), dst + r * dim_p, rows * dim_p);
-}
-
-// Largest finite magnitudes, one of each workgroup: of W in part[0..MAXIMA), of
-// the rows of x with a target in part[MAXIMA..2 MAXIMA) (blockIdx.y = 1).
-__global__ __launch_bounds__(256) void maxima_kernel(const float* __restrict__ w, int64_t nw, const float* __restrict__ x,
-                                                     int64_t dim, int64_t nx, const int32_t* __restrict__ targets,
-                                                     int64_t vocab, float* __restrict__ part) {
-    __shared__ float waves[4];
-    const float* p = blockIdx.y ? x : w;
-    const int64_t n = blockIdx.y ? nx : nw;
-    float m = 0.0f;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += MAXIMA * 256 * 8) {
-        const dev::Vec16<MLXHIP_DTYPE_F32> a = dev::load_raw<MLXHIP_DTYPE_F32>(p, i, n),
-                                           b = dev::load_raw<MLXHIP_DTYPE_F32>(p, i + 4, n);
+    for (int p = 0; p < P; ++p) {
+        float h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = finite_abs(__uint_as_float(e < 4 ? a.q[e] : b.q[e - 4]));
-            if (blockIdx.y == 0 || (i + e < n && counted(targets[(i + e) / dim], vocab))) m = fmaxf(m, v);
+            h[e] = dev::to_f32<MT>(dev::from_f32<MT>(v[e]));
+            v[e] -= h[e];
+        }
+        dev::store_vec<MT>(dst + p * plane, c, c + 8, h);
+    }
+}
+
+// Eight columns from c on of a row as f32.
+template <int OT>
+__device__ inline void load8(const typename Elem<OT>::type* src, int64_t c, int64_t dim, float (&v)[8]) {
+    constexpr int VEC = Elem<OT>::VEC;
+#pragma unroll
+    for (int k = 0; k < 8 / VEC; ++k) dev::unpack<OT>(dev::load_raw<OT>(src, c + k * VEC, dim), v + k * VEC);
+}
+
+// src [rows][dim] of 16-bit values as they are into z [rows][dim_p] and, f16 ones times
+// dloss and *scale, as planes into g (either may be null): zeros past dim and, where
+// targets are given, in the rows without one. 8 columns a thread.
+template <int OT>
+__global__ __launch_bounds__(1024) void pack_kernel(const typename Elem<OT>::type* __restrict__ src, int64_t rows,
+                                                    int64_t dim, int64_t dim_p, const int32_t* __restrict__ targets,
+                                                    int64_t vocab, const float* __restrict__ dloss,
+                                                    const float* __restrict__ scale, uint16_t* __restrict__ z,
+                                                    uint16_t* __restrict__ g) {
+    const int64_t chunks = dim_p / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < rows * chunks; i += (int64_t)gridDim.x * 1024) {
+        const int64_t r = i / chunks, c = (i - r * chunks) * 8;
+        const dev::u32x4 raw = dev::load_raw<OT>(src + r * dim, c, dim).q, none = {0, 0, 0, 0};
+        const bool on = !targets || counted(targets[r], vocab);
+        const dev::u32x4 q = on ? raw : none;
+        if (z) *reinterpret_cast<dev::u32x4*>(z + r * dim_p + c) = q;
+        if (OT == MLXHIP_DTYPE_F16 && g) {
+            const float f = on ? dloss[r] * *scale : 0.0f;
+            float v[8];
+            dev::unpack<OT>(dev::Vec16<OT>{q}, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= f;
+            store_planes<OT, ce::X_PLANES<OT>>(v, c, rows * dim_p, g + r * dim_p);
         }
     }
+}
+
+// The largest finite |dloss x| of each row with a target (0 for the others), a wave to
+// a row; and, by one workgroup, from those the power of two that brings them below
+// 2^15 (scale[0]) and what undoes it and dS's own (scale[1]).
+template <int OT>
+__global__ __launch_bounds__(256) void peak_kernel(const typename Elem<OT>::type* __restrict__ x, int64_t rows, int64_t dim,
+                                                   const int32_t* __restrict__ targets, int64_t vocab,
+                                                   const float* __restrict__ dloss, float* __restrict__ peak) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+        float m = 0.0f;
+        if (counted(targets[r], vocab))
+            for (int64_t c = lane * 8; c < dim; c += 512) {
+                float v[8];
+                load8<OT>(x + r * dim, c, dim, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+            }
+        m = dev::wave_max(m);
+        if (lane == 0) peak[r] = finite_abs(m * dloss[r]);
+    }
+}
+__global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ peak, int64_t rows, float* __restrict__ scale) {
+    __shared__ float waves[16];
+    float m = 0.0f;
+#pragma unroll 4
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) m = fmaxf(m, peak[r]);
     m = dev::wave_max(m);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0)
-        part[blockIdx.y * MAXIMA + blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, waves[i]);
+    const int e = exponent(m);
+    scale[0] = ldexpf(1.0f, 15 - e);
+    scale[1] = ldexpf(1.0f / ce::DS_F16, e - 15);
+}
+
+// As pack_kernel for f32: z is two f16 planes of the row times a power of two made from
+// its own largest magnitude (row_scale: what undoes it), so that no row takes digits
+// from another. A wave to a row.
+__global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t dim,
+                                                        int64_t dim_p, const int32_t* __restrict__ targets, int64_t vocab,
+                                                        float* __restrict__ row_scale, uint16_t* __restrict__ z,
+                                                        uint16_t* __restrict__ g) {
+    constexpr int F32 = MLXHIP_DTYPE_F32;
+    const int lane = threadIdx.x & 63;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+        const float* p = src + r * dim;
+        const bool on = !targets || counted(targets[r], vocab);
+        float m = 0.0f;
+        for (int64_t c = lane * 8; c < dim; c += 512) {
+            float v[8];
+            load8<F32>(p, c, dim, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+        }
+        const int e2 = exponent(dev::wave_max(m));
+        if (lane == 0) row_scale[r] = ldexpf(1.0f, e2 - 15);
+        const float f = ldexpf(1.0f, 15 - e2);
+        for (int64_t c = lane * 8; c < dim_p; c += 512) {
+            float v[8], u[8];
+            load8<F32>(p, c, dim, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = on ? v[e] : 0.0f;
+                u[e] = v[e] * f;
+            }
+            store_planes<MLXHIP_DTYPE_F16, ce::Z_PLANES<F32>>(u, c, rows * dim_p, z + r * dim_p);
+            if (g) store_planes<MLXHIP_DTYPE_BF16, ce::X_PLANES<F32>>(v, c, rows * dim_p, g + r * dim_p);
+        }
+    }
 }
 
 // A row's maxima and sums over the tiles joined: 16 rows of a workgroup, 64
@@ -234,16 +206,17 @@ __global__ __launch_bounds__(JOIN_ROWS * JOIN) void loss_kernel(const float2* __
     loss[r] = counted(targets[r], vocab) ? l - target_z[r] : 0.0f;
 }
 
-// dx from the f32 sums of its slices of K, zeros where there is no target: 64
+// dx from the f32 sums of its slices of K (f16 operands: times dloss, where the sums are
+// of dS without it), zeros where there is no target: 64
 // quads of columns of a workgroup, four threads to each, which add up a quarter
 // of the slices each and then those, in order.
 template <int OT>
 __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums, int splits, int64_t rows, int64_t dim,
                                                  int64_t ld, const int32_t* __restrict__ targets, int64_t vocab,
-                                                 const float* __restrict__ scale, typename Elem<OT>::type* __restrict__ dx) {
+                                                 const float* __restrict__ dloss,
+                                                 typename Elem<OT>::type* __restrict__ dx) {
     __shared__ float4 part[4][64];
     const int64_t quads = ld / 4, n = rows * quads;
-    const float f = scale ? scale[ce::SCALE_DX] : 1.0f;
     const int q = threadIdx.x & 63, g = threadIdx.x >> 6;
     const int each = (splits + 3) / 4, k0 = g * each, k1 = min(k0 + each, splits);
     for (int64_t base = (int64_t)blockIdx.x * 64; base < n; base += (int64_t)gridDim.x * 64) {
@@ -266,7 +239,8 @@ __global__ __launch_bounds__(256) void dx_kernel(const float* __restrict__ sums,
                 const float4 v = part[k][q];
                 a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
             }
-            const float v[4] = {a.x * f, a.y * f, a.z * f, a.w * f};
+            const float f = on && dloss ? dloss[r] : 1.0f, down = dloss ? 1.0f / ce::DS_F16 : 1.0f;
+            const float v[4] = {a.x * down * f, a.y * down * f, a.z * down * f, a.w * down * f};
             typename Elem<OT>::type* to = dx + r * dim + c;
             if (c + 4 <= dim) {
                 if constexpr (OT == MLXHIP_DTYPE_F32) {
@@ -319,49 +293,62 @@ struct Carve {
 template <int OT>
 struct Op {
     typedef typename Elem<OT>::type T;
-    static constexpr int P = OT == MLXHIP_DTYPE_F32 ? 2 : 1;
+    static constexpr int ZP = ce::Z_PLANES<OT>, SP = ce::DS_PLANES<OT>, XP = ce::X_PLANES<OT>, WP = ce::W_PLANES<OT>;
+    using ZTiles = ce::Tiling<ZP, ZP>;   // of the logits
+    using DXTiles = ce::Tiling<SP, WP>;
+    using DWTiles = ce::Tiling<SP, XP>;
     const T *x, *w;
     const int32_t* targets;
     int64_t rows, dim, vocab;
     hipStream_t s;
     int64_t dim_p() const { return ceil_div(dim, 8) * 8; }
-    // Whether a matrix of rows of dim is read as it is.
-    bool in_place(const T* p) const { return P == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-    size_t packed(int64_t n) const { return (size_t)n * dim_p() * P * 2; }
-    // factor: what planes hold their values times; with dloss (16-bit operands,
-    // x's rows) also the factors into scale.
-    int pack(const T* src, int64_t n, const int32_t* t, const float* factor, uint16_t* dst, const float* dloss = nullptr,
-             float* scale = nullptr) const {
-        const int64_t groups = std::min<int64_t>(ceil_div(n * dim_p() / 8, 1024), 2048) + (dloss ? 1 : 0);
-        hipLaunchKernelGGL((pack_kernel<OT, P>), dim3((unsigned)groups), dim3(1024), 0, s, src, n, dim, dim_p(), t, vocab,
-                           factor, dst, dloss, scale);
+    // Whether the logits' product reads a matrix of rows of dim as it is.
+    bool in_place(const T* p) const { return ZP == 1 && dim % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+    // Bytes of n rows' planes.
+    size_t bytes(int64_t n, int planes) const { return (size_t)n * dim_p() * planes * 2; }
+    // n rows of src into z and g where not null; scale: f32 rows' factors, or of f16
+    // operands' dloss x.
+    int pack(const T* src, int64_t n, const int32_t* t, const float* dloss, float* scale, uint16_t* z, uint16_t* g) const {
+        if constexpr (OT == MLXHIP_DTYPE_F32) {
+            const int64_t groups = std::min<int64_t>(ceil_div(n, 4), 16384);
+            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)groups), dim3(256), 0, s, src, n, dim, dim_p(), t, vocab, scale,
+                               z, g);
+        } else {
+            const int64_t groups = std::min<int64_t>(ceil_div(n * dim_p() / 8, 1024), 2048);
+            hipLaunchKernelGGL((pack_kernel<OT>), dim3((unsigned)groups), dim3(1024), 0, s, src, n, dim, dim_p(), t, vocab,
+                               dloss, scale, z, g);
+        }
         return launch_check("pack_kernel");
     }
-    // The factors of f32 operands into scale (part: room for the maxima).
-    int scales(const float* dloss, float* part, float* scale) const {
-        hipLaunchKernelGGL(maxima_kernel, dim3(MAXIMA, dloss ? 2 : 1), dim3(256), 0, s, (const float*)w, vocab * dim,
-                           (const float*)x, dim, rows * dim, targets, vocab, part);
-        MLXHIP_TRY(launch_check("maxima_kernel"));
-        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, part, dloss, targets, rows, vocab, scale);
+    // The scales of f16 operands' dloss x (peak: room for a value a row).
+    int scales(const float* dloss, float* peak, float* scale) const {
+        const int64_t groups = std::min<int64_t>(ceil_div(rows, 4), 16384);
+        hipLaunchKernelGGL((peak_kernel<OT>), dim3((unsigned)groups), dim3(256), 0, s, x, rows, dim, targets, vocab, dloss,
+                           peak);
+        MLXHIP_TRY(launch_check("peak_kernel"));
+        hipLaunchKernelGGL(scale_kernel, dim3(1), dim3(1024), 0, s, peak, rows, scale);
         return launch_check("scale_kernel");
     }
     int product(int which, bool large, const Args& a) const {
         if (OT == MLXHIP_DTYPE_F32) return ce_gemm_f32(which, large, a, s);
         return OT == MLXHIP_DTYPE_BF16 ? ce_gemm_bf16(which, large, a, s) : ce_gemm_f16(which, large, a, s);
     }
+    template <class Tiles>
     static int64_t tiles(int64_t m, int64_t n, bool large) {
-        const int64_t bm = large ? ce::large_bm<P>() : 128, bn = large ? ce::large_bn<P>() : 128;
-        return ceil_div(m, bm) * ceil_div(n, bn);
+        typedef typename Tiles::Large L;
+        typedef typename Tiles::Small S;
+        return large ? ceil_div(m, L::BM) * ceil_div(n, L::BN) : ceil_div(m, S::BM) * ceil_div(n, S::BN);
     }
     // Large tiles where they fill most of the compute units, one each.
-    static bool large(int64_t m, int64_t n) { return tiles(m, n, true) >= 192; }
-    // Columns of a piece: a copied piece of W and, with `ds`, dS within
-    // PIECE_BYTES, offsets within a piece and the count of its tiles within 32 bits.
-    int64_t width(bool ds, bool copy) const {
+    template <class Tiles>
+    static bool large(int64_t m, int64_t n) { return tiles<Tiles>(m, n, true) >= 192; }
+    // Columns of a piece: with `ds`, dS, and `copied` planes of a copied piece of W within
+    // the piece's bytes, offsets within a piece and the count of its tiles within 32 bits.
+    int64_t width(bool ds, int copied) const {
         int64_t w = std::min<int64_t>(vocab, (int64_t(1) << 29) / dim_p());
         w = std::min(w, (int64_t(1) << 43) / rows);
-        if (ds) w = std::min(w, PIECE_BYTES / (2 * P) / rows);
-        if (copy) w = std::min(w, PIECE_BYTES / (2 * P) / dim_p());
+        if (ds) w = std::min(w, PIECE_BYTES / (2 * SP) / rows);
+        if (copied) w = std::min(w, PIECE_BYTES / (2 * copied) / dim_p());
         if (w >= vocab) return vocab;
         w = std::max<int64_t>(w / 256 * 256, 256);
         // Pieces of like width: a short last one leaves compute units idle (1105 of
@@ -432,17 +419,18 @@ int few_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
 
 template <int OT>
 int run_loss(const Op<OT>& o, float* loss, float* lse) {
+    typedef Op<OT> O;
     const bool copy_x = !o.in_place(o.x), copy_w = !o.in_place(o.w);
     if (ce::few_loss(OT, copy_w, o.rows, o.vocab)) return few_loss(o, loss, lse);
-    const int64_t width = o.width(false, copy_w);
+    const int64_t width = o.width(false, copy_w ? O::ZP : 0);
     // One tile size for all pieces, whose widths are multiples of its columns.
-    const bool large = Op<OT>::large(o.rows, o.vocab);
-    const int64_t bn = large ? ce::large_bn<Op<OT>::P>() : 128, tiles = ceil_div(o.vocab, bn);
+    const bool large = O::template large<typename O::ZTiles>(o.rows, o.vocab);
+    const int64_t bn = large ? O::ZTiles::Large::BN : O::ZTiles::Small::BN, tiles = ceil_div(o.vocab, bn);
     Carve c;
     const size_t os = c.take((size_t)tiles * o.rows * sizeof(float2)), oz = c.take((size_t)o.rows * 4),
-                 ox = c.take(copy_x ? o.packed(o.rows) : 0), ow = c.take(copy_w ? o.packed(width) : 0),
-                 osc = c.take(ce::SCALES * 4), op = c.take(Op<OT>::P > 1 ? 2 * MAXIMA * 4 : 0),
-                 ors = c.take(Op<OT>::P > 1 ? (size_t)o.rows * 4 : 0);
+                 ox = c.take(copy_x ? o.bytes(o.rows, O::ZP) : 0), ow = c.take(copy_w ? o.bytes(width, O::ZP) : 0),
+                 orow = c.take(O::ZP > 1 ? (size_t)o.rows * 4 : 0),
+                 ocol = c.take(O::ZP > 1 ? (size_t)ceil_div(width, 256) * 256 * 4 : 0);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     Args a;
@@ -453,24 +441,17 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
     a.targets = o.targets;
     a.vocab = o.vocab;
     a.target_z = (float*)(ws + oz);
-    float* scale = (float*)(ws + osc);
-    if constexpr (Op<OT>::P > 1) {
-        a.scale = scale;
-        a.row_scale = (float*)(ws + ors);
-        MLXHIP_TRY(o.scales(nullptr, (float*)(ws + op), scale));
-        hipLaunchKernelGGL((pack_rows_kernel<Op<OT>::P>), dim3((unsigned)ceil_div(o.rows, 4)), dim3(256), 0, o.s, o.x, o.rows,
-                           o.dim, o.dim_p(), (float*)(ws + ors), (uint16_t*)(ws + ox));
-        MLXHIP_TRY(launch_check("pack_rows_kernel"));
-    } else if (copy_x) {
-        MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, nullptr, (uint16_t*)(ws + ox)));
-    }
+    a.row_scale = (float*)(ws + orow);
+    a.col_scale = (float*)(ws + ocol);
+    if (copy_x) MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, nullptr, (float*)(ws + orow), (uint16_t*)(ws + ox), nullptr));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         a.n = std::min(width, o.vocab - v0);
         a.b = copy_w ? (uint16_t*)(ws + ow) : (const uint16_t*)o.w + v0 * o.dim;
         a.b_plane = a.n * o.dim_p();
         a.v0 = v0;
         a.stats = (float2*)(ws + os) + v0 / bn * o.rows;
-        if (copy_w) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, scale + ce::SCALE_W, (uint16_t*)(ws + ow)));
+        if (copy_w)
+            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, a.n, nullptr, nullptr, (float*)(ws + ocol), (uint16_t*)(ws + ow), nullptr));
         MLXHIP_TRY(o.product(ce::CE_STATS, large, a));
     }
     return finish_loss((const float2*)(ws + os), tiles, a.target_z, o.targets, o.rows, o.vocab, loss, lse, o.s);
@@ -480,47 +461,51 @@ template <int OT>
 int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Elem<OT>::type* dx,
              typename Elem<OT>::type* dw) {
     typedef typename Elem<OT>::type T;
-    constexpr int P = Op<OT>::P;
+    typedef Op<OT> O;
+    typedef typename O::DXTiles DX;
+    constexpr int ZP = O::ZP, SP = O::SP, XP = O::XP, WP = O::WP;
+    constexpr bool F16 = OT == MLXHIP_DTYPE_F16;
     if (o.rows == 0) {  // a sum over no rows
         if (!dw) return MLXHIP_OK;
         hipLaunchKernelGGL((zero_kernel<T>), dim3(grid_for(o.vocab * o.dim)), dim3(256), 0, o.s, dw, o.vocab * o.dim);
         return launch_check("zero_kernel");
     }
     if (ce::few_grad(OT, o.rows, o.vocab)) return few_grad(o, lse, dloss, dx, dw);
-    const bool copy_w = !o.in_place(o.w);
-    const int64_t width = o.width(true, copy_w), ld = ceil_div(width, 256) * 256, dim_p = o.dim_p();
-    // dx: few tiles, so K is cut into slices until every compute unit has one
-    // (two of the small tiles), of at least 512 each.
-    const bool dx_large = Op<OT>::tiles(o.rows, o.dim, true) >= 16;
-    const int64_t dx_tiles = Op<OT>::tiles(o.rows, o.dim, dx_large), room = dx_large || P > 1 ? 256 : 512;
+    // One plane of x or W serves z and the gradient, but x's then has to be a copy.
+    const bool copy_x = XP == 1 || !o.in_place(o.x), copy_w = !o.in_place(o.w), planes_x = XP > 1 && dw,
+               planes_w = WP > 1 && dx;
+    const int64_t width = o.width(true, (copy_w ? ZP : 0) + (planes_w ? WP : 0)), ld = ceil_div(width, 256) * 256,
+                  dim_p = o.dim_p();
+    // dx: few tiles, so K is cut into slices until every place on the chip has one,
+    // of at least 512 each.
+    const bool dx_large = O::template tiles<DX>(o.rows, o.dim, true) >= 16;
+    const int64_t dx_tiles = O::template tiles<DX>(o.rows, o.dim, dx_large);
+    const int64_t room = 256 * (dx_large ? DX::Large::PER_CU : DX::Small::PER_CU);
     const int64_t most = std::max<int64_t>(1, std::min(room / dx_tiles, width / 512));
     const int64_t chunk = ceil_div(ceil_div(width, most), 32) * 32;
     const int splits = (int)ceil_div(width, chunk);
     const int64_t ldx = ceil_div(o.dim, 4) * 4;
     Carve c;
-    const size_t ods = c.take((size_t)P * o.rows * ld * 2), ox = c.take(o.packed(o.rows)),
-                 ow = c.take(copy_w ? o.packed(width) : 0), osc = c.take(ce::SCALES * 4),
-                 op = c.take(P > 1 ? 2 * MAXIMA * 4 : 0), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
+    const size_t ods = c.take((size_t)SP * o.rows * ld * 2), ox = c.take(copy_x ? o.bytes(o.rows, ZP) : 0),
+                 oxg = c.take(planes_x ? o.bytes(o.rows, XP) : 0), ow = c.take(copy_w ? o.bytes(width, ZP) : 0),
+                 owg = c.take(planes_w ? o.bytes(width, WP) : 0), orow = c.take(ZP > 1 || F16 ? (size_t)o.rows * 4 : 0),
+                 osc = c.take(F16 ? 2 * 4 : 0), ocol = c.take(ZP > 1 ? (size_t)ld * 4 : 0), osum = c.take(dx ? (size_t)splits * o.rows * ldx * 4 : 0);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
-    uint16_t *ds = (uint16_t*)(ws + ods), *xp = (uint16_t*)(ws + ox);
-    float *scale = (float*)(ws + osc), *sums = (float*)(ws + osum);
-    if constexpr (P > 1) {
-        MLXHIP_TRY(o.scales(dloss, (float*)(ws + op), scale));
-        MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, scale + ce::SCALE_X, xp));
-    } else {
-        MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, nullptr, xp, dloss, scale));
-    }
+    uint16_t *ds = (uint16_t*)(ws + ods), *xz = copy_x ? (uint16_t*)(ws + ox) : nullptr,
+             *xg = planes_x ? (uint16_t*)(ws + oxg) : nullptr, *wz = copy_w ? (uint16_t*)(ws + ow) : nullptr,
+             *wg = planes_w ? (uint16_t*)(ws + owg) : nullptr;
+    float *sums = (float*)(ws + osum), *row_scale = (float*)(ws + orow), *col_scale = (float*)(ws + ocol);
+    float* scale = F16 ? (float*)(ws + osc) : row_scale;
+    if constexpr (F16)
+        if (dw) MLXHIP_TRY(o.scales(dloss, row_scale, scale));
+    if (xz || xg) MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, dloss, scale, xz, xg));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
         const int64_t n = std::min(width, o.vocab - v0);
-        const uint16_t* wp = (const uint16_t*)o.w + v0 * o.dim;
-        if (copy_w) {
-            wp = (uint16_t*)(ws + ow);
-            MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, scale + ce::SCALE_W, (uint16_t*)(ws + ow)));
-        }
+        if (wz || wg) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, nullptr, col_scale, wz, wg));
         Args z;
-        z.a = xp;
-        z.b = wp;
+        z.a = xz ? xz : (const uint16_t*)o.x;
+        z.b = wz ? wz : (const uint16_t*)o.w + v0 * o.dim;
         z.lda = z.ldb = z.ka = z.kb = dim_p;
         z.a_plane = o.rows * dim_p;
         z.b_plane = n * dim_p;
@@ -531,16 +516,17 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         z.vocab = o.vocab;
         z.lse = lse;
         z.dloss = dloss;
-        z.scale = scale;
+        z.row_scale = row_scale;
+        z.col_scale = col_scale;
         z.ds = ds;
         z.ldc = ceil_div(n, 256) * 256;
-        MLXHIP_TRY(o.product(ce::CE_DS, Op<OT>::large(o.rows, n), z));
+        MLXHIP_TRY(o.product(ce::CE_DS, O::template large<typename O::ZTiles>(o.rows, n), z));
         if (dw) {
             Args p;
             p.a = ds;
             p.lda = z.ldc;
             p.a_plane = o.rows * z.ldc;
-            p.b = xp;
+            p.b = XP > 1 ? xg : xz;
             p.ldb = dim_p;
             p.b_plane = z.a_plane;
             p.ka = p.kb = o.rows;
@@ -548,8 +534,8 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
             p.n = o.dim;
             p.dw = dw + v0 * o.dim;
             p.ldc = o.dim;
-            p.scale = scale;
-            MLXHIP_TRY(o.product(ce::CE_DW, Op<OT>::large(n, o.dim), p));
+            p.scale = scale + 1;
+            MLXHIP_TRY(o.product(ce::CE_DW, O::template large<typename O::DWTiles>(n, o.dim), p));
         }
         if (dx) {
             Args p;
@@ -557,7 +543,7 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
             p.lda = z.ldc;
             p.a_plane = o.rows * z.ldc;
             p.ka = ceil_div(n, 8) * 8;  // dS holds zeros behind the piece
-            p.b = wp;
+            p.b = WP > 1 ? wg : z.b;
             p.ldb = dim_p;
             p.b_plane = z.b_plane;
             p.kb = n;
@@ -574,7 +560,7 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
     }
     if (!dx) return MLXHIP_OK;
     hipLaunchKernelGGL((dx_kernel<OT>), dim3(grid_for(o.rows * ldx)), dim3(256), 0, o.s, sums, splits, o.rows, o.dim, ldx,
-                       o.targets, o.vocab, scale, dx);
+                       o.targets, o.vocab, F16 ? dloss : nullptr, dx);
     return launch_check("dx_kernel");
 }
 
