@@ -486,10 +486,13 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * dw's terms dloss x have a floor of 2^-39 of the largest), f32 for up to 16 rows.
  * Sums are formed in a fixed order. Operands contiguous, at any address
  * aligned to their elements; results must not overlap operands. A non-finite
- * value of x reaches its row's results, one of w all rows': they may be NaN.
+ * value of x or dloss reaches its row's results, which may be NaN, and dw. One of w
+ * reaches the rows' logits as it is: -inf times a positive x rules its entry
+ * out (a logit of -inf, a probability of 0), and dx, where it sums 0 times infinity,
+ * is NaN in that column.
  * rows up to 2^21, dim up to 2^20, vocab up to 2^31 - 1, rows times dim (rounded
- * up to a multiple of 8) up to 2^29: cut a larger batch by its rows. The workspace (per stream) holds dS for one piece of
- * the vocabulary, 512 MiB or 256 columns (the few rows above: of the whole, up to
+ * up to a multiple of 8) up to 2^29: cut a larger batch by its rows. The workspace
+ * (per stream) holds dS for one piece of the vocabulary, 512 MiB or 256 columns (the few rows above: of the whole, up to
  * 1 GiB), copies of x and of a piece of w where needed, and f32 sums of dx. No reference counterpart. */
 int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, const int32_t* targets,
                                 float* loss, float* lse, int64_t rows, int64_t dim, int64_t vocab,

@@ -49,7 +49,10 @@ __device__ inline int exponent(float m) { return m > 0.0f && m < INFINITY ? min(
 
 __device__ inline float finite_abs(float v) { return __builtin_isfinite(v) ? fabsf(v) : 0.0f; }
 
-// v as P planes of type MT, from column c on, `plane` elements apart.
+// v as P planes of type MT, from column c on, `plane` elements apart. A value that is
+// not finite is all in the last plane, which meets the other operand's first one
+// only: it reaches the product as itself, with the other's sign. A finite value
+// that rounds to infinity is cut off instead.
 template <int MT, int P>
 __device__ inline void store_planes(float (&v)[8], int64_t c, int64_t plane, uint16_t* dst) {
 #pragma unroll
@@ -58,9 +61,15 @@ __device__ inline void store_planes(float (&v)[8], int64_t c, int64_t plane, uin
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             h[e] = dev::to_f32<MT>(dev::from_f32<MT>(v[e]));
-            v[e] -= h[e];
+            if (p + 1 < P) {
+                if (MT == MLXHIP_DTYPE_BF16 && __builtin_isinf(h[e]))
+                    h[e] = __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+                if (!__builtin_isfinite(v[e])) h[e] = 0.0f;
+            }
         }
         dev::store_vec<MT>(dst + p * plane, c, c + 8, h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] -= h[e];
     }
 }
 

@@ -1,4 +1,5 @@
-"""Linear cross entropy on operands whose sizes differ widely: each result against 64 bits within a bound made from its own row's and
+"""Linear cross entropy on operands whose sizes differ widely, and with
+infinities: each result against 64 bits within a bound made from its own row's and
 column's terms, whatever the rest of the operands hold.
 
 Bounds (u = 2^-24). A logit is a sum of dim terms in f32, of operands that are
@@ -135,3 +136,46 @@ def test_improbable_words_keep_their_digits(rows, dt):
     w[::3, 7] = -5.0
     t = np.where((t >= 0) & (t < 700) & (t % 3 == 0), t + 1, t).astype(np.int32)
     check_all(run(x, w, t, g, dt), x, w, t, g, dt)
+
+
+@pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("dim", [72, 77])
+def test_an_entry_ruled_out_by_an_infinity(rows, dim, dt):
+    """-inf in one row of w where x is positive: that logit is -inf, its
+    probability 0, and losses and gradients are those without the entry; dx is NaN
+    in the infinity's column (0 times infinity), rows without a target have no
+    gradient all the same."""
+    vocab = 515
+    x, w, t, g = inputs(rows, dim, vocab, dt)
+    x[:, 4] = 0.5 + np.abs(x[:, 4])
+    x = R.rounded(x, dt)
+    t[t == vocab - 1] = 3
+    w[vocab - 1, 4] = -np.inf
+    t[t == vocab] = -1
+    t[0] = 3
+    t[1] = -100
+    got = run(x, w, t, g, dt)
+    want = forward(x, w[:-1], t, dt) + backward(x, w[:-1], t, g, dt)
+    R.check(got[0], *want[0], "loss")
+    R.check(got[1], *want[1], "lse")
+    on = (t >= 0) & (t < vocab)
+    keep = np.arange(dim) != 4
+    R.check(got[2][:, keep], want[2][0][:, keep], want[2][1][:, keep], "dx")
+    assert np.isnan(got[2][on, 4]).all() and not got[2][~on].any()
+    R.check(got[3][:-1], *want[3], "dw")
+    assert not got[3][-1].any()
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_values_next_to_the_largest_one(rows):
+    """f32 values that fewer bits would round to infinity, where x has zeros:
+    nothing but the sums over them (column 6 of dx) may leave the range."""
+    x, w, t, g = inputs(rows, 72, 300, abi.F32)
+    x[:, 6] = 0.0
+    w[5, 6] = np.finfo(np.float32).max
+    w[6, 6] = -np.finfo(np.float32).max
+    got = run(x, w, t, g, abi.F32)
+    got[2] = got[2][:, np.arange(72) != 6]
+    for name, a in zip(("loss", "lse", "dx", "dw"), got):
+        assert np.isfinite(a).all(), name
