@@ -101,7 +101,7 @@ int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t
 int linear_cross_entropy_lse(const float* x, const float* w, const int32_t* targets, const float* loss, float* lse,
                              int64_t rows, int64_t dim, int64_t vocab, hipStream_t s);
 // Whole numbers held as f32 as int32: saturating, NaN to 0 (the Embedding
-// op's ids), or with `targets` -1 for NaN and what is out of int32's range.
+// op's ids), or with `targets` -1 for what is no whole number of int32's range from 0 on.
 int ids_from_f32(const float* x, int32_t* ids, int64_t n, bool targets, hipStream_t s);
 
 // ── decode.hip (greedy decode step of a decoder-only model) ───────────────

@@ -720,7 +720,7 @@ __global__ __launch_bounds__(BLOCK) void ids_kernel(const float* __restrict__ x,
                                                     bool targets) {
     FOR_EACH_ELEMENT(i, n) {
         const float f = x[i];
-        ids[i] = targets && !(f >= 0.0f && f < 2147483648.0f) ? -1 : f2i_sat(f);
+        ids[i] = targets && !(f >= 0.0f && f < 2147483648.0f && f == truncf(f)) ? -1 : f2i_sat(f);
     }
 }
 

@@ -337,20 +337,21 @@ class Embedding:
 
 class LinearCrossEntropy:
     """Mean cross entropy of the logits x W^T of an output projection (weight
-    [vocab, dim], no bias) over the rows whose target lies in [0, vocab); HIP
-    streams only. The logits are never kept."""
+    [vocab, dim], no bias) over the rows whose target is a whole number of
+    [0, vocab); HIP streams only. The logits are never kept."""
 
     def __init__(self, weight: Tensor):
         self.weight = weight
 
     def forward(self, x: Tensor, targets: np.ndarray) -> Tensor:
-        """x [rows, dim], targets [rows] whole numbers -> a scalar; 0 where no
-        row has a target."""
+        """x [rows, dim], targets [rows] -> a scalar; 0 where no row has a
+        target."""
         t = np.asarray(targets).reshape(-1)
         vocab = self.weight.shape[0]
-        counted = max(1, int(np.count_nonzero((t >= 0) & (t < vocab))))
+        on = (t >= 0) & (t < vocab) & (t == np.floor(t))
+        counted = max(1, int(np.count_nonzero(on)))
         # Whole numbers up to 2^24 are exact in f32: a larger id must not round into the vocabulary.
-        ids = Tensor.from_f32_on_stream(np.where((t >= 0) & (t < vocab), t, -1).astype(np.float32), t.shape, x.stream)
+        ids = Tensor.from_f32_on_stream(np.where(on, t, -1).astype(np.float32), t.shape, x.stream)
         share = Tensor.from_f32_on_stream(np.array([1.0 / counted], np.float32), (1,), x.stream)
         loss = x.linear_cross_entropy(self.weight, ids)
         return loss.mul(share.broadcast_to(loss.shape)).sum_all()

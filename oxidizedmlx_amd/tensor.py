@@ -239,8 +239,8 @@ class Tensor:
 
     def linear_cross_entropy(self, weight: "Tensor", targets: "Tensor") -> "Tensor":
         """Cross entropy of the logits x W^T of this x [rows, dim] and a weight
-        [vocab, dim] against ``targets`` [rows] (ids as f32; one outside
-        [0, vocab) takes its row out): the loss of each row. The logits are
+        [vocab, dim] against ``targets`` [rows] (ids as f32; one that is no whole
+        number of [0, vocab) takes its row out): the loss of each row. The logits are
         formed in pieces of the vocabulary and never kept. HIP streams only;
         with VJPs for x and the weight."""
         if len(self.shape) != 2 or len(weight.shape) != 2 or self.shape[1] != weight.shape[1]:
