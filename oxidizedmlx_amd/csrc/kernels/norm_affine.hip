@@ -14,9 +14,11 @@
 // Rows of up to 16384 columns stay in registers: WPR waves own a row, each
 // lane NV 16-byte vectors of it (at most 16 values), so x and dy are read
 // once and y or dx written once. The statistics take two exchanges between a
-// row's lanes: the mean, then the sums of (x - mean)^2 and, going back, of g
-// and g (x - mean) as well (the deviations are from the true mean, so a large
-// mean costs no digits). Workgroups walk over rows with the weights held in
+// row's lanes: the mean, then the sums of the deviations d from it, of d^2 and, going
+// back, of g and g d as well. The mean of d is what the f32 mean is off by, by its own
+// rounding and those of its sum: it is taken off d and out of the other sums, so a
+// large mean costs no digits (a row of 3000.7s has deviations of 1e-9, and of 5e-4
+// without). Workgroups walk over rows with the weights held in
 // registers; going back each lane also keeps its columns' dw and db sums and
 // writes them at the end as one partial row per workgroup, which a second
 // launch adds up in a fixed order (no atomics: the same bits every time).
@@ -68,6 +70,13 @@ __device__ inline void row_sums(float (&v)[N], float* slots, int wave, int lane)
     }
 }
 
+// 1 / sqrt(var + eps) of a row whose deviations have the sum s1, the sum of squares s2
+// and the mean off. Squares past f32's range make it 0, whatever the product gives.
+__device__ inline float inverse_std(float s1, float s2, float off, float inv, float eps) {
+    const float rest = s2 - off * s1, sum = s2 == INFINITY ? s2 : rest < 0.0f ? 0.0f : rest;  // NaN stays
+    return 1.0f / sqrtf(sum * inv + eps);
+}
+
 // A row's columns in lane t of 64 * WPR: NV vectors, of which every one but the
 // last is whole in all lanes (the launch picks NV so). The last begins at the
 // row's end less VEC where it would run past it: its elements below `from` belong
@@ -104,7 +113,7 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_fwd_kernel(
     const typename Elem<DT>::type* __restrict__ b, typename Elem<DT>::type* __restrict__ y, int64_t rows, int64_t cols,
     float eps) {
     constexpr int VEC = Elem<DT>::VEC, RPB = WPR < 4 ? 4 / WPR : 1;  // rows of a workgroup
-    __shared__ float slots[2][RPB][WPR];
+    __shared__ float slots[2][RPB][2 * WPR];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave / WPR, wr = wave % WPR;
     const Columns<DT, WPR, NV> col(wr * 64 + lane, cols);
     const float inv = 1.0f / (float)cols;
@@ -121,14 +130,18 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_fwd_kernel(
         for (int i = 0; i < NV * VEC; ++i) s[0] += col.own(i / VEC, i % VEC) ? v[i] : 0.0f;
         row_sums<WPR, 1>(s, slots[0][sub], wr, lane);
         const float mean = s[0] / (float)cols;
-        s[0] = 0.0f;
+        float m[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < NV * VEC; ++i) {
             v[i] -= mean;
-            s[0] += col.own(i / VEC, i % VEC) ? v[i] * v[i] : 0.0f;
+            const float d = col.own(i / VEC, i % VEC) ? v[i] : 0.0f;
+            m[0] += d;
+            m[1] += d * d;
         }
-        row_sums<WPR, 1>(s, slots[1][sub], wr, lane);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
+        row_sums<WPR, 2>(m, slots[1][sub], wr, lane);
+        const float off = m[0] * inv, rstd = inverse_std(m[0], m[1], off, inv, eps);
+#pragma unroll
+        for (int i = 0; i < NV * VEC; ++i) v[i] -= off;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float wf[VEC], bf[VEC];
@@ -148,7 +161,7 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
     const typename Elem<DT>::type* __restrict__ w, typename Elem<DT>::type* __restrict__ dx, float* __restrict__ part,
     int64_t rows, int64_t cols, float eps) {
     constexpr int VEC = Elem<DT>::VEC, RPB = WPR < 4 ? 4 / WPR : 1, EPL = NV * VEC;
-    __shared__ float slots[2][RPB][3 * WPR];
+    __shared__ float slots[2][RPB][4 * WPR];
     __shared__ float fold[RPB > 1 ? RPB * 64 * EPL : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave / WPR, wr = wave % WPR;
     const Columns<DT, WPR, NV> col(wr * 64 + lane, cols);
@@ -184,7 +197,7 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
         for (int i = 0; i < EPL; ++i) s1[0] += col.own(i / VEC, i % VEC) ? v[i] : 0.0f;
         row_sums<WPR, 1>(s1, slots[0][sub], wr, lane);
         const float mean = s1[0] / (float)cols;
-        float s[3] = {0.0f, 0.0f, 0.0f};
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float wf[VEC];
@@ -196,14 +209,15 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
                 v[i] -= mean;
                 ab[i] += g[i];
                 const float gw = col.own(j, e) ? g[i] * wf[e] : 0.0f, d = col.own(j, e) ? v[i] : 0.0f;
-                s[0] += d * d;
-                s[1] += gw;
-                s[2] += gw * d;
+                s[0] += d;
+                s[1] += d * d;
+                s[2] += gw;
+                s[3] += gw * d;
             }
         }
-        row_sums<WPR, 3>(s, slots[1][sub], wr, lane);
-        const float rstd = 1.0f / sqrtf(s[0] * inv + eps);
-        const float c1 = s[1] * inv, c2 = s[2] * inv * rstd;
+        row_sums<WPR, 4>(s, slots[1][sub], wr, lane);
+        const float off = s[0] * inv, rstd = inverse_std(s[0], s[1], off, inv, eps);
+        const float c1 = s[2] * inv, c2 = (s[3] - off * s[2]) * inv * rstd;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float wf[VEC];
@@ -211,7 +225,7 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const int i = j * VEC + e;
-                const float xh = v[i] * rstd;
+                const float xh = (v[i] - off) * rstd;
                 aw[i] += g[i] * xh;
                 wf[e] = rstd * (g[i] * wf[e] - c1 - xh * c2);
             }
@@ -271,19 +285,21 @@ __global__ __launch_bounds__(32 * FOLD) void affine_fold_kernel(const float* __r
     else db[to - cols] = dev::from_f32<DT>(s);
 }
 
-// Longer rows: mean, rstd and, with dy, the means of g and g xh of a row per workgroup.
+// Longer rows: mean, what it is off by, rstd and, with dy, the means of g and g xh (c2) of
+// a row per workgroup.
 template <int DT, bool GRAD>
 __global__ __launch_bounds__(1024) void long_stats_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                           const typename Elem<DT>::type* __restrict__ x,
                                                           const typename Elem<DT>::type* __restrict__ w,
-                                                          float4* __restrict__ stats, int64_t rows, int64_t cols,
-                                                          float eps) {
+                                                          float4* __restrict__ stats, float* __restrict__ c2,
+                                                          int64_t rows, int64_t cols, float eps) {
     constexpr int VEC = Elem<DT>::VEC;
-    __shared__ float slots[2][3 * 16];
+    __shared__ float slots[2][4 * 16];
+    const float inv = 1.0f / (float)cols;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const typename Elem<DT>::type *xr = x + r * cols, *gr = GRAD ? dy + r * cols : nullptr;
-        float s1[1] = {0.0f}, s[3] = {0.0f, 0.0f, 0.0f};
+        float s1[1] = {0.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < cols; c += 1024 * VEC) {
             float v[VEC];
             unpack<DT>(load_raw<DT>(xr, c, cols), v);
@@ -302,17 +318,19 @@ __global__ __launch_bounds__(1024) void long_stats_kernel(const typename Elem<DT
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float d = c + e < cols ? v[e] - mean : 0.0f;
-                s[0] += d * d;
+                s[0] += d;
+                s[1] += d * d;
                 if constexpr (GRAD) {
-                    s[1] += g[e] * wf[e];
-                    s[2] += g[e] * wf[e] * d;
+                    s[2] += g[e] * wf[e];
+                    s[3] += g[e] * wf[e] * d;
                 }
             }
         }
-        row_sums<16, 3>(s, slots[1], wave, lane);
+        row_sums<16, 4>(s, slots[1], wave, lane);
         if (threadIdx.x == 0) {
-            const float rstd = 1.0f / sqrtf(s[0] / (float)cols + eps);
-            stats[r] = make_float4(mean, rstd, s[1] / (float)cols, s[2] / (float)cols * rstd);
+            const float off = s[0] * inv, rstd = inverse_std(s[0], s[1], off, inv, eps);
+            stats[r] = make_float4(mean, off, rstd, s[2] * inv);
+            if constexpr (GRAD) c2[r] = (s[3] - off * s[2]) * inv * rstd;
         }
     }
 }
@@ -323,8 +341,8 @@ template <int DT, bool GRAD>
 __global__ __launch_bounds__(LONG_TILE / Elem<DT>::VEC) void long_apply_kernel(
     const typename Elem<DT>::type* __restrict__ dy, const typename Elem<DT>::type* __restrict__ x,
     const typename Elem<DT>::type* __restrict__ w, const typename Elem<DT>::type* __restrict__ b,
-    const float4* __restrict__ stats, typename Elem<DT>::type* __restrict__ out, float* __restrict__ part, int64_t rows,
-    int64_t cols) {
+    const float4* __restrict__ stats, const float* __restrict__ c2, typename Elem<DT>::type* __restrict__ out,
+    float* __restrict__ part, int64_t rows, int64_t cols) {
     constexpr int VEC = Elem<DT>::VEC;
     const int64_t c = (int64_t)blockIdx.x * LONG_TILE + threadIdx.x * VEC;
     if (c >= cols) return;
@@ -335,16 +353,17 @@ __global__ __launch_bounds__(LONG_TILE / Elem<DT>::VEC) void long_apply_kernel(
     for (int e = 0; e < VEC; ++e) aw[e] = ab[e] = 0.0f;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const float4 st = stats[r];
+        const float k = GRAD ? c2[r] : 0.0f;
         float v[VEC], g[VEC];
         unpack<DT>(load_raw<DT>(x + r * cols, c, cols), v);
         if constexpr (GRAD) unpack<DT>(load_raw<DT>(dy + r * cols, c, cols), g);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float xh = (v[e] - st.x) * st.y;
+            const float xh = (v[e] - st.x - st.y) * st.z;
             if constexpr (GRAD) {
                 aw[e] += g[e] * xh;
                 ab[e] += g[e];
-                v[e] = st.y * (g[e] * wf[e] - st.z - xh * st.w);
+                v[e] = st.z * (g[e] * wf[e] - st.w - xh * k);
             } else {
                 v[e] = xh * wf[e] + bf[e];
             }
@@ -410,7 +429,7 @@ int run_affine(Args<DT> a) {
     int64_t groups = registers ? std::min<int64_t>(ceil_div(a.rows, rpb), a.grad ? PARTIALS : 2048)
                                : std::min<int64_t>(a.rows, 64);
     const size_t part = a.grad ? (size_t)groups * 2 * a.cols * sizeof(float) : 0;
-    const size_t stats = registers ? 0 : (size_t)a.rows * sizeof(float4);
+    const size_t stats = registers ? 0 : (size_t)a.rows * (sizeof(float4) + sizeof(float));  // and c2
     char* ws = nullptr;
     if (part + stats) MLXHIP_TRY(stream_workspace(a.s, WS_NORM, part + stats, reinterpret_cast<void**>(&ws)));
     a.part = reinterpret_cast<float*>(ws + stats);
@@ -418,21 +437,22 @@ int run_affine(Args<DT> a) {
         // No rows: the fold below writes the zeros of dw and db.
     } else if (!registers) {
         float4* st = reinterpret_cast<float4*>(ws);
+        float* c2 = reinterpret_cast<float*>(st + a.rows);
         const dim3 grid((unsigned)ceil_div(a.cols, LONG_TILE), (unsigned)groups);
         const int threads = LONG_TILE / Elem<DT>::VEC;
         const unsigned blocks = (unsigned)std::min<int64_t>(a.rows, 4096);
         if (a.grad) {
-            hipLaunchKernelGGL((long_stats_kernel<DT, true>), dim3(blocks), dim3(1024), 0, a.s, a.dy, a.x, a.w, st, a.rows,
-                               a.cols, a.eps);
+            hipLaunchKernelGGL((long_stats_kernel<DT, true>), dim3(blocks), dim3(1024), 0, a.s, a.dy, a.x, a.w, st, c2,
+                               a.rows, a.cols, a.eps);
             MLXHIP_TRY(launch_check("long_stats_kernel"));
-            hipLaunchKernelGGL((long_apply_kernel<DT, true>), grid, dim3(threads), 0, a.s, a.dy, a.x, a.w, a.b, st, a.out,
-                               a.part, a.rows, a.cols);
+            hipLaunchKernelGGL((long_apply_kernel<DT, true>), grid, dim3(threads), 0, a.s, a.dy, a.x, a.w, a.b, st,
+                               c2, a.out, a.part, a.rows, a.cols);
         } else {
-            hipLaunchKernelGGL((long_stats_kernel<DT, false>), dim3(blocks), dim3(1024), 0, a.s, a.dy, a.x, a.w, st, a.rows,
-                               a.cols, a.eps);
+            hipLaunchKernelGGL((long_stats_kernel<DT, false>), dim3(blocks), dim3(1024), 0, a.s, a.dy, a.x, a.w, st, c2,
+                               a.rows, a.cols, a.eps);
             MLXHIP_TRY(launch_check("long_stats_kernel"));
-            hipLaunchKernelGGL((long_apply_kernel<DT, false>), grid, dim3(threads), 0, a.s, a.dy, a.x, a.w, a.b, st, a.out,
-                               a.part, a.rows, a.cols);
+            hipLaunchKernelGGL((long_apply_kernel<DT, false>), grid, dim3(threads), 0, a.s, a.dy, a.x, a.w, a.b, st,
+                               c2, a.out, a.part, a.rows, a.cols);
         }
         MLXHIP_TRY(launch_check("long_apply_kernel"));
     } else if (a.cols <= 1024) {
