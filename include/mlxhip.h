@@ -456,8 +456,9 @@ int mlxhip_layernorm_affine_vjp_rows(int32_t dtype, const void* dy, const void* 
  * an order that only the ids fix (no atomics: the same bits every time).
  * Operands contiguous, at any address aligned to their elements; results must
  * not overlap operands. n and vocab up to 2^31 - 1, dim up to 2^20. The
- * gradient of over 64 ids sorts their positions in a per-stream workspace (8 or 16
- * bytes per id and 4096 rows of dim f32 sums at most). No reference
+ * gradient of over 64 ids, or of fewer where dy or dw are large (512 KiB, 192 MiB at
+ * most), sorts their positions in a per-stream workspace (8 or 16 bytes per id and
+ * 4096 rows of dim f32 sums at most). No reference
  * counterpart for the gradient (crates/mlx-autograd/src/vjp.rs:173-176). */
 int mlxhip_embedding_rows(int32_t dtype, const void* w, const int32_t* ids, void* y, int64_t n,
                           int64_t vocab, int64_t dim, float scale, void* stream);

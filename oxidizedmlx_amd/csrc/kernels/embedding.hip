@@ -522,10 +522,18 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const uint32_t* __restr
 // Up to 64 positions: one launch, in which a workgroup owns `each` rows of dW. It
 // finds the positions of its rows (in order) and their bits among its rows, writes
 // zeros to the others, and gives each id's sum to a wave, 64 pieces of columns at a
-// time. With the lookup, 64 positions over 32000 f32 rows of 768: 18.4 us (65, by
-// sorting: 23.4). 64 times one id, which one compute unit then adds up: 11 us for
-// rows of 1024 (65 sorted: 14), 30 for 4096 (18).
+// time. Against sorting (64 distinct positions and 65, 2000 rows of 1024 f32 values: 4.4
+// and 11.8 us) it saves three launches, but one compute unit adds up all positions of
+// one id, behind its zeros: 64 of them take 5 us more for rows of 4 KiB, 8 for 8, 17 for
+// 16 and 34 for 32, where sorting stays at 13 to 17 in all. So it takes up to 512 KiB
+// of dy where dW has up to 32 MiB (64 rows of 8 KiB of one id 13.0 us, sorted 15.2; 32 of
+// 16 KiB 15.5 and 15.3, 64 of them 24 and 16). The sort's launches hide behind a larger
+// dW's zeros: there half of that dy (131 MB, 64 rows of 4 KiB of one id 20.6, 65 sorted
+// 23.8), and none from 192 MiB on (262 MB: 39 distinct either way, 24 of one id 45 and 40).
 constexpr int FEW = 64, FEW_ROWS = 4096;  // most rows of a workgroup
+inline bool few_positions(int64_t n, int64_t dy_bytes, int64_t dw_bytes) {
+    return n <= FEW && dw_bytes <= (192 << 20) && dy_bytes <= (dw_bytes <= (32 << 20) ? 512 << 10 : 256 << 10);
+}
 template <int DT, int N>
 __global__ __launch_bounds__(1024) void embed_few_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                          const int32_t* __restrict__ ids, int n, int64_t vocab,
@@ -615,12 +623,12 @@ int run_embed_vjp(const void* dy, const int32_t* ids, void* dw, int64_t n, int64
     typedef typename Elem<DT>::type T;
     // 512 workgroups, two to a compute unit; `all` above within 32 bits.
     const int64_t each = std::min<int64_t>(ceil_div(vocab, 512), std::min<int64_t>(FEW_ROWS, (int64_t(1) << 30) / dim));
-    if (n <= FEW) {
+    const int64_t dw_bytes = vocab * dim * (int64_t)sizeof(T);
+    if (n == 0 || few_positions(n, n * dim * (int64_t)sizeof(T), dw_bytes)) {
         hipLaunchKernelGGL((embed_few_kernel<DT, N>), dim3((unsigned)ceil_div(vocab, each)), dim3(1024), 0, s, (const T*)dy,
                            ids, (int)n, vocab, dim, scale, (int)each, (T*)dw);
         return launch_check("embed_few_kernel");
     }
-    const int64_t dw_bytes = vocab * dim * (int64_t)sizeof(T);
     const int fill = (int)std::min<int64_t>(ceil_div(dw_bytes, 16 * SORT_THREADS), 512);
     const int64_t blocks = n <= LDS_SORT ? 0 : ceil_div(n, BLOCK_SORT);
     // 2048 shares fill the compute units (8 waves each, times the chunks of
