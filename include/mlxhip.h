@@ -678,8 +678,9 @@ void mlxhip_stream_destroy_hip(void* stream);
  * mlxhip_graph_end, by the calling thread, are recorded instead of run;
  * mlxhip_graph_launch replays the whole sequence with the same arguments.
  * `stream` must be a created stream (not NULL). A graph holds workspaces of its
- * own for the calls recorded in it until it is freed (which waits for the
- * device): different graphs may replay at once, on any streams, but one graph's
+ * own for the calls recorded in it until it is freed, which waits for the stream of its
+ * last launch (while that is captured, the workspaces return later; destroy it before
+ * the graph by mlxhip_stream_destroy_hip only): different graphs may replay at once, on any streams, but one graph's
  * launches must not overlap each other. A graph captured by other means uses the
  * workspaces of the stream it was captured on, as eager calls on that stream do:
  * none of these may overlap. The Stream and decoder

@@ -17,6 +17,7 @@
 #include <initializer_list>
 #include <map>
 #include <mutex>
+#include <set>
 #include <string>
 
 #include "common.hpp"
@@ -257,6 +258,19 @@ struct WsKey {
         return slot < o.slot;
     }
 };
+}  // namespace
+}  // namespace mlxhip
+
+struct mlxhip_graph_t {
+    hipGraph_t graph = nullptr;
+    hipGraphExec_t exec = nullptr;
+    std::vector<void*> blocks;   // workspaces that its kernels use
+    bool pending = false;        // launched on `last`, not known to be over
+    hipStream_t last = nullptr;
+};
+
+namespace mlxhip {
+namespace {
 struct WsCache {
     std::mutex mu;
     std::map<WsKey, WsBlock> live;
@@ -268,8 +282,10 @@ struct WsCache {
         std::vector<void*> all;
     };
     std::map<std::pair<int, hipStream_t>, Recording> recordings;
-    // Blocks, and their devices, of graphs freed while the device could not be waited for.
-    std::vector<std::pair<int, void*>> freed;
+    // Graphs with workspaces, and those freed while their last launch's stream could not
+    // be waited for.
+    std::set<mlxhip_graph_t*> graphs;
+    std::vector<mlxhip_graph_t*> freed;
 };
 WsCache& ws_cache() {
     static WsCache* c = new WsCache();  // never destroyed: outlives late calls at exit
@@ -328,17 +344,70 @@ bool begin_recording(hipStream_t s) {
     return C.recordings.emplace(std::make_pair(dev, s), WsCache::Recording{}).second;
 }
 
-// Ends it (on any device: the caller's may have changed) and hands over its blocks.
-std::vector<void*> end_recording(hipStream_t s) {
+// Ends it (on any device: the caller's may have changed) and hands over its blocks;
+// false if none was under way.
+bool end_recording(hipStream_t s, std::vector<void*>* blocks) {
     WsCache& C = ws_cache();
     std::lock_guard<std::mutex> g(C.mu);
     for (auto it = C.recordings.begin(); it != C.recordings.end(); ++it)
         if (it->first.second == s) {
-            std::vector<void*> blocks = std::move(it->second.all);
+            *blocks = std::move(it->second.all);
             C.recordings.erase(it);
-            return blocks;
+            return true;
         }
-    return {};
+    return false;
+}
+
+void release_blocks(const std::vector<void*>& blocks) {
+    for (void* p : blocks) pool_release(p);
+}
+
+// Calls that wait for other streams are allowed in this scope while the thread captures.
+struct RelaxedCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool exchanged = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    ~RelaxedCapture() {
+        if (exchanged) (void)hipThreadExchangeStreamCaptureMode(&mode);
+        (void)hipGetLastError();
+    }
+};
+
+// Whether `s` may be asked for its work: not while it is captured, which that would end.
+bool may_ask(hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(s, &status);
+    if (e != hipSuccess) (void)hipGetLastError();
+    return e != hipErrorStreamCaptureImplicit && status == hipStreamCaptureStatusNone;
+}
+
+void drop_graph(mlxhip_graph_t* g) {
+    release_blocks(g->blocks);
+    (void)hipGraphExecDestroy(g->exec);
+    (void)hipGraphDestroy(g->graph);
+    delete g;
+}
+
+// Drops the freed graphs whose last launch is over by now.
+void release_freed() {
+    WsCache& C = ws_cache();
+    std::lock_guard<std::mutex> l(C.mu);
+    if (C.freed.empty()) return;
+    RelaxedCapture relaxed;
+    auto over = std::partition(C.freed.begin(), C.freed.end(), [](mlxhip_graph_t* g) {
+        return g->pending && !(may_ask(g->last) && hipStreamQuery(g->last) == hipSuccess);
+    });
+    for (auto it = over; it != C.freed.end(); ++it) drop_graph(*it);
+    C.freed.erase(over, C.freed.end());
+}
+
+// The work on `s` is over, and `s` about to be destroyed.
+void forget_launches(hipStream_t s) {
+    WsCache& C = ws_cache();
+    std::lock_guard<std::mutex> l(C.mu);
+    for (mlxhip_graph_t* g : C.graphs)
+        if (g->last == s) g->pending = false;
+    for (mlxhip_graph_t* g : C.freed)
+        if (g->last == s) g->pending = false;
 }
 }  // namespace
 
@@ -1379,25 +1448,35 @@ void* mlxhip_stream_create_hip(void) {
 
 void mlxhip_stream_destroy_hip(void* stream) {
     if (!stream) return;
+    // A recording under way on it ends; nothing of it has run.
+    std::vector<void*> blocks;
+    if (end_recording(as_stream(stream), &blocks)) {
+        hipGraph_t g = nullptr;
+        if (hipStreamEndCapture(as_stream(stream), &g) == hipSuccess && g) (void)hipGraphDestroy(g);
+        release_blocks(blocks);
+    }
     // The stream's cached workspaces go back to the pool once its work ends.
-    if (hipStreamSynchronize(as_stream(stream)) == hipSuccess) release_stream_workspaces(as_stream(stream));
+    if (hipStreamSynchronize(as_stream(stream)) == hipSuccess) {
+        release_stream_workspaces(as_stream(stream));
+        forget_launches(as_stream(stream));
+    }
     (void)hipGetLastError();
     (void)hipStreamDestroy(as_stream(stream));
 }
 
-struct mlxhip_graph_t {
-    hipGraph_t graph = nullptr;
-    hipGraphExec_t exec = nullptr;
-    std::vector<void*> blocks;  // workspaces that its kernels use
-    int device = 0;
-};
-
 int mlxhip_graph_begin(void* stream) {
     MLXHIP_TRY(ensure_device());
     if (!stream) return fail(MLXHIP_ERR_NULL_PTR, "graph_begin: the null stream cannot be recorded");
+    release_freed();
     MLXHIP_HIP(hipStreamBeginCapture(as_stream(stream), hipStreamCaptureModeThreadLocal));
-    for (void* p : end_recording(as_stream(stream))) pool_release(p);  // of a stream destroyed while recorded
-    (void)begin_recording(as_stream(stream));
+    std::vector<void*> blocks;
+    if (end_recording(as_stream(stream), &blocks)) release_blocks(blocks);  // of a stream that HIP destroyed
+    if (!begin_recording(as_stream(stream))) {
+        hipGraph_t g = nullptr;
+        if (hipStreamEndCapture(as_stream(stream), &g) == hipSuccess && g) (void)hipGraphDestroy(g);
+        (void)hipGetLastError();
+        return fail(MLXHIP_ERR_FFI_FAILED, "graph_begin: no current device");
+    }
     return MLXHIP_OK;
 }
 
@@ -1407,59 +1486,58 @@ mlxhip_graph_t* mlxhip_graph_end(void* stream) {
         return nullptr;
     }
     hipGraph_t g = nullptr;
-    const hipError_t e = hipStreamEndCapture(as_stream(stream), &g);
-    std::vector<void*> blocks = end_recording(as_stream(stream));
-    auto release = [&] {  // nothing recorded has run
-        for (void* p : blocks) pool_release(p);
-    };
-    if (e != hipSuccess || !g) {
-        if (g) (void)hipGraphDestroy(g);
-        release();
-        hip_fail(e != hipSuccess ? e : hipErrorInvalidValue, "hipStreamEndCapture");
-        return nullptr;
-    }
     hipGraphExec_t x = nullptr;
-    const hipError_t ei = hipGraphInstantiate(&x, g, nullptr, nullptr, 0);
-    if (ei != hipSuccess) {
-        (void)hipGraphDestroy(g);
-        release();
-        hip_fail(ei, "hipGraphInstantiate");
+    const hipError_t e = hipStreamEndCapture(as_stream(stream), &g);
+    std::vector<void*> blocks;
+    (void)end_recording(as_stream(stream), &blocks);
+    auto undo = [&](hipError_t why, const char* what) -> mlxhip_graph_t* {  // nothing recorded has run
+        if (g) (void)hipGraphDestroy(g);
+        release_blocks(blocks);
+        hip_fail(why, what);
         return nullptr;
+    };
+    if (e != hipSuccess || !g) return undo(e != hipSuccess ? e : hipErrorInvalidValue, "hipStreamEndCapture");
+    const hipError_t ei = hipGraphInstantiate(&x, g, nullptr, nullptr, 0);
+    if (ei != hipSuccess) return undo(ei, "hipGraphInstantiate");
+    release_freed();
+    mlxhip_graph_t* out = new mlxhip_graph_t{g, x, std::move(blocks), false, nullptr};
+    if (!out->blocks.empty()) {
+        WsCache& C = ws_cache();
+        std::lock_guard<std::mutex> l(C.mu);
+        C.graphs.insert(out);
     }
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    return new mlxhip_graph_t{g, x, std::move(blocks), dev};
+    return out;
 }
 
 int mlxhip_graph_launch(mlxhip_graph_t* g, void* stream) {
     if (!g) return fail(MLXHIP_ERR_NULL_PTR, "graph_launch: null graph");
     MLXHIP_HIP(hipGraphLaunch(g->exec, as_stream(stream)));
+    g->last = as_stream(stream);
+    g->pending = true;
     return MLXHIP_OK;
 }
 
 void mlxhip_graph_free(mlxhip_graph_t* g) {
     if (!g) return;
-    // Launches may still use the workspaces: they return to the pool once the
-    // device is idle. While a stream is recorded that cannot be waited for; they
-    // then return with a graph that is freed later.
-    if (!g->blocks.empty()) {
-        int cur = 0;
-        (void)hipGetDevice(&cur);
-        if (cur != g->device) (void)hipSetDevice(g->device);
-        WsCache& C = ws_cache();
+    release_freed();
+    WsCache& C = ws_cache();
+    bool pending;
+    {
         std::lock_guard<std::mutex> l(C.mu);
-        for (void* p : g->blocks) C.freed.emplace_back(g->device, p);
-        if (C.recordings.empty() && hipDeviceSynchronize() == hipSuccess) {
-            auto keep = std::partition(C.freed.begin(), C.freed.end(), [&](const auto& b) { return b.first != g->device; });
-            for (auto it = keep; it != C.freed.end(); ++it) pool_release(it->second);
-            C.freed.erase(keep, C.freed.end());
-        }
-        (void)hipGetLastError();
-        if (cur != g->device) (void)hipSetDevice(cur);
+        C.graphs.erase(g);
+        pending = g->pending;
     }
-    (void)hipGraphExecDestroy(g->exec);
-    (void)hipGraphDestroy(g->graph);
-    delete g;
+    // The last launch may still use the workspaces: they return to the pool behind it (an
+    // event recorded behind every launch would say so too, and took 2.5 to 4 us a launch).
+    // No other stream is waited for; while that one is captured the graph is left to a later
+    // call of these.
+    RelaxedCapture relaxed;
+    if (g->blocks.empty() || !pending || (may_ask(g->last) && hipStreamSynchronize(g->last) == hipSuccess)) {
+        drop_graph(g);
+    } else {
+        std::lock_guard<std::mutex> l(C.mu);
+        C.freed.push_back(g);
+    }
 }
 
 }  // extern "C"
