@@ -200,6 +200,10 @@ int mlxhip_last_shape_mismatch(int64_t* expected, size_t* expected_ndim,
  * after < 0. Cached blocks count as allocations. The environment variable
  * MLXHIP_FAIL_ALLOC_AFTER=n sets it at the first allocation. Returns MLXHIP_OK. */
 int mlxhip_debug_fail_allocations(int64_t after);
+/* For tests: pieces of the linear cross entropy's vocabulary hold at most
+ * piece_bytes (0: the default) from now on, 256 columns at least. Returns how many
+ * pieces the calls since the last one of this took. Process-wide. */
+int64_t mlxhip_debug_cross_entropy_pieces(int64_t piece_bytes);
 
 /* Number of visible HIP devices (0 when no GPU; never fails). */
 int mlxhip_device_count(void);

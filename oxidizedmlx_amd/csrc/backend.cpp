@@ -1035,6 +1035,8 @@ extern "C" {
 
 int mlxhip_abi_version(void) { return MLXHIP_ABI_VERSION; }
 
+int64_t mlxhip_debug_cross_entropy_pieces(int64_t piece_bytes) { return linear_cross_entropy_pieces(piece_bytes); }
+
 int mlxhip_debug_fail_allocations(int64_t after) {
     g_alloc_budget.store(after < 0 ? -1 : after);
     return MLXHIP_OK;

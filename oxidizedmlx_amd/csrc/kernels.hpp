@@ -97,6 +97,9 @@ int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t
                              const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
                              hipStream_t s);
 
+// mlxhip_debug_cross_entropy_pieces.
+int64_t linear_cross_entropy_pieces(int64_t piece_bytes);
+
 // lse of rows with a target from their loss: loss + x_r . w_target (f32).
 int linear_cross_entropy_lse(const float* x, const float* w, const int32_t* targets, const float* loss, float* lse,
                              int64_t rows, int64_t dim, int64_t vocab, hipStream_t s);

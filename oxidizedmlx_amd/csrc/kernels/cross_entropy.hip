@@ -31,6 +31,7 @@
 #include "elem.hpp"
 
 #include <algorithm>
+#include <atomic>
 
 namespace mlxhip {
 namespace {
@@ -40,8 +41,10 @@ using ce::counted;
 using dev::Elem;
 
 constexpr float LN2 = 0.69314718055994530942f;
-// Bytes of a piece's dS, and of a copied piece of W.
+// Bytes of a piece's dS, and of a copied piece of W; mlxhip_debug_cross_entropy_pieces
+// sets others and counts the pieces.
 constexpr int64_t PIECE_BYTES = int64_t(512) << 20;
+std::atomic<int64_t> g_piece_bytes{PIECE_BYTES}, g_pieces{0};
 
 // 2^e with the largest magnitude m below it (1/2 of it at least); 15 for an m
 // that says nothing, so that the factors made from it are 1.
@@ -354,10 +357,11 @@ struct Op {
     // Columns of a piece: with `ds`, dS, and `copied` planes of a copied piece of W within
     // the piece's bytes, offsets within a piece and the count of its tiles within 32 bits.
     int64_t width(bool ds, int copied) const {
+        const int64_t bytes = g_piece_bytes.load();
         int64_t w = std::min<int64_t>(vocab, (int64_t(1) << 29) / dim_p());
         w = std::min(w, (int64_t(1) << 43) / rows);
-        if (ds) w = std::min(w, PIECE_BYTES / (2 * SP) / rows);
-        if (copied) w = std::min(w, PIECE_BYTES / (2 * copied) / dim_p());
+        if (ds) w = std::min(w, bytes / (2 * SP) / rows);
+        if (copied) w = std::min(w, bytes / (2 * copied) / dim_p());
         if (w >= vocab) return vocab;
         w = std::max<int64_t>(w / 256 * 256, 256);
         // Pieces of like width: a short last one leaves compute units idle (1105 of
@@ -454,6 +458,7 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
     a.col_scale = (float*)(ws + ocol);
     if (copy_x) MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, nullptr, (float*)(ws + orow), (uint16_t*)(ws + ox), nullptr));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
+        g_pieces.fetch_add(1);
         a.n = std::min(width, o.vocab - v0);
         a.b = copy_w ? (uint16_t*)(ws + ow) : (const uint16_t*)o.w + v0 * o.dim;
         a.b_plane = a.n * o.dim_p();
@@ -510,6 +515,7 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         if (dw) MLXHIP_TRY(o.scales(dloss, row_scale, scale));
     if (xz || xg) MLXHIP_TRY(o.pack(o.x, o.rows, o.targets, dloss, scale, xz, xg));
     for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
+        g_pieces.fetch_add(1);
         const int64_t n = std::min(width, o.vocab - v0);
         if (wz || wg) MLXHIP_TRY(o.pack(o.w + v0 * o.dim, n, nullptr, nullptr, col_scale, wz, wg));
         Args z;
@@ -584,6 +590,11 @@ int linear_cross_entropy(int dt, const void* x, const void* w, const int32_t* ta
         }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "linear_cross_entropy: dtype %d (f32, bf16 or f16)", dt);
     return rc;
+}
+
+int64_t linear_cross_entropy_pieces(int64_t piece_bytes) {
+    g_piece_bytes.store(piece_bytes > 0 ? piece_bytes : PIECE_BYTES);
+    return g_pieces.exchange(0);
 }
 
 int linear_cross_entropy_lse(const float* x, const float* w, const int32_t* targets, const float* loss, float* lse,
