@@ -149,27 +149,28 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ p
 
 // As pack_kernel for f32: z is two f16 planes of the row times a power of two made from
 // its own largest magnitude (row_scale: what undoes it), so that no row takes digits
-// from another. A wave to a row.
+// from another. `lanes` (a power of two) to a row: a wave, fewer for short rows.
 __global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t dim,
                                                         int64_t dim_p, const int32_t* __restrict__ targets, int64_t vocab,
-                                                        float* __restrict__ row_scale, uint16_t* __restrict__ z,
-                                                        uint16_t* __restrict__ g) {
+                                                        int lanes, float* __restrict__ row_scale,
+                                                        uint16_t* __restrict__ z, uint16_t* __restrict__ g) {
     constexpr int F32 = MLXHIP_DTYPE_F32;
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+    const int lane = threadIdx.x % lanes, each = 256 / lanes;
+    for (int64_t r = (int64_t)blockIdx.x * each + threadIdx.x / lanes; r < rows; r += (int64_t)gridDim.x * each) {
         const float* p = src + r * dim;
         const bool on = !targets || counted(targets[r], vocab);
         float m = 0.0f;
-        for (int64_t c = lane * 8; c < dim; c += 512) {
+        for (int64_t c = lane * 8; c < dim; c += lanes * 8) {
             float v[8];
             load8<F32>(p, c, dim, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
         }
-        const int e2 = exponent(dev::wave_max(m));
+        for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const int e2 = exponent(m);
         if (lane == 0) row_scale[r] = ldexpf(1.0f, e2 - 15);
         const float f = ldexpf(1.0f, 15 - e2);
-        for (int64_t c = lane * 8; c < dim_p; c += 512) {
+        for (int64_t c = lane * 8; c < dim_p; c += lanes * 8) {
             float v[8], u[8];
             load8<F32>(p, c, dim, v);
 #pragma unroll
@@ -322,9 +323,11 @@ struct Op {
     // operands' dloss x.
     int pack(const T* src, int64_t n, const int32_t* t, const float* dloss, float* scale, uint16_t* z, uint16_t* g) const {
         if constexpr (OT == MLXHIP_DTYPE_F32) {
-            const int64_t groups = std::min<int64_t>(ceil_div(n, 4), 16384);
-            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)groups), dim3(256), 0, s, src, n, dim, dim_p(), t, vocab, scale,
-                               z, g);
+            int lanes = 1;
+            while (lanes < 64 && lanes * 8 < dim) lanes *= 2;
+            const int64_t groups = std::min<int64_t>(ceil_div(n, 256 / lanes), 16384);
+            hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)groups), dim3(256), 0, s, src, n, dim, dim_p(), t, vocab, lanes,
+                               scale, z, g);
         } else {
             const int64_t groups = std::min<int64_t>(ceil_div(n * dim_p() / 8, 1024), 2048);
             hipLaunchKernelGGL((pack_kernel<OT>), dim3((unsigned)groups), dim3(1024), 0, s, src, n, dim, dim_p(), t, vocab,
