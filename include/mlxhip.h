@@ -483,7 +483,8 @@ int mlxhip_embedding_vjp_rows(int32_t dtype, const void* dy, const int32_t* ids,
  * dtype: F32, BF16 or F16, of x, w, dx and dw; loss, lse and dloss are f32, as
  * are the logits, sums and products' accumulators. dx and dw are rounded once,
  * as they are stored. F32 products are f32 for the loss of up to 128 rows and the
- * gradients of up to 64 (vocab up to 2^22). Beyond that the logits are formed of
+ * gradients of up to 64 (vocab up to 2^26 at 128 rows, 2^22 at 64: what they keep
+ * of each entry within 1 GiB). Beyond that the logits are formed of
  * operands of 22 bits each, with an absolute error of 2^-39 of the largest value of
  * the same row of x or w where that is more, products below 2^-22 of a term left out,
  * and the gradients of operands and dS of 24 bits of any size. dS of 16-bit operands is

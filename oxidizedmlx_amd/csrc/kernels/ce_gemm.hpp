@@ -170,14 +170,15 @@ struct Args {
 
 // Few rows (ce_few.hip, with what each bound measured): the loss of up to 128 f32
 // rows, or 64 of 16 bits where the tiles would need a copy of W; the gradients of up
-// to 64 f32 rows, or 16 of 16 bits. Beyond FEW_VOCAB entries the grids would pass 2^32
-// work items and dS^T 1 GiB.
-constexpr int64_t FEW_VOCAB = int64_t(1) << 22;
+// to 64 f32 rows, or 16 of 16 bits. What they keep of each entry stays within FEW_BYTES:
+// the statistics of its 64th and the row of dS^T.
+constexpr int64_t FEW_BYTES = int64_t(1) << 30;
+inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 inline bool few_loss(int dt, bool copy_w, int64_t rows, int64_t vocab) {
-    return copy_w && rows <= (dt == MLXHIP_DTYPE_F32 ? 128 : 64) && vocab <= FEW_VOCAB;
+    return copy_w && rows <= (dt == MLXHIP_DTYPE_F32 ? 128 : 64) && vocab / 64 * rows * 8 <= FEW_BYTES;
 }
 inline bool few_grad(int dt, int64_t rows, int64_t vocab) {
-    return rows <= (dt == MLXHIP_DTYPE_F32 ? 64 : 16) && vocab <= FEW_VOCAB;
+    return rows <= (dt == MLXHIP_DTYPE_F32 ? 64 : 16) && vocab * few_ds_rows(rows) * 4 <= FEW_BYTES;
 }
 struct FewArgs {
     const void *x = nullptr, *w = nullptr;
@@ -191,7 +192,6 @@ struct FewArgs {
     void* dw = nullptr;         // [vocab][dim] or null
     int64_t ldx = 0, slices = 0, slice = 0;  // of 4 * slice entries each; slice a multiple of 16
 };
-inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 // Max and sum of exp(z - max) of two groups of a row.
 __device__ inline void merge(float& m, float& s, float m2, float s2) {
