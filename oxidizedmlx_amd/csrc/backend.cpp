@@ -448,6 +448,11 @@ void Scratch::release_all() {
 
 // ── eval_node on device operands ──────────────────────────────────────────
 
+// mlxhip_linear_cross_entropy_vjp, with the loss where it is known (or null).
+int cross_entropy_vjp(int32_t dtype, const void* x, const void* w, const int32_t* targets, const float* lse,
+                      const float* loss, const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
+                      hipStream_t s);
+
 namespace {
 
 bool same_shape(const mlxhip_input_t& a, const mlxhip_input_t& b) {
@@ -731,8 +736,8 @@ int eval_linear_cross_entropy(const mlxhip_op_t& op, const mlxhip_input_t* in, s
     const bool dx = !op.has_axis || op.axis == 0, dw = !op.has_axis || op.axis == 1;
     MLXHIP_TRY(expect_len((dx ? rows * dim : 0) + (dw ? vocab * dim : 0), out_n, what));
     MLXHIP_TRY(linear_cross_entropy_lse(x.data, w.data, ids, in[4].data, lse, rows, dim, vocab, s));
-    return mlxhip_linear_cross_entropy_vjp(MLXHIP_DTYPE_F32, x.data, w.data, ids, lse, in[0].data, dx && rows ? out : nullptr,
-                                           dw ? out + (dx ? rows * dim : 0) : nullptr, rows, dim, vocab, s);
+    return cross_entropy_vjp(MLXHIP_DTYPE_F32, x.data, w.data, ids, lse, in[4].data, in[0].data, dx && rows ? out : nullptr,
+                             dw ? out + (dx ? rows * dim : 0) : nullptr, rows, dim, vocab, s);
 }
 
 }  // namespace
@@ -1354,15 +1359,7 @@ int mlxhip_linear_cross_entropy(int32_t dtype, const void* x, const void* w, con
 int mlxhip_linear_cross_entropy_vjp(int32_t dtype, const void* x, const void* w, const int32_t* targets,
                                     const float* lse, const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim,
                                     int64_t vocab, void* stream) {
-    const char* what = "linear_cross_entropy_vjp";
-    MLXHIP_TRY(check_cross_entropy(what, rows, dim, vocab));
-    if (rows > 0) MLXHIP_TRY(check_operands(what, dtype, {x, w}, {targets, lse, dloss}));
-    if (dx) MLXHIP_TRY(check_operands(what, dtype, {dx}));
-    if (dw) MLXHIP_TRY(check_operands(what, dtype, {dw}));
-    if (!dx && !dw) return check_operands(what, dtype, {});
-    MLXHIP_TRY(ensure_device());
-    const auto lock = launches_together(as_stream(stream));
-    return linear_cross_entropy_vjp(dtype, x, w, targets, lse, dloss, dx, dw, rows, dim, vocab, as_stream(stream));
+    return cross_entropy_vjp(dtype, x, w, targets, lse, nullptr, dloss, dx, dw, rows, dim, vocab, as_stream(stream));
 }
 
 int mlxhip_ew_chain(const mlxhip_ew_instr_t* prog, size_t n_instr, const float* const* inputs, size_t n_inputs,
@@ -1543,3 +1540,21 @@ void mlxhip_graph_free(mlxhip_graph_t* g) {
 }
 
 }  // extern "C"
+
+namespace mlxhip {
+
+int cross_entropy_vjp(int32_t dtype, const void* x, const void* w, const int32_t* targets, const float* lse,
+                      const float* loss, const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
+                      hipStream_t s) {
+    const char* what = "linear_cross_entropy_vjp";
+    MLXHIP_TRY(check_cross_entropy(what, rows, dim, vocab));
+    if (rows > 0) MLXHIP_TRY(check_operands(what, dtype, {x, w}, {targets, lse, dloss}));
+    if (dx) MLXHIP_TRY(check_operands(what, dtype, {dx}));
+    if (dw) MLXHIP_TRY(check_operands(what, dtype, {dw}));
+    if (!dx && !dw) return check_operands(what, dtype, {});
+    MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(s);
+    return linear_cross_entropy_vjp(dtype, x, w, targets, lse, loss, dloss, dx, dw, rows, dim, vocab, s);
+}
+
+}  // namespace mlxhip

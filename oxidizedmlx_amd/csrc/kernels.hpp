@@ -92,9 +92,10 @@ int embedding_vjp_rows(int dt, const void* dy, const int32_t* ids, void* dw, int
                        float scale, hipStream_t s);
 int linear_cross_entropy(int dt, const void* x, const void* w, const int32_t* targets, float* loss, float* lse,
                          int64_t rows, int64_t dim, int64_t vocab, hipStream_t s);
-// dx or dw may be null (that gradient is not formed).
+// dx or dw may be null (that gradient is not formed), and loss, which for f32 operands
+// says what p of a target misses to 1 more exactly than an lse made from it.
 int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t* targets, const float* lse,
-                             const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
+                             const float* loss, const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
                              hipStream_t s);
 
 // mlxhip_debug_cross_entropy_pieces.

@@ -233,6 +233,12 @@ __device__ inline void leave_stats(const FewArgs& g, int64_t v0, int64_t r0, int
     g.stats[tile * g.rows + r0 + r] = make_float2(m, s);
 }
 
+// p less 1 at the target, there from the loss where that is known (hit).
+__device__ inline float p_of(float z, float lse, bool target, bool known, float hit) {
+    const float p = __builtin_amdgcn_exp2f((z - lse) * LOG2E);
+    return !target ? p : known ? hit : p - 1.0f;
+}
+
 // dS^T of the same from z.
 template <int T, int NB>
 __device__ inline void leave_ds(const FewArgs& g, int64_t v0, const f32x4 (&acc)[T][NB]) {
@@ -243,14 +249,50 @@ __device__ inline void leave_ds(const FewArgs& g, int64_t v0, const f32x4 (&acc)
         const int64_t target = r < g.rows ? g.targets[r] : -1;
         const bool on = target >= 0 && target < g.vocab;
         const float lse = on ? g.lse[r] : 0.0f, f = on ? g.dloss[r] : 0.0f;
+        const float hit = on && g.loss ? expm1f(-g.loss[r]) : 0.0f;
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int64_t v = v0 + 16 * t + 4 * q + e;
-                const float p = __builtin_amdgcn_exp2f((acc[t][b][e] - lse) * LOG2E) - (v == target ? 1.0f : 0.0f);
+                const float p = p_of(acc[t][b][e], lse, v == target, g.loss, hit);
                 if (v < g.vocab) g.ds[v * (16 * NB) + r] = on ? p * f : 0.0f;
             }
+    }
+}
+
+// dS of the same from z, for NB tiles of 16 rows from r0 on, as CE_DS leaves it; zeros
+// behind the entries up to a multiple of 8.
+template <int DT, int T, int NB>
+__device__ inline void leave_planes(const FewArgs& g, int64_t v0, int64_t r0, const f32x4 (&acc)[T][NB]) {
+    constexpr int GT = G_TYPE<DT>, SP = DS_PLANES<DT>;
+    const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int64_t r = r0 + 16 * b + i;
+        if (r >= g.rows) continue;
+        const int64_t target = g.targets[r];
+        const bool on = target >= 0 && target < g.whole;
+        const float hit = on && g.loss ? expm1f(-g.loss[r]) : 0.0f;
+        const float lse = on ? g.lse[r] : 0.0f, f = !on ? 0.0f : DT == MLXHIP_DTYPE_F16 ? DS_F16 : g.dloss[r];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const int64_t v = v0 + 16 * t + 4 * q;
+            if (v >= (g.vocab + 7) / 8 * 8) continue;
+            float d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = p_of(acc[t][b][e], lse, g.first + v + e == target, g.loss, hit);
+                d[e] = on && v + e < g.vocab ? p * f : 0.0f;
+            }
+#pragma unroll
+            for (int p = 0; p < SP; ++p) {
+                *reinterpret_cast<u32x2*>(g.planes + p * g.plane + r * g.ldc + v) =
+                    u32x2{gemm16::pack2<GT>(d[0], d[1]), gemm16::pack2<GT>(d[2], d[3])};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] -= dev::to_f32<GT>(dev::from_f32<GT>(d[e]));
+            }
+        }
     }
 }
 
@@ -270,7 +312,8 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
 // reaches 154 TFLOP/s). 32 entries a wave, 32 columns a chunk, or two or five waves
 // to a SIMD: 1 - 15 % slower; 128 rows a workgroup: 64 rows take 97 instead of 57.
 constexpr int WIDE_ROWS = 64, WIDE_T = 1, WIDE_ENTRIES = 64 * WIDE_T;
-template <bool DS>
+enum Wide { WIDE_STATS, WIDE_DS, WIDE_PLANES };
+template <int OUT>
 __global__ __launch_bounds__(256, 4) void wide_kernel(FewArgs g, int64_t row_blocks, int64_t tiles) {
     constexpr int NB = WIDE_ROWS / 16, T = WIDE_T, KC = 64, S = KC / 16, PIECES = WIDE_ROWS * KC / 4 / 256;
     constexpr int DT = MLXHIP_DTYPE_F32;
@@ -345,7 +388,8 @@ __global__ __launch_bounds__(256, 4) void wide_kernel(FewArgs g, int64_t row_blo
         use(wv[1], 1);
         if (k + 2 * KC < g.dim) stage(0);
     }
-    if constexpr (DS) leave_ds<T, NB>(g, v0, acc);  // of one block of rows
+    if constexpr (OUT == WIDE_DS) leave_ds<T, NB>(g, v0, acc);  // of one block of rows
+    else if constexpr (OUT == WIDE_PLANES) leave_planes<DT, T, NB>(g, v0, r0, acc);
     else leave_stats<T, NB>(g, v0, r0, tile, acc);
 }
 
@@ -357,6 +401,16 @@ __global__ __launch_bounds__(256) void few_ds_kernel(FewArgs g) {
     f32x4 acc[T][NB];
     few_logits<DT, NB, ODD>(g, v0, threadIdx.x & 63, acc);
     leave_ds<T, NB>(g, v0, acc);
+}
+
+template <int DT, int NB, bool ODD>
+__global__ __launch_bounds__(256) void few_planes_kernel(FewArgs g) {
+    constexpr int T = TILES<NB>;
+    const int64_t v0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 * T;
+    if (v0 >= g.vocab) return;
+    f32x4 acc[T][NB];
+    few_logits<DT, NB, ODD>(g, v0, threadIdx.x & 63, acc);
+    leave_planes<DT, T, NB>(g, v0, 0, acc);
 }
 
 template <int DT, int NB>
@@ -498,15 +552,37 @@ int launch_loss(const FewArgs& g, hipStream_t s) {
     return launch_check("few_stats_kernel");
 }
 
+template <int OUT>
+int launch_wide(const FewArgs& g, hipStream_t s) {
+    const int64_t blocks = ceil_div(g.rows, WIDE_ROWS), tiles = ceil_div(g.vocab, WIDE_ENTRIES);
+    hipLaunchKernelGGL((wide_kernel<OUT>), dim3((unsigned)(ceil_div(tiles, 8) * 8 * blocks)), dim3(256), 0, s, g, blocks, tiles);
+    return launch_check("wide_kernel");
+}
+
+template <int DT, int NB>
+int launch_planes(const FewArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div(g.vocab, ENTRIES<NB>));
+    if (DT != MLXHIP_DTYPE_F32 && odd_rows(g))
+        hipLaunchKernelGGL((few_planes_kernel<DT, NB, DT != MLXHIP_DTYPE_F32>), grid, dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((few_planes_kernel<DT, NB, false>), grid, dim3(256), 0, s, g);
+    return launch_check("few_planes_kernel");
+}
+
+template <int DT>
+int typed_planes(const FewArgs& g, hipStream_t s) {
+    if (g.rows <= 16) return launch_planes<DT, 1>(g, s);
+    if (g.rows <= 32) return launch_planes<DT, 2>(g, s);
+    if constexpr (DT == MLXHIP_DTYPE_F32) return launch_wide<WIDE_PLANES>(g, s);
+    else return launch_planes<DT, 4>(g, s);
+}
+
 template <int DT>
 int typed_loss(const FewArgs& g, hipStream_t s) {
     if (g.rows <= 16) return launch_loss<DT, 1>(g, s);
     if (g.rows <= 32) return launch_loss<DT, 2>(g, s);
     if constexpr (DT == MLXHIP_DTYPE_F32) {
-        const int64_t blocks = ceil_div(g.rows, WIDE_ROWS), tiles = ceil_div(g.vocab, WIDE_ENTRIES);
-        hipLaunchKernelGGL((wide_kernel<false>), dim3((unsigned)(ceil_div(tiles, 8) * 8 * blocks)), dim3(256), 0, s, g, blocks,
-                           tiles);
-        return launch_check("wide_kernel");
+        return launch_wide<WIDE_STATS>(g, s);
     } else {
         return launch_loss<DT, 4>(g, s);
     }
@@ -515,9 +591,8 @@ int typed_loss(const FewArgs& g, hipStream_t s) {
 template <int DT, int NB>
 int launch_grad(const FewArgs& g, hipStream_t s) {
     if constexpr (NB == 4) {
-        const int64_t tiles = ceil_div(g.vocab, WIDE_ENTRIES);
-        hipLaunchKernelGGL((wide_kernel<true>), dim3((unsigned)(ceil_div(tiles, 8) * 8)), dim3(256), 0, s, g, (int64_t)1, tiles);
-    } else {
+        MLXHIP_TRY(launch_wide<WIDE_DS>(g, s));
+    } else if (g.form_ds) {
         const dim3 grid((unsigned)ceil_div(g.vocab, ENTRIES<NB>));
         if (DT != MLXHIP_DTYPE_F32 && odd_rows(g))
             hipLaunchKernelGGL((few_ds_kernel<DT, NB, DT != MLXHIP_DTYPE_F32>), grid, dim3(256), 0, s, g);
@@ -542,6 +617,11 @@ int64_t ce_few_tiles(int dt, int64_t rows, int64_t vocab) {
 int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s) {
     if (dt == MLXHIP_DTYPE_F32) return ce::typed_loss<MLXHIP_DTYPE_F32>(g, s);
     return dt == MLXHIP_DTYPE_BF16 ? ce::typed_loss<MLXHIP_DTYPE_BF16>(g, s) : ce::typed_loss<MLXHIP_DTYPE_F16>(g, s);
+}
+
+int ce_few_planes(int dt, const ce::FewArgs& g, hipStream_t s) {
+    if (dt == MLXHIP_DTYPE_F32) return ce::typed_planes<MLXHIP_DTYPE_F32>(g, s);
+    return dt == MLXHIP_DTYPE_BF16 ? ce::typed_planes<MLXHIP_DTYPE_BF16>(g, s) : ce::typed_planes<MLXHIP_DTYPE_F16>(g, s);
 }
 
 int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s) {

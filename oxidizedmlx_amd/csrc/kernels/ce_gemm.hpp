@@ -9,6 +9,8 @@
 //   CE_DX     f32 sums of dS W over a slice of K, added to those of the
 //             pieces of the vocabulary before.
 //   CE_DW     dS^T x, in the operands' type.
+//   CE_DST    dS^T of up to 16 rows of 16 bits in f32, for ce_few.hip: z as CE_STATS forms
+//             it, or p - 1 of a certain target would be the difference.
 //
 // A plane is a 16-bit value: hi is the f32 value rounded, the next plane what that
 // leaves, rounded. The products run over pairs of planes, those whose places add
@@ -61,7 +63,7 @@ using gemm16::f32x4;
 using gemm16::u32x2;
 using gemm16::u32x4;
 
-enum Product { CE_STATS = 0, CE_DS = 1, CE_DX = 2, CE_DW = 3 };
+enum Product { CE_STATS = 0, CE_DS = 1, CE_DX = 2, CE_DW = 3, CE_DST = 4 };
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -151,13 +153,15 @@ struct Args {
     int tiles_m = 0, tiles_n = 0;
     int splits = 1;          // CE_DX: slices of K, of k_chunk (a multiple of 32) each
     int64_t k_chunk = 0;
-    // Of each row of x: its target, and for CE_DS the forward's lse and dloss.
+    // Of each row of x: its target, and for CE_DS the forward's lse, dloss and, of f32
+    // operands, its loss or null (p - 1 of the target is then made from that).
     const int32_t* targets = nullptr;
     int64_t v0 = 0, vocab = 0;  // the piece's first column, the whole vocabulary
-    const float *lse = nullptr, *dloss = nullptr;
+    const float *lse = nullptr, *dloss = nullptr, *loss = nullptr;
     float2* stats = nullptr;    // CE_STATS: [tiles of columns][m], from this launch's first tile on
     float* target_z = nullptr;  // CE_STATS: [m]
     uint16_t* ds = nullptr;     // CE_DS: [DS_PLANES][m][ldc]
+    float* dst = nullptr;       // CE_DST: [n][16]
     float* dx = nullptr;        // CE_DX: [splits][m][ldc]
     bool add = false;           // CE_DX: add to what is there
     void* dw = nullptr;         // CE_DW: [m][ldc]
@@ -170,7 +174,8 @@ struct Args {
 
 // Few rows (ce_few.hip, with what each bound measured): the loss of up to 128 f32
 // rows, or 64 of 16 bits where the tiles would need a copy of W; the gradients of up
-// to 64 f32 rows, or 16 of 16 bits. What they keep of each entry stays within FEW_BYTES:
+// to 64 f32 rows, or 16 of 16 bits. Where only the loss is formed there, it leaves dS of
+// more rows to the tiles as CE_DS does: z has to be the same in both. What they keep of each entry stays within FEW_BYTES:
 // the statistics of its 64th and the row of dS^T.
 constexpr int64_t FEW_BYTES = int64_t(1) << 30;
 inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
@@ -184,13 +189,18 @@ struct FewArgs {
     const void *x = nullptr, *w = nullptr;
     int64_t rows = 0, dim = 0, vocab = 0;
     const int32_t* targets = nullptr;
-    const float *lse = nullptr, *dloss = nullptr;
+    const float *lse = nullptr, *dloss = nullptr, *loss = nullptr;
     float2* stats = nullptr;    // [ce_few_tiles()][rows]
     float* target_z = nullptr;
     float* ds = nullptr;        // dS^T [vocab][few_ds_rows(rows)]
+    bool form_ds = true;        // or it is there
     float* dx = nullptr;        // [slices][rows][ldx] or null
     void* dw = nullptr;         // [vocab][dim] or null
     int64_t ldx = 0, slices = 0, slice = 0;  // of 4 * slice entries each; slice a multiple of 16
+    // dS as CE_DS leaves it instead, of the entries `first` on of `whole`: planes of
+    // [rows][ldc], `plane` elements apart.
+    uint16_t* planes = nullptr;
+    int64_t ldc = 0, plane = 0, first = 0, whole = 0;
 };
 
 // Max and sum of exp(z - max) of two groups of a row.
@@ -349,7 +359,7 @@ __device__ inline void scale_columns(f32x16 (&acc)[TM][TN], const float* col_sca
 template <int PRODUCT, int MT, int OT, class C>
 __global__ __attribute__((amdgpu_flat_work_group_size(C::THREADS, C::THREADS), amdgpu_waves_per_eu(2, 2)))
 void ce_gemm_kernel(Args g) {
-    constexpr bool KCA = PRODUCT != CE_DW, KCB = PRODUCT <= CE_DS;
+    constexpr bool KCA = PRODUCT != CE_DW, KCB = PRODUCT <= CE_DS || PRODUCT == CE_DST;
     constexpr int STAGES = C::STAGES, TM = C::TM, TN = C::TN, WAVES = C::WAVES, PA = C::PA, PB = C::PB;
     constexpr Pairs<PA, PB> pairs;
     __shared__ __attribute__((aligned(1024))) char smem_raw[STAGES * C::STAGE_BYTES + WAVES * C::EPI];
@@ -538,18 +548,21 @@ void ce_gemm_kernel(Args g) {
                 for (int w = 1; w < C::WN; ++w) merge(a.x, a.y, red[2 * w * C::BM + tid], red[(2 * w + 1) * C::BM + tid]);
                 g.stats[n0 / C::BN * g.m + m0 + tid] = a;
             }
-        } else if constexpr (PRODUCT == CE_DS) {
+        } else if constexpr (PRODUCT == CE_DS || PRODUCT == CE_DST) {
             if constexpr (PA > 1) scale_columns(acc, g.col_scale + col0);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 const int64_t r = row0 + 32 * i;
-                float shift = 0.0f, f = 0.0f, up = LOG2E;
+                float shift = 0.0f, f = 0.0f, fix = 1.0f, up = LOG2E;
                 int tc = -1;
                 if (r < g.m) {
                     const int32_t t = g.targets[r];
                     if (counted(t, g.vocab)) {
                         shift = -g.lse[r] * LOG2E;
-                        f = OT == MLXHIP_DTYPE_F16 ? DS_F16 : g.dloss[r];
+                        f = OT == MLXHIP_DTYPE_F16 && PRODUCT == CE_DS ? DS_F16 : g.dloss[r];
+                        // What the rounding of shift leaves: near a certain target it would be
+                        // most of p - 1.
+                        fix = __builtin_amdgcn_exp2f(__builtin_fmaf(-g.lse[r], LOG2E, -shift));
                     }
                     if constexpr (PA > 1) up *= g.row_scale[r];
                     tc = column_of(t, g.v0 + col0, 32 * TN);
@@ -558,13 +571,15 @@ void ce_gemm_kernel(Args g) {
                 for (int j = 0; j < TN; ++j)
 #pragma unroll
                     for (int v = 0; v < 16; ++v)
-                        acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], up, shift)) * f;
+                        acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], up, shift)) * (f * fix);
                 if (__ballot(tc >= 0)) {  // some lane holds its row's target
+                    const bool known = OT == MLXHIP_DTYPE_F32 && g.loss;
+                    const float hit = known && tc >= 0 ? expm1f(-g.loss[r]) * f : 0.0f;
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int v = 0; v < 16; ++v)
-                            if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) acc[i][j][v] -= f;
+                            if (tc == 32 * j + 8 * (v >> 2) + (v & 3)) acc[i][j][v] = known ? hit : acc[i][j][v] - f;
                 }
                 // A row without a target has no dS, whatever x, lse and dloss hold.
                 const bool on = r < g.m && counted(g.targets[r], g.vocab);
@@ -574,6 +589,18 @@ void ce_gemm_kernel(Args g) {
 #pragma unroll
                         for (int v = 0; v < 16; ++v) acc[i][j][v] = on ? acc[i][j][v] : 0.0f;
                 }
+            }
+            if constexpr (PRODUCT == CE_DST) {
+                if (row0 < 16) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const int64_t c = col0 + 32 * j + 8 * (v >> 2) + (v & 3);
+                            if (c < g.n) g.dst[c * 16 + row0] = acc[0][j][v];
+                        }
+                }
+                continue;
             }
             if (n0 + C::BN > g.n) {
 #pragma unroll
@@ -646,6 +673,9 @@ int dispatch(int which, bool large, const Args& a, hipStream_t s) {
     switch (which) {
         case CE_STATS: return product<CE_STATS, ZT, OT, ZP, ZP>(large, a, s);
         case CE_DS: return product<CE_DS, ZT, OT, ZP, ZP>(large, a, s);
+        case CE_DST:
+            if constexpr (OT != MLXHIP_DTYPE_F32) return product<CE_DST, ZT, OT, ZP, ZP>(large, a, s);
+            return fail(MLXHIP_ERR_INVALID_ARGUMENT, "linear_cross_entropy: no dS^T of f32 tiles");
         case CE_DX: return product<CE_DX, GT, OT, SP, W_PLANES<OT>>(large, a, s);
         default: return product<CE_DW, GT, OT, SP, X_PLANES<OT>>(large, a, s);
     }
@@ -658,6 +688,7 @@ int ce_gemm_bf16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f16(int which, bool large, const ce::Args& a, hipStream_t s);
 int ce_gemm_f32(int which, bool large, const ce::Args& a, hipStream_t s);
 // ce_few.hip
+int ce_few_planes(int dt, const ce::FewArgs& g, hipStream_t s);
 int ce_few_loss(int dt, const ce::FewArgs& g, hipStream_t s);
 int ce_few_grad(int dt, const ce::FewArgs& g, hipStream_t s);
 int64_t ce_few_tiles(int dt, int64_t rows, int64_t vocab);  // of the loss's statistics

@@ -149,7 +149,7 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* __restrict__ p
 
 // As pack_kernel for f32: z is two f16 planes of the row times a power of two made from
 // its own largest magnitude (row_scale: what undoes it), so that no row takes digits
-// from another. `lanes` (a power of two) to a row: a wave, fewer for short rows.
+// from another; either of z and g may be null. `lanes` (a power of two) to a row: a wave, fewer for short rows.
 __global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t dim,
                                                         int64_t dim_p, const int32_t* __restrict__ targets, int64_t vocab,
                                                         int lanes, float* __restrict__ row_scale,
@@ -159,17 +159,20 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict_
     for (int64_t r = (int64_t)blockIdx.x * each + threadIdx.x / lanes; r < rows; r += (int64_t)gridDim.x * each) {
         const float* p = src + r * dim;
         const bool on = !targets || counted(targets[r], vocab);
-        float m = 0.0f;
-        for (int64_t c = lane * 8; c < dim; c += lanes * 8) {
-            float v[8];
-            load8<F32>(p, c, dim, v);
+        float f = 1.0f;
+        if (z) {
+            float m = 0.0f;
+            for (int64_t c = lane * 8; c < dim; c += lanes * 8) {
+                float v[8];
+                load8<F32>(p, c, dim, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(v[e]));
+            }
+            for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            const int e2 = exponent(m);
+            if (lane == 0) row_scale[r] = ldexpf(1.0f, e2 - 15);
+            f = ldexpf(1.0f, 15 - e2);
         }
-        for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        const int e2 = exponent(m);
-        if (lane == 0) row_scale[r] = ldexpf(1.0f, e2 - 15);
-        const float f = ldexpf(1.0f, 15 - e2);
         for (int64_t c = lane * 8; c < dim_p; c += lanes * 8) {
             float v[8], u[8];
             load8<F32>(p, c, dim, v);
@@ -178,7 +181,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const float* __restrict_
                 v[e] = on ? v[e] : 0.0f;
                 u[e] = v[e] * f;
             }
-            store_planes<MLXHIP_DTYPE_F16, ce::Z_PLANES<F32>>(u, c, rows * dim_p, z + r * dim_p);
+            if (z) store_planes<MLXHIP_DTYPE_F16, ce::Z_PLANES<F32>>(u, c, rows * dim_p, z + r * dim_p);
             if (g) store_planes<MLXHIP_DTYPE_BF16, ce::X_PLANES<F32>>(v, c, rows * dim_p, g + r * dim_p);
         }
     }
@@ -408,12 +411,14 @@ int few_loss(const Op<OT>& o, float* loss, float* lse) {
 }
 
 template <int OT>
-int few_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Elem<OT>::type* dx,
+int few_grad(const Op<OT>& o, const float* lse, const float* loss, const float* dloss, typename Elem<OT>::type* dx,
              typename Elem<OT>::type* dw) {
     ce::FewArgs g = few_args(o);
     g.lse = lse;
+    g.loss = loss;
     g.dloss = dloss;
     g.dw = dw;
+    const bool tiles_z = !ce::few_loss(OT, !o.in_place(o.w), o.rows, o.vocab), copy_x = tiles_z && !o.in_place(o.x);
     // Eight waves to a compute unit, four of a workgroup along the vocabulary.
     g.ldx = ceil_div(o.dim, 4) * 4;
     const int64_t most = std::max<int64_t>(512 / ceil_div(o.dim, 16 * Elem<OT>::VEC), 1);
@@ -421,11 +426,33 @@ int few_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
     g.slices = ceil_div(o.vocab, 4 * g.slice);
     Carve c;
     const size_t od = c.take((size_t)o.vocab * ce::few_ds_rows(o.rows) * 4),
-                 ox = c.take(dx ? (size_t)g.slices * o.rows * g.ldx * 4 : 0);
+                 ox = c.take(dx ? (size_t)g.slices * o.rows * g.ldx * 4 : 0), oxz = c.take(copy_x ? o.bytes(o.rows, 1) : 0);
     char* ws = nullptr;
     MLXHIP_TRY(stream_workspace(o.s, WS_CE, c.used, reinterpret_cast<void**>(&ws)));
     g.ds = (float*)(ws + od);
     g.dx = dx ? (float*)(ws + ox) : nullptr;
+    if (tiles_z) {
+        // The loss took z from the tiles.
+        g.form_ds = false;
+        uint16_t* xz = copy_x ? (uint16_t*)(ws + oxz) : nullptr;
+        if (copy_x) MLXHIP_TRY(o.pack(o.x, o.rows, nullptr, nullptr, nullptr, xz, nullptr));
+        const int64_t width = o.width(false, 0);
+        for (int64_t v0 = 0; v0 < o.vocab; v0 += width) {
+            Args z;
+            z.a = xz ? xz : (const uint16_t*)o.x;
+            z.b = (const uint16_t*)o.w + v0 * o.dim;
+            z.lda = z.ldb = z.ka = z.kb = o.dim_p();
+            z.m = o.rows;
+            z.n = std::min(width, o.vocab - v0);
+            z.targets = o.targets;
+            z.v0 = v0;
+            z.vocab = o.vocab;
+            z.lse = lse;
+            z.dloss = dloss;
+            z.dst = g.ds + v0 * 16;
+            MLXHIP_TRY(o.product(ce::CE_DST, Op<OT>::template large<typename Op<OT>::ZTiles>(o.rows, z.n), z));
+        }
+    }
     MLXHIP_TRY(ce_few_grad(OT, g, o.s));
     if (!dx) return MLXHIP_OK;
     hipLaunchKernelGGL((dx_kernel<OT>), dim3(grid_for(o.rows * g.ldx)), dim3(256), 0, o.s, g.dx,
@@ -475,7 +502,7 @@ int run_loss(const Op<OT>& o, float* loss, float* lse) {
 }
 
 template <int OT>
-int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Elem<OT>::type* dx,
+int run_grad(const Op<OT>& o, const float* lse, const float* loss, const float* dloss, typename Elem<OT>::type* dx,
              typename Elem<OT>::type* dw) {
     typedef typename Elem<OT>::type T;
     typedef Op<OT> O;
@@ -487,9 +514,12 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         hipLaunchKernelGGL((zero_kernel<T>), dim3(grid_for(o.vocab * o.dim)), dim3(256), 0, o.s, dw, o.vocab * o.dim);
         return launch_check("zero_kernel");
     }
-    if (ce::few_grad(OT, o.rows, o.vocab)) return few_grad(o, lse, dloss, dx, dw);
+    if (ce::few_grad(OT, o.rows, o.vocab)) return few_grad(o, lse, loss, dloss, dx, dw);
     // One plane of x or W serves z and the gradient, but x's then has to be a copy.
-    const bool copy_x = XP == 1 || !o.in_place(o.x), copy_w = !o.in_place(o.w), planes_x = XP > 1 && dw,
+    // Rows whose loss ce_few.hip forms take z from there.
+    const bool few_z = ce::few_loss(OT, !o.in_place(o.w), o.rows, o.vocab);
+    const bool copy_x = XP == 1 ? !few_z || dw : !few_z && !o.in_place(o.x), planes_x = XP > 1 && dw,
+               copy_w = !o.in_place(o.w) && (!few_z || (WP == 1 && dx)),
                planes_w = WP > 1 && dx;
     const int64_t width = o.width(true, (copy_w ? ZP : 0) + (planes_w ? WP : 0)), ld = ceil_div(width, 256) * 256,
                   dim_p = o.dim_p();
@@ -533,12 +563,28 @@ int run_grad(const Op<OT>& o, const float* lse, const float* dloss, typename Ele
         z.v0 = v0;
         z.vocab = o.vocab;
         z.lse = lse;
+        z.loss = loss;
         z.dloss = dloss;
         z.row_scale = row_scale;
         z.col_scale = col_scale;
         z.ds = ds;
         z.ldc = ceil_div(n, 256) * 256;
-        MLXHIP_TRY(o.product(ce::CE_DS, O::template large<typename O::ZTiles>(o.rows, n), z));
+        if (few_z) {
+            ce::FewArgs f = few_args(o);
+            f.w = o.w + v0 * o.dim;
+            f.vocab = n;
+            f.first = v0;
+            f.whole = o.vocab;
+            f.lse = lse;
+            f.loss = loss;
+            f.dloss = dloss;
+            f.planes = ds;
+            f.ldc = z.ldc;
+            f.plane = o.rows * z.ldc;
+            MLXHIP_TRY(ce_few_planes(OT, f, o.s));
+        } else {
+            MLXHIP_TRY(o.product(ce::CE_DS, O::template large<typename O::ZTiles>(o.rows, n), z));
+        }
         if (dw) {
             Args p;
             p.a = ds;
@@ -609,12 +655,13 @@ int linear_cross_entropy_lse(const float* x, const float* w, const int32_t* targ
 }
 
 int linear_cross_entropy_vjp(int dt, const void* x, const void* w, const int32_t* targets, const float* lse,
-                             const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
+                             const float* loss, const float* dloss, void* dx, void* dw, int64_t rows, int64_t dim, int64_t vocab,
                              hipStream_t s) {
     int rc = MLXHIP_OK;
     if (!with_float_dtype(dt, [&](auto d) {
             typedef typename Elem<d.value>::type T;
-            rc = run_grad<d.value>({(const T*)x, (const T*)w, targets, rows, dim, vocab, s}, lse, dloss, (T*)dx, (T*)dw);
+            rc = run_grad<d.value>({(const T*)x, (const T*)w, targets, rows, dim, vocab, s}, lse, loss, dloss, (T*)dx,
+                                   (T*)dw);
         }))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "linear_cross_entropy gradient: dtype %d (f32, bf16 or f16)", dt);
     return rc;
