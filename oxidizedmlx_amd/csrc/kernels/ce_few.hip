@@ -104,6 +104,21 @@ struct Row {
     __device__ dev::u32x4 load_end(int64_t k, int64_t n) const { return dev::load_raw<DT>(p + shift / 16, k, n).q; }
 };
 
+template <int T, int NB>
+__device__ inline void zero(f32x4 (&a)[T][NB]) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) a[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+template <int T, int NB>
+__device__ inline void add(f32x4 (&to)[T][NB], const f32x4 (&a)[T][NB]) {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) to[t][b] += a[t][b];
+}
+
 // z[v][r] of the wave's TILES * 16 entries from v0 on and NB tiles of 16 rows. KB
 // blocks along K are loaded at once.
 template <int DT, int NB, bool ODD>
@@ -117,10 +132,9 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         x[b].set(static_cast<const E*>(g.x) + min((int64_t)(16 * b + i), g.rows - 1) * g.dim);
-#pragma unroll
-        for (int t = 0; t < T; ++t) acc[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    auto step = [&](const dev::u32x4 (&a)[T], const dev::u32x4 (&c)[NB]) {
+    zero(acc);
+    auto step = [&](const dev::u32x4 (&a)[T], const dev::u32x4 (&c)[NB], f32x4 (&to)[T][NB]) {
         if constexpr (DT == MLXHIP_DTYPE_F32) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
@@ -128,12 +142,12 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int t = 0; t < T; ++t)
-                        acc[t][b] = mfma4(__uint_as_float(a[t][e]), __uint_as_float(c[b][e]), acc[t][b]);
+                        to[t][b] = mfma4(__uint_as_float(a[t][e]), __uint_as_float(c[b][e]), to[t][b]);
         } else {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int t = 0; t < T; ++t) acc[t][b] = mfma32<DT>(a[t], c[b], acc[t][b]);
+                for (int t = 0; t < T; ++t) to[t][b] = mfma32<DT>(a[t], c[b], to[t][b]);
         }
     };
     // Two batches of loads in turn: one on its way while the other is used.
@@ -151,7 +165,12 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
             for (int b = 0; b < NB; ++b) to.c[s][b] = x[b].load(k + BLOCK * s);
         }
     };
+    // f32 products are summed batch by batch: four to an instruction, one chain of 2000
+    // columns is 500 roundings long and three times as far off as sums of its pieces.
+    constexpr bool PIECES = DT == MLXHIP_DTYPE_F32;
     auto use = [&](const Batch& from, int steps) {
+        f32x4 part[T][NB];
+        zero(part);
 #pragma unroll
         for (int s = 0; s < KB; ++s) {
             if (s >= steps) break;
@@ -160,8 +179,10 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
             for (int t = 0; t < T; ++t) a[t] = w[t].join(from.a[s][t]);
 #pragma unroll
             for (int b = 0; b < NB; ++b) c[b] = x[b].join(from.c[s][b]);
-            step(a, c);
+            if constexpr (PIECES) step(a, c, part);
+            else step(a, c, acc);
         }
+        if constexpr (PIECES) add(acc, part);
     };
     const int64_t batches = g.dim / (BLOCK * KB);
     if (batches) fetch(0, KB, batch[0]);
@@ -186,7 +207,7 @@ __device__ inline void few_logits(const FewArgs& g, int64_t v0, int lane, f32x4 
         for (int b = 0; b < NB; ++b) c[b] = x[b].load_end(end + VEC * q, g.dim);
     }
     use(batch[0], left);
-    if (end < g.dim) step(a, c);
+    if (end < g.dim) step(a, c, acc);
 }
 
 // The maxima and sums of z over the T tiles of 16 entries from v0 on of each of the
@@ -356,11 +377,10 @@ __global__ __launch_bounds__(256, 4) void wide_kernel(FewArgs g, int64_t row_blo
         __syncthreads();
     };
     f32x4 acc[T][NB];
-#pragma unroll
-    for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) acc[t][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    zero(acc);
     auto use = [&](const dev::u32x4 (&a)[T][S], int buf) {
+        f32x4 part[T][NB];  // a chunk's sums, as in few_logits
+        zero(part);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             dev::u32x4 c[NB];
@@ -372,8 +392,9 @@ __global__ __launch_bounds__(256, 4) void wide_kernel(FewArgs g, int64_t row_blo
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int t = 0; t < T; ++t)
-                        acc[t][b] = mfma4(__uint_as_float(a[t][s][e]), __uint_as_float(c[b][e]), acc[t][b]);
+                        part[t][b] = mfma4(__uint_as_float(a[t][s][e]), __uint_as_float(c[b][e]), part[t][b]);
         }
+        add(acc, part);
     };
     fetch(0, wv[0]);
     stage(0);

@@ -12,6 +12,7 @@ import operators_ref as R
 from oxidizedmlx_amd import abi, synth
 from oxidizedmlx_amd import backend as hb
 from oxidizedmlx_amd.tensor import Tensor, eval_all, value_and_grad
+import test_gpu_cross_entropy as T
 from test_gpu_cross_entropy import run
 
 pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("hip")]
@@ -33,7 +34,7 @@ def bounds(x, w, t, g, dt):
     """(dx, bound), (dw, bound)."""
     x, w, g = (np.asarray(a, np.float64) for a in (x, w, g))
     z = x @ w.T
-    lse = np.log(np.exp(z - z.max(1, keepdims=True)).sum(1)) + z.max(1)
+    lse = lse_of(z)
     i = np.arange(len(t))
     rest = np.exp(z - lse[:, None])
     rest[i, t] = 0.0
@@ -76,3 +77,28 @@ def test_certain_rows_through_lazy_streams(rows, dim, vocab):
     for name, a, (v, b) in zip(("dx", "dw"), grads, bounds(x, w, t, g, abi.F32)):
         R.check(a.to_numpy().astype(np.float64), v, b, name)
     s.close()
+
+
+@pytest.mark.parametrize("rows", [8, 16, 30, 64, 128])
+@pytest.mark.parametrize("dim", [768, 2000, 4001])
+def test_long_rows_are_not_summed_in_one_chain(rows, dim):
+    """f32 logits of few rows are as exact, in the mean square, as sums of 48 columns
+    that are added up: half as far off again, for other orders, and u / 2 for lse's own
+    rounding, exponentials and logarithm."""
+    x, w, t, g = T.inputs(rows, dim, 600, abi.F32, ignored=0.0)
+    lse = run(x, w, t, g, abi.F32)[1]
+    z = np.zeros((rows, 600), np.float32)
+    for k in range(0, dim, 48):
+        part = np.zeros_like(z)
+        for j in range(k, min(k + 48, dim)):
+            part += x[:, j:j + 1] * w[:, j]
+        z += part
+    exact = lse_of(x.astype(np.float64) @ w.astype(np.float64).T)
+    rms = lambda a: np.sqrt((((a - exact) / exact) ** 2).mean())
+    print(f"{rows} rows of {dim}: {rms(lse) / U:.2f} u, in pieces {rms(lse_of(z.astype(np.float64))) / U:.2f} u", flush=True)
+    assert rms(lse) <= 1.5 * rms(lse_of(z.astype(np.float64))) + U / 2
+
+
+def lse_of(z):
+    m = z.max(1)
+    return np.log(np.exp(z - m[:, None]).sum(1)) + m
