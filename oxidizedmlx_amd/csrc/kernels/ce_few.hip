@@ -2,13 +2,13 @@
 // rows, or 64 of 16 bits where W's rows are no whole 16-byte chunks; the gradients
 // of up to 64 f32 rows, or 16 of 16 bits), which reading W (and writing dW) bounds:
 // W goes from memory straight into the matrix instructions (f32 ones but for the
-// logits of 16-bit operands), with no copies and no planes. dS stays f32: with a few rows one value may make most of a
-// gradient, and its rounding to 16 bits would not average out (one f16 row: dx
-// twice as far off as its own rounding).
+// logits of 16-bit operands), with no copies and no planes; dS stays f32.
 //
 //   stats: z = x W^T, a wave per 16 or 32 entries of the vocabulary; the row maxima
 //          and sums of a workgroup's entries, and the targets' logits.
-//   ds:    z again, kept as dS^T [vocab][16 NB] (zeros behind the rows).
+//   ds:    z again, kept as dS^T [vocab][16 NB] (zeros behind the rows); planes: as
+//          CE_DS of ce_gemm.hpp leaves it, for rows whose loss is formed here and whose
+//          gradients are not.
 //   grad:  a wave per 16 VEC columns (VEC values in 16 bytes) and slice of the
 //          vocabulary: dW = dS^T x of 16 entries at a time, and its sums of
 //          dx = dS W.
@@ -20,15 +20,14 @@
 // the stores undo.
 //
 // Measured over 32000 entries of 1024, f32: 8 rows 29 us (stats, 4.6 TB/s), 29 (ds),
-// 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69. On two f16 planes each
-// (ce_gemm.hpp), whose copies read W twice and write it once before, 1 to 64 rows
-// take 107 - 113 us forward and 157 - 190 backward; the gradients of 64 rows 164 (ds
-// 52, grad 107), of 2044 over 50257 537 (650 on planes); the loss of 256 rows 164 (130).
-// bf16: 8 rows 16 us (ds, 4.2 TB/s), 38 (grad, 3.5 TB/s), 77 with the loss; the tiles of
-// ce_gemm.hpp take 69 for 17, with errors of dx and dw up to twice as large. The
-// loss where the tiles read W in place: 15 us a call there, 21 here (8 rows of 768
-// over 32000); where they would copy it (2044 columns over 50257): 47 - 89 here,
-// 144 there for 65 rows.
+// 49 (grad, 5.3 TB/s read and written); 32 rows 42, 38, 69; 64 rows 54 (loss), 159 (gradients).
+// On planes (ce_gemm.hpp), whose copies read W twice and write it two and five times,
+// the loss of 129 to 256 rows takes 104 - 112 us (128 here: 92; over 50257 of 2044: 350
+// and 279) and the gradients of 65 rows 255 (of 2044 over 50257: 900, 64 rows here 540).
+// bf16: 8 rows 73 us with the loss, 17 on the tiles 78 (2044 columns over 50257: 279
+// for 16, 369 for 17). The loss where the tiles read W in place: 15 us a call there, 21
+// here (8 rows of 768 over 32000); where they would copy it (2044 columns over 50257):
+// 44 - 83 here, 144 there for 65 rows.
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "ce_gemm.hpp"
@@ -65,8 +64,8 @@ constexpr int ENTRIES = 64 * TILES<NB>;  // of a workgroup
 // Rows whose elements may begin in the middle of a dword (16-bit types, ODD): the
 // 16 bytes from the dword that a vector begins in and the dword behind them (of
 // one that begins with its dword: the fourth again, unused), moved together as
-// they are used: every dword read holds an element of the row. Loads at such addresses take several times as long: 8 rows of
-// 2047 over 50257 took 171 us with them.
+// they are used: every dword read holds an element of the row. Loads at such
+// addresses take several times as long: 8 rows of 2047 over 50257 took 171 us with them.
 template <bool ODD>
 struct Loaded {
     dev::u32x4 q;
@@ -328,9 +327,9 @@ __global__ __launch_bounds__(256) void few_stats_kernel(FewArgs g) {
 
 // f32 rows by 64: x goes through LDS, KC columns at a time, and serves a
 // workgroup's four waves of 16 T entries each; W comes straight from memory, a
-// chunk ahead. 128 rows of 1024 over 32000: 82 us, 102 TFLOP/s of f32, and 280 for
-// 2044 over 50257 (whole calls 90 and 290; on planes 121 and 450; a large f32 product
-// reaches 154 TFLOP/s). 32 entries a wave, 32 columns a chunk, or two or five waves
+// chunk ahead. 128 rows of 1024 over 32000: 82 us, 102 TFLOP/s of f32, and 270 for
+// 2044 over 50257 (whole calls 92 and 279; 129 rows on planes 104 and 350; a large f32
+// product reaches 154 TFLOP/s). 32 entries a wave, 32 columns a chunk, or two or five waves
 // to a SIMD: 1 - 15 % slower; 128 rows a workgroup: 64 rows take 97 instead of 57.
 constexpr int WIDE_ROWS = 64, WIDE_T = 1, WIDE_ENTRIES = 64 * WIDE_T;
 enum Wide { WIDE_STATS, WIDE_DS, WIDE_PLANES };

@@ -44,11 +44,12 @@
 //
 // Bound by the matrix cores. 2048 rows of 1024 over 32000 (134 GFLOP a product of one
 // pair of planes; a library product of 8192^3 reaches 1.17 PFLOP/s), in a trace: bf16
-// stats 152 us, dS 190 (262 MB of its planes stored), dx 253 and dW 246 of two pairs
-// each (1.06 - 1.09 PFLOP/s); f32 stats 374, dS 434 of three pairs, dx 650 and dW 667
-// of six (1.2 PFLOP/s). 1000 rows of 777 over 32003, f16: stats 67, dS 84, dx 120 of
-// two pairs, dW 165 of three, 0.6 - 0.9 PFLOP/s: 504 tiles of 256 x 256 on 256 compute
-// units, of 25 steps of K each, so a workgroup's first loads and last epilogue weigh more.
+// stats 147 us, dS 187 (262 MB of its planes stored), dx 238 and dW 235 of two pairs
+// each (1.13 PFLOP/s); f32 stats 368, dS 429 of three pairs (393 MB stored), dx 637 and
+// dW 646 of six (1.25 PFLOP/s). 1000 rows of 777 over 32003, f16: stats 68, dS 87, dx
+// 121 of two pairs, dW 162 of three, 0.6 - 0.92 PFLOP/s: 504 tiles of 256 x 256 on 256
+// compute units, of 25 steps of K each, so a workgroup's first loads and last epilogue
+// weigh more.
 #pragma once
 
 #include "elem.hpp"

@@ -15,9 +15,9 @@
 // rounds. At several hundred rows the matrix cores bound the products.
 //
 // Measured, forward and backward (products and copies; what bounds each product:
-// ce_gemm.hpp): bf16 2048 rows of 1024 over 32000 730 - 785 us, 8192 of 2048 over 50257
-// 9.2 ms (1.1 PFLOP/s); f32 2048 of 1024 over 32000 2.3 ms, of which the copies of W
-// to planes take 50 (forward, two planes) and 100 (backward, five).
+// ce_gemm.hpp): bf16 2048 rows of 1024 over 32000 722 - 785 us, 8192 of 2048 over 50257
+// 8.4 - 9.2 ms (1.1 - 1.2 PFLOP/s); f32 2048 of 1024 over 32000 2.15 - 2.3 ms, of which the
+// copies of W to planes take 55 us (forward, two planes) and 100 (backward, five).
 //
 // For dW, x is copied once with zeros in the rows without a target (whatever they
 // hold must not reach dW through a product with 0) and its rows rounded up to whole

@@ -390,9 +390,9 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(const int32_t* 
 // of the one that goes on after it (an id that does both: the first only).
 // The lanes hold 64 positions' keys and places, so the rows' addresses come
 // from registers and AHEAD rows are loaded at once. 65536 bf16 rows of 1024 with
-// ids as frequent as words: 40 us for some 190 MB (rows read, sums and partial
-// sums written), 4.7 TB/s, whatever the length of the shares; the join then takes
-// 9 us for shares of 32 rows, 16 for 16 and 31 for 8.
+// ids as frequent as words: 51 us for some 190 MB (rows read, sums and partial
+// sums written), 3.7 TB/s, whatever the length of the shares; the join then takes
+// 12 us for shares of 32 rows, and some two and four times that for 16 and 8.
 template <int DT, int N>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const typename Elem<DT>::type* __restrict__ dy,
                                                         const uint32_t* __restrict__ keys,

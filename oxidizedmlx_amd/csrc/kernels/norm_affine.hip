@@ -27,7 +27,7 @@
 //
 // Bound by memory, small ones by the launches. 4096 rows of 4096, f32: 27 us forward
 // (4.9 TB/s) and 34 back (5.9 TB/s, x and dy partly cached), the fold 4.8; 2048 bf16
-// rows of 1024: 4.2, 7.7 and 2.7; 1000 f16 rows of 777: 3.9, 5.8 and 4.8.
+// rows of 1024: 4.2, 8.2 and 2.5; 1000 f16 rows of 777: 3.8, 6.0 and 4.8.
 #include "../common.hpp"
 #include "../kernels.hpp"
 #include "device_math.hpp"
@@ -257,9 +257,10 @@ __global__ __launch_bounds__(WPR < 4 ? 256 : 64 * WPR) void affine_bwd_kernel(
 }
 
 // Sums of n partial rows of 2 * cols values into dw and db: 32 columns of a
-// workgroup, 32 threads to each, which fold every 32nd row (their loads all in
-// flight: a fold of 256 rows by 8 threads waited 9 us for 32 loads in turn) and
-// then each other.
+// workgroup, 32 threads to each, which fold every 32nd row (of 256 partial rows all
+// eight loads in flight: by 8 threads the fold waited 9 us for 32 loads in turn; of fewer
+// rows, what is no whole eight is loaded one by one: 250 rows of 1554 sums take 4.8 us
+// where 256 of 2048 take 2.5) and then each other.
 constexpr int FOLD = 32;
 template <int DT>
 __global__ __launch_bounds__(32 * FOLD) void affine_fold_kernel(const float* __restrict__ part, int64_t n, int64_t cols,
