@@ -176,12 +176,14 @@ struct Args {
 // Few rows (ce_few.hip, with what each bound measured): the loss of up to 128 f32
 // rows, or 64 of 16 bits where the tiles would need a copy of W; the gradients of up
 // to 64 f32 rows, or 16 of 16 bits. Where only the loss is formed there, it leaves dS of
-// more rows to the tiles as CE_DS does: z has to be the same in both. What they keep of each entry stays within FEW_BYTES:
-// the statistics of its 64th and the row of dS^T.
-constexpr int64_t FEW_BYTES = int64_t(1) << 30;
+// more rows to the tiles as CE_DS does: z has to be the same in both. What they keep of
+// each entry stays within FEW_BYTES (the statistics of its 64th, the row of dS^T), and
+// their launches, four work items to an entry and block of 64 rows, within the 2^32
+// that a dispatch counts.
+constexpr int64_t FEW_BYTES = int64_t(1) << 30, FEW_ENTRIES = int64_t(1) << 29;
 inline int64_t few_ds_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 inline bool few_loss(int dt, bool copy_w, int64_t rows, int64_t vocab) {
-    return copy_w && rows <= (dt == MLXHIP_DTYPE_F32 ? 128 : 64) && vocab / 64 * rows * 8 <= FEW_BYTES;
+    return copy_w && rows <= (dt == MLXHIP_DTYPE_F32 ? 128 : 64) && vocab / 64 * rows * 8 <= FEW_BYTES && vocab <= FEW_ENTRIES;
 }
 inline bool few_grad(int dt, int64_t rows, int64_t vocab) {
     return rows <= (dt == MLXHIP_DTYPE_F32 ? 64 : 16) && vocab * few_ds_rows(rows) * 4 <= FEW_BYTES;

@@ -57,10 +57,23 @@ def test_a_piece_of_several_tiles(pieces, dt):
     check_all(got, x, w, t, g, dt)
 
 
-@pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
+@pytest.mark.parametrize("dt", [abi.BF16, abi.F16], ids=R.NAMES.get)
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("rows,dim,vocab", [(17, 131, 600), (40, 77, 700), (64, 390, 515)])
+def test_pieces_of_rows_whose_logits_come_straight_from_w(pieces, rows, dim, vocab, offset, dt):
+    x, w, t, g = inputs(rows, dim, vocab, dt)
+    t = spread_targets(t, vocab)
+    pieces(1)
+    got = run(x, w, t, g, dt, offset)
+    assert pieces(0) >= 3
+    check_all(got, x, w, t, g, dt)
+
+
+@pytest.mark.parametrize("rows,dim,dt", [(200, 72, dt) for dt in R.DTYPES] + [(100, 77, dt) for dt in R.DTYPES] +
+                         [(24, 77, abi.BF16), (24, 77, abi.F16)])
 @pytest.mark.parametrize("want", ["x", "w"])
-def test_one_gradient_alone_in_pieces(pieces, want, dt):
-    a = inputs(200, 72, 700, dt)
+def test_one_gradient_alone_in_pieces(pieces, want, rows, dim, dt):
+    a = inputs(rows, dim, 700, dt)
     pieces(1)
     both = run(*a, dt)
     pieces(1)
