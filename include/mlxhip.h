@@ -577,6 +577,97 @@ int mlxhip_attention_vjp(const float* q, const float* k, const float* v, const f
                          const float* dout, float* dq, float* dk, float* dv, int64_t batch,
                          int64_t t, int64_t dh, float scale, int32_t causal, void* stream);
 
+/* Rotary positions of rows x [tokens, heads, head_dim]: of each head the pairs
+ * (i, i + rotary_dim/2) (interleaved 0) or (2i, 2i + 1) (1), i < rotary_dim/2, turn by
+ * the angle a = positions[t] * freqs[i],
+ *   (u, v) -> magnitude (u cos a - v sin a, v cos a + u sin a),
+ * the head's other values are copied; and the gradient, dx for the cotangent dy:
+ * the same with the angle's sign turned round. RoPE and Rope of the reference
+ * (cpu_kernels.rs:608-645,896-956) take f32, one sequence and positions from an offset.
+ * dtype: F32, BF16 or F16, of x and y; angles are formed in 64 bits (any int32
+ * position), cosines, sines and products in f32, each result is rounded once.
+ * freqs: device doubles (rotary_dim/2 of them), the caller's own or those of
+ * mlxhip_rope_frequencies: f_i = base^(-2i/rotary_dim), for long contexts divided by
+ * factor where a turn is long: with r = original_len f_i / 2 pi turns in an original
+ * context, by factor where r <= low_turns, not where r >= high_turns, in between
+ * f_i (g + (1 - g) / factor) with g = (r - low_turns) / (high_turns - low_turns);
+ * original_len 0 divides all.
+ * A token's heads are contiguous, tokens x_stride / y_stride elements apart (heads *
+ * head_dim at least: queries and keys of one projection side by side are one call).
+ * Any address aligned to the elements. y may be x (equal strides), and must not
+ * overlap it otherwise. tokens up to 2^25, heads * head_dim and strides up to 2^20,
+ * rotary_dim even, 2 to 1024 and at most head_dim. */
+int mlxhip_rope_frequencies(double* freqs, int64_t rotary_dim, double base, double factor, double low_turns,
+                            double high_turns, int64_t original_len, void* stream);
+int mlxhip_rope_rows(int32_t dtype, const void* x, const int32_t* positions, const double* freqs, void* y,
+                     int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim, int64_t x_stride,
+                     int64_t y_stride, int32_t interleaved, float magnitude, void* stream);
+int mlxhip_rope_vjp_rows(int32_t dtype, const void* dy, const int32_t* positions, const double* freqs, void* dx,
+                         int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim, int64_t dy_stride,
+                         int64_t dx_stride, int32_t interleaved, float magnitude, void* stream);
+
+/* Attention of packed sequences with grouped heads. Sequence s is the tokens
+ * starts[s] .. starts[s + 1] - 1 (n_seqs + 1 device int32, ascending, in [0, tokens];
+ * sequences may be empty); query head h reads K/V head h / (heads / kv_heads). With P the
+ * softmax of a row's scores scale q k^T over the keys of its sequence (causal: up to
+ * its own token),
+ *   o = P v,  lse = log sum exp(scale q k^T)  (f32 [tokens, heads]; may be NULL),
+ * and the gradients for the cotangent dout of o, with the forward's o and lse,
+ *   dP = dout v^T,  dS = P o (dP - rowsum(dout o o)),
+ *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout  (summed over a group's heads).
+ * Tokens outside every sequence are not read as keys, and their results are left as
+ * they were. A token's heads are contiguous; tokens of q and dq are q_stride elements
+ * apart, of k, v, dk and dv kv_stride, of o and dout o_stride, so that q, k and v may be
+ * parts of one projection's rows.
+ * dtype: F32, BF16 or F16, of every operand but lse. Scores, softmax and sums are f32;
+ * P and dS are rounded to a 16-bit type's own precision for their products (f16: scaled,
+ * so that small ones keep it), results once. Sums are formed in a fixed order.
+ * A non-finite value stays within its sequence: with v's the rows that see it are
+ * not finite, others are as without it; the gradients of its sequence may be NaN.
+ * head_dim a multiple of 8 up to 128; addresses 16-byte aligned, strides a multiple of 16
+ * bytes, up to 2^20. heads a multiple of kv_heads; tokens * heads up to 2^30, n_seqs *
+ * kv_heads up to 2^22. Results must not overlap operands. The gradient keeps two f32 values
+ * of each row, and where there are few keys parts of dk and dv, in a per-stream workspace.
+ * mlxhip_attention is the f32 form for heads of one length, mlxhip_attention_vjp its
+ * gradient (cpu_attention, cpu_kernels.rs:738-812). */
+int mlxhip_packed_attention(int32_t dtype, const void* q, const void* k, const void* v, const int32_t* starts, void* o,
+                            float* lse, int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads,
+                            int64_t head_dim, int64_t q_stride, int64_t kv_stride, int64_t o_stride, float scale,
+                            int32_t causal, void* stream);
+int mlxhip_packed_attention_vjp(int32_t dtype, const void* q, const void* k, const void* v, const void* o,
+                                const void* dout, const float* lse, const int32_t* starts, void* dq, void* dk, void* dv,
+                                int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                int64_t q_stride, int64_t kv_stride, int64_t o_stride, float scale, int32_t causal,
+                                void* stream);
+
+/* A cache in pages: k_pages and v_pages [pages, kv_heads, page_size, head_dim]; position
+ * p of sequence s lies in page table[s][p / page_size] (device int32 [n_seqs,
+ * table_width]) at row p % page_size. In one step sequence s gets the new tokens
+ * starts[s] .. starts[s + 1] - 1 (as above) and has lens[s] positions with them, so its
+ * j-th of n new tokens is position lens[s] - n + j.
+ * paged_append stores the new tokens' k and v (kv_stride elements apart; with
+ * freqs, k turned by its position as mlxhip_rope_rows does; freqs NULL: as it is). A
+ * position outside [0, table_width * page_size), or whose page number is outside [0, pages), is
+ * not stored. Two new tokens must not name one place.
+ * paged_attention: o = softmax(scale q k^T) v of each new token over the positions
+ * 0 .. its own (lens beyond the table's are cut to it); a token that sees none (a
+ * negative position) gives zeros, a page number outside [0, pages) reads as zeros. Tokens
+ * outside every sequence are left as they were. Other positions' contents, non-finite ones
+ * too, do not enter. The keys of a sequence may be split over workgroups, whose parts, f32 in a
+ * per-stream workspace (256 MiB at most), are joined in order.
+ * dtype, head_dim, alignment, heads and sizes as for mlxhip_packed_attention; page_size a power
+ * of two from 16 to 4096, table_width * page_size up to 2^31 - 1. HipDecoder keeps its own
+ * cache (mlxhip_decoder_*); the reference's is a host vector (ttft_behavior.rs:101-216). */
+int mlxhip_paged_append(int32_t dtype, const void* k, const void* v, const int32_t* starts, const int32_t* lens,
+                        const int32_t* table, void* k_pages, void* v_pages, int64_t n_seqs, int64_t tokens,
+                        int64_t kv_heads, int64_t head_dim, int64_t kv_stride, int64_t pages, int64_t page_size,
+                        int64_t table_width, const double* freqs, int64_t rotary_dim, int32_t interleaved,
+                        float magnitude, void* stream);
+int mlxhip_paged_attention(int32_t dtype, const void* q, const void* k_pages, const void* v_pages, const int32_t* starts,
+                           const int32_t* lens, const int32_t* table, void* o, int64_t n_seqs, int64_t tokens,
+                           int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride, int64_t o_stride,
+                           int64_t pages, int64_t page_size, int64_t table_width, float scale, void* stream);
+
 /* 2-D transpose y[cols, rows] = x[rows, cols]^T of 4-byte elements
  * (transpose, cpu_kernels.rs:232-274, axes = None on rank 2). Bit-exact. */
 int mlxhip_transpose2d(const float* x, float* y, int64_t rows, int64_t cols, void* stream);

@@ -154,6 +154,7 @@ _i64 = C.c_int64
 _u64 = C.c_uint64
 _sz = C.c_size_t
 _f = C.c_float
+_d = C.c_double
 _vp = C.c_void_p
 _fp = C.c_void_p  # float* passed as raw address
 
@@ -219,6 +220,13 @@ PROTOTYPES = {
                              _fp, _i64, _vp]),
     "mlxhip_attention": (_i, [_fp, _fp, _fp, _fp, _i64, _i64, _i64, _i64, _f, _i32, _vp]),
     "mlxhip_attention_vjp": (_i, [_fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _i64, _i64, _i64, _f, _i32, _vp]),
+    "mlxhip_rope_frequencies": (_i, [_vp, _i64, _d, _d, _d, _d, _i64, _vp]),
+    "mlxhip_rope_rows": (_i, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f, _vp]),
+    "mlxhip_rope_vjp_rows": (_i, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f, _vp]),
+    "mlxhip_packed_attention": (_i, [_i32] + [_vp] * 6 + [_i64] * 8 + [_f, _i32, _vp]),
+    "mlxhip_packed_attention_vjp": (_i, [_i32] + [_vp] * 10 + [_i64] * 8 + [_f, _i32, _vp]),
+    "mlxhip_paged_append": (_i, [_i32] + [_vp] * 7 + [_i64] * 8 + [_vp, _i64, _i32, _f, _vp]),
+    "mlxhip_paged_attention": (_i, [_i32] + [_vp] * 7 + [_i64] * 10 + [_f, _vp]),
     "mlxhip_transpose2d": (_i, [_fp, _fp, _i64, _i64, _vp]),
     "mlxhip_cast": (_i, [_vp, _i32, _vp, _i32, _i64, _vp]),
     "mlxhip_decoder_new": (_vp, [C.POINTER(mlxhip_decoder_config_t)]),

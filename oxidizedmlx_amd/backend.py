@@ -364,6 +364,71 @@ def attention_vjp(q, k, v, o, do, dq, dk, dv, batch: int, t: int, dh: int, scale
                                          scale, int(causal), stream))
 
 
+def rope_frequencies(freqs, rotary_dim: int, base: float, factor: float = 1.0, low_turns: float = 0.0,
+                     high_turns: float = 0.0, original_len: int = 0, stream=None) -> None:
+    """Writes rotary_dim / 2 float64 angles per position, base^(-2i/rotary_dim),
+    for long contexts divided by ``factor``: all of them (original_len 0), or
+    those of at most ``low_turns`` turns in ``original_len`` positions, less up to ``high_turns``."""
+    abi.check(lib().mlxhip_rope_frequencies(_p(freqs), rotary_dim, base, factor, low_turns, high_turns, original_len, stream))
+
+
+def rope_rows(dtype: int, x, positions, freqs, y, tokens: int, heads: int, head_dim: int, rotary_dim: int, x_stride: int,
+              y_stride: int, interleaved: bool = False, magnitude: float = 1.0, stream=None) -> None:
+    """y = x [tokens, heads, head_dim] turned by int32 positions times float64
+    ``freqs``: pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) if ``interleaved``.
+    Strides are elements between tokens; y may be x."""
+    abi.check(lib().mlxhip_rope_rows(dtype, _p(x), _p(positions), _p(freqs), _p(y), tokens, heads, head_dim, rotary_dim,
+                                     x_stride, y_stride, int(interleaved), magnitude, stream))
+
+
+def rope_vjp_rows(dtype: int, dy, positions, freqs, dx, tokens: int, heads: int, head_dim: int, rotary_dim: int,
+                  dy_stride: int, dx_stride: int, interleaved: bool = False, magnitude: float = 1.0, stream=None) -> None:
+    """dx of ``rope_rows``: dy turned the other way."""
+    abi.check(lib().mlxhip_rope_vjp_rows(dtype, _p(dy), _p(positions), _p(freqs), _p(dx), tokens, heads, head_dim, rotary_dim,
+                                         dy_stride, dx_stride, int(interleaved), magnitude, stream))
+
+
+def packed_attention(dtype: int, q, k, v, starts, o, lse, n_seqs: int, tokens: int, heads: int, kv_heads: int, head_dim: int,
+                     q_stride: int, kv_stride: int, o_stride: int, scale: float, causal: bool = True, stream=None) -> None:
+    """Attention within each of n_seqs sequences, tokens starts[s] ..
+    starts[s + 1] - 1 of q and o [tokens, heads, head_dim], k and v [tokens,
+    kv_heads, head_dim] (strides in elements between tokens); f32 lse [tokens,
+    heads], or None."""
+    abi.check(lib().mlxhip_packed_attention(dtype, _p(q), _p(k), _p(v), _p(starts), _p(o), _p(lse), n_seqs, tokens, heads,
+                                            kv_heads, head_dim, q_stride, kv_stride, o_stride, scale, int(causal), stream))
+
+
+def packed_attention_vjp(dtype: int, q, k, v, o, dout, lse, starts, dq, dk, dv, n_seqs: int, tokens: int, heads: int,
+                         kv_heads: int, head_dim: int, q_stride: int, kv_stride: int, o_stride: int, scale: float,
+                         causal: bool = True, stream=None) -> None:
+    """dq, dk and dv of ``packed_attention`` for o's cotangent dout and the
+    forward's o and lse; dk and dv summed over the heads of a group."""
+    abi.check(lib().mlxhip_packed_attention_vjp(dtype, _p(q), _p(k), _p(v), _p(o), _p(dout), _p(lse), _p(starts), _p(dq),
+                                                _p(dk), _p(dv), n_seqs, tokens, heads, kv_heads, head_dim, q_stride,
+                                                kv_stride, o_stride, scale, int(causal), stream))
+
+
+def paged_append(dtype: int, k, v, starts, lens, table, k_pages, v_pages, n_seqs: int, tokens: int, kv_heads: int,
+                 head_dim: int, kv_stride: int, pages: int, page_size: int, table_width: int, freqs=None,
+                 rotary_dim: int = 0, interleaved: bool = False, magnitude: float = 1.0, stream=None) -> None:
+    """New tokens' k (turned by position where ``freqs`` is given) and v into
+    pages [pages, kv_heads, page_size, head_dim]: the last starts[s + 1] -
+    starts[s] of sequence s's lens[s] positions, by its row of ``table``."""
+    abi.check(lib().mlxhip_paged_append(dtype, _p(k), _p(v), _p(starts), _p(lens), _p(table), _p(k_pages), _p(v_pages),
+                                        n_seqs, tokens, kv_heads, head_dim, kv_stride, pages, page_size, table_width,
+                                        _p(freqs), rotary_dim, int(interleaved), magnitude, stream))
+
+
+def paged_attention(dtype: int, q, k_pages, v_pages, starts, lens, table, o, n_seqs: int, tokens: int, heads: int,
+                    kv_heads: int, head_dim: int, q_stride: int, o_stride: int, pages: int, page_size: int,
+                    table_width: int, scale: float, stream=None) -> None:
+    """Attention of the new tokens of each sequence (as ``paged_append`` places
+    them) over its positions up to their own."""
+    abi.check(lib().mlxhip_paged_attention(dtype, _p(q), _p(k_pages), _p(v_pages), _p(starts), _p(lens), _p(table), _p(o),
+                                           n_seqs, tokens, heads, kv_heads, head_dim, q_stride, o_stride, pages, page_size,
+                                           table_width, scale, stream))
+
+
 def transpose2d(x, y, rows: int, cols: int, stream=None) -> None:
     abi.check(lib().mlxhip_transpose2d(_p(x), _p(y), rows, cols, stream))
 

@@ -73,16 +73,24 @@ SOURCES = [
     "kernels/prefill.hip",
     "kernels/attention.hip",
     "kernels/attention_bwd.hip",
+    "kernels/rope.hip",
+    "kernels/packed_attn.hip",
+    "kernels/packed_attn_bf16.hip",
+    "kernels/packed_attn_f16.hip",
+    "kernels/packed_attn_f32.hip",
 ]
 
 
-# Per-source flags. The attention kernel rescales its MFMA accumulators with
-# VALU multiplies every key tile; in the VGPR form of the MFMA instructions
+# Per-source flags. The attention kernels rescale their MFMA accumulators with
+# VALU multiplies; in the VGPR form of the MFMA instructions
 # they are not copied to and from the accumulation registers for that. The
 # prefill GEMM adds its accumulators up after every k-slice.
 EXTRA = {
     "kernels/prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "kernels/attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kernels/packed_attn_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kernels/packed_attn_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kernels/packed_attn_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

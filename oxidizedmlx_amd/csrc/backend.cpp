@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <functional>
@@ -1390,6 +1391,201 @@ int mlxhip_attention_vjp(const float* q, const float* k, const float* v, const f
     if (!q || !k || !v || !o || !dout || !dq || !dk || !dv)
         return fail(MLXHIP_ERR_NULL_PTR, "attention vjp: null operand");
     return attention_vjp(q, k, v, o, dout, dq, dk, dv, batch, t, dh, scale, causal, as_stream(stream));
+}
+
+namespace {
+constexpr int64_t MAX_TOKENS = int64_t(1) << 25;  // of a rotated batch (grids within 2^32 work items)
+
+// Addresses and strides that the attention kernels read 16 bytes at a time.
+int check_vectors(const char* what, int dtype, std::initializer_list<const void*> typed, std::initializer_list<int64_t> strides) {
+    const int64_t size = dtype == MLXHIP_DTYPE_F32 ? 4 : 2;
+    for (const void* p : typed)
+        if (reinterpret_cast<uintptr_t>(p) % 16)
+            return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: operand not aligned to 16 bytes", what);
+    for (int64_t v : strides)
+        if (v * size % 16) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: stride %lld is no multiple of 16 bytes", what, (long long)v);
+    return MLXHIP_OK;
+}
+
+int check_words(const char* what, std::initializer_list<const void*> doubles) {
+    for (const void* p : doubles) {
+        if (!p) return fail(MLXHIP_ERR_NULL_PTR, "%s: null operand", what);
+        if (reinterpret_cast<uintptr_t>(p) % 8) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: operand not aligned to its elements", what);
+    }
+    return MLXHIP_OK;
+}
+
+int check_rotary(const char* what, int64_t rotary_dim, int64_t head_dim, int32_t interleaved) {
+    if (rotary_dim < 2 || rotary_dim > 1024 || rotary_dim % 2 || rotary_dim > head_dim)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: rotary_dim %lld of head_dim %lld (even, 2 to 1024)", what,
+                    (long long)rotary_dim, (long long)head_dim);
+    if (interleaved != 0 && interleaved != 1)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: interleaved %d (0 or 1)", what, interleaved);
+    return MLXHIP_OK;
+}
+
+// Strides of tokens of `heads` heads.
+int check_strides(const char* what, int64_t heads, int64_t head_dim, std::initializer_list<int64_t> strides) {
+    if (heads > MAX_DIM || heads * head_dim > MAX_DIM)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: heads * head_dim is over %lld", what, (long long)MAX_DIM);
+    for (int64_t v : strides)
+        if (v < heads * head_dim || v > MAX_DIM)
+            return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: stride %lld (%lld to %lld)", what, (long long)v,
+                        (long long)(heads * head_dim), (long long)MAX_DIM);
+    return MLXHIP_OK;
+}
+
+int rope_call(const char* what, int32_t dtype, const void* x, const int32_t* positions, const double* freqs, void* y,
+              int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim, int64_t x_stride, int64_t y_stride,
+              int32_t interleaved, float magnitude, bool vjp, hipStream_t s) {
+    MLXHIP_TRY(check_sizes(what, {tokens, heads, head_dim, rotary_dim}, {MAX_TOKENS, MAX_DIM, MAX_DIM, MAX_DIM}));
+    MLXHIP_TRY(check_rotary(what, rotary_dim, head_dim, interleaved));
+    MLXHIP_TRY(check_strides(what, heads, head_dim, {x_stride, y_stride}));
+    if (tokens == 0 || heads == 0) return check_operands(what, dtype, {});
+    MLXHIP_TRY(check_operands(what, dtype, {x, y}, {positions}));
+    MLXHIP_TRY(check_words(what, {freqs}));
+    if (x == y && x_stride != y_stride)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: in place with strides %lld and %lld", what, (long long)x_stride,
+                    (long long)y_stride);
+    MLXHIP_TRY(ensure_device());
+    return rope_rows(dtype, x, positions, freqs, y, tokens, heads, head_dim, rotary_dim, x_stride, y_stride, interleaved,
+                     magnitude, vjp, s);
+}
+
+// Sizes that the attention over packed sequences and over pages share.
+int check_heads(const char* what, int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+    constexpr int64_t ROWS = int64_t(1) << 30, SEQS = int64_t(1) << 22;
+    MLXHIP_TRY(check_sizes(what, {n_seqs, tokens, heads, kv_heads, head_dim}, {SEQS, ROWS, MAX_DIM, MAX_DIM, 128}));
+    if (kv_heads ? heads % kv_heads != 0 : heads != 0)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: %lld heads on %lld K/V heads", what, (long long)heads, (long long)kv_heads);
+    if (head_dim % 8) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: head_dim %lld is no multiple of 8", what, (long long)head_dim);
+    if (tokens * heads > ROWS || n_seqs * kv_heads > SEQS)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: tokens * heads is over 2^30 or n_seqs * kv_heads over 2^22", what);
+    return MLXHIP_OK;
+}
+
+int check_scale(const char* what, float scale) {
+    if (!std::isfinite(scale)) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: scale is not finite", what);
+    return MLXHIP_OK;
+}
+
+int paged_args(const char* what, const int32_t* starts, const int32_t* lens, const int32_t* table, int64_t n_seqs,
+               int64_t pages, int64_t page_size, int64_t table_width, PagedArgs* out) {
+    MLXHIP_TRY(check_sizes(what, {pages, page_size, table_width}, {INT32_MAX, 4096, INT32_MAX}));
+    if (page_size < 16 || (page_size & (page_size - 1)))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: page_size %lld (a power of two from 16 to 4096)", what, (long long)page_size);
+    if (table_width * page_size > INT32_MAX)
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: table_width * page_size is over 2^31 - 1", what);
+    *out = {starts, lens, table, (int)n_seqs, (int)pages, __builtin_ctzll((unsigned long long)page_size), table_width};
+    return MLXHIP_OK;
+}
+}  // namespace
+
+int mlxhip_rope_frequencies(double* freqs, int64_t rotary_dim, double base, double factor, double low_turns,
+                            double high_turns, int64_t original_len, void* stream) {
+    const char* what = "rope_frequencies";
+    MLXHIP_TRY(check_rotary(what, rotary_dim, rotary_dim, 0));
+    if (!(base > 0) || !(factor > 0) || !std::isfinite(base) || !std::isfinite(factor))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: base and factor must be positive", what);
+    if (original_len < 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (factor != 1 && original_len && !(low_turns < high_turns && std::isfinite(high_turns - low_turns)))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: low_turns must be below high_turns", what);
+    MLXHIP_TRY(check_words(what, {freqs}));
+    MLXHIP_TRY(ensure_device());
+    return rope_frequencies(freqs, rotary_dim, base, factor, low_turns, high_turns, original_len, as_stream(stream));
+}
+
+int mlxhip_rope_rows(int32_t dtype, const void* x, const int32_t* positions, const double* freqs, void* y, int64_t tokens,
+                     int64_t heads, int64_t head_dim, int64_t rotary_dim, int64_t x_stride, int64_t y_stride,
+                     int32_t interleaved, float magnitude, void* stream) {
+    return rope_call("rope_rows", dtype, x, positions, freqs, y, tokens, heads, head_dim, rotary_dim, x_stride, y_stride,
+                     interleaved, magnitude, false, as_stream(stream));
+}
+
+int mlxhip_rope_vjp_rows(int32_t dtype, const void* dy, const int32_t* positions, const double* freqs, void* dx,
+                         int64_t tokens, int64_t heads, int64_t head_dim, int64_t rotary_dim, int64_t dy_stride,
+                         int64_t dx_stride, int32_t interleaved, float magnitude, void* stream) {
+    return rope_call("rope_vjp_rows", dtype, dy, positions, freqs, dx, tokens, heads, head_dim, rotary_dim, dy_stride,
+                     dx_stride, interleaved, magnitude, true, as_stream(stream));
+}
+
+int mlxhip_packed_attention(int32_t dtype, const void* q, const void* k, const void* v, const int32_t* starts, void* o,
+                            float* lse, int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t q_stride, int64_t kv_stride, int64_t o_stride, float scale, int32_t causal,
+                            void* stream) {
+    const char* what = "packed_attention";
+    MLXHIP_TRY(check_heads(what, n_seqs, tokens, heads, kv_heads, head_dim));
+    MLXHIP_TRY(check_strides(what, heads, head_dim, {q_stride, o_stride}));
+    MLXHIP_TRY(check_strides(what, kv_heads, head_dim, {kv_stride}));
+    MLXHIP_TRY(check_scale(what, scale));
+    if (n_seqs == 0 || tokens == 0 || heads == 0 || head_dim == 0) return check_operands(what, dtype, {});
+    MLXHIP_TRY(check_operands(what, dtype, {q, k, v, o}, {starts}));
+    if (lse) MLXHIP_TRY(check_operands(what, dtype, {}, {lse}));
+    MLXHIP_TRY(check_vectors(what, dtype, {q, k, v, o}, {q_stride, kv_stride, o_stride}));
+    MLXHIP_TRY(ensure_device());
+    return packed_attention(dtype, q, k, v, starts, o, lse, n_seqs, tokens, heads, kv_heads, head_dim, q_stride, kv_stride,
+                            o_stride, scale, causal != 0, as_stream(stream));
+}
+
+int mlxhip_packed_attention_vjp(int32_t dtype, const void* q, const void* k, const void* v, const void* o,
+                                const void* dout, const float* lse, const int32_t* starts, void* dq, void* dk, void* dv,
+                                int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                int64_t q_stride, int64_t kv_stride, int64_t o_stride, float scale, int32_t causal,
+                                void* stream) {
+    const char* what = "packed_attention_vjp";
+    MLXHIP_TRY(check_heads(what, n_seqs, tokens, heads, kv_heads, head_dim));
+    MLXHIP_TRY(check_strides(what, heads, head_dim, {q_stride, o_stride}));
+    MLXHIP_TRY(check_strides(what, kv_heads, head_dim, {kv_stride}));
+    MLXHIP_TRY(check_scale(what, scale));
+    if (n_seqs == 0 || tokens == 0 || heads == 0 || head_dim == 0) return check_operands(what, dtype, {});
+    MLXHIP_TRY(check_operands(what, dtype, {q, k, v, o, dout, dq, dk, dv}, {lse, starts}));
+    MLXHIP_TRY(check_vectors(what, dtype, {q, k, v, o, dout, dq, dk, dv}, {q_stride, kv_stride, o_stride}));
+    MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
+    return packed_attention_vjp(dtype, q, k, v, o, dout, lse, starts, dq, dk, dv, n_seqs, tokens, heads, kv_heads, head_dim,
+                                q_stride, kv_stride, o_stride, scale, causal != 0, as_stream(stream));
+}
+
+int mlxhip_paged_append(int32_t dtype, const void* k, const void* v, const int32_t* starts, const int32_t* lens,
+                        const int32_t* table, void* k_pages, void* v_pages, int64_t n_seqs, int64_t tokens,
+                        int64_t kv_heads, int64_t head_dim, int64_t kv_stride, int64_t pages, int64_t page_size,
+                        int64_t table_width, const double* freqs, int64_t rotary_dim, int32_t interleaved, float magnitude,
+                        void* stream) {
+    const char* what = "paged_append";
+    MLXHIP_TRY(check_heads(what, n_seqs, tokens, kv_heads, kv_heads, head_dim));
+    MLXHIP_TRY(check_sizes(what, {tokens}, {MAX_TOKENS}));
+    MLXHIP_TRY(check_strides(what, kv_heads, head_dim, {kv_stride}));
+    PagedArgs a;
+    MLXHIP_TRY(paged_args(what, starts, lens, table, n_seqs, pages, page_size, table_width, &a));
+    if (freqs) MLXHIP_TRY(check_rotary(what, rotary_dim, head_dim, interleaved));
+    if (n_seqs == 0 || tokens == 0 || kv_heads == 0 || head_dim == 0 || pages == 0 || table_width == 0)
+        return check_operands(what, dtype, {});
+    MLXHIP_TRY(check_operands(what, dtype, {k, v, k_pages, v_pages}, {starts, lens, table}));
+    if (freqs) MLXHIP_TRY(check_words(what, {freqs}));
+    MLXHIP_TRY(check_vectors(what, dtype, {k, v, k_pages, v_pages}, {kv_stride}));
+    MLXHIP_TRY(ensure_device());
+    return paged_append(dtype, k, v, k_pages, v_pages, a, tokens, kv_heads, head_dim, kv_stride, freqs, rotary_dim,
+                        interleaved, magnitude, as_stream(stream));
+}
+
+int mlxhip_paged_attention(int32_t dtype, const void* q, const void* k_pages, const void* v_pages, const int32_t* starts,
+                           const int32_t* lens, const int32_t* table, void* o, int64_t n_seqs, int64_t tokens,
+                           int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t q_stride, int64_t o_stride,
+                           int64_t pages, int64_t page_size, int64_t table_width, float scale, void* stream) {
+    const char* what = "paged_attention";
+    MLXHIP_TRY(check_heads(what, n_seqs, tokens, heads, kv_heads, head_dim));
+    MLXHIP_TRY(check_strides(what, heads, head_dim, {q_stride, o_stride}));
+    MLXHIP_TRY(check_scale(what, scale));
+    PagedArgs a;
+    MLXHIP_TRY(paged_args(what, starts, lens, table, n_seqs, pages, page_size, table_width, &a));
+    if (n_seqs == 0 || tokens == 0 || heads == 0 || head_dim == 0) return check_operands(what, dtype, {});
+    if (pages == 0 || table_width == 0) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: no pages", what);
+    MLXHIP_TRY(check_operands(what, dtype, {q, k_pages, v_pages, o}, {starts, lens, table}));
+    MLXHIP_TRY(check_vectors(what, dtype, {q, k_pages, v_pages, o}, {q_stride, o_stride}));
+    MLXHIP_TRY(ensure_device());
+    const auto lock = launches_together(as_stream(stream));
+    return paged_attention(dtype, q, k_pages, v_pages, a, o, tokens, heads, kv_heads, head_dim, q_stride, o_stride, scale,
+                           as_stream(stream));
 }
 
 int mlxhip_transpose2d(const float* x, float* y, int64_t rows, int64_t cols, void* stream) {

@@ -75,7 +75,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // release_stream_workspaces(s) after `s` has drained. Calls on different streams
 // use different blocks, and so does every recording of mlxhip_graph_begin: its
 // blocks belong to the graph until that is freed.
-enum WsSlot { WS_PACK = 0, WS_SPLITK = 1, WS_REDUCE = 2, WS_ATTN = 3, WS_NORM = 4, WS_EMBED = 5, WS_CE = 6 };
+enum WsSlot { WS_PACK = 0, WS_SPLITK = 1, WS_REDUCE = 2, WS_ATTN = 3, WS_NORM = 4, WS_EMBED = 5, WS_CE = 6, WS_PACKED = 7 };
 int stream_workspace(hipStream_t s, int slot, size_t bytes, void** out);
 void release_stream_workspaces(hipStream_t s);
 

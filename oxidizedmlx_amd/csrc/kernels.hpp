@@ -29,6 +29,35 @@ int row_op(int op, const float* a, const float* b, float* y, int64_t rows, int64
 int fibre_softmax(bool vjp, const float* a, const float* b, float* y, int64_t outer, int64_t dim,
                   int64_t inner, hipStream_t s);
 
+// ── rope.hip ──────────────────────────────────────────────────────────────
+// A cache in pages of 2^page_shift positions and the sequences in it: starts
+// [n_seqs + 1] of the new tokens, lens [n_seqs] with them, table [n_seqs][table_width].
+struct PagedArgs {
+    const int32_t *starts, *lens, *table;
+    int n_seqs, pages, page_shift;
+    int64_t table_width;
+};
+int rope_frequencies(double* freqs, int64_t rotary, double base, double factor, double low, double high, int64_t original,
+                     hipStream_t s);
+int rope_rows(int dtype, const void* x, const int32_t* positions, const double* freqs, void* y, int64_t tokens,
+              int64_t heads, int64_t dim, int64_t rotary, int64_t x_stride, int64_t y_stride, int interleaved,
+              float magnitude, bool vjp, hipStream_t s);
+int paged_append(int dtype, const void* k, const void* v, void* k_pages, void* v_pages, const PagedArgs& a, int64_t tokens,
+                 int64_t kv_heads, int64_t dim, int64_t kv_stride, const double* freqs, int64_t rotary, int interleaved,
+                 float magnitude, hipStream_t s);
+
+// ── packed_attn.hip ───────────────────────────────────────────────────────
+int packed_attention(int dtype, const void* q, const void* k, const void* v, const int32_t* starts, void* o, float* lse,
+                     int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride,
+                     int64_t kv_stride, int64_t o_stride, float scale, int causal, hipStream_t s);
+int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
+                         const float* lse, const int32_t* starts, void* dq, void* dk, void* dv, int64_t n_seqs,
+                         int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride, int64_t kv_stride,
+                         int64_t o_stride, float scale, int causal, hipStream_t s);
+int paged_attention(int dtype, const void* q, const void* k_pages, const void* v_pages, const PagedArgs& pages, void* o,
+                    int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride, int64_t o_stride,
+                    float scale, hipStream_t s);
+
 // ── elementwise.hip ───────────────────────────────────────────────────────
 int ew_chain(const mlxhip_ew_instr_t* prog, int n_instr, const float* const* inputs,
              int n_inputs, float* out, int64_t numel, hipStream_t s);

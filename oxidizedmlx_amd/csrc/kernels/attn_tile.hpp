@@ -1,0 +1,254 @@
+// attn_tile.hpp — tiles of attention over packed sequences: rows of a head in LDS,
+// the matrix fragments read from them, and which rows a workgroup has.
+//
+// Every product is 32 x 32 outputs a wave and 16 of the inner index a step:
+// v_mfma_f32_32x32x16 for 16-bit operands, eight v_mfma_f32_32x32x2 for f32. Of a
+// step's operand a lane (half h = lane / 32) holds eight inner values of row or
+// column lane % 32. Which eight is free as long as both operands agree:
+//   along a row of LDS     8 h + (0..7): 16-byte reads;
+//   against a product's    4 h + (0..3), 8 + 4 h + (0..3): an accumulator's
+//   own result             registers 8 s .. 8 s + 7 hold rows 16 s + those.
+// So the scores are formed transposed where their rows are what the next product
+// sums over, and go from accumulator to operand with no exchange between lanes.
+//
+// LDS: a row of DP values (head_dim rounded up to 64 or 128, zeros behind), chunk c of 16
+// bytes at c ^ swizzle(row). Row reads (lane = row, one chunk) then spread 16
+// rows over all banks, and the transposed reads (ds_read_b64_tr_b16: 4 rows x 64
+// bytes; f32: 32 values of one row) do too. The swizzle is applied by which
+// chunk a lane fetches; loads go straight from memory to LDS, 1 KiB to an instruction,
+// and chunks past the head or past the last row are zeros by the buffer's bounds.
+#pragma once
+
+#include "elem.hpp"
+#include "gemm16_impl.hpp"
+
+namespace mlxhip {
+namespace attn {
+
+using gemm16::f32x16;
+using gemm16::f32x4;
+using gemm16::u32x2;
+using gemm16::u32x4;
+
+constexpr int WAVES = 4, THREADS = 64 * WAVES;
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+
+template <int DT>
+constexpr int ELEM = DT == MLXHIP_DTYPE_F32 ? 4 : 2;
+
+template <int DT>
+struct Frag {  // eight inner values
+    u32x4 q[DT == MLXHIP_DTYPE_F32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ inline void mma(const Frag<DT>& a, const Frag<DT>& b, f32x16& acc) {
+    if constexpr (DT == MLXHIP_DTYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.q[j / 4][j % 4]), __uint_as_float(b.q[j / 4][j % 4]),
+                                                       acc, 0, 0, 0);
+    } else {
+        gemm16::mfma<DT>(a.q[0], b.q[0], acc);
+    }
+}
+
+// Registers 8 s .. 8 s + 7 of an accumulator as an operand.
+template <int DT>
+__device__ inline Frag<DT> frag_of(const float* v) {
+    Frag<DT> f;
+    if constexpr (DT == MLXHIP_DTYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.q[j / 4][j % 4] = __float_as_uint(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.q[0][j] = gemm16::pack2<DT>(v[2 * j], v[2 * j + 1]);
+    }
+    return f;
+}
+
+// The non-finite values of f as ones, zeros elsewhere; f is left with zeros in their place.
+template <int DT>
+__device__ inline Frag<DT> take_non_finite(Frag<DT>& f) {
+    Frag<DT> bad;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(f) / 16); ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t ones = 0;
+            if constexpr (DT == MLXHIP_DTYPE_F32) {
+                const bool b = (f.q[i][j] & 0x7F800000u) == 0x7F800000u;
+                ones = b ? 0x3F800000u : 0u;
+                f.q[i][j] = b ? 0u : f.q[i][j];
+            } else {
+                constexpr uint32_t EXP = DT == MLXHIP_DTYPE_BF16 ? 0x7F80u : 0x7C00u, ONE = DT == MLXHIP_DTYPE_BF16 ? 0x3F80u : 0x3C00u;
+#pragma unroll
+                for (int k = 0; k < 32; k += 16)
+                    if ((f.q[i][j] >> k & EXP) == EXP) {
+                        ones |= ONE << k;
+                        f.q[i][j] &= ~(0xFFFFu << k);
+                    }
+            }
+            bad.q[i][j] = ones;
+        }
+    return bad;
+}
+
+// A tile of ROWS rows of a head in LDS.
+template <int DT, int DP, int ROWS>
+struct Tile {
+    static constexpr int ROWB = DP * ELEM<DT>;       // bytes of a row
+    static constexpr int CPR = ROWB / 16;            // its chunks
+    static constexpr int RPI = 64 / CPR;             // rows of one load instruction
+    static constexpr int BYTES = ROWS * ROWB;
+    static constexpr int INSTR = ROWS / RPI;         // load instructions
+    static_assert(CPR >= 8 && CPR <= 32 && INSTR >= 1, "row of 128 to 512 bytes");
+
+    __device__ static inline int swizzle(int row) {
+        if constexpr (CPR == 8) return ((row >> 1) & 1) << 2 | ((row >> 2) & 3);  // two rows to 256 bytes
+        else return (row & 3) << 2 | ((row >> 2) & 3);
+    }
+};
+
+// One wave's loads of a tile: LW waves share its instructions, wave w takes
+// w, w + LW, ... voff: the lane's offset for each, from the first row of the
+// tile (or of the instruction, GROUPED), past any buffer where the chunk is past the head.
+template <int DT, int DP, int ROWS, int LW, bool GROUPED>
+struct TileLoader {
+    using T = Tile<DT, DP, ROWS>;
+    static constexpr int L = T::INSTR / LW;  // instructions of a wave
+    static_assert(L * LW == T::INSTR, "whole instructions to a wave");
+    uint32_t voff[L];
+    __device__ inline void init(int wave, int lane, int dim, uint32_t stride_bytes) {
+        const int r = lane / T::CPR, slot = lane % T::CPR;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int row = (i * LW + wave) * T::RPI + r;
+            const int c = slot ^ T::swizzle(row);
+            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(GROUPED ? r : row) * stride_bytes + c * 16 : gemm16::OOB;
+        }
+    }
+};
+
+// p and bytes are the same in all lanes; arithmetic on them may have gone through
+// vector registers, the descriptor is scalar.
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)hi << 32 | lo), 0,
+                                             __builtin_amdgcn_readfirstlane(bytes), gemm16::BUF_FLAGS);
+}
+
+// Row fragments: lane = row base + lane % 32, inner values 16 s + 8 h + (0..7).
+template <int DT, int DP, int ROWS>
+struct RowFrag {
+    using T = Tile<DT, DP, ROWS>;
+    uint32_t row, key;
+    __device__ inline void init(int lane) {
+        row = (uint32_t)(lane & 31) * T::ROWB;
+        key = (uint32_t)(T::swizzle(lane & 31) ^ ((lane >> 5) * (DT == MLXHIP_DTYPE_F32 ? 2 : 1)));
+    }
+    __device__ inline Frag<DT> read(const MLXHIP_LDS char* tile, int base_row, int s) const {
+        Frag<DT> f;
+        const MLXHIP_LDS char* p = tile + base_row * T::ROWB + row;
+        if constexpr (DT == MLXHIP_DTYPE_F32) {
+            f.q[0] = *(const MLXHIP_LDS u32x4*)(p + ((4 * s) ^ key) * 16);
+            f.q[1] = *(const MLXHIP_LDS u32x4*)(p + ((4 * s + 1) ^ key) * 16);
+        } else {
+            f.q[0] = *(const MLXHIP_LDS u32x4*)(p + ((2 * s) ^ key) * 16);
+        }
+        return f;
+    }
+};
+
+// Transposed fragments: lane = column 32 b + lane % 32, inner rows base + 4 h + (0..3),
+// base + 8 + 4 h + (0..3); base a multiple of 16.
+template <int DT, int DP, int ROWS>
+struct ColFrag {
+    using T = Tile<DT, DP, ROWS>;
+    int lane;
+    uint32_t at, key;  // 16 bits: the lane's source row and its chunk
+    __device__ inline void init(int l) {
+        lane = l;
+        const int g = l >> 4, t = l & 15;
+        at = (uint32_t)((4 * (g >> 1) + (t >> 2)) * T::ROWB + (t & 1) * 8);
+        key = (uint32_t)(2 * (g & 1) + ((t >> 1) & 1));
+    }
+    __device__ inline Frag<DT> read(const MLXHIP_LDS char* tile, int base, int b) const {
+        Frag<DT> f;
+        const MLXHIP_LDS char* p = tile + base * T::ROWB;
+        if constexpr (DT == MLXHIP_DTYPE_F32) {
+            const int h = lane >> 5, chunk = 8 * b + ((lane & 31) >> 2);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = 8 * (j / 4) + 4 * h + j % 4;
+                f.q[j / 4][j % 4] = *(const MLXHIP_LDS uint32_t*)(p + row * T::ROWB + ((chunk ^ T::swizzle(row)) << 4) + (lane & 3) * 4);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = 8 * r + 4 * (lane >> 5) + ((lane & 15) >> 2);  // of the source lane
+                const uint32_t c = (uint32_t)(4 * b) ^ (key ^ (uint32_t)T::swizzle(row));
+                const MLXHIP_LDS char* a = p + 8 * r * T::ROWB + at + c * 16;
+                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MLXHIP_LDS gemm16::i16x4*)a));
+                f.q[0][2 * r] = v.x;
+                f.q[0][2 * r + 1] = v.y;
+            }
+        }
+        return f;
+    }
+};
+
+// Row fragment of memory: eight values from element 16 s + 8 h of a row, zeros
+// past its end (head_dim is a multiple of 8) or where ok is false.
+template <int DT>
+__device__ inline Frag<DT> load_frag(const typename dev::Elem<DT>::type* row, int lane, int s, int dim, bool ok) {
+    Frag<DT> f;
+    const int d = 16 * s + 8 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < (DT == MLXHIP_DTYPE_F32 ? 2 : 1); ++i)
+        f.q[i] = ok && d < dim ? *reinterpret_cast<const u32x4*>(row + d + 4 * i) : u32x4{0, 0, 0, 0};
+    return f;
+}
+
+// The sequence and the tile in it that work item `item` names: the sequences' rows
+// (tokens times per_token) in tiles of `rows`, one after another. starts is the
+// caller's: what it says is brought into [0, tokens], a sequence that ends before it
+// starts has no rows. 64 sequences at a time, a wave together; false past the last tile.
+struct Place {
+    int seq, first, tokens, tile, tiles;
+};
+__device__ inline bool find_tile(const int32_t* __restrict__ starts, int n_seqs, int tokens, int per_token, int rows,
+                                 int item, Place* out) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < n_seqs; base += 64) {
+        const int i = base + lane;
+        int first = 0, n = 0;
+        if (i < n_seqs) {
+            first = min(max(starts[i], 0), tokens);
+            n = max(min(max(starts[i + 1], 0), tokens) - first, 0);
+        }
+        const int tiles = (int)(((int64_t)n * per_token + rows - 1) / rows);
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += up;
+        }
+        const uint64_t past = __ballot(sum > item);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            out->seq = base + at;
+            out->first = __builtin_amdgcn_readlane(first, at);
+            out->tokens = __builtin_amdgcn_readlane(n, at);
+            out->tiles = __builtin_amdgcn_readlane(tiles, at);
+            out->tile = item - (__builtin_amdgcn_readlane(sum, at) - out->tiles);
+            return true;
+        }
+        item -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+}  // namespace attn
+}  // namespace mlxhip

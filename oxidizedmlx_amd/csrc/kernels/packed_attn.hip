@@ -1,0 +1,102 @@
+// packed_attn.hip — which kernels a call of the packed or paged attention takes.
+#include "packed_attn.hpp"
+#include "elem.hpp"
+#include "../common.hpp"
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+namespace mlxhip {
+namespace {
+
+// Work items of sequences whose lengths are known on the device only: a tile more for each.
+int items_of(int64_t tokens, int64_t per_token, int64_t n_seqs, int64_t rows) {
+    return (int)(tokens * per_token / rows + std::min(n_seqs, tokens));
+}
+
+uint32_t flip_of(int dtype, float scale) {
+    return !(scale < 0) ? 0u : dtype == MLXHIP_DTYPE_F32 ? 0x80000000u : 0x80008000u;
+}
+
+// |scale| log2 e; never 0, which a masked score of -inf would not survive (scores
+// times the smallest normal number are 0 beside any other).
+float factor_of(float scale) { return std::max(std::fabs(scale) * 1.44269504088896340736f, FLT_MIN); }
+
+template <class F>
+int by_dtype(int dtype, F&& f) {
+    int rc = MLXHIP_OK;
+    with_float_dtype(dtype, [&](auto dt) { rc = f(dt); });
+    return rc;
+}
+
+}  // namespace
+
+int packed_attention(int dtype, const void* q, const void* k, const void* v, const int32_t* starts, void* o, float* lse,
+                     int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride,
+                     int64_t kv_stride, int64_t o_stride, float scale, int causal, hipStream_t s) {
+    attn::FwdArgs a{};
+    a.q = q, a.k = k, a.v = v, a.o = o, a.lse = lse, a.starts = starts;
+    a.n_seqs = (int)n_seqs, a.tokens = (int)tokens, a.heads = (int)heads, a.kv_heads = (int)kv_heads;
+    a.group = (int)(heads / kv_heads), a.dim = (int)dim;
+    a.q_stride = q_stride, a.kv_stride = kv_stride, a.o_stride = o_stride;
+    a.c = factor_of(scale), a.flip = flip_of(dtype, scale);
+    a.causal = causal, a.splits = 1;
+    a.items = items_of(tokens, a.group, n_seqs, attn::ROW_TILE);
+    return by_dtype(dtype, [&](auto dt) { return attn::fwd<decltype(dt)::value>(a, false, false, s); });
+}
+
+int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
+                         const float* lse, const int32_t* starts, void* dq, void* dk, void* dv, int64_t n_seqs,
+                         int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride, int64_t kv_stride,
+                         int64_t o_stride, float scale, int causal, hipStream_t s) {
+    attn::BwdArgs a{};
+    a.q = q, a.k = k, a.v = v, a.o = o, a.dout = dout, a.lse = lse, a.starts = starts;
+    a.dq = dq, a.dk = dk, a.dv = dv;
+    a.n_seqs = (int)n_seqs, a.tokens = (int)tokens, a.heads = (int)heads, a.kv_heads = (int)kv_heads;
+    a.group = (int)(heads / kv_heads), a.dim = (int)dim;
+    a.q_stride = q_stride, a.kv_stride = kv_stride, a.o_stride = o_stride;
+    a.c = factor_of(scale), a.scale = scale, a.flip = flip_of(dtype, scale);
+    a.causal = causal;
+    a.row_items = items_of(tokens, a.group, n_seqs, attn::ROW_TILE);
+    a.key_items = items_of(tokens, 1, n_seqs, attn::KEY_TILE);
+    // Few tiles of keys: a group's heads over several workgroups, their sums joined.
+    const int64_t wgs = a.key_items * kv_heads;
+    a.shares = (int)std::clamp<int64_t>(512 / std::max<int64_t>(wgs, 1), 1, a.group);
+    const size_t stats = (((size_t)tokens * heads + 63) & ~size_t(63)) * sizeof(float);
+    const size_t part = a.shares > 1 ? (size_t)a.shares * 2 * tokens * kv_heads * dim * sizeof(float) : 0;
+    void* ws = nullptr;
+    MLXHIP_TRY(stream_workspace(s, WS_PACKED, 2 * stats + part, &ws));
+    a.lse2 = (float*)ws, a.delta = (float*)((char*)ws + stats), a.part = (float*)((char*)ws + 2 * stats);
+    return by_dtype(dtype, [&](auto dt) { return attn::bwd<decltype(dt)::value>(a, s); });
+}
+
+int paged_attention(int dtype, const void* q, const void* k_pages, const void* v_pages, const PagedArgs& pages, void* o,
+                    int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride, int64_t o_stride,
+                    float scale, hipStream_t s) {
+    attn::FwdArgs a{};
+    a.q = q, a.k = k_pages, a.v = v_pages, a.o = o, a.starts = pages.starts, a.pages = pages;
+    a.n_seqs = pages.n_seqs, a.tokens = (int)tokens, a.heads = (int)heads, a.kv_heads = (int)kv_heads;
+    a.group = (int)(heads / kv_heads), a.dim = (int)dim;
+    a.q_stride = q_stride, a.o_stride = o_stride;
+    a.c = factor_of(scale), a.flip = flip_of(dtype, scale);
+    a.causal = 1;
+    // Up to 32 rows a sequence on average (single tokens of up to 32 heads to a K/V head, say).
+    const bool keys = tokens * a.group <= (int64_t)attn::FEW_ROWS * a.n_seqs;
+    a.items = items_of(tokens, a.group, a.n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
+    // The keys over several workgroups until there are 1024 (two rounds of two to a
+    // compute unit, so that sequences of different lengths even out), within 256 MiB of parts.
+    const int64_t most = pages.table_width << pages.page_shift, wgs = (int64_t)a.items * kv_heads;
+    int64_t splits = std::min<int64_t>({1024 / std::max<int64_t>(wgs, 1), ceil_div(most, attn::MIN_SPAN), 64});
+    const int64_t row = tokens * heads * (dim + 2) * (int64_t)sizeof(float);
+    splits = std::min<int64_t>(splits, (int64_t(256) << 20) / std::max<int64_t>(row, 1));
+    a.splits = (int)std::max<int64_t>(splits, 1);
+    if (a.splits > 1) {
+        void* ws = nullptr;
+        MLXHIP_TRY(stream_workspace(s, WS_PACKED, (size_t)(a.splits * row), &ws));
+        a.part = (float*)ws;
+    }
+    return by_dtype(dtype, [&](auto dt) { return attn::fwd<decltype(dt)::value>(a, true, keys, s); });
+}
+
+}  // namespace mlxhip

@@ -1,0 +1,447 @@
+// packed_attn_impl.hpp — attention of packed sequences with grouped heads, and of new
+// tokens over a cache in pages.
+//
+// For each sequence and K/V head the query rows are the pairs (token, head of the
+// group), row = token * group + head, so that a tile of K and V serves the whole group.
+// With c = scale log2 e and a row's running maximum m,
+//   S^T = K Q^T,  p = 2^(c S - c m),  l += sum p,  O^T += V^T p^T,
+// O and l rescaled when m moves: one pass over the keys. The transposed scores put a
+// query in a lane, its keys in the lane's registers: the maximum needs one exchange
+// between the two halves of a wave, p none before it is the next product's operand.
+//
+// Roundings: scores, p's sum and O are f32. p is rounded to the operands' type for its
+// product (relative 2^-9 or 2^-12 each, as many independent ones as keys, beside the one
+// that the result itself gets); f16's p is scaled by 2^6, which keeps probabilities
+// down to 2^-20 normal. A maximum moves only once it is passed by 2^8: p stays below
+// 2^14 and most tiles rescale nothing.
+//
+// ROWS: four waves of 32 rows share tiles of 64 keys (f32: 32), two in LDS, the next
+// on its way. KEYS, for few rows: the four waves have the same 32 rows and every fourth
+// tile of 32 keys each, with LDS of their own and no barrier, and join at the end.
+// Where there are few tiles of rows the keys are split over workgroups too; the parts
+// (O, m, l in f32) are joined by a second kernel.
+#pragma once
+
+#include "attn_tile.hpp"
+#include "packed_attn.hpp"
+
+namespace mlxhip {
+namespace attn {
+
+// A sequence's parts: as many as its keys are worth, up to the launch's.
+__device__ inline int parts_of(int keys, int splits) { return min(splits, max(1, (keys + MIN_SPAN - 1) / MIN_SPAN)); }
+
+__device__ inline int length_of(const PagedArgs& p, int seq) { return __builtin_amdgcn_readfirstlane(max(p.lens[seq], 0)); }
+// Of a length's positions those that the table has room for.
+__device__ inline int keys_of(const PagedArgs& p, int length) { return (int)min((int64_t)length, p.table_width << p.page_shift); }
+
+template <int DT, int DP, bool PAGED, bool KEYS>
+__global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS), amdgpu_waves_per_eu(KEYS && DT == MLXHIP_DTYPE_F32 ? 1 : 2, 2)))
+void attn_fwd_kernel(FwdArgs a) {
+    constexpr int BM = KEYS ? FEW_ROWS : ROW_TILE, BN = KEYS || DT == MLXHIP_DTYPE_F32 ? 32 : 64;
+    constexpr int LW = KEYS ? 1 : WAVES, STAGES = KEYS ? 1 : 2;
+    constexpr int KB = BN / 32, KS = DP / 16, DB = DP / 32, EB = ELEM<DT>;
+    constexpr float SHIFT = DT == MLXHIP_DTYPE_F16 ? 6.0f : 0.0f, MOVE = 8.0f;
+    using T = Tile<DT, DP, BN>;
+    constexpr int TILES = (KEYS ? WAVES : 1) * STAGES * 2 * T::BYTES, JOIN = KEYS ? WAVES * 32 * (DP + 2) * 4 : 0;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[TILES > JOIN ? TILES : JOIN];
+    typedef typename dev::Elem<DT>::type E;
+
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw + (KEYS ? wave * STAGES * 2 * T::BYTES : 0);
+
+    // Workgroups go round the 8 dies: with a multiple of 8 K/V heads each die keeps
+    // to its own, whose keys its L2 then holds. Long tiles of a causal sequence first.
+    const int lin = blockIdx.x;
+    const int per8 = a.kv_heads & 7 ? 1 : 8;
+    const int item = per8 == 8 ? (lin >> 3) % a.items : lin / a.kv_heads;
+    const int kvh = per8 == 8 ? (lin >> 3) / a.items * 8 + (lin & 7) : lin % a.kv_heads;
+    Place at;
+    if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return;
+    const int row0 = (at.tiles - 1 - at.tile) * BM, rows = at.tokens * a.group;
+    const int length = PAGED ? length_of(a.pages, at.seq) : at.tokens, keys = PAGED ? keys_of(a.pages, length) : length;
+    const int shift = length - at.tokens;  // position of the first new token
+    const int parts = PAGED ? parts_of(keys, a.splits) : 1, part = PAGED ? blockIdx.y : 0;
+    if (part >= parts) return;
+
+    // This lane's row and the last key it sees.
+    const int wrow = row0 + (KEYS ? 0 : 32 * wave), row = wrow + (lane & 31);
+    const bool live = row < rows;
+    const int tok = (int)((uint32_t)row / (uint32_t)a.group), head = kvh * a.group + (row - tok * a.group);
+    const int lim = !live ? -1 : a.causal ? min(tok + shift, keys - 1) : keys - 1;
+    const auto last_key = [&](int r) {  // of row r, or of the last row
+        return a.causal ? min((min(r, rows - 1)) / a.group + shift, keys - 1) : keys - 1;
+    };
+    const int wave_last = last_key(wrow + 31), wave_first = last_key(wrow);
+    const int n_tiles = max(0, last_key(row0 + BM - 1) + BN) / BN;
+    const int t0 = (int)((int64_t)n_tiles * part / parts), t1 = (int)((int64_t)n_tiles * (part + 1) / parts);
+
+    Frag<DT> q[KS];
+    const E* qrow = (const E*)a.q + (int64_t)(at.first + (live ? tok : 0)) * a.q_stride + (int64_t)(live ? head : 0) * a.dim;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        q[s] = load_frag<DT>(qrow, lane, s, a.dim, live);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(q[s]) / 16); ++i) q[s].q[i] ^= a.flip;
+    }
+
+    // Loads: a tile's rows one after another in memory, or page by page (an
+    // instruction's rows lie in one page: pages hold a multiple of 16).
+    TileLoader<DT, DP, BN, LW, PAGED> loader;
+    const uint32_t stride_bytes = (uint32_t)((PAGED ? a.dim : a.kv_stride) * EB);
+    loader.init(KEYS ? 0 : wave, lane, a.dim, stride_bytes);
+    const char* kbase = (const char*)a.k;
+    const char* vbase = (const char*)a.v;
+    if constexpr (!PAGED) {
+        const int64_t off = ((int64_t)at.first * a.kv_stride + (int64_t)kvh * a.dim) * EB;
+        kbase += off;
+        vbase += off;
+    }
+    // Page numbers of the tile's instructions, one to a lane, read a tile ahead.
+    const int32_t* table = PAGED ? a.pages.table + (int64_t)at.seq * a.pages.table_width : nullptr;
+    const auto pages_of = [&](int j) {
+        int page = -1;
+        if constexpr (PAGED) {
+            const int r = j * BN + (lane * LW + (KEYS ? 0 : wave)) * T::RPI;
+            if (lane < loader.L && r < keys) page = table[r >> a.pages.page_shift];
+        }
+        return page;
+    };
+    const auto issue = [&](const char* base, MLXHIP_LDS char* tile, int j, int pages) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < loader.L; ++i) {
+                const int qi = i * LW + (KEYS ? 0 : wave), r = j * BN + qi * T::RPI;
+                const int left = min(keys - r, T::RPI), page = __builtin_amdgcn_readlane(pages, i);
+                const bool ok = page >= 0 && page < a.pages.pages;
+                const int64_t at_row = (((int64_t)(ok ? page : 0) * a.kv_heads + kvh) << a.pages.page_shift) +
+                                       (r & ((1 << a.pages.page_shift) - 1));
+                gemm16::lds_load16(buffer(base + at_row * stride_bytes, ok ? (uint32_t)left * stride_bytes : 0u),
+                                   tile + qi * 1024, loader.voff[i]);
+            }
+        } else {
+            const int left = max(0, min(keys - j * BN, BN));
+            const auto rsrc = buffer(base + (int64_t)j * BN * stride_bytes, (uint32_t)left * stride_bytes);
+#pragma unroll
+            for (int i = 0; i < loader.L; ++i)
+                gemm16::lds_load16(rsrc, tile + (i * LW + (KEYS ? 0 : wave)) * 1024, loader.voff[i]);
+        }
+    };
+
+    RowFrag<DT, DP, BN> kf;
+    ColFrag<DT, DP, BN> vf;
+    kf.init(lane);
+    vf.init(lane);
+    f32x16 o[DB] = {};
+    float m = -INFINITY, l = 0.0f;
+
+    // One tile of keys from k0 on. after_scores: what may start once K has been read.
+    const auto compute = [&](auto careful, const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int k0, auto&& after_scores) {
+        f32x16 sc[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            sc[b] = f32x16{};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) mma<DT>(kf.read(kt, 32 * b, s), q[s], sc[b]);
+        }
+        after_scores();
+        const bool masked = k0 + BN - 1 > wave_first || !live;
+        const bool any_masked = __ballot(masked) != 0;
+        if (any_masked) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (k0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4 > lim) sc[b][r] = -INFINITY;
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[b][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (__ballot(mx > m && !((mx - m) * a.c <= MOVE))) {
+            const float to = fmaxf(m, mx);
+            const float by = to == m ? 1.0f : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - to) * a.c);
+            m = to;
+            l *= by;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= by;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * a.c - SHIFT;
+        Frag<DT> p[2 * KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            float e[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r], a.c, -mc));
+                l += e[r];
+            }
+            p[2 * b] = frag_of<DT>(e);
+            p[2 * b + 1] = frag_of<DT>(e + 8);
+        }
+        if (decltype(careful)::value && any_masked) {
+            // p = 0 of a masked key would make NaN of a non-finite v: those are taken out of the
+            // product, and what is counted of them among the keys that a row sees makes it NaN.
+#pragma unroll 1
+            for (int s = 0; s < 2 * KB; ++s) {
+                float sees[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sees[j] = k0 + 16 * s + 8 * (j / 4) + 4 * h + j % 4 <= lim ? 1.0f : 0.0f;
+                Frag<DT> ps = p[0];
+#pragma unroll
+                for (int i = 1; i < 2 * KB; ++i)
+                    if (i == s) ps = p[i];
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    Frag<DT> v = vf.read(vt, 16 * s, d);
+                    const Frag<DT> bad = take_non_finite<DT>(v);
+                    mma<DT>(v, ps, o[d]);
+                    f32x16 count = {};
+                    mma<DT>(bad, frag_of<DT>(sees), count);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] = count[r] > 0.0f ? NAN : o[d][r];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int s = 0; s < 2 * KB; ++s) mma<DT>(vf.read(vt, 16 * s, d), p[s], o[d]);
+        }
+    };
+
+    const auto walk = [&](auto careful) {
+
+        if constexpr (KEYS) {
+            MLXHIP_LDS char* kt = smem;
+            MLXHIP_LDS char* vt = smem + T::BYTES;
+            int j = t0 + wave, pages = pages_of(j), next = pages_of(j + WAVES);
+            if (j < t1) {
+                issue(kbase, kt, j, pages);
+                issue(vbase, vt, j, pages);
+            }
+            for (; j < t1; j += WAVES) {
+                gemm16::wait_vmcnt<0>();
+                const int then = pages_of(j + 2 * WAVES);
+                compute(careful, kt, vt, j * BN, [&] {  // K has been read
+                    __builtin_amdgcn_s_waitcnt(0xC07F);
+                    if (j + WAVES < t1) issue(kbase, kt, j + WAVES, next);
+                });
+                __builtin_amdgcn_s_waitcnt(0xC07F);
+                if (j + WAVES < t1) issue(vbase, vt, j + WAVES, next);
+                next = then;
+            }
+        } else {
+            int pages = pages_of(t0);
+            if (t0 < t1) {
+                issue(kbase, smem, t0, pages);
+                issue(vbase, smem + T::BYTES, t0, pages);
+            }
+            pages = pages_of(t0 + 1);
+            for (int j = t0; j < t1; ++j) {
+                MLXHIP_LDS char* tile = smem + ((j - t0) & 1) * 2 * T::BYTES;
+                MLXHIP_LDS char* other = smem + ((j - t0 + 1) & 1) * 2 * T::BYTES;
+                gemm16::wait_vmcnt<0>();
+                gemm16::lds_barrier();
+                if (j + 1 < t1) {
+                    issue(kbase, other, j + 1, pages);
+                    issue(vbase, other + T::BYTES, j + 1, pages);
+                    pages = pages_of(j + 2);
+                }
+                if (wrow < rows && j * BN <= wave_last) compute(careful, tile, tile + T::BYTES, j * BN, [] {});
+            }
+        }
+    };
+    walk(std::false_type{});
+    // Where a result is not finite, a second walk that keeps non-finite values of v from
+    // rows that do not see them.
+    float finite = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) finite = __builtin_fmaf(o[d][r], 0.0f, finite);
+    if (__syncthreads_or(finite != 0.0f)) {  // NaN is not 0
+        // Addresses formed anew, or those of both walks take registers from the first.
+        int again = lane;
+        asm volatile("" : "+v"(again));
+        kf.init(again);
+        vf.init(again);
+        loader.init(KEYS ? 0 : wave, again, a.dim, stride_bytes);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+        m = -INFINITY;
+        l = 0.0f;
+        walk(std::true_type{});
+    }
+    l += __shfl_xor(l, 32, 64);
+    float mc = m == -INFINITY ? 0.0f : m * a.c - SHIFT;  // l and o are sums of 2^(c S - mc)
+    bool empty = m == -INFINITY && l == 0.0f;            // no key seen (by this wave)
+
+    if constexpr (KEYS) {
+        // Joined through LDS: each wave's o, mc, l for the 32 rows; wave w then sums
+        // the four for every fourth part of the head.
+        __syncthreads();
+        float* all = reinterpret_cast<float*>(smem_raw);
+        float* mine = all + wave * 32 * (DP + 2);
+        const int r = lane & 31;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mine[(32 * d + 8 * (i / 4) + 4 * h + i % 4) * 32 + r] = o[d][i];
+        if (h == 0) {
+            mine[DP * 32 + r] = empty ? -INFINITY : mc;
+            mine[(DP + 1) * 32 + r] = l;
+        }
+        __syncthreads();
+        float top = -INFINITY, w[WAVES];
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            w[i] = all[i * 32 * (DP + 2) + DP * 32 + r];
+            top = w[i] > top || w[i] != w[i] ? w[i] : top;
+        }
+        empty = top == -INFINITY;
+        mc = empty ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            w[i] = w[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[i] - mc);
+            l += w[i] * all[i * 32 * (DP + 2) + (DP + 1) * 32 + r];
+        }
+        // Head values 4 (h + 2 wave + 8 i) .. + 3 of the lane's row.
+        const float inv = 1.0f / l;
+        const bool whole = parts == 1;
+        for (int d0 = 4 * (h + 2 * wave); d0 < a.dim; d0 += 32) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) {
+                    const float x = all[i * 32 * (DP + 2) + (d0 + e) * 32 + r];
+                    if (w[i] != 0.0f) v[e] += w[i] * x;
+                }
+                if (whole) v[e] = lim < 0 ? 0.0f : v[e] * inv;
+            }
+            if (!live) continue;
+            if (!whole) {
+                float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 2);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[d0 + e] = v[e];
+                if (d0 == 0) {
+                    to[a.dim] = empty ? -INFINITY : mc;
+                    to[a.dim + 1] = l;
+                }
+                continue;
+            }
+            E* to = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim + d0;
+            if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+            else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
+        }
+        return;
+    }
+
+    if (!live) return;
+    if (parts > 1) {
+        float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 2);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int at_d = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
+                if (at_d < a.dim) to[at_d] = o[d][r];
+            }
+        if (h == 0) {
+            to[a.dim] = empty ? -INFINITY : mc;
+            to[a.dim + 1] = l;
+        }
+        return;
+    }
+    if (a.lse && h == 0) a.lse[(int64_t)(at.first + tok) * a.heads + head] = lim < 0 ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
+    const float inv = 1.0f / l;
+    E* orow = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at_d = 32 * d + 8 * g + 4 * h;
+            if (at_d >= a.dim) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = lim < 0 ? 0.0f : o[d][4 * g + e] * inv;
+            if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(orow + at_d) = f32x4{v[0], v[1], v[2], v[3]};
+            else *reinterpret_cast<u32x2*>(orow + at_d) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
+        }
+}
+
+// The parts of a row joined: a wave to a row of a token's head.
+template <int DT>
+__global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * WAVES + threadIdx.x / 64;
+    const int lane = threadIdx.x & 63;
+    if (row >= (int64_t)a.tokens * a.heads) return;
+    const int token = (int)(row / a.heads), head = (int)(row - (int64_t)token * a.heads);
+    Place at;
+    // Of a sequence's tokens each is a tile: `item` counts the sequences' tokens.
+    const int first = max(a.starts[0], 0);
+    if (token < first || !find_tile(a.starts, a.n_seqs, a.tokens, 1, 1, token - first, &at) || at.first + at.tile != token) return;
+    const int length = length_of(a.pages, at.seq), parts = parts_of(keys_of(a.pages, length), a.splits);
+    if (parts == 1) return;
+    const int64_t step = (int64_t)a.tokens * a.heads * (a.dim + 2);
+    const float* p = a.part + row * (a.dim + 2);
+    float m = -INFINITY;
+    if (lane < parts) m = p[lane * step + a.dim];
+    float top = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float other = __shfl_xor(top, o, 64);
+        top = other > top || other != other ? other : top;
+    }
+    const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    float l = w == 0.0f ? 0.0f : w * p[lane * step + a.dim + 1];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    const bool none = at.tile + length - at.tokens < 0;
+    typedef typename dev::Elem<DT>::type E;
+    E* to = (E*)a.o + (int64_t)token * a.o_stride + (int64_t)head * a.dim;
+    for (int d = 2 * lane; d < a.dim; d += 128) {
+        float x = 0.0f, y = 0.0f;
+        for (int i = 0; i < parts; ++i) {
+            const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
+            if (wi == 0.0f) continue;
+            x += wi * p[i * step + d];
+            y += wi * p[i * step + d + 1];
+        }
+        x = none ? 0.0f : x / l;
+        y = none ? 0.0f : y / l;
+        if constexpr (DT == MLXHIP_DTYPE_F32) {
+            to[d] = x;
+            to[d + 1] = y;
+        } else {
+            *reinterpret_cast<uint32_t*>(to + d) = gemm16::pack2<DT>(x, y);
+        }
+    }
+}
+
+template <int DT, int DP, bool PAGED, bool KEYS>
+int launch_fwd(const FwdArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((attn_fwd_kernel<DT, DP, PAGED, KEYS>), dim3((unsigned)(a.items * a.kv_heads), (unsigned)a.splits),
+                       dim3(THREADS), 0, s, a);
+    MLXHIP_TRY(launch_check("attn_fwd_kernel"));
+    if (a.splits == 1) return MLXHIP_OK;
+    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)ceil_div((int64_t)a.tokens * a.heads, WAVES)), dim3(THREADS), 0, s, a);
+    return launch_check("attn_join_kernel");
+}
+
+template <int DT>
+int fwd(const FwdArgs& a, bool paged, bool keys, hipStream_t s) {
+    const bool wide = a.dim > 64;
+    if (!paged) return wide ? launch_fwd<DT, 128, false, false>(a, s) : launch_fwd<DT, 64, false, false>(a, s);
+    if (keys) return wide ? launch_fwd<DT, 128, true, true>(a, s) : launch_fwd<DT, 64, true, true>(a, s);
+    return wide ? launch_fwd<DT, 128, true, false>(a, s) : launch_fwd<DT, 64, true, false>(a, s);
+}
+
+}  // namespace attn
+}  // namespace mlxhip
