@@ -67,6 +67,18 @@ __device__ inline Frag<DT> frag_of(const float* v) {
     return f;
 }
 
+// What frag_of rounds off: v less the operand, as another operand.
+template <int DT>
+__device__ inline Frag<DT> rest_of(const float* v, const Frag<DT>& f) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        r[2 * j] = v[2 * j] - dev::to_f32<DT>((uint16_t)f.q[0][j]);
+        r[2 * j + 1] = v[2 * j + 1] - dev::to_f32<DT>((uint16_t)(f.q[0][j] >> 16));
+    }
+    return frag_of<DT>(r);
+}
+
 // The non-finite values of f as ones, zeros elsewhere; f is left with zeros in their place.
 template <int DT>
 __device__ inline Frag<DT> take_non_finite(Frag<DT>& f) {
@@ -110,26 +122,6 @@ struct Tile {
     }
 };
 
-// One wave's loads of a tile: LW waves share its instructions, wave w takes
-// w, w + LW, ... voff: the lane's offset for each, from the first row of the
-// tile (or of the instruction, GROUPED), past any buffer where the chunk is past the head.
-template <int DT, int DP, int ROWS, int LW, bool GROUPED>
-struct TileLoader {
-    using T = Tile<DT, DP, ROWS>;
-    static constexpr int L = T::INSTR / LW;  // instructions of a wave
-    static_assert(L * LW == T::INSTR, "whole instructions to a wave");
-    uint32_t voff[L];
-    __device__ inline void init(int wave, int lane, int dim, uint32_t stride_bytes) {
-        const int r = lane / T::CPR, slot = lane % T::CPR;
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const int row = (i * LW + wave) * T::RPI + r;
-            const int c = slot ^ T::swizzle(row);
-            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(GROUPED ? r : row) * stride_bytes + c * 16 : gemm16::OOB;
-        }
-    }
-};
-
 // p and bytes are the same in all lanes; arithmetic on them may have gone through
 // vector registers, the descriptor is scalar.
 __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
@@ -138,6 +130,49 @@ __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)hi << 32 | lo), 0,
                                              __builtin_amdgcn_readfirstlane(bytes), gemm16::BUF_FLAGS);
 }
+
+// lds_load16 and its 4-byte form (lane i to dst + 4 i), behind the five cycles that a scalar
+// register written by the vector unit (as the descriptor's parts may be, see buffer)
+// takes to reach a memory instruction: the compiler counts them for its own
+// instructions only, and an asm block that follows too soon loads by the old descriptor.
+__device__ inline void lds_load16(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* dst, uint32_t voff) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
+}
+__device__ inline void lds_load4(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* dst, uint32_t voff) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+    asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
+}
+
+// One wave's loads of a tile: LW waves share its instructions, wave w takes
+// w, w + LW, ...; instruction i from the row where it starts. voff: the lane's offset there,
+// past any buffer where the chunk is past the head. The swizzle comes round after 16
+// rows, so that a few offsets serve all.
+template <int DT, int DP, int ROWS, int LW>
+struct TileLoader {
+    using T = Tile<DT, DP, ROWS>;
+    static constexpr int L = T::INSTR / LW, STEP = LW * T::RPI;  // instructions of a wave, rows from one to the next
+    static constexpr int ROUND = STEP >= 16 ? 1 : L < 16 / STEP ? L : 16 / STEP;
+    static_assert(L * LW == T::INSTR && (16 % STEP == 0 || STEP % 16 == 0), "whole instructions to a wave");
+    uint32_t voff[ROUND];
+    __device__ inline void init(int wave, int lane, int dim, uint32_t stride_bytes) {
+        const int r = lane / T::CPR, slot = lane % T::CPR;
+#pragma unroll
+        for (int i = 0; i < ROUND; ++i) {
+            const int c = slot ^ T::swizzle((i * LW + wave) * T::RPI + r);
+            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)r * stride_bytes + c * 16 : gemm16::OOB;
+        }
+    }
+    // `left` rows (1 or more) from p on, stride_bytes apart, to the tile; zeros behind them.
+    __device__ inline void rows(const char* p, int left, uint32_t stride_bytes, MLXHIP_LDS char* tile, int wave) const {
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const int row = (i * LW + wave) * T::RPI;
+            lds_load16(buffer(p + (int64_t)row * stride_bytes, (uint32_t)max(0, min(left - row, T::RPI)) * stride_bytes),
+                       tile + (i * LW + wave) * 1024, voff[i % ROUND]);
+        }
+    }
+};
 
 // Row fragments: lane = row base + lane % 32, inner values 16 s + 8 h + (0..7).
 template <int DT, int DP, int ROWS>

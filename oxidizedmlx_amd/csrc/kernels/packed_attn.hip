@@ -62,7 +62,7 @@ int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v,
     a.key_items = items_of(tokens, 1, n_seqs, attn::KEY_TILE);
     // Few tiles of keys: a group's heads over several workgroups, their sums joined.
     const int64_t wgs = a.key_items * kv_heads;
-    a.shares = (int)std::clamp<int64_t>(512 / std::max<int64_t>(wgs, 1), 1, a.group);
+    a.shares = (int)std::clamp<int64_t>(256 / std::max<int64_t>(wgs, 1), 1, a.group);
     const size_t stats = (((size_t)tokens * heads + 63) & ~size_t(63)) * sizeof(float);
     const size_t part = a.shares > 1 ? (size_t)a.shares * 2 * tokens * kv_heads * dim * sizeof(float) : 0;
     void* ws = nullptr;

@@ -26,7 +26,7 @@ int fwd(const FwdArgs& a, bool paged, bool keys, hipStream_t s);
 struct BwdArgs {
     const void *q, *k, *v, *o, *dout;
     const float* lse;        // [tokens][heads]
-    float *lse2, *delta;     // [heads][tokens]: lse log2 e less the shift of p, rowsum(dO o O)
+    float *lse2, *delta;     // [heads][tokens], dQ's kernel for dK and dV's: lse log2 e less the shift of p, rowsum(dO o O)
     float* part;             // [shares][2][tokens][kv_heads][dim] (shares > 1): dK, dV
     void *dq, *dk, *dv;
     const int32_t* starts;
@@ -41,6 +41,8 @@ int bwd(const BwdArgs& a, hipStream_t s);
 
 // Rows of a work item: query rows (token, head of the group) and keys.
 constexpr int ROW_TILE = 128, FEW_ROWS = 32, KEY_TILE = 128;
+// Rows that see up to as many keys get P and dS in two terms in the gradients of 16-bit types.
+constexpr int FINE_KEYS = 256;
 // Keys that are worth a workgroup of their own.
 constexpr int MIN_SPAN = 256;
 

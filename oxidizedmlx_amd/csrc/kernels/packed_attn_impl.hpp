@@ -88,7 +88,7 @@ void attn_fwd_kernel(FwdArgs a) {
 
     // Loads: a tile's rows one after another in memory, or page by page (an
     // instruction's rows lie in one page: pages hold a multiple of 16).
-    TileLoader<DT, DP, BN, LW, PAGED> loader;
+    TileLoader<DT, DP, BN, LW> loader;
     const uint32_t stride_bytes = (uint32_t)((PAGED ? a.dim : a.kv_stride) * EB);
     loader.init(KEYS ? 0 : wave, lane, a.dim, stride_bytes);
     const char* kbase = (const char*)a.k;
@@ -117,15 +117,11 @@ void attn_fwd_kernel(FwdArgs a) {
                 const bool ok = page >= 0 && page < a.pages.pages;
                 const int64_t at_row = (((int64_t)(ok ? page : 0) * a.kv_heads + kvh) << a.pages.page_shift) +
                                        (r & ((1 << a.pages.page_shift) - 1));
-                gemm16::lds_load16(buffer(base + at_row * stride_bytes, ok ? (uint32_t)left * stride_bytes : 0u),
-                                   tile + qi * 1024, loader.voff[i]);
+                lds_load16(buffer(base + at_row * stride_bytes, ok ? (uint32_t)left * stride_bytes : 0u),
+                                   tile + qi * 1024, loader.voff[i % loader.ROUND]);
             }
         } else {
-            const int left = max(0, min(keys - j * BN, BN));
-            const auto rsrc = buffer(base + (int64_t)j * BN * stride_bytes, (uint32_t)left * stride_bytes);
-#pragma unroll
-            for (int i = 0; i < loader.L; ++i)
-                gemm16::lds_load16(rsrc, tile + (i * LW + (KEYS ? 0 : wave)) * 1024, loader.voff[i]);
+            loader.rows(base + (int64_t)j * BN * stride_bytes, keys - j * BN, stride_bytes, tile, KEYS ? 0 : wave);
         }
     };
 

@@ -1,16 +1,21 @@
 // packed_attn_vjp_impl.hpp — gradients of attention over packed sequences.
 //
-// With P = 2^(c S - lse log2 e), D = rowsum(dO o O) (one small kernel writes lse log2 e
-// and D as the others read them):
+// With P = 2^(c S - lse log2 e), D = rowsum(dO o O):
 //   dS = P o (dO V^T - D),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
 // Two kernels, so that every sum has one owner and a fixed order: dQ by tiles of query rows
-// (S and dO V^T transposed, a query to a lane), dK and dV by tiles of keys (a key to a lane), which
-// walk over the group's heads and their tokens. S and dO V^T are formed in both: seven
-// products where one kernel with atomic sums of dQ would take five.
+// (S and dO V^T transposed, a query to a lane; it leaves lse log2 e and D as the other reads
+// them), then dK and dV by tiles of keys (a key to a lane), which walk over the group's heads
+// and their tokens. S and dO V^T are formed in both: seven products where one kernel
+// with atomic sums of dQ would take five.
 //
-// Roundings: P and dS to the operands' type for their products, sums in f32. f16 would
-// lose dS below 2^-24: each column of dS (a query's in dQ, a key's in dK) has a power of two
-// of its own that brings it to about 2^12, changed (with the sum so far) when a later
+// Roundings: sums are f32; P and dS are rounded to the operands' type for their products, as
+// many independent errors as keys or rows, together about the one that a result itself gets.
+// Rows that see few keys carry most of a causal sequence's gradient (P is about 1 / keys), so
+// those that see up to 256 have P and dS in two terms, the second what the first
+// rounds off; and D, which the rounding of O moves (by as much as dS itself after a few keys),
+// is formed anew for them, as the row's sum of P dP, in a walk before the one over dS.
+// f16 would lose dS below 2^-24: each column of dS (a query's in dQ, a key's in dK) has a power of
+// two of its own that brings it to about 2^12, changed (with the sum so far) when a later
 // tile outgrows it; P is scaled by 2^14. bf16 and f32 have the range.
 #pragma once
 
@@ -22,30 +27,6 @@ namespace attn {
 
 template <int DT>
 constexpr float P_SHIFT = DT == MLXHIP_DTYPE_F16 ? 14.0f : 0.0f;
-
-// 16 lanes to a row (token, head).
-template <int DT>
-__global__ __launch_bounds__(THREADS) void attn_stats_kernel(BwdArgs a) {
-    const int64_t row = (int64_t)blockIdx.x * (THREADS / 16) + threadIdx.x / 16;
-    if (row >= (int64_t)a.tokens * a.heads) return;
-    const int token = (int)(row / a.heads), head = (int)(row - (int64_t)token * a.heads);
-    const int64_t at = token * a.o_stride + (int64_t)head * a.dim;
-    typedef typename dev::Elem<DT>::type E;
-    constexpr int V = dev::Elem<DT>::VEC;
-    float sum = 0.0f;
-    for (int d = (threadIdx.x & 15) * V; d < a.dim; d += 16 * V) {
-        float o[V], g[V];
-        dev::unpack<DT>({*reinterpret_cast<const u32x4*>((const E*)a.o + at + d)}, o);
-        dev::unpack<DT>({*reinterpret_cast<const u32x4*>((const E*)a.dout + at + d)}, g);
-#pragma unroll
-        for (int e = 0; e < V; ++e) sum += o[e] * g[e];
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (threadIdx.x & 15) return;
-    a.delta[(int64_t)head * a.tokens + token] = sum;
-    a.lse2[(int64_t)head * a.tokens + token] = a.lse[row] * LOG2E - P_SHIFT<DT>;
-}
 
 // f16: the power of two of a lane's column of dS, and the sums in it.
 template <int DT>
@@ -133,17 +114,31 @@ void attn_dq_kernel(BwdArgs a) {
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(q[s]) / 16); ++i) q[s].q[i] ^= a.flip;
     }
-    const float lse2 = a.lse2[(int64_t)head * a.tokens + token], delta = a.delta[(int64_t)head * a.tokens + token];
+    const float lse2 = a.lse[token * a.heads + head] * LOG2E - P_SHIFT<DT>;
+    float delta = 0.0f;
+    {
+        const E* orow = (const E*)a.o + token * a.o_stride + (int64_t)head * a.dim;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const Frag<DT> y = load_frag<DT>(orow, lane, s, a.dim, live);
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(y) / 16); ++i) {
+                float u[dev::Elem<DT>::VEC], w[dev::Elem<DT>::VEC];
+                dev::unpack<DT>({y.q[i]}, u);
+                dev::unpack<DT>({g[s].q[i]}, w);
+#pragma unroll
+                for (int e = 0; e < dev::Elem<DT>::VEC; ++e) delta = __builtin_fmaf(u[e], w[e], delta);
+            }
+        }
+        delta += __shfl_xor(delta, 32, 64);
+    }
 
-    TileLoader<DT, DP, BN, WAVES, false> loader;
+    TileLoader<DT, DP, BN, WAVES> loader;
     const uint32_t stride_bytes = (uint32_t)(a.kv_stride * EB);
     loader.init(wave, lane, a.dim, stride_bytes);
     const int64_t off = ((int64_t)at.first * a.kv_stride + (int64_t)kvh * a.dim) * EB;
     const auto issue = [&](const void* p, MLXHIP_LDS char* tile, int j) {
-        const int left = max(0, min(n - j * BN, BN));
-        const auto rsrc = buffer((const char*)p + off + (int64_t)j * BN * stride_bytes, (uint32_t)left * stride_bytes);
-#pragma unroll
-        for (int i = 0; i < loader.L; ++i) gemm16::lds_load16(rsrc, tile + (i * WAVES + wave) * 1024, loader.voff[i]);
+        loader.rows((const char*)p + off + (int64_t)j * BN * stride_bytes, n - j * BN, stride_bytes, tile, wave);
     };
 
     RowFrag<DT, DP, BN> rf;
@@ -152,75 +147,103 @@ void attn_dq_kernel(BwdArgs a) {
     cf.init(lane);
     f32x16 dq[DB] = {};
     Column<DT> column;
-    if (n_tiles > 0) {
-        issue(a.k, smem, 0);
-        issue(a.v, smem + T::BYTES, 0);
-    }
-    for (int j = 0; j < n_tiles; ++j) {
-        const MLXHIP_LDS char* kt = smem + (j & 1) * 2 * T::BYTES;
-        const MLXHIP_LDS char* vt = kt + T::BYTES;
-        MLXHIP_LDS char* other = smem + ((j + 1) & 1) * 2 * T::BYTES;
-        gemm16::wait_vmcnt<0>();
-        gemm16::lds_barrier();
-        if (j + 1 < n_tiles) {
-            issue(a.k, other, j + 1);
-            issue(a.v, other + T::BYTES, j + 1);
+    enum { PLAIN, ROW_SUM, FINE };
+    float sum = 0.0f;  // ROW_SUM: of P (dP - D), 0 were D exact
+    const auto walk = [&](auto which) {
+        constexpr int KIND = decltype(which)::value;
+        if (n_tiles > 0) {
+            issue(a.k, smem, 0);
+            issue(a.v, smem + T::BYTES, 0);
         }
-        if (wrow >= rows) continue;
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const int k0 = j * BN + 32 * b;
-            if (k0 > wave_last) break;
-            f32x16 sc = {}, dp = {};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                mma<DT>(rf.read(kt, 32 * b, s), q[s], sc);
-                mma<DT>(rf.read(vt, 32 * b, s), g[s], dp);
+        for (int j = 0; j < n_tiles; ++j) {
+            const MLXHIP_LDS char* kt = smem + (j & 1) * 2 * T::BYTES;
+            const MLXHIP_LDS char* vt = kt + T::BYTES;
+            MLXHIP_LDS char* other = smem + ((j + 1) & 1) * 2 * T::BYTES;
+            gemm16::wait_vmcnt<0>();
+            gemm16::lds_barrier();
+            if (j + 1 < n_tiles) {
+                issue(a.k, other, j + 1);
+                issue(a.v, other + T::BYTES, j + 1);
             }
-            float e[16];
+            if (wrow >= rows) continue;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], a.c, -lse2)) * (dp[r] - delta);
-            if (__ballot(k0 + 31 > wave_first || !live)) {
+            for (int b = 0; b < KB; ++b) {
+                const int k0 = j * BN + 32 * b;
+                if (k0 > wave_last) break;
+                f32x16 sc = {}, dp = {};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    mma<DT>(rf.read(kt, 32 * b, s), q[s], sc);
+                    mma<DT>(rf.read(vt, 32 * b, s), g[s], dp);
+                }
+                float e[16];
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (k0 + 8 * (r / 4) + 4 * h + r % 4 > lim) e[r] = 0.0f;
+                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], a.c, -lse2)) * (dp[r] - delta);
+                if (__ballot(k0 + 31 > wave_first || !live)) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (k0 + 8 * (r / 4) + 4 * h + r % 4 > lim) e[r] = 0.0f;
+                }
+                if constexpr (KIND == ROW_SUM) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum += e[r];
+                } else {
+                    column.fit(e, dq);
+                    const Frag<DT> ds[2] = {frag_of<DT>(e), frag_of<DT>(e + 8)};
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            const Frag<DT> kc = cf.read(kt, 32 * b + 16 * s, d);
+                            if constexpr (KIND == FINE) mma<DT>(kc, rest_of<DT>(e + 8 * s, ds[s]), dq[d]);
+                            mma<DT>(kc, ds[s], dq[d]);
+                        }
+                    }
+                }
             }
-            column.fit(e, dq);
-            const Frag<DT> ds[2] = {frag_of<DT>(e), frag_of<DT>(e + 8)};
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) mma<DT>(cf.read(kt, 32 * b + 16 * s, d), ds[s], dq[d]);
         }
+    };
+    if (DT != MLXHIP_DTYPE_F32 && last_key(row0 + BM - 1) < FINE_KEYS) {
+        walk(std::integral_constant<int, ROW_SUM>{});
+        sum += __shfl_xor(sum, 32, 64);
+        delta += sum * __builtin_amdgcn_exp2f(-P_SHIFT<DT>);
+        gemm16::lds_barrier();  // the first tiles are loaded again
+        walk(std::integral_constant<int, DT == MLXHIP_DTYPE_F32 ? PLAIN : FINE>{});
+    } else {
+        walk(std::integral_constant<int, PLAIN>{});
+    }
+    if (live && h == 0) {
+        a.lse2[(int64_t)head * a.tokens + token] = lse2;
+        a.delta[(int64_t)head * a.tokens + token] = delta;
     }
     if (live)
         store_row<DT, DB>((E*)a.dq + token * a.q_stride + (int64_t)head * a.dim, dq, h, a.dim,
                           a.scale / column.by * __builtin_amdgcn_exp2f(-P_SHIFT<DT>));
 }
 
-// 64 floats from `first` of p (records: as many bytes as there are) to LDS, lane i the i-th.
-__device__ inline void lds_load4(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* dst, uint32_t voff) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
-    asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
-}
-
-// dK and dV of a tile of keys, 32 to a wave, over share blockIdx.y of the group's
-// heads: the keys' K and V in registers, tiles of a head's Q and dO in LDS with the
-// rows' lse and delta.
+// dK and dV of a tile of keys over share blockIdx.y of the group's heads: a wave's 32 keys'
+// K and V in registers, tiles of a head's Q and dO in LDS with the rows' lse and
+// delta. GROUPS groups of four waves have the same keys, every other tile each, and join at the
+// end: a causal sequence's first keys are seen by all its rows, and the longest such walk
+// is what the kernel waits for.
 template <int DT, int DP>
-__global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS), amdgpu_waves_per_eu(1, 2)))
+constexpr int DKDV_GROUPS = DT == MLXHIP_DTYPE_F32 && DP == 128 ? 1 : 2;  // f32 of 128: over 256 registers
+
+template <int DT, int DP>
+__global__ __attribute__((amdgpu_flat_work_group_size(THREADS * DKDV_GROUPS<DT, DP>, THREADS * DKDV_GROUPS<DT, DP>),
+                          amdgpu_waves_per_eu(DKDV_GROUPS<DT, DP>, DKDV_GROUPS<DT, DP>)))
 void attn_dkdv_kernel(BwdArgs a) {
-    constexpr int BR = DT == MLXHIP_DTYPE_F32 ? 32 : 64, EB = ELEM<DT>;
+    constexpr int GROUPS = DKDV_GROUPS<DT, DP>, BR = DT == MLXHIP_DTYPE_F32 ? 32 : 64, EB = ELEM<DT>;
     constexpr int RB = BR / 32, KS = DP / 16, DB = DP / 32;
     using T = Tile<DT, DP, BR>;
-    constexpr int STATS = 256, STAGE = 2 * T::BYTES + 2 * STATS;
-    __shared__ __attribute__((aligned(1024))) char smem_raw[2 * STAGE];
-    MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw;
+    constexpr int STATS = 256, STAGE = 2 * T::BYTES + 2 * STATS, JOIN = GROUPS > 1 ? THREADS * 2 * DB * 16 * 4 : 0;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[GROUPS * 2 * STAGE > JOIN ? GROUPS * 2 * STAGE : JOIN];
     typedef typename dev::Elem<DT>::type E;
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((tid >> 6) % WAVES), part = __builtin_amdgcn_readfirstlane((tid >> 6) / WAVES);
+    MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw + part * 2 * STAGE;
     const int lin = blockIdx.x;
     const bool per8 = (a.kv_heads & 7) == 0;
     const int item = per8 ? (lin >> 3) % a.key_items : lin / a.kv_heads;
@@ -230,6 +253,7 @@ void attn_dkdv_kernel(BwdArgs a) {
     const int n = at.tokens, tile0 = at.tile * KEY_TILE;
     const int g0 = (int)((int64_t)a.group * blockIdx.y / a.shares), g1 = (int)((int64_t)a.group * (blockIdx.y + 1) / a.shares);
     const int first = a.causal ? tile0 / BR : 0, per = (n + BR - 1) / BR - first, steps = (g1 - g0) * per;
+    const int fine_rows = a.causal ? FINE_KEYS : n <= FINE_KEYS ? n : 0;
 
     const int wkey = tile0 + 32 * wave, key = wkey + (lane & 31);
     const bool live = key < n;
@@ -243,20 +267,15 @@ void attn_dkdv_kernel(BwdArgs a) {
         for (int i = 0; i < (int)(sizeof(kf[s]) / 16); ++i) kf[s].q[i] ^= a.flip;
     }
 
-    TileLoader<DT, DP, BR, WAVES, false> lq, lo;
+    TileLoader<DT, DP, BR, WAVES> lq, lo;
     const uint32_t q_bytes = (uint32_t)(a.q_stride * EB), o_bytes = (uint32_t)(a.o_stride * EB);
     lq.init(wave, lane, a.dim, q_bytes);
     lo.init(wave, lane, a.dim, o_bytes);
     const auto issue = [&](int i, MLXHIP_LDS char* stage) {
         const int head = kvh * a.group + g0 + i / per, j = first + i % per, left = min(n - j * BR, BR);
         const int64_t token = at.first + (int64_t)j * BR;
-        const auto rq = buffer((const char*)a.q + (token * a.q_stride + (int64_t)head * a.dim) * EB, (uint32_t)left * q_bytes);
-        const auto ro = buffer((const char*)a.dout + (token * a.o_stride + (int64_t)head * a.dim) * EB, (uint32_t)left * o_bytes);
-#pragma unroll
-        for (int x = 0; x < lq.L; ++x) {
-            gemm16::lds_load16(rq, stage + (x * WAVES + wave) * 1024, lq.voff[x]);
-            gemm16::lds_load16(ro, stage + T::BYTES + (x * WAVES + wave) * 1024, lo.voff[x]);
-        }
+        lq.rows((const char*)a.q + (token * a.q_stride + (int64_t)head * a.dim) * EB, left, q_bytes, stage, wave);
+        lo.rows((const char*)a.dout + (token * a.o_stride + (int64_t)head * a.dim) * EB, left, o_bytes, stage + T::BYTES, wave);
         if (wave < 2) {
             const float* p = (wave ? a.delta : a.lse2) + (int64_t)head * a.tokens + token;
             lds_load4(buffer(p, (uint32_t)left * 4), stage + 2 * T::BYTES + wave * STATS, (uint32_t)lane * 4);
@@ -269,20 +288,22 @@ void attn_dkdv_kernel(BwdArgs a) {
     cf.init(lane);
     f32x16 dk[DB] = {}, dv[DB] = {};
     Column<DT> column;
-    if (steps > 0) issue(0, smem);
-    for (int i = 0; i < steps; ++i) {
-        const MLXHIP_LDS char* qt = smem + (i & 1) * STAGE;
+    if (part < steps) issue(part, smem);
+    for (int at_step = 0; at_step < steps; at_step += GROUPS) {  // all waves as often: they share the barrier
+        const int i = at_step + part, odd = at_step / GROUPS & 1;
+        const MLXHIP_LDS char* qt = smem + odd * STAGE;
         const MLXHIP_LDS char* gt = qt + T::BYTES;
         const MLXHIP_LDS float* stats = (const MLXHIP_LDS float*)(qt + 2 * T::BYTES);
         gemm16::wait_vmcnt<0>();
         gemm16::lds_barrier();
-        if (i + 1 < steps) issue(i + 1, smem + ((i + 1) & 1) * STAGE);
-        if (wkey >= n) continue;
+        if (i + GROUPS < steps) issue(i + GROUPS, smem + (odd ^ 1) * STAGE);
+        if (wkey >= n || i >= steps) continue;
         const int j = first + i % per;
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
+        const int b0 = a.causal && j * BR + 31 < wkey ? min((wkey - j * BR) / 32, RB) : 0, b1 = min(RB, (n - j * BR + 31) / 32);
+#pragma unroll 1
+        for (int b = b0; b < b1; ++b) {  // blocks of 32 rows that see any of the keys
             const int r0 = j * BR + 32 * b;
-            if (r0 >= n || (a.causal && r0 + 31 < wkey)) continue;
+            asm volatile("" : "+v"(rf.key), "+v"(cf.key));  // addresses formed here: kept, they take registers
             f32x16 sc = {}, dp = {};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -305,19 +326,58 @@ void attn_dkdv_kernel(BwdArgs a) {
                 for (int r = 0; r < 16; ++r)
                     if (r0 + 8 * (r / 4) + 4 * h + r % 4 < key) p[r] = e[r] = 0.0f;
             }
+            // dV, then dK: what one needs is gone before the other's is made.
+            const bool fine = DT != MLXHIP_DTYPE_F32 && r0 < fine_rows;
+            const auto product = [&](const float (&x)[16], const MLXHIP_LDS char* tile, f32x16 (&acc)[DB]) {
+                const Frag<DT> f[2] = {frag_of<DT>(x), frag_of<DT>(x + 8)};
+                if constexpr (DT != MLXHIP_DTYPE_F32) {
+                    if (fine) {
+                        const Frag<DT> rest[2] = {rest_of<DT>(x, f[0]), rest_of<DT>(x + 8, f[1])};
+#pragma unroll
+                        for (int d = 0; d < DB; ++d)
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) mma<DT>(cf.read(tile, 32 * b + 16 * s, d), rest[s], acc[d]);
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) mma<DT>(cf.read(tile, 32 * b + 16 * s, d), f[s], acc[d]);
+            };
+            __builtin_amdgcn_sched_barrier(0);
+            product(p, gt, dv);
+            __builtin_amdgcn_sched_barrier(0);
             column.fit(e, dk);
-            const Frag<DT> pf[2] = {frag_of<DT>(p), frag_of<DT>(p + 8)}, ds[2] = {frag_of<DT>(e), frag_of<DT>(e + 8)};
+            product(e, qt, dk);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    const float unshift = __builtin_amdgcn_exp2f(-P_SHIFT<DT>);
+    float fk = a.scale / column.by * unshift;
+    if constexpr (GROUPS > 1) {
+        __syncthreads();
+        float* sums = reinterpret_cast<float*>(smem_raw) + (tid & (THREADS - 1));
+        if (part == 1) {
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    mma<DT>(cf.read(gt, 32 * b + 16 * s, d), pf[s], dv[d]);
-                    mma<DT>(cf.read(qt, 32 * b + 16 * s, d), ds[s], dk[d]);
+                for (int r = 0; r < 16; ++r) {
+                    sums[(d * 16 + r) * THREADS] = dk[d][r] * fk;
+                    sums[((DB + d) * 16 + r) * THREADS] = dv[d][r];
                 }
         }
+        __syncthreads();
+        if (part == 1) return;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dk[d][r] = dk[d][r] * fk + sums[(d * 16 + r) * THREADS];
+                dv[d][r] += sums[((DB + d) * 16 + r) * THREADS];
+            }
+        fk = 1.0f;
     }
     if (!live) return;
-    const float unshift = __builtin_amdgcn_exp2f(-P_SHIFT<DT>), fk = a.scale / column.by * unshift;
     if (a.shares > 1) {
         const int64_t each = (int64_t)a.tokens * a.kv_heads * a.dim;
         float* to = a.part + 2 * each * blockIdx.y + ((int64_t)(at.first + key) * a.kv_heads + kvh) * a.dim;
@@ -354,19 +414,15 @@ __global__ __launch_bounds__(THREADS) void attn_dkdv_join_kernel(BwdArgs a) {
 
 template <int DT, int DP>
 int launch_bwd(const BwdArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL(attn_stats_kernel<DT>, dim3((unsigned)ceil_div((int64_t)a.tokens * a.heads, THREADS / 16)), dim3(THREADS),
-                       0, s, a);
-    MLXHIP_TRY(launch_check("attn_stats_kernel"));
-    hipLaunchKernelGGL((attn_dkdv_kernel<DT, DP>), dim3((unsigned)(a.key_items * a.kv_heads), (unsigned)a.shares), dim3(THREADS),
-                       0, s, a);
-    MLXHIP_TRY(launch_check("attn_dkdv_kernel"));
-    if (a.shares > 1) {
-        hipLaunchKernelGGL(attn_dkdv_join_kernel<DT>, dim3((unsigned)ceil_div((int64_t)a.tokens * a.kv_heads * a.dim / 4, THREADS)),
-                           dim3(THREADS), 0, s, a);
-        MLXHIP_TRY(launch_check("attn_dkdv_join_kernel"));
-    }
     hipLaunchKernelGGL((attn_dq_kernel<DT, DP>), dim3((unsigned)(a.row_items * a.kv_heads)), dim3(THREADS), 0, s, a);
-    return launch_check("attn_dq_kernel");
+    MLXHIP_TRY(launch_check("attn_dq_kernel"));
+    hipLaunchKernelGGL((attn_dkdv_kernel<DT, DP>), dim3((unsigned)(a.key_items * a.kv_heads), (unsigned)a.shares),
+                       dim3(THREADS * DKDV_GROUPS<DT, DP>), 0, s, a);
+    MLXHIP_TRY(launch_check("attn_dkdv_kernel"));
+    if (a.shares == 1) return MLXHIP_OK;
+    hipLaunchKernelGGL(attn_dkdv_join_kernel<DT>, dim3((unsigned)ceil_div((int64_t)a.tokens * a.kv_heads * a.dim / 4, THREADS)),
+                       dim3(THREADS), 0, s, a);
+    return launch_check("attn_dkdv_join_kernel");
 }
 
 template <int DT>
