@@ -123,54 +123,62 @@ struct Tile {
 };
 
 // p and bytes are the same in all lanes; arithmetic on them may have gone through
-// vector registers, the descriptor is scalar.
+// vector registers, the descriptor is scalar. A scalar register that the vector unit
+// writes takes five cycles to reach a memory instruction: the compiler counts them for its own
+// instructions only, and the asm loads below would go by the old descriptor.
 __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
     const uint64_t at = (uint64_t)(uintptr_t)p;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)hi << 32 | lo), 0,
-                                             __builtin_amdgcn_readfirstlane(bytes), gemm16::BUF_FLAGS);
+    __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)hi << 32 | lo), 0,
+                                                                 __builtin_amdgcn_readfirstlane(bytes), gemm16::BUF_FLAGS);
+    asm volatile("s_nop 4" : "+s"(r));
+    return r;
 }
 
-// lds_load16 and its 4-byte form (lane i to dst + 4 i), behind the five cycles that a scalar
-// register written by the vector unit (as the descriptor's parts may be, see buffer)
-// takes to reach a memory instruction: the compiler counts them for its own
-// instructions only, and an asm block that follows too soon loads by the old descriptor.
+// 16 or 4 bytes per lane from buffer offset voff to LDS at dst + 16 or 4 * lane (M0's wait in front).
 __device__ inline void lds_load16(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* dst, uint32_t voff) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
-    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
 }
 __device__ inline void lds_load4(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* dst, uint32_t voff) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
-    asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
+    asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
 }
 
 // One wave's loads of a tile: LW waves share its instructions, wave w takes
-// w, w + LW, ...; instruction i from the row where it starts. voff: the lane's offset there,
-// past any buffer where the chunk is past the head. The swizzle comes round after 16
-// rows, so that a few offsets serve all.
-template <int DT, int DP, int ROWS, int LW>
+// w, w + LW, ... voff: the lane's offset, past any buffer where the chunk is past the head.
+// WHOLE: from the first row of the tile, one descriptor for all and an offset for each instruction;
+// else from the first row of 16 (which lie in one page), a descriptor for each 16 rows and as many
+// offsets as such rows take instructions.
+template <int DT, int DP, int ROWS, int LW, bool WHOLE>
 struct TileLoader {
     using T = Tile<DT, DP, ROWS>;
     static constexpr int L = T::INSTR / LW, STEP = LW * T::RPI;  // instructions of a wave, rows from one to the next
-    static constexpr int ROUND = STEP >= 16 ? 1 : L < 16 / STEP ? L : 16 / STEP;
+    static constexpr int PER16 = STEP >= 16 ? 1 : 16 / STEP, ROUND = WHOLE ? L : PER16;
     static_assert(L * LW == T::INSTR && (16 % STEP == 0 || STEP % 16 == 0), "whole instructions to a wave");
     uint32_t voff[ROUND];
     __device__ inline void init(int wave, int lane, int dim, uint32_t stride_bytes) {
-        const int r = lane / T::CPR, slot = lane % T::CPR;
 #pragma unroll
         for (int i = 0; i < ROUND; ++i) {
-            const int c = slot ^ T::swizzle((i * LW + wave) * T::RPI + r);
-            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)r * stride_bytes + c * 16 : gemm16::OOB;
+            const int row = (i * LW + wave) * T::RPI + lane / T::CPR, c = lane % T::CPR ^ T::swizzle(row);
+            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(WHOLE ? row : row % 16) * stride_bytes + c * 16 : gemm16::OOB;
         }
     }
-    // `left` rows (1 or more) from p on, stride_bytes apart, to the tile; zeros behind them.
-    __device__ inline void rows(const char* p, int left, uint32_t stride_bytes, MLXHIP_LDS char* tile, int wave) const {
+    // All loads; rows_at(r): the buffer of rows r .. r + 15 of the tile (WHOLE: of all, r = 0).
+    template <class F>
+    __device__ inline void load(MLXHIP_LDS char* tile, int wave, F&& rows_at) const {
+        __amdgpu_buffer_rsrc_t rsrc;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int row = (i * LW + wave) * T::RPI;
-            lds_load16(buffer(p + (int64_t)row * stride_bytes, (uint32_t)max(0, min(left - row, T::RPI)) * stride_bytes),
-                       tile + (i * LW + wave) * 1024, voff[i % ROUND]);
+            if (WHOLE ? i == 0 : i % PER16 == 0) rsrc = rows_at(WHOLE ? 0 : (i * LW + wave) * T::RPI & ~15);
+            lds_load16(rsrc, tile + (i * LW + wave) * 1024, voff[i % ROUND]);
         }
+    }
+    // `left` rows (1 or more) from p on, stride_bytes apart; zeros behind them.
+    __device__ inline void rows(const char* p, int left, uint32_t stride_bytes, MLXHIP_LDS char* tile, int wave) const {
+        load(tile, wave, [&](int r) {
+            return buffer(p + (int64_t)r * stride_bytes, (uint32_t)max(0, min(left - r, WHOLE ? ROWS : 16)) * stride_bytes);
+        });
     }
 };
 
@@ -246,12 +254,29 @@ __device__ inline Frag<DT> load_frag(const typename dev::Elem<DT>::type* row, in
     return f;
 }
 
-// The sequence and the tile in it that work item `item` names: the sequences' rows
-// (tokens times per_token) in tiles of `rows`, one after another. starts is the
-// caller's: what it says is brought into [0, tokens], a sequence that ends before it
-// starts has no rows. 64 sequences at a time, a wave together; false past the last tile.
+// Keeps what follows in a branch of its own: made into selects, work for the few tiles that a
+// mask cuts would be done for all.
+__device__ inline void own_branch() { asm volatile(""); }
+
+// Sum over a wave, the same in all lanes: row shifts and broadcasts, no LDS.
+__device__ inline int wave_total(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // within rows of 16 lanes: by 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // a row's last lane to the next row
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the first half's to the second
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The sequence and the tile in it that work item `item` names, of the sequences' rows
+// (tokens times per_token) in tiles of `rows`. Items go down by the number of the tile, 1 for each
+// sequence's shortest walk under a causal mask: the longest walks of all sequences come first, so
+// that none is left to run alone at the end (64 sequences at a time, then the
+// next 64). starts is the caller's: what it says is brought into [0, tokens], a sequence that ends
+// before it starts has no rows. A wave together; false past the last tile.
 struct Place {
-    int seq, first, tokens, tile, tiles;
+    int seq, first, tokens, level, tiles;  // level: 1 .. tiles
 };
 __device__ inline bool find_tile(const int32_t* __restrict__ starts, int n_seqs, int tokens, int per_token, int rows,
                                  int item, Place* out) {
@@ -264,23 +289,57 @@ __device__ inline bool find_tile(const int32_t* __restrict__ starts, int n_seqs,
             n = max(min(max(starts[i + 1], 0), tokens) - first, 0);
         }
         const int tiles = (int)(((int64_t)n * per_token + rows - 1) / rows);
-        int sum = tiles;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += up;
+        const int all = n_seqs == 1 ? __builtin_amdgcn_readfirstlane(tiles) : wave_total(tiles);
+        if (item >= all) {
+            item -= all;
+            continue;
         }
-        const uint64_t past = __ballot(sum > item);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            out->seq = base + at;
-            out->first = __builtin_amdgcn_readlane(first, at);
-            out->tokens = __builtin_amdgcn_readlane(n, at);
-            out->tiles = __builtin_amdgcn_readlane(tiles, at);
-            out->tile = item - (__builtin_amdgcn_readlane(sum, at) - out->tiles);
-            return true;
+        // The highest level that more than `item` tiles reach: those from it on.
+        int lo = 1, over = 0;
+        if (n_seqs == 1) {
+            lo = all - item;
+            over = item;
+        } else {
+            for (int hi = all + 1; hi - lo > 1;) {  // above(lo) > item >= above(hi)
+                const int mid = lo + (hi - lo) / 2, above = wave_total(max(0, tiles - mid + 1));
+                if (above > item) {
+                    lo = mid;
+                } else {
+                    hi = mid;
+                    over = above;
+                }
+            }
         }
-        item -= __builtin_amdgcn_readlane(sum, 63);
+        uint64_t reach = __ballot(tiles >= lo);
+        for (int k = item - over; k > 0; --k) reach &= reach - 1;
+        const int at = __builtin_ctzll(reach);
+        out->seq = base + at;
+        out->first = __builtin_amdgcn_readlane(first, at);
+        out->tokens = __builtin_amdgcn_readlane(n, at);
+        out->tiles = __builtin_amdgcn_readlane(tiles, at);
+        out->level = lo;
+        return true;
+    }
+    return false;
+}
+
+// The sequence that a token lies in (first and tokens of it), a wave together.
+__device__ inline bool find_token(const int32_t* __restrict__ starts, int n_seqs, int tokens, int token, Place* out) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < n_seqs; base += 64) {
+        const int i = base + lane;
+        int first = 0, n = 0;
+        if (i < n_seqs) {
+            first = min(max(starts[i], 0), tokens);
+            n = max(min(max(starts[i + 1], 0), tokens) - first, 0);
+        }
+        const uint64_t in = __ballot(token >= first && token - first < n);
+        if (!in) continue;
+        const int at = __builtin_ctzll(in);
+        out->seq = base + at;
+        out->first = __builtin_amdgcn_readlane(first, at);
+        out->tokens = __builtin_amdgcn_readlane(n, at);
+        return true;
     }
     return false;
 }

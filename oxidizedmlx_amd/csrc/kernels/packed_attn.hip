@@ -62,7 +62,7 @@ int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v,
     a.key_items = items_of(tokens, 1, n_seqs, attn::KEY_TILE);
     // Few tiles of keys: a group's heads over several workgroups, their sums joined.
     const int64_t wgs = a.key_items * kv_heads;
-    a.shares = (int)std::clamp<int64_t>(256 / std::max<int64_t>(wgs, 1), 1, a.group);
+    a.shares = (int)std::clamp<int64_t>((512 + wgs - 1) / std::max<int64_t>(wgs, 1), 1, a.group);
     const size_t stats = (((size_t)tokens * heads + 63) & ~size_t(63)) * sizeof(float);
     const size_t part = a.shares > 1 ? (size_t)a.shares * 2 * tokens * kv_heads * dim * sizeof(float) : 0;
     void* ws = nullptr;
@@ -84,10 +84,11 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     // Up to 32 rows a sequence on average (single tokens of up to 32 heads to a K/V head, say).
     const bool keys = tokens * a.group <= (int64_t)attn::FEW_ROWS * a.n_seqs;
     a.items = items_of(tokens, a.group, a.n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
-    // The keys over several workgroups until there are 1024 (two rounds of two to a
-    // compute unit, so that sequences of different lengths even out), within 256 MiB of parts.
+    // The keys over several workgroups: few rows until there are 2048 (four rounds of two to a
+    // compute unit, so that sequences of different lengths even out), tiles of rows until
+    // there are 512 (their parts cost more to join); within 256 MiB of parts.
     const int64_t most = pages.table_width << pages.page_shift, wgs = (int64_t)a.items * kv_heads;
-    int64_t splits = std::min<int64_t>({1024 / std::max<int64_t>(wgs, 1), ceil_div(most, attn::MIN_SPAN), 64});
+    int64_t splits = std::min<int64_t>({(keys ? 2048 : 512) / std::max<int64_t>(wgs, 1), ceil_div(most, attn::MIN_SPAN), 64});
     const int64_t row = tokens * heads * (dim + 2) * (int64_t)sizeof(float);
     splits = std::min<int64_t>(splits, (int64_t(256) << 20) / std::max<int64_t>(row, 1));
     a.splits = (int)std::max<int64_t>(splits, 1);

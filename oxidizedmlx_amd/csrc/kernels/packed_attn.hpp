@@ -26,7 +26,7 @@ int fwd(const FwdArgs& a, bool paged, bool keys, hipStream_t s);
 struct BwdArgs {
     const void *q, *k, *v, *o, *dout;
     const float* lse;        // [tokens][heads]
-    float *lse2, *delta;     // [heads][tokens], dQ's kernel for dK and dV's: lse log2 e less the shift of p, rowsum(dO o O)
+    float *lse2, *delta;     // [heads][tokens], dQ's kernel for dK and dV's: lse log2 e less the shift of p, -rowsum(dO o O)
     float* part;             // [shares][2][tokens][kv_heads][dim] (shares > 1): dK, dV
     void *dq, *dk, *dv;
     const int32_t* starts;

@@ -59,7 +59,7 @@ void attn_fwd_kernel(FwdArgs a) {
     const int kvh = per8 == 8 ? (lin >> 3) / a.items * 8 + (lin & 7) : lin % a.kv_heads;
     Place at;
     if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return;
-    const int row0 = (at.tiles - 1 - at.tile) * BM, rows = at.tokens * a.group;
+    const int row0 = (at.level - 1) * BM, rows = at.tokens * a.group;
     const int length = PAGED ? length_of(a.pages, at.seq) : at.tokens, keys = PAGED ? keys_of(a.pages, length) : length;
     const int shift = length - at.tokens;  // position of the first new token
     const int parts = PAGED ? parts_of(keys, a.splits) : 1, part = PAGED ? blockIdx.y : 0;
@@ -88,7 +88,7 @@ void attn_fwd_kernel(FwdArgs a) {
 
     // Loads: a tile's rows one after another in memory, or page by page (an
     // instruction's rows lie in one page: pages hold a multiple of 16).
-    TileLoader<DT, DP, BN, LW> loader;
+    TileLoader<DT, DP, BN, LW, !PAGED> loader;
     const uint32_t stride_bytes = (uint32_t)((PAGED ? a.dim : a.kv_stride) * EB);
     loader.init(KEYS ? 0 : wave, lane, a.dim, stride_bytes);
     const char* kbase = (const char*)a.k;
@@ -98,28 +98,29 @@ void attn_fwd_kernel(FwdArgs a) {
         kbase += off;
         vbase += off;
     }
-    // Page numbers of the tile's instructions, one to a lane, read a tile ahead.
+    // Page numbers of 64 pages, one to a lane, read anew where the tiles reach the next 64. The
+    // wait is there, or the compiler would wait at every use for all loads under way.
     const int32_t* table = PAGED ? a.pages.table + (int64_t)at.seq * a.pages.table_width : nullptr;
-    const auto pages_of = [&](int j) {
-        int page = -1;
+    int window = -64, numbers = -1;
+    const auto turn_to = [&](int j) {
         if constexpr (PAGED) {
-            const int r = j * BN + (lane * LW + (KEYS ? 0 : wave)) * T::RPI;
-            if (lane < loader.L && r < keys) page = table[r >> a.pages.page_shift];
+            const int first = (j * BN >> a.pages.page_shift) & ~63;
+            if (first == window) return;
+            window = first;
+            numbers = (int64_t)first + lane < a.pages.table_width ? table[first + lane] : -1;
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
         }
-        return page;
     };
-    const auto issue = [&](const char* base, MLXHIP_LDS char* tile, int j, int pages) {
+    const auto issue = [&](const char* base, MLXHIP_LDS char* tile, int j) {
         if constexpr (PAGED) {
-#pragma unroll
-            for (int i = 0; i < loader.L; ++i) {
-                const int qi = i * LW + (KEYS ? 0 : wave), r = j * BN + qi * T::RPI;
-                const int left = min(keys - r, T::RPI), page = __builtin_amdgcn_readlane(pages, i);
-                const bool ok = page >= 0 && page < a.pages.pages;
+            loader.load(tile, KEYS ? 0 : wave, [&](int from) {
+                const int r = j * BN + from, left = min(keys - r, 16);
+                const int page = __builtin_amdgcn_readlane(numbers, (r >> a.pages.page_shift) & 63);
+                const bool ok = left > 0 && page >= 0 && page < a.pages.pages;
                 const int64_t at_row = (((int64_t)(ok ? page : 0) * a.kv_heads + kvh) << a.pages.page_shift) +
                                        (r & ((1 << a.pages.page_shift) - 1));
-                lds_load16(buffer(base + at_row * stride_bytes, ok ? (uint32_t)left * stride_bytes : 0u),
-                                   tile + qi * 1024, loader.voff[i % loader.ROUND]);
-            }
+                return buffer(base + at_row * stride_bytes, ok ? (uint32_t)left * stride_bytes : 0u);
+            });
         } else {
             loader.rows(base + (int64_t)j * BN * stride_bytes, keys - j * BN, stride_bytes, tile, KEYS ? 0 : wave);
         }
@@ -132,8 +133,9 @@ void attn_fwd_kernel(FwdArgs a) {
     f32x16 o[DB] = {};
     float m = -INFINITY, l = 0.0f;
 
-    // One tile of keys from k0 on. after_scores: what may start once K has been read.
-    const auto compute = [&](auto careful, const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int k0, auto&& after_scores) {
+    // One tile of keys from k0 on. after_scores: what may start once K has been read; before_v: what V waits for.
+    const auto compute = [&](auto careful, const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int k0, auto&& after_scores,
+                             auto&& before_v) {
         f32x16 sc[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
@@ -145,6 +147,7 @@ void attn_fwd_kernel(FwdArgs a) {
         const bool masked = k0 + BN - 1 > wave_first || !live;
         const bool any_masked = __ballot(masked) != 0;
         if (any_masked) {
+            own_branch();
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -178,6 +181,7 @@ void attn_fwd_kernel(FwdArgs a) {
             p[2 * b] = frag_of<DT>(e);
             p[2 * b + 1] = frag_of<DT>(e + 8);
         }
+        before_v();
         if (decltype(careful)::value && any_masked) {
             // p = 0 of a masked key would make NaN of a non-finite v: those are taken out of the
             // product, and what is counted of them among the keys that a row sees makes it NaN.
@@ -212,42 +216,53 @@ void attn_fwd_kernel(FwdArgs a) {
     const auto walk = [&](auto careful) {
 
         if constexpr (KEYS) {
+            // K of the next tile loads during this one's softmax and second product, V during
+            // the next one's first; a wait leaves the newest loads under way.
             MLXHIP_LDS char* kt = smem;
             MLXHIP_LDS char* vt = smem + T::BYTES;
-            int j = t0 + wave, pages = pages_of(j), next = pages_of(j + WAVES);
+            constexpr int L = decltype(loader)::L;
+            int j = t0 + wave;
             if (j < t1) {
-                issue(kbase, kt, j, pages);
-                issue(vbase, vt, j, pages);
+                turn_to(j);
+                issue(kbase, kt, j);
+                issue(vbase, vt, j);
             }
             for (; j < t1; j += WAVES) {
-                gemm16::wait_vmcnt<0>();
-                const int then = pages_of(j + 2 * WAVES);
-                compute(careful, kt, vt, j * BN, [&] {  // K has been read
-                    __builtin_amdgcn_s_waitcnt(0xC07F);
-                    if (j + WAVES < t1) issue(kbase, kt, j + WAVES, next);
-                });
+                const bool more = j + WAVES < t1;
+                gemm16::wait_vmcnt<L>();
+                compute(
+                    careful, kt, vt, j * BN,
+                    [&] {
+                        __builtin_amdgcn_s_waitcnt(0xC07F);
+                        if (more) {
+                            turn_to(j + WAVES);
+                            issue(kbase, kt, j + WAVES);
+                        }
+                    },
+                    [&] {
+                        if (more) gemm16::wait_vmcnt<L>();
+                        else gemm16::wait_vmcnt<0>();
+                    });
                 __builtin_amdgcn_s_waitcnt(0xC07F);
-                if (j + WAVES < t1) issue(vbase, vt, j + WAVES, next);
-                next = then;
+                if (more) issue(vbase, vt, j + WAVES);
             }
         } else {
-            int pages = pages_of(t0);
             if (t0 < t1) {
-                issue(kbase, smem, t0, pages);
-                issue(vbase, smem + T::BYTES, t0, pages);
+                turn_to(t0);
+                issue(kbase, smem, t0);
+                issue(vbase, smem + T::BYTES, t0);
             }
-            pages = pages_of(t0 + 1);
             for (int j = t0; j < t1; ++j) {
                 MLXHIP_LDS char* tile = smem + ((j - t0) & 1) * 2 * T::BYTES;
                 MLXHIP_LDS char* other = smem + ((j - t0 + 1) & 1) * 2 * T::BYTES;
                 gemm16::wait_vmcnt<0>();
                 gemm16::lds_barrier();
                 if (j + 1 < t1) {
-                    issue(kbase, other, j + 1, pages);
-                    issue(vbase, other + T::BYTES, j + 1, pages);
-                    pages = pages_of(j + 2);
+                    turn_to(j + 1);
+                    issue(kbase, other, j + 1);
+                    issue(vbase, other + T::BYTES, j + 1);
                 }
-                if (wrow < rows && j * BN <= wave_last) compute(careful, tile, tile + T::BYTES, j * BN, [] {});
+                if (wrow < rows && j * BN <= wave_last) compute(careful, tile, tile + T::BYTES, j * BN, [] {}, [] {});
             }
         }
     };
@@ -266,6 +281,7 @@ void attn_fwd_kernel(FwdArgs a) {
         kf.init(again);
         vf.init(again);
         loader.init(KEYS ? 0 : wave, again, a.dim, stride_bytes);
+        window = -64;
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = f32x16{};
         m = -INFINITY;
@@ -372,23 +388,34 @@ void attn_fwd_kernel(FwdArgs a) {
         }
 }
 
-// The parts of a row joined: a wave to a row of a token's head.
+// The parts of a row of a token's head joined, a workgroup to a row: eight groups of 32
+// threads, four values each, take every eighth part (up to 64: all loads at once), then join in order.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a) {
-    const int64_t row = (int64_t)blockIdx.x * WAVES + threadIdx.x / 64;
-    const int lane = threadIdx.x & 63;
-    if (row >= (int64_t)a.tokens * a.heads) return;
+    __shared__ f32x4 sums[8][32];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63, t = threadIdx.x % 32, g = threadIdx.x / 32;
     const int token = (int)(row / a.heads), head = (int)(row - (int64_t)token * a.heads);
     Place at;
-    // Of a sequence's tokens each is a tile: `item` counts the sequences' tokens.
-    const int first = max(a.starts[0], 0);
-    if (token < first || !find_tile(a.starts, a.n_seqs, a.tokens, 1, 1, token - first, &at) || at.first + at.tile != token) return;
+    if (!find_token(a.starts, a.n_seqs, a.tokens, token, &at)) return;
     const int length = length_of(a.pages, at.seq), parts = parts_of(keys_of(a.pages, length), a.splits);
     if (parts == 1) return;
     const int64_t step = (int64_t)a.tokens * a.heads * (a.dim + 2);
     const float* p = a.part + row * (a.dim + 2);
-    float m = -INFINITY;
-    if (lane < parts) m = p[lane * step + a.dim];
+    float m = -INFINITY, l = 0.0f;
+    if (lane < parts) {
+        m = p[lane * step + a.dim];
+        l = p[lane * step + a.dim + 1];
+    }
+    f32x4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (g + 8 * i < parts && 4 * t < a.dim) {
+            // Rows of dim + 2 values: pairs are aligned, quads are not.
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            const f32x2* q = reinterpret_cast<const f32x2*>(p + (g + 8 * i) * step + 4 * t);
+            x[i] = f32x4{q[0][0], q[0][1], q[1][0], q[1][1]};
+        }
     float top = m;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -396,29 +423,26 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a) {
         top = other > top || other != other ? other : top;
     }
     const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    float l = w == 0.0f ? 0.0f : w * p[lane * step + a.dim + 1];
+    l = w == 0.0f ? 0.0f : w * l;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-    const bool none = at.tile + length - at.tokens < 0;
-    typedef typename dev::Elem<DT>::type E;
-    E* to = (E*)a.o + (int64_t)token * a.o_stride + (int64_t)head * a.dim;
-    for (int d = 2 * lane; d < a.dim; d += 128) {
-        float x = 0.0f, y = 0.0f;
-        for (int i = 0; i < parts; ++i) {
-            const float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i));
-            if (wi == 0.0f) continue;
-            x += wi * p[i * step + d];
-            y += wi * p[i * step + d + 1];
-        }
-        x = none ? 0.0f : x / l;
-        y = none ? 0.0f : y / l;
-        if constexpr (DT == MLXHIP_DTYPE_F32) {
-            to[d] = x;
-            to[d + 1] = y;
-        } else {
-            *reinterpret_cast<uint32_t*>(to + d) = gemm16::pack2<DT>(x, y);
-        }
+    f32x4 sum = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl(w, g + 8 * i, 64);
+        if (g + 8 * i < parts && wi != 0.0f && 4 * t < a.dim) sum += wi * x[i];
     }
+    sums[g][t] = sum;
+    __syncthreads();
+    if (g != 0 || 4 * t >= a.dim) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += sums[i][t];
+    const bool none = token - at.first + length - at.tokens < 0;
+    sum = none ? f32x4{} : sum / l;
+    typedef typename dev::Elem<DT>::type E;
+    E* to = (E*)a.o + (int64_t)token * a.o_stride + (int64_t)head * a.dim + 4 * t;
+    if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = sum;
+    else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(sum[0], sum[1]), gemm16::pack2<DT>(sum[2], sum[3])};
 }
 
 template <int DT, int DP, bool PAGED, bool KEYS>
@@ -427,7 +451,7 @@ int launch_fwd(const FwdArgs& a, hipStream_t s) {
                        dim3(THREADS), 0, s, a);
     MLXHIP_TRY(launch_check("attn_fwd_kernel"));
     if (a.splits == 1) return MLXHIP_OK;
-    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)ceil_div((int64_t)a.tokens * a.heads, WAVES)), dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)(a.tokens * a.heads)), dim3(THREADS), 0, s, a);
     return launch_check("attn_join_kernel");
 }
 

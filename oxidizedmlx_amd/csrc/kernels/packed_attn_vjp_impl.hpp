@@ -93,7 +93,7 @@ void attn_dq_kernel(BwdArgs a) {
     const int kvh = per8 ? (lin >> 3) / a.row_items * 8 + (lin & 7) : lin % a.kv_heads;
     Place at;
     if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return;
-    const int row0 = (at.tiles - 1 - at.tile) * BM, rows = at.tokens * a.group, n = at.tokens;
+    const int row0 = (at.level - 1) * BM, rows = at.tokens * a.group, n = at.tokens;
 
     const int wrow = row0 + 32 * wave, row = wrow + (lane & 31);
     const bool live = row < rows;
@@ -133,7 +133,7 @@ void attn_dq_kernel(BwdArgs a) {
         delta += __shfl_xor(delta, 32, 64);
     }
 
-    TileLoader<DT, DP, BN, WAVES> loader;
+    TileLoader<DT, DP, BN, WAVES, true> loader;
     const uint32_t stride_bytes = (uint32_t)(a.kv_stride * EB);
     loader.init(wave, lane, a.dim, stride_bytes);
     const int64_t off = ((int64_t)at.first * a.kv_stride + (int64_t)kvh * a.dim) * EB;
@@ -181,6 +181,7 @@ void attn_dq_kernel(BwdArgs a) {
                 for (int r = 0; r < 16; ++r)
                     e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], a.c, -lse2)) * (dp[r] - delta);
                 if (__ballot(k0 + 31 > wave_first || !live)) {
+                    own_branch();
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (k0 + 8 * (r / 4) + 4 * h + r % 4 > lim) e[r] = 0.0f;
@@ -215,7 +216,7 @@ void attn_dq_kernel(BwdArgs a) {
     }
     if (live && h == 0) {
         a.lse2[(int64_t)head * a.tokens + token] = lse2;
-        a.delta[(int64_t)head * a.tokens + token] = delta;
+        a.delta[(int64_t)head * a.tokens + token] = -delta;
     }
     if (live)
         store_row<DT, DB>((E*)a.dq + token * a.q_stride + (int64_t)head * a.dim, dq, h, a.dim,
@@ -250,7 +251,7 @@ void attn_dkdv_kernel(BwdArgs a) {
     const int kvh = per8 ? (lin >> 3) / a.key_items * 8 + (lin & 7) : lin % a.kv_heads;
     Place at;
     if (!find_tile(a.starts, a.n_seqs, a.tokens, 1, KEY_TILE, item, &at)) return;
-    const int n = at.tokens, tile0 = at.tile * KEY_TILE;
+    const int n = at.tokens, tile0 = (at.tiles - at.level) * KEY_TILE;
     const int g0 = (int)((int64_t)a.group * blockIdx.y / a.shares), g1 = (int)((int64_t)a.group * (blockIdx.y + 1) / a.shares);
     const int first = a.causal ? tile0 / BR : 0, per = (n + BR - 1) / BR - first, steps = (g1 - g0) * per;
     const int fine_rows = a.causal ? FINE_KEYS : n <= FINE_KEYS ? n : 0;
@@ -267,7 +268,7 @@ void attn_dkdv_kernel(BwdArgs a) {
         for (int i = 0; i < (int)(sizeof(kf[s]) / 16); ++i) kf[s].q[i] ^= a.flip;
     }
 
-    TileLoader<DT, DP, BR, WAVES> lq, lo;
+    TileLoader<DT, DP, BR, WAVES, false> lq, lo;
     const uint32_t q_bytes = (uint32_t)(a.q_stride * EB), o_bytes = (uint32_t)(a.o_stride * EB);
     lq.init(wave, lane, a.dim, q_bytes);
     lo.init(wave, lane, a.dim, o_bytes);
@@ -304,7 +305,13 @@ void attn_dkdv_kernel(BwdArgs a) {
         for (int b = b0; b < b1; ++b) {  // blocks of 32 rows that see any of the keys
             const int r0 = j * BR + 32 * b;
             asm volatile("" : "+v"(rf.key), "+v"(cf.key));  // addresses formed here: kept, they take registers
-            f32x16 sc = {}, dp = {};
+            f32x16 sc = {}, dp;  // dp starts as -delta
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 delta = *(const MLXHIP_LDS f32x4*)(stats + STATS / 4 + 32 * b + 8 * q + 4 * h);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) dp[4 * q + x] = delta[x];
+            }
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 mma<DT>(rf.read(qt, 32 * b, s), kf[s], sc);
@@ -314,14 +321,14 @@ void attn_dkdv_kernel(BwdArgs a) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const f32x4 lse2 = *(const MLXHIP_LDS f32x4*)(stats + 32 * b + 8 * q + 4 * h);
-                const f32x4 delta = *(const MLXHIP_LDS f32x4*)(stats + STATS / 4 + 32 * b + 8 * q + 4 * h);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     p[4 * q + x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[4 * q + x], a.c, -lse2[x]));
-                    e[4 * q + x] = p[4 * q + x] * (dp[4 * q + x] - delta[x]);
+                    e[4 * q + x] = p[4 * q + x] * dp[4 * q + x];
                 }
             }
             if (a.causal && r0 < wkey + 31) {
+                own_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (r0 + 8 * (r / 4) + 4 * h + r % 4 < key) p[r] = e[r] = 0.0f;
