@@ -145,40 +145,55 @@ __device__ inline void lds_load4(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* d
     asm volatile("s_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(m0) : "memory");
 }
 
-// One wave's loads of a tile: LW waves share its instructions, wave w takes
-// w, w + LW, ... voff: the lane's offset, past any buffer where the chunk is past the head.
-// WHOLE: from the first row of the tile, one descriptor for all and an offset for each instruction;
-// else from the first row of 16 (which lie in one page), a descriptor for each 16 rows and as many
-// offsets as such rows take instructions.
-template <int DT, int DP, int ROWS, int LW, bool WHOLE>
+// One wave's loads of a tile that LW waves share. voff: the lane's offset, past any buffer where
+// the chunk is past the head.
+//   TILE   rows one after another in memory, one descriptor: an offset for each instruction, from
+//          the tile's first row.
+//   PAGES  16 rows (which lie in one page) to a descriptor, a wave's instructions side by side, so that
+//          it has one or two: an offset for each instruction of 16 rows, from the first of them.
+//   LEAN   rows one after another, the waves' instructions in turn and a descriptor each: the swizzle
+//          comes round after 16 rows, so that one or two offsets serve all where registers are short.
+enum LoadMode { TILE, PAGES, LEAN };
+template <int DT, int DP, int ROWS, int LW, int MODE>
 struct TileLoader {
     using T = Tile<DT, DP, ROWS>;
-    static constexpr int L = T::INSTR / LW, STEP = LW * T::RPI;  // instructions of a wave, rows from one to the next
-    static constexpr int PER16 = STEP >= 16 ? 1 : 16 / STEP, ROUND = WHOLE ? L : PER16;
+    static constexpr int L = T::INSTR / LW;  // instructions of a wave
+    static constexpr int STEP = (MODE == PAGES ? 1 : LW) * T::RPI, PER16 = STEP >= 16 ? 1 : 16 / STEP;
+    static constexpr int ROUND = MODE == TILE || L < PER16 ? L : PER16;
     static_assert(L * LW == T::INSTR && (16 % STEP == 0 || STEP % 16 == 0), "whole instructions to a wave");
     uint32_t voff[ROUND];
+    __device__ static inline int instr(int wave, int i) { return MODE == PAGES ? wave * L + i : i * LW + wave; }
     __device__ inline void init(int wave, int lane, int dim, uint32_t stride_bytes) {
 #pragma unroll
         for (int i = 0; i < ROUND; ++i) {
-            const int row = (i * LW + wave) * T::RPI + lane / T::CPR, c = lane % T::CPR ^ T::swizzle(row);
-            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(WHOLE ? row : row % 16) * stride_bytes + c * 16 : gemm16::OOB;
+            const int row = instr(wave, i) * T::RPI + lane / T::CPR, c = lane % T::CPR ^ T::swizzle(row);
+            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(MODE == TILE ? row : row % 16) * stride_bytes + c * 16 : gemm16::OOB;
         }
     }
-    // All loads; rows_at(r): the buffer of rows r .. r + 15 of the tile (WHOLE: of all, r = 0).
-    template <class F>
-    __device__ inline void load(MLXHIP_LDS char* tile, int wave, F&& rows_at) const {
+    // TILE, LEAN: `left` rows (1 or more) from p on, stride_bytes apart; zeros behind them.
+    __device__ inline void rows(const char* p, int left, uint32_t stride_bytes, MLXHIP_LDS char* tile, int wave) const {
         __amdgpu_buffer_rsrc_t rsrc;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            if (WHOLE ? i == 0 : i % PER16 == 0) rsrc = rows_at(WHOLE ? 0 : (i * LW + wave) * T::RPI & ~15);
-            lds_load16(rsrc, tile + (i * LW + wave) * 1024, voff[i % ROUND]);
+            const int r = MODE == TILE ? 0 : instr(wave, i) * T::RPI & ~15;
+            if (MODE == TILE ? i == 0 : i % PER16 == 0)
+                rsrc = buffer(p + (int64_t)r * stride_bytes, (uint32_t)max(0, min(left - r, MODE == TILE ? ROWS : 16)) * stride_bytes);
+            lds_load16(rsrc, tile + instr(wave, i) * 1024, voff[i % ROUND]);
         }
     }
-    // `left` rows (1 or more) from p on, stride_bytes apart; zeros behind them.
-    __device__ inline void rows(const char* p, int left, uint32_t stride_bytes, MLXHIP_LDS char* tile, int wave) const {
-        load(tile, wave, [&](int r) {
-            return buffer(p + (int64_t)r * stride_bytes, (uint32_t)max(0, min(left - r, WHOLE ? ROWS : 16)) * stride_bytes);
-        });
+    // PAGES: at(r, &bytes): where rows r .. r + 15 of the tile lie from p on, and how many bytes of them.
+    template <class F>
+    __device__ inline void paged(const char* p, MLXHIP_LDS char* tile, int wave, F&& at) const {
+        __amdgpu_buffer_rsrc_t rsrc;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (i % PER16 == 0) {
+                uint32_t bytes;
+                const int64_t off = at(instr(wave, i) * T::RPI & ~15, &bytes);
+                rsrc = buffer(p + off, bytes);
+            }
+            lds_load16(rsrc, tile + instr(wave, i) * 1024, voff[i % ROUND]);
+        }
     }
 };
 

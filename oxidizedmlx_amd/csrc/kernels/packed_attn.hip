@@ -89,7 +89,7 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     // there are 512 (their parts cost more to join); within 256 MiB of parts.
     const int64_t most = pages.table_width << pages.page_shift, wgs = (int64_t)a.items * kv_heads;
     int64_t splits = std::min<int64_t>({(keys ? 2048 : 512) / std::max<int64_t>(wgs, 1), ceil_div(most, attn::MIN_SPAN), 64});
-    const int64_t row = tokens * heads * (dim + 2) * (int64_t)sizeof(float);
+    const int64_t row = tokens * heads * (dim + 4) * (int64_t)sizeof(float);
     splits = std::min<int64_t>(splits, (int64_t(256) << 20) / std::max<int64_t>(row, 1));
     a.splits = (int)std::max<int64_t>(splits, 1);
     if (a.splits > 1) {

@@ -11,7 +11,7 @@ struct FwdArgs {
     const void *q, *k, *v;   // k, v: the K/V rows, or the pages
     void* o;
     float* lse;              // [tokens][heads], or null
-    float* part;             // [splits][tokens * heads][dim + 2] (splits > 1)
+    float* part;             // [splits][tokens * heads][dim + 4] (splits > 1): o, its base, its sum
     const int32_t* starts;
     PagedArgs pages;         // paged
     int n_seqs, tokens, heads, kv_heads, group, dim;

@@ -28,12 +28,22 @@
 namespace mlxhip {
 namespace attn {
 
-// A sequence's parts: as many as its keys are worth, up to the launch's.
-__device__ inline int parts_of(int keys, int splits) { return min(splits, max(1, (keys + MIN_SPAN - 1) / MIN_SPAN)); }
-
 __device__ inline int length_of(const PagedArgs& p, int seq) { return __builtin_amdgcn_readfirstlane(max(p.lens[seq], 0)); }
 // Of a length's positions those that the table has room for.
 __device__ inline int keys_of(const PagedArgs& p, int length) { return (int)min((int64_t)length, p.table_width << p.page_shift); }
+
+// Parts of a sequence: of as many keys as the longest one has in each of the launch's `splits`, so that
+// workgroups take about as long whatever their sequence, and MIN_SPAN at least.
+__device__ inline int parts_of(const PagedArgs& p, int keys, int splits) {
+    if (splits == 1) return 1;
+    int most = 0;
+    for (int i = threadIdx.x & 63; i < p.n_seqs; i += 64) most = max(most, p.lens[i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    most = __builtin_amdgcn_readfirstlane(keys_of(p, most));
+    const int span = max(MIN_SPAN, (most + splits - 1) / splits);
+    return max(1, (keys + span - 1) / span);
+}
 
 template <int DT, int DP, bool PAGED, bool KEYS>
 __global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS), amdgpu_waves_per_eu(KEYS && DT == MLXHIP_DTYPE_F32 ? 1 : 2, 2)))
@@ -62,7 +72,7 @@ void attn_fwd_kernel(FwdArgs a) {
     const int row0 = (at.level - 1) * BM, rows = at.tokens * a.group;
     const int length = PAGED ? length_of(a.pages, at.seq) : at.tokens, keys = PAGED ? keys_of(a.pages, length) : length;
     const int shift = length - at.tokens;  // position of the first new token
-    const int parts = PAGED ? parts_of(keys, a.splits) : 1, part = PAGED ? blockIdx.y : 0;
+    const int parts = PAGED ? parts_of(a.pages, keys, a.splits) : 1, part = PAGED ? blockIdx.y : 0;
     if (part >= parts) return;
 
     // This lane's row and the last key it sees.
@@ -88,7 +98,7 @@ void attn_fwd_kernel(FwdArgs a) {
 
     // Loads: a tile's rows one after another in memory, or page by page (an
     // instruction's rows lie in one page: pages hold a multiple of 16).
-    TileLoader<DT, DP, BN, LW, !PAGED> loader;
+    TileLoader<DT, DP, BN, LW, PAGED ? PAGES : TILE> loader;
     const uint32_t stride_bytes = (uint32_t)((PAGED ? a.dim : a.kv_stride) * EB);
     loader.init(KEYS ? 0 : wave, lane, a.dim, stride_bytes);
     const char* kbase = (const char*)a.k;
@@ -113,13 +123,14 @@ void attn_fwd_kernel(FwdArgs a) {
     };
     const auto issue = [&](const char* base, MLXHIP_LDS char* tile, int j) {
         if constexpr (PAGED) {
-            loader.load(tile, KEYS ? 0 : wave, [&](int from) {
+            loader.paged(base, tile, KEYS ? 0 : wave, [&](int from, uint32_t* bytes) {
                 const int r = j * BN + from, left = min(keys - r, 16);
                 const int page = __builtin_amdgcn_readlane(numbers, (r >> a.pages.page_shift) & 63);
                 const bool ok = left > 0 && page >= 0 && page < a.pages.pages;
+                *bytes = ok ? (uint32_t)left * stride_bytes : 0u;
                 const int64_t at_row = (((int64_t)(ok ? page : 0) * a.kv_heads + kvh) << a.pages.page_shift) +
                                        (r & ((1 << a.pages.page_shift) - 1));
-                return buffer(base + at_row * stride_bytes, ok ? (uint32_t)left * stride_bytes : 0u);
+                return at_row * stride_bytes;
             });
         } else {
             loader.rows(base + (int64_t)j * BN * stride_bytes, keys - j * BN, stride_bytes, tile, KEYS ? 0 : wave);
@@ -339,9 +350,8 @@ void attn_fwd_kernel(FwdArgs a) {
             }
             if (!live) continue;
             if (!whole) {
-                float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 2);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[d0 + e] = v[e];
+                float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
+                *reinterpret_cast<f32x4*>(to + d0) = f32x4{v[0], v[1], v[2], v[3]};
                 if (d0 == 0) {
                     to[a.dim] = empty ? -INFINITY : mc;
                     to[a.dim + 1] = l;
@@ -357,13 +367,13 @@ void attn_fwd_kernel(FwdArgs a) {
 
     if (!live) return;
     if (parts > 1) {
-        float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 2);
+        float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int at_d = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
-                if (at_d < a.dim) to[at_d] = o[d][r];
+            for (int g = 0; g < 4; ++g) {
+                const int at_d = 32 * d + 8 * g + 4 * h;
+                if (at_d < a.dim) *reinterpret_cast<f32x4*>(to + at_d) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
             }
         if (h == 0) {
             to[a.dim] = empty ? -INFINITY : mc;
@@ -388,61 +398,48 @@ void attn_fwd_kernel(FwdArgs a) {
         }
 }
 
-// The parts of a row of a token's head joined, a workgroup to a row: eight groups of 32
-// threads, four values each, take every eighth part (up to 64: all loads at once), then join in order.
-template <int DT>
+// The parts of a tile of rows joined, in order: 32 threads to a row, four values each, eight
+// rows at a time; a row's parts are read 16 at a time.
+template <int DT, int BM>
 __global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a) {
-    __shared__ f32x4 sums[8][32];
-    const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x & 63, t = threadIdx.x % 32, g = threadIdx.x / 32;
-    const int token = (int)(row / a.heads), head = (int)(row - (int64_t)token * a.heads);
+    const int t = threadIdx.x % 32, item = blockIdx.x / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
     Place at;
-    if (!find_token(a.starts, a.n_seqs, a.tokens, token, &at)) return;
-    const int length = length_of(a.pages, at.seq), parts = parts_of(keys_of(a.pages, length), a.splits);
-    if (parts == 1) return;
-    const int64_t step = (int64_t)a.tokens * a.heads * (a.dim + 2);
-    const float* p = a.part + row * (a.dim + 2);
-    float m = -INFINITY, l = 0.0f;
-    if (lane < parts) {
-        m = p[lane * step + a.dim];
-        l = p[lane * step + a.dim + 1];
-    }
-    f32x4 x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (g + 8 * i < parts && 4 * t < a.dim) {
-            // Rows of dim + 2 values: pairs are aligned, quads are not.
-            typedef float f32x2 __attribute__((ext_vector_type(2)));
-            const f32x2* q = reinterpret_cast<const f32x2*>(p + (g + 8 * i) * step + 4 * t);
-            x[i] = f32x4{q[0][0], q[0][1], q[1][0], q[1][1]};
-        }
-    float top = m;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float other = __shfl_xor(top, o, 64);
-        top = other > top || other != other ? other : top;
-    }
-    const float w = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    l = w == 0.0f ? 0.0f : w * l;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
-    f32x4 sum = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float wi = __shfl(w, g + 8 * i, 64);
-        if (g + 8 * i < parts && wi != 0.0f && 4 * t < a.dim) sum += wi * x[i];
-    }
-    sums[g][t] = sum;
-    __syncthreads();
-    if (g != 0 || 4 * t >= a.dim) return;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) sum += sums[i][t];
-    const bool none = token - at.first + length - at.tokens < 0;
-    sum = none ? f32x4{} : sum / l;
+    if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return;
+    const int length = length_of(a.pages, at.seq), parts = parts_of(a.pages, keys_of(a.pages, length), a.splits);
+    if (parts == 1 || 4 * t >= a.dim) return;
+    const int row0 = (at.level - 1) * BM, rows = min(at.tokens * a.group - row0, BM);
+    const int64_t step = (int64_t)a.tokens * a.heads * (a.dim + 4);
     typedef typename dev::Elem<DT>::type E;
-    E* to = (E*)a.o + (int64_t)token * a.o_stride + (int64_t)head * a.dim + 4 * t;
-    if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = sum;
-    else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(sum[0], sum[1]), gemm16::pack2<DT>(sum[2], sum[3])};
+    for (int r = threadIdx.x / 32; r < rows; r += THREADS / 32) {
+        const int tok = (row0 + r) / a.group, head = kvh * a.group + (row0 + r - tok * a.group);
+        const float* p = a.part + ((int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
+        f32x4 sum = {};
+        float top = -INFINITY, l = 0.0f;
+        for (int i0 = 0; i0 < parts; i0 += 16) {
+            f32x4 x[16];
+            float2 ml[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i0 + i < parts) {
+                    x[i] = *reinterpret_cast<const f32x4*>(p + (i0 + i) * step + 4 * t);
+                    ml[i] = *reinterpret_cast<const float2*>(p + (i0 + i) * step + a.dim);
+                }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i0 + i < parts && ml[i].x != -INFINITY) {  // -inf: no key seen
+                    const float to = ml[i].x > top || ml[i].x != ml[i].x ? ml[i].x : top;
+                    const float u = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - to), w = __builtin_amdgcn_exp2f(ml[i].x - to);
+                    sum = sum * u + x[i] * w;
+                    l = l * u + ml[i].y * w;
+                    top = to;
+                }
+        }
+        const bool none = tok + length - at.tokens < 0;
+        sum = none ? f32x4{} : sum / l;
+        E* to = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim + 4 * t;
+        if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = sum;
+        else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(sum[0], sum[1]), gemm16::pack2<DT>(sum[2], sum[3])};
+    }
 }
 
 template <int DT, int DP, bool PAGED, bool KEYS>
@@ -451,7 +448,8 @@ int launch_fwd(const FwdArgs& a, hipStream_t s) {
                        dim3(THREADS), 0, s, a);
     MLXHIP_TRY(launch_check("attn_fwd_kernel"));
     if (a.splits == 1) return MLXHIP_OK;
-    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)(a.tokens * a.heads)), dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL((attn_join_kernel<DT, KEYS ? FEW_ROWS : ROW_TILE>), dim3((unsigned)(a.items * a.kv_heads)), dim3(THREADS), 0, s,
+                       a);
     return launch_check("attn_join_kernel");
 }
 

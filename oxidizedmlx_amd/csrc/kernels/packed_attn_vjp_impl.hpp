@@ -133,7 +133,7 @@ void attn_dq_kernel(BwdArgs a) {
         delta += __shfl_xor(delta, 32, 64);
     }
 
-    TileLoader<DT, DP, BN, WAVES, true> loader;
+    TileLoader<DT, DP, BN, WAVES, TILE> loader;
     const uint32_t stride_bytes = (uint32_t)(a.kv_stride * EB);
     loader.init(wave, lane, a.dim, stride_bytes);
     const int64_t off = ((int64_t)at.first * a.kv_stride + (int64_t)kvh * a.dim) * EB;
@@ -268,7 +268,7 @@ void attn_dkdv_kernel(BwdArgs a) {
         for (int i = 0; i < (int)(sizeof(kf[s]) / 16); ++i) kf[s].q[i] ^= a.flip;
     }
 
-    TileLoader<DT, DP, BR, WAVES, false> lq, lo;
+    TileLoader<DT, DP, BR, WAVES, LEAN> lq, lo;
     const uint32_t q_bytes = (uint32_t)(a.q_stride * EB), o_bytes = (uint32_t)(a.o_stride * EB);
     lq.init(wave, lane, a.dim, q_bytes);
     lo.init(wave, lane, a.dim, o_bytes);
