@@ -204,6 +204,10 @@ int mlxhip_debug_fail_allocations(int64_t after);
  * piece_bytes (0: the default) from now on, 256 columns at least. Returns how many
  * pieces the calls since the last one of this took. Process-wide. */
 int64_t mlxhip_debug_cross_entropy_pieces(int64_t piece_bytes);
+/* For tests: mlxhip_packed_attention and its gradient take tiles of few rows (1) or of
+ * many (0), whatever the sizes (-1: by the sizes), and the gradient's sums over keys are cut into
+ * so many shares (0: by the sizes; 16 at most) from now on. Process-wide. */
+void mlxhip_debug_attention_plan(int32_t few_rows, int32_t shares);
 
 /* Number of visible HIP devices (0 when no GPU; never fails). */
 int mlxhip_device_count(void);

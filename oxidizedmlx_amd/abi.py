@@ -220,6 +220,7 @@ PROTOTYPES = {
                              _fp, _i64, _vp]),
     "mlxhip_attention": (_i, [_fp, _fp, _fp, _fp, _i64, _i64, _i64, _i64, _f, _i32, _vp]),
     "mlxhip_attention_vjp": (_i, [_fp, _fp, _fp, _fp, _fp, _fp, _fp, _fp, _i64, _i64, _i64, _f, _i32, _vp]),
+    "mlxhip_debug_attention_plan": (None, [_i32, _i32]),
     "mlxhip_rope_frequencies": (_i, [_vp, _i64, _d, _d, _d, _d, _i64, _vp]),
     "mlxhip_rope_rows": (_i, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f, _vp]),
     "mlxhip_rope_vjp_rows": (_i, [_i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f, _vp]),

@@ -1041,6 +1041,7 @@ extern "C" {
 
 int mlxhip_abi_version(void) { return MLXHIP_ABI_VERSION; }
 
+void mlxhip_debug_attention_plan(int32_t few_rows, int32_t shares) { attention_plan(few_rows, shares); }
 int64_t mlxhip_debug_cross_entropy_pieces(int64_t piece_bytes) { return linear_cross_entropy_pieces(piece_bytes); }
 
 int mlxhip_debug_fail_allocations(int64_t after) {

@@ -47,6 +47,8 @@ int paged_append(int dtype, const void* k, const void* v, void* k_pages, void* v
                  float magnitude, hipStream_t s);
 
 // ── packed_attn.hip ───────────────────────────────────────────────────────
+// For tests: few_rows 0 or 1 (-1: by the sizes) and shares up to 16 (0: by the sizes) from now on.
+void attention_plan(int few_rows, int shares);
 int packed_attention(int dtype, const void* q, const void* k, const void* v, const int32_t* starts, void* o, float* lse,
                      int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride,
                      int64_t kv_stride, int64_t o_stride, float scale, int causal, hipStream_t s);

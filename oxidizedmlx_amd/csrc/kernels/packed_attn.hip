@@ -4,11 +4,15 @@
 #include "../common.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 
 namespace mlxhip {
 namespace {
+
+// For tests (attention_plan): tiles of few rows or not, and shares, whatever the sizes.
+std::atomic<int> forced_few_rows{-1}, forced_shares{0};
 
 // Work items of sequences whose lengths are known on the device only: a tile more for each.
 int items_of(int64_t tokens, int64_t per_token, int64_t n_seqs, int64_t rows) {
@@ -23,6 +27,16 @@ uint32_t flip_of(int dtype, float scale) {
 // times the smallest normal number are 0 beside any other).
 float factor_of(float scale) { return std::max(std::fabs(scale) * 1.44269504088896340736f, FLT_MIN); }
 
+// Whether a prompt's rows go in tiles of 32 whose keys four waves share out, not in tiles of 128: where
+// those would leave compute units without work. Forward, us, tiles of 128 / 32: f16, 123 tiles (1537
+// tokens, 9 heads on 3 of 80) 19.4 / 13.5; bf16, 320 (2048, 16 heads of 64) 13.0 / 16.9; f32, 320 (the
+// same) 52 / 38, 516 (4096, 16 on 4 of 128) 762 / 648.
+bool few_rows(int dtype, int64_t tokens, int64_t group, int64_t n_seqs, int64_t kv_heads) {
+    if (const int forced = forced_few_rows.load(); forced >= 0) return forced;
+    const int64_t wgs = items_of(tokens, group, n_seqs, attn::ROW_TILE) * kv_heads;
+    return wgs < (dtype == MLXHIP_DTYPE_F32 ? 640 : 192);
+}
+
 template <class F>
 int by_dtype(int dtype, F&& f) {
     int rc = MLXHIP_OK;
@@ -31,6 +45,11 @@ int by_dtype(int dtype, F&& f) {
 }
 
 }  // namespace
+
+void attention_plan(int few_rows, int shares) {
+    forced_few_rows = few_rows;
+    forced_shares = std::clamp(shares, 0, attn::MAX_SHARES);
+}
 
 int packed_attention(int dtype, const void* q, const void* k, const void* v, const int32_t* starts, void* o, float* lse,
                      int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_stride,
@@ -42,8 +61,9 @@ int packed_attention(int dtype, const void* q, const void* k, const void* v, con
     a.q_stride = q_stride, a.kv_stride = kv_stride, a.o_stride = o_stride;
     a.c = factor_of(scale), a.flip = flip_of(dtype, scale);
     a.causal = causal, a.splits = 1;
-    a.items = items_of(tokens, a.group, n_seqs, attn::ROW_TILE);
-    return by_dtype(dtype, [&](auto dt) { return attn::fwd<decltype(dt)::value>(a, false, false, s); });
+    const bool keys = few_rows(dtype, tokens, a.group, n_seqs, kv_heads);
+    a.items = items_of(tokens, a.group, n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
+    return by_dtype(dtype, [&](auto dt) { return attn::fwd<decltype(dt)::value>(a, false, keys, s); });
 }
 
 int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
@@ -58,11 +78,14 @@ int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v,
     a.q_stride = q_stride, a.kv_stride = kv_stride, a.o_stride = o_stride;
     a.c = factor_of(scale), a.scale = scale, a.flip = flip_of(dtype, scale);
     a.causal = causal;
-    a.row_items = items_of(tokens, a.group, n_seqs, attn::ROW_TILE);
+    a.few_rows = few_rows(dtype, tokens, a.group, n_seqs, kv_heads);
+    a.row_items = items_of(tokens, a.group, n_seqs, a.few_rows ? attn::FEW_ROWS : attn::ROW_TILE);
     a.key_items = items_of(tokens, 1, n_seqs, attn::KEY_TILE);
-    // Few tiles of keys: a group's heads over several workgroups, their sums joined.
-    const int64_t wgs = a.key_items * kv_heads;
-    a.shares = (int)std::clamp<int64_t>((512 + wgs - 1) / std::max<int64_t>(wgs, 1), 1, a.group);
+    // Few tiles of keys: each one's walk over several workgroups until there are 512, of three blocks of
+    // 32 rows or more on average, their sums joined.
+    const int64_t wgs = a.key_items * kv_heads, blocks = a.group * (tokens / n_seqs) / (causal ? 64 : 32);
+    a.shares = (int)std::clamp<int64_t>(std::min<int64_t>(ceil_div(512, wgs), blocks / 3), 1, attn::MAX_SHARES);
+    if (const int forced = forced_shares.load()) a.shares = forced;
     const size_t stats = (((size_t)tokens * heads + 63) & ~size_t(63)) * sizeof(float);
     const size_t part = a.shares > 1 ? (size_t)a.shares * 2 * tokens * kv_heads * dim * sizeof(float) : 0;
     void* ws = nullptr;

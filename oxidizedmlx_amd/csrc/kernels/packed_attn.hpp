@@ -35,14 +35,16 @@ struct BwdArgs {
     float c, scale;
     uint32_t flip;
     int causal, row_items, key_items, shares;
+    bool few_rows;  // rows in tiles of FEW_ROWS
 };
 template <int DT>
 int bwd(const BwdArgs& a, hipStream_t s);
 
 // Rows of a work item: query rows (token, head of the group) and keys.
 constexpr int ROW_TILE = 128, FEW_ROWS = 32, KEY_TILE = 128;
+constexpr int MAX_SHARES = 16;
 // Rows that see up to as many keys get P and dS in two terms in the gradients of 16-bit types.
-constexpr int FINE_KEYS = 256;
+constexpr int FINE_KEYS = 64;
 // Keys that are worth a workgroup of their own.
 constexpr int MIN_SPAN = 256;
 

@@ -349,6 +349,8 @@ void attn_fwd_kernel(FwdArgs a) {
                 if (whole) v[e] = lim < 0 ? 0.0f : v[e] * inv;
             }
             if (!live) continue;
+            if (!PAGED && a.lse && d0 == 0)
+                a.lse[(int64_t)(at.first + tok) * a.heads + head] = lim < 0 ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
             if (!whole) {
                 float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
                 *reinterpret_cast<f32x4*>(to + d0) = f32x4{v[0], v[1], v[2], v[3]};
@@ -447,6 +449,7 @@ int launch_fwd(const FwdArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((attn_fwd_kernel<DT, DP, PAGED, KEYS>), dim3((unsigned)(a.items * a.kv_heads), (unsigned)a.splits),
                        dim3(THREADS), 0, s, a);
     MLXHIP_TRY(launch_check("attn_fwd_kernel"));
+    if constexpr (!PAGED) return MLXHIP_OK;
     if (a.splits == 1) return MLXHIP_OK;
     hipLaunchKernelGGL((attn_join_kernel<DT, KEYS ? FEW_ROWS : ROW_TILE>), dim3((unsigned)(a.items * a.kv_heads)), dim3(THREADS), 0, s,
                        a);
@@ -456,6 +459,7 @@ int launch_fwd(const FwdArgs& a, hipStream_t s) {
 template <int DT>
 int fwd(const FwdArgs& a, bool paged, bool keys, hipStream_t s) {
     const bool wide = a.dim > 64;
+    if (!paged && keys) return wide ? launch_fwd<DT, 128, false, true>(a, s) : launch_fwd<DT, 64, false, true>(a, s);
     if (!paged) return wide ? launch_fwd<DT, 128, false, false>(a, s) : launch_fwd<DT, 64, false, false>(a, s);
     if (keys) return wide ? launch_fwd<DT, 128, true, true>(a, s) : launch_fwd<DT, 64, true, true>(a, s);
     return wide ? launch_fwd<DT, 128, true, false>(a, s) : launch_fwd<DT, 64, true, false>(a, s);

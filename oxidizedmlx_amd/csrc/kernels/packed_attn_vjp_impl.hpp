@@ -11,7 +11,7 @@
 // Roundings: sums are f32; P and dS are rounded to the operands' type for their products, as
 // many independent errors as keys or rows, together about the one that a result itself gets.
 // Rows that see few keys carry most of a causal sequence's gradient (P is about 1 / keys), so
-// those that see up to 256 have P and dS in two terms, the second what the first
+// those that see up to 64 have P and dS in two terms, the second what the first
 // rounds off; and D, which the rounding of O moves (by as much as dS itself after a few keys),
 // is formed anew for them, as the row's sum of P dP, in a walk before the one over dS.
 // f16 would lose dS below 2^-24: each column of dS (a query's in dQ, a key's in dK) has a power of
@@ -73,20 +73,24 @@ __device__ inline void store_row(typename dev::Elem<DT>::type* to, const f32x16 
         }
 }
 
-// dQ of a tile of query rows: as the forward kernel, K and V tiles in LDS, the
-// rows' Q and dO in registers.
-template <int DT, int DP>
-__global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS), amdgpu_waves_per_eu(DT == MLXHIP_DTYPE_F32 ? 1 : 2, 2)))
+// dQ of a tile of query rows: as the forward kernel (ROWS: four waves of 32 rows share tiles of K and
+// V in LDS; KEYS: four waves have the same 32 rows and every fourth tile), the rows'
+// Q and dO in registers.
+template <int DT, int DP, bool KEYS>
+__global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS),
+                          amdgpu_waves_per_eu(DT == MLXHIP_DTYPE_F32 && (KEYS || DP == 128) ? 1 : 2, 2)))
 void attn_dq_kernel(BwdArgs a) {
-    constexpr int BM = ROW_TILE, BN = DT == MLXHIP_DTYPE_F32 ? 32 : 64, EB = ELEM<DT>;
-    constexpr int KB = BN / 32, KS = DP / 16, DB = DP / 32;
+    constexpr int BM = KEYS ? FEW_ROWS : ROW_TILE, BN = KEYS || DT == MLXHIP_DTYPE_F32 ? 32 : 64, EB = ELEM<DT>;
+    constexpr int KB = BN / 32, KS = DP / 16, DB = DP / 32, LW = KEYS ? 1 : WAVES;
     using T = Tile<DT, DP, BN>;
-    __shared__ __attribute__((aligned(1024))) char smem_raw[4 * T::BYTES];
-    MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw;
+    constexpr int TILES = (KEYS ? WAVES : 2) * 2 * T::BYTES, JOIN = KEYS ? WAVES * 32 * DP * 4 : 0;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[TILES > JOIN ? TILES : JOIN];
+    __shared__ float row_sums[WAVES][32];
     typedef typename dev::Elem<DT>::type E;
 
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw + (KEYS ? wave * 2 * T::BYTES : 0);
     const int lin = blockIdx.x;
     const bool per8 = (a.kv_heads & 7) == 0;
     const int item = per8 ? (lin >> 3) % a.row_items : lin / a.kv_heads;
@@ -95,7 +99,7 @@ void attn_dq_kernel(BwdArgs a) {
     if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return;
     const int row0 = (at.level - 1) * BM, rows = at.tokens * a.group, n = at.tokens;
 
-    const int wrow = row0 + 32 * wave, row = wrow + (lane & 31);
+    const int wrow = row0 + (KEYS ? 0 : 32 * wave), row = wrow + (lane & 31);
     const bool live = row < rows;
     const int tok = live ? (int)((uint32_t)row / (uint32_t)a.group) : 0, head = kvh * a.group + (live ? row - tok * a.group : 0);
     const int lim = !live ? -1 : a.causal ? tok : n - 1;
@@ -133,12 +137,12 @@ void attn_dq_kernel(BwdArgs a) {
         delta += __shfl_xor(delta, 32, 64);
     }
 
-    TileLoader<DT, DP, BN, WAVES, TILE> loader;
+    TileLoader<DT, DP, BN, LW, TILE> loader;
     const uint32_t stride_bytes = (uint32_t)(a.kv_stride * EB);
-    loader.init(wave, lane, a.dim, stride_bytes);
+    loader.init(KEYS ? 0 : wave, lane, a.dim, stride_bytes);
     const int64_t off = ((int64_t)at.first * a.kv_stride + (int64_t)kvh * a.dim) * EB;
     const auto issue = [&](const void* p, MLXHIP_LDS char* tile, int j) {
-        loader.rows((const char*)p + off + (int64_t)j * BN * stride_bytes, n - j * BN, stride_bytes, tile, wave);
+        loader.rows((const char*)p + off + (int64_t)j * BN * stride_bytes, n - j * BN, stride_bytes, tile, KEYS ? 0 : wave);
     };
 
     RowFrag<DT, DP, BN> rf;
@@ -149,96 +153,149 @@ void attn_dq_kernel(BwdArgs a) {
     Column<DT> column;
     enum { PLAIN, ROW_SUM, FINE };
     float sum = 0.0f;  // ROW_SUM: of P (dP - D), 0 were D exact
-    const auto walk = [&](auto which) {
+    // A tile of keys. after_v: what may start once V has been read.
+    const auto compute = [&](auto which, const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int first, auto&& after_v) {
         constexpr int KIND = decltype(which)::value;
-        if (n_tiles > 0) {
-            issue(a.k, smem, 0);
-            issue(a.v, smem + T::BYTES, 0);
-        }
-        for (int j = 0; j < n_tiles; ++j) {
-            const MLXHIP_LDS char* kt = smem + (j & 1) * 2 * T::BYTES;
-            const MLXHIP_LDS char* vt = kt + T::BYTES;
-            MLXHIP_LDS char* other = smem + ((j + 1) & 1) * 2 * T::BYTES;
-            gemm16::wait_vmcnt<0>();
-            gemm16::lds_barrier();
-            if (j + 1 < n_tiles) {
-                issue(a.k, other, j + 1);
-                issue(a.v, other + T::BYTES, j + 1);
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int k0 = first + 32 * b;
+            if (k0 > wave_last) break;
+            f32x16 sc = {}, dp = {};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                mma<DT>(rf.read(kt, 32 * b, s), q[s], sc);
+                mma<DT>(rf.read(vt, 32 * b, s), g[s], dp);
             }
-            if (wrow >= rows) continue;
+            if (b == KB - 1) after_v();
+            float e[16];
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                const int k0 = j * BN + 32 * b;
-                if (k0 > wave_last) break;
-                f32x16 sc = {}, dp = {};
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    mma<DT>(rf.read(kt, 32 * b, s), q[s], sc);
-                    mma<DT>(rf.read(vt, 32 * b, s), g[s], dp);
-                }
-                float e[16];
+            for (int r = 0; r < 16; ++r)
+                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], a.c, -lse2)) * (dp[r] - delta);
+            if (__ballot(k0 + 31 > wave_first || !live)) {
+                own_branch();
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], a.c, -lse2)) * (dp[r] - delta);
-                if (__ballot(k0 + 31 > wave_first || !live)) {
-                    own_branch();
+                    if (k0 + 8 * (r / 4) + 4 * h + r % 4 > lim) e[r] = 0.0f;
+            }
+            if constexpr (KIND == ROW_SUM) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (k0 + 8 * (r / 4) + 4 * h + r % 4 > lim) e[r] = 0.0f;
-                }
-                if constexpr (KIND == ROW_SUM) {
+                for (int r = 0; r < 16; ++r) sum += e[r];
+            } else {
+                column.fit(e, dq);
+                const Frag<DT> ds[2] = {frag_of<DT>(e), frag_of<DT>(e + 8)};
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += e[r];
-                } else {
-                    column.fit(e, dq);
-                    const Frag<DT> ds[2] = {frag_of<DT>(e), frag_of<DT>(e + 8)};
+                for (int s = 0; s < 2; ++s) {
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                        for (int d = 0; d < DB; ++d) {
-                            const Frag<DT> kc = cf.read(kt, 32 * b + 16 * s, d);
-                            if constexpr (KIND == FINE) mma<DT>(kc, rest_of<DT>(e + 8 * s, ds[s]), dq[d]);
-                            mma<DT>(kc, ds[s], dq[d]);
-                        }
+                    for (int d = 0; d < DB; ++d) {
+                        const Frag<DT> kc = cf.read(kt, 32 * b + 16 * s, d);
+                        if constexpr (KIND == FINE) mma<DT>(kc, rest_of<DT>(e + 8 * s, ds[s]), dq[d]);
+                        mma<DT>(kc, ds[s], dq[d]);
                     }
                 }
+            }
+        }
+    };
+    const auto walk = [&](auto which) {
+        if constexpr (KEYS) {
+            // A wave's own tiles: V of the next one loads during this one's second product.
+            MLXHIP_LDS char* kt = smem;
+            MLXHIP_LDS char* vt = smem + T::BYTES;
+            int j = wave;
+            if (j < n_tiles) {
+                issue(a.v, vt, j);
+                issue(a.k, kt, j);
+            }
+            for (; j < n_tiles; j += WAVES) {
+                gemm16::wait_vmcnt<0>();
+                compute(which, kt, vt, j * BN, [&] {
+                    __builtin_amdgcn_s_waitcnt(0xC07F);
+                    if (j + WAVES < n_tiles) issue(a.v, vt, j + WAVES);
+                });
+                __builtin_amdgcn_s_waitcnt(0xC07F);
+                if (j + WAVES < n_tiles) issue(a.k, kt, j + WAVES);
+            }
+        } else {
+            if (n_tiles > 0) {
+                issue(a.k, smem, 0);
+                issue(a.v, smem + T::BYTES, 0);
+            }
+            for (int j = 0; j < n_tiles; ++j) {
+                const MLXHIP_LDS char* kt = smem + (j & 1) * 2 * T::BYTES;
+                MLXHIP_LDS char* other = smem + ((j + 1) & 1) * 2 * T::BYTES;
+                gemm16::wait_vmcnt<0>();
+                gemm16::lds_barrier();
+                if (j + 1 < n_tiles) {
+                    issue(a.k, other, j + 1);
+                    issue(a.v, other + T::BYTES, j + 1);
+                }
+                if (wrow < rows) compute(which, kt, kt + T::BYTES, j * BN, [] {});
             }
         }
     };
     if (DT != MLXHIP_DTYPE_F32 && last_key(row0 + BM - 1) < FINE_KEYS) {
         walk(std::integral_constant<int, ROW_SUM>{});
         sum += __shfl_xor(sum, 32, 64);
+        if constexpr (KEYS) {
+            if (h == 0) row_sums[wave][lane] = sum;
+            __syncthreads();
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) sum += row_sums[i][lane & 31];
+        } else {
+            gemm16::lds_barrier();  // the first tiles are loaded again
+        }
         delta += sum * __builtin_amdgcn_exp2f(-P_SHIFT<DT>);
-        gemm16::lds_barrier();  // the first tiles are loaded again
         walk(std::integral_constant<int, DT == MLXHIP_DTYPE_F32 ? PLAIN : FINE>{});
     } else {
         walk(std::integral_constant<int, PLAIN>{});
     }
-    if (live && h == 0) {
+    float f = a.scale / column.by * __builtin_amdgcn_exp2f(-P_SHIFT<DT>);
+    if (live && h == 0 && (!KEYS || wave == 0)) {
         a.lse2[(int64_t)head * a.tokens + token] = lse2;
         a.delta[(int64_t)head * a.tokens + token] = -delta;
     }
-    if (live)
-        store_row<DT, DB>((E*)a.dq + token * a.q_stride + (int64_t)head * a.dim, dq, h, a.dim,
-                          a.scale / column.by * __builtin_amdgcn_exp2f(-P_SHIFT<DT>));
+    if constexpr (KEYS) {
+        // The waves' sums joined in order, value by value; wave w then holds every fourth block of the head.
+        __syncthreads();
+        float* all = reinterpret_cast<float*>(smem_raw);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) all[(wave * DB * 16 + d * 16 + r) * 64 + lane] = dq[d][r] * f;
+        __syncthreads();
+        E* to = (E*)a.dq + token * a.q_stride + (int64_t)head * a.dim;
+        for (int i = wave; i < DB * 4; i += WAVES) {  // registers 4 i .. 4 i + 3
+            f32x4 v = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) v[e] += all[(w * DB * 16 + 4 * i + e) * 64 + lane];
+            const int at_d = 32 * (i / 4) + 8 * (i % 4) + 4 * h;
+            if (!live || at_d >= a.dim) continue;
+            if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to + at_d) = v;
+            else *reinterpret_cast<u32x2*>(to + at_d) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
+        }
+        return;
+    }
+    if (live) store_row<DT, DB>((E*)a.dq + token * a.q_stride + (int64_t)head * a.dim, dq, h, a.dim, f);
 }
 
-// dK and dV of a tile of keys over share blockIdx.y of the group's heads: a wave's 32 keys'
+// dK and dV of a tile of keys over share blockIdx.y of its walk (the group's heads, their rows): a wave's 32 keys'
 // K and V in registers, tiles of a head's Q and dO in LDS with the rows' lse and
-// delta. GROUPS groups of four waves have the same keys, every other tile each, and join at the
-// end: a causal sequence's first keys are seen by all its rows, and the longest such walk
-// is what the kernel waits for.
+// delta. Two groups of four waves (f32 heads of 128, over 256 registers: one) have the same keys, every
+// other tile each, and join at the end: a causal sequence's first keys are seen by all its
+// rows, and the longest such walk is what the kernel waits for.
 template <int DT, int DP>
-constexpr int DKDV_GROUPS = DT == MLXHIP_DTYPE_F32 && DP == 128 ? 1 : 2;  // f32 of 128: over 256 registers
+constexpr int DKDV_GROUPS = DT == MLXHIP_DTYPE_F32 && DP == 128 ? 1 : 2;
 
 template <int DT, int DP>
 __global__ __attribute__((amdgpu_flat_work_group_size(THREADS * DKDV_GROUPS<DT, DP>, THREADS * DKDV_GROUPS<DT, DP>),
-                          amdgpu_waves_per_eu(DKDV_GROUPS<DT, DP>, DKDV_GROUPS<DT, DP>)))
+                          amdgpu_waves_per_eu(DKDV_GROUPS<DT, DP>, 2)))
 void attn_dkdv_kernel(BwdArgs a) {
     constexpr int GROUPS = DKDV_GROUPS<DT, DP>, BR = DT == MLXHIP_DTYPE_F32 ? 32 : 64, EB = ELEM<DT>;
     constexpr int RB = BR / 32, KS = DP / 16, DB = DP / 32;
     using T = Tile<DT, DP, BR>;
-    constexpr int STATS = 256, STAGE = 2 * T::BYTES + 2 * STATS, JOIN = GROUPS > 1 ? THREADS * 2 * DB * 16 * 4 : 0;
+    constexpr int STATS = 256, STAGE = 2 * T::BYTES + 2 * STATS, JOIN = (GROUPS - 1) * THREADS * 2 * DB * 16 * 4;
     __shared__ __attribute__((aligned(1024))) char smem_raw[GROUPS * 2 * STAGE > JOIN ? GROUPS * 2 * STAGE : JOIN];
     typedef typename dev::Elem<DT>::type E;
 
@@ -252,8 +309,9 @@ void attn_dkdv_kernel(BwdArgs a) {
     Place at;
     if (!find_tile(a.starts, a.n_seqs, a.tokens, 1, KEY_TILE, item, &at)) return;
     const int n = at.tokens, tile0 = (at.tiles - at.level) * KEY_TILE;
-    const int g0 = (int)((int64_t)a.group * blockIdx.y / a.shares), g1 = (int)((int64_t)a.group * (blockIdx.y + 1) / a.shares);
-    const int first = a.causal ? tile0 / BR : 0, per = (n + BR - 1) / BR - first, steps = (g1 - g0) * per;
+    const int share = blockIdx.y;
+    const int first = a.causal ? tile0 / BR : 0, per = (n + BR - 1) / BR - first, all_steps = a.group * per;
+    const int step0 = (int)((int64_t)all_steps * share / a.shares), steps = (int)((int64_t)all_steps * (share + 1) / a.shares) - step0;
     const int fine_rows = a.causal ? FINE_KEYS : n <= FINE_KEYS ? n : 0;
 
     const int wkey = tile0 + 32 * wave, key = wkey + (lane & 31);
@@ -268,25 +326,29 @@ void attn_dkdv_kernel(BwdArgs a) {
         for (int i = 0; i < (int)(sizeof(kf[s]) / 16); ++i) kf[s].q[i] ^= a.flip;
     }
 
-    TileLoader<DT, DP, BR, WAVES, LEAN> lq, lo;
+    // The sums and the keys' rows leave few registers: what goes by the lane is formed anew
+    // where it is used. A spilled register in the loop would wait for the loads behind it.
+    const auto lane_now = [&] {
+        int l = tid;
+        asm volatile("" : "+v"(l));
+        return l & 63;
+    };
     const uint32_t q_bytes = (uint32_t)(a.q_stride * EB), o_bytes = (uint32_t)(a.o_stride * EB);
-    lq.init(wave, lane, a.dim, q_bytes);
-    lo.init(wave, lane, a.dim, o_bytes);
     const auto issue = [&](int i, MLXHIP_LDS char* stage) {
-        const int head = kvh * a.group + g0 + i / per, j = first + i % per, left = min(n - j * BR, BR);
+        const int at_i = step0 + i, g = at_i / per, head = kvh * a.group + g, j = first + at_i - g * per, left = min(n - j * BR, BR);
         const int64_t token = at.first + (int64_t)j * BR;
+        const int l = lane_now();
+        TileLoader<DT, DP, BR, WAVES, LEAN> lq, lo;
+        lq.init(wave, l, a.dim, q_bytes);
+        lo.init(wave, l, a.dim, o_bytes);
         lq.rows((const char*)a.q + (token * a.q_stride + (int64_t)head * a.dim) * EB, left, q_bytes, stage, wave);
         lo.rows((const char*)a.dout + (token * a.o_stride + (int64_t)head * a.dim) * EB, left, o_bytes, stage + T::BYTES, wave);
         if (wave < 2) {
             const float* p = (wave ? a.delta : a.lse2) + (int64_t)head * a.tokens + token;
-            lds_load4(buffer(p, (uint32_t)left * 4), stage + 2 * T::BYTES + wave * STATS, (uint32_t)lane * 4);
+            lds_load4(buffer(p, (uint32_t)left * 4), stage + 2 * T::BYTES + wave * STATS, (uint32_t)l * 4);
         }
     };
 
-    RowFrag<DT, DP, BR> rf;
-    ColFrag<DT, DP, BR> cf;
-    rf.init(lane);
-    cf.init(lane);
     f32x16 dk[DB] = {}, dv[DB] = {};
     Column<DT> column;
     if (part < steps) issue(part, smem);
@@ -299,12 +361,16 @@ void attn_dkdv_kernel(BwdArgs a) {
         gemm16::lds_barrier();
         if (i + GROUPS < steps) issue(i + GROUPS, smem + (odd ^ 1) * STAGE);
         if (wkey >= n || i >= steps) continue;
-        const int j = first + i % per;
+        const int j = first + (step0 + i) % per;
         const int b0 = a.causal && j * BR + 31 < wkey ? min((wkey - j * BR) / 32, RB) : 0, b1 = min(RB, (n - j * BR + 31) / 32);
 #pragma unroll 1
         for (int b = b0; b < b1; ++b) {  // blocks of 32 rows that see any of the keys
             const int r0 = j * BR + 32 * b;
-            asm volatile("" : "+v"(rf.key), "+v"(cf.key));  // addresses formed here: kept, they take registers
+            const int l = lane_now(), h = l >> 5, key = wkey + (l & 31);
+            RowFrag<DT, DP, BR> rf;
+            ColFrag<DT, DP, BR> cf;
+            rf.init(l);
+            cf.init(l);
             f32x16 sc = {}, dp;  // dp starts as -delta
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -364,30 +430,36 @@ void attn_dkdv_kernel(BwdArgs a) {
     if constexpr (GROUPS > 1) {
         __syncthreads();
         float* sums = reinterpret_cast<float*>(smem_raw) + (tid & (THREADS - 1));
-        if (part == 1) {
+        constexpr int EACH = 2 * DB * 16 * THREADS;
+        if (part > 0) {
+            float* to = sums + (part - 1) * EACH;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    sums[(d * 16 + r) * THREADS] = dk[d][r] * fk;
-                    sums[((DB + d) * 16 + r) * THREADS] = dv[d][r];
+                    to[(d * 16 + r) * THREADS] = dk[d][r] * fk;
+                    to[((DB + d) * 16 + r) * THREADS] = dv[d][r];
                 }
         }
         __syncthreads();
-        if (part == 1) return;
+        if (part > 0) return;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                dk[d][r] = dk[d][r] * fk + sums[(d * 16 + r) * THREADS];
-                dv[d][r] += sums[((DB + d) * 16 + r) * THREADS];
+                dk[d][r] *= fk;
+#pragma unroll
+                for (int g = 0; g < GROUPS - 1; ++g) {
+                    dk[d][r] += sums[g * EACH + (d * 16 + r) * THREADS];
+                    dv[d][r] += sums[g * EACH + ((DB + d) * 16 + r) * THREADS];
+                }
             }
         fk = 1.0f;
     }
     if (!live) return;
     if (a.shares > 1) {
         const int64_t each = (int64_t)a.tokens * a.kv_heads * a.dim;
-        float* to = a.part + 2 * each * blockIdx.y + ((int64_t)(at.first + key) * a.kv_heads + kvh) * a.dim;
+        float* to = a.part + 2 * each * share + ((int64_t)(at.first + key) * a.kv_heads + kvh) * a.dim;
         store_row<MLXHIP_DTYPE_F32, DB>(to, dk, h, a.dim, fk);
         store_row<MLXHIP_DTYPE_F32, DB>(to + each, dv, h, a.dim, unshift);
         return;
@@ -396,24 +468,26 @@ void attn_dkdv_kernel(BwdArgs a) {
     store_row<DT, DB>((E*)a.dv + kv_at, dv, h, a.dim, unshift);
 }
 
-// The shares of dK and dV summed in order; only the tokens of sequences.
+// The shares of dK and dV summed in order, a wave to a token.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void attn_dkdv_join_kernel(BwdArgs a) {
-    const int quads = a.kv_heads * a.dim / 4;
-    const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-    const int64_t token = i / quads;
-    if (token >= a.tokens) return;
-    bool of_sequence = false;
-    for (int s = 0; s < a.n_seqs && !of_sequence; ++s) of_sequence = a.starts[s] <= token && token < a.starts[s + 1];
-    if (!of_sequence) return;
-    const int64_t each = (int64_t)a.tokens * a.kv_heads * a.dim, at = 4 * (i - token * quads);
+    const int token = (int)blockIdx.x * WAVES + threadIdx.x / 64, quads = a.kv_heads * a.dim / 4;
+    Place at;
+    if (token >= a.tokens || !find_token(a.starts, a.n_seqs, a.tokens, token, &at)) return;
+    const int64_t each = (int64_t)a.tokens * a.kv_heads * a.dim;
     typedef typename dev::Elem<DT>::type E;
+    for (int i = threadIdx.x & 63; i < 2 * quads; i += 64) {
+        const int w = i >= quads, d = 4 * (i - w * quads);
+        const float* p = a.part + w * each + (int64_t)token * a.kv_heads * a.dim + d;
+        f32x4 x[MAX_SHARES];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        const float* p = a.part + w * each + 4 * i;
-        f32x4 v = *reinterpret_cast<const f32x4*>(p);
-        for (int s = 1; s < a.shares; ++s) v += *reinterpret_cast<const f32x4*>(p + 2 * each * s);
-        E* to = (E*)(w ? a.dv : a.dk) + token * a.kv_stride + at;
+        for (int s = 0; s < MAX_SHARES; ++s)
+            if (s < a.shares) x[s] = *reinterpret_cast<const f32x4*>(p + 2 * each * s);
+        f32x4 v = x[0];
+#pragma unroll
+        for (int s = 1; s < MAX_SHARES; ++s)
+            if (s < a.shares) v += x[s];
+        E* to = (E*)(w ? a.dv : a.dk) + (int64_t)token * a.kv_stride + d;
         if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = v;
         else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
     }
@@ -421,14 +495,14 @@ __global__ __launch_bounds__(THREADS) void attn_dkdv_join_kernel(BwdArgs a) {
 
 template <int DT, int DP>
 int launch_bwd(const BwdArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((attn_dq_kernel<DT, DP>), dim3((unsigned)(a.row_items * a.kv_heads)), dim3(THREADS), 0, s, a);
+    const dim3 rows((unsigned)(a.row_items * a.kv_heads)), keys((unsigned)(a.key_items * a.kv_heads), (unsigned)a.shares);
+    if (a.few_rows) hipLaunchKernelGGL((attn_dq_kernel<DT, DP, true>), rows, dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((attn_dq_kernel<DT, DP, false>), rows, dim3(THREADS), 0, s, a);
     MLXHIP_TRY(launch_check("attn_dq_kernel"));
-    hipLaunchKernelGGL((attn_dkdv_kernel<DT, DP>), dim3((unsigned)(a.key_items * a.kv_heads), (unsigned)a.shares),
-                       dim3(THREADS * DKDV_GROUPS<DT, DP>), 0, s, a);
+    hipLaunchKernelGGL((attn_dkdv_kernel<DT, DP>), keys, dim3(THREADS * DKDV_GROUPS<DT, DP>), 0, s, a);
     MLXHIP_TRY(launch_check("attn_dkdv_kernel"));
     if (a.shares == 1) return MLXHIP_OK;
-    hipLaunchKernelGGL(attn_dkdv_join_kernel<DT>, dim3((unsigned)ceil_div((int64_t)a.tokens * a.kv_heads * a.dim / 4, THREADS)),
-                       dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL(attn_dkdv_join_kernel<DT>, dim3((unsigned)ceil_div(a.tokens, WAVES)), dim3(THREADS), 0, s, a);
     return launch_check("attn_dkdv_join_kernel");
 }
 

@@ -13,6 +13,14 @@ pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("hip")]
 LEFT = 7.0  # what results hold before the call
 
 
+@pytest.fixture(params=[(-1, 0), (0, 0), (1, 0), (0, 5)], ids=["by size", "many rows", "few rows", "shares"])
+def plan(request):
+    """The kernels that larger or smaller calls take, at these sizes."""
+    abi.load_library().mlxhip_debug_attention_plan(*request.param)
+    yield
+    abi.load_library().mlxhip_debug_attention_plan(-1, 0)
+
+
 def inputs(tokens, heads, kv_heads, dim, dt, seed=1, std=1.0):
     return [R.rounded(synth.normal(seed + i, (tokens, h, dim), std=std), dt)
             for i, h in enumerate((heads, kv_heads, kv_heads, heads))]
@@ -87,24 +95,24 @@ CASES = [(1, 1, 1, 8, [0, 1]), (2, 2, 1, 64, [0, 1, 2]), (33, 3, 3, 16, [0, 33])
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("tokens,heads,kv,dim,starts", CASES)
-def test_matches_64_bits(tokens, heads, kv, dim, starts, causal, dt):
+def test_matches_64_bits(tokens, heads, kv, dim, starts, causal, dt, plan):
     print(f"packed {tokens} {heads}/{kv} {dim} {starts} causal {causal} {R.NAMES[dt]}", flush=True)
     compare(*inputs(tokens, heads, kv, dim, dt, seed=dim), starts, dim ** -0.5, causal, dt)
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 2.0 ** -40])
-def test_other_scales(scale, dt):
+def test_other_scales(scale, dt, plan):
     compare(*inputs(70, 4, 2, 32, dt), [0, 20, 70], scale, True, dt)
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-def test_rows_apart(dt):
+def test_rows_apart(dt, plan):
     compare(*inputs(100, 4, 2, 48, dt), [0, 37, 100], 0.2, True, dt, extra=24)
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-def test_certain_rows(dt):
+def test_certain_rows(dt, plan):
     """Scores of +-100: probabilities of 1 and 0, a maximum that moves late and far."""
     q, k, v, do = inputs(150, 2, 1, 64, dt)
     q = R.rounded(4 * q, dt)
@@ -113,7 +121,7 @@ def test_certain_rows(dt):
 
 
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -12, 2.0 ** 8])
-def test_f16_gradients_keep_their_digits(size):
+def test_f16_gradients_keep_their_digits(size, plan):
     """Cotangents whose dS lies below or far above f16's normal range; q, k and v so that
     the results are in it."""
     q, k, v, do = inputs(260, 4, 2, 64, abi.F16)
@@ -124,7 +132,7 @@ def test_f16_gradients_keep_their_digits(size):
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 @pytest.mark.parametrize("dim", [64, 128])
-def test_non_finite_values_stay_with_those_that_see_them(dim, dt):
+def test_non_finite_values_stay_with_those_that_see_them(dim, dt, plan):
     """Of another sequence, of keys that a causal row does not see, of tokens of no
     sequence: rows that see none are as without them."""
     q, k, v, do = inputs(300, 4, 2, dim, dt)
@@ -148,7 +156,7 @@ def test_non_finite_values_stay_with_those_that_see_them(dim, dt):
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
-def test_rows_without_any_score(dt):
+def test_rows_without_any_score(dt, plan):
     """Scores of -inf everywhere a row sees: 0/0, as the formula says."""
     q, k, v, do = inputs(40, 1, 1, 16, dt)
     q, k = np.abs(q) + 1, k.copy()
@@ -163,7 +171,7 @@ def test_rows_without_any_score(dt):
     R.check(o[4:, 0], want, bound + R.U * 8 * np.abs(want), "the others")
 
 
-def test_gradients_against_differences():
+def test_gradients_against_differences(plan):
     tokens, starts, scale = 50, [0, 17, 50], 0.3
     q, k, v, do = inputs(tokens, 4, 2, 16, abi.F32)
     c = Call(q, k, v, do, starts, abi.F32)
@@ -196,7 +204,7 @@ def test_no_tokens_and_no_sequences():
 
 
 @pytest.mark.parametrize("starts", [[0, 40, 20, 64], [-5, 30, 1000], [64, 0, 0], [2**31 - 1, -2**31, 10]])
-def test_any_starts_stay_in_bounds(starts):
+def test_any_starts_stay_in_bounds(starts, plan):
     """Not ascending, or outside: no values are promised, nothing outside the arrays is touched."""
     c = Call(*inputs(64, 4, 2, 32, abi.BF16), starts, abi.BF16)
     c.forward(0.2, True)
@@ -205,14 +213,14 @@ def test_any_starts_stay_in_bounds(starts):
     c.results()
 
 
-def test_many_short_sequences():
+def test_many_short_sequences(plan):
     lengths = (synth.uniform01(3, 150) * 6).astype(int)
     starts = np.concatenate([[0], np.cumsum(lengths)])
     compare(*inputs(int(starts[-1]) + 3, 4, 2, 16, abi.F32), starts, 0.25, True, abi.F32)
 
 
 @pytest.mark.parametrize("dt", [abi.F32, abi.F16], ids=R.NAMES.get)
-def test_same_bits_every_time_and_replayed(dt):
+def test_same_bits_every_time_and_replayed(dt, plan):
     data, starts = inputs(333, 8, 2, 64, dt), [0, 100, 333]
     def fresh():
         return Call(*data, starts, dt)
