@@ -599,7 +599,7 @@ int mlxhip_attention_vjp(const float* q, const float* k, const float* v, const f
  * A token's heads are contiguous, tokens x_stride / y_stride elements apart (heads *
  * head_dim at least: queries and keys of one projection side by side are one call).
  * Any address aligned to the elements. y may be x (equal strides), and must not
- * overlap it otherwise. tokens up to 2^25, heads * head_dim and strides up to 2^20,
+ * overlap it otherwise. tokens up to 2^24, heads * head_dim and strides up to 2^20,
  * rotary_dim even, 2 to 1024 and at most head_dim. */
 int mlxhip_rope_frequencies(double* freqs, int64_t rotary_dim, double base, double factor, double low_turns,
                             double high_turns, int64_t original_len, void* stream);
@@ -629,8 +629,8 @@ int mlxhip_rope_vjp_rows(int32_t dtype, const void* dy, const int32_t* positions
  * A non-finite value stays within its sequence: with v's the rows that see it are
  * not finite, others are as without it; the gradients of its sequence may be NaN.
  * head_dim a multiple of 8 up to 128; addresses 16-byte aligned, strides a multiple of 16
- * bytes, up to 2^20. heads a multiple of kv_heads; tokens * heads up to 2^30, n_seqs *
- * kv_heads up to 2^22. Results must not overlap operands. The gradient keeps two f32 values
+ * bytes, up to 2^20. heads a multiple of kv_heads; tokens * heads up to 2^29, n_seqs *
+ * kv_heads up to 2^21. Results must not overlap operands. The gradient keeps two f32 values
  * of each row, and where there are few keys parts of dk and dv, in a per-stream workspace.
  * mlxhip_attention is the f32 form for heads of one length, mlxhip_attention_vjp its
  * gradient (cpu_attention, cpu_kernels.rs:738-812). */
@@ -660,7 +660,7 @@ int mlxhip_packed_attention_vjp(int32_t dtype, const void* q, const void* k, con
  * too, do not enter. The keys of a sequence may be split over workgroups, whose parts, f32 in a
  * per-stream workspace (256 MiB at most), are joined in order.
  * dtype, head_dim, alignment, heads and sizes as for mlxhip_packed_attention; page_size a power
- * of two from 16 to 4096, table_width * page_size up to 2^31 - 1. HipDecoder keeps its own
+ * of two from 16 to 4096, table_width * page_size up to 2^31 - 1, of an append tokens up to 2^24. HipDecoder keeps its own
  * cache (mlxhip_decoder_*); the reference's is a host vector (ttft_behavior.rs:101-216). */
 int mlxhip_paged_append(int32_t dtype, const void* k, const void* v, const int32_t* starts, const int32_t* lens,
                         const int32_t* table, void* k_pages, void* v_pages, int64_t n_seqs, int64_t tokens,

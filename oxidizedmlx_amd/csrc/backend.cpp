@@ -1395,7 +1395,7 @@ int mlxhip_attention_vjp(const float* q, const float* k, const float* v, const f
 }
 
 namespace {
-constexpr int64_t MAX_TOKENS = int64_t(1) << 25;  // of a rotated batch (grids within 2^32 work items)
+constexpr int64_t MAX_TOKENS = int64_t(1) << 24;  // of a rotated or appended batch (grids within 2^32 work items)
 
 // Addresses and strides that the attention kernels read 16 bytes at a time.
 int check_vectors(const char* what, int dtype, std::initializer_list<const void*> typed, std::initializer_list<int64_t> strides) {
@@ -1455,13 +1455,14 @@ int rope_call(const char* what, int32_t dtype, const void* x, const int32_t* pos
 
 // Sizes that the attention over packed sequences and over pages share.
 int check_heads(const char* what, int64_t n_seqs, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-    constexpr int64_t ROWS = int64_t(1) << 30, SEQS = int64_t(1) << 22;
+    // Grids within 2^32 work items: 512 to a tile of 128 rows, and a tile more for each sequence.
+    constexpr int64_t ROWS = int64_t(1) << 29, SEQS = int64_t(1) << 21;
     MLXHIP_TRY(check_sizes(what, {n_seqs, tokens, heads, kv_heads, head_dim}, {SEQS, ROWS, MAX_DIM, MAX_DIM, 128}));
     if (kv_heads ? heads % kv_heads != 0 : heads != 0)
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: %lld heads on %lld K/V heads", what, (long long)heads, (long long)kv_heads);
     if (head_dim % 8) return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: head_dim %lld is no multiple of 8", what, (long long)head_dim);
     if (tokens * heads > ROWS || n_seqs * kv_heads > SEQS)
-        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: tokens * heads is over 2^30 or n_seqs * kv_heads over 2^22", what);
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: tokens * heads is over 2^29 or n_seqs * kv_heads over 2^21", what);
     return MLXHIP_OK;
 }
 

@@ -95,7 +95,8 @@ __device__ inline void unpack(const Vec16<DT>& x, float* out) {
     }
 }
 
-template <int DT>
+// NT: past the caches, for arrays larger than they are.
+template <int DT, bool NT = false>
 __device__ inline void store_vec(typename Elem<DT>::type* p, int64_t i, int64_t n, const float* v) {
     constexpr int VEC = Elem<DT>::VEC;
     if (i + VEC <= n) {
@@ -105,7 +106,8 @@ __device__ inline void store_vec(typename Elem<DT>::type* p, int64_t i, int64_t 
             if constexpr (DT == MLXHIP_DTYPE_F32) q[k] = __float_as_uint(v[k]);
             else q[k] = from_f32<DT>(v[2 * k]) | (uint32_t)from_f32<DT>(v[2 * k + 1]) << 16;
         }
-        reinterpret_cast<AnyVec<DT>*>(p + i)->q = q;
+        if constexpr (NT) __builtin_nontemporal_store(q, &reinterpret_cast<AnyVec<DT>*>(p + i)->q);
+        else reinterpret_cast<AnyVec<DT>*>(p + i)->q = q;
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)

@@ -24,7 +24,8 @@ using dev::Elem;
 using dev::Vec16;
 
 constexpr int THREADS = 256;
-constexpr int TK = 4;            // tokens of a workgroup: 4 waves, one to a token
+constexpr int TK = 2;         // tokens of a workgroup (16384 tokens of 40 heads of 128, bf16, both ways: 121 us; 4: 124, 1: 126)
+constexpr int APPEND_TK = 4;  // of an append: 4 waves, one to a token
 
 // cos and sin of `turns` whole turns, any size.
 __device__ inline float2 cos_sin_turns(double turns) {
@@ -78,14 +79,14 @@ __device__ inline Unit<DT> load_unit(const Rotation& r, const typename Elem<DT>:
     return out;
 }
 // Turns it by the table's (cos, sin) of the token's pairs and stores it.
-template <int DT>
+template <int DT, bool NT = false>
 __device__ inline void store_unit(const Rotation& r, typename Elem<DT>::type* y, int u, const Unit<DT>& in,
                                   const float2* cs) {
     constexpr int V = Elem<DT>::VEC;
     float a[V], b[V];
     dev::unpack<DT>(in.a, a);
     if (u >= r.rot) {
-        dev::store_vec<DT>(y + 2 * r.half, (int64_t)(u - r.rot) * V, r.dim - 2 * r.half, a);
+        dev::store_vec<DT, NT>(y + 2 * r.half, (int64_t)(u - r.rot) * V, r.dim - 2 * r.half, a);
     } else if (r.interleaved) {
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
@@ -94,7 +95,7 @@ __device__ inline void store_unit(const Rotation& r, typename Elem<DT>::type* y,
             a[e] = p * t.x - q * t.y;
             a[e + 1] = q * t.x + p * t.y;
         }
-        dev::store_vec<DT>(y, (int64_t)u * V, 2 * r.half, a);
+        dev::store_vec<DT, NT>(y, (int64_t)u * V, 2 * r.half, a);
     } else {
         dev::unpack<DT>(in.b, b);
 #pragma unroll
@@ -104,15 +105,15 @@ __device__ inline void store_unit(const Rotation& r, typename Elem<DT>::type* y,
             a[e] = p * t.x - q * t.y;
             b[e] = q * t.x + p * t.y;
         }
-        dev::store_vec<DT>(y, (int64_t)u * V, r.half, a);
-        dev::store_vec<DT>(y + r.half, (int64_t)u * V, r.half, b);
+        dev::store_vec<DT, NT>(y, (int64_t)u * V, r.half, a);
+        dev::store_vec<DT, NT>(y + r.half, (int64_t)u * V, r.half, b);
     }
 }
 
 // x and y may be the same rows: a unit is read before it is written, and by its
 // thread alone (what a vector at a part's end holds of its neighbour is not used).
 // blockIdx.y takes a share of the heads.
-template <int DT>
+template <int DT, bool NT>
 __global__ __launch_bounds__(THREADS) void rope_kernel(const typename Elem<DT>::type* x, const int32_t* positions,
                                                        const double* freqs, typename Elem<DT>::type* y, int64_t tokens,
                                                        int heads, int heads_each, Rotation r, int64_t x_stride,
@@ -123,22 +124,19 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(const typename Elem<DT>::
     const int h0 = blockIdx.y * heads_each, hn = min(heads_each, heads - h0);
     // A token's heads' units in a row: unit fastest, so that a wave's vectors lie side by side.
     const int per = hn * r.units, all = n * per;
-    constexpr int DEPTH = 4;
+    constexpr int DEPTH = 3;
     Unit<DT> in[DEPTH];
-    const auto at = [&](int i, int& tk, int& h, int& u) {
-        tk = i / per;
-        const int rest = i - tk * per;
-        h = rest / r.units;
-        u = rest - h * r.units;
-    };
+    int tk[DEPTH], h[DEPTH], u[DEPTH];  // token, head and unit of each
     const auto load = [&](int i0) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             const int i = i0 + d * THREADS;
             if (i < all) {
-                int tk, h, u;
-                at(i, tk, h, u);
-                in[d] = load_unit<DT>(r, x + (t0 + tk) * x_stride + (h0 + h) * r.dim, u);
+                tk[d] = (int)((uint32_t)i / (uint32_t)per);
+                const int rest = i - tk[d] * per;
+                h[d] = (int)((uint32_t)rest / (uint32_t)r.units);
+                u[d] = rest - h[d] * r.units;
+                in[d] = load_unit<DT>(r, x + (t0 + tk[d]) * x_stride + (h0 + h[d]) * r.dim, u[d]);
             }
         }
     };
@@ -154,11 +152,7 @@ __global__ __launch_bounds__(THREADS) void rope_kernel(const typename Elem<DT>::
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             const int i = i0 + d * THREADS;
-            if (i < all) {
-                int tk, h, u;
-                at(i, tk, h, u);
-                store_unit<DT>(r, y + (t0 + tk) * y_stride + (h0 + h) * r.dim, u, in[d], cs + tk * half);
-            }
+            if (i < all) store_unit<DT, NT>(r, y + (t0 + tk[d]) * y_stride + (h0 + h[d]) * r.dim, u[d], in[d], cs + tk[d] * half);
         }
     }
 }
@@ -175,28 +169,31 @@ __global__ void rope_frequencies_kernel(double* freqs, int half, double rotary, 
 
 // ── append to pages ───────────────────────────────────────────────────────
 
-// Where a new token goes: its sequence by a count of the sequences that end at or
-// before it (64 at a time, a wave together), its position from the sequence's
-// length. page -1: nowhere (no sequence's token, or outside the table or the pages).
+// Where a new token goes: its sequence (64 looked at together, a wave), its position from the
+// sequence's length. page -1: nowhere (no sequence's token, or outside the table or the pages).
 struct Place {
     int position, page;
 };
 __device__ inline Place place_of(int token, const PagedArgs& a) {
     const int lane = threadIdx.x & 63;
-    int seq = 0;
     for (int base = 0; base < a.n_seqs; base += 64) {
-        const bool over = base + lane < a.n_seqs && a.starts[base + lane + 1] <= token;
-        seq += __popcll(__ballot(over));
+        const int i = base + lane;
+        int first = 0, end = 0, length = 0;
+        if (i < a.n_seqs) {
+            first = a.starts[i];
+            end = a.starts[i + 1];
+            length = a.lens[i];
+        }
+        const uint64_t in = __ballot(first >= 0 && token >= first && token < end);
+        if (!in) continue;
+        const int at = __builtin_ctzll(in);
+        const int64_t position = (int64_t)__builtin_amdgcn_readlane(length, at) - __builtin_amdgcn_readlane(end, at) + token;
+        if (position < 0 || position >> a.page_shift >= a.table_width) break;
+        const int page = a.table[(int64_t)(base + at) * a.table_width + (position >> a.page_shift)];
+        if (page < 0 || page >= a.pages) break;
+        return {(int)position, page};
     }
-    Place out{0, -1};
-    if (seq >= a.n_seqs) return out;
-    const int first = a.starts[seq], n = a.starts[seq + 1] - first;
-    if (token < first || first < 0) return out;
-    const int64_t position = (int64_t)a.lens[seq] - n + (token - first);
-    if (position < 0 || position >> a.page_shift >= a.table_width) return out;
-    const int page = a.table[(int64_t)seq * a.table_width + (position >> a.page_shift)];
-    if (page < 0 || page >= a.pages) return out;
-    return {(int)position, page};
+    return {0, -1};
 }
 
 template <int DT>
@@ -207,9 +204,30 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(const typename El
                                                                int64_t tokens, int kv_heads, int64_t kv_stride, Rotation r,
                                                                float magnitude) {
     extern __shared__ float2 cs[];
-    __shared__ Place places[TK];
-    const int64_t t0 = (int64_t)blockIdx.x * TK;
-    const int n = (int)min((int64_t)TK, tokens - t0), half = (int)r.half;
+    __shared__ Place places[APPEND_TK];
+    const int64_t t0 = (int64_t)blockIdx.x * APPEND_TK;
+    const int n = (int)min((int64_t)APPEND_TK, tokens - t0), half = (int)r.half;
+    constexpr int V = Elem<DT>::VEC, DEPTH = 1;
+    // A head's units: K's, then V's, which are copied.
+    const int per_head = r.units + (int)((r.dim + V - 1) / V), per = kv_heads * per_head, all = n * per;
+    Unit<DT> in[DEPTH];
+    int tk[DEPTH], h[DEPTH], u[DEPTH];
+    const auto load = [&](int i0) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int i = i0 + d * THREADS;
+            if (i < all) {
+                tk[d] = (int)((uint32_t)i / (uint32_t)per);
+                const int rest = i - tk[d] * per;
+                h[d] = (int)((uint32_t)rest / (uint32_t)per_head);
+                u[d] = rest - h[d] * per_head;
+                const int64_t from = (t0 + tk[d]) * kv_stride + h[d] * r.dim;
+                if (u[d] < r.units) in[d] = load_unit<DT>(r, k + from, u[d]);
+                else in[d].a = dev::load_raw<DT>(v + from, (int64_t)(u[d] - r.units) * V, r.dim);
+            }
+        }
+    };
+    load((int)threadIdx.x);  // on its way while the places are found
     const int w = (int)threadIdx.x / 64;
     if (w < n) {
         const Place p = place_of((int)(t0 + w), a);
@@ -217,27 +235,27 @@ __global__ __launch_bounds__(THREADS) void paged_append_kernel(const typename El
     }
     __syncthreads();
     for (int i = (int)threadIdx.x; i < n * half; i += THREADS) {
-        const int tk = i / half, p = i - tk * half;
-        const float2 c = cos_sin_turns((double)places[tk].position * freqs[p] * TURNS);
+        const int t = i / half, p = i - t * half;
+        const float2 c = cos_sin_turns((double)places[t].position * freqs[p] * TURNS);
         cs[i] = {magnitude * c.x, magnitude * c.y};
     }
     if (half) __syncthreads();
-    constexpr int V = Elem<DT>::VEC;
-    const int plain = (int)((r.dim + V - 1) / V), per_head = r.units + plain;
-    const int per = kv_heads * per_head;
-    for (int i = (int)threadIdx.x; i < n * per; i += THREADS) {
-        const int tk = i / per, rest = i - tk * per, h = rest / per_head, u = rest - h * per_head;
-        const Place p = places[tk];
-        if (p.page < 0) continue;
-        const int64_t from = (t0 + tk) * kv_stride + h * r.dim;
-        const int64_t to = ((((int64_t)p.page * kv_heads + h) << a.page_shift) + (p.position & ((1 << a.page_shift) - 1))) * r.dim;
-        if (u < r.units) {
-            store_unit<DT>(r, k_pages + to, u, load_unit<DT>(r, k + from, u), cs + tk * half);
-        } else {
-            float x[V];
-            const int64_t e = (int64_t)(u - r.units) * V;
-            dev::unpack<DT>(dev::load_raw<DT>(v + from, e, r.dim), x);
-            dev::store_vec<DT>(v_pages + to, e, r.dim, x);
+    for (int i0 = (int)threadIdx.x; i0 < all; i0 += DEPTH * THREADS) {
+        if (i0 != (int)threadIdx.x) load(i0);
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (i0 + d * THREADS >= all) continue;
+            const Place p = places[tk[d]];
+            if (p.page < 0) continue;
+            const int row = p.position & ((1 << a.page_shift) - 1);
+            const int64_t to = ((((int64_t)p.page * kv_heads + h[d]) << a.page_shift) + row) * r.dim;
+            if (u[d] < r.units) {
+                store_unit<DT>(r, k_pages + to, u[d], in[d], cs + tk[d] * half);
+            } else {
+                float x[V];
+                dev::unpack<DT>(in[d].a, x);
+                dev::store_vec<DT>(v_pages + to, (int64_t)(u[d] - r.units) * V, r.dim, x);
+            }
         }
     }
 }
@@ -265,9 +283,15 @@ int rope_rows(int dtype, const void* x, const int32_t* positions, const double* 
     with_float_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         typedef typename Elem<DT>::type E;
-        hipLaunchKernelGGL(rope_kernel<DT>, dim3((unsigned)groups, (unsigned)ceil_div(heads, each)), dim3(THREADS), lds, s,
-                           (const E*)x, positions, freqs, (E*)y, tokens, (int)heads, (int)each,
-                           rotation<DT>(dim, rotary, interleaved), x_stride, y_stride, magnitude, vjp ? -1.0f : 1.0f);
+        const auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)ceil_div(heads, each)), dim3(THREADS), lds, s, (const E*)x,
+                               positions, freqs, (E*)y, tokens, (int)heads, (int)each, rotation<DT>(dim, rotary, interleaved),
+                               x_stride, y_stride, magnitude, vjp ? -1.0f : 1.0f);
+        };
+        // Rows of 64 MiB and more are stored past the caches (16384 tokens of 40 heads of 128,
+        // bf16, both ways: 124 us, 132 through them); smaller ones stay there for whoever reads them next.
+        if (tokens * heads * dim * (int64_t)sizeof(E) >= (int64_t(64) << 20)) launch(rope_kernel<DT, true>);
+        else launch(rope_kernel<DT, false>);
     });
     return launch_check("rope_kernel");
 }
@@ -276,11 +300,11 @@ int paged_append(int dtype, const void* k, const void* v, void* k_pages, void* v
                  int64_t kv_heads, int64_t dim, int64_t kv_stride, const double* freqs, int64_t rotary, int interleaved,
                  float magnitude, hipStream_t s) {
     if (!freqs) rotary = 0;
-    const size_t lds = sizeof(float2) * (size_t)(std::min<int64_t>(TK, tokens) * rotary / 2);
+    const size_t lds = sizeof(float2) * (size_t)(std::min<int64_t>(APPEND_TK, tokens) * rotary / 2);
     with_float_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         typedef typename Elem<DT>::type E;
-        hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((unsigned)ceil_div(tokens, TK)), dim3(THREADS), lds, s, (const E*)k,
+        hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((unsigned)ceil_div(tokens, APPEND_TK)), dim3(THREADS), lds, s, (const E*)k,
                            (const E*)v, freqs, (E*)k_pages, (E*)v_pages, a, tokens, (int)kv_heads, kv_stride,
                            rotation<DT>(dim, rotary, interleaved), magnitude);
     });

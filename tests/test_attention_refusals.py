@@ -78,27 +78,27 @@ def test_other_types(f, dt):
         f(dt=dt)
 
 
-HEADS = [{"dim": 12}, {"dim": 136}, {"dim": -8}, {"kv": 0}, {"kv": -1}, {"seqs": -1}, {"tokens": -1}, {"seqs": (1 << 21) + 1},
-         {"tokens": (1 << 30) + 1}]
+HEADS = [{"dim": 12}, {"dim": 136}, {"dim": -8}, {"kv": 0}, {"kv": -1}, {"seqs": -1}, {"tokens": -1}, {"seqs": (1 << 20) + 1},
+         {"tokens": (1 << 29) + 1}]
 SIZES = [
     (freqs, [{"rotary": 0}, {"rotary": 7}, {"rotary": 1026}, {"rotary": -2}, {"base": 0.0}, {"base": NAN}, {"base": INF},
              {"factor": 0.0}, {"factor": -1.0}, {"factor": NAN}, {"original": -1}, {"factor": 2.0, "original": 4096},
              {"factor": 2.0, "original": 4096, "low": 4.0, "high": 1.0}, {"factor": 2.0, "original": 4096, "low": NAN, "high": 1.0}]),
     (packed, HEADS + [{"heads": 5}, {"heads": -4}, {"qs": 28}, {"ks": 12}, {"os": 28}, {"qs": 33}, {"ks": 18}, {"os": 34},
                       {"qs": (1 << 20) + 4}, {"dt": abi.BF16, "qs": 36}, {"scale": NAN}, {"scale": INF},
-                      {"tokens": 1 << 29}]),
-    (append, HEADS[:3] + HEADS[4:] + [{"ks": 12}, {"ks": 18}, {"tokens": (1 << 25) + 1}, {"page": 8}, {"page": 24}, {"page": 0},
+                      {"tokens": (1 << 27) + 1}]),
+    (append, HEADS[:3] + HEADS[4:] + [{"ks": 12}, {"ks": 18}, {"tokens": (1 << 24) + 1}, {"page": 8}, {"page": 24}, {"page": 0},
                           {"page": 8192}, {"page": -16}, {"pages": -1}, {"pages": BIG}, {"width": -1},
                           {"width": 1 << 28}, {"freqs": P, "rotary": 9}, {"freqs": P, "rotary": 16}, {"freqs": P, "rotary": 0},
                           {"freqs": P, "rotary": 8, "inter": 2}]),
     (paged, HEADS + [{"heads": 5}, {"qs": 28}, {"os": 28}, {"qs": 33}, {"page": 8}, {"page": 48}, {"page": 8192},
                      {"pages": 0}, {"pages": -1}, {"width": 0}, {"width": -1}, {"width": 1 << 28}, {"scale": NAN},
-                     {"tokens": 1 << 29}]),
+                     {"tokens": (1 << 27) + 1}]),
 ]
 SIZES.append((packed_vjp, SIZES[1][1]))
 for f in (rope, rope_vjp):
     SIZES.append((f, [{"tokens": -1}, {"heads": -1}, {"dim": -1}, {"rotary": 10}, {"rotary": 7}, {"rotary": 0}, {"xs": 15},
-                      {"ys": 15}, {"xs": (1 << 20) + 1}, {"tokens": (1 << 25) + 1}, {"heads": 1 << 18, "xs": 1 << 20, "ys": 1 << 20},
+                      {"ys": 15}, {"xs": (1 << 20) + 1}, {"tokens": (1 << 24) + 1}, {"heads": 1 << 18, "xs": 1 << 20, "ys": 1 << 20},
                       {"inter": 2}, {"inter": -1}, {"xs": 17}, {"ys": 17}]))
 
 

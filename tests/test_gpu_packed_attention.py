@@ -248,3 +248,65 @@ def test_same_bits_every_time_and_replayed(dt, plan):
         g.close()
     finally:
         hb.destroy_stream(s)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2 MiB apart: the last of 2200 tokens lies 4.6 GB behind the first."""
+    tokens, row, dt = 2200, 1 << 20, abi.BF16
+    q, k, v, do = inputs(tokens, 2, 1, 16, dt)
+    starts = [0, 2150, 2200]
+    buf = hb.DeviceBuffer(tokens * row * 2)
+    part = np.concatenate([t.reshape(tokens, -1) for t in (q, k, v)], 1)
+    bits = synth.bf16_bits(part).reshape(tokens, -1)
+    for t in range(tokens):
+        buf.upload(bits[t], t * row * 2)
+    S, O, L = R.Dev(starts, abi.I32), R.Dev(dt=dt, shape=(tokens, 32)), R.Dev(dt=abi.F32, shape=(tokens, 2))
+    G = R.Dev(do, dt)
+    args = (2, tokens, 2, 1, 16, row, row, 32, 0.25, True)
+    at = [buf.ptr + 2 * c for c in (0, 32, 48)]
+    hb.packed_attention(dt, *at, S.ptr, O.ptr, L.ptr, *args)
+    grads = [buf.ptr + 2 * c for c in (64, 96, 112)]
+    hb.packed_attention_vjp(dt, *at, O.ptr, G.ptr, L.ptr, S.ptr, *grads, *args)
+    hb.synchronize()
+    i = slice(2150, 2200)
+    got = np.stack([buf.download(np.uint16, 64, t * row * 2 + 128) for t in range(2150, 2200)])
+    got = synth.bf16_to_f32(got).astype(np.float64)
+    wo, eo, wl, el = A.packed(q[i], k[i], v[i], [0, 50], 0.25, True, dt)
+    R.check(O.get().reshape(tokens, 2, 16)[i], wo, eo, "o")
+    wants = A.packed_vjp(q[i], k[i], v[i], do[i], [0, 50], 0.25, True, dt)
+    for name, cols, (want, bound) in zip(("dq", "dk", "dv"), (slice(0, 32), slice(32, 48), slice(48, 64)), wants):
+        R.check(got[:, cols].reshape(want.shape), want, bound, name)
+    buf.free()
+
+
+@pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
+def test_a_training_step_of_rotated_heads(dt):
+    """Rotary positions that start anew with each sequence, attention, and back: queries
+    and keys turned in place in the projection's rows, their gradients turned back."""
+    from test_gpu_rope_rows import frequencies
+    q, k, v, do = inputs(120, 4, 2, 32, dt)
+    starts, f = [0, 50, 120], frequencies(24)
+    pos = np.concatenate([np.arange(50), np.arange(70)]).astype(np.int32)
+    c = Call(q, k, v, do, starts, dt)
+    P, F = R.Dev(pos, abi.I32), hb.DeviceBuffer.from_array(f)
+    turn = (120, 6, 32, 24, c.row, c.row, False)  # q's and k's heads lie side by side
+    hb.rope_rows(dt, c.QKV.ptr, P.ptr, F, c.QKV.ptr, *turn)
+    c.forward(0.2, True)
+    c.backward(0.2, True)
+    hb.rope_vjp_rows(dt, c.D.ptr, P.ptr, F, c.D.ptr, *turn)
+    hb.synchronize()
+    o, lse, dq, dk, dv = c.results()
+    tq, tk = (R.rounded(A.rope(t, pos, f, 24, False, 1.0, dt)[0].astype(np.float32), dt) for t in (q, k))
+    wo, eo, _, _ = A.packed(tq, tk, v, starts, 0.2, True, dt)
+    wants = A.packed_vjp(tq, tk, v, do, starts, 0.2, True, dt)
+    # A value turned in f32 may round to the other neighbour, a step of 2 HALF of it: scores move by 4 HALF of
+    # their terms' magnitudes, and dS, a product of two such, by as much of itself.
+    z = 0.2 * 4 * R.HALF[dt] * (np.abs(tq).sum(2).max() * np.abs(tk).max())
+    R.check(o, wo, eo + 2 * z * np.abs(v).max(), "o")
+    for name, got, (want, bound), turned in zip(("dq", "dk", "dv"), (dq, dk, dv), wants, (True, True, False)):
+        size = np.abs(want).max() + 0.2 * np.abs(do).sum(2).max() * np.abs(v).max() * (np.abs(tq).max() + np.abs(tk).max())
+        bound = bound + 4 * z * size * (1 if turned else 2)
+        if turned:
+            want, e = A.rope(want, pos, f, 24, False, 1.0, dt, -1.0)
+            bound = e + 2 * bound.max(2, keepdims=True)
+        R.check(got, want, bound, name)

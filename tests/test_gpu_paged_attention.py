@@ -269,3 +269,26 @@ def test_same_bits_on_another_stream_and_replayed(new):
         g.close()
     finally:
         hb.destroy_stream(s)
+
+
+def test_pages_beyond_32_bits():
+    """Pages of 1 MiB, 4.6 GB of them: a sequence on the last ones, its rows appended there too."""
+    dt, page, pages, n = abi.F16, 4096, 4600, 5000
+    k, v = (R.rounded(synth.normal(i, (n, 1, 128)), dt) for i in (1, 2))
+    q = R.rounded(synth.normal(3, (2, 4, 128)), dt)
+    K, V = (hb.DeviceBuffer(pages * page * 128 * 2) for _ in range(2))
+    table = np.array([[4599, 4501]], np.int32)
+    T, S, N = R.Dev(table, abi.I32), R.Dev(np.array([0, 2], np.int32), abi.I32), R.Dev(np.array([n], np.int32), abi.I32)
+    for dev, rows in ((K, k), (V, v)):
+        for i, p in enumerate(table[0]):
+            dev.upload(synth.f16_bits(rows[page * i:min(page * (i + 1), n - 2)].reshape(-1)), int(p) * page * 128 * 2)
+    X, Y, Q, O = R.Dev(k[-2:], dt), R.Dev(v[-2:], dt), R.Dev(q, dt), R.Dev(dt=dt, shape=q.shape)
+    hb.paged_append(dt, X.ptr, Y.ptr, S.ptr, N.ptr, T.ptr, K, V, 1, 2, 1, 128, 128, pages, page, 2)
+    hb.paged_attention(dt, Q.ptr, K, V, S.ptr, N.ptr, T.ptr, O.ptr, 1, 2, 4, 1, 128, 512, 512, pages, page, 2, 0.1)
+    hb.synchronize()
+    got = O.get()
+    for h in range(4):
+        o, e, *_ = A.attend(*(t.astype(np.float64) for t in (q[:, h], k[:, 0], v[:, 0])), n - 2, 0.1, True, dt)
+        R.check(got[:, h], o, e, f"head {h}")
+    K.free()
+    V.free()
