@@ -106,6 +106,26 @@ __device__ inline Frag<DT> take_non_finite(Frag<DT>& f) {
     return bad;
 }
 
+// N products whose operands from LDS are read DEPTH ahead: read(i) gives product i's fragment, use(i, f)
+// forms it. Left alone the compiler reads a fragment into the registers of the one before and waits for
+// it every time.
+template <int DT, int N, int DEPTH, class Read, class Use>
+__device__ inline void stream(Read&& read, Use&& use) {
+    constexpr int D = DEPTH < N ? DEPTH : N;
+    Frag<DT> f[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i) f[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        use(i, f[i % D]);
+        if (i + D < N) {
+            f[i % D] = read(i + D);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
 // A tile of ROWS rows of a head in LDS.
 template <int DT, int DP, int ROWS>
 struct Tile {

@@ -81,10 +81,14 @@ int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v,
     a.few_rows = few_rows(dtype, tokens, a.group, n_seqs, kv_heads);
     a.row_items = items_of(tokens, a.group, n_seqs, a.few_rows ? attn::FEW_ROWS : attn::ROW_TILE);
     a.key_items = items_of(tokens, 1, n_seqs, attn::KEY_TILE);
-    // Few tiles of keys: each one's walk over several workgroups until there are 512, of three blocks of
-    // 32 rows or more on average, their sums joined.
+    // Few tiles of keys: each one's walk over several workgroups, their sums joined, until there are 512, of
+    // three blocks of 32 rows or more on average; where every compute unit has a tile, only of long
+    // walks, which end far apart. us, whole and in shares: the kernel of 51 tiles (1537 tokens, 9 heads on 3 of
+    // 80, f16) 75 and 29 + 5; steps of 260 tiles (8192 tokens, 16 heads on 4 of 128, bf16) 1750 and 1320;
+    // of 320 tiles with walks of 8 blocks (4 x 512 tokens, 16 heads of 64, bf16) 46 and 63, so not there.
     const int64_t wgs = a.key_items * kv_heads, blocks = a.group * (tokens / n_seqs) / (causal ? 64 : 32);
-    a.shares = (int)std::clamp<int64_t>(std::min<int64_t>(ceil_div(512, wgs), blocks / 3), 1, attn::MAX_SHARES);
+    const int64_t most = wgs < 256 || blocks >= 64 ? ceil_div(512, wgs) : 1;
+    a.shares = (int)std::clamp<int64_t>(std::min(most, blocks / 3), 1, attn::MAX_SHARES);
     if (const int forced = forced_shares.load()) a.shares = forced;
     const size_t stats = (((size_t)tokens * heads + 63) & ~size_t(63)) * sizeof(float);
     const size_t part = a.shares > 1 ? (size_t)a.shares * 2 * tokens * kv_heads * dim * sizeof(float) : 0;
@@ -107,11 +111,13 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     // Up to 32 rows a sequence on average (single tokens of up to 32 heads to a K/V head, say).
     const bool keys = tokens * a.group <= (int64_t)attn::FEW_ROWS * a.n_seqs;
     a.items = items_of(tokens, a.group, a.n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
-    // The keys over several workgroups: few rows until there are 2048 (four rounds of two to a
-    // compute unit, so that sequences of different lengths even out), tiles of rows until
-    // there are 512 (their parts cost more to join); within 256 MiB of parts.
-    const int64_t most = pages.table_width << pages.page_shift, wgs = (int64_t)a.items * kv_heads;
-    int64_t splits = std::min<int64_t>({(keys ? 2048 : 512) / std::max<int64_t>(wgs, 1), ceil_div(most, attn::MIN_SPAN), 64});
+    // The keys over several workgroups. Few rows: until there are 1024, or 2048 where the tiles alone are a
+    // round of two to a compute unit and what is left is to even out sequences of different lengths (us: 64
+    // sequences of up to 8192, bf16, 576 tiles: 179 at 1024, 150 at 2048; 16 of up to 4096, f32, 144 tiles:
+    // 106 and 131). Tiles of rows until there are 512: their parts cost more to join (256 tokens over
+    // 32768: 185, at 1024 203). Within 256 MiB of parts.
+    const int64_t most = pages.table_width << pages.page_shift, wgs = std::max<int64_t>((int64_t)a.items * kv_heads, 1);
+    int64_t splits = std::min<int64_t>({(!keys ? 512 : wgs < 512 ? 1024 : 2048) / wgs, ceil_div(most, attn::MIN_SPAN), 64});
     const int64_t row = tokens * heads * (dim + 4) * (int64_t)sizeof(float);
     splits = std::min<int64_t>(splits, (int64_t(256) << 20) / std::max<int64_t>(row, 1));
     a.splits = (int)std::max<int64_t>(splits, 1);

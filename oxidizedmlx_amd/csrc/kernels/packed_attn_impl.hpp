@@ -51,6 +51,7 @@ void attn_fwd_kernel(FwdArgs a) {
     constexpr int BM = KEYS ? FEW_ROWS : ROW_TILE, BN = KEYS || DT == MLXHIP_DTYPE_F32 ? 32 : 64;
     constexpr int LW = KEYS ? 1 : WAVES, STAGES = KEYS ? 1 : 2;
     constexpr int KB = BN / 32, KS = DP / 16, DB = DP / 32, EB = ELEM<DT>;
+    constexpr int AHEAD = DT == MLXHIP_DTYPE_F32 ? 2 : 4;  // fragments read ahead
     constexpr float SHIFT = DT == MLXHIP_DTYPE_F16 ? 6.0f : 0.0f, MOVE = 8.0f;
     using T = Tile<DT, DP, BN>;
     constexpr int TILES = (KEYS ? WAVES : 1) * STAGES * 2 * T::BYTES, JOIN = KEYS ? WAVES * 32 * (DP + 2) * 4 : 0;
@@ -147,13 +148,9 @@ void attn_fwd_kernel(FwdArgs a) {
     // One tile of keys from k0 on. after_scores: what may start once K has been read; before_v: what V waits for.
     const auto compute = [&](auto careful, const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int k0, auto&& after_scores,
                              auto&& before_v) {
-        f32x16 sc[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            sc[b] = f32x16{};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) mma<DT>(kf.read(kt, 32 * b, s), q[s], sc[b]);
-        }
+        f32x16 sc[KB] = {};
+        stream<DT, KB * KS, AHEAD>([&](int i) { return kf.read(kt, 32 * (i / KS), i % KS); },
+                                   [&](int i, const Frag<DT>& f) { mma<DT>(f, q[i % KS], sc[i / KS]); });
         after_scores();
         const bool masked = k0 + BN - 1 > wave_first || !live;
         const bool any_masked = __ballot(masked) != 0;
@@ -217,10 +214,8 @@ void attn_fwd_kernel(FwdArgs a) {
                 }
             }
         } else {
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int s = 0; s < 2 * KB; ++s) mma<DT>(vf.read(vt, 16 * s, d), p[s], o[d]);
+            stream<DT, DB * 2 * KB, AHEAD>([&](int i) { return vf.read(vt, 16 * (i % (2 * KB)), i / (2 * KB)); },
+                                           [&](int i, const Frag<DT>& f) { mma<DT>(f, p[i % (2 * KB)], o[i / (2 * KB)]); });
         }
     };
 
