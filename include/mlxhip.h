@@ -660,7 +660,7 @@ int mlxhip_packed_attention_vjp(int32_t dtype, const void* q, const void* k, con
  * too, do not enter. The keys of a sequence may be split over workgroups, whose parts, f32 in a
  * per-stream workspace (256 MiB at most), are joined in order.
  * dtype, head_dim, alignment, heads and sizes as for mlxhip_packed_attention; page_size a power
- * of two from 16 to 4096, table_width * page_size up to 2^31 - 1, of an append tokens up to 2^24. HipDecoder keeps its own
+ * of two from 16 to 4096, table_width * page_size up to 2^30, of an append tokens up to 2^24. HipDecoder keeps its own
  * cache (mlxhip_decoder_*); the reference's is a host vector (ttft_behavior.rs:101-216). */
 int mlxhip_paged_append(int32_t dtype, const void* k, const void* v, const int32_t* starts, const int32_t* lens,
                         const int32_t* table, void* k_pages, void* v_pages, int64_t n_seqs, int64_t tokens,

@@ -1476,8 +1476,8 @@ int paged_args(const char* what, const int32_t* starts, const int32_t* lens, con
     MLXHIP_TRY(check_sizes(what, {pages, page_size, table_width}, {INT32_MAX, 4096, INT32_MAX}));
     if (page_size < 16 || (page_size & (page_size - 1)))
         return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: page_size %lld (a power of two from 16 to 4096)", what, (long long)page_size);
-    if (table_width * page_size > INT32_MAX)
-        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: table_width * page_size is over 2^31 - 1", what);
+    if (table_width * page_size > (1 << 30))
+        return fail(MLXHIP_ERR_INVALID_ARGUMENT, "%s: table_width * page_size is over 2^30", what);
     *out = {starts, lens, table, (int)n_seqs, (int)pages, __builtin_ctzll((unsigned long long)page_size), table_width};
     return MLXHIP_OK;
 }

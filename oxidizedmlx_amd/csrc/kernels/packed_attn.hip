@@ -111,13 +111,15 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     // Up to 32 rows a sequence on average (single tokens of up to 32 heads to a K/V head, say).
     const bool keys = tokens * a.group <= (int64_t)attn::FEW_ROWS * a.n_seqs;
     a.items = items_of(tokens, a.group, a.n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
-    // The keys over several workgroups. Few rows: until there are 1024, or 2048 where the tiles alone are a
-    // round of two to a compute unit and what is left is to even out sequences of different lengths (us: 64
-    // sequences of up to 8192, bf16, 576 tiles: 179 at 1024, 150 at 2048; 16 of up to 4096, f32, 144 tiles:
-    // 106 and 131). Tiles of rows until there are 512: their parts cost more to join (256 tokens over
+    // The keys over several workgroups. Few rows: until there are 512, one round of two to a compute unit
+    // (us: 2 sequences of 131072, f16, 16 tiles: 197, at 1024 203: more parts to join); with 64 tiles and more,
+    // whose sequences differ, 1024 (16 of up to 4096, f32, 144 tiles: 106, at 512 115, at 2048 131); 2048
+    // where the tiles alone are a round and what is left is to even out (64 of up to 8192, bf16, 576 tiles:
+    // 150, at 1024 179). Tiles of rows until there are 512: their parts cost more to join (256 tokens over
     // 32768: 185, at 1024 203). Within 256 MiB of parts.
     const int64_t most = pages.table_width << pages.page_shift, wgs = std::max<int64_t>((int64_t)a.items * kv_heads, 1);
-    int64_t splits = std::min<int64_t>({(!keys ? 512 : wgs < 512 ? 1024 : 2048) / wgs, ceil_div(most, attn::MIN_SPAN), 64});
+    const int64_t target = !keys || wgs < 64 ? 512 : wgs < 512 ? 1024 : 2048;
+    int64_t splits = std::min<int64_t>({target / wgs, ceil_div(most, attn::MIN_SPAN), 64});
     const int64_t row = tokens * heads * (dim + 4) * (int64_t)sizeof(float);
     splits = std::min<int64_t>(splits, (int64_t(256) << 20) / std::max<int64_t>(row, 1));
     a.splits = (int)std::max<int64_t>(splits, 1);

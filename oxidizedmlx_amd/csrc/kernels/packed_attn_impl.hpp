@@ -10,7 +10,7 @@
 // between the two halves of a wave, p none before it is the next product's operand.
 //
 // Roundings: scores, p's sum and O are f32. p is rounded to the operands' type for its
-// product (relative 2^-9 or 2^-12 each, as many independent ones as keys, beside the one
+// product (relative 2^-8 or 2^-11 at most each, as many independent ones as keys, beside the one
 // that the result itself gets); f16's p is scaled by 2^6, which keeps probabilities
 // down to 2^-20 normal. A maximum moves only once it is passed by 2^8: p stays below
 // 2^14 and most tiles rescale nothing.
@@ -220,7 +220,6 @@ void attn_fwd_kernel(FwdArgs a) {
     };
 
     const auto walk = [&](auto careful) {
-
         if constexpr (KEYS) {
             // K of the next tile loads during this one's softmax and second product, V during
             // the next one's first; a wait leaves the newest loads under way.

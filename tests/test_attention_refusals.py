@@ -89,10 +89,10 @@ SIZES = [
                       {"tokens": (1 << 27) + 1}]),
     (append, HEADS[:3] + HEADS[4:] + [{"ks": 12}, {"ks": 18}, {"tokens": (1 << 24) + 1}, {"page": 8}, {"page": 24}, {"page": 0},
                           {"page": 8192}, {"page": -16}, {"pages": -1}, {"pages": BIG}, {"width": -1},
-                          {"width": 1 << 28}, {"freqs": P, "rotary": 9}, {"freqs": P, "rotary": 16}, {"freqs": P, "rotary": 0},
+                          {"width": (1 << 26) + 1}, {"freqs": P, "rotary": 9}, {"freqs": P, "rotary": 16}, {"freqs": P, "rotary": 0},
                           {"freqs": P, "rotary": 8, "inter": 2}]),
     (paged, HEADS + [{"heads": 5}, {"qs": 28}, {"os": 28}, {"qs": 33}, {"page": 8}, {"page": 48}, {"page": 8192},
-                     {"pages": 0}, {"pages": -1}, {"width": 0}, {"width": -1}, {"width": 1 << 28}, {"scale": NAN},
+                     {"pages": 0}, {"pages": -1}, {"width": 0}, {"width": -1}, {"width": (1 << 26) + 1}, {"scale": NAN},
                      {"tokens": (1 << 27) + 1}]),
 ]
 SIZES.append((packed_vjp, SIZES[1][1]))
