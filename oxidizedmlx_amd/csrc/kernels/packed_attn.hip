@@ -115,10 +115,16 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     // (us: 2 sequences of 131072, f16, 16 tiles: 197, at 1024 203: more parts to join); with 64 tiles and more,
     // whose sequences differ, 1024 (16 of up to 4096, f32, 144 tiles: 106, at 512 115, at 2048 131); 2048
     // where the tiles alone are a round and what is left is to even out (64 of up to 8192, bf16, 576 tiles:
-    // 150, at 1024 179). Tiles of rows until there are 512: their parts cost more to join (256 tokens over
-    // 32768: 185, at 1024 203). Within 256 MiB of parts.
+    // 150, at 1024 179). Tiles of rows: 512 for one sequence, whose walks are alike (256 tokens over 32768:
+    // 183, at 1100 196, at 1600 220; 2048 over 16384: 500, 522 and 526); for several, 800 where the tiles are
+    // less than a round (256 tokens in 4 over up to 32768: 153, at 512 207, at 1600 183; 1024 in 8 over up to
+    // 8192: 146, 192 and 150) and 1600 from there on (2000 in 4 over 16384: 632, at 512 and 800 756; over up
+    // to 16384: 417, at both 440). Within 256 MiB of parts.
     const int64_t most = pages.table_width << pages.page_shift, wgs = std::max<int64_t>((int64_t)a.items * kv_heads, 1);
-    const int64_t target = !keys || wgs < 64 ? 512 : wgs < 512 ? 1024 : 2048;
+    const int64_t target = keys                ? (wgs < 64 ? 512 : wgs < 512 ? 1024 : 2048)
+                           : pages.n_seqs == 1 ? 512
+                           : wgs < 512         ? 800
+                                               : 1600;
     int64_t splits = std::min<int64_t>({target / wgs, ceil_div(most, attn::MIN_SPAN), 64});
     const int64_t row = tokens * heads * (dim + 4) * (int64_t)sizeof(float);
     splits = std::min<int64_t>(splits, (int64_t(256) << 20) / std::max<int64_t>(row, 1));
