@@ -336,10 +336,7 @@ void attn_fwd_kernel(FwdArgs a) {
             for (int e = 0; e < 4; ++e) {
                 v[e] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < WAVES; ++i) {
-                    const float x = all[i * 32 * (DP + 2) + (d0 + e) * 32 + r];
-                    if (w[i] != 0.0f) v[e] += w[i] * x;
-                }
+                for (int i = 0; i < WAVES; ++i) v[e] += w[i] * all[i * 32 * (DP + 2) + (d0 + e) * 32 + r];
                 if (whole) v[e] = lim < 0 ? 0.0f : v[e] * inv;
             }
             if (!live) continue;

@@ -156,6 +156,21 @@ def test_non_finite_values_stay_with_those_that_see_them(dim, dt, plan):
 
 
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
+def test_non_finite_values_that_carry_no_weight(dt, plan):
+    """0 times NaN: of 32 keys whose scores lie 400 below the others', one in v."""
+    q, k, v, do = inputs(100, 2, 1, 16, dt)
+    q[:], k[:] = 10.0, 0.0
+    k[:32, :, 0] = -40.0
+    v[5, 0, 3] = np.nan
+    c = Call(q, k, v, do, [0, 100], dt)
+    c.forward(1.0, True)
+    hb.synchronize()
+    o = c.results()[0]
+    assert np.isnan(o[5:, :, 3]).all() and np.isfinite(o[:5]).all()
+    assert np.isfinite(np.delete(o, 3, axis=2)).all()
+
+
+@pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 def test_rows_without_any_score(dt, plan):
     """Scores of -inf everywhere a row sees: 0/0, as the formula says."""
     q, k, v, do = inputs(40, 1, 1, 16, dt)

@@ -131,6 +131,18 @@ def _skipping(c, rows, table):
     return out
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("lens", [[100], [2000]])
+def test_non_finite_values_that_carry_no_weight(lens, new):
+    """0 times NaN: of 32 positions whose scores lie 400 below the others', one in v."""
+    c = Cache(lens, [new], 2, 1, 16, 16, abi.BF16)
+    c.q[:], c.k[0][:] = 10.0, 0.0
+    c.k[0][:32, :, 0] = -40.0
+    c.v[0][5, 0, 3] = np.nan
+    o = c.attend(1.0)
+    assert np.isnan(o[:, :, 3]).all() and np.isfinite(np.delete(o, 3, axis=2)).all()
+
+
 def test_two_sequences_share_pages():
     c = Cache([64, 64], [1, 1], 4, 2, 64, 16, abi.F16)
     c.table[1, :3] = c.table[0, :3]
