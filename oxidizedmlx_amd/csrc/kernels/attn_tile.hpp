@@ -304,79 +304,85 @@ __device__ inline int wave_total(int v) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+// Of sequence `i`: its first token and how many it has. starts is the caller's: what it says is
+// brought into [0, tokens], a sequence that ends before it starts has no rows.
+__device__ inline int first_of(const int32_t* __restrict__ starts, int tokens, int i) { return min(max(starts[i], 0), tokens); }
+
 // The sequence and the tile in it that work item `item` names, of the sequences' rows
-// (tokens times per_token) in tiles of `rows`. Items go down by the number of the tile, 1 for each
-// sequence's shortest walk under a causal mask: the longest walks of all sequences come first, so
-// that none is left to run alone at the end (64 sequences at a time, then the
-// next 64). starts is the caller's: what it says is brought into [0, tokens], a sequence that ends
-// before it starts has no rows. A wave together; false past the last tile.
+// (tokens times per_token) in tiles of `rows`. Sequences go 64 at a time (a group), the groups' items
+// from what lies before them on: a tile for each `rows` rows and one for each sequence with any, which
+// is enough, and found without a sum over all lengths. A group's items go down by the number of the
+// tile, 1 for each sequence's shortest walk under a causal mask: the longest walks of its sequences come
+// first, so that none is left to run alone at the end. A wave together; false past a group's last tile.
 struct Place {
     int seq, first, tokens, level, tiles;  // level: 1 .. tiles
 };
 __device__ inline bool find_tile(const int32_t* __restrict__ starts, int n_seqs, int tokens, int per_token, int rows,
                                  int item, Place* out) {
     const int lane = threadIdx.x & 63;
-    for (int base = 0; base < n_seqs; base += 64) {
-        const int i = base + lane;
-        int first = 0, n = 0;
-        if (i < n_seqs) {
-            first = min(max(starts[i], 0), tokens);
-            n = max(min(max(starts[i + 1], 0), tokens) - first, 0);
-        }
-        const int tiles = (int)(((int64_t)n * per_token + rows - 1) / rows);
-        const int all = n_seqs == 1 ? __builtin_amdgcn_readfirstlane(tiles) : wave_total(tiles);
-        if (item >= all) {
-            item -= all;
-            continue;
-        }
-        // The highest level that more than `item` tiles reach: those from it on.
-        int lo = 1, over = 0;
-        if (n_seqs == 1) {
-            lo = all - item;
-            over = item;
-        } else {
-            for (int hi = all + 1; hi - lo > 1;) {  // above(lo) > item >= above(hi)
-                const int mid = lo + (hi - lo) / 2, above = wave_total(max(0, tiles - mid + 1));
-                if (above > item) {
-                    lo = mid;
-                } else {
-                    hi = mid;
-                    over = above;
-                }
+    int base = 0;
+    if (n_seqs > 64) {
+        const auto before = [&](int g) {  // rows are fewer than 2^29
+            const int first = first_of(starts, tokens, 64 * g);
+            return (int)((uint32_t)(first * per_token) / (uint32_t)rows) + min(64 * g, first);
+        };
+        base = dev::last_group((n_seqs + 63) / 64, [&](int g) { return before(g) <= item; });
+        if (base > 0) item -= before(base);
+        base *= 64;
+    }
+    const int i = base + lane;
+    int first = 0, n = 0;
+    if (i < n_seqs) {
+        first = first_of(starts, tokens, i);
+        n = max(first_of(starts, tokens, i + 1) - first, 0);
+    }
+    const int tiles = (int)(((int64_t)n * per_token + rows - 1) / rows);
+    const int all = n_seqs == 1 ? __builtin_amdgcn_readfirstlane(tiles) : wave_total(tiles);
+    if (item >= all) return false;
+    // The highest level that more than `item` tiles reach: those from it on.
+    int lo = 1, over = 0;
+    if (n_seqs == 1) {
+        lo = all - item;
+        over = item;
+    } else {
+        for (int hi = all + 1; hi - lo > 1;) {  // above(lo) > item >= above(hi)
+            const int mid = lo + (hi - lo) / 2, above = wave_total(max(0, tiles - mid + 1));
+            if (above > item) {
+                lo = mid;
+            } else {
+                hi = mid;
+                over = above;
             }
         }
-        uint64_t reach = __ballot(tiles >= lo);
-        for (int k = item - over; k > 0; --k) reach &= reach - 1;
-        const int at = __builtin_ctzll(reach);
-        out->seq = base + at;
-        out->first = __builtin_amdgcn_readlane(first, at);
-        out->tokens = __builtin_amdgcn_readlane(n, at);
-        out->tiles = __builtin_amdgcn_readlane(tiles, at);
-        out->level = lo;
-        return true;
     }
-    return false;
+    uint64_t reach = __ballot(tiles >= lo);
+    for (int k = item - over; k > 0; --k) reach &= reach - 1;
+    const int at = __builtin_ctzll(reach);
+    out->seq = base + at;
+    out->first = __builtin_amdgcn_readlane(first, at);
+    out->tokens = __builtin_amdgcn_readlane(n, at);
+    out->tiles = __builtin_amdgcn_readlane(tiles, at);
+    out->level = lo;
+    return true;
 }
 
 // The sequence that a token lies in (first and tokens of it), a wave together.
 __device__ inline bool find_token(const int32_t* __restrict__ starts, int n_seqs, int tokens, int token, Place* out) {
     const int lane = threadIdx.x & 63;
-    for (int base = 0; base < n_seqs; base += 64) {
-        const int i = base + lane;
-        int first = 0, n = 0;
-        if (i < n_seqs) {
-            first = min(max(starts[i], 0), tokens);
-            n = max(min(max(starts[i + 1], 0), tokens) - first, 0);
-        }
-        const uint64_t in = __ballot(token >= first && token - first < n);
-        if (!in) continue;
-        const int at = __builtin_ctzll(in);
-        out->seq = base + at;
-        out->first = __builtin_amdgcn_readlane(first, at);
-        out->tokens = __builtin_amdgcn_readlane(n, at);
-        return true;
+    const int base = 64 * dev::last_group((n_seqs + 63) / 64, [&](int g) { return first_of(starts, tokens, 64 * g) <= token; });
+    const int i = base + lane;
+    int first = 0, n = 0;
+    if (i < n_seqs) {
+        first = first_of(starts, tokens, i);
+        n = max(first_of(starts, tokens, i + 1) - first, 0);
     }
-    return false;
+    const uint64_t in = __ballot(token >= first && token - first < n);
+    if (!in) return false;
+    const int at = __builtin_ctzll(in);
+    out->seq = base + at;
+    out->first = __builtin_amdgcn_readlane(first, at);
+    out->tokens = __builtin_amdgcn_readlane(n, at);
+    return true;
 }
 
 }  // namespace attn

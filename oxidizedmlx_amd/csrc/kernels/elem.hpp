@@ -115,6 +115,20 @@ __device__ inline void store_vec(typename Elem<DT>::type* p, int64_t i, int64_t 
     }
 }
 
+// The last of `groups` (1 or more) for which reached(group) holds, which a beginning of them does, the
+// first in any case: 64 looked at together, so that 4096 take two rounds. A wave together.
+template <class F>
+__device__ inline int last_group(int groups, F&& reached) {
+    int lo = 0;
+    while (groups > 1) {
+        const int step = (groups + 63) / 64, at = (int)(threadIdx.x & 63) * step;
+        const int top = 63 - __builtin_clzll(__ballot(at == 0 || (at < groups && reached(lo + at))));
+        lo += top * step;
+        groups = min(step, groups - top * step);
+    }
+    return lo;
+}
+
 }  // namespace dev
 
 // Runs f.template operator()<DT>() for the dtype `dt`; false for one that is

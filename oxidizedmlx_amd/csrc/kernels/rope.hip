@@ -169,31 +169,27 @@ __global__ void rope_frequencies_kernel(double* freqs, int half, double rotary, 
 
 // ── append to pages ───────────────────────────────────────────────────────
 
-// Where a new token goes: its sequence (64 looked at together, a wave), its position from the
+// Where a new token goes: its sequence (of the 64 that it may lie in), its position from the
 // sequence's length. page -1: nowhere (no sequence's token, or outside the table or the pages).
 struct Place {
     int position, page;
 };
 __device__ inline Place place_of(int token, const PagedArgs& a) {
     const int lane = threadIdx.x & 63;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-        const int i = base + lane;
-        int first = 0, end = 0, length = 0;
-        if (i < a.n_seqs) {
-            first = a.starts[i];
-            end = a.starts[i + 1];
-            length = a.lens[i];
-        }
-        const uint64_t in = __ballot(first >= 0 && token >= first && token < end);
-        if (!in) continue;
-        const int at = __builtin_ctzll(in);
-        const int64_t position = (int64_t)__builtin_amdgcn_readlane(length, at) - __builtin_amdgcn_readlane(end, at) + token;
-        if (position < 0 || position >> a.page_shift >= a.table_width) break;
-        const int page = a.table[(int64_t)(base + at) * a.table_width + (position >> a.page_shift)];
-        if (page < 0 || page >= a.pages) break;
-        return {(int)position, page};
+    const int base = 64 * dev::last_group((a.n_seqs + 63) / 64, [&](int g) { return a.starts[64 * g] <= token; }), i = base + lane;
+    int first = 0, end = 0, length = 0;
+    if (i < a.n_seqs) {
+        first = a.starts[i];
+        end = a.starts[i + 1];
+        length = a.lens[i];
     }
-    return {0, -1};
+    const uint64_t in = __ballot(first >= 0 && token >= first && token < end);
+    if (!in) return {0, -1};
+    const int at = __builtin_ctzll(in);
+    const int64_t position = (int64_t)__builtin_amdgcn_readlane(length, at) - __builtin_amdgcn_readlane(end, at) + token;
+    if (position < 0 || position >> a.page_shift >= a.table_width) return {0, -1};
+    const int page = a.table[(int64_t)(base + at) * a.table_width + (position >> a.page_shift)];
+    return {(int)position, page >= 0 && page < a.pages ? page : -1};
 }
 
 template <int DT>

@@ -234,6 +234,14 @@ def test_many_short_sequences(plan):
     compare(*inputs(int(starts[-1]) + 3, 4, 2, 16, abi.F32), starts, 0.25, True, abi.F32)
 
 
+@pytest.mark.parametrize("n,most,first", [(5000, 3, 0), (5000, 2, 9), (130, 90, 3), (64, 50, 0), (65, 50, 1)])
+def test_thousands_of_sequences(n, most, first, plan):
+    """More than 64 times 64, empty ones among them, tokens in front of and behind them."""
+    lengths = (synth.uniform01(4, n) * most).astype(int)
+    starts = first + np.concatenate([[0], np.cumsum(lengths)])
+    compare(*inputs(int(starts[-1]) + 2, 2, 1, 8, abi.F32), starts, 0.25, True, abi.F32)
+
+
 @pytest.mark.parametrize("dt", [abi.F32, abi.F16], ids=R.NAMES.get)
 def test_same_bits_every_time_and_replayed(dt, plan):
     data, starts = inputs(333, 8, 2, 64, dt), [0, 100, 333]

@@ -205,6 +205,28 @@ def test_append_leaves_out_what_has_no_place():
     np.testing.assert_array_equal(V.get(), want)
 
 
+@pytest.mark.parametrize("n,most", [(5000, 2), (5000, 4), (150, 3), (65, 40)])
+def test_thousands_of_sequences(n, most):
+    """More than 64 times 64, some without a new token: the append's places and the attention over them."""
+    new = (synth.uniform01(8, n) * most).astype(int)
+    lens = new + (synth.uniform01(9, n) * 20).astype(int)
+    c = Cache(lens, new, 2, 1, 8, 16, abi.F32)
+    got, (want, bound) = c.attend(0.3), c.want(0.3)
+    R.check(got, want, bound, "o")
+    rows = [t[len(t) - m:] for t, m in zip(c.k, new)]
+    k = R.Dev(np.concatenate(rows + [np.full((2, 1, 8), LEFT, np.float32)]), abi.F32)
+    K, V = (R.Dev(np.full((c.pages, 1, 16, 8), LEFT), abi.F32) for _ in range(2))
+    S, N, T = (R.Dev(t, abi.I32) for t in (c.starts, c.lens, c.table))
+    hb.paged_append(abi.F32, k.ptr, k.ptr, S.ptr, N.ptr, T.ptr, K.ptr, V.ptr, n, c.tokens + 2, 1, 8, 8, c.pages, 16, c.width)
+    hb.synchronize()
+    places = np.full((c.pages, 1, 16, 8), LEFT)
+    for s, (r, m) in enumerate(zip(rows, new)):
+        for j, p in enumerate(range(int(lens[s]) - int(m), int(lens[s]))):
+            places[c.table[s, p // 16], :, p % 16] = r[j]
+    np.testing.assert_array_equal(K.get(), places)
+    np.testing.assert_array_equal(V.get(), places)
+
+
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 def test_steps_of_a_sequence_are_its_whole_attention(dt):
     """Prompts in one step, then chunks and single tokens through append and paged
