@@ -28,13 +28,19 @@ uint32_t flip_of(int dtype, float scale) {
 float factor_of(float scale) { return std::max(std::fabs(scale) * 1.44269504088896340736f, FLT_MIN); }
 
 // Whether a prompt's rows go in tiles of 32 whose keys four waves share out, not in tiles of 128: where
-// those would leave compute units without work. Forward, us, tiles of 128 / 32: f16, 123 tiles (1537
-// tokens, 9 heads on 3 of 80) 19.4 / 13.5; bf16, 320 (2048, 16 heads of 64) 13.0 / 16.9; f32, 320 (the
-// same) 52 / 38, 516 (4096, 16 on 4 of 128) 762 / 648.
-bool few_rows(int dtype, int64_t tokens, int64_t group, int64_t n_seqs, int64_t kv_heads) {
+// those would leave compute units without work, or with a causal sequence's longest walks alone at the end,
+// which the more tiles make up for the longer the walks are. Tiles of 32 reach about four fifths of the other's
+// rate where both fill the card. Forward, us, tiles of 128 / 32:
+//   f16: 123 tiles (1537 tokens, 9 heads on 3 of 80) 18.2 / 12.0;
+//   bf16, 8 heads of 128: 224 tiles (3500 tokens) 75.6 / 48.1, 288 (4500) 98.7 / 72.7, 376 (6000) 135.9 / 116,
+//   304 (4500 in 3 sequences) 57.6 / 40.4; but 320 (8 of 512) 17.5 / 20.5, 408 (1600, 32 heads on 8) 39.4 / 50.3;
+//   not causal: 176 (2800) 63.1 / 59.1, but 288 (4500) 123.6 / 139.9;
+//   f32: 320 (4 of 512, 16 heads of 64) 50.4 / 36.6, 516 (4096, 16 on 4 of 128) 748 / 642.
+bool few_rows(int dtype, int64_t tokens, int64_t group, int64_t n_seqs, int64_t kv_heads, int causal) {
     if (const int forced = forced_few_rows.load(); forced >= 0) return forced;
     const int64_t wgs = items_of(tokens, group, n_seqs, attn::ROW_TILE) * kv_heads;
-    return wgs < (dtype == MLXHIP_DTYPE_F32 ? 640 : 192);
+    if (dtype == MLXHIP_DTYPE_F32) return wgs < 640;
+    return wgs < (causal ? std::min<int64_t>(192 + tokens / n_seqs / 12, 480) : 192);
 }
 
 template <class F>
@@ -61,7 +67,7 @@ int packed_attention(int dtype, const void* q, const void* k, const void* v, con
     a.q_stride = q_stride, a.kv_stride = kv_stride, a.o_stride = o_stride;
     a.c = factor_of(scale), a.flip = flip_of(dtype, scale);
     a.causal = causal, a.splits = 1;
-    const bool keys = few_rows(dtype, tokens, a.group, n_seqs, kv_heads);
+    const bool keys = few_rows(dtype, tokens, a.group, n_seqs, kv_heads, causal);
     a.items = items_of(tokens, a.group, n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
     return by_dtype(dtype, [&](auto dt) { return attn::fwd<decltype(dt)::value>(a, false, keys, s); });
 }
@@ -78,7 +84,7 @@ int packed_attention_vjp(int dtype, const void* q, const void* k, const void* v,
     a.q_stride = q_stride, a.kv_stride = kv_stride, a.o_stride = o_stride;
     a.c = factor_of(scale), a.scale = scale, a.flip = flip_of(dtype, scale);
     a.causal = causal;
-    a.few_rows = few_rows(dtype, tokens, a.group, n_seqs, kv_heads);
+    a.few_rows = few_rows(dtype, tokens, a.group, n_seqs, kv_heads, causal);
     a.row_items = items_of(tokens, a.group, n_seqs, a.few_rows ? attn::FEW_ROWS : attn::ROW_TILE);
     a.key_items = items_of(tokens, 1, n_seqs, attn::KEY_TILE);
     // Few tiles of keys: each one's walk over several workgroups, their sums joined, until there are 512, of
@@ -112,10 +118,10 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     const bool keys = tokens * a.group <= (int64_t)attn::FEW_ROWS * a.n_seqs;
     a.items = items_of(tokens, a.group, a.n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
     // The keys over several workgroups. Few rows: until there are 512, one round of two to a compute unit
-    // (us: 2 sequences of 131072, f16, 16 tiles: 197, at 1024 203: more parts to join); with 64 tiles and more,
-    // whose sequences differ, 1024 (16 of up to 4096, f32, 144 tiles: 106, at 512 115, at 2048 131); 2048
+    // (us: 2 sequences of 131072, f16, 16 tiles: 193, at 1024 199: more parts to join); with 64 tiles and more,
+    // whose sequences differ, 1024 (16 of up to 4096, f32, 144 tiles: 100, at 512 110, at 2048 121); 2048
     // where the tiles alone are a round and what is left is to even out (64 of up to 8192, bf16, 576 tiles:
-    // 150, at 1024 179). Tiles of rows: 512 for one sequence, whose walks are alike (256 tokens over 32768:
+    // 148, at 1024 176). Tiles of rows: 512 for one sequence, whose walks are alike (256 tokens over 32768:
     // 183, at 1100 196, at 1600 220; 2048 over 16384: 500, 522 and 526); for several, 800 where the tiles are
     // less than a round (256 tokens in 4 over up to 32768: 153, at 512 207, at 1600 183; 1024 in 8 over up to
     // 8192: 146, 192 and 150) and 1600 from there on (2000 in 4 over 16384: 632, at 512 and 800 756; over up
