@@ -17,6 +17,10 @@
 // f16 would lose dS below 2^-24: each column of dS (a query's in dQ, a key's in dK) has a power of
 // two of its own that brings it to about 2^12, changed (with the sum so far) when a later
 // tile outgrows it; P is scaled by 2^14. bf16 and f32 have the range.
+//
+// Bound by the matrix cores, and what their operands wait for: 8192 tokens in 6 sequences, 32 heads on 8 of 128, bf16:
+// dQ 228 us (46 % of the cycles busy), dK and dV 371 (36 %): their sums leave one workgroup of
+// eight waves to a compute unit, which wait 47 % of their cycles.
 #pragma once
 
 #include "attn_tile.hpp"
