@@ -171,8 +171,8 @@ __device__ inline void lds_load4(__amdgpu_buffer_rsrc_t rsrc, MLXHIP_LDS char* d
 //          the tile's first row.
 //   PAGES  16 rows (which lie in one page) to a descriptor, a wave's instructions side by side, so that
 //          it has one or two: an offset for each instruction of 16 rows, from the first of them.
-//   LEAN   rows one after another, the waves' instructions in turn and a descriptor each: the swizzle
-//          comes round after 16 rows, so that one or two offsets serve all where registers are short.
+//   LEAN   rows one after another, one descriptor: the swizzle comes round after 16 rows, so that one or
+//          two offsets, and an addition for each instruction, serve all where registers are short.
 enum LoadMode { TILE, PAGES, LEAN };
 template <int DT, int DP, int ROWS, int LW, int MODE>
 struct TileLoader {
@@ -181,24 +181,25 @@ struct TileLoader {
     static constexpr int STEP = (MODE == PAGES ? 1 : LW) * T::RPI, PER16 = STEP >= 16 ? 1 : 16 / STEP;
     static constexpr int ROUND = MODE == TILE || L < PER16 ? L : PER16;
     static_assert(L * LW == T::INSTR && (16 % STEP == 0 || STEP % 16 == 0), "whole instructions to a wave");
+    // Past any buffer: LEAN's with a row's offset added too, which must not come round (a tile is 2^27
+    // bytes at most: strides up to 2^20 elements, 64 rows of 16 bits, 32 of f32).
+    static constexpr uint32_t PAST = MODE == LEAN ? 0x80000000u : gemm16::OOB;
     uint32_t voff[ROUND];
     __device__ static inline int instr(int wave, int i) { return MODE == PAGES ? wave * L + i : i * LW + wave; }
     __device__ inline void init(int wave, int lane, int dim, uint32_t stride_bytes) {
 #pragma unroll
         for (int i = 0; i < ROUND; ++i) {
             const int row = instr(wave, i) * T::RPI + lane / T::CPR, c = lane % T::CPR ^ T::swizzle(row);
-            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(MODE == TILE ? row : row % 16) * stride_bytes + c * 16 : gemm16::OOB;
+            voff[i] = c * 16 < dim * ELEM<DT> ? (uint32_t)(MODE == TILE ? row : row % 16) * stride_bytes + c * 16 : PAST;
         }
     }
     // TILE, LEAN: `left` rows (1 or more) from p on, stride_bytes apart; zeros behind them.
     __device__ inline void rows(const char* p, int left, uint32_t stride_bytes, MLXHIP_LDS char* tile, int wave) const {
-        __amdgpu_buffer_rsrc_t rsrc;
+        const __amdgpu_buffer_rsrc_t rsrc = buffer(p, (uint32_t)max(0, min(left, ROWS)) * stride_bytes);
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int r = MODE == TILE ? 0 : instr(wave, i) * T::RPI & ~15;
-            if (MODE == TILE ? i == 0 : i % PER16 == 0)
-                rsrc = buffer(p + (int64_t)r * stride_bytes, (uint32_t)max(0, min(left - r, MODE == TILE ? ROWS : 16)) * stride_bytes);
-            lds_load16(rsrc, tile + instr(wave, i) * 1024, voff[i % ROUND]);
+            const uint32_t at = MODE == TILE ? 0 : (uint32_t)(instr(wave, i) * T::RPI & ~15) * stride_bytes;
+            lds_load16(rsrc, tile + instr(wave, i) * 1024, voff[i % ROUND] + at);
         }
     }
     // PAGES: at(r, &bytes): where rows r .. r + 15 of the tile lie from p on, and how many bytes of them.

@@ -19,7 +19,7 @@
 // tile outgrows it; P is scaled by 2^14. bf16 and f32 have the range.
 //
 // Bound by the matrix cores, and what their operands wait for: 8192 tokens in 6 sequences, 32 heads on 8 of 128, bf16:
-// dQ 228 us (46 % of the cycles busy), dK and dV 371 (36 %): their sums leave one workgroup of
+// dQ 228 us (46 % of the cycles busy), dK and dV 363 (37 %): their sums leave one workgroup of
 // eight waves to a compute unit, which wait 47 % of their cycles.
 #pragma once
 

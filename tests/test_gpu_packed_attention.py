@@ -111,6 +111,12 @@ def test_rows_apart(dt, plan):
     compare(*inputs(100, 4, 2, 48, dt), [0, 37, 100], 0.2, True, dt, extra=24)
 
 
+@pytest.mark.parametrize("dt", [abi.F32, abi.BF16], ids=R.NAMES.get)
+def test_rows_as_far_apart_as_may_be(dt):
+    """2^20 elements, and heads that end inside a tile's row: what is past them stays zeros."""
+    compare(*inputs(70, 1, 1, 40, dt), [0, 70], 0.2, True, dt, extra=(1 << 20) - 120)
+
+
 @pytest.mark.parametrize("dt", R.DTYPES, ids=R.NAMES.get)
 def test_certain_rows(dt, plan):
     """Scores of +-100: probabilities of 1 and 0, a maximum that moves late and far."""
