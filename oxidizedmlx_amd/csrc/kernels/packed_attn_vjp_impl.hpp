@@ -236,7 +236,9 @@ void attn_dq_kernel(BwdArgs a) {
             }
         }
     };
-    if (DT != MLXHIP_DTYPE_F32 && last_key(row0 + BM - 1) < FINE_KEYS) {
+    // By the tile's first row, so that none that sees few keys is left out: 128 rows of ungrouped heads
+    // are 128 tokens, of which the first 64 see up to 64 keys.
+    if (DT != MLXHIP_DTYPE_F32 && last_key(row0) < FINE_KEYS) {
         walk(std::integral_constant<int, ROW_SUM>{});
         sum += __shfl_xor(sum, 32, 64);
         if constexpr (KEYS) {
