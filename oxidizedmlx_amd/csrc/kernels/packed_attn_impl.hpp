@@ -424,9 +424,10 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a) {
                 }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (i0 + i < parts && ml[i].x != -INFINITY) {  // -inf: no key seen
+                if (i0 + i < parts) {  // -inf: no key seen, or none with a score; 0 times what v made of those
                     const float to = ml[i].x > top || ml[i].x != ml[i].x ? ml[i].x : top;
-                    const float u = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - to), w = __builtin_amdgcn_exp2f(ml[i].x - to);
+                    const float u = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - to);
+                    const float w = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - to);
                     sum = sum * u + x[i] * w;
                     l = l * u + ml[i].y * w;
                     top = to;
