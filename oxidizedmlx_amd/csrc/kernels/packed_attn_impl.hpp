@@ -13,7 +13,9 @@
 // product (relative 2^-8 or 2^-11 at most each, as many independent ones as keys, beside the one
 // that the result itself gets); f16's p is scaled by 2^6, which keeps probabilities
 // down to 2^-20 normal. A maximum moves only once it is passed by 2^8: p stays below
-// 2^14 and most tiles rescale nothing.
+// 2^14 and most tiles rescale nothing. Sums of p v may then pass the range of f32 and bf16 where the
+// result does not (v from about 2^120 / keys on): rows that end non-finite are formed again with p times
+// 2^-40, parts are joined again in such units.
 //
 // ROWS: four waves of 32 rows share tiles of 64 keys (f32: 32), two in LDS, the next
 // on its way. KEYS, for few rows: the four waves have the same 32 rows and every fourth
@@ -50,36 +52,47 @@ __device__ inline int parts_of(const PagedArgs& p, int keys, int splits) {
     return max(1, (keys + span - 1) / span);
 }
 
-template <int DT, int DP, bool PAGED, bool KEYS>
-__global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS), amdgpu_waves_per_eu(KEYS && DT == MLXHIP_DTYPE_F32 ? 1 : 2, 2)))
-void attn_fwd_kernel(FwdArgs a) {
-    constexpr int BM = KEYS ? FEW_ROWS : ROW_TILE, BN = KEYS || DT == MLXHIP_DTYPE_F32 ? 32 : 64;
-    constexpr int LW = KEYS ? 1 : WAVES, STAGES = KEYS ? 1 : 2;
+template <int DT, int DP, bool KEYS>
+struct FwdShape {
+    static constexpr int BM = KEYS ? FEW_ROWS : ROW_TILE, BN = KEYS || DT == MLXHIP_DTYPE_F32 ? 32 : 64;
+    static constexpr int LW = KEYS ? 1 : WAVES, STAGES = KEYS ? 1 : 2;
+    using T = Tile<DT, DP, BN>;
+    static constexpr int TILES = (KEYS ? WAVES : 1) * STAGES * 2 * T::BYTES, JOIN = KEYS ? WAVES * 32 * (DP + 3) * 4 : 0;
+    static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
+};
+
+// A workgroup's tile of rows over its part of the keys. False where a result is not finite: nothing is
+// stored then, and the CAREFUL form, which keeps non-finite values of v from rows that do not see them,
+// forms it all anew. That form takes tid and lin through registers of their own, so that nothing of
+// it is kept while the other runs.
+template <int DT, int DP, bool PAGED, bool KEYS, bool CAREFUL>
+__device__ __attribute__((always_inline)) inline bool fwd_tile(const FwdArgs& a, char* smem_raw, int tid, int lin) {
+    using S = FwdShape<DT, DP, KEYS>;
+    constexpr int BM = S::BM, BN = S::BN, LW = S::LW, STAGES = S::STAGES;
     constexpr int KB = BN / 32, KS = DP / 16, DB = DP / 32, EB = ELEM<DT>;
     constexpr int AHEAD = DT == MLXHIP_DTYPE_F32 ? 2 : 4;  // fragments read ahead
     constexpr float SHIFT = DT == MLXHIP_DTYPE_F16 ? 6.0f : 0.0f, MOVE = 8.0f;
-    using T = Tile<DT, DP, BN>;
-    constexpr int TILES = (KEYS ? WAVES : 1) * STAGES * 2 * T::BYTES, JOIN = KEYS ? WAVES * 32 * (DP + 2) * 4 : 0;
-    __shared__ __attribute__((aligned(1024))) char smem_raw[TILES > JOIN ? TILES : JOIN];
+    constexpr bool RANGE = DT != MLXHIP_DTYPE_F16;  // v as large as f32's largest
+    constexpr float DOWN = 0x1p-40f, DOWN_LOG2 = -40.0f;
+    using T = typename S::T;
     typedef typename dev::Elem<DT>::type E;
 
-    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+    const int lane = tid & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     MLXHIP_LDS char* smem = (MLXHIP_LDS char*)smem_raw + (KEYS ? wave * STAGES * 2 * T::BYTES : 0);
 
     // Workgroups go round the 8 dies: with a multiple of 8 K/V heads each die keeps
     // to its own, whose keys its L2 then holds. Long tiles of a causal sequence first.
-    const int lin = blockIdx.x;
     const int per8 = a.kv_heads & 7 ? 1 : 8;
     const int item = per8 == 8 ? (lin >> 3) % a.items : lin / a.kv_heads;
     const int kvh = per8 == 8 ? (lin >> 3) / a.items * 8 + (lin & 7) : lin % a.kv_heads;
     Place at;
-    if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return;
+    if (!find_tile(a.starts, a.n_seqs, a.tokens, a.group, BM, item, &at)) return true;
     const int row0 = (at.level - 1) * BM, rows = at.tokens * a.group;
     const int length = PAGED ? length_of(a.pages, at.seq) : at.tokens, keys = PAGED ? keys_of(a.pages, length) : length;
     const int shift = length - at.tokens;  // position of the first new token
     const int parts = PAGED ? parts_of(a.pages, keys, a.splits) : 1, part = PAGED ? blockIdx.y : 0;
-    if (part >= parts) return;
+    if (part >= parts) return true;
 
     // This lane's row and the last key it sees.
     const int wrow = row0 + (KEYS ? 0 : 32 * wave), row = wrow + (lane & 31);
@@ -91,7 +104,9 @@ void attn_fwd_kernel(FwdArgs a) {
     };
     const int wave_last = last_key(wrow + 31), wave_first = last_key(wrow);
     const int n_tiles = max(0, last_key(row0 + BM - 1) + BN) / BN;
-    const int t0 = (int)((int64_t)n_tiles * part / parts), t1 = (int)((int64_t)n_tiles * (part + 1) / parts);
+    // Divided by the vector unit; in scalar registers, or the walk and its loads go by vector ones.
+    const int t0 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * part / parts));
+    const int t1 = __builtin_amdgcn_readfirstlane((int)((int64_t)n_tiles * (part + 1) / parts));
 
     Frag<DT> q[KS];
     const E* qrow = (const E*)a.q + (int64_t)(at.first + (live ? tok : 0)) * a.q_stride + (int64_t)(live ? head : 0) * a.dim;
@@ -149,9 +164,10 @@ void attn_fwd_kernel(FwdArgs a) {
     vf.init(lane);
     f32x16 o[DB] = {};
     float m = -INFINITY, l = 0.0f;
+    float down = 1.0f;  // of a row's p in its sums with v (not in l)
 
     // One tile of keys from k0 on. after_scores: what may start once K has been read; before_v: what V waits for.
-    const auto compute = [&](auto careful, const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int k0, auto&& after_scores,
+    const auto compute = [&](const MLXHIP_LDS char* kt, const MLXHIP_LDS char* vt, int k0, auto&& after_scores,
                              auto&& before_v) {
         f32x16 sc[KB] = {};
         stream<DT, KB * KS, AHEAD>([&](int i) { return kf.read(kt, 32 * (i / KS), i % KS); },
@@ -190,12 +206,13 @@ void attn_fwd_kernel(FwdArgs a) {
             for (int r = 0; r < 16; ++r) {
                 e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r], a.c, -mc));
                 l += e[r];
+                if constexpr (CAREFUL) e[r] *= down;
             }
             p[2 * b] = frag_of<DT>(e);
             p[2 * b + 1] = frag_of<DT>(e + 8);
         }
         before_v();
-        if (decltype(careful)::value && any_masked) {
+        if (CAREFUL && any_masked) {
             // p = 0 of a masked key would make NaN of a non-finite v: those are taken out of the
             // product, and what is counted of them among the keys that a row sees makes it NaN.
 #pragma unroll 1
@@ -224,7 +241,7 @@ void attn_fwd_kernel(FwdArgs a) {
         }
     };
 
-    const auto walk = [&](auto careful) {
+    const auto walk = [&] {
         if constexpr (KEYS) {
             // K of the next tile loads during this one's softmax and second product, V during
             // the next one's first; a wait leaves the newest loads under way.
@@ -241,7 +258,7 @@ void attn_fwd_kernel(FwdArgs a) {
                 const bool more = j + WAVES < t1;
                 gemm16::wait_vmcnt<L>();
                 compute(
-                    careful, kt, vt, j * BN,
+                    kt, vt, j * BN,
                     [&] {
                         __builtin_amdgcn_s_waitcnt(0xC07F);
                         if (more) {
@@ -272,128 +289,153 @@ void attn_fwd_kernel(FwdArgs a) {
                     issue(kbase, other, j + 1);
                     issue(vbase, other + T::BYTES, j + 1);
                 }
-                if (wrow < rows && j * BN <= wave_last) compute(careful, tile, tile + T::BYTES, j * BN, [] {}, [] {});
+                if (wrow < rows && j * BN <= wave_last) compute(tile, tile + T::BYTES, j * BN, [] {}, [] {});
             }
         }
     };
-    walk(std::false_type{});
-    // Where a result is not finite, a second walk that keeps non-finite values of v from
-    // rows that do not see them.
-    float finite = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) finite = __builtin_fmaf(o[d][r], 0.0f, finite);
-    if (__syncthreads_or(finite != 0.0f)) {  // NaN is not 0
-        // Addresses formed anew, or those of both walks take registers from the first.
-        int again = lane;
-        asm volatile("" : "+v"(again));
-        kf.init(again);
-        vf.init(again);
-        loader.init(KEYS ? 0 : wave, again, a.dim, stride_bytes);
-        window = -64;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] = f32x16{};
-        m = -INFINITY;
-        l = 0.0f;
-        walk(std::true_type{});
-    }
-    l += __shfl_xor(l, 32, 64);
-    float mc = m == -INFINITY ? 0.0f : m * a.c - SHIFT;  // l and o are sums of 2^(c S - mc)
-    bool empty = m == -INFINITY && l == 0.0f;            // no key seen (by this wave)
-
-    if constexpr (KEYS) {
-        // Joined through LDS: each wave's o, mc, l for the 32 rows; wave w then sums
-        // the four for every fourth part of the head.
-        __syncthreads();
-        float* all = reinterpret_cast<float*>(smem_raw);
-        float* mine = all + wave * 32 * (DP + 2);
-        const int r = lane & 31;
+    // KEYS: what the four waves' sums make together, too.
+    const auto finite = [&] {
+        float sum = 0.0f;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mine[(32 * d + 8 * (i / 4) + 4 * h + i % 4) * 32 + r] = o[d][i];
-        if (h == 0) {
-            mine[DP * 32 + r] = empty ? -INFINITY : mc;
-            mine[(DP + 1) * 32 + r] = l;
-        }
-        __syncthreads();
-        float top = -INFINITY, w[WAVES];
-        l = 0.0f;
+            for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(KEYS && RANGE ? o[d][r] * WAVES : o[d][r], 0.0f, sum);
+        return sum == 0.0f;  // NaN is not 0
+    };
+    if constexpr (!CAREFUL) {
+        walk();
+        if (__builtin_expect(__syncthreads_or(!finite()) != 0, 0)) return false;
+    } else {
+        // Rows that are still not finite once more, with p taken down; the others have the same bits again.
+#pragma unroll 1
+        for (int last = !RANGE;; last = 1) {
+            walk();
+            const bool bad = !finite();
+            if (last || !__syncthreads_or(bad)) break;
+            if (__ballot(bad) >> (lane & 31) & 0x100000001ull) down = DOWN;  // either half of the row's values
+            window = -64;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            w[i] = all[i * 32 * (DP + 2) + DP * 32 + r];
-            top = w[i] > top || w[i] != w[i] ? w[i] : top;
+            for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+            m = -INFINITY;
+            l = 0.0f;
         }
-        empty = top == -INFINITY;
-        mc = empty ? 0.0f : top;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            w[i] = w[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[i] - mc);
-            l += w[i] * all[i * 32 * (DP + 2) + (DP + 1) * 32 + r];
-        }
-        // Head values 4 (h + 2 wave + 8 i) .. + 3 of the lane's row.
-        const float inv = 1.0f / l;
-        const bool whole = parts == 1;
-        for (int d0 = 4 * (h + 2 * wave); d0 < a.dim; d0 += 32) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < WAVES; ++i) v[e] += w[i] * all[i * 32 * (DP + 2) + (d0 + e) * 32 + r];
-                if (whole) v[e] = lim < 0 ? 0.0f : v[e] * inv;
-            }
-            if (!live) continue;
-            if (!PAGED && a.lse && d0 == 0)
-                a.lse[(int64_t)(at.first + tok) * a.heads + head] = lim < 0 ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
-            if (!whole) {
-                float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
-                *reinterpret_cast<f32x4*>(to + d0) = f32x4{v[0], v[1], v[2], v[3]};
-                if (d0 == 0) {
-                    to[a.dim] = empty ? -INFINITY : mc;
-                    to[a.dim + 1] = l;
-                }
-                continue;
-            }
-            E* to = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim + d0;
-            if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-            else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
-        }
-        return;
     }
+    const float up = 1.0f / down;
+    const auto store = [&] {
+        l += __shfl_xor(l, 32, 64);
+        float mc = m == -INFINITY ? 0.0f : m * a.c - SHIFT;  // l and o are sums of 2^(c S - mc)
+        bool empty = m == -INFINITY && l == 0.0f;            // no key seen (by this wave)
+        // A part's base and sum; where o is taken down, in its units.
+        const auto store_part = [&](float* to, float base, float sum, float up) {
+            to[0] = empty ? -INFINITY : up > 1.0f ? base - DOWN_LOG2 : base;
+            to[1] = up > 1.0f ? sum * DOWN : sum;
+        };
 
-    if (!live) return;
-    if (parts > 1) {
-        float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
+        if constexpr (KEYS) {
+            // Joined through LDS: each wave's o, mc, l for the 32 rows; wave w then sums
+            // the four for every fourth part of the head.
+            __syncthreads();
+            float* all = reinterpret_cast<float*>(smem_raw);
+            constexpr int EACH = 32 * (DP + 3);
+            float* mine = all + wave * EACH;
+            const int r = lane & 31;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine[(32 * d + 8 * (i / 4) + 4 * h + i % 4) * 32 + r] = o[d][i];
+            if (h == 0) {
+                mine[DP * 32 + r] = empty ? -INFINITY : mc;
+                mine[(DP + 1) * 32 + r] = l;
+                mine[(DP + 2) * 32 + r] = up;
+            }
+            __syncthreads();
+            float top = -INFINITY, w[WAVES], lift = 0.0f;
+            l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                w[i] = all[i * EACH + DP * 32 + r];
+                top = w[i] > top || w[i] != w[i] ? w[i] : top;
+            }
+            empty = top == -INFINITY;
+            mc = empty ? 0.0f : top;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                w[i] = w[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(w[i] - mc);
+                l += w[i] * all[i * EACH + (DP + 1) * 32 + r];
+                lift = fmaxf(lift, all[i * EACH + (DP + 2) * 32 + r]);
+            }
+            // The four sums weighed by what they are divided by in the end; of a part they stay taken down.
+            const bool whole = parts == 1;
+            const float by = 1.0f / (whole ? l : lift);
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) w[i] *= by * all[i * EACH + (DP + 2) * 32 + r];
+            // Head values 4 (h + 2 wave + 8 i) .. + 3 of the lane's row.
+            for (int d0 = 4 * (h + 2 * wave); d0 < a.dim; d0 += 32) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < WAVES; ++i) v[e] += w[i] * all[i * EACH + (d0 + e) * 32 + r];
+                    if (whole && lim < 0) v[e] = 0.0f;
+                }
+                if (!live) continue;
+                if (!PAGED && a.lse && d0 == 0)
+                    a.lse[(int64_t)(at.first + tok) * a.heads + head] = lim < 0 ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
+                if (!whole) {
+                    float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
+                    *reinterpret_cast<f32x4*>(to + d0) = f32x4{v[0], v[1], v[2], v[3]};
+                    if (d0 == 0) store_part(to + a.dim, mc, l, lift);
+                    continue;
+                }
+                E* to = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim + d0;
+                if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+                else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
+            }
+            return;
+        }
+
+        if (!live) return;
+        if (parts > 1) {
+            float* to = a.part + ((int64_t)part * a.tokens * a.heads + (int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int at_d = 32 * d + 8 * g + 4 * h;
+                    if (at_d < a.dim) *reinterpret_cast<f32x4*>(to + at_d) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                }
+            if (h == 0) store_part(to + a.dim, mc, l, up);
+            return;
+        }
+        if (a.lse && h == 0) a.lse[(int64_t)(at.first + tok) * a.heads + head] = lim < 0 ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
+        const float inv = 1.0f / l * up;
+        E* orow = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int at_d = 32 * d + 8 * g + 4 * h;
-                if (at_d < a.dim) *reinterpret_cast<f32x4*>(to + at_d) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                if (at_d >= a.dim) continue;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = lim < 0 ? 0.0f : o[d][4 * g + e] * inv;
+                if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(orow + at_d) = f32x4{v[0], v[1], v[2], v[3]};
+                else *reinterpret_cast<u32x2*>(orow + at_d) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
             }
-        if (h == 0) {
-            to[a.dim] = empty ? -INFINITY : mc;
-            to[a.dim + 1] = l;
-        }
-        return;
-    }
-    if (a.lse && h == 0) a.lse[(int64_t)(at.first + tok) * a.heads + head] = lim < 0 ? -INFINITY : (mc + __builtin_amdgcn_logf(l)) * LN2;
-    const float inv = 1.0f / l;
-    E* orow = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int at_d = 32 * d + 8 * g + 4 * h;
-            if (at_d >= a.dim) continue;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = lim < 0 ? 0.0f : o[d][4 * g + e] * inv;
-            if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(orow + at_d) = f32x4{v[0], v[1], v[2], v[3]};
-            else *reinterpret_cast<u32x2*>(orow + at_d) = u32x2{gemm16::pack2<DT>(v[0], v[1]), gemm16::pack2<DT>(v[2], v[3])};
-        }
+    };
+    store();
+    return true;
+}
+
+template <int DT, int DP, bool PAGED, bool KEYS>
+__global__ __attribute__((amdgpu_flat_work_group_size(THREADS, THREADS), amdgpu_waves_per_eu(KEYS && DP == 128 && DT == MLXHIP_DTYPE_F32 ? 1 : 2, 2)))
+void attn_fwd_kernel(FwdArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[FwdShape<DT, DP, KEYS>::LDS];
+    int tid = threadIdx.x, lin = blockIdx.x;
+    if (__builtin_expect(fwd_tile<DT, DP, PAGED, KEYS, false>(a, smem, tid, lin), 1)) return;
+    asm volatile("" : "+v"(tid), "+s"(lin));
+    fwd_tile<DT, DP, PAGED, KEYS, true>(a, smem, tid, lin);
 }
 
 // The parts of a tile of rows joined, in order: 32 threads to a row, four values each, eight
@@ -411,30 +453,38 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a) {
     for (int r = threadIdx.x / 32; r < rows; r += THREADS / 32) {
         const int tok = (row0 + r) / a.group, head = kvh * a.group + (row0 + r - tok * a.group);
         const float* p = a.part + ((int64_t)(at.first + tok) * a.heads + head) * (a.dim + 4);
-        f32x4 sum = {};
-        float top = -INFINITY, l = 0.0f;
-        for (int i0 = 0; i0 < parts; i0 += 16) {
-            f32x4 x[16];
-            float2 ml[16];
+        const auto join = [&](float unit) {  // what the sum is counted in
+            f32x4 sum = {};
+            float top = -INFINITY, l = 0.0f;
+            for (int i0 = 0; i0 < parts; i0 += 16) {
+                f32x4 x[16];
+                float2 ml[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i0 + i < parts) {
-                    x[i] = *reinterpret_cast<const f32x4*>(p + (i0 + i) * step + 4 * t);
-                    ml[i] = *reinterpret_cast<const float2*>(p + (i0 + i) * step + a.dim);
-                }
+                for (int i = 0; i < 16; ++i)
+                    if (i0 + i < parts) {
+                        x[i] = *reinterpret_cast<const f32x4*>(p + (i0 + i) * step + 4 * t);
+                        ml[i] = *reinterpret_cast<const float2*>(p + (i0 + i) * step + a.dim);
+                    }
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i0 + i < parts) {  // -inf: no key seen, or none with a score; 0 times what v made of those
-                    const float to = ml[i].x > top || ml[i].x != ml[i].x ? ml[i].x : top;
-                    const float u = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - to);
-                    const float w = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - to);
-                    sum = sum * u + x[i] * w;
-                    l = l * u + ml[i].y * w;
-                    top = to;
-                }
+                for (int i = 0; i < 16; ++i)
+                    if (i0 + i < parts) {  // -inf: no key seen, or none with a score; 0 times what v made of those
+                        const float to = ml[i].x > top || ml[i].x != ml[i].x ? ml[i].x : top;
+                        const float u = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - to);
+                        const float w = ml[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - to);
+                        sum = sum * u + x[i] * (w * unit);
+                        l = l * u + ml[i].y * w;
+                        top = to;
+                    }
+            }
+            return sum / l;
+        };
+        f32x4 sum = join(1.0f);
+        if constexpr (DT != MLXHIP_DTYPE_F16) {
+            const f32x4 zero = sum * 0.0f;
+            if (__builtin_expect(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.0f), 0)) sum = join(0x1p-44f) * 0x1p44f;
         }
         const bool none = tok + length - at.tokens < 0;
-        sum = none ? f32x4{} : sum / l;
+        if (none) sum = f32x4{};
         E* to = (E*)a.o + (int64_t)(at.first + tok) * a.o_stride + (int64_t)head * a.dim + 4 * t;
         if constexpr (DT == MLXHIP_DTYPE_F32) *reinterpret_cast<f32x4*>(to) = sum;
         else *reinterpret_cast<u32x2*>(to) = u32x2{gemm16::pack2<DT>(sum[0], sum[1]), gemm16::pack2<DT>(sum[2], sum[3])};
