@@ -627,7 +627,8 @@ int mlxhip_rope_vjp_rows(int32_t dtype, const void* dy, const int32_t* positions
  * P and dS are rounded to a 16-bit type's own precision for their products (f16: scaled,
  * so that small ones keep it), results once. Sums are formed in a fixed order.
  * A non-finite value stays within its sequence: with v's the rows that see it are
- * not finite, others are as without it; the gradients of its sequence may be NaN.
+ * not finite, others are as without it; the gradients of its sequence may be NaN. Values
+ * of v up to 2^127 (or the type's largest) keep o finite, though sums before the division pass f32's range.
  * head_dim a multiple of 8 up to 128; addresses 16-byte aligned, strides a multiple of 16
  * bytes, up to 2^20. heads a multiple of kv_heads; tokens * heads up to 2^29, n_seqs *
  * kv_heads up to 2^21. Results must not overlap operands. The gradient keeps two f32 values

@@ -35,7 +35,13 @@ float factor_of(float scale) { return std::max(std::fabs(scale) * 1.442695040888
 //   bf16, 8 heads of 128: 224 tiles (3500 tokens) 75.6 / 48.1, 288 (4500) 98.7 / 72.7, 376 (6000) 135.9 / 116,
 //   304 (4500 in 3 sequences) 57.6 / 40.4; but 320 (8 of 512) 17.5 / 20.5, 408 (1600, 32 heads on 8) 39.4 / 50.3;
 //   not causal: 176 (2800) 63.1 / 59.1, but 288 (4500) 123.6 / 139.9;
-//   f32: 320 (4 of 512, 16 heads of 64) 50.4 / 36.6, 516 (4096, 16 on 4 of 128) 748 / 642.
+//   f32: 320 (4 of 512, 16 heads of 64) 50.4 / 36.6, 516 (4096, 16 on 4 of 128) 741 / 642, 632 (10000, 8 of
+//   128) 1950 / 1791, 640 (8 of 512, 16 of 64) 68.1 / 66.7; but 752 (6000, 16 on 4 of 128) 1213 / 1322, 776
+//   (12288, 8 of 128) 2529 / 2643, 1280 (16 of 512, 16 of 64) 106 / 130; and not causal, which the limit does
+//   not look at, 264 (4096, 8 of 128) 541 / 606.
+// dQ takes the same tiles. Whole gradients: bf16: 288 (4500) 269 / 227, 376 (6000) 385 / 340; but 320 (8 of 512)
+// 52.7 / 56.7, 408 (1600, 32 heads on 8) 150 / 166; f32: 264 (4096, 8 of 128) 1491 / 1133, 520 (8192) 4154 / 4168,
+// 640 (8 of 512, 16 of 64) 203 / 200, 1280 (16 of 512) 361 / 388.
 bool few_rows(int dtype, int64_t tokens, int64_t group, int64_t n_seqs, int64_t kv_heads, int causal) {
     if (const int forced = forced_few_rows.load(); forced >= 0) return forced;
     const int64_t wgs = items_of(tokens, group, n_seqs, attn::ROW_TILE) * kv_heads;
@@ -114,7 +120,9 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     a.q_stride = q_stride, a.o_stride = o_stride;
     a.c = factor_of(scale), a.flip = flip_of(dtype, scale);
     a.causal = 1;
-    // Up to 32 rows a sequence on average (single tokens of up to 32 heads to a K/V head, say).
+    // Up to 32 rows a sequence on average (single tokens of up to 32 heads to a K/V head, say): one tile of 32 to
+    // a sequence. us, tiles of 128 / 32 rows, 16 sequences of up to 8192, 32 heads on 8 of 128: bf16 at 16 rows
+    // a sequence 54 / 52, at 32 71 / 56, at 64 84 / 73, at 128 103 / 104; f32 at 32 434 / 171, at 128 698 / 432.
     const bool keys = tokens * a.group <= (int64_t)attn::FEW_ROWS * a.n_seqs;
     a.items = items_of(tokens, a.group, a.n_seqs, keys ? attn::FEW_ROWS : attn::ROW_TILE);
     // The keys over several workgroups. Few rows: until there are 512, one round of two to a compute unit
@@ -125,7 +133,9 @@ int paged_attention(int dtype, const void* q, const void* k_pages, const void* v
     // 183, at 1100 196, at 1600 220; 2048 over 16384: 500, 522 and 526); for several, 800 where the tiles are
     // less than a round (256 tokens in 4 over up to 32768: 153, at 512 207, at 1600 183; 1024 in 8 over up to
     // 8192: 146, 192 and 150) and 1600 from there on (2000 in 4 over 16384: 632, at 512 and 800 756; over up
-    // to 16384: 417, at both 440). Within 256 MiB of parts.
+    // to 16384: 417, at both 440). Within 256 MiB of parts, and 64 of them at most: what more of them save in the
+    // walks the join takes (one sequence of 131072, f16: 8 heads on 1, 39.1, with 32 parts 52.9, 128 38.3, 256
+    // 53.1; 16 on 2, 39.2, with 128 46.7; two of them, 16 on 2, 58.1, with 32 54.3, 128 66.9).
     const int64_t most = pages.table_width << pages.page_shift, wgs = std::max<int64_t>((int64_t)a.items * kv_heads, 1);
     const int64_t target = keys                ? (wgs < 64 ? 512 : wgs < 512 ? 1024 : 2048)
                            : pages.n_seqs == 1 ? 512

@@ -9,7 +9,8 @@
 // with atomic sums of dQ would take five.
 //
 // Roundings: sums are f32; P and dS are rounded to the operands' type for their products, as
-// many independent errors as keys or rows, together about the one that a result itself gets.
+// many independent errors as keys or rows, together about the one that a result itself gets (8192 tokens in 6
+// sequences, bf16, o and gradients: 2.1e-3 from 64 bits, 1.7e-3 by rounding exact results).
 // Rows that see few keys carry most of a causal sequence's gradient (P is about 1 / keys), so
 // those that see up to 64 have P and dS in two terms, the second what the first
 // rounds off; and D, which the rounding of O moves (by as much as dS itself after a few keys),

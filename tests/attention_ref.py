@@ -125,7 +125,7 @@ def packed_vjp(q, k, v, do, starts, scale, causal, dt):
 
 
 def pages_of(seqs, page, table_width, pages, rng):
-    """(table, k or v pages filler): page numbers in no order for sequences of these lengths."""
+    """The table: page numbers in no order for sequences of these lengths."""
     order = rng.permutation(pages)
     table, at = np.full((len(seqs), table_width), -7, np.int32), 0
     for i, n in enumerate(seqs):
